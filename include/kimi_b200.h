@@ -68,7 +68,11 @@ KB_API int kb_get_pdl(void);
  * safely (an expert index outside [0, E)) substitute a safe value (expert 0)
  * and set a bit here.
  * kb_device_errors() copies the word to the host (synchronizes the stream)
- * and clears it.  Bit 0: expert index out of range. */
+ * and clears it.  Bit 0: expert index out of range.  Bit 1: a bounded wait
+ * ran out.  Bit 2: a page, slot or token outside its table, cache or buffer
+ * (skipped; attention treats its keys as absent).  Bit 3: a tree parent that
+ * is not before its child, a tree of over 64 tokens, or a drafted token id
+ * outside the vocabulary (the token is never taken). */
 KB_API int kb_device_errors(void* stream, uint32_t* out_bits);
 
 /* ------------------------------------------------------------------------- */
@@ -407,6 +411,97 @@ KB_API int kb_step_info(const kb_step* step, int* n_ops, int* stages, int* stage
 /* gate/up), spare.  NULL switches it off.                                    */
 KB_API int kb_step_set_trace(kb_step* step, int64_t* trace, int64_t entries);
 KB_API int64_t kb_step_trace_entries(const kb_step* step);
+
+/* ------------------------------------------------------------------------- */
+/* Speculative serving over a paged cache.                                     */
+/* B requests; request b has context_lens[b] cached tokens and the tokens      */
+/* [cu_tokens[b], cu_tokens[b+1]) of this step.  Caches are logically          */
+/* [pages, page_size, heads, width] with any page, row and head strides        */
+/* (k_strides / v_strides: those three, host memory, in elements), unit stride */
+/* along the width.  A tree is given by each token's parent, an index in its   */
+/* request smaller than its own (-1 for token 0, the root).  dtype: 0 bf16,    */
+/* 1 f16, 2 f32.                                                               */
+/* ------------------------------------------------------------------------- */
+
+/* Pages and slots for the new tokens.  Request b takes the pages it lacks for
+ * context_lens[b] + new_lens[b] tokens from free_pages, from *free_head on, in
+ * request order, and their ids are written to its row of block_table.
+ * cu_tokens [B+1]: running sums of new_lens; slots [n_tokens]: page * page_size
+ * + row of each new token, -1 past the last token or without a page; positions
+ * [n_tokens]: context + index, or context + depth with parents [n_tokens];
+ * tree_mask [n_tokens] (with parents): bit j set when token j of the request is
+ * the token itself or an ancestor (at most 64 tokens a request).
+ * *free_head_out: the next free_head; *missing: pages that were needed and not
+ * given (the pool is empty, or the table too narrow).  B <= 12288. */
+KB_API int kb_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+                   int32_t* block_table, int64_t table_stride, int64_t table_width,
+                   const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                   int64_t page_size, int64_t n_tokens, const int32_t* parents,
+                   int32_t* cu_tokens, int64_t* slots, int32_t* positions, int64_t* tree_mask,
+                   int32_t* free_head_out, int32_t* missing, void* stream);
+
+/* k_cache[slot] = k[t], v_cache[slot] = v[t] for every token t with slots[t] >=
+ * 0.  16-bit elements; Dk and Dv multiples of 8; pointers 16-byte aligned and
+ * strides multiples of 8.  Two tokens must not name one slot. */
+KB_API int kb_paged_append(const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                   const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, int64_t N,
+                   int64_t H, int64_t Dk, int64_t Dv, uint16_t* k_cache,
+                   const int64_t* k_strides, uint16_t* v_cache, const int64_t* v_strides,
+                   int64_t n_pages, int64_t page_size, const int64_t* slots, void* stream);
+
+/* Causal attention of packed prompts: query i of a request sees its keys j <=
+ * i + (keys - queries).  out [total_q, Hq, Dv] contiguous; lse [total_q, Hq]
+ * fp32 or NULL (natural logarithm).  A query without keys gives 0 and
+ * -infinity.  Hq a multiple of Hkv; Dk <= 192, Dv <= 128, multiples of 8.
+ * max_q: no request has more queries.  dtype 0 or 1, the outputs' type too;
+ * products and sums in fp32. */
+KB_API int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                   const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                   const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                   const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t total_q,
+                   int64_t total_k, int64_t max_q, int64_t Hq, int64_t Hkv, int64_t Dk,
+                   int64_t Dv, float scale, uint16_t* out, float* lse, void* stream);
+
+/* Attention of this step's tokens over the paged cache, which already holds
+ * their keys and values at places context + index.  A token sees the whole
+ * context and, of its step, the tokens whose bit is set in its tree_mask word
+ * (NULL: itself and those before it).  max_tokens: no request has more tokens
+ * (at most 64 with tree_mask).  page_size: a power of two from 8 to 4096.
+ * Other arguments as kb_prompt_attention; the workspace of
+ * kb_tree_attention_workspace_size bytes is zeroed once and left zeroed where
+ * a call needs it so. */
+KB_API size_t kb_tree_attention_workspace_size(int64_t Hkv, int64_t group, int64_t max_tokens,
+                   int64_t Dv);
+KB_API int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                   const uint16_t* k_cache, const int64_t* k_strides, const uint16_t* v_cache,
+                   const int64_t* v_strides, int dtype, int64_t n_pages, int64_t page_size,
+                   const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                   const int32_t* context_lens, const int32_t* cu_tokens,
+                   const int64_t* tree_mask, int64_t B, int64_t total, int64_t max_tokens,
+                   int64_t Hq, int64_t Hkv, int64_t Dk, int64_t Dv, float scale, uint16_t* out,
+                   float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafted tokens the target accepts, and the token after them.  logits
+ * [rows, V]: row cu_tokens[b] + t is the target's prediction after token t of
+ * request b; tokens [rows] (token 0 of a request is its root).  From the root,
+ * children are tried in index order with p = softmax(logits / temperature[b]):
+ * child x is taken if accept_u * rem < p(x) (rem: the mass of p that refused
+ * children left), or, with draft_probs [rows, V] (row: the distribution the
+ * token was drawn from; chains only), if accept_u * q(x) < p(x).  The last
+ * node's token is argmax_i left_i / noise[b, i], lowest index first, where left
+ * is p without the refused tokens, or max(p - q, 0).  Temperature 0: the argmax
+ * is accepted and emitted.  out_tokens [B, max_tokens]: the accepted tokens and
+ * the last one, then -1; path [B, max_tokens]: 0 and the accepted tokens' tree
+ * indices, then -1; accepted [B].  parents NULL: chains.  max_tokens <= 64; a
+ * not-a-number logit counts as -infinity.  Workspace: zeroed once. */
+KB_API size_t kb_verify_drafts_workspace_size(int64_t B, int64_t rows);
+KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows, int64_t V,
+                   int dtype, const int64_t* tokens, const int32_t* parents,
+                   const int32_t* cu_tokens, int64_t B, int64_t max_tokens,
+                   const float* accept_u, const float* noise, int64_t noise_stride,
+                   const float* temperature, const float* draft_probs, int64_t probs_stride,
+                   int64_t* out_tokens, int32_t* path, int32_t* accepted, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -172,6 +172,45 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "kb_step_set_trace": (c_int, [c_void_p, c_void_p, c_int64]),
     "kb_step_trace_entries": (c_int64, [c_void_p]),
+    "kb_paged_plan": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+         c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p],
+    ),
+    "kb_paged_append": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+         c_void_p],
+    ),
+    "kb_prompt_attention": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+         c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p],
+    ),
+    "kb_tree_attention_workspace_size": (
+        c_size_t,
+        [c_int64, c_int64, c_int64, c_int64],
+    ),
+    "kb_tree_attention": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
+         c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "kb_verify_drafts_workspace_size": (
+        c_size_t,
+        [c_int64, c_int64],
+    ),
+    "kb_verify_drafts": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64,
+         c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
     "kb_kda_decode_step": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -64,6 +64,11 @@ int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
 // Device helpers.
 // ---------------------------------------------------------------------------
 
+// Bits of the device error word set by the paged-cache and drafting kernels
+// (bits 0 and 1, expert index and timeout, are kb_engine.cuh's).
+constexpr uint32_t ERR_PAGE = 4u;   // a page, slot or token outside its range
+constexpr uint32_t ERR_TREE = 8u;   // a parent not before its child, or a token id outside V
+
 // Wait until the grid this launch depends on (programmatic dependent launch)
 // has completed and its memory is visible.  No-op without the attribute.
 __device__ __forceinline__ void pdl_wait() {

@@ -1,0 +1,337 @@
+// kb_paged.cu - block tables, slot maps and tree masks from request lengths,
+// and storing new keys and values by slot.
+//
+// Request b has c_b cached tokens and n_b new ones; a page holds ps token rows.
+//   need_b  = ceil((c_b + n_b) / ps) - ceil(c_b / ps)          pages to take
+//   first_b = head + sum_{a < b} need_a                        in the free list
+//   table[b, ceil(c_b / ps) + i] = free[first_b + i]
+//   token t of b: place p = c_b + t, slot = table[b, p / ps] * ps + p % ps
+//   with a tree: mask_t = bit t | mask_parent(t), position = c_b + depth(t)
+//
+// One launch, no dependence between CTAs: every CTA sums the requests' needs
+// itself (two ints a request, from L2), keeps the running sums in shared
+// memory and then takes its share of the fresh pages and of the new tokens,
+// each found by a binary search in the sums.  A token in a fresh page reads
+// the free list, not the table entry another CTA may be writing.  A few
+// kilobytes of traffic: the time is launch and dependent-load latency.
+#include "kb_common.cuh"
+
+namespace kb {
+namespace paged {
+
+constexpr int THREADS = 256;
+constexpr int MAX_REQUESTS = 12288;          // two int arrays of shared memory
+
+struct PlanArgs {
+  const int* context;
+  const int* fresh;        // new tokens of each request
+  int* table;
+  int64_t table_stride;
+  const int* free_pages;
+  const int* free_head;
+  const int* parents;      // NULL: no tree
+  int B, width, nfree, ps, N;
+  int* cu;
+  int64_t* slots;
+  int* positions;
+  int64_t* mask;
+  int* head_out;
+  int* missing;
+  uint32_t* err;
+};
+
+__device__ __forceinline__ int pages_of(int64_t tokens, int ps) {
+  return (int)((tokens + ps - 1) / ps);
+}
+
+// Largest i in [0, n) with sums[i] <= v (sums ascending, sums[0] = 0).
+__device__ __forceinline__ int find(const int* sums, int n, int v) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sums[mid] <= v) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int warp_scan(int v, int lane) {
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
+  extern __shared__ int sums[];
+  int* s_tok = sums;                 // [B + 1] first token of each request
+  int* s_page = sums + A.B + 1;      // [B + 1] first fresh page of each request
+  __shared__ int s_part[THREADS / 32][3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  // Each thread takes a run of consecutive requests.
+  const int per = (A.B + THREADS - 1) / THREADS;
+  const int b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
+  int tok = 0, page = 0, lost = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int c = max(0, A.context[b]), n = max(0, A.fresh[b]);
+    const int have = pages_of(c, A.ps), want = pages_of((int64_t)c + n, A.ps);
+    const int need = max(0, min(want, A.width) - have);
+    s_tok[b] = tok;
+    s_page[b] = page;
+    tok += n;
+    page += need;
+    lost += want - have - need;
+  }
+  const int tok_in = warp_scan(tok, lane), page_in = warp_scan(page, lane);
+  const int lost_in = warp_scan(lost, lane);
+  if (lane == 31) {
+    s_part[warp][0] = tok_in;
+    s_part[warp][1] = page_in;
+    s_part[warp][2] = lost_in;
+  }
+  __syncthreads();
+  int tok0 = tok_in - tok, page0 = page_in - page, tokens = 0, pages = 0, beyond = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) {
+      tok0 += s_part[w][0];
+      page0 += s_part[w][1];
+    }
+    tokens += s_part[w][0];
+    pages += s_part[w][1];
+    beyond += s_part[w][2];
+  }
+  for (int b = b0; b < b1; ++b) {
+    s_tok[b] += tok0;
+    s_page[b] += page0;
+  }
+  if (tid == 0) {
+    s_tok[A.B] = tokens;
+    s_page[A.B] = pages;
+  }
+  const int head = max(0, *A.free_head);
+  const int avail = max(0, A.nfree - head);
+  __syncthreads();
+  pdl_launch_dependents();
+
+  const int at = blockIdx.x * THREADS + tid, step = gridDim.x * THREADS;
+  for (int b = at; b <= A.B; b += step) A.cu[b] = min(s_tok[b], A.N);
+  if (at == 0) {
+    *A.head_out = head + min(pages, avail);
+    *A.missing = beyond + max(0, pages - avail);
+    if (tokens > A.N) atomicOr(A.err, ERR_PAGE);
+  }
+  for (int i = at; i < pages; i += step) {
+    const int b = find(s_page, A.B, i);
+    const int col = pages_of(max(0, A.context[b]), A.ps) + i - s_page[b];
+    A.table[(int64_t)b * A.table_stride + col] = i < avail ? A.free_pages[head + i] : -1;
+  }
+  for (int i = at; i < A.N; i += step) {
+    int64_t slot = -1, word = 0;
+    int position = 0;
+    if (i < tokens) {
+      const int b = find(s_tok, A.B, i);
+      const int t = i - s_tok[b];
+      const int c = max(0, A.context[b]);
+      const int64_t place = (int64_t)c + t;
+      const int col = (int)(place / A.ps), have = pages_of(c, A.ps);
+      int id = -1;
+      if (col < A.width) {
+        if (col < have) {
+          id = A.table[(int64_t)b * A.table_stride + col];
+        } else {
+          const int f = s_page[b] + col - have;
+          id = f < avail ? A.free_pages[head + f] : -1;
+        }
+      }
+      if (id >= 0) slot = (int64_t)id * A.ps + place % A.ps;
+      position = (int)place;
+      if (A.parents != nullptr) {
+        // Up the tree: parents come before their children, so this ends.
+        int node = t, depth = 0;
+        if (t < 64) {
+          word = (int64_t)1 << t;
+          while (node > 0) {
+            const int up = A.parents[s_tok[b] + node];
+            if (up < 0 || up >= node) {
+              atomicOr(A.err, ERR_TREE);
+              break;
+            }
+            word |= (int64_t)1 << up;
+            node = up;
+            ++depth;
+          }
+        } else {
+          atomicOr(A.err, ERR_TREE);
+        }
+        position = c + depth;
+      }
+    }
+    A.slots[i] = slot;
+    A.positions[i] = position;
+    if (A.mask != nullptr) A.mask[i] = word;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Keys and values into their slots.
+// ---------------------------------------------------------------------------
+
+struct AppendArgs {
+  const uint16_t *k, *v;
+  int64_t k_tok, k_head, v_tok, v_head;            // element strides
+  uint16_t *kc, *vc;
+  int64_t kc_page, kc_row, kc_head, vc_page, vc_row, vc_head;
+  const int64_t* slots;
+  int64_t nslots;
+  int N, H, ps, ck, cv;                            // ck, cv: 16-byte pieces of a row
+  uint32_t* err;
+};
+
+// A thread per 16-byte piece; a token's pieces are its heads' key rows and
+// then its heads' value rows, so neighbouring threads read neighbouring bytes.
+__global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs A) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int pieces = A.H * (A.ck + A.cv);
+  const int64_t total = (int64_t)A.N * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * THREADS) {
+    const int t = (int)(i / pieces);
+    int r = (int)(i - (int64_t)t * pieces);
+    const int64_t slot = A.slots[t];
+    if (slot < 0) continue;
+    if (slot >= A.nslots) {
+      atomicOr(A.err, ERR_PAGE);
+      continue;
+    }
+    const int64_t page = slot / A.ps, row = slot - page * A.ps;
+    if (r < A.H * A.ck) {
+      const int h = r / A.ck, c = r - h * A.ck;
+      const uint4 x = *reinterpret_cast<const uint4*>(A.k + t * A.k_tok + h * A.k_head + c * 8);
+      *reinterpret_cast<uint4*>(A.kc + page * A.kc_page + row * A.kc_row + h * A.kc_head +
+                                c * 8) = x;
+    } else {
+      r -= A.H * A.ck;
+      const int h = r / A.cv, c = r - h * A.cv;
+      const uint4 x = *reinterpret_cast<const uint4*>(A.v + t * A.v_tok + h * A.v_head + c * 8);
+      *reinterpret_cast<uint4*>(A.vc + page * A.vc_page + row * A.vc_row + h * A.vc_head +
+                                c * 8) = x;
+    }
+  }
+}
+
+}  // namespace paged
+}  // namespace kb
+
+extern "C" int kb_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+                             int32_t* block_table, int64_t table_stride, int64_t table_width,
+                             const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                             int64_t page_size, int64_t n_tokens, const int32_t* parents,
+                             int32_t* cu_tokens, int64_t* slots, int32_t* positions,
+                             int64_t* tree_mask, int32_t* free_head_out, int32_t* missing,
+                             void* stream) {
+  kb::clear_error();
+  constexpr int64_t kMax = (int64_t)1 << 30;
+  KB_REQUIRE(B > 0 && table_width > 0 && table_stride >= table_width && n_free >= 0 &&
+                 n_tokens >= 0 && page_size > 0,
+             KB_ERR_BAD_SHAPE, "paged plan: bad shape");
+  KB_REQUIRE(B <= kb::paged::MAX_REQUESTS && n_tokens <= kMax && n_free <= kMax &&
+                 table_width <= kMax && page_size <= kMax,
+             KB_ERR_UNSUPPORTED, "paged plan: more than %d requests or 2^30 tokens or pages",
+             kb::paged::MAX_REQUESTS);
+  KB_REQUIRE(context_lens && new_lens && block_table && (free_pages || n_free == 0) &&
+                 free_head && cu_tokens && (n_tokens == 0 || (slots && positions)) &&
+                 free_head_out && missing && (!parents || tree_mask || n_tokens == 0),
+             KB_ERR_NULL_POINTER, "paged plan: NULL pointer");
+  const int dev = kb::bind_stream_device(stream);
+  kb::paged::PlanArgs A = {};
+  A.context = context_lens;
+  A.fresh = new_lens;
+  A.table = block_table;
+  A.table_stride = table_stride;
+  A.free_pages = free_pages;
+  A.free_head = free_head;
+  A.parents = parents;
+  A.B = (int)B;
+  A.width = (int)table_width;
+  A.nfree = (int)n_free;
+  A.ps = (int)page_size;
+  A.N = (int)n_tokens;
+  A.cu = cu_tokens;
+  A.slots = slots;
+  A.positions = positions;
+  A.mask = parents ? tree_mask : nullptr;
+  A.head_out = free_head_out;
+  A.missing = missing;
+  A.err = kb::device_error_word(dev);
+  KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
+  const size_t smem = (size_t)(2 * (B + 1)) * sizeof(int);
+  static_assert(2 * (kb::paged::MAX_REQUESTS + 1) * sizeof(int) <= 100 * 1024, "shared memory");
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kb::paged::plan_kernel,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    KB_REQUIRE(e == cudaSuccess, KB_ERR_DEVICE, "paged plan: shared-memory limit: %s",
+               cudaGetErrorString(e));
+  }
+  const int64_t items = n_tokens > B ? n_tokens : B;
+  int64_t grid = (items + kb::paged::THREADS - 1) / kb::paged::THREADS;
+  const int sms = kb::num_sms(dev);
+  if (grid > sms) grid = sms;
+  return kb::launch(kb::paged::plan_kernel, dim3((unsigned)grid), dim3(kb::paged::THREADS), smem,
+                    stream, A);
+}
+
+extern "C" int kb_paged_append(const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                               const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride,
+                               int64_t N, int64_t H, int64_t Dk, int64_t Dv, uint16_t* k_cache,
+                               const int64_t* k_strides, uint16_t* v_cache,
+                               const int64_t* v_strides, int64_t n_pages, int64_t page_size,
+                               const int64_t* slots, void* stream) {
+  kb::clear_error();
+  KB_REQUIRE(N >= 0 && H > 0 && Dk > 0 && Dv > 0 && n_pages >= 0 && page_size > 0,
+             KB_ERR_BAD_SHAPE, "paged append: bad shape");
+  if (N == 0) return KB_OK;
+  KB_REQUIRE(k && v && slots && k_strides && v_strides &&
+                 (n_pages == 0 || (k_cache && v_cache)),
+             KB_ERR_NULL_POINTER, "paged append: NULL pointer");
+  KB_REQUIRE(Dk % 8 == 0 && Dv % 8 == 0 && N < ((int64_t)1 << 31) &&
+                 H * (Dk + Dv) < ((int64_t)1 << 31),
+             KB_ERR_UNSUPPORTED, "paged append: head widths must be multiples of 8");
+  bool ok = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0 &&
+            ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && ((k_strides[i] | v_strides[i]) & 7) == 0;
+  KB_REQUIRE(ok, KB_ERR_ALIGNMENT,
+             "paged append: pointers must be 16-byte aligned and strides multiples of 8");
+  const int dev = kb::bind_stream_device(stream);
+  kb::paged::AppendArgs A = {};
+  A.k = k;
+  A.v = v;
+  A.k_tok = k_token_stride;
+  A.k_head = k_head_stride;
+  A.v_tok = v_token_stride;
+  A.v_head = v_head_stride;
+  A.kc = k_cache;
+  A.vc = v_cache;
+  A.kc_page = k_strides[0];
+  A.kc_row = k_strides[1];
+  A.kc_head = k_strides[2];
+  A.vc_page = v_strides[0];
+  A.vc_row = v_strides[1];
+  A.vc_head = v_strides[2];
+  A.slots = slots;
+  A.nslots = n_pages * page_size;
+  A.N = (int)N;
+  A.H = (int)H;
+  A.ps = (int)page_size;
+  A.ck = (int)(Dk / 8);
+  A.cv = (int)(Dv / 8);
+  A.err = kb::device_error_word(dev);
+  KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
+  const int64_t total = N * H * (A.ck + A.cv);
+  int64_t grid = (total + kb::paged::THREADS - 1) / kb::paged::THREADS;
+  const int64_t most = (int64_t)kb::num_sms(dev) * 8;
+  if (grid > most) grid = most;
+  return kb::launch(kb::paged::append_kernel, dim3((unsigned)grid), dim3(kb::paged::THREADS), 0,
+                    stream, A);
+}

@@ -39,6 +39,11 @@ MOE_COMBINE = "moe_combine"
 W4A16_QKV = "w4a16_qkv"
 KDA_STEP = "kda_step"
 MOE_ROUTER = "moe_router"
+PAGED_PLAN = "paged_plan"
+PAGED_APPEND = "paged_append"
+PROMPT_ATTENTION = "prompt_attention"
+TREE_ATTENTION = "tree_attention"
+VERIFY_DRAFTS = "verify_drafts"
 
 _DESCRIPTIONS = {
     W4A16_DENSE: "sm_100a W4A16 projection: HBM-streamed INT4 codes, bf16x2 decode in "
@@ -53,6 +58,12 @@ _DESCRIPTIONS = {
     KDA_STEP: "sm_100a KDA decode step, state read and written once, in place.",
     MOE_ROUTER: "sm_100a sigmoid router: fp32 logits, top-k by (score desc, index asc), "
     "renormalised and scaled weights.",
+    PAGED_PLAN: "sm_100a pages, slots, positions and tree masks from request lengths.",
+    PAGED_APPEND: "sm_100a keys and values into the slots of the paged caches.",
+    PROMPT_ATTENTION: "sm_100a causal attention over packed prompts, grouped heads.",
+    TREE_ATTENTION: "sm_100a attention of drafted trees (or single tokens) over the paged cache.",
+    VERIFY_DRAFTS: "sm_100a acceptance of drafted tokens against the target's logits, and the "
+    "token after them.",
 }
 
 _OPS = {
@@ -63,6 +74,11 @@ _OPS = {
     W4A16_QKV: ops.fused_qkv_w4a16,
     KDA_STEP: ops.kda_decode_step,
     MOE_ROUTER: ops.moe_router,
+    PAGED_PLAN: ops.paged_plan,
+    PAGED_APPEND: ops.paged_append,
+    PROMPT_ATTENTION: ops.prompt_attention,
+    TREE_ATTENTION: ops.tree_attention,
+    VERIFY_DRAFTS: ops.verify_drafts,
 }
 
 

@@ -19,11 +19,17 @@ Reference entry points mirrored here:
   kda_decode_step   engine/kernels/kda_step.py:273-293 (validation :137-170)
   moe_router        engine/klinear/router.py:47-85
   quantise          engine/quant/w4a16.py:68-105 (group size as a parameter)
+
+Operators of a speculative serving step that the reference has no kernel for
+(its MLA attention is torch einsum and softmax over projected keys and values,
+engine/klinear/attention.py:586-598): paged_plan, paged_append,
+prompt_attention, tree_attention, verify_drafts.
 """
 
 from __future__ import annotations
 
 from ctypes import c_float, c_int64, c_size_t, c_void_p
+from typing import NamedTuple
 
 import torch
 
@@ -911,3 +917,392 @@ def quantise(weight: torch.Tensor, group_size: int = 128) -> tuple[torch.Tensor,
     if int(flag.item()):
         raise ValueError("weight must contain only finite values")
     return packed, scales
+
+
+# ---------------------------------------------------------------------------
+# speculative serving over a paged cache
+# ---------------------------------------------------------------------------
+
+_ELEMENT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TREE_TOKENS = 64
+
+
+class PagedPlan(NamedTuple):
+    """What ``paged_plan`` returns (all on the device)."""
+
+    cu_tokens: torch.Tensor         # int32 [B + 1], running sums of the new lengths
+    slots: torch.Tensor             # int64 [num_tokens], -1 where a token has no slot
+    positions: torch.Tensor         # int32 [num_tokens]
+    tree_mask: torch.Tensor | None  # int64 [num_tokens], with parents
+    free_head: torch.Tensor         # int32 [1], the next call's free_head
+    missing: torch.Tensor           # int32 [1], pages needed and not given
+
+
+class Verification(NamedTuple):
+    """What ``verify_drafts`` returns (all on the device)."""
+
+    tokens: torch.Tensor    # int64 [B, max_tokens]: accepted tokens, the next token, then -1
+    path: torch.Tensor      # int32 [B, max_tokens]: 0 and the accepted tree indices, then -1
+    accepted: torch.Tensor  # int32 [B]
+
+
+def _vector(t: torch.Tensor, dtype: torch.dtype, what: str, device: torch.device,
+            length: int | None = None) -> torch.Tensor:
+    """A 1-D contiguous tensor of a type, length and device."""
+    if t.dtype != dtype or t.ndim != 1:
+        raise TypeError(f"{what} must be a one-dimensional {dtype} tensor")
+    if length is not None and t.shape[0] != length:
+        raise ValueError(f"{what} must have {length} entries")
+    if t.device != device:
+        raise ValueError(f"{what} must be on the device of the other tensors")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def paged_plan(
+    context_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_head: torch.Tensor,
+    page_size: int,
+    num_tokens: int,
+    *,
+    parents: torch.Tensor | None = None,
+) -> PagedPlan:
+    """Pages, slots and positions for every request's new tokens.
+
+    Request b has ``context_lens[b]`` cached tokens and gets ``new_lens[b]``
+    more.  The pages it lacks are taken from ``free_pages`` (from
+    ``free_head`` on, in request order) and written to its row of
+    ``block_table`` in place.  ``num_tokens`` is the length of the per-token
+    outputs: the sum of ``new_lens``, or more (the rest gets slot -1).  With
+    ``parents`` (int32 [num_tokens], the tree parent's index in the request,
+    -1 for the root) positions count the depth and ``tree_mask`` holds each
+    token's ancestors for ``tree_attention``.
+    """
+    device = context_lens.device
+    if block_table.dtype != torch.int32 or block_table.ndim != 2:
+        raise TypeError("block_table must be an int32 [requests, pages] matrix")
+    _require_cuda(context_lens, "paged plan")
+    requests, width = block_table.shape
+    ctx = _vector(context_lens, torch.int32, "context_lens", device, requests)
+    new = _vector(new_lens, torch.int32, "new_lens", device, requests)
+    free = _vector(free_pages, torch.int32, "free_pages", device)
+    head = _vector(free_head, torch.int32, "free_head", device, 1)
+    if block_table.device != device:
+        raise ValueError("block_table must be on the device of the other tensors")
+    if requests == 0 or width == 0:
+        raise ValueError("paged plan requires at least one request and one table column")
+    if block_table.stride(1) != 1 or (requests > 1 and block_table.stride(0) < width):
+        raise ValueError("block_table is updated in place and needs rows of unit stride")
+    if page_size <= 0 or num_tokens < 0:
+        raise ValueError("page_size must be positive and num_tokens not negative")
+    par = mask = None
+    if parents is not None:
+        par = _vector(parents, torch.int32, "parents", device, num_tokens)
+        mask = torch.empty((num_tokens,), dtype=torch.long, device=device)
+    cu = torch.empty((requests + 1,), dtype=torch.int32, device=device)
+    slots = torch.empty((num_tokens,), dtype=torch.long, device=device)
+    positions = torch.empty((num_tokens,), dtype=torch.int32, device=device)
+    head_out = torch.empty((1,), dtype=torch.int32, device=device)
+    missing = torch.empty((1,), dtype=torch.int32, device=device)
+    _lib.call(
+        "kb_paged_plan", ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
+        max(block_table.stride(0), width), width, free.data_ptr(), free.shape[0],
+        head.data_ptr(), page_size, num_tokens, None if par is None else par.data_ptr(),
+        cu.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+        None if mask is None else mask.data_ptr(), head_out.data_ptr(), missing.data_ptr(),
+        _stream(device),
+    )
+    return PagedPlan(cu, slots, positions, mask, head_out, missing)
+
+
+def _rows_of_heads(t: torch.Tensor, what: str) -> torch.Tensor:
+    """[tokens, heads, width] with unit inner stride and 16-byte aligned rows."""
+    if t.ndim != 3:
+        raise ValueError(f"{what} must have shape [tokens, heads, width]")
+    s = t.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+def _cache_strides(t: torch.Tensor, what: str) -> object:
+    """The page, row and head strides of a cache that kernels use in place."""
+    if t.ndim != 4:
+        raise ValueError(f"{what} must have shape [pages, page_size, heads, width]")
+    s = t.stride()
+    if t.numel() and (s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or t.data_ptr() % 16):
+        raise ValueError(f"{what} needs unit stride along the width, other strides multiples "
+                         "of 8 and a 16-byte aligned start")
+    return (c_int64 * 3)(s[0], s[1], s[2])
+
+
+def _check_widths(dk: int, dv: int) -> None:
+    if not (0 < dk <= 192 and dk % 8 == 0 and 0 < dv <= 128 and dv % 8 == 0):
+        raise ValueError("head widths must be multiples of 8, keys up to 192 and values up to 128")
+
+
+def paged_append(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+) -> None:
+    """Store each token's keys and values in its slot of the paged caches.
+
+    ``k`` [tokens, heads, Dk] and ``v`` [tokens, heads, Dv] go to
+    ``k_cache`` / ``v_cache`` [pages, page_size, heads, width] (any strides),
+    at page ``slot // page_size``, row ``slot % page_size``; a negative slot
+    is skipped.  No two tokens may name one slot.
+    """
+    if k.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("keys and values must be BF16 or FP16")
+    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+        raise TypeError("keys, values and caches must share one type")
+    _require_cuda(k, "paged append")
+    device = k.device
+    if not (v.device == k_cache.device == v_cache.device == device):
+        raise ValueError("paged append inputs must share one device")
+    ks, vs = _cache_strides(k_cache, "k_cache"), _cache_strides(v_cache, "v_cache")
+    kr, vr = _rows_of_heads(k, "k"), _rows_of_heads(v, "v")
+    n, heads, dk = k.shape
+    dv = v.shape[2]
+    if v.shape[:2] != (n, heads):
+        raise ValueError("k and v must have the same tokens and heads")
+    if k_cache.shape[2:] != (heads, dk) or v_cache.shape[2:] != (heads, dv):
+        raise ValueError("the caches' heads and widths must match k and v")
+    if k_cache.shape[:2] != v_cache.shape[:2]:
+        raise ValueError("the caches must have the same pages")
+    _check_widths(dk, dv)
+    sl = _vector(slots, torch.long, "slots", device, n)
+    if n == 0 or heads == 0:
+        return
+    _lib.call(
+        "kb_paged_append", kr.data_ptr(), kr.stride(0), kr.stride(1), vr.data_ptr(),
+        vr.stride(0), vr.stride(1), n, heads, dk, dv, k_cache.data_ptr(), ks,
+        v_cache.data_ptr(), vs, k_cache.shape[0], k_cache.shape[1], sl.data_ptr(),
+        _stream(device),
+    )
+
+
+def _attention_heads(q: torch.Tensor, heads: int, dk: int, dv: int) -> None:
+    if q.shape[1] == 0 or heads == 0 or q.shape[1] % heads:
+        raise ValueError("query heads must be a multiple of key/value heads")
+    if q.shape[2] != dk:
+        raise ValueError("queries and keys must have one width")
+    _check_widths(dk, dv)
+
+
+def prompt_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    max_seqlen: int,
+    *,
+    cu_seqlens_k: torch.Tensor | None = None,
+    scale: float | None = None,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Causal attention over packed prompts, grouped heads.
+
+    ``q`` [tokens, Hq, Dk], ``k`` [keys, Hkv, Dk], ``v`` [keys, Hkv, Dv], bf16
+    or f16; request b has the queries ``cu_seqlens[b]:cu_seqlens[b+1]`` (int32)
+    and the keys of ``cu_seqlens_k`` (default: the same).  Query i sees keys up
+    to ``i + keys - queries``.  No request has more than ``max_seqlen``
+    queries.  Returns [tokens, Hq, Dv] and, with ``return_lse``, the fp32
+    log-sum-exp [tokens, Hq]; a query without keys gives 0 and -infinity.
+    """
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("queries, keys and values must be BF16 or FP16")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("queries, keys and values must share one type")
+    _require_cuda(q, "prompt attention")
+    device = q.device
+    if not (k.device == v.device == device):
+        raise ValueError("prompt attention inputs must share one device")
+    qr, kr, vr = _rows_of_heads(q, "q"), _rows_of_heads(k, "k"), _rows_of_heads(v, "v")
+    total, hq, dk = q.shape
+    keys, hkv, dv = v.shape
+    if k.shape != (keys, hkv, dk):
+        raise ValueError("k must have the tokens and heads of v and the width of q")
+    _attention_heads(q, hkv, dk, dv)
+    if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must have one entry more than there are requests")
+    requests = cu_seqlens.shape[0] - 1
+    cq = _vector(cu_seqlens, torch.int32, "cu_seqlens", device)
+    if cu_seqlens_k is None:
+        if keys != total:
+            raise ValueError("cu_seqlens_k is needed where keys and queries differ in number")
+        ck = cq
+    else:
+        ck = _vector(cu_seqlens_k, torch.int32, "cu_seqlens_k", device, requests + 1)
+    if max_seqlen < 0:
+        raise ValueError("max_seqlen must not be negative")
+    out = torch.empty((total, hq, dv), dtype=q.dtype, device=device)
+    lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
+    _lib.call(
+        "kb_prompt_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), kr.data_ptr(),
+        kr.stride(0), kr.stride(1), vr.data_ptr(), vr.stride(0), vr.stride(1),
+        _ELEMENT[q.dtype], cq.data_ptr(), ck.data_ptr(), requests, total, keys, max_seqlen, hq,
+        hkv, dk, dv, dk ** -0.5 if scale is None else float(scale), out.data_ptr(),
+        None if lse is None else lse.data_ptr(), _stream(device),
+    )
+    return out if lse is None else (out, lse)
+
+
+def tree_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    cu_tokens: torch.Tensor,
+    max_tokens: int,
+    *,
+    tree_mask: torch.Tensor | None = None,
+    scale: float | None = None,
+    return_lse: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Attention of this step's tokens (one each, or drafted trees) over the paged cache.
+
+    Request b's tokens are ``q[cu_tokens[b]:cu_tokens[b+1]]`` (at most
+    ``max_tokens``); their keys and values already are in the caches
+    [pages, page_size, Hkv, width], after its ``context_lens[b]`` cached ones,
+    in the pages of ``block_table[b]``.  A token sees the context and, of its
+    step, the tokens whose bits its ``tree_mask`` word (int64, at most 64
+    tokens) has; without masks itself and those before it.  Outputs as
+    ``prompt_attention``.
+    """
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("queries and caches must be BF16 or FP16")
+    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+        raise TypeError("queries and caches must share one type")
+    if block_table.dtype != torch.int32 or block_table.ndim != 2:
+        raise TypeError("block_table must be an int32 [requests, pages] matrix")
+    _require_cuda(q, "tree attention")
+    device = q.device
+    if not (k_cache.device == v_cache.device == block_table.device == device):
+        raise ValueError("tree attention inputs must share one device")
+    ks, vs = _cache_strides(k_cache, "k_cache"), _cache_strides(v_cache, "v_cache")
+    qr = _rows_of_heads(q, "q")
+    total, hq, dk = q.shape
+    pages, page_size, hkv, dv = v_cache.shape
+    if k_cache.shape != (pages, page_size, hkv, dk):
+        raise ValueError("k_cache must have the pages and heads of v_cache and the width of q")
+    _attention_heads(q, hkv, dk, dv)
+    if page_size < 8 or page_size > 4096 or page_size & (page_size - 1):
+        raise ValueError("the page size must be a power of two from 8 to 4096")
+    requests, width = block_table.shape
+    table = block_table
+    if width and (table.stride(1) != 1 or (requests > 1 and table.stride(0) < width)):
+        table = table.contiguous()
+    ctx = _vector(context_lens, torch.int32, "context_lens", device, requests)
+    cu = _vector(cu_tokens, torch.int32, "cu_tokens", device, requests + 1)
+    if max_tokens < 0:
+        raise ValueError("max_tokens must not be negative")
+    mask = None
+    if tree_mask is not None:
+        if max_tokens > MAX_TREE_TOKENS:
+            raise ValueError(f"a masked tree has at most {MAX_TREE_TOKENS} tokens")
+        mask = _vector(tree_mask, torch.long, "tree_mask", device, total)
+    out = torch.empty((total, hq, dv), dtype=q.dtype, device=device)
+    lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
+    need = _lib.lib().kb_tree_attention_workspace_size(hkv, hq // hkv, max_tokens, dv)
+    ws = _workspace("tree_attention", device, need, (need,))
+    _lib.call(
+        "kb_tree_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), k_cache.data_ptr(), ks,
+        v_cache.data_ptr(), vs, _ELEMENT[q.dtype], pages, page_size, table.data_ptr(),
+        max(table.stride(0), width), width, ctx.data_ptr(), cu.data_ptr(),
+        None if mask is None else mask.data_ptr(), requests, total, max_tokens, hq, hkv, dk, dv,
+        dk ** -0.5 if scale is None else float(scale), out.data_ptr(),
+        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device),
+    )
+    return out if lse is None else (out, lse)
+
+
+def verify_drafts(
+    logits: torch.Tensor,
+    tokens: torch.Tensor,
+    cu_tokens: torch.Tensor,
+    max_tokens: int,
+    accept_u: torch.Tensor,
+    noise: torch.Tensor,
+    temperature: torch.Tensor,
+    *,
+    parents: torch.Tensor | None = None,
+    draft_probs: torch.Tensor | None = None,
+) -> Verification:
+    """Accept drafted tokens against the target's logits, and draw the next token.
+
+    ``logits`` [rows, V] (bf16, f16 or f32): row ``cu_tokens[b] + t`` is the
+    prediction after token t of request b, whose token 0 is the root;
+    ``tokens`` int64 [rows].  ``parents`` int32 [rows] gives a tree (default:
+    chains).  ``accept_u`` fp32 [rows] in [0, 1) decides each drafted token,
+    ``noise`` fp32 [B, V] (exponential, positive) the token after the last
+    accepted one, ``temperature`` fp32 [B] (0: greedy).  ``draft_probs`` fp32
+    [rows, V] are the distributions the tokens of chains were drawn from;
+    without them drafted tokens count as given.  The outputs follow the
+    target's distribution exactly (speculative sampling).
+    """
+    if logits.ndim != 2 or logits.dtype not in _ELEMENT:
+        raise TypeError("logits must be a BF16, FP16 or FP32 [rows, vocabulary] matrix")
+    _require_cuda(logits, "draft verification")
+    device = logits.device
+    rows, vocab = logits.shape
+    requests = temperature.shape[0] if temperature.ndim == 1 else -1
+    temps = _vector(temperature, torch.float32, "temperature", device)
+    cu = _vector(cu_tokens, torch.int32, "cu_tokens", device, requests + 1)
+    tok = _vector(tokens, torch.long, "tokens", device, rows)
+    coin = _vector(accept_u, torch.float32, "accept_u", device, rows)
+    if vocab == 0:
+        raise ValueError("draft verification requires a vocabulary")
+    if not 0 < max_tokens <= MAX_TREE_TOKENS:
+        raise ValueError(f"max_tokens must be from 1 to {MAX_TREE_TOKENS}")
+    if noise.dtype != torch.float32 or noise.ndim != 2:
+        raise TypeError("noise must be an FP32 [requests, vocabulary] matrix")
+    if noise.shape != (requests, vocab) or noise.device != device:
+        raise ValueError("noise must have a row for each request, on the logits' device")
+    par = probs = None
+    if parents is not None:
+        par = _vector(parents, torch.int32, "parents", device, rows)
+    if draft_probs is not None:
+        if parents is not None:
+            raise ValueError("draft_probs go with chains of drafted tokens, not with parents")
+        if draft_probs.dtype != torch.float32 or draft_probs.ndim != 2:
+            raise TypeError("draft_probs must be an FP32 [rows, vocabulary] matrix")
+        if draft_probs.shape != (rows, vocab) or draft_probs.device != device:
+            raise ValueError("draft_probs must have the shape and device of the logits")
+        probs = _unit_rows(draft_probs)
+    out = torch.empty((requests, max_tokens), dtype=torch.long, device=device)
+    path = torch.empty((requests, max_tokens), dtype=torch.int32, device=device)
+    accepted = torch.empty((requests,), dtype=torch.int32, device=device)
+    if requests == 0:
+        return Verification(out, path, accepted)
+    x, e = _unit_rows(logits), _unit_rows(noise)
+    need = _lib.lib().kb_verify_drafts_workspace_size(requests, rows)
+    # The size says how many requests and rows (each rounded up to a power of
+    # two) the buffer holds, so calls of one size share one layout.
+    ws = _workspace("verify", device, need, (_power_of_two(requests), need))
+    _lib.call(
+        "kb_verify_drafts", x.data_ptr(), max(x.stride(0), vocab), rows, vocab,
+        _ELEMENT[x.dtype], tok.data_ptr(), None if par is None else par.data_ptr(),
+        cu.data_ptr(), requests, max_tokens, coin.data_ptr(), e.data_ptr(),
+        max(e.stride(0), vocab), temps.data_ptr(), None if probs is None else probs.data_ptr(),
+        vocab if probs is None else max(probs.stride(0), vocab), out.data_ptr(),
+        path.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device),
+    )
+    return Verification(out, path, accepted)
+
+
+def _power_of_two(n: int) -> int:
+    return 1 << max(4, (n - 1).bit_length())
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix whose rows have unit stride and do not overlap."""
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t

@@ -1,0 +1,514 @@
+"""The speculative serving operators against their definitions in 64 bits (GPU).
+
+Attention tolerance.  Products of 16-bit inputs and their sums are held in
+fp32, the softmax weights are rounded once to the inputs' type before they
+meet the values (relative 2^-9 bf16, 2^-12 f16, so at most that times
+sum_j p_j |v_j|) and the result once more (that times |o|).  The tests allow
+twice this bound, for the fp32 sums and exponentials in between.  The
+log-sum-exp comes from fp32 scores alone: a score of up to 192 products is
+within 192 * 2^-24 * sum |q k| * scale, below 2e-4 for the inputs here.
+Whole numbers (slots, tokens, paths) have to be equal.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+from local_kimi_b200 import _lib, ops
+from oracle import speculative as ref
+
+pytestmark = pytest.mark.gpu
+
+STEP = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+LSE_TOL = 2e-4
+
+
+def check_attention(out, lse, want, want_lse, size, dtype):
+    o, e = out.detach().double().cpu(), want
+    assert torch.isfinite(o).all()
+    room = 2 * STEP[dtype] * (size + e.abs()) + 1e-6
+    bad = (o - e).abs() > room
+    assert not bool(bad.any()), (
+        f"{int(bad.sum())} of {bad.numel()} outputs off by up to "
+        f"{float(((o - e).abs() / room).max()):.3g} times the bound; first at "
+        f"{bad.nonzero()[0].tolist()}")
+    if lse is not None:
+        got = lse.double().cpu()
+        assert torch.equal(torch.isinf(got), torch.isinf(want_lse))
+        fin = torch.isfinite(want_lse)
+        assert float((got[fin] - want_lse[fin]).abs().max() if fin.any() else 0.0) < LSE_TOL
+
+
+def sums(values):
+    out = [0]
+    for v in values:
+        out.append(out[-1] + v)
+    return out
+
+
+def ints(values, cuda, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype, device=cuda)
+
+
+# ---------------------------------------------------------------------------
+# prompts
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,extra,heads,kv,dk,dv", [
+    ([1], [0], 1, 1, 64, 64),
+    ([5, 1, 0, 17], [0, 0, 0, 0], 4, 4, 192, 128),
+    ([130, 3, 127, 128, 129], [0, 1, 200, 0, 64], 8, 2, 128, 128),
+    ([257, 31], [0, 300], 6, 2, 72, 40),
+    ([300], [0], 7, 1, 96, 96),
+    ([513, 2], [0, 0], 3, 3, 192, 128),
+    ([64, 200, 1], [100, 0, 511], 16, 1, 128, 64),
+    ([40, 600], [0, 1], 5, 5, 8, 8),
+])
+def test_prompt_attention(cuda, dtype, lens, extra, heads, kv, dk, dv):
+    gen = torch.Generator().manual_seed(sum(lens) + heads)
+    keys = [n + x for n, x in zip(lens, extra)]
+    q = torch.randn(sum(lens), heads, dk, generator=gen).to(dtype)
+    k = torch.randn(sum(keys), kv, dk, generator=gen).to(dtype)
+    v = torch.randn(sum(keys), kv, dv, generator=gen).to(dtype)
+    cq, ck, scale = sums(lens), sums(keys), dk ** -0.5
+    out, lse = ops.prompt_attention(q.to(cuda), k.to(cuda), v.to(cuda), ints(cq, cuda),
+                                    max(lens), cu_seqlens_k=ints(ck, cuda), return_lse=True)
+    check_attention(out, lse, *ref.prompt_attention(q, k, v, cq, ck, scale), dtype)
+
+
+def test_prompt_attention_rows_without_keys(cuda):
+    # More queries than keys: the first rows of a request see nothing.
+    gen = torch.Generator().manual_seed(7)
+    lens, keys = [200, 5, 3], [60, 0, 3]
+    q = torch.randn(sum(lens), 4, 64, generator=gen).bfloat16()
+    k = torch.randn(sum(keys), 2, 64, generator=gen).bfloat16()
+    v = torch.randn(sum(keys), 2, 64, generator=gen).bfloat16()
+    cq, ck = sums(lens), sums(keys)
+    out, lse = ops.prompt_attention(q.to(cuda), k.to(cuda), v.to(cuda), ints(cq, cuda), 200,
+                                    cu_seqlens_k=ints(ck, cuda), return_lse=True)
+    check_attention(out, lse, *ref.prompt_attention(q, k, v, cq, ck, 0.125), torch.bfloat16)
+    assert float(out[:140].abs().max()) == 0.0 and torch.isinf(lse[:140]).all()
+
+
+def test_prompt_attention_strided_inputs_and_a_side_stream(cuda):
+    # Slices of one projection output, on a stream of their own.
+    gen = torch.Generator().manual_seed(8)
+    fused = torch.randn(333, 10, 128, generator=gen).half()
+    dev = fused.to(cuda)
+    q, k, v = fused[:, :6], fused[:, 6:8], fused[:, 8:]
+    cq = sums([133, 200])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = ops.prompt_attention(dev[:, :6], dev[:, 6:8], dev[:, 8:], ints(cq, cuda), 200,
+                                   scale=0.1)
+    side.synchronize()
+    want, _, size = ref.prompt_attention(q, k, v, cq, cq, 0.1)
+    check_attention(out, None, want, None, size, torch.float16)
+    # A width that is not a multiple of the row alignment's stride: copied first.
+    odd = torch.randn(50, 3, 67, generator=gen).half().to(cuda)[..., :64]
+    got = ops.prompt_attention(odd, odd, odd, ints([0, 50], cuda), 50)
+    x = odd.cpu()
+    want, _, size = ref.prompt_attention(x, x, x, [0, 50], [0, 50], 0.125)
+    check_attention(got, None, want, None, size, torch.float16)
+
+
+def test_prompt_attention_large_scores_and_infinite_neighbours(cuda):
+    # Scores up to several hundred (the running maximum moves), and a request
+    # whose neighbours hold infinities and not-a-numbers.
+    gen = torch.Generator().manual_seed(9)
+    lens = [100, 190, 70]
+    q = 6 * torch.randn(sum(lens), 2, 128, generator=gen)
+    k = 6 * torch.randn(sum(lens), 2, 128, generator=gen)
+    v = torch.randn(sum(lens), 2, 128, generator=gen)
+    for t in (q, k, v):
+        t[290:] = float("nan")
+        t[:100] = float("inf")
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    cq = sums(lens)
+    out, lse = ops.prompt_attention(q.to(cuda), k.to(cuda), v.to(cuda), ints(cq, cuda), 190,
+                                    return_lse=True)
+    want = ref.prompt_attention(q[100:290], k[100:290], v[100:290], [0, 190], [0, 190],
+                                128 ** -0.5)
+    # The scores are ~36 times larger than in the other tests, and so is their room.
+    o, e = out[100:290].double().cpu(), want[0]
+    assert torch.isfinite(o).all()
+    assert bool(((o - e).abs() <= 4 * STEP[torch.bfloat16] * (want[2] + e.abs()) + 1e-6).all())
+    assert float((lse[100:290].double().cpu() - want[1]).abs().max()) < 36 * LSE_TOL
+
+
+def test_prompt_attention_hidden_later_tokens_do_not_matter(cuda):
+    # What a row does not see does not change it, infinities included.
+    gen = torch.Generator().manual_seed(10)
+    x = torch.randn(150, 2, 64, generator=gen).bfloat16().to(cuda)
+    cu = ints([0, 150], cuda)
+    base = ops.prompt_attention(x, x, x, cu, 150)
+    y = x.clone()
+    y[100] = float("inf")
+    y[120] = float("nan")
+    got = ops.prompt_attention(x, x, y, cu, 150)
+    assert torch.equal(got[:100], base[:100])
+    assert not torch.isfinite(got[100:]).any()
+    got = ops.prompt_attention(x, y, x, cu, 150)
+    assert torch.equal(got[:100], base[:100])
+
+
+def test_prompt_attention_empty(cuda):
+    q = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device=cuda)
+    assert ops.prompt_attention(q, q, q, ints([0], cuda), 0).shape == (0, 2, 64)
+    assert ops.prompt_attention(q, q, q, ints([0, 0], cuda), 0).shape == (0, 2, 64)
+
+
+# ---------------------------------------------------------------------------
+# drafted tokens over the paged cache
+# ---------------------------------------------------------------------------
+
+
+def paged_case(cuda, dtype, ctx, new, heads, kv, dk, dv, ps, seed, head_major=True, tree=True):
+    """Caches with not-a-numbers wherever nothing was written."""
+    r, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+    need = [-(-(c + n) // ps) for c, n in zip(ctx, new)]
+    ids = list(range(sum(need) + 3))
+    r.shuffle(ids)
+    table = [[0] * (max(need) + 1) for _ in ctx]
+    shape = (len(ids), kv, ps) if head_major else (len(ids), ps, kv)
+    caches = []
+    for d in (dk, dv):
+        full = torch.full((*shape, d), float("nan"))
+        caches.append(full.transpose(1, 2) if head_major else full)
+    at = 0
+    for b, (c, n) in enumerate(zip(ctx, new)):
+        for i in range(need[b]):
+            table[b][i] = ids[at]
+            rows = min(ps, c + n - i * ps)
+            for cache in caches:
+                cache[ids[at], :rows] = torch.randn(rows, kv, cache.shape[3], generator=gen)
+            at += 1
+    kc, vc = (c.to(dtype) for c in caches)
+    q = torch.randn(sum(new), heads, dk, generator=gen).to(dtype)
+    parents = [([-1] + [r.randint(max(0, t - 3), t - 1) for t in range(1, n)])[:n] for n in new]
+    sees = [a for p in parents for a in ref.ancestors(p)] if tree else None
+    words = [w for p in parents for w in ref.tree_words(p)] if tree else None
+    dev = dict(q=q.to(cuda), k_cache=kc.to(cuda), v_cache=vc.to(cuda),
+               block_table=ints(table, cuda), context_lens=ints(ctx, cuda),
+               cu_tokens=ints(sums(new), cuda), max_tokens=max(new),
+               tree_mask=ints(words, cuda, torch.long) if tree else None)
+    want = ref.tree_attention(q, kc, vc, table, ctx, sums(new), sees, dk ** -0.5)
+    return dev, want
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ctx,new,heads,kv,dk,dv,ps,tree", [
+    ([0], [1], 1, 1, 64, 64, 8, False),
+    ([5, 64, 0, 63], [1, 1, 1, 1], 4, 4, 192, 128, 64, False),
+    ([300, 1, 700], [1, 1, 1], 32, 2, 128, 128, 16, False),
+    ([129, 31, 0, 500], [7, 12, 3, 1], 8, 2, 128, 128, 16, True),
+    ([100, 257], [24, 9], 8, 8, 192, 128, 32, True),
+    ([77, 10, 400], [48, 64, 33], 4, 1, 64, 64, 8, True),
+    ([200, 3], [5, 17], 6, 2, 72, 40, 128, True),
+    ([64, 90], [9, 40], 3, 3, 96, 96, 64, False),
+    ([1000, 0], [100, 70], 2, 1, 128, 128, 32, False),
+    ([33, 0, 8], [2, 0, 5], 5, 1, 128, 64, 256, True),
+    ([1500], [3], 64, 64, 192, 128, 64, True),
+])
+def test_tree_attention(cuda, dtype, ctx, new, heads, kv, dk, dv, ps, tree):
+    dev, want = paged_case(cuda, dtype, ctx, new, heads, kv, dk, dv, ps, 31 + heads, tree=tree)
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    check_attention(out, lse, *want, dtype)
+    # The workspace is left as it was found: the same call again.
+    again = ops.tree_attention(**dev)
+    assert torch.equal(out, again)
+
+
+def test_tree_attention_row_major_pages(cuda):
+    dev, want = paged_case(cuda, torch.bfloat16, [99, 200], [3, 6], 8, 2, 128, 128, 16, 5,
+                           head_major=False)
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    check_attention(out, lse, *want, torch.bfloat16)
+
+
+def test_tree_attention_many_requests(cuda):
+    r = random.Random(3)
+    ctx = [r.choice([0, 1, 15, 16, 17, r.randint(0, 300)]) for _ in range(150)]
+    new = [r.choice([0, 1, 1, 4]) for _ in range(150)]
+    new[0] = 4
+    dev, want = paged_case(cuda, torch.float16, ctx, new, 4, 2, 64, 64, 16, 6)
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    check_attention(out, lse, *want, torch.float16)
+
+
+def test_tree_attention_masks_that_hide_everything(cuda):
+    # No context and an empty word: the row is zero.
+    dev, _ = paged_case(cuda, torch.bfloat16, [0, 20], [3, 3], 4, 2, 64, 64, 16, 7)
+    dev["tree_mask"] = ints([0, 2, 7, 0, 1, 4], cuda, torch.long)
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    assert float(out[0].abs().max()) == 0.0 and torch.isinf(lse[0]).all()
+    q, kc, vc = (dev[n].cpu() for n in ("q", "k_cache", "v_cache"))
+    want = ref.tree_attention(q, kc, vc, dev["block_table"].tolist(), [0, 20], [0, 3, 6],
+                              [[], [1], [0, 1, 2], [], [0], [2]], 0.125)
+    check_attention(out, lse, *want, torch.bfloat16)
+
+
+def test_tree_attention_hidden_tokens_may_hold_anything(cuda):
+    # A drafted token with infinities is seen by itself alone.
+    dev, _ = paged_case(cuda, torch.bfloat16, [37], [4], 4, 2, 64, 64, 16, 8)
+    dev["tree_mask"] = ints([1, 3, 5, 9], cuda, torch.long)
+    base = ops.tree_attention(**dev)
+    page, row = divmod(37 + 2, 16)
+    page = int(dev["block_table"][0, page])
+    dev["v_cache"][page, row] = float("inf")
+    dev["k_cache"][page, row] = float("nan")
+    got = ops.tree_attention(**dev)
+    assert torch.equal(got[[0, 1, 3]], base[[0, 1, 3]])
+
+
+def test_tree_attention_pages_outside_the_cache_count_as_absent(cuda):
+    dev, _ = paged_case(cuda, torch.bfloat16, [50, 20], [2, 2], 4, 2, 64, 64, 16, 9, tree=False)
+    _lib_errors()
+    table = dev["block_table"]
+    table[0, 1] = -1
+    table[1, 0] = 10 ** 6
+    dev["block_table"] = table[:, :3]      # request 0 needs a fourth page
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    assert _lib_errors() == 4
+    q, kc, vc = (dev[n].cpu() for n in ("q", "k_cache", "v_cache"))
+    want = ref.tree_attention(q, kc, vc, dev["block_table"].tolist(), [50, 20], [0, 2, 4], None,
+                              0.125)
+    check_attention(out, lse, *want, torch.bfloat16)
+
+
+def _lib_errors():
+    torch.cuda.synchronize()
+    return _lib.device_errors()
+
+
+# ---------------------------------------------------------------------------
+# plan and append
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("requests,ps,longest,most,tree,pool,narrow", [
+    (1, 16, 0, 1, False, 1, 0),
+    (5, 8, 40, 9, True, 100, 0),
+    (300, 16, 500, 20, False, 5000, 0),
+    (3000, 64, 4000, 3, True, 9000, 0),
+    (40, 32, 200, 64, True, 7, 0),          # the pool runs out
+    (20, 8, 100, 30, False, 500, 4),        # the table is too narrow
+])
+def test_paged_plan(cuda, requests, ps, longest, most, tree, pool, narrow):
+    r = random.Random(requests + ps)
+    ctx = [r.choice([0, ps, ps - 1, r.randint(0, longest)]) for _ in range(requests)]
+    ctx = [min(c, longest) for c in ctx]
+    new = [r.choice([0, 1, most, r.randint(0, most)]) for _ in range(requests)]
+    width = max(max(-(-(c + n) // ps) for c, n in zip(ctx, new)) - narrow, 1) + (0 if narrow else 1)
+    table = [[r.randint(0, 10 ** 6) if i < -(-c // ps) else -7 for i in range(width)] for c in ctx]
+    free = [r.randint(0, 10 ** 6) for _ in range(pool + 2)]
+    total = sum(new) + 5
+    parents = [p for n in new for p in
+               ([-1] + [r.randint(max(0, t - 5), t - 1) for t in range(1, n)])[:n]]
+    parents = (parents + [-1] * 5) if tree else None
+    dev_table = ints(table, cuda)
+    got = ops.paged_plan(ints(ctx, cuda), ints(new, cuda), dev_table, ints(free, cuda),
+                         ints([2], cuda), ps, total,
+                         parents=ints(parents, cuda) if tree else None)
+    cu, slots, positions, masks, want_table, head, missing = ref.plan(
+        ctx, new, table, free, 2, ps, total, parents)
+    assert got.cu_tokens.tolist() == cu
+    assert got.slots.tolist() == slots
+    assert got.positions.tolist() == positions
+    assert dev_table.tolist() == want_table
+    assert got.free_head.tolist() == [head] and got.missing.tolist() == [missing]
+    if tree:
+        assert got.tree_mask.tolist() == masks
+    else:
+        assert got.tree_mask is None
+
+
+def test_paged_plan_flags_bad_trees_and_short_outputs(cuda):
+    _lib_errors()
+    table = torch.full((1, 4), -1, dtype=torch.int32, device=cuda)
+    args = (ints([0], cuda), ints([3], cuda), table, ints([5, 6], cuda), ints([0], cuda), 8)
+    got = ops.paged_plan(*args, 3, parents=ints([-1, 2, 0], cuda))
+    assert _lib_errors() == 8
+    assert got.tree_mask.tolist() == [1, 2, 5]
+    got = ops.paged_plan(*args, 2)
+    assert _lib_errors() == 4
+    assert got.cu_tokens.tolist() == [0, 2] and got.slots.tolist() == [40, 41]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,heads,dk,dv,ps,head_major", [
+    (1, 1, 64, 64, 8, True), (7, 3, 72, 40, 16, False), (300, 32, 192, 128, 64, True),
+    (1000, 2, 8, 128, 8, True),
+])
+def test_paged_append(cuda, dtype, tokens, heads, dk, dv, ps, head_major):
+    gen = torch.Generator().manual_seed(tokens)
+    pages = tokens // ps + 2
+    slots = torch.randperm(pages * ps, generator=gen)[:tokens]
+    if tokens > 3:
+        slots[2] = -1
+    kv = [torch.randn(tokens, heads + 1, d, generator=gen).to(dtype)[:, 1:] for d in (dk, dv)]
+    shape = (pages, heads, ps) if head_major else (pages, ps, heads)
+    caches = [torch.randn(*shape, d, generator=gen).to(dtype) for d in (dk, dv)]
+    views = [c.transpose(1, 2) if head_major else c for c in caches]
+    dev = [v.to(cuda) for v in views]
+    ops.paged_append(kv[0].to(cuda), kv[1].to(cuda), *dev, slots.to(cuda))
+    for x, view, got in zip(kv, views, dev):
+        want = view.clone()
+        for t, s in enumerate(slots.tolist()):
+            if s >= 0:
+                want[s // ps, s % ps] = x[t]
+        assert torch.equal(got.cpu(), want)
+
+
+def test_paged_append_flags_slots_outside_the_cache(cuda):
+    _lib_errors()
+    x = torch.ones(2, 1, 64, dtype=torch.half, device=cuda)
+    c = torch.zeros(2, 8, 1, 64, dtype=torch.half, device=cuda)
+    ops.paged_append(x, x, c, c.clone(), ints([16, 3], cuda, torch.long))
+    assert _lib_errors() == 4
+    assert float(c.sum()) == 64 and float(c[0, 3].sum()) == 64
+
+
+# ---------------------------------------------------------------------------
+# verification
+# ---------------------------------------------------------------------------
+
+
+def verify_case(requests, vocab, most, tree, probs, greedy, dtype, seed, sharp=2.0, empty=False):
+    r, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+    new = [r.randint(0 if empty else 1, most) for _ in range(requests)]
+    new[0] = most
+    cu = sums(new)
+    parents = [p for n in new for p in
+               ([-1] + [r.randint(max(0, t - 3), t - 1) if tree else t - 1
+                        for t in range(1, n)])[:n]]
+    logits = (sharp * torch.randn(cu[-1], vocab, generator=gen)).to(dtype)
+    q = torch.empty(cu[-1], vocab)
+    tokens = torch.zeros(cu[-1], dtype=torch.long)
+    for b in range(requests):
+        for t in range(new[b]):
+            row = cu[b] + t
+            base = logits[cu[b] + max(0, parents[row])].float()
+            q[row] = torch.softmax(base + 0.7 * torch.randn(vocab, generator=gen), 0)
+            tokens[row] = torch.multinomial(q[row], 1, generator=gen)
+    coin = torch.rand(cu[-1], generator=gen)
+    noise = torch.empty(requests, vocab).exponential_(generator=gen).clamp_min(1e-30)
+    temps = torch.tensor([0.0 if i < greedy else 0.8 for i in range(requests)])
+    return dict(logits=logits, tokens=tokens, parents=parents, cu=cu, most=most, coin=coin,
+                noise=noise, temps=temps, probs=q if probs else None)
+
+
+def run_verify(c, cuda, tree):
+    return ops.verify_drafts(
+        c["logits"].to(cuda), c["tokens"].to(cuda), ints(c["cu"], cuda), c["most"],
+        c["coin"].to(cuda), c["noise"].to(cuda), c["temps"].to(cuda),
+        parents=ints(c["parents"], cuda) if tree else None,
+        draft_probs=None if c["probs"] is None else c["probs"].to(cuda))
+
+
+@pytest.mark.parametrize("requests,vocab,most,tree,probs,greedy,dtype", [
+    (1, 7, 1, False, False, 0, torch.float32),
+    (6, 100, 5, False, True, 1, torch.float32),
+    (9, 1003, 9, True, False, 2, torch.bfloat16),
+    (40, 5000, 64, True, False, 0, torch.float16),
+    (3, 163840, 9, True, False, 1, torch.bfloat16),
+    (5, 50257, 6, False, True, 0, torch.bfloat16),
+    (33, 777, 4, False, False, 33, torch.float16),
+    (200, 257, 3, False, True, 7, torch.float32),
+])
+def test_verify_drafts(cuda, requests, vocab, most, tree, probs, greedy, dtype):
+    c = verify_case(requests, vocab, most, tree, probs, greedy, dtype, 50 + requests,
+                    empty=requests > 30)
+    want = ref.verify(c["logits"], c["tokens"], c["parents"], c["cu"], most, c["coin"],
+                      c["noise"], c["temps"], c["probs"])
+    for _ in range(2):          # the counters are left at zero
+        got = run_verify(c, cuda, tree)
+        assert got.accepted.tolist() == want[2]
+        assert got.path.tolist() == want[1]
+        assert got.tokens.tolist() == want[0]
+
+
+def test_verify_drafts_keeps_the_targets_distribution(cuda):
+    # 4000 requests, one drafted token each from q: the first emitted token is
+    # distributed as p, with and without q (5 sigma of a binomial count).
+    vocab, n = 12, 4000
+    gen = torch.Generator().manual_seed(77)
+    row = torch.randn(vocab, generator=gen)
+    p = torch.softmax(row.double(), 0)
+    q = torch.softmax(row + torch.randn(vocab, generator=gen), 0)
+    for probs in (True, False):
+        drafts = torch.multinomial(q, n, replacement=True, generator=gen)
+        tokens = torch.stack((torch.zeros_like(drafts), drafts), 1).flatten()
+        got = ops.verify_drafts(
+            row.expand(2 * n, vocab).contiguous().to(cuda), tokens.to(cuda),
+            torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=cuda), 2,
+            torch.rand(2 * n, generator=gen).to(cuda),
+            torch.empty(n, vocab).exponential_(generator=gen).to(cuda),
+            torch.ones(n, device=cuda),
+            draft_probs=q.expand(2 * n, vocab).contiguous().to(cuda) if probs else None)
+        count = torch.bincount(got.tokens[:, 0].cpu(), minlength=vocab).double()
+        off = (count - n * p).abs() / (n * p * (1 - p)).sqrt()
+        assert float(off.max()) < 5.0
+
+
+def test_verify_drafts_not_a_number_and_infinite_logits(cuda):
+    c = verify_case(4, 300, 3, True, False, 1, torch.float32, 9)
+    c["logits"][:, 5] = float("nan")
+    c["logits"][:, 9] = float("-inf")
+    want = ref.verify(c["logits"], c["tokens"], c["parents"], c["cu"], 3, c["coin"], c["noise"],
+                      c["temps"])
+    got = run_verify(c, cuda, True)
+    assert got.tokens.tolist() == want[0] and got.path.tolist() == want[1]
+    # One infinite logit takes everything.
+    c["logits"][:, 17] = float("inf")
+    got = run_verify(c, cuda, True)
+    last = got.tokens.gather(1, got.accepted.long()[:, None])
+    taken = (got.tokens == 17).any(dim=1)
+    assert bool(((last[:, 0] == 17) | taken).all())
+
+
+def test_verify_drafts_flags_bad_trees_and_tokens(cuda):
+    _lib_errors()
+    c = verify_case(2, 50, 3, False, False, 0, torch.float32, 10)
+    c["tokens"][1] = 50
+    got = run_verify(c, cuda, False)
+    assert _lib_errors() == 8
+    assert got.accepted.tolist()[0] == 0
+
+
+def test_operators_in_a_cuda_graph(cuda):
+    # Plan, append, attention and verification replayed from one graph.
+    dev, want = paged_case(cuda, torch.bfloat16, [50, 20], [4, 2], 4, 2, 64, 64, 16, 11)
+    c = verify_case(2, 500, 3, True, False, 0, torch.bfloat16, 12)
+    cd = {n: (t.to(cuda) if torch.is_tensor(t) else t) for n, t in c.items()}
+    cu, par = ints(c["cu"], cuda), ints(c["parents"], cuda)
+
+    def step():
+        out = ops.tree_attention(**dev)
+        got = ops.verify_drafts(cd["logits"], cd["tokens"], cu, 3, cd["coin"], cd["noise"],
+                                cd["temps"], parents=par)
+        return out, got
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = step()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        held = step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held[0], eager[0])
+    assert torch.equal(held[1].tokens, eager[1].tokens)
+    check_attention(held[0], None, want[0], None, want[2], torch.bfloat16)
+    assert math.isfinite(float(held[0].float().sum()))
