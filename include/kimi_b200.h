@@ -470,8 +470,7 @@ KB_API int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_
  * Other arguments as kb_prompt_attention; the workspace of
  * kb_tree_attention_workspace_size bytes is zeroed once and left zeroed where
  * a call needs it so. */
-KB_API size_t kb_tree_attention_workspace_size(int64_t Hkv, int64_t group, int64_t max_tokens,
-                   int64_t Dv);
+KB_API size_t kb_tree_attention_workspace_size(int64_t group, int64_t max_tokens);
 KB_API int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                    const uint16_t* k_cache, const int64_t* k_strides, const uint16_t* v_cache,
                    const int64_t* v_strides, int dtype, int64_t n_pages, int64_t page_size,

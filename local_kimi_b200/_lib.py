@@ -190,10 +190,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
          c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p],
     ),
-    "kb_tree_attention_workspace_size": (
-        c_size_t,
-        [c_int64, c_int64, c_int64, c_int64],
-    ),
+    "kb_tree_attention_workspace_size": (c_size_t, [c_int64, c_int64]),
     "kb_tree_attention": (
         c_int,
         [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
@@ -201,10 +198,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p,
          c_size_t, c_void_p],
     ),
-    "kb_verify_drafts_workspace_size": (
-        c_size_t,
-        [c_int64, c_int64],
-    ),
+    "kb_verify_drafts_workspace_size": (c_size_t, [c_int64, c_int64]),
     "kb_verify_drafts": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int64,

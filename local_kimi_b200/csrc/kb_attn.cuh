@@ -1,0 +1,148 @@
+// kb_attn.cuh - pieces shared by the attention kernels: the error path of
+// bounded waits, 16-bit element types, warp-level matrix steps and the host's
+// argument checks and tensor maps.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "kb_common.cuh"
+
+namespace kb {
+namespace attn {
+
+constexpr uint32_t ERR_WAIT = 2u;               // bounded wait ran out (device error bit 1)
+constexpr long long WAIT_NS = 2000000000LL;
+constexpr long long DRAIN_NS = 200000000LL;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ long long now_ns() {
+  long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Bounded wait on a barrier phase; false on abort or after 2 s (recorded, and
+// the CTA's other roles are told through the abort flag).
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_f,
+                                           uint32_t* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = now_ns();
+  while (true) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_f) return false;
+    if (now_ns() - t0 > WAIT_NS) {
+      *abort_f = 1;
+      atomicOr(err, ERR_WAIT);
+      return false;
+    }
+  }
+}
+
+// Wait on the error path for copies in flight: short limit, nothing recorded.
+__device__ __forceinline__ void drain_phase(uint64_t* bar, uint32_t parity) {
+  const long long t0 = now_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (now_ns() - t0 > DRAIN_NS) return;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 values rounded to a pair of 16-bit elements, `lo` in the low half.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t d;
+  if (F16) {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  }
+  return d;
+}
+
+template <bool F16>
+__device__ __forceinline__ float element(uint16_t bits) {
+  return F16 ? __half2float(__ushort_as_half(bits)) : bf16_bits_to_float(bits);
+}
+
+// Whether a 16-bit element is an infinity or not-a-number (exponent all ones).
+template <bool F16>
+__device__ __forceinline__ bool odd_element(uint16_t bits) {
+  const uint16_t m = F16 ? 0x7c00 : 0x7f80;
+  return (bits & m) == m;
+}
+
+// D[16x8] += A[16x16] * B[16x8], fp32 accumulate.
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if (F16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    mma_bf16_16816(d, a[0], a[1], a[2], a[3], b0, b1);
+  }
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            int w, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z),
+        "r"(w), "r"(smem_addr(bar)), "l"(policy)
+      : "memory");
+}
+
+__device__ __forceinline__ void fence_proxy_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Rows [first, end) of request b, cut to the rows there are.
+__device__ __forceinline__ void request_rows(const int* cu, int b, int64_t total, int64_t& first,
+                                             int64_t& end) {
+  first = min(max((int64_t)cu[b], (int64_t)0), total);
+  end = min(max((int64_t)cu[b + 1], first), total);
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+// ---------------------------------------------------------------------------
+int check_heads(int64_t Hq, int64_t Hkv, int64_t Dk, int64_t Dv, int dtype);
+
+// Tensor map over 16-bit elements [dims[3]][dims[2]][dims[1]][dims[0]], element
+// strides of the outer three, boxes of 64 x rows x box2 x 1 elements written in
+// the 128-byte swizzle; what lies outside the tensor reads as zero.
+int make_map_4d(CUtensorMap* map, const void* base, int f16, const int64_t (&dims)[4],
+                const int64_t (&strides)[3], int rows, int box2);
+
+// Dynamic shared-memory limit of a kernel, set once per device.
+int allow_smem(const void* kernel, int bytes, bool (&done)[64], std::mutex& mu);
+
+}  // namespace attn
+}  // namespace kb

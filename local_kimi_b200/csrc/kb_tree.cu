@@ -1,0 +1,840 @@
+// kb_tree.cu - attention of this step's tokens (one each, or drafted trees)
+// over the paged cache.
+//
+//   o_i = sum_j exp(s_ij - m_i) v_j / l_i,  s_ij = scale * q_i . k_j over the visible j,
+//   m_i = max_j s_ij, l_i = sum_j exp(s_ij - m_i), lse_i = m_i + log(l_i)
+// visible: j < context, or bit j - context of the token's tree word (without
+// words: j <= context + i).  A row that sees no key gives 0 and lse -infinity.
+//
+// Every cached key and value is read once and meets few rows (tokens x heads
+// of a group), so the bytes of the cache bound the work.  The rows of one
+// (request, key/value head) are one A operand of 16, 32 or 64 rows for the
+// warp-level matrix instruction (more rows: several blocks, which find the
+// cache in L2); at 16 rows the 5th-generation tensor core would spend 7/8 of
+// its 128-row tile on padding and need its results moved back for the softmax.
+//
+// Work split.  All (request, head, row block, 64-key tile) units form one line
+// of tiles, cut into equal runs, one per CTA: any mix of lengths keeps every SM
+// reading to the end.  A (request, head, block) whose tiles fall to several
+// CTAs is joined from their fp32 partial sums by the CTA that finishes last
+// (in CTA order, so results do not change from run to run).
+//
+// A CTA: one producer warp walks the run, looks pages up (32 table entries at a
+// time) and brings each tile in by tensor copies in the 128-byte swizzle (box:
+// one page's rows, 64 elements), several tiles ahead; the rows of q come the
+// same way, one row a copy.  4 or 8 consumer warps: each takes 16 rows and a
+// share of the tile's keys with its own running maximum and sum in registers,
+// so no barrier among them is needed until the run's or the unit's end.
+//
+// Rows of a page past the request's end were never written and may hold
+// anything: they are masked as keys and zeroed as values.  A value that is
+// infinite or not a number in a hidden drafted token must not meet a zero
+// weight: such elements are taken out of the tile and added to the rows that
+// see them.
+#include <algorithm>
+
+#include "kb_attn.cuh"
+
+namespace kb {
+namespace attn {
+
+constexpr int KT = 64;                     // keys of a tile
+constexpr int CHUNK = KT * 128;            // bytes of 64 keys x 64 elements
+constexpr int MAX_CTAS = 320;              // counters in the workspace
+constexpr int MIN_TILES = 2;               // tiles that make another CTA worth its partial sums
+
+struct TreeArgs {
+  const uint16_t* q;
+  int64_t q_tok, q_head;
+  uint16_t* out;            // [total, Hq, Dv] contiguous
+  float* lse;               // [total, Hq] or NULL
+  const int* cu;
+  const int* table;
+  int64_t table_stride;
+  const int* context;
+  const int64_t* mask;
+  int64_t n_pages, total;
+  int B, width, ps, Hq, Hkv, g, Dk, Dv;
+  float scale2;             // scale * log2(e)
+  int* counters;            // [MAX_CTAS], zero between calls
+  float* part_ml;           // [2 * CTAs][rows][2]: m (log2), l
+  float* part_o;            // [2 * CTAs][rows][DVP]
+  uint32_t* err;
+};
+
+// What the consumers need to know about the run's part of one unit.
+struct Segment {
+  int64_t first;            // first row (token) of the request
+  int64_t ctx;              // cached tokens before this step's
+  int n;                    // this step's tokens
+  int hk, row0, rows;       // head, first row of the block (token * g + head), rows in it
+  int whole;                // the run holds all of the unit's tiles
+  int starts;               // ... its first tile
+  int c0, parts;            // the CTAs that share the unit: first, number
+};
+
+template <int DKP, int DVP, int MT>
+struct TreeShape {
+  static constexpr int RB = 16 * MT;                       // rows of a block
+  static constexpr int WK = MT == 4 ? 2 : 4;               // warps sharing a tile's keys
+  static constexpr int NW = MT * WK;                       // consumer warps
+  static constexpr int KPW = KT / WK;                      // keys of a warp
+  static constexpr int THREADS = (NW + 1) * 32;
+  static constexpr int KC = DKP / 64, VC = DVP / 64;
+  static constexpr int STAGE = (KC + VC) * CHUNK;
+  static constexpr int QP = DKP * 2 + 16;                  // row pitch of q: no bank conflicts
+  static constexpr int Q_BYTES = RB * QP;
+  static constexpr int X_BYTES = MT * (WK / 2) * 32 * (DVP / 2 + 4) * 4;
+  static constexpr int CTAS_PER_SM = MT == 1 ? 2 : 1;
+  static constexpr int BUDGET = MT == 1 ? 113 * 1024 : 224 * 1024;
+  static constexpr int FIXED = 2 * Q_BYTES + X_BYTES + 1024 + 2048;   // alignment, barriers
+  static constexpr int FIT = (BUDGET - FIXED) / STAGE;
+  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr int SMEM = FIXED + STAGES * STAGE;
+  static_assert(STAGES >= 2, "two tiles in flight at least");
+};
+
+template <int STAGES>
+struct TreeBars {
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t all, share[4];     // consumer warps together; those with the same keys
+  uint64_t valid[STAGES];     // which keys of the tile exist
+  int64_t key0[STAGES];       // first key of the tile
+  int last[STAGES];           // last tile of its segment
+  Segment seg[2];
+  int64_t scan[16];
+  int64_t total, base;
+  int b, abort_flag, joined;
+};
+
+// Keys [lo, hi) of the line of tiles that CTA c of n takes.
+__device__ __forceinline__ int64_t run_start(int64_t tiles, int n, int c) { return tiles * c / n; }
+__device__ __forceinline__ int run_of(int64_t tiles, int n, int64_t x) {
+  return (int)(((x + 1) * n - 1) / tiles);
+}
+
+template <int DKP, int DVP, int MT, bool F16>
+__global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
+                                  TreeShape<DKP, DVP, MT>::CTAS_PER_SM)
+    tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                const TreeArgs A) {
+  using S = TreeShape<DKP, DVP, MT>;
+  using Bars = TreeBars<S::STAGES>;
+  static_assert(sizeof(Bars) <= 2048, "barrier block");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      smem_raw + ((1024u - (static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw)) & 1023u)) &
+                  1023u);
+  uint8_t* ring = smem;                                       // [STAGES][K chunks, V chunks]
+  uint8_t* qbuf = ring + S::STAGES * S::STAGE;                // [2][RB][QP]
+  float* xbuf = reinterpret_cast<float*>(qbuf + 2 * S::Q_BYTES);
+  Bars* B = reinterpret_cast<Bars*>(qbuf + 2 * S::Q_BYTES + S::X_BYTES);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile int* abort_f = &B->abort_flag;
+
+  if (tid == 0) {
+    for (int i = 0; i < S::STAGES; ++i) {
+      mbar_init(&B->full[i], 1);
+      mbar_init(&B->empty[i], S::NW);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->q_full[i], 1);
+      mbar_init(&B->q_empty[i], S::NW);
+    }
+    mbar_init(&B->all, S::NW);
+    for (int i = 0; i < S::WK; ++i) mbar_init(&B->share[i], MT);
+    B->abort_flag = 0;
+    B->b = 0;
+    B->base = 0;
+    mbar_fence_init();
+  }
+  // Columns of q past the head's width stay zero (the copies do not write them).
+  for (int i = tid; i < 2 * S::Q_BYTES / 16; i += S::THREADS)
+    reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // Tiles of each request and their running sum; the request this run starts in.
+  const int per = (A.B + S::THREADS - 1) / S::THREADS;
+  const int b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
+  auto tiles_of = [&](int b, int64_t& first, int& n, int64_t& ctx, int64_t& t, int& blocks) {
+    int64_t end;
+    request_rows(A.cu, b, A.total, first, end);
+    n = (int)(end - first);
+    ctx = max(A.context[b], 0);
+    t = n ? (ctx + n + KT - 1) / KT : 0;
+    blocks = (int)(((int64_t)n * A.g + S::RB - 1) / S::RB);
+  };
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    int64_t first, ctx, t;
+    int n, blocks;
+    tiles_of(b, first, n, ctx, t, blocks);
+    mine += t * blocks * A.Hkv;
+  }
+  int64_t incl = mine;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) B->scan[warp] = incl;
+  __syncthreads();
+  int64_t excl = incl - mine, total = 0;
+  for (int w = 0; w < S::NW + 1; ++w) {
+    if (w < warp) excl += B->scan[w];
+    total += B->scan[w];
+  }
+  // Rows outside every request: zero.
+  {
+    const int64_t lead = min(max((int64_t)A.cu[0], (int64_t)0), A.total);
+    const int64_t tail = min(max((int64_t)A.cu[A.B], lead), A.total);
+    const int64_t spare = (lead + A.total - tail) * A.Hq;
+    for (int64_t i = (int64_t)blockIdx.x * S::THREADS + tid; i < spare;
+         i += (int64_t)gridDim.x * S::THREADS) {
+      const int64_t r = i < lead * A.Hq ? i : i - lead * A.Hq + tail * A.Hq;
+      for (int d = 0; d < A.Dv; d += 8)
+        *reinterpret_cast<uint4*>(A.out + r * A.Dv + d) = make_uint4(0, 0, 0, 0);
+      if (A.lse) A.lse[r] = -INFINITY;
+    }
+  }
+  const int ctas = (int)min((int64_t)gridDim.x, max((total + MIN_TILES - 1) / MIN_TILES,
+                                                    (int64_t)1));
+  const int cta = blockIdx.x;
+  if (cta >= ctas || total == 0) return;
+  const int64_t lo = run_start(total, ctas, cta), hi = run_start(total, ctas, cta + 1);
+  if (mine > 0 && excl <= lo && lo < excl + mine) {
+    int64_t at = excl;
+    for (int b = b0; b < b1; ++b) {
+      int64_t first, ctx, t;
+      int n, blocks;
+      tiles_of(b, first, n, ctx, t, blocks);
+      const int64_t w = t * blocks * A.Hkv;
+      if (lo < at + w) {
+        B->b = b;
+        B->base = at;
+        break;
+      }
+      at += w;
+    }
+  }
+  __syncthreads();
+
+  if (warp == S::NW) {
+    // ---------------------------------------------------------------- producer
+    const uint64_t pol = l2_evict_first_policy();
+    const int ps = A.ps, shift = 31 - __clz(ps);
+    const int box = min(ps, KT), ppt = KT / box;
+    int64_t pos = lo, base = B->base;
+    int b = B->b, seg = 0, stage = 0;
+    uint32_t phase = 0;
+    bool ok = true, again = false;
+    while (pos < hi && ok) {
+      int64_t first, ctx, t;
+      int n, blocks;
+      tiles_of(b, first, n, ctx, t, blocks);
+      const int64_t w = t * blocks;
+      if (pos >= base + w * A.Hkv) {
+        base += w * A.Hkv;
+        ++b;
+        continue;
+      }
+      const int64_t off = pos - base;
+      const int hk = (int)(off / w);
+      const int64_t rem = off - hk * w;
+      const int rb = (int)(rem / t);
+      const int64_t t0 = rem - rb * t, u0 = pos - t0;
+      const int64_t t1 = min(t, t0 + (hi - pos));
+      const int sb = seg & 1;
+      if (seg >= 2 && !wait_phase(&B->q_empty[sb], ((seg >> 1) - 1) & 1, abort_f, A.err)) break;
+      const int row0 = rb * S::RB;
+      const int rows = (int)min((int64_t)S::RB, (int64_t)n * A.g - row0);
+      if (lane == 0) {
+        Segment& G = B->seg[sb];
+        G.first = first;
+        G.ctx = ctx;
+        G.n = n;
+        G.hk = hk;
+        G.row0 = row0;
+        G.rows = rows;
+        G.whole = t0 == 0 && t1 == t;
+        G.starts = t0 == 0;
+        G.c0 = run_of(total, ctas, u0);
+        G.parts = run_of(total, ctas, u0 + t - 1) - G.c0 + 1;
+        mbar_arrive_expect_tx(&B->q_full[sb], (uint32_t)(rows * A.Dk * 2));
+      }
+      __syncwarp();
+      for (int r = lane; r < rows; r += 32) {
+        const int tok = (row0 + r) / A.g, h = row0 + r - tok * A.g;
+        bulk_g2s(qbuf + sb * S::Q_BYTES + r * S::QP,
+                 A.q + (first + tok) * A.q_tok + (int64_t)(hk * A.g + h) * A.q_head,
+                 (uint32_t)(A.Dk * 2), &B->q_full[sb], pol);
+      }
+      const int64_t end = ctx + n;
+      int64_t have = -1;         // first table entry held by lane 0
+      int ids = -1;
+      for (int64_t tile = t0; tile < t1; ++tile) {
+        if (again && !wait_phase(&B->empty[stage], phase ^ 1u, abort_f, A.err)) {
+          ok = false;
+          break;
+        }
+        const int64_t key0 = tile * KT, entry = key0 >> shift;
+        if (have < 0 || entry + ppt > have + 32) {
+          have = entry;
+          const int64_t e = have + lane;
+          ids = e < A.width && e * ps < end ? A.table[(int64_t)b * A.table_stride + e] : -1;
+        }
+        const int at = (int)(entry - have);
+        const int mine_id = __shfl_sync(0xffffffffu, ids, min(at + min(lane, ppt - 1), 31));
+        const bool there = mine_id >= 0 && mine_id < A.n_pages;
+        const unsigned live = __ballot_sync(0xffffffffu, lane < ppt && there);
+        const int64_t left = end - key0;
+        uint64_t valid = left >= KT ? ~0ull : (1ull << left) - 1ull;
+        if (live != (ppt == 32 ? 0xffffffffu : (1u << ppt) - 1u)) {
+          uint64_t got = 0;
+          for (int i = 0; i < ppt; ++i)
+            if ((live >> i) & 1)
+              got |= (box == 64 ? ~0ull : ((1ull << box) - 1ull)) << (i * box);
+          if (lane == 0 && (valid & ~got)) atomicOr(A.err, ERR_PAGE);
+          valid &= got;
+        }
+        if (lane == 0) {
+          B->valid[stage] = valid;
+          B->key0[stage] = key0;
+          B->last[stage] = tile + 1 == t1;
+          mbar_arrive_expect_tx(&B->full[stage],
+                                (uint32_t)(__popc(live) * box * 128 * (S::KC + S::VC)));
+        }
+        __syncwarp();
+        // One copy per page and 64-element column block.
+        uint8_t* dst = ring + stage * S::STAGE;
+        const int row = ppt > 1 ? 0 : (int)(key0 & (ps - 1));
+        for (int i0 = 0; i0 < ppt * (S::KC + S::VC); i0 += 32) {
+          const int i = i0 + lane;
+          const int p = min(i / (S::KC + S::VC), ppt - 1), c = i - p * (S::KC + S::VC);
+          const int id = __shfl_sync(0xffffffffu, mine_id, p);
+          if (i >= ppt * (S::KC + S::VC) || !((live >> p) & 1)) continue;
+          if (c < S::KC)
+            tma_load_4d(dst + c * CHUNK + p * box * 128, &tk, c * 64, row, hk, id,
+                        &B->full[stage], pol);
+          else
+            tma_load_4d(dst + c * CHUNK + p * box * 128, &tv, (c - S::KC) * 64, row, hk, id,
+                        &B->full[stage], pol);
+        }
+        __syncwarp();
+        if (++stage == S::STAGES) {
+          stage = 0;
+          phase ^= 1u;
+          again = true;
+        }
+      }
+      pos += t1 - t0;
+      ++seg;
+    }
+    // On the error path, copies in flight land before the CTA may exit.
+    if (*abort_f) {
+      for (int i = 0; i < S::STAGES; ++i) {
+        drain_phase(&B->full[i], 0);
+        drain_phase(&B->full[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        drain_phase(&B->q_full[i], 0);
+        drain_phase(&B->q_full[i], 1);
+      }
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int wm = warp / S::WK, wk = warp - wm * S::WK;
+  int stage = 0, seg = 0;
+  uint32_t phase = 0;
+  int64_t pos = lo;
+  const int frow = lane >> 2, fcol = (lane & 3) * 2;     // accumulator row and column
+  // Barriers among consumer warps, bounded like every wait.
+  uint32_t all_phase = 0, share_phase = 0;
+  auto meet = [&](uint64_t* bar, uint32_t& ph) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+    const bool ok = wait_phase(bar, ph, abort_f, A.err);
+    ph ^= 1u;
+    return ok;
+  };
+  while (pos < hi) {
+    const int sb = seg & 1;
+    if (!wait_phase(&B->q_full[sb], (seg >> 1) & 1, abort_f, A.err)) return;
+    const Segment G = B->seg[sb];
+    uint32_t qf[DKP / 16][4];
+    {
+      const uint32_t base = smem_addr(qbuf + sb * S::Q_BYTES) +
+                            (uint32_t)((wm * 16 + (lane & 15)) * S::QP + (lane >> 4) * 16);
+#pragma unroll
+      for (int k = 0; k < DKP / 16; ++k) ldmatrix_x4(qf[k], base + k * 32);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B->q_empty[sb]);
+    // The tree words of this thread's two rows.
+    int tok[2];
+    uint64_t word[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = wm * 16 + frow + i * 8;
+      tok[i] = (G.row0 + min(r, G.rows - 1)) / A.g;
+      word[i] = A.mask ? (uint64_t)A.mask[G.first + tok[i]] : 0;
+    }
+    auto sees = [&](int i, int64_t key) {
+      const int64_t j = key - G.ctx;
+      if (j < 0) return true;
+      return A.mask ? (j < 64 && ((word[i] >> j) & 1)) : j <= tok[i];
+    };
+    float o[DVP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DVP / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (bool last = false; !last;) {
+      if (!wait_phase(&B->full[stage], phase, abort_f, A.err)) return;
+      last = B->last[stage] != 0;
+      const uint64_t valid = B->valid[stage];
+      const int64_t key0 = B->key0[stage];
+      const bool step_keys = key0 + KT > G.ctx;
+      uint8_t* kt = ring + stage * S::STAGE;
+      uint8_t* vt = kt + S::KC * CHUNK;
+      float s[S::KPW / 8][4];
+#pragma unroll
+      for (int i = 0; i < S::KPW / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < DKP / 16; ++k) {
+#pragma unroll
+        for (int n = 0; n < S::KPW / 16; ++n) {
+          const int row = wk * S::KPW + n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+          const int piece = (k & 3) * 2 + ((lane >> 3) & 1);
+          uint32_t b[4];
+          ldmatrix_x4(b, smem_addr(kt) + (uint32_t)((k >> 2) * CHUNK + row * 128 +
+                                                    ((piece ^ (row & 7)) << 4)));
+          mma_16816<F16>(s[2 * n], qf[k], b[0], b[1]);
+          mma_16816<F16>(s[2 * n + 1], qf[k], b[2], b[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S::KPW / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] *= A.scale2;
+      if (step_keys || valid != ~0ull) {
+#pragma unroll
+        for (int i = 0; i < S::KPW / 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = wk * S::KPW + i * 8 + fcol + (j & 1);
+            if (!((valid >> c) & 1) || !sees(j >> 1, key0 + c)) s[i][j] = -INFINITY;
+          }
+        // Elements of this step's values that are no numbers go to the rows
+        // that see them and leave the tile, which the warps with the same keys
+        // do together; values of keys that do not exist become zero.
+        constexpr uint32_t KEYS = S::KPW == 32 ? 0xffffffffu : (1u << S::KPW) - 1u;
+        const uint32_t gone = ~(uint32_t)(valid >> (wk * S::KPW)) & KEYS;
+        uint32_t odd_rows = 0;
+        if (step_keys && (G.n > 1 || A.mask)) {
+          for (int r = 0; r < S::KPW; ++r) {
+            const int c = wk * S::KPW + r;
+            if (((gone >> r) & 1) || key0 + c < G.ctx) continue;
+            bool odd = false;
+            for (int x = lane; x < DVP / 2; x += 32) {
+              const uint32_t u = *reinterpret_cast<const uint32_t*>(
+                  vt + (x >> 5) * CHUNK + c * 128 + ((((x >> 2) & 7) ^ (c & 7)) << 4) +
+                  (x & 3) * 4);
+              odd = odd || odd_element<F16>((uint16_t)u) || odd_element<F16>((uint16_t)(u >> 16));
+            }
+            if (!__any_sync(0xffffffffu, odd)) continue;
+            odd_rows |= 1u << r;
+#pragma unroll
+            for (int i = 0; i < DVP / 8; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int d = i * 8 + fcol + j;
+                const uint16_t u = *reinterpret_cast<const uint16_t*>(
+                    vt + (d >> 6) * CHUNK + c * 128 + ((((d >> 3) & 7) ^ (c & 7)) << 4) +
+                    (d & 7) * 2);
+                if (!odd_element<F16>(u)) continue;
+                if (sees(0, key0 + c)) o[i][j] += element<F16>(u);
+                if (sees(1, key0 + c)) o[i][j + 2] += element<F16>(u);
+              }
+          }
+          if (MT > 1 && !meet(&B->share[wk], share_phase)) return;
+        }
+        if (gone | odd_rows) {
+          __syncwarp();
+          for (int x = lane; x < S::KPW * (DVP / 8); x += 32) {
+            const int r = x / (DVP / 8), c = wk * S::KPW + r, piece = x - r * (DVP / 8);
+            uint4* at = reinterpret_cast<uint4*>(vt + (piece >> 3) * CHUNK + c * 128 +
+                                                 (((piece & 7) ^ (c & 7)) << 4));
+            if ((gone >> r) & 1) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else if ((odd_rows >> r) & 1) {
+              uint16_t* e = reinterpret_cast<uint16_t*>(at);
+              for (int j = 0; j < 8; ++j)
+                if (odd_element<F16>(e[j])) e[j] = 0;
+            }
+          }
+          fence_proxy_async();     // before the next copy into this stage
+          __syncwarp();
+        }
+      }
+      float top[2] = {m[0], m[1]};
+#pragma unroll
+      for (int i = 0; i < S::KPW / 8; ++i) {
+        top[0] = fmaxf(top[0], fmaxf(s[i][0], s[i][1]));
+        top[1] = fmaxf(top[1], fmaxf(s[i][2], s[i][3]));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      }
+      if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+        float fix[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fix[i] = top[i] == -INFINITY ? 1.f : exp2_fast(m[i] - top[i]);
+          l[i] *= fix[i];
+          m[i] = top[i];
+        }
+#pragma unroll
+        for (int i = 0; i < DVP / 8; ++i) {
+          o[i][0] *= fix[0];
+          o[i][1] *= fix[0];
+          o[i][2] *= fix[1];
+          o[i][3] *= fix[1];
+        }
+      }
+      const float at0 = m[0] == -INFINITY ? 0.f : m[0], at1 = m[1] == -INFINITY ? 0.f : m[1];
+      uint32_t p[S::KPW / 16][4];
+#pragma unroll
+      for (int i = 0; i < S::KPW / 8; ++i) {
+        const float e0 = exp2_fast(s[i][0] - at0), e1 = exp2_fast(s[i][1] - at0);
+        const float e2 = exp2_fast(s[i][2] - at1), e3 = exp2_fast(s[i][3] - at1);
+        l[0] += e0 + e1;
+        l[1] += e2 + e3;
+        // One rounding of the weights, to the type the tensor core multiplies.
+        p[i >> 1][(i & 1) * 2] = pack2<F16>(e0, e1);
+        p[i >> 1][(i & 1) * 2 + 1] = pack2<F16>(e2, e3);
+      }
+#pragma unroll
+      for (int n = 0; n < S::KPW / 16; ++n) {
+        const int row = wk * S::KPW + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < DVP / 16; ++i) {
+          const int piece = (i & 3) * 2 + (lane >> 4);
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, smem_addr(vt) + (uint32_t)((i >> 2) * CHUNK + row * 128 +
+                                                          ((piece ^ (row & 7)) << 4)));
+          mma_16816<F16>(o[2 * i], p[n], b[0], b[1]);
+          mma_16816<F16>(o[2 * i + 1], p[n], b[2], b[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B->empty[stage]);
+      if (++stage == S::STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+      ++pos;
+    }
+    ++seg;
+
+    // Join the warps that shared the keys: half of them hand over, then half
+    // of the rest.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    constexpr int XF = DVP / 2 + 4;
+#pragma unroll
+    for (int half = S::WK / 2; half >= 1; half >>= 1) {
+      float* x = xbuf + (size_t)(wm * (S::WK / 2) + (wk & (half - 1))) * 32 * XF + lane;
+      if (wk >= half && wk < 2 * half) {
+#pragma unroll
+        for (int i = 0; i < DVP / 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[(i * 4 + j) * 32] = o[i][j];
+        x[(XF - 4) * 32] = m[0];
+        x[(XF - 3) * 32] = m[1];
+        x[(XF - 2) * 32] = l[0];
+        x[(XF - 1) * 32] = l[1];
+      }
+      if (!meet(&B->all, all_phase)) return;
+      if (wk < half) {
+        float f0[2], f1[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float om = x[(XF - 4 + i) * 32], ol = x[(XF - 2 + i) * 32];
+          const float t = fmaxf(m[i], om);
+          f0[i] = t == -INFINITY ? 1.f : exp2_fast(m[i] - t);
+          f1[i] = t == -INFINITY ? 1.f : exp2_fast(om - t);
+          m[i] = t;
+          l[i] = l[i] * f0[i] + ol * f1[i];
+        }
+#pragma unroll
+        for (int i = 0; i < DVP / 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[i][j] = o[i][j] * f0[j >> 1] + x[(i * 4 + j) * 32] * f1[j >> 1];
+      }
+      if (!meet(&B->all, all_phase)) return;
+    }
+
+    if (wk == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = wm * 16 + frow + h * 8;
+        if (r >= G.rows) continue;
+        if (G.whole) {
+          const int t = (G.row0 + r) / A.g;
+          const int64_t at = (G.first + t) * A.Hq + G.hk * A.g + (G.row0 + r - t * A.g);
+          const float inv = l[h] > 0.f ? 1.f / l[h] : l[h] == 0.f ? 0.f : l[h];
+          uint16_t* out = A.out + at * A.Dv;
+#pragma unroll
+          for (int i = 0; i < DVP / 8; ++i)
+            if (i * 8 < A.Dv)
+              *reinterpret_cast<uint32_t*>(out + i * 8 + fcol) =
+                  pack2<F16>(o[i][2 * h] * inv, o[i][2 * h + 1] * inv);
+          if (A.lse && (lane & 3) == 0)
+            A.lse[at] = l[h] == 0.f ? -INFINITY : (m[h] + log2f(l[h])) * LN2;
+        } else {
+          const int64_t slot = ((int64_t)cta * 2 + G.starts) * S::RB + r;
+          float* po = A.part_o + slot * DVP;
+#pragma unroll
+          for (int i = 0; i < DVP / 8; ++i)
+            *reinterpret_cast<float2*>(po + i * 8 + fcol) =
+                make_float2(o[i][2 * h], o[i][2 * h + 1]);
+          if ((lane & 3) == 0)
+            *reinterpret_cast<float2*>(A.part_ml + slot * 2) = make_float2(m[h], l[h]);
+        }
+      }
+    }
+    if (G.whole) continue;
+
+    // The last of the unit's CTAs joins their sums, in CTA order.
+    __threadfence();
+    if (!meet(&B->all, all_phase)) return;
+    if (tid == 0) {
+      const int old = atomicAdd(&A.counters[G.c0], 1);
+      B->joined = old == G.parts - 1;
+      if (B->joined) A.counters[G.c0] = 0;
+    }
+    if (!meet(&B->all, all_phase)) return;
+    if (B->joined) {
+      __threadfence();
+      // Few items: several threads share an item's partial sums.
+      constexpr int T = S::NW * 32;
+      const int quads = A.Dv / 4, items = G.rows * quads;
+      int share = 1;
+      while (share < 32 && share * 2 * items <= T) share *= 2;
+      for (int base = 0; base < items; base += T / share) {
+        const int it = base + tid % (T / share), sh = tid / (T / share);
+        const int r = min(it, items - 1) / quads, d = (min(it, items - 1) - r * quads) * 4;
+        float tm = -INFINITY, tl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = sh; c < G.parts; c += 4 * share) {
+          float2 ml[4];
+          float4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int cc = c + u * share;
+            ml[u] = make_float2(-INFINITY, 0.f);
+            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (cc < G.parts) {
+              const int64_t slot = ((int64_t)(G.c0 + cc) * 2 + (cc == 0)) * S::RB + r;
+              ml[u] = __ldcg(reinterpret_cast<const float2*>(A.part_ml + slot * 2));
+              v[u] = __ldcg(reinterpret_cast<const float4*>(A.part_o + slot * DVP + d));
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float t = fmaxf(tm, ml[u].x);
+            if (t == -INFINITY) continue;
+            const float f0 = exp2_fast(tm - t), f1 = exp2_fast(ml[u].x - t);
+            tm = t;
+            tl = tl * f0 + ml[u].y * f1;
+            acc[0] = acc[0] * f0 + v[u].x * f1;
+            acc[1] = acc[1] * f0 + v[u].y * f1;
+            acc[2] = acc[2] * f0 + v[u].z * f1;
+            acc[3] = acc[3] * f0 + v[u].w * f1;
+          }
+        }
+        if (share > 1) {
+          // Through shared memory, in order.
+          float* x = xbuf + tid * 6;
+          x[0] = tm;
+          x[1] = tl;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[2 + j] = acc[j];
+          if (!meet(&B->all, all_phase)) return;
+          if (sh == 0)
+            for (int u = 1; u < share; ++u) {
+              const float* y = xbuf + (tid + u * (T / share)) * 6;
+              const float t = fmaxf(tm, y[0]);
+              if (t == -INFINITY) continue;
+              const float f0 = exp2_fast(tm - t), f1 = exp2_fast(y[0] - t);
+              tm = t;
+              tl = tl * f0 + y[1] * f1;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[j] = acc[j] * f0 + y[2 + j] * f1;
+            }
+          if (!meet(&B->all, all_phase)) return;
+        }
+        if (sh == 0 && it < items) {
+          const int t = (G.row0 + r) / A.g;
+          const int64_t at = (G.first + t) * A.Hq + G.hk * A.g + (G.row0 + r - t * A.g);
+          const float inv = tl > 0.f ? 1.f / tl : tl == 0.f ? 0.f : tl;
+          uint2 w;
+          w.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
+          w.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
+          *reinterpret_cast<uint2*>(A.out + at * A.Dv + d) = w;
+          if (A.lse && d == 0) A.lse[at] = tl == 0.f ? -INFINITY : (tm + log2f(tl)) * LN2;
+        }
+      }
+    }
+    if (!meet(&B->all, all_phase)) return;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+// ---------------------------------------------------------------------------
+
+// CTAs of a launch at most: two an SM for 16-row blocks, else one.
+static int max_ctas(int mt) { return mt == 1 ? MAX_CTAS : MAX_CTAS / 2; }
+
+static int row_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+template <int DKP, int DVP, int MT, bool F16>
+static int launch_tree(const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A, int sms,
+                       void* stream) {
+  using S = TreeShape<DKP, DVP, MT>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  const void* fn = reinterpret_cast<const void*>(&tree_kernel<DKP, DVP, MT, F16>);
+  const int st = allow_smem(fn, S::SMEM, done, mu);
+  if (st != KB_OK) return st;
+  const int grid = std::min(sms * S::CTAS_PER_SM, max_ctas(MT));
+  return launch(tree_kernel<DKP, DVP, MT, F16>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM,
+                stream, mk, mv, A);
+}
+
+template <int DKP, int DVP>
+static int launch_rows(int mt, int f16, const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A,
+                       int sms, void* stream) {
+  if (f16) {
+    if (mt == 1) return launch_tree<DKP, DVP, 1, true>(mk, mv, A, sms, stream);
+    if (mt == 2) return launch_tree<DKP, DVP, 2, true>(mk, mv, A, sms, stream);
+    return launch_tree<DKP, DVP, 4, true>(mk, mv, A, sms, stream);
+  }
+  if (mt == 1) return launch_tree<DKP, DVP, 1, false>(mk, mv, A, sms, stream);
+  if (mt == 2) return launch_tree<DKP, DVP, 2, false>(mk, mv, A, sms, stream);
+  return launch_tree<DKP, DVP, 4, false>(mk, mv, A, sms, stream);
+}
+
+constexpr size_t COUNTER_BYTES = MAX_CTAS * sizeof(int);
+
+// Counters, then two partial sums a CTA (the end of one unit and the start of
+// another): maximum and sum of a row, and up to 128 values of it.
+static size_t tree_workspace(int mt) {
+  return COUNTER_BYTES + (size_t)2 * max_ctas(mt) * 16 * mt * (2 + 128) * sizeof(float);
+}
+
+}  // namespace attn
+}  // namespace kb
+
+extern "C" size_t kb_tree_attention_workspace_size(int64_t group, int64_t max_tokens) {
+  if (group <= 0 || max_tokens <= 0) return 0;
+  return kb::attn::tree_workspace(kb::attn::row_tiles(group * max_tokens));
+}
+
+extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                                 const uint16_t* k_cache, const int64_t* k_strides,
+                                 const uint16_t* v_cache, const int64_t* v_strides, int dtype,
+                                 int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                                 int64_t table_stride, int64_t table_width,
+                                 const int32_t* context_lens, const int32_t* cu_tokens,
+                                 const int64_t* tree_mask, int64_t B, int64_t total,
+                                 int64_t max_tokens, int64_t Hq, int64_t Hkv, int64_t Dk,
+                                 int64_t Dv, float scale, uint16_t* out, float* lse,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  namespace at = kb::attn;
+  kb::clear_error();
+  KB_REQUIRE(B >= 0 && total >= 0 && max_tokens >= 0 && n_pages >= 0 && table_width >= 0,
+             KB_ERR_BAD_SHAPE, "tree attention: bad shape");
+  int st = at::check_heads(Hq, Hkv, Dk, Dv, dtype);
+  if (st != KB_OK) return st;
+  KB_REQUIRE(page_size >= 8 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
+             KB_ERR_UNSUPPORTED, "tree attention: the page size must be a power of two from 8");
+  if (B == 0 || total == 0) return KB_OK;
+  KB_REQUIRE(max_tokens > 0 && n_pages > 0, KB_ERR_BAD_SHAPE,
+             "tree attention: tokens but max_tokens 0, or a cache without pages");
+  KB_REQUIRE(q && k_strides && v_strides && cu_tokens && context_lens && out && k_cache &&
+                 v_cache && (table_width == 0 || block_table),
+             KB_ERR_NULL_POINTER, "tree attention: NULL pointer");
+  KB_REQUIRE(!tree_mask || max_tokens <= 64, KB_ERR_UNSUPPORTED,
+             "tree attention: a masked tree has at most 64 tokens");
+  constexpr int64_t kMax = (int64_t)1 << 30;
+  KB_REQUIRE(B <= kMax && total <= kMax && n_pages <= kMax && table_width <= kMax && Hq <= 65535,
+             KB_ERR_UNSUPPORTED, "tree attention: more than 2^30 tokens, pages or requests");
+  bool ok = (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) == 0 &&
+            ((q_token_stride | q_head_stride) & 7) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && ((k_strides[i] | v_strides[i]) & 7) == 0;
+  KB_REQUIRE(ok, KB_ERR_ALIGNMENT,
+             "tree attention: pointers must be 16-byte aligned and strides multiples of 8");
+  const size_t need = kb_tree_attention_workspace_size(Hq / Hkv, max_tokens);
+  KB_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0,
+             KB_ERR_WORKSPACE,
+             "tree attention: workspace of %zu bytes (256-byte aligned, zeroed once) required, "
+             "%zu given",
+             need, workspace_bytes);
+  const int dev = kb::bind_stream_device(stream);
+  at::TreeArgs A = {};
+  A.q = q;
+  A.q_tok = q_token_stride;
+  A.q_head = q_head_stride;
+  A.out = out;
+  A.lse = lse;
+  A.cu = cu_tokens;
+  A.table = block_table;
+  A.table_stride = table_stride;
+  A.context = context_lens;
+  A.mask = tree_mask;
+  A.n_pages = n_pages;
+  A.total = total;
+  A.B = (int)B;
+  A.width = (int)table_width;
+  A.ps = (int)page_size;
+  A.Hq = (int)Hq;
+  A.Hkv = (int)Hkv;
+  A.g = (int)(Hq / Hkv);
+  A.Dk = (int)Dk;
+  A.Dv = (int)Dv;
+  A.scale2 = scale * at::LOG2E;
+  const int mt = at::row_tiles(max_tokens * A.g);
+  A.counters = static_cast<int*>(workspace);
+  A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at::COUNTER_BYTES);
+  A.part_o = A.part_ml + (size_t)2 * at::max_ctas(mt) * 16 * mt * 2;
+  A.err = kb::device_error_word(dev);
+  KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
+  const int rows = (int)std::min<int64_t>(page_size, at::KT);
+  CUtensorMap mk, mv;
+  st = at::make_map_4d(&mk, k_cache, dtype, {Dk, page_size, Hkv, n_pages},
+                       {k_strides[1], k_strides[2], k_strides[0]}, rows, 1);
+  if (st != KB_OK) return st;
+  st = at::make_map_4d(&mv, v_cache, dtype, {Dv, page_size, Hkv, n_pages},
+                       {v_strides[1], v_strides[2], v_strides[0]}, rows, 1);
+  if (st != KB_OK) return st;
+  const int sms = kb::num_sms(dev);
+  if (Dk <= 64 && Dv <= 64) return at::launch_rows<64, 64>(mt, dtype, mk, mv, A, sms, stream);
+  if (Dk <= 128) return at::launch_rows<128, 128>(mt, dtype, mk, mv, A, sms, stream);
+  return at::launch_rows<192, 128>(mt, dtype, mk, mv, A, sms, stream);
+}

@@ -1203,6 +1203,8 @@ def tree_attention(
     cu = _vector(cu_tokens, torch.int32, "cu_tokens", device, requests + 1)
     if max_tokens < 0:
         raise ValueError("max_tokens must not be negative")
+    if total and (max_tokens == 0 or pages == 0):
+        raise ValueError("tokens need max_tokens of at least 1 and a cache with pages")
     mask = None
     if tree_mask is not None:
         if max_tokens > MAX_TREE_TOKENS:
@@ -1210,7 +1212,9 @@ def tree_attention(
         mask = _vector(tree_mask, torch.long, "tree_mask", device, total)
     out = torch.empty((total, hq, dv), dtype=q.dtype, device=device)
     lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
-    need = _lib.lib().kb_tree_attention_workspace_size(hkv, hq // hkv, max_tokens, dv)
+    if total == 0 or requests == 0:
+        return out if lse is None else (out, lse)
+    need = _lib.lib().kb_tree_attention_workspace_size(hq // hkv, max_tokens)
     ws = _workspace("tree_attention", device, need, (need,))
     _lib.call(
         "kb_tree_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), k_cache.data_ptr(), ks,
