@@ -453,8 +453,8 @@ KB_API int kb_paged_append(const uint16_t* k, int64_t k_token_stride, int64_t k_
  * i + (keys - queries).  out [total_q, Hq, Dv] contiguous; lse [total_q, Hq]
  * fp32 or NULL (natural logarithm).  A query without keys gives 0 and
  * -infinity.  Hq a multiple of Hkv; Dk <= 192, Dv <= 128, multiples of 8.
- * max_q: no request has more queries.  dtype 0 or 1, the outputs' type too;
- * products and sums in fp32. */
+ * max_q: no request has more queries (rows past it are not written).  scale > 0.
+ * dtype 0 or 1, the outputs' type too; products and sums in fp32. */
 KB_API int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                    const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
                    const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, int dtype,

@@ -81,6 +81,26 @@ __device__ __forceinline__ bool odd_element(uint16_t bits) {
   return (bits & m) == m;
 }
 
+// Whether any of eight elements is no number.  Adding one exponent step to the
+// exponent bits carries into the sign bit's place only where they are all ones.
+template <bool F16>
+__device__ __forceinline__ bool has_odd(const uint4& v) {
+  constexpr uint32_t M = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
+  const uint32_t t = ((v.x & M) + ONE) | ((v.y & M) + ONE) | ((v.z & M) + ONE) | ((v.w & M) + ONE);
+  return (t & 0x80008000u) != 0;
+}
+
+// Zeroes the elements of eight that are no numbers.
+template <bool F16>
+__device__ __forceinline__ void clear_odd(uint4& v) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (odd_element<F16>((uint16_t)w[i])) w[i] &= 0xffff0000u;
+    if (odd_element<F16>((uint16_t)(w[i] >> 16))) w[i] &= 0x0000ffffu;
+  }
+}
+
 // D[16x8] += A[16x16] * B[16x8], fp32 accumulate.
 template <bool F16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -117,6 +137,10 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z),
         "r"(w), "r"(smem_addr(bar)), "l"(policy)
       : "memory");
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 __device__ __forceinline__ void fence_proxy_async() {

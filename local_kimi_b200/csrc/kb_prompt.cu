@@ -1,97 +1,632 @@
-// kb_prompt.cu - causal attention over packed prompts.
+// kb_prompt.cu - causal attention over packed prompts on the 5th-generation
+// tensor cores.
 //
 //   o_i = sum_j exp(s_ij - m_i) v_j / l_i,  s_ij = scale * q_i . k_j over the visible j,
 //   m_i = max_j s_ij, l_i = sum_j exp(s_ij - m_i), lse_i = m_i + log(l_i)
 // visible: j <= i + (Lk - Lq).  A row that sees no key gives 0 and lse -infinity.
 //
-// One warp per (row, head); the lanes hold the head's dimensions, and keys are
-// visited one at a time with a running maximum and sum.
+// One persistent CTA per SM.  A unit is 256 rows of one request, two tiles A
+// and B of 128, against all the keys they see, 128 at a time.  The heads of a
+// group that share keys lie side by side in the rows (row = token * pack +
+// head, pack the largest power of two in the group), so short prompts fill
+// tiles and keys are read once for them.  Units go out heaviest (latest rows)
+// first, there and back over the CTAs.
+//
+//   warp 9: copies.  Q tiles, and a ring of 16 KB slots with the keys (128
+//     rows x 64 elements a slot) and values (64 or 128 rows) in use order, by
+//     tensor copies in the 128-byte swizzle; a barrier pair per key or value
+//     tile, not per slot.
+//   warp 8: one thread issues the MMAs.  S = Q K^T (both from shared memory)
+//     into tensor memory, O += P V with P from tensor memory (it replaces the
+//     S it came from) and V from shared memory, rows of V as they lie
+//     (MN-major).  Order A, B, A, B: while the softmax of one tile runs, the
+//     tensor core works for the other.  P V of a tile is issued before the
+//     next S of the same tile, so S never overwrites a P still being read.
+//   warps 0-3 and 4-7: softmax of tiles A and B, a row per thread: maximum,
+//     exponentials in base 2, row sum in fp32, and P rounded once to the
+//     inputs' type.  The running maximum only moves, and O is only rescaled,
+//     when a row's maximum rose by more than 2^8: weights stay within fp32
+//     and the 16-bit types, and the final division makes up for the rest.
+//
+// 512 columns of tensor memory: S A, S B, O A, O B.  The math is bound by the
+// MMAs (2 (Dk + Dv) flops a pair) and, at Dk = 128, as much by the
+// exponentials: 16 a clock and SM, 1024 clocks a tile of 128 x 128.
+//
+// In the last tiles of a unit some rows do not see some keys, or the tile
+// reaches past the request's end into its neighbour.  A value there that is
+// infinite or not a number must not meet a zero weight: warps 10 and 11 zero
+// such elements in those tiles before the MMA reads them, and at the end the
+// rows that do see them take them from memory.
+#include <algorithm>
+
 #include "kb_attn.cuh"
+#include "kb_tcgen05.cuh"
 
 namespace kb {
 namespace attn {
 
-constexpr int THREADS = 256;
-constexpr int MAX_DIM = 256;
-constexpr int PER = MAX_DIM / 32;
+constexpr int TILE = 128;                  // rows of a tile, keys of a step
+constexpr int SLOT = 16384;                // bytes of a ring slot
+constexpr int PROMPT_THREADS = 384;
+constexpr int MMA_WARP = 8, COPY_WARP = 9, CLEAN_WARP = 10;   // and 11
+constexpr int ENTRIES = 8;                 // key and value tiles with a barrier pair
+constexpr float RESCALE = 8.0f;            // log2 of the growth that moves the maximum
 
-struct Args {
+struct PromptArgs {
   const uint16_t *q, *k, *v;
-  int64_t q_tok, q_head, k_row, k_head, v_row, v_head;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
   uint16_t* out;            // [total, Hq, Dv] contiguous
   float* lse;               // [total, Hq] or NULL
   const int *cu_q, *cu_k;
   int64_t total_q, total_k;
-  int B, Hq, Hkv, Dk, Dv, f16;
-  float scale;
+  int B, Hq, g, Dk, Dv;
+  int pack_shift;           // log2 of the heads that share a tile's rows
+  int blocks;               // 256-row units of the longest request
+  float scale2;             // scale * log2(e)
+  uint32_t* err;
 };
 
-__device__ __forceinline__ float value(uint16_t bits, int f16) {
-  return f16 ? __half2float(__ushort_as_half(bits)) : bf16_bits_to_float(bits);
-}
+template <int DKP, int DVP>
+struct PromptShape {
+  static constexpr int KC = DKP / 64;                    // slots of a key tile
+  static constexpr int VC = DVP / 64;                    // ... of a value tile
+  static constexpr int VKEYS = TILE / VC;                // keys of a value slot
+  static constexpr int Q_BYTES = 2 * KC * SLOT;
+  static constexpr int FIXED = 1024 + 1024;              // alignment, barriers
+  static constexpr int FIT = (227 * 1024 - FIXED - Q_BYTES) / SLOT;
+  static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
+  static constexpr int SMEM = FIXED + Q_BYTES + SLOTS * SLOT;
+  static_assert(SLOTS >= KC + 2 * VC, "a key tile beside the value tile in use, and one to come");
+};
 
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Args A) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-  if (item >= A.total_q * A.Hq) return;
-  const int64_t row = item / A.Hq;
-  const int h = (int)(item - row * A.Hq), hk = h / (A.Hq / A.Hkv);
-  int lo = 0, hi = A.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (A.cu_q[mid] <= row) lo = mid; else hi = mid - 1;
+struct PromptBars {
+  uint64_t full[ENTRIES], empty[ENTRIES];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t clean[ENTRIES];  // a value tile is there, without odd elements
+  uint64_t drain;
+  int odd[16];              // units (counted by the CTA) that had some, by their last four bits
+  uint32_t tmem;
+  int abort_flag;
+};
+static_assert(sizeof(PromptBars) <= 1024, "barrier block");
+
+// A unit of the walk, the same for every role.
+struct Unit {
+  int64_t q0, k0;           // first query and key of the request
+  int n, m;                 // its queries and keys
+  int head0;                // first head
+  int t0;                   // first token of tile A
+  int tiles[2];             // key tiles that tiles A and B see
+  int whole;                // of them, those that every row of A and B sees whole
+};
+
+// Units u = blockIdx.x, ... in rounds of gridDim.x, every other round backwards.
+struct Walk {
+  const PromptArgs& A;
+  int round, total;
+  int count;                // units walked
+  __device__ __forceinline__ explicit Walk(const PromptArgs& a) : A(a), round(0), count(-1) {
+    total = A.blocks * A.B * (A.Hq >> A.pack_shift);
   }
-  const int b = lo;
-  const int64_t first = A.cu_q[b], end = min((int64_t)A.cu_q[b + 1], A.total_q);
-  float acc[PER] = {};
-  float m = -INFINITY, l = 0.f;
-  if (row >= first && row < end) {
-    const int i = (int)(row - first), n = (int)(end - first);
-    const int64_t base = min(max((int64_t)A.cu_k[b], (int64_t)0), A.total_k);
-    const int64_t lk = min(max((int64_t)A.cu_k[b + 1], base), A.total_k) - base;
-    const int64_t keys = i + 1 + lk - n;
-    float qv[PER];
-    const uint16_t* q = A.q + row * A.q_tok + h * A.q_head;
+  // The next unit with rows; false at the end.
+  __device__ __forceinline__ bool next(Unit& U) {
+    const int groups = A.Hq >> A.pack_shift;
+    while (true) {
+      const int at = round * gridDim.x;
+      if (at >= total) return false;
+      const int u = at + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      ++round;
+      if (u >= total) continue;
+      const int block = A.blocks - 1 - u / (A.B * groups);
+      const int rest = u % (A.B * groups);
+      const int b = rest / groups;
+      int64_t end;
+      request_rows(A.cu_q, b, A.total_q, U.q0, end);
+      U.n = (int)(end - U.q0);
+      U.t0 = (block * 2 * TILE) >> A.pack_shift;
+      if (U.t0 >= U.n) continue;
+      request_rows(A.cu_k, b, A.total_k, U.k0, end);
+      U.m = (int)(end - U.k0);
+      U.head0 = (rest - b * groups) << A.pack_shift;
+      const int span = TILE >> A.pack_shift;
 #pragma unroll
-    for (int c = 0; c < PER; ++c)
-      qv[c] = lane + 32 * c < A.Dk ? value(q[lane + 32 * c], A.f16) * A.scale : 0.f;
-    for (int64_t j = 0; j < keys; ++j) {
-      const uint16_t* k = A.k + (base + j) * A.k_row + hk * A.k_head;
-      const uint16_t* v = A.v + (base + j) * A.v_row + hk * A.v_head;
-      float s = 0.f;
-#pragma unroll
-      for (int c = 0; c < PER; ++c)
-        if (lane + 32 * c < A.Dk) s += qv[c] * value(k[lane + 32 * c], A.f16);
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (s == -INFINITY) continue;
-      const float top = fmaxf(m, s);
-      const float fix = expf(m - top), w = expf(s - top);
-      m = top;
-      l = l * fix + w;
-#pragma unroll
-      for (int c = 0; c < PER; ++c)
-        if (lane + 32 * c < A.Dv) acc[c] = acc[c] * fix + w * value(v[lane + 32 * c], A.f16);
+      for (int i = 0; i < 2; ++i) {
+        const int first = U.t0 + i * span, last = min(U.n, first + span) - 1;
+        const int keys = first < U.n ? min(max(last + U.m - U.n + 1, 0), U.m) : 0;
+        U.tiles[i] = (keys + TILE - 1) / TILE;
+      }
+      ++count;
+      U.whole = max(U.t0 + U.m - U.n + 1, 0) / TILE;
+      return true;
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int c = 0; c < PER; ++c) {
-    const int d = lane + 32 * c;
-    if (d >= A.Dv) continue;
-    const float o = l == 0.f ? 0.f : acc[c] * inv;
-    A.out[item * A.Dv + d] = A.f16 ? __half_as_ushort(__float2half_rn(o)) : float_to_bf16_bits(o);
-  }
-  if (A.lse && lane == 0) A.lse[item] = l == 0.f ? -INFINITY : m + logf(l);
+};
+
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
 }
 
-static int launch_rows(Args& A, void* stream) {
-  const int64_t items = A.total_q * A.Hq;
-  const int64_t grid = (items + THREADS / 32 - 1) / (THREADS / 32);
-  KB_REQUIRE(grid < ((int64_t)1 << 31), KB_ERR_UNSUPPORTED, "attention: too many rows");
-  return launch(rows_kernel, dim3((unsigned)grid), dim3(THREADS), 0, stream, A);
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
 }
+
+// Adds to a row's outputs d0..d0+31 the values that are no numbers of the keys
+// [first, last]: they were kept out of the tile products.
+template <bool F16>
+__device__ __noinline__ void add_odd(const PromptArgs& A, const uint16_t* v, int first, int last,
+                                     int d0, float (&o)[32]) {
+  for (int64_t j = first; j <= last; ++j)
+    for (int i = 0; i < 32 && d0 + i < A.Dv; ++i) {
+      const uint16_t u = v[j * A.v_tok + d0 + i];
+      if (odd_element<F16>(u)) o[i] += element<F16>(u);
+    }
+}
+
+template <int DKP, int DVP, bool F16>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                  const __grid_constant__ CUtensorMap tv, const PromptArgs A) {
+  using S = PromptShape<DKP, DVP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      smem_raw + ((1024u - (static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw)) & 1023u)) &
+                  1023u);
+  uint8_t* qs = smem;                           // [2][KC] slots
+  uint8_t* ring = qs + S::Q_BYTES;              // [SLOTS]
+  PromptBars* B = reinterpret_cast<PromptBars*>(ring + S::SLOTS * SLOT);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_f = &B->abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ENTRIES; ++i) {
+      mbar_init(&B->full[i], 1);
+      mbar_init(&B->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->q_full[i], 1);
+      mbar_init(&B->q_empty[i], 1);
+      mbar_init(&B->s_full[i], 1);
+      mbar_init(&B->p_full[i], 4);
+      mbar_init(&B->o_full[i], 1);
+    }
+    for (int i = 0; i < ENTRIES; ++i) mbar_init(&B->clean[i], 2);
+    for (int i = 0; i < 16; ++i) B->odd[i] = -1;
+    mbar_init(&B->drain, 1);
+    B->abort_flag = 0;
+    mbar_fence_init();
+    prefetch_map(&tq);
+    prefetch_map(&tk);
+    prefetch_map(&tv);
+  }
+  if (warp == CLEAN_WARP) tc::tmem_alloc_all(&B->tmem);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = B->tmem;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // Rows outside every request: zero.
+  {
+    const int64_t lead = min(max((int64_t)A.cu_q[0], (int64_t)0), A.total_q);
+    const int64_t tail = min(max((int64_t)A.cu_q[A.B], lead), A.total_q);
+    const int64_t spare = (lead + A.total_q - tail) * A.Hq;
+    for (int64_t i = (int64_t)blockIdx.x * PROMPT_THREADS + threadIdx.x; i < spare;
+         i += (int64_t)gridDim.x * PROMPT_THREADS) {
+      const int64_t r = i < lead * A.Hq ? i : i - lead * A.Hq + tail * A.Hq;
+      for (int d = 0; d < A.Dv; d += 8)
+        *reinterpret_cast<uint4*>(A.out + r * A.Dv + d) = make_uint4(0, 0, 0, 0);
+      if (A.lse) A.lse[r] = -INFINITY;
+    }
+  }
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int tile = warp >> 2;
+    const int row = threadIdx.x & (TILE - 1);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + tile * TILE;
+    const uint32_t o_at = tmem + lanes + 256 + tile * TILE;
+    const float scale2 = A.scale2;
+    const int span = TILE >> A.pack_shift;
+    uint32_t s_phase = 0, o_phase = 0;
+    Unit U;
+    for (Walk walk(A); walk.next(U);) {
+      const int first = U.t0 + tile * span;
+      if (first >= U.n) continue;
+      const int tok = first + (row >> A.pack_shift);
+      const int head = U.head0 + (row & ((1 << A.pack_shift) - 1));
+      const bool real = tok < U.n;
+      const int limit = min(tok, U.n - 1) + U.m - U.n;      // last key the row sees
+      const int clear = first + U.m - U.n;                  // ... and the tile's first row
+      float top = -INFINITY, sum = 0.f;                     // in log2 units
+      bool ok = true;
+      for (int j = 0; j < U.tiles[tile]; ++j) {
+        if (!wait_phase(&B->s_full[tile], s_phase, abort_f, A.err)) {
+          ok = false;
+          break;
+        }
+        s_phase ^= 1u;
+        tc::tc_fence_after();
+        float s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_at + c * 32, s[c]);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::hold_regs(s[c]);
+        if (j * TILE + TILE - 1 > clear) {
+          const int last = limit - j * TILE;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i > last) s[c][i] = -INFINITY;
+        }
+        float mx[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
+#pragma unroll
+        for (int i = 1; i < 32; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[c][i]);
+        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+        // S being there means that every MMA issued before it is done, the
+        // last P V of this tile among them: O may be touched.
+        const bool grow = mine > top + RESCALE || top == -INFINITY;
+        if (__any_sync(0xffffffffu, grow && j > 0)) {
+          const float now = grow ? fmaxf(mine, top) : top;
+          const float fix = now == top ? 1.f : exp2_fast(top - now);
+          sum *= fix;
+          top = now;
+#pragma unroll
+          for (int c = 0; c < DVP / 32; ++c) {
+            float o[32];
+            tc::tmem_ld32(o_at + c * 32, o);
+            tc::tmem_ld_wait();
+            tc::hold_regs(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= fix;
+            tc::tmem_st32(o_at + c * 32, o);
+          }
+          tc::tmem_st_wait();
+        } else if (j == 0) {
+          top = mine;
+        }
+        const float at = top == -INFINITY ? 0.f : top;
+        const float2 mul = make_float2(scale2, scale2), off = make_float2(-at, -at);
+        float2 part[4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t p[32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2 x = make_float2(s[h * 2 + c][2 * i], s[h * 2 + c][2 * i + 1]);
+              x = ffma2(x, mul, off);
+              x.x = exp2_fast(x.x);
+              x.y = exp2_fast(x.y);
+              part[i & 3] = fadd2(part[i & 3], x);
+              p[c * 16 + i] = pack2<F16>(x.x, x.y);
+            }
+          tc::tmem_st32(s_at + h * 32, p);
+        }
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->p_full[tile]);
+        part[0] = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
+        sum += part[0].x + part[0].y;
+      }
+      if (!ok) break;
+      const int64_t at = (U.q0 + tok) * A.Hq + head;
+      uint16_t* out = A.out + at * A.Dv;
+      if (U.tiles[tile] == 0) {
+        if (real) {
+          for (int d = 0; d < A.Dv; d += 8)
+            *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
+          if (A.lse) A.lse[at] = -INFINITY;
+        }
+        continue;
+      }
+      if (!wait_phase(&B->o_full[tile], o_phase, abort_f, A.err)) break;
+      o_phase ^= 1u;
+      tc::tc_fence_after();
+      // A row that saw no key (or only keys of score -infinity) is zero.
+      const bool none = sum == 0.f || limit < 0;
+      const float inv = none ? 0.f : 1.f / sum;
+      const bool odd = *const_cast<volatile int*>(&B->odd[walk.count & 15]) == walk.count;
+#pragma unroll
+      for (int c = 0; c < DVP / 32; ++c) {
+        float o[32];
+        tc::tmem_ld32(o_at + c * 32, o);
+        tc::tmem_ld_wait();
+        tc::hold_regs(o);
+        if (odd)
+          add_odd<F16>(A, A.v + U.k0 * A.v_tok + head / A.g * A.v_head, U.whole * TILE, limit,
+                       c * 32, o);
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          uint4 w;
+          w.x = pack2<F16>(o[i] * inv, o[i + 1] * inv);
+          w.y = pack2<F16>(o[i + 2] * inv, o[i + 3] * inv);
+          w.z = pack2<F16>(o[i + 4] * inv, o[i + 5] * inv);
+          w.w = pack2<F16>(o[i + 6] * inv, o[i + 7] * inv);
+          if (none) w = make_uint4(0, 0, 0, 0);
+          if (real && c * 32 + i < A.Dv) *reinterpret_cast<uint4*>(out + c * 32 + i) = w;
+        }
+      }
+      tc::tc_fence_before();
+      if (real && A.lse) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == MMA_WARP && lane == 0) {
+      // --------------------------------------------------------------- MMA issue
+      constexpr uint32_t TYPE = F16 ? 0u : 1u;
+      constexpr uint32_t COMMON = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((TILE >> 4) << 24);
+      constexpr uint32_t ID_S = COMMON | ((TILE >> 3) << 17);
+      constexpr uint32_t ID_O = COMMON | (1u << 16) | ((DVP >> 3) << 17);    // V: MN-major
+      const uint32_t q_at = smem_addr(qs), r_at = smem_addr(ring);
+      int entry = 0, slot = 0;            // next tile of the ring and its first slot
+      uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      bool ok = true;
+      auto need = [&](uint64_t* bar, uint32_t ph) {
+        ok = ok && wait_phase(bar, ph, abort_f, A.err);
+        return ok;
+      };
+      auto score = [&](int i, int at) {
+        uint32_t acc = 0;
+#pragma unroll
+        for (int c = 0; c < S::KC; ++c) {
+          int sl = at + c;
+          if (sl >= S::SLOTS) sl -= S::SLOTS;
+          const uint64_t a = tc::sw128_desc(q_at + (i * S::KC + c) * SLOT);
+          const uint64_t b = tc::sw128_desc(r_at + sl * SLOT);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            tc::umma(tmem + i * TILE, a + k * 2, b + k * 2, ID_S, acc);
+            acc = 1;
+          }
+        }
+      };
+      auto product = [&](int i, int at, bool first) {
+        uint32_t acc = first ? 0 : 1;
+#pragma unroll
+        for (int c = 0; c < S::VC; ++c) {
+          int sl = at + c;
+          if (sl >= S::SLOTS) sl -= S::SLOTS;
+          const uint64_t b = tc::sw128_desc_mn(r_at + sl * SLOT, S::VKEYS * 128);
+#pragma unroll
+          for (int k = 0; k < S::VKEYS / 16; ++k) {
+            tc::umma_ts(tmem + 256 + i * TILE, tmem + i * TILE + (c * (S::VKEYS / 16) + k) * 8,
+                        b + k * (2048 >> 4), ID_O, acc);
+            acc = 1;
+          }
+        }
+      };
+      auto step = [&](int slots) {          // past the ring's current tile
+        slot += slots;
+        if (slot >= S::SLOTS) slot -= S::SLOTS;
+        if (++entry == ENTRIES) {
+          entry = 0;
+          phase ^= 1u;
+        }
+      };
+      Unit U;
+      for (Walk walk(A); ok && walk.next(U);) {
+        const int steps = max(U.tiles[0], U.tiles[1]);
+        if (steps == 0) continue;
+        if (!need(&B->full[entry], phase)) break;
+        for (int i = 0; i < 2; ++i) {
+          if (U.tiles[i] == 0) continue;
+          if (!need(&B->q_full[i], q_phase[i])) break;
+          q_phase[i] ^= 1u;
+          tc::tc_fence_after();
+          score(i, slot);
+          tc::umma_commit(&B->s_full[i]);
+          if (U.tiles[i] == 1) tc::umma_commit(&B->q_empty[i]);
+        }
+        if (!ok) break;
+        tc::umma_commit(&B->empty[entry]);
+        step(S::KC);
+        for (int j = 0; j < steps; ++j) {
+          // This step's values, and the next step's keys behind them.
+          const int v_entry = entry, v_slot = slot;
+          if (!need(&B->clean[v_entry], phase)) break;
+          step(S::VC);
+          bool keys = false;
+          for (int i = 0; i < 2; ++i) {
+            if (j >= U.tiles[i]) continue;
+            if (!need(&B->p_full[i], p_phase[i])) break;
+            p_phase[i] ^= 1u;
+            tc::tc_fence_after();
+            product(i, v_slot, j == 0);
+            if (j + 1 == U.tiles[i]) {
+              tc::umma_commit(&B->o_full[i]);
+              continue;
+            }
+            if (!keys && !need(&B->full[entry], phase)) break;
+            keys = true;
+            score(i, slot);
+            tc::umma_commit(&B->s_full[i]);
+            if (j + 2 == U.tiles[i]) tc::umma_commit(&B->q_empty[i]);
+          }
+          if (!ok) break;
+          tc::umma_commit(&B->empty[v_entry]);
+          if (j + 1 < steps) {
+            tc::umma_commit(&B->empty[entry]);
+            step(S::KC);
+          }
+        }
+      }
+      // Every product issued is done before the tensor memory goes.
+      tc::umma_commit(&B->drain);
+      drain_phase(&B->drain, 0);
+    } else if (warp == COPY_WARP && lane == 0) {
+      // ------------------------------------------------------------------ copies
+      const uint64_t keep = l2_evict_last_policy(), once = l2_evict_first_policy();
+      int entry = 0, slot = 0;             // next tile of the ring and its first slot
+      int oldest = 0, held = 0, used = 0;  // oldest tile not known to be free; tiles, slots held
+      uint32_t old_phase = 0, q_phase[2] = {1, 1};
+      bool ok = true;
+      // Starts the next tile of the ring, once it has a barrier pair and slots.
+      auto begin = [&](int slots) {
+        while (held == ENTRIES || used + slots > S::SLOTS) {
+          ok = ok && wait_phase(&B->empty[oldest], old_phase, abort_f, A.err);
+          if (!ok) return false;
+          used -= (oldest & 1) ? S::VC : S::KC;      // keys and values alternate
+          --held;
+          if (++oldest == ENTRIES) {
+            oldest = 0;
+            old_phase ^= 1u;
+          }
+        }
+        used += slots;
+        ++held;
+        mbar_arrive_expect_tx(&B->full[entry], (uint32_t)(slots * SLOT));
+        return true;
+      };
+      auto place = [&]() {                 // the next slot
+        uint8_t* at = ring + slot * SLOT;
+        if (++slot == S::SLOTS) slot = 0;
+        return at;
+      };
+      auto end = [&]() {
+        if (++entry == ENTRIES) entry = 0;
+      };
+      Unit U;
+      for (Walk walk(A); ok && walk.next(U);) {
+        const int steps = max(U.tiles[0], U.tiles[1]);
+        const int hk = U.head0 / A.g, span = TILE >> A.pack_shift;
+        auto queries = [&](int i) {
+          if (U.tiles[i] == 0) return;
+          ok = ok && wait_phase(&B->q_empty[i], q_phase[i], abort_f, A.err);
+          if (!ok) return;
+          q_phase[i] ^= 1u;
+          mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)(S::KC * SLOT));
+          for (int c = 0; c < S::KC; ++c)
+            tma_load_4d(qs + (i * S::KC + c) * SLOT, &tq, c * 64, U.head0,
+                        (int)U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
+        };
+        for (int j = 0; j < steps && ok; ++j) {
+          if (j == 0) queries(0);
+          if (!ok || !begin(S::KC)) break;
+          const int key0 = (int)U.k0 + j * TILE;
+          for (int c = 0; c < S::KC; ++c)
+            tma_load_4d(place(), &tk, c * 64, hk, key0, 0, &B->full[entry], keep);
+          end();
+          if (j == 0) queries(1);
+          if (!ok || !begin(S::VC)) break;
+          for (int c = 0; c < S::VC; ++c) {
+            uint8_t* at = place();
+            for (int d = 0; d < DVP / 64; ++d)
+              tma_load_4d(at + d * S::VKEYS * 128, &tv, d * 64, hk, key0 + c * S::VKEYS, 0,
+                          &B->full[entry], keep);
+          }
+          end();
+        }
+      }
+      // On the error path, copies in flight land before the CTA may exit.
+      if (*abort_f) {
+        for (int i = 0; i < ENTRIES; ++i) {
+          drain_phase(&B->full[i], 0);
+          drain_phase(&B->full[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+          drain_phase(&B->q_full[i], 0);
+          drain_phase(&B->q_full[i], 1);
+        }
+      }
+    }
+    if (warp >= CLEAN_WARP) {
+      // ------------------------------------------------------------ odd elements
+      int entry = 0, slot = 0;
+      uint32_t phase = 0;
+      auto step = [&](int slots) {
+        slot += slots;
+        if (slot >= S::SLOTS) slot -= S::SLOTS;
+        if (++entry == ENTRIES) {
+          entry = 0;
+          phase ^= 1u;
+        }
+      };
+      bool ok = true;
+      Unit U;
+      for (Walk walk(A); ok && walk.next(U);) {
+        const int steps = max(U.tiles[0], U.tiles[1]);
+        for (int j = 0; j < steps; ++j) {
+          step(S::KC);
+          // Every tile is waited for, so that these warps stay within one
+          // round of the ring of the others.
+          ok = wait_phase(&B->full[entry], phase, abort_f, A.err);
+          if (!ok) break;
+          if (j >= U.whole) {
+            bool any = false;
+            for (int c = 0; c < S::VC; ++c) {
+              int sl = slot + c;
+              if (sl >= S::SLOTS) sl -= S::SLOTS;
+              uint4* at = reinterpret_cast<uint4*>(ring + sl * SLOT) + (warp - CLEAN_WARP) * 32 +
+                          lane;
+#pragma unroll 8
+              for (int i = 0; i < SLOT / 1024; ++i) {
+                uint4 x = at[i * 64];
+                if (has_odd<F16>(x)) {
+                  clear_odd<F16>(x);
+                  at[i * 64] = x;
+                  any = true;
+                }
+              }
+            }
+            if (any) {
+              B->odd[walk.count & 15] = walk.count;
+              fence_proxy_async();
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->clean[entry]);
+          step(S::VC);
+        }
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == CLEAN_WARP) {
+    tc::tc_fence_after();
+    tc::tmem_free_all(tmem);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host.
+// ---------------------------------------------------------------------------
+
+template <int DKP, int DVP, bool F16>
+static int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                         const PromptArgs& A, int grid, void* stream) {
+  using S = PromptShape<DKP, DVP>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  const void* fn = reinterpret_cast<const void*>(&prompt_kernel<DKP, DVP, F16>);
+  const int st = allow_smem(fn, S::SMEM, done, mu);
+  if (st != KB_OK) return st;
+  return launch(prompt_kernel<DKP, DVP, F16>, dim3(grid), dim3(PROMPT_THREADS), (size_t)S::SMEM,
+                stream, mq, mk, mv, A);
+}
+
+// Values up to 64 wide beside keys up to 64, else both padded to 128 (192).
+static int value_keys(int64_t Dk, int64_t Dv) { return Dk <= 64 && Dv <= 64 ? 128 : 64; }
 
 }  // namespace attn
 }  // namespace kb
@@ -105,25 +640,36 @@ extern "C" int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride,
                                    int64_t total_k, int64_t max_q, int64_t Hq, int64_t Hkv,
                                    int64_t Dk, int64_t Dv, float scale, uint16_t* out, float* lse,
                                    void* stream) {
+  namespace at = kb::attn;
   kb::clear_error();
   KB_REQUIRE(B >= 0 && total_q >= 0 && total_k >= 0 && max_q >= 0, KB_ERR_BAD_SHAPE,
              "prompt attention: bad shape");
-  const int st = kb::attn::check_heads(Hq, Hkv, Dk, Dv, dtype);
+  int st = at::check_heads(Hq, Hkv, Dk, Dv, dtype);
   if (st != KB_OK) return st;
   if (B == 0 || total_q == 0) return KB_OK;
+  KB_REQUIRE(scale > 0.f, KB_ERR_BAD_SHAPE, "attention: the scale must be positive");
+  KB_REQUIRE(max_q > 0, KB_ERR_BAD_SHAPE, "prompt attention: tokens but max_q 0");
   KB_REQUIRE(q && cu_q && cu_k && out && (total_k == 0 || (k && v)), KB_ERR_NULL_POINTER,
              "prompt attention: NULL pointer");
-  KB_REQUIRE(B < ((int64_t)1 << 30) && total_q < ((int64_t)1 << 31) && total_k < ((int64_t)1 << 31),
-             KB_ERR_UNSUPPORTED, "prompt attention: too many tokens");
-  kb::attn::Args A = {};
+  constexpr int64_t kMax = (int64_t)1 << 30;
+  KB_REQUIRE(B <= 65535 && total_q <= kMax && total_k <= kMax && Hq <= 65535, KB_ERR_UNSUPPORTED,
+             "prompt attention: more than 2^30 tokens or 65535 requests or heads");
+  const bool ok =
+      (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 &&
+      ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride |
+        v_head_stride) & 7) == 0;
+  KB_REQUIRE(ok, KB_ERR_ALIGNMENT,
+             "prompt attention: pointers must be 16-byte aligned and strides multiples of 8");
+  const int dev = kb::bind_stream_device(stream);
+  at::PromptArgs A = {};
   A.q = q;
   A.k = k;
   A.v = v;
   A.q_tok = q_token_stride;
   A.q_head = q_head_stride;
-  A.k_row = k_token_stride;
+  A.k_tok = k_token_stride;
   A.k_head = k_head_stride;
-  A.v_row = v_token_stride;
+  A.v_tok = v_token_stride;
   A.v_head = v_head_stride;
   A.out = out;
   A.lse = lse;
@@ -133,10 +679,38 @@ extern "C" int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride,
   A.total_k = total_k;
   A.B = (int)B;
   A.Hq = (int)Hq;
-  A.Hkv = (int)Hkv;
+  A.g = (int)(Hq / Hkv);
   A.Dk = (int)Dk;
   A.Dv = (int)Dv;
-  A.f16 = dtype;
-  A.scale = scale;
-  return kb::attn::launch_rows(A, stream);
+  while (A.pack_shift < 7 && A.g % (2 << A.pack_shift) == 0) ++A.pack_shift;
+  A.scale2 = scale * at::LOG2E;
+  A.err = kb::device_error_word(dev);
+  KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
+  const int pack = 1 << A.pack_shift;
+  const int64_t longest = std::min(max_q, total_q);
+  const int64_t blocks = (longest * pack + 2 * at::TILE - 1) / (2 * at::TILE);
+  const int64_t units = blocks * B * (Hq / pack);
+  KB_REQUIRE(units <= kMax, KB_ERR_UNSUPPORTED, "prompt attention: too many units of rows");
+  A.blocks = (int)blocks;
+  CUtensorMap mq, mk, mv;
+  st = at::make_map_4d(&mq, q, dtype, {Dk, Hq, total_q, 1}, {q_head_stride, q_token_stride, 8},
+                       pack, at::TILE / pack);
+  if (st != KB_OK) return st;
+  // Without keys no tile is ever copied: any valid map will do.
+  const int64_t keys = std::max<int64_t>(total_k, 1);
+  st = at::make_map_4d(&mk, total_k ? k : q, dtype, {Dk, Hkv, keys, 1},
+                       {k_head_stride, k_token_stride, 8}, 1, at::TILE);
+  if (st != KB_OK) return st;
+  st = at::make_map_4d(&mv, total_k ? v : q, dtype, {Dv, Hkv, keys, 1},
+                       {v_head_stride, v_token_stride, 8}, 1, at::value_keys(Dk, Dv));
+  if (st != KB_OK) return st;
+  const int grid = (int)std::min<int64_t>(kb::num_sms(dev), units);
+  if (Dk <= 64 && Dv <= 64)
+    return dtype ? at::launch_prompt<64, 64, true>(mq, mk, mv, A, grid, stream)
+                 : at::launch_prompt<64, 64, false>(mq, mk, mv, A, grid, stream);
+  if (Dk <= 128)
+    return dtype ? at::launch_prompt<128, 128, true>(mq, mk, mv, A, grid, stream)
+                 : at::launch_prompt<128, 128, false>(mq, mk, mv, A, grid, stream);
+  return dtype ? at::launch_prompt<192, 128, true>(mq, mk, mv, A, grid, stream)
+               : at::launch_prompt<192, 128, false>(mq, mk, mv, A, grid, stream);
 }

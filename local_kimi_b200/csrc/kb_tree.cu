@@ -29,8 +29,8 @@
 // Rows of a page past the request's end were never written and may hold
 // anything: they are masked as keys and zeroed as values.  A value that is
 // infinite or not a number in a hidden drafted token must not meet a zero
-// weight: such elements are taken out of the tile and added to the rows that
-// see them.
+// weight: such elements are zeroed in the tile, and at the end the rows that
+// see them take them from the cache.
 #include <algorithm>
 
 #include "kb_attn.cuh"
@@ -42,12 +42,15 @@ constexpr int KT = 64;                     // keys of a tile
 constexpr int CHUNK = KT * 128;            // bytes of 64 keys x 64 elements
 constexpr int MAX_CTAS = 320;              // counters in the workspace
 constexpr int MIN_TILES = 2;               // tiles that make another CTA worth its partial sums
+constexpr int UNIT_COST = 1;               // a unit's start and end, in tiles
 
 struct TreeArgs {
   const uint16_t* q;
   int64_t q_tok, q_head;
   uint16_t* out;            // [total, Hq, Dv] contiguous
   float* lse;               // [total, Hq] or NULL
+  const uint16_t* v;        // the value cache, for values that are no numbers
+  int64_t v_page, v_row, v_head;
   const int* cu;
   const int* table;
   int64_t table_stride;
@@ -66,10 +69,12 @@ struct TreeArgs {
 struct Segment {
   int64_t first;            // first row (token) of the request
   int64_t ctx;              // cached tokens before this step's
-  int n;                    // this step's tokens
+  int64_t t0, t1;           // tiles of the unit
+  int b, n;                 // request; this step's tokens
   int hk, row0, rows;       // head, first row of the block (token * g + head), rows in it
   int whole;                // the run holds all of the unit's tiles
   int starts;               // ... its first tile
+  int end;                  // no segment: the run is over
   int c0, parts;            // the CTAs that share the unit: first, number
 };
 
@@ -94,24 +99,46 @@ struct TreeShape {
   static_assert(STAGES >= 2, "two tiles in flight at least");
 };
 
+// A request: its rows, context, tiles of KT keys and blocks of rows.
+struct Request {
+  int64_t first, ctx, tiles;
+  int n, blocks;
+};
+
+// The request a run starts in, and where its tiles start on the line.
+struct Start {
+  Request r;
+  int64_t base;
+  int b;
+};
+
 template <int STAGES>
 struct TreeBars {
   uint64_t full[STAGES], empty[STAGES];
   uint64_t q_full[2], q_empty[2];
-  uint64_t all, share[4];     // consumer warps together; those with the same keys
+  uint64_t all;               // consumer warps together
   uint64_t valid[STAGES];     // which keys of the tile exist
   int64_t key0[STAGES];       // first key of the tile
   int last[STAGES];           // last tile of its segment
   Segment seg[2];
   int64_t scan[16];
-  int64_t total, base;
-  int b, abort_flag, joined;
+  int odd[2];                 // a value of the segment's step is no number
+  Start start;
+  int abort_flag, joined;
 };
 
-// Keys [lo, hi) of the line of tiles that CTA c of n takes.
-__device__ __forceinline__ int64_t run_start(int64_t tiles, int n, int c) { return tiles * c / n; }
+// Quotient of non-negative numbers; the 64-bit division takes most of a
+// microsecond of the producer's start.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// Where run c of n starts on a line of tiles, and the run that holds place x.
+__device__ __forceinline__ int64_t run_start(int64_t tiles, int n, int c) {
+  return quotient(tiles * c, n);
+}
 __device__ __forceinline__ int run_of(int64_t tiles, int n, int64_t x) {
-  return (int)(((x + 1) * n - 1) / tiles);
+  return (int)quotient((x + 1) * n - 1, tiles);
 }
 
 template <int DKP, int DVP, int MT, bool F16>
@@ -143,36 +170,46 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       mbar_init(&B->q_empty[i], S::NW);
     }
     mbar_init(&B->all, S::NW);
-    for (int i = 0; i < S::WK; ++i) mbar_init(&B->share[i], MT);
     B->abort_flag = 0;
-    B->b = 0;
-    B->base = 0;
+    B->odd[0] = B->odd[1] = 0;
     mbar_fence_init();
+    prefetch_map(&tk);
+    prefetch_map(&tv);
   }
   // Columns of q past the head's width stay zero (the copies do not write them).
-  for (int i = tid; i < 2 * S::Q_BYTES / 16; i += S::THREADS)
-    reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
-  fence_proxy_async();
+  if (A.Dk < DKP) {
+    for (int i = tid; i < 2 * S::Q_BYTES / 16; i += S::THREADS)
+      reinterpret_cast<uint4*>(qbuf)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+  }
   pdl_wait();
   pdl_launch_dependents();
 
   // Tiles of each request and their running sum; the request this run starts in.
   const int per = (A.B + S::THREADS - 1) / S::THREADS;
   const int b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
-  auto tiles_of = [&](int b, int64_t& first, int& n, int64_t& ctx, int64_t& t, int& blocks) {
+  // A request's rows, tiles and blocks; a unit counts one tile more than it
+  // has, for the cost of its start and its end.
+  auto look = [&](int b) {
+    Request R;
     int64_t end;
-    request_rows(A.cu, b, A.total, first, end);
-    n = (int)(end - first);
-    ctx = max(A.context[b], 0);
-    t = n ? (ctx + n + KT - 1) / KT : 0;
-    blocks = (int)(((int64_t)n * A.g + S::RB - 1) / S::RB);
+    const int ctx = A.context[b];
+    request_rows(A.cu, b, A.total, R.first, end);
+    R.n = (int)(end - R.first);
+    R.ctx = max(ctx, 0);
+    R.tiles = R.n ? (R.ctx + R.n + KT - 1) / KT : 0;
+    R.blocks = (int)(((int64_t)R.n * A.g + S::RB - 1) / S::RB);
+    return R;
+  };
+  auto length = [&](const Request& R) {
+    return R.n ? (R.tiles + UNIT_COST) * R.blocks * A.Hkv : (int64_t)0;
   };
   int64_t mine = 0;
+  Request R0 = {};
   for (int b = b0; b < b1; ++b) {
-    int64_t first, ctx, t;
-    int n, blocks;
-    tiles_of(b, first, n, ctx, t, blocks);
-    mine += t * blocks * A.Hkv;
+    const Request R = look(b);
+    if (b == b0) R0 = R;
+    mine += length(R);
   }
   int64_t incl = mine;
   for (int o = 1; o < 32; o <<= 1) {
@@ -207,13 +244,12 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
   if (mine > 0 && excl <= lo && lo < excl + mine) {
     int64_t at = excl;
     for (int b = b0; b < b1; ++b) {
-      int64_t first, ctx, t;
-      int n, blocks;
-      tiles_of(b, first, n, ctx, t, blocks);
-      const int64_t w = t * blocks * A.Hkv;
+      if (b > b0) R0 = look(b);
+      const int64_t w = length(R0);
       if (lo < at + w) {
-        B->b = b;
-        B->base = at;
+        B->start.r = R0;
+        B->start.base = at;
+        B->start.b = b;
         break;
       }
       at += w;
@@ -226,52 +262,56 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
     const uint64_t pol = l2_evict_first_policy();
     const int ps = A.ps, shift = 31 - __clz(ps);
     const int box = min(ps, KT), ppt = KT / box;
-    int64_t pos = lo, base = B->base;
-    int b = B->b, seg = 0, stage = 0;
+    int64_t pos = lo, base = B->start.base;
+    Request R = B->start.r;
+    int b = B->start.b, seg = 0, stage = 0;
     uint32_t phase = 0;
     bool ok = true, again = false;
     while (pos < hi && ok) {
-      int64_t first, ctx, t;
-      int n, blocks;
-      tiles_of(b, first, n, ctx, t, blocks);
-      const int64_t w = t * blocks;
-      if (pos >= base + w * A.Hkv) {
-        base += w * A.Hkv;
-        ++b;
+      const int64_t w = length(R);
+      if (pos >= base + w) {
+        base += w;
+        R = look(++b);
         continue;
       }
-      const int64_t off = pos - base;
-      const int hk = (int)(off / w);
-      const int64_t rem = off - hk * w;
-      const int rb = (int)(rem / t);
-      const int64_t t0 = rem - rb * t, u0 = pos - t0;
-      const int64_t t1 = min(t, t0 + (hi - pos));
+      const int64_t len = R.tiles + UNIT_COST;
+      const int unit = (int)quotient(pos - base, len);       // of the request: head, row block
+      const int hk = unit / R.blocks, rb = unit - hk * R.blocks;
+      const int64_t u0 = base + unit * len + UNIT_COST;   // where the unit's first tile is
+      const int64_t until = min(hi, u0 + R.tiles);
+      const int64_t t0 = max(pos - u0, (int64_t)0), t1 = until - u0;
+      pos = until;
+      if (t1 <= t0) continue;                           // the run ends in the unit's start
       const int sb = seg & 1;
       if (seg >= 2 && !wait_phase(&B->q_empty[sb], ((seg >> 1) - 1) & 1, abort_f, A.err)) break;
       const int row0 = rb * S::RB;
-      const int rows = (int)min((int64_t)S::RB, (int64_t)n * A.g - row0);
+      const int rows = (int)min((int64_t)S::RB, (int64_t)R.n * A.g - row0);
       if (lane == 0) {
         Segment& G = B->seg[sb];
-        G.first = first;
-        G.ctx = ctx;
-        G.n = n;
+        G.first = R.first;
+        G.ctx = R.ctx;
+        G.b = b;
+        G.n = R.n;
+        G.t0 = t0;
+        G.t1 = t1;
         G.hk = hk;
         G.row0 = row0;
         G.rows = rows;
-        G.whole = t0 == 0 && t1 == t;
+        G.whole = t0 == 0 && t1 == R.tiles;
         G.starts = t0 == 0;
         G.c0 = run_of(total, ctas, u0);
-        G.parts = run_of(total, ctas, u0 + t - 1) - G.c0 + 1;
+        G.parts = run_of(total, ctas, u0 + R.tiles - 1) - G.c0 + 1;
+        G.end = 0;
         mbar_arrive_expect_tx(&B->q_full[sb], (uint32_t)(rows * A.Dk * 2));
       }
       __syncwarp();
       for (int r = lane; r < rows; r += 32) {
         const int tok = (row0 + r) / A.g, h = row0 + r - tok * A.g;
         bulk_g2s(qbuf + sb * S::Q_BYTES + r * S::QP,
-                 A.q + (first + tok) * A.q_tok + (int64_t)(hk * A.g + h) * A.q_head,
+                 A.q + (R.first + tok) * A.q_tok + (int64_t)(hk * A.g + h) * A.q_head,
                  (uint32_t)(A.Dk * 2), &B->q_full[sb], pol);
       }
-      const int64_t end = ctx + n;
+      const int64_t end = R.ctx + R.n;
       int64_t have = -1;         // first table entry held by lane 0
       int ids = -1;
       for (int64_t tile = t0; tile < t1; ++tile) {
@@ -329,8 +369,13 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
           again = true;
         }
       }
-      pos += t1 - t0;
       ++seg;
+    }
+    if (seg < 2 || wait_phase(&B->q_empty[seg & 1], ((seg >> 1) - 1) & 1, abort_f, A.err)) {
+      if (lane == 0) {
+        B->seg[seg & 1].end = 1;
+        mbar_arrive(&B->q_full[seg & 1]);
+      }
     }
     // On the error path, copies in flight land before the CTA may exit.
     if (*abort_f) {
@@ -350,10 +395,9 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
   const int wm = warp / S::WK, wk = warp - wm * S::WK;
   int stage = 0, seg = 0;
   uint32_t phase = 0;
-  int64_t pos = lo;
   const int frow = lane >> 2, fcol = (lane & 3) * 2;     // accumulator row and column
   // Barriers among consumer warps, bounded like every wait.
-  uint32_t all_phase = 0, share_phase = 0;
+  uint32_t all_phase = 0;
   auto meet = [&](uint64_t* bar, uint32_t& ph) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
@@ -361,10 +405,12 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
     ph ^= 1u;
     return ok;
   };
-  while (pos < hi) {
+  for (;; ++seg) {
     const int sb = seg & 1;
     if (!wait_phase(&B->q_full[sb], (seg >> 1) & 1, abort_f, A.err)) return;
-    const Segment G = B->seg[sb];
+    const Segment& G = B->seg[sb];     // the producer waits for q_empty to reuse it
+    if (G.end) return;
+    const int64_t ctx = G.ctx;
     uint32_t qf[DKP / 16][4];
     {
       const uint32_t base = smem_addr(qbuf + sb * S::Q_BYTES) +
@@ -372,8 +418,6 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
 #pragma unroll
       for (int k = 0; k < DKP / 16; ++k) ldmatrix_x4(qf[k], base + k * 32);
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&B->q_empty[sb]);
     // The tree words of this thread's two rows.
     int tok[2];
     uint64_t word[2];
@@ -384,7 +428,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       word[i] = A.mask ? (uint64_t)A.mask[G.first + tok[i]] : 0;
     }
     auto sees = [&](int i, int64_t key) {
-      const int64_t j = key - G.ctx;
+      const int64_t j = key - ctx;
       if (j < 0) return true;
       return A.mask ? (j < 64 && ((word[i] >> j) & 1)) : j <= tok[i];
     };
@@ -400,7 +444,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       last = B->last[stage] != 0;
       const uint64_t valid = B->valid[stage];
       const int64_t key0 = B->key0[stage];
-      const bool step_keys = key0 + KT > G.ctx;
+      const bool step_keys = key0 + KT > ctx;
       uint8_t* kt = ring + stage * S::STAGE;
       uint8_t* vt = kt + S::KC * CHUNK;
       float s[S::KPW / 8][4];
@@ -433,57 +477,33 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
             const int c = wk * S::KPW + i * 8 + fcol + (j & 1);
             if (!((valid >> c) & 1) || !sees(j >> 1, key0 + c)) s[i][j] = -INFINITY;
           }
-        // Elements of this step's values that are no numbers go to the rows
-        // that see them and leave the tile, which the warps with the same keys
-        // do together; values of keys that do not exist become zero.
-        constexpr uint32_t KEYS = S::KPW == 32 ? 0xffffffffu : (1u << S::KPW) - 1u;
-        const uint32_t gone = ~(uint32_t)(valid >> (wk * S::KPW)) & KEYS;
-        uint32_t odd_rows = 0;
-        if (step_keys && (G.n > 1 || A.mask)) {
-          for (int r = 0; r < S::KPW; ++r) {
-            const int c = wk * S::KPW + r;
-            if (((gone >> r) & 1) || key0 + c < G.ctx) continue;
-            bool odd = false;
-            for (int x = lane; x < DVP / 2; x += 32) {
-              const uint32_t u = *reinterpret_cast<const uint32_t*>(
-                  vt + (x >> 5) * CHUNK + c * 128 + ((((x >> 2) & 7) ^ (c & 7)) << 4) +
-                  (x & 3) * 4);
-              odd = odd || odd_element<F16>((uint16_t)u) || odd_element<F16>((uint16_t)(u >> 16));
-            }
-            if (!__any_sync(0xffffffffu, odd)) continue;
-            odd_rows |= 1u << r;
-#pragma unroll
-            for (int i = 0; i < DVP / 8; ++i)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int d = i * 8 + fcol + j;
-                const uint16_t u = *reinterpret_cast<const uint16_t*>(
-                    vt + (d >> 6) * CHUNK + c * 128 + ((((d >> 3) & 7) ^ (c & 7)) << 4) +
-                    (d & 7) * 2);
-                if (!odd_element<F16>(u)) continue;
-                if (sees(0, key0 + c)) o[i][j] += element<F16>(u);
-                if (sees(1, key0 + c)) o[i][j + 2] += element<F16>(u);
-              }
-          }
-          if (MT > 1 && !meet(&B->share[wk], share_phase)) return;
-        }
-        if (gone | odd_rows) {
-          __syncwarp();
+        // Values of keys that do not exist become zero, and so do elements of
+        // this step's values that are no numbers (noted for the end).  Warps
+        // with the same keys may do so at the same time: they write the same.
+        const bool scan = step_keys && (G.n > 1 || A.mask);
+        const uint32_t there = (uint32_t)(valid >> (wk * S::KPW));
+        bool wrote = false;
+        if (scan || valid != ~0ull)
+#pragma unroll 4
           for (int x = lane; x < S::KPW * (DVP / 8); x += 32) {
             const int r = x / (DVP / 8), c = wk * S::KPW + r, piece = x - r * (DVP / 8);
             uint4* at = reinterpret_cast<uint4*>(vt + (piece >> 3) * CHUNK + c * 128 +
                                                  (((piece & 7) ^ (c & 7)) << 4));
-            if ((gone >> r) & 1) {
+            if (!((there >> r) & 1)) {
               *at = make_uint4(0, 0, 0, 0);
-            } else if ((odd_rows >> r) & 1) {
-              uint16_t* e = reinterpret_cast<uint16_t*>(at);
-              for (int j = 0; j < 8; ++j)
-                if (odd_element<F16>(e[j])) e[j] = 0;
+              wrote = true;
+            } else if (scan && key0 + c >= ctx) {
+              uint4 v = *at;
+              if (has_odd<F16>(v)) {
+                clear_odd<F16>(v);
+                B->odd[sb] = 1;
+                *at = v;
+                wrote = true;
+              }
             }
           }
-          fence_proxy_async();     // before the next copy into this stage
-          __syncwarp();
-        }
+        if (__any_sync(0xffffffffu, wrote)) fence_proxy_async();   // before the next copy
+        __syncwarp();
       }
       float top[2] = {m[0], m[1]};
 #pragma unroll
@@ -543,9 +563,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
         stage = 0;
         phase ^= 1u;
       }
-      ++pos;
     }
-    ++seg;
 
     // Join the warps that shared the keys: half of them hand over, then half
     // of the rest.
@@ -555,14 +573,22 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
     constexpr int XF = DVP / 2 + 4;
+    const bool upper = G.rows > wm * 16 + 8;      // rows in the second half of the 16
 #pragma unroll
     for (int half = S::WK / 2; half >= 1; half >>= 1) {
       float* x = xbuf + (size_t)(wm * (S::WK / 2) + (wk & (half - 1))) * 32 * XF + lane;
       if (wk >= half && wk < 2 * half) {
 #pragma unroll
-        for (int i = 0; i < DVP / 8; ++i)
+        for (int i = 0; i < DVP / 8; ++i) {
+          x[(i * 4) * 32] = o[i][0];
+          x[(i * 4 + 1) * 32] = o[i][1];
+        }
+        if (upper)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[(i * 4 + j) * 32] = o[i][j];
+          for (int i = 0; i < DVP / 8; ++i) {
+            x[(i * 4 + 2) * 32] = o[i][2];
+            x[(i * 4 + 3) * 32] = o[i][3];
+          }
         x[(XF - 4) * 32] = m[0];
         x[(XF - 3) * 32] = m[1];
         x[(XF - 2) * 32] = l[0];
@@ -581,15 +607,39 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
           l[i] = l[i] * f0[i] + ol * f1[i];
         }
 #pragma unroll
-        for (int i = 0; i < DVP / 8; ++i)
+        for (int i = 0; i < DVP / 8; ++i) {
+          o[i][0] = o[i][0] * f0[0] + x[(i * 4) * 32] * f1[0];
+          o[i][1] = o[i][1] * f0[0] + x[(i * 4 + 1) * 32] * f1[0];
+        }
+        if (upper)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[i][j] = o[i][j] * f0[j >> 1] + x[(i * 4 + j) * 32] * f1[j >> 1];
+          for (int i = 0; i < DVP / 8; ++i) {
+            o[i][2] = o[i][2] * f0[1] + x[(i * 4 + 2) * 32] * f1[1];
+            o[i][3] = o[i][3] * f0[1] + x[(i * 4 + 3) * 32] * f1[1];
+          }
       }
       if (!meet(&B->all, all_phase)) return;
     }
 
     if (wk == 0) {
+      if (B->odd[sb]) {
+        // Values that are no numbers, from the cache, to the rows that see them.
+        for (int64_t key = max(ctx, G.t0 * KT); key < min(ctx + G.n, G.t1 * KT); ++key) {
+          const int64_t e = key / A.ps;
+          const int id = e < A.width ? A.table[(int64_t)G.b * A.table_stride + e] : -1;
+          if (id < 0 || id >= A.n_pages) continue;
+          const uint16_t* v = A.v + id * A.v_page + (key - e * A.ps) * A.v_row + G.hk * A.v_head;
+          const bool s0 = sees(0, key), s1 = sees(1, key);
+#pragma unroll
+          for (int i = 0; i < DVP / 8; ++i)
+            for (int j = 0; j < 2 && i * 8 < A.Dv; ++j) {
+              const uint16_t u = v[i * 8 + fcol + j];
+              if (!odd_element<F16>(u)) continue;
+              if (s0) o[i][j] += element<F16>(u);
+              if (s1) o[i][2 + j] += element<F16>(u);
+            }
+        }
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = wm * 16 + frow + h * 8;
@@ -618,89 +668,95 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
         }
       }
     }
-    if (G.whole) continue;
-
-    // The last of the unit's CTAs joins their sums, in CTA order.
-    __threadfence();
-    if (!meet(&B->all, all_phase)) return;
-    if (tid == 0) {
-      const int old = atomicAdd(&A.counters[G.c0], 1);
-      B->joined = old == G.parts - 1;
-      if (B->joined) A.counters[G.c0] = 0;
-    }
-    if (!meet(&B->all, all_phase)) return;
-    if (B->joined) {
+    if (!G.whole) {
+      // The last of the unit's CTAs joins their sums, in CTA order.
       __threadfence();
-      // Few items: several threads share an item's partial sums.
-      constexpr int T = S::NW * 32;
-      const int quads = A.Dv / 4, items = G.rows * quads;
-      int share = 1;
-      while (share < 32 && share * 2 * items <= T) share *= 2;
-      for (int base = 0; base < items; base += T / share) {
-        const int it = base + tid % (T / share), sh = tid / (T / share);
-        const int r = min(it, items - 1) / quads, d = (min(it, items - 1) - r * quads) * 4;
-        float tm = -INFINITY, tl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int c = sh; c < G.parts; c += 4 * share) {
-          float2 ml[4];
-          float4 v[4];
+      if (!meet(&B->all, all_phase)) return;
+      if (tid == 0) {
+        const int old = atomicAdd(&A.counters[G.c0], 1);
+        B->joined = old == G.parts - 1;
+        if (B->joined) A.counters[G.c0] = 0;
+      }
+      if (!meet(&B->all, all_phase)) return;
+      if (B->joined) {
+        __threadfence();
+        // Few items: several threads share an item's partial sums.
+        constexpr int T = S::NW * 32;
+        const int quads = A.Dv / 4, items = G.rows * quads;
+        int share = 1;
+        while (share < 32 && share * 2 * items <= T) share *= 2;
+        for (int base = 0; base < items; base += T / share) {
+          const int it = base + tid % (T / share), sh = tid / (T / share);
+          const int r = min(it, items - 1) / quads, d = (min(it, items - 1) - r * quads) * 4;
+          float tm = -INFINITY, tl = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int c = sh; c < G.parts; c += 4 * share) {
+            float2 ml[4];
+            float4 v[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int cc = c + u * share;
-            ml[u] = make_float2(-INFINITY, 0.f);
-            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (cc < G.parts) {
-              const int64_t slot = ((int64_t)(G.c0 + cc) * 2 + (cc == 0)) * S::RB + r;
-              ml[u] = __ldcg(reinterpret_cast<const float2*>(A.part_ml + slot * 2));
-              v[u] = __ldcg(reinterpret_cast<const float4*>(A.part_o + slot * DVP + d));
+            for (int u = 0; u < 4; ++u) {
+              const int cc = c + u * share;
+              ml[u] = make_float2(-INFINITY, 0.f);
+              v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (cc < G.parts) {
+                const int64_t slot = ((int64_t)(G.c0 + cc) * 2 + (cc == 0)) * S::RB + r;
+                ml[u] = __ldcg(reinterpret_cast<const float2*>(A.part_ml + slot * 2));
+                v[u] = __ldcg(reinterpret_cast<const float4*>(A.part_o + slot * DVP + d));
+              }
             }
-          }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float t = fmaxf(tm, ml[u].x);
-            if (t == -INFINITY) continue;
-            const float f0 = exp2_fast(tm - t), f1 = exp2_fast(ml[u].x - t);
-            tm = t;
-            tl = tl * f0 + ml[u].y * f1;
-            acc[0] = acc[0] * f0 + v[u].x * f1;
-            acc[1] = acc[1] * f0 + v[u].y * f1;
-            acc[2] = acc[2] * f0 + v[u].z * f1;
-            acc[3] = acc[3] * f0 + v[u].w * f1;
-          }
-        }
-        if (share > 1) {
-          // Through shared memory, in order.
-          float* x = xbuf + tid * 6;
-          x[0] = tm;
-          x[1] = tl;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[2 + j] = acc[j];
-          if (!meet(&B->all, all_phase)) return;
-          if (sh == 0)
-            for (int u = 1; u < share; ++u) {
-              const float* y = xbuf + (tid + u * (T / share)) * 6;
-              const float t = fmaxf(tm, y[0]);
+            for (int u = 0; u < 4; ++u) {
+              const float t = fmaxf(tm, ml[u].x);
               if (t == -INFINITY) continue;
-              const float f0 = exp2_fast(tm - t), f1 = exp2_fast(y[0] - t);
+              const float f0 = exp2_fast(tm - t), f1 = exp2_fast(ml[u].x - t);
               tm = t;
-              tl = tl * f0 + y[1] * f1;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[j] = acc[j] * f0 + y[2 + j] * f1;
+              tl = tl * f0 + ml[u].y * f1;
+              acc[0] = acc[0] * f0 + v[u].x * f1;
+              acc[1] = acc[1] * f0 + v[u].y * f1;
+              acc[2] = acc[2] * f0 + v[u].z * f1;
+              acc[3] = acc[3] * f0 + v[u].w * f1;
             }
-          if (!meet(&B->all, all_phase)) return;
-        }
-        if (sh == 0 && it < items) {
-          const int t = (G.row0 + r) / A.g;
-          const int64_t at = (G.first + t) * A.Hq + G.hk * A.g + (G.row0 + r - t * A.g);
-          const float inv = tl > 0.f ? 1.f / tl : tl == 0.f ? 0.f : tl;
-          uint2 w;
-          w.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
-          w.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
-          *reinterpret_cast<uint2*>(A.out + at * A.Dv + d) = w;
-          if (A.lse && d == 0) A.lse[at] = tl == 0.f ? -INFINITY : (tm + log2f(tl)) * LN2;
+          }
+          if (share > 1) {
+            // Through shared memory, in order.
+            float* x = xbuf + tid * 6;
+            x[0] = tm;
+            x[1] = tl;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[2 + j] = acc[j];
+            if (!meet(&B->all, all_phase)) return;
+            if (sh == 0)
+              for (int u = 1; u < share; ++u) {
+                const float* y = xbuf + (tid + u * (T / share)) * 6;
+                const float t = fmaxf(tm, y[0]);
+                if (t == -INFINITY) continue;
+                const float f0 = exp2_fast(tm - t), f1 = exp2_fast(y[0] - t);
+                tm = t;
+                tl = tl * f0 + y[1] * f1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = acc[j] * f0 + y[2 + j] * f1;
+              }
+            if (!meet(&B->all, all_phase)) return;
+          }
+          if (sh == 0 && it < items) {
+            const int t = (G.row0 + r) / A.g;
+            const int64_t at = (G.first + t) * A.Hq + G.hk * A.g + (G.row0 + r - t * A.g);
+            const float inv = tl > 0.f ? 1.f / tl : tl == 0.f ? 0.f : tl;
+            uint2 w;
+            w.x = pack2<F16>(acc[0] * inv, acc[1] * inv);
+            w.y = pack2<F16>(acc[2] * inv, acc[3] * inv);
+            *reinterpret_cast<uint2*>(A.out + at * A.Dv + d) = w;
+            if (A.lse && d == 0) A.lse[at] = tl == 0.f ? -INFINITY : (tm + log2f(tl)) * LN2;
+          }
         }
       }
     }
+    // Everyone is done with the segment and the exchange buffer.
+    if (B->odd[sb]) {
+      if (!meet(&B->all, all_phase)) return;
+      if (tid == 0) B->odd[sb] = 0;
+    }
     if (!meet(&B->all, all_phase)) return;
+    if (lane == 0) mbar_arrive(&B->q_empty[sb]);
   }
 }
 
@@ -775,6 +831,7 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   KB_REQUIRE(page_size >= 8 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
              KB_ERR_UNSUPPORTED, "tree attention: the page size must be a power of two from 8");
   if (B == 0 || total == 0) return KB_OK;
+  KB_REQUIRE(scale > 0.f, KB_ERR_BAD_SHAPE, "attention: the scale must be positive");
   KB_REQUIRE(max_tokens > 0 && n_pages > 0, KB_ERR_BAD_SHAPE,
              "tree attention: tokens but max_tokens 0, or a cache without pages");
   KB_REQUIRE(q && k_strides && v_strides && cu_tokens && context_lens && out && k_cache &&
@@ -801,6 +858,10 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   A.q = q;
   A.q_tok = q_token_stride;
   A.q_head = q_head_stride;
+  A.v = v_cache;
+  A.v_page = v_strides[0];
+  A.v_row = v_strides[1];
+  A.v_head = v_strides[2];
   A.out = out;
   A.lse = lse;
   A.cu = cu_tokens;

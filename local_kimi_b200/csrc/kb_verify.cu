@@ -333,16 +333,17 @@ static size_t power_of_two(int64_t n) {
   return p;
 }
 
-// The counters come first, in room for the next power of two of requests, so
-// that every call whose requests round to the same power finds them zero.
-static size_t counter_bytes(int64_t B) { return power_of_two(B) * sizeof(Race); }
+// The counters of up to MAX_REQUESTS requests come first, at the same place
+// for every call, so that whatever call used the buffer before left them zero.
+constexpr int MAX_REQUESTS = 65536;
+constexpr size_t COUNTER_BYTES = MAX_REQUESTS * sizeof(Race);
 
 }  // namespace verify
 }  // namespace kb
 
 extern "C" size_t kb_verify_drafts_workspace_size(int64_t B, int64_t rows) {
   if (B <= 0 || rows < 0) return 0;
-  return kb::verify::counter_bytes(B) +
+  return kb::verify::COUNTER_BYTES +
          kb::verify::power_of_two(rows) * kb::verify::MAX_SEGMENTS * sizeof(kb::verify::Stat);
 }
 
@@ -395,7 +396,7 @@ extern "C" int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t 
   A.path = path;
   A.accepted = accepted;
   A.race = static_cast<v::Race*>(workspace);
-  A.stats = reinterpret_cast<v::Stat*>(static_cast<uint8_t*>(workspace) + v::counter_bytes(B));
+  A.stats = reinterpret_cast<v::Stat*>(static_cast<uint8_t*>(workspace) + v::COUNTER_BYTES);
   v::split(B, max_tokens, V, kb::num_sms(dev), &A.segments, &A.parts);
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");

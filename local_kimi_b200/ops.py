@@ -949,13 +949,32 @@ class Verification(NamedTuple):
 def _vector(t: torch.Tensor, dtype: torch.dtype, what: str, device: torch.device,
             length: int | None = None) -> torch.Tensor:
     """A 1-D contiguous tensor of a type, length and device."""
-    if t.dtype != dtype or t.ndim != 1:
+    if t.dtype != dtype or t.dim() != 1:
         raise TypeError(f"{what} must be a one-dimensional {dtype} tensor")
-    if length is not None and t.shape[0] != length:
+    if length is not None and t.numel() != length:
         raise ValueError(f"{what} must have {length} entries")
     if t.device != device:
         raise ValueError(f"{what} must be on the device of the other tensors")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _raw_stream(device: torch.device) -> int:
+    """The current stream's handle, without a torch.cuda.Stream object around it (a
+    microsecond or two that these calls, short beside their launch, would notice)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _zeroed(kind: str, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Scratch of the operators below, kept per (kind, device, stream, size).
+
+    Calls of one kind and size share one layout and leave the counters in it
+    at zero (see _workspace).
+    """
+    key = (kind, device.index, stream, nbytes)
+    ws = _WORKSPACES.get(key)
+    if ws is None:
+        ws = _WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return ws
 
 
 def paged_plan(
@@ -1012,7 +1031,7 @@ def paged_plan(
         head.data_ptr(), page_size, num_tokens, None if par is None else par.data_ptr(),
         cu.data_ptr(), slots.data_ptr(), positions.data_ptr(),
         None if mask is None else mask.data_ptr(), head_out.data_ptr(), missing.data_ptr(),
-        _stream(device),
+        _raw_stream(device),
     )
     return PagedPlan(cu, slots, positions, mask, head_out, missing)
 
@@ -1083,7 +1102,7 @@ def paged_append(
         "kb_paged_append", kr.data_ptr(), kr.stride(0), kr.stride(1), vr.data_ptr(),
         vr.stride(0), vr.stride(1), n, heads, dk, dv, k_cache.data_ptr(), ks,
         v_cache.data_ptr(), vs, k_cache.shape[0], k_cache.shape[1], sl.data_ptr(),
-        _stream(device),
+        _raw_stream(device),
     )
 
 
@@ -1093,6 +1112,14 @@ def _attention_heads(q: torch.Tensor, heads: int, dk: int, dv: int) -> None:
     if q.shape[2] != dk:
         raise ValueError("queries and keys must have one width")
     _check_widths(dk, dv)
+
+
+def _scale_of(scale: float | None, dk: int) -> float:
+    if scale is None:
+        return dk ** -0.5
+    if not scale > 0:
+        raise ValueError("the scale must be positive")
+    return float(scale)
 
 
 def prompt_attention(
@@ -1139,16 +1166,16 @@ def prompt_attention(
         ck = cq
     else:
         ck = _vector(cu_seqlens_k, torch.int32, "cu_seqlens_k", device, requests + 1)
-    if max_seqlen < 0:
-        raise ValueError("max_seqlen must not be negative")
+    if max_seqlen < 0 or (total and not max_seqlen):
+        raise ValueError("max_seqlen must not be negative, nor 0 with tokens")
     out = torch.empty((total, hq, dv), dtype=q.dtype, device=device)
     lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
     _lib.call(
         "kb_prompt_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), kr.data_ptr(),
         kr.stride(0), kr.stride(1), vr.data_ptr(), vr.stride(0), vr.stride(1),
         _ELEMENT[q.dtype], cq.data_ptr(), ck.data_ptr(), requests, total, keys, max_seqlen, hq,
-        hkv, dk, dv, dk ** -0.5 if scale is None else float(scale), out.data_ptr(),
-        None if lse is None else lse.data_ptr(), _stream(device),
+        hkv, dk, dv, _scale_of(scale, dk), out.data_ptr(),
+        None if lse is None else lse.data_ptr(), _raw_stream(device),
     )
     return out if lse is None else (out, lse)
 
@@ -1214,15 +1241,16 @@ def tree_attention(
     lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
     if total == 0 or requests == 0:
         return out if lse is None else (out, lse)
-    need = _lib.lib().kb_tree_attention_workspace_size(hq // hkv, max_tokens)
-    ws = _workspace("tree_attention", device, need, (need,))
+    stream = _raw_stream(device)
+    ws = _zeroed("tree_attention", device, stream,
+                 _lib.lib().kb_tree_attention_workspace_size(hq // hkv, max_tokens))
     _lib.call(
         "kb_tree_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), k_cache.data_ptr(), ks,
         v_cache.data_ptr(), vs, _ELEMENT[q.dtype], pages, page_size, table.data_ptr(),
         max(table.stride(0), width), width, ctx.data_ptr(), cu.data_ptr(),
         None if mask is None else mask.data_ptr(), requests, total, max_tokens, hq, hkv, dk, dv,
-        dk ** -0.5 if scale is None else float(scale), out.data_ptr(),
-        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device),
+        _scale_of(scale, dk), out.data_ptr(),
+        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream,
     )
     return out if lse is None else (out, lse)
 
@@ -1286,23 +1314,18 @@ def verify_drafts(
     if requests == 0:
         return Verification(out, path, accepted)
     x, e = _unit_rows(logits), _unit_rows(noise)
-    need = _lib.lib().kb_verify_drafts_workspace_size(requests, rows)
-    # The size says how many requests and rows (each rounded up to a power of
-    # two) the buffer holds, so calls of one size share one layout.
-    ws = _workspace("verify", device, need, (_power_of_two(requests), need))
+    stream = _raw_stream(device)
+    ws = _zeroed("verify_drafts", device, stream,
+                 _lib.lib().kb_verify_drafts_workspace_size(requests, rows))
     _lib.call(
         "kb_verify_drafts", x.data_ptr(), max(x.stride(0), vocab), rows, vocab,
         _ELEMENT[x.dtype], tok.data_ptr(), None if par is None else par.data_ptr(),
         cu.data_ptr(), requests, max_tokens, coin.data_ptr(), e.data_ptr(),
         max(e.stride(0), vocab), temps.data_ptr(), None if probs is None else probs.data_ptr(),
         vocab if probs is None else max(probs.stride(0), vocab), out.data_ptr(),
-        path.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device),
+        path.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), stream,
     )
     return Verification(out, path, accepted)
-
-
-def _power_of_two(n: int) -> int:
-    return 1 << max(4, (n - 1).bit_length())
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:

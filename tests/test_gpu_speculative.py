@@ -82,6 +82,30 @@ def test_prompt_attention(cuda, dtype, lens, extra, heads, kv, dk, dv):
     check_attention(out, lse, *ref.prompt_attention(q, k, v, cq, ck, scale), dtype)
 
 
+@pytest.mark.parametrize("lens,heads,kv,dk,dv", [
+    ([40, 7], 400, 400, 64, 64), ([1500, 1, 900], 32, 32, 192, 128), ([2100, 300], 24, 3, 128, 128),
+])
+def test_prompt_attention_many_units(cuda, lens, heads, kv, dk, dv):
+    # More units of rows than SMs, so a CTA goes through several; the softmax
+    # by its definition in 64 bits, all heads at once on the device.
+    gen = torch.Generator(device=cuda).manual_seed(len(lens) + heads)
+    q = torch.randn(sum(lens), heads, dk, generator=gen, device=cuda).bfloat16()
+    k = torch.randn(sum(lens), kv, dk, generator=gen, device=cuda).bfloat16()
+    v = torch.randn(sum(lens), kv, dv, generator=gen, device=cuda).bfloat16()
+    cu = sums(lens)
+    out, lse = ops.prompt_attention(q, k, v, ints(cu, cuda), max(lens), return_lse=True)
+    for a, b in zip(cu, cu[1:]):
+        x = q[a:b].double().view(b - a, kv, heads // kv, dk)
+        s = torch.einsum("tkgd,skd->kgts", x, k[a:b].double()) * dk ** -0.5
+        s.masked_fill_(torch.ones(b - a, b - a, dtype=torch.bool, device=cuda).triu(1),
+                       float("-inf"))
+        w, p = s.logsumexp(-1), s.softmax(-1)
+        want = torch.einsum("kgts,skd->tkgd", p, v[a:b].double()).reshape(b - a, heads, dv)
+        size = torch.einsum("kgts,skd->tkgd", p, v[a:b].double().abs()).reshape(b - a, heads, dv)
+        check_attention(out[a:b], lse[a:b], want.cpu(), w.permute(2, 0, 1).reshape(b - a, heads).cpu(),
+                        size.cpu(), torch.bfloat16)
+
+
 def test_prompt_attention_rows_without_keys(cuda):
     # More queries than keys: the first rows of a request see nothing.
     gen = torch.Generator().manual_seed(7)
