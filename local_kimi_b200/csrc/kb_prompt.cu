@@ -12,6 +12,9 @@
 // tiles and keys are read once for them.  Units go out heaviest (latest rows)
 // first, there and back over the CTAs.
 //
+//   warp 11: the list of units.  It counts, 32 requests at a time, which have
+//     rows that late, and tells the other warps this CTA's units through a
+//     ring of four.
 //   warp 9: copies.  Q tiles, and a ring of 16 KB slots with the keys (128
 //     rows x 64 elements a slot) and values (64 or 128 rows) in use order, by
 //     tensor copies in the 128-byte swizzle; a barrier pair per key or value
@@ -24,20 +27,26 @@
 //     next S of the same tile, so S never overwrites a P still being read.
 //   warps 0-3 and 4-7: softmax of tiles A and B, a row per thread: maximum,
 //     exponentials in base 2, row sum in fp32, and P rounded once to the
-//     inputs' type.  The running maximum only moves, and O is only rescaled,
-//     when a row's maximum rose by more than 2^8: weights stay within fp32
-//     and the 16-bit types, and the final division makes up for the rest.
+//     inputs' type, handed over in two halves of 64 keys.  The running maximum
+//     only moves, and O is only rescaled, when a row's maximum rose by more
+//     than 2^8: weights stay within fp32 and the 16-bit types, and the final
+//     division makes up for the rest.
 //
-// 512 columns of tensor memory: S A, S B, O A, O B.  The math is bound by the
-// MMAs (2 (Dk + Dv) flops a pair) and, at Dk = 128, as much by the
-// exponentials: 16 a clock and SM, 1024 clocks a tile of 128 x 128.
+// 512 columns of tensor memory: S A, S B, O A, O B.  MMAs are 2 (Dk + Dv) flops
+// a pair, 1024 to 1280 clocks a tile of 128 x 128 at 128 to 192 + 128 wide
+// heads; the exponentials at 16 a clock and SM are 1024 clocks a tile.  With
+// two tiles in turn the period is one tile's softmax plus its MMAs, so every
+// clock of the softmax counts: measured on the way, maximum 500 -> 250 clocks
+// with three-input maxima, exponentials 1650 with the special function unit
+// alone.  One in POLY_EVERY pairs is computed on the FMA pipes instead.
 //
 // In the last tiles of a unit some rows do not see some keys, or the tile
 // reaches past the request's end into its neighbour.  A value there that is
-// infinite or not a number must not meet a zero weight: warps 10 and 11 zero
-// such elements in those tiles before the MMA reads them, and at the end the
-// rows that do see them take them from memory.
+// infinite or not a number must not meet a zero weight: warp 10 zeroes such
+// elements in those tiles before the MMA reads them, and at the end the rows
+// that do see them take them from memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "kb_attn.cuh"
 #include "kb_tcgen05.cuh"
@@ -48,7 +57,9 @@ namespace attn {
 constexpr int TILE = 128;                  // rows of a tile, keys of a step
 constexpr int SLOT = 16384;                // bytes of a ring slot
 constexpr int PROMPT_THREADS = 384;
-constexpr int MMA_WARP = 8, COPY_WARP = 9, CLEAN_WARP = 10;   // and 11
+constexpr int MMA_WARP = 8, COPY_WARP = 9, CLEAN_WARP = 10, LIST_WARP = 11;
+constexpr int UNITS = 4;                   // units told ahead
+constexpr int POLY_EVERY = 4;              // one in so many pairs of exponentials on the FMA pipes
 constexpr int ENTRIES = 8;                 // key and value tiles with a barrier pair
 constexpr float RESCALE = 8.0f;            // log2 of the growth that moves the maximum
 
@@ -79,69 +90,53 @@ struct PromptShape {
   static_assert(SLOTS >= KC + 2 * VC, "a key tile beside the value tile in use, and one to come");
 };
 
-struct PromptBars {
-  uint64_t full[ENTRIES], empty[ENTRIES];
-  uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2];
-  uint64_t clean[ENTRIES];  // a value tile is there, without odd elements
-  uint64_t drain;
-  int odd[16];              // units (counted by the CTA) that had some, by their last four bits
-  uint32_t tmem;
-  int abort_flag;
-};
-static_assert(sizeof(PromptBars) <= 1024, "barrier block");
-
-// A unit of the walk, the same for every role.
+// A unit as warp 11 tells it to the others.
 struct Unit {
-  int64_t q0, k0;           // first query and key of the request
+  int q0, k0;               // first query and key of the request
   int n, m;                 // its queries and keys
   int head0;                // first head
   int t0;                   // first token of tile A
   int tiles[2];             // key tiles that tiles A and B see
   int whole;                // of them, those that every row of A and B sees whole
+  int count;                // number of the unit in this CTA, -1: the end
 };
 
-// Units u = blockIdx.x, ... in rounds of gridDim.x, every other round backwards.
+struct PromptBars {
+  uint64_t full[ENTRIES], empty[ENTRIES];
+  uint64_t clean[ENTRIES];  // a value tile is there, without odd elements
+  uint64_t unit_full[UNITS], unit_empty[UNITS];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2];
+  uint64_t drain;
+  Unit unit[UNITS];
+  int odd[16];              // units that had odd elements, by their number's last four bits
+  uint32_t tmem;
+  int abort_flag;
+};
+static_assert(sizeof(PromptBars) <= 1024, "barrier block");
+
+// A warp's (or single thread's) way through the CTA's units.
 struct Walk {
-  const PromptArgs& A;
-  int round, total;
-  int count;                // units walked
-  __device__ __forceinline__ explicit Walk(const PromptArgs& a) : A(a), round(0), count(-1) {
-    total = A.blocks * A.B * (A.Hq >> A.pack_shift);
-  }
-  // The next unit with rows; false at the end.
+  PromptBars* B;
+  uint32_t* err;
+  int slot;
+  uint32_t phase;
+  __device__ __forceinline__ Walk(PromptBars* b, uint32_t* e) : B(b), err(e), slot(0), phase(0) {}
+  // The next unit; false at the end or on abort.
+  template <bool WARP>
   __device__ __forceinline__ bool next(Unit& U) {
-    const int groups = A.Hq >> A.pack_shift;
-    while (true) {
-      const int at = round * gridDim.x;
-      if (at >= total) return false;
-      const int u = at + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-      ++round;
-      if (u >= total) continue;
-      const int block = A.blocks - 1 - u / (A.B * groups);
-      const int rest = u % (A.B * groups);
-      const int b = rest / groups;
-      int64_t end;
-      request_rows(A.cu_q, b, A.total_q, U.q0, end);
-      U.n = (int)(end - U.q0);
-      U.t0 = (block * 2 * TILE) >> A.pack_shift;
-      if (U.t0 >= U.n) continue;
-      request_rows(A.cu_k, b, A.total_k, U.k0, end);
-      U.m = (int)(end - U.k0);
-      U.head0 = (rest - b * groups) << A.pack_shift;
-      const int span = TILE >> A.pack_shift;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int first = U.t0 + i * span, last = min(U.n, first + span) - 1;
-        const int keys = first < U.n ? min(max(last + U.m - U.n + 1, 0), U.m) : 0;
-        U.tiles[i] = (keys + TILE - 1) / TILE;
-      }
-      ++count;
-      U.whole = max(U.t0 + U.m - U.n + 1, 0) / TILE;
-      return true;
+    if (!wait_phase(&B->unit_full[slot], phase, &B->abort_flag, err)) return false;
+    U = B->unit[slot];
+    if (WARP) __syncwarp();
+    if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&B->unit_empty[slot]);
+    if (++slot == UNITS) {
+      slot = 0;
+      phase ^= 1u;
     }
+    return U.count >= 0;
   }
 };
+constexpr int WALKERS = 8 + 3;               // softmax warps, MMA, copies, cleaning
 
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   uint64_t d;
@@ -160,16 +155,56 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x for a pair of x <= 64 on the FMA pipes: x = n + f with n the nearest
+// whole number (left in the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a
+// polynomial of degree 4 fitted here to least relative error (2.7e-6, and
+// 4e-8 on average, far below the rounding of the weights), n added to the exponent.  Below
+// 2^-126 the result stays there.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 big = make_float2(12582912.f, 12582912.f);
+  const float2 nbig = make_float2(-12582912.f, -12582912.f);
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = fadd2(x, big);
+  const float2 n = fadd2(t, nbig);
+  const float2 f = ffma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = make_float2(0.00957010221f, 0.00957010221f);
+  p = ffma2(p, f, make_float2(0.0559178591f, 0.0559178591f));
+  p = ffma2(p, f, make_float2(0.240247443f, 0.240247443f));
+  p = ffma2(p, f, make_float2(0.693121791f, 0.693121791f));
+  p = ffma2(p, f, make_float2(0.999999285f, 0.999999285f));
+  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(p.x)),
+                     __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
+}
+
 // Adds to a row's outputs d0..d0+31 the values that are no numbers of the keys
 // [first, last]: they were kept out of the tile products.
 template <bool F16>
-__device__ __noinline__ void add_odd(const PromptArgs& A, const uint16_t* v, int first, int last,
-                                     int d0, float (&o)[32]) {
-  for (int64_t j = first; j <= last; ++j)
-    for (int i = 0; i < 32 && d0 + i < A.Dv; ++i) {
-      const uint16_t u = v[j * A.v_tok + d0 + i];
+__device__ __forceinline__ void add_odd(const PromptArgs& A, const uint16_t* v, int first,
+                                        int last, int d0, float (&o)[32]) {
+  for (int64_t j = first; j <= last; ++j) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint16_t u = d0 + i < A.Dv ? v[j * A.v_tok + d0 + i] : 0;
       if (odd_element<F16>(u)) o[i] += element<F16>(u);
     }
+  }
+}
+
+// Half of a transposition: lanes `step` apart keep one piece and swap the other.
+__device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int upper, int step) {
+  uint4 give = upper ? a : b;
+  give.x = __shfl_xor_sync(0xffffffffu, give.x, step);
+  give.y = __shfl_xor_sync(0xffffffffu, give.y, step);
+  give.z = __shfl_xor_sync(0xffffffffu, give.z, step);
+  give.w = __shfl_xor_sync(0xffffffffu, give.w, step);
+  if (upper) a = give; else b = give;
 }
 
 template <int DKP, int DVP, bool F16>
@@ -196,10 +231,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       mbar_init(&B->q_full[i], 1);
       mbar_init(&B->q_empty[i], 1);
       mbar_init(&B->s_full[i], 1);
-      mbar_init(&B->p_full[i], 4);
+      mbar_init(&B->p_full[i][0], 4);
+      mbar_init(&B->p_full[i][1], 4);
       mbar_init(&B->o_full[i], 1);
     }
-    for (int i = 0; i < ENTRIES; ++i) mbar_init(&B->clean[i], 2);
+    for (int i = 0; i < ENTRIES; ++i) mbar_init(&B->clean[i], 1);
+    for (int i = 0; i < UNITS; ++i) {
+      mbar_init(&B->unit_full[i], 1);
+      mbar_init(&B->unit_empty[i], WALKERS);
+    }
     for (int i = 0; i < 16; ++i) B->odd[i] = -1;
     mbar_init(&B->drain, 1);
     B->abort_flag = 0;
@@ -242,7 +282,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     const int span = TILE >> A.pack_shift;
     uint32_t s_phase = 0, o_phase = 0;
     Unit U;
-    for (Walk walk(A); walk.next(U);) {
+    for (Walk walk(B, A.err); walk.next<true>(U);) {
       const int first = U.t0 + tile * span;
       if (first >= U.n) continue;
       const int tok = first + (row >> A.pack_shift);
@@ -265,7 +305,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         tc::tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 4; ++c) tc::hold_regs(s[c]);
-        if (j * TILE + TILE - 1 > clear) {
+        const bool edge = j * TILE + TILE - 1 > clear;     // keys that some rows do not see
+        if (edge) {
           const int last = limit - j * TILE;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -275,9 +316,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         }
         float mx[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
 #pragma unroll
-        for (int i = 1; i < 32; ++i)
+        for (int i = 1; i < 31; i += 2)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[c][i]);
+          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], s[c][i], s[c][i + 1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[c][31]);
         const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
         // S being there means that every MMA issued before it is done, the
         // last P V of this tile among them: O may be touched.
@@ -287,15 +330,16 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           const float fix = now == top ? 1.f : exp2_fast(top - now);
           sum *= fix;
           top = now;
-#pragma unroll
-          for (int c = 0; c < DVP / 32; ++c) {
-            float o[32];
-            tc::tmem_ld32(o_at + c * 32, o);
+          // 16 columns at a time: the 128 scores stay in registers beside them.
+#pragma unroll 1
+          for (int c = 0; c < DVP / 16; ++c) {
+            uint32_t o[16];
+            tc::tmem_ld16(o_at + c * 16, o);
             tc::tmem_ld_wait();
             tc::hold_regs(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= fix;
-            tc::tmem_st32(o_at + c * 32, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+            tc::tmem_st16(o_at + c * 16, o);
           }
           tc::tmem_st_wait();
         } else if (j == 0) {
@@ -304,66 +348,92 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         const float at = top == -INFINITY ? 0.f : top;
         const float2 mul = make_float2(scale2, scale2), off = make_float2(-at, -at);
         float2 part[4] = {};
+        // A masked key's weight has to be zero, which the polynomial's is not.
+        auto weights = [&](auto every) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t p[32];
+          for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c) {
+              uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float2 x = make_float2(s[h * 2 + c][2 * i], s[h * 2 + c][2 * i + 1]);
-              x = ffma2(x, mul, off);
-              x.x = exp2_fast(x.x);
-              x.y = exp2_fast(x.y);
-              part[i & 3] = fadd2(part[i & 3], x);
-              p[c * 16 + i] = pack2<F16>(x.x, x.y);
+              for (int i = 0; i < 16; ++i) {
+                float2 x = make_float2(s[h * 2 + c][2 * i], s[h * 2 + c][2 * i + 1]);
+                x = ffma2(x, mul, off);
+                if (i % decltype(every)::value + 1 == decltype(every)::value) {
+                  x = exp2_poly(x);
+                } else {
+                  x.x = exp2_fast(x.x);
+                  x.y = exp2_fast(x.y);
+                }
+                part[i & 3] = fadd2(part[i & 3], x);
+                p[i] = pack2<F16>(x.x, x.y);
+              }
+              tc::tmem_st16(s_at + h * 32 + c * 16, p);
             }
-          tc::tmem_st32(s_at + h * 32, p);
-        }
-        tc::tmem_st_wait();
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->p_full[tile]);
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B->p_full[tile][h]);
+          }
+        };
+        if (edge)
+          weights(std::integral_constant<int, 64>{});   // none
+        else
+          weights(std::integral_constant<int, POLY_EVERY>{});
         part[0] = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
         sum += part[0].x + part[0].y;
       }
       if (!ok) break;
-      const int64_t at = (U.q0 + tok) * A.Hq + head;
-      uint16_t* out = A.out + at * A.Dv;
-      if (U.tiles[tile] == 0) {
-        if (real) {
-          for (int d = 0; d < A.Dv; d += 8)
-            *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
-          if (A.lse) A.lse[at] = -INFINITY;
-        }
-        continue;
+      const int64_t at = (int64_t)(U.q0 + tok) * A.Hq + head;
+      // The four rows whose pieces this lane stores: four lanes side by side
+      // exchange 16-byte pieces, so a store covers 64 bytes of eight rows and not
+      // 16 bytes of 32.
+      uint16_t* out[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (row & ~3) + i, t = first + (r >> A.pack_shift);
+        const int h = U.head0 + (r & ((1 << A.pack_shift) - 1));
+        out[i] = t < U.n ? A.out + ((int64_t)(U.q0 + t) * A.Hq + h) * A.Dv + (lane & 3) * 8
+                         : nullptr;
       }
-      if (!wait_phase(&B->o_full[tile], o_phase, abort_f, A.err)) break;
-      o_phase ^= 1u;
-      tc::tc_fence_after();
+      bool odd = false;
+      if (U.tiles[tile] > 0) {
+        if (!wait_phase(&B->o_full[tile], o_phase, abort_f, A.err)) break;
+        o_phase ^= 1u;
+        tc::tc_fence_after();
+        odd = *const_cast<volatile int*>(&B->odd[U.count & 15]) == U.count;
+      }
       // A row that saw no key (or only keys of score -infinity) is zero.
       const bool none = sum == 0.f || limit < 0;
       const float inv = none ? 0.f : 1.f / sum;
-      const bool odd = *const_cast<volatile int*>(&B->odd[walk.count & 15]) == walk.count;
 #pragma unroll
       for (int c = 0; c < DVP / 32; ++c) {
         float o[32];
-        tc::tmem_ld32(o_at + c * 32, o);
-        tc::tmem_ld_wait();
-        tc::hold_regs(o);
-        if (odd)
-          add_odd<F16>(A, A.v + U.k0 * A.v_tok + head / A.g * A.v_head, U.whole * TILE, limit,
-                       c * 32, o);
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          uint4 w;
-          w.x = pack2<F16>(o[i] * inv, o[i + 1] * inv);
-          w.y = pack2<F16>(o[i + 2] * inv, o[i + 3] * inv);
-          w.z = pack2<F16>(o[i + 4] * inv, o[i + 5] * inv);
-          w.w = pack2<F16>(o[i + 6] * inv, o[i + 7] * inv);
-          if (none) w = make_uint4(0, 0, 0, 0);
-          if (real && c * 32 + i < A.Dv) *reinterpret_cast<uint4*>(out + c * 32 + i) = w;
+        if (U.tiles[tile] > 0) {
+          tc::tmem_ld32(o_at + c * 32, o);
+          tc::tmem_ld_wait();
+          tc::hold_regs(o);
+          if (odd)
+            add_odd<F16>(A, A.v + U.k0 * A.v_tok + head / A.g * A.v_head, U.whole * TILE, limit,
+                         c * 32, o);
         }
+        uint4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i].x = pack2<F16>(o[8 * i] * inv, o[8 * i + 1] * inv);
+          w[i].y = pack2<F16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
+          w[i].z = pack2<F16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
+          w[i].w = pack2<F16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
+          if (none) w[i] = make_uint4(0, 0, 0, 0);
+        }
+        swap_pieces(w[0], w[1], lane & 1, 1);
+        swap_pieces(w[2], w[3], lane & 1, 1);
+        swap_pieces(w[0], w[2], lane & 2, 2);
+        swap_pieces(w[1], w[3], lane & 2, 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (out[i] && c * 32 + (lane & 3) * 8 < A.Dv)
+            *reinterpret_cast<uint4*>(out[i] + c * 32) = w[i];
       }
       tc::tc_fence_before();
       if (real && A.lse) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
@@ -400,19 +470,18 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           }
         }
       };
-      auto product = [&](int i, int at, bool first) {
+      // O += P V for one half of the tile's keys.
+      auto product = [&](int i, int at, int half, bool first) {
         uint32_t acc = first ? 0 : 1;
+        int sl = at + (S::VC == 2 ? half : 0);
+        if (sl >= S::SLOTS) sl -= S::SLOTS;
+        const uint64_t b = tc::sw128_desc_mn(r_at + sl * SLOT, S::VKEYS * 128) +
+                           (S::VC == 2 ? 0 : half * 4 * (2048 >> 4));
 #pragma unroll
-        for (int c = 0; c < S::VC; ++c) {
-          int sl = at + c;
-          if (sl >= S::SLOTS) sl -= S::SLOTS;
-          const uint64_t b = tc::sw128_desc_mn(r_at + sl * SLOT, S::VKEYS * 128);
-#pragma unroll
-          for (int k = 0; k < S::VKEYS / 16; ++k) {
-            tc::umma_ts(tmem + 256 + i * TILE, tmem + i * TILE + (c * (S::VKEYS / 16) + k) * 8,
-                        b + k * (2048 >> 4), ID_O, acc);
-            acc = 1;
-          }
+        for (int k = 0; k < 4; ++k) {
+          tc::umma_ts(tmem + 256 + i * TILE, tmem + i * TILE + (half * 4 + k) * 8,
+                      b + k * (2048 >> 4), ID_O, acc);
+          acc = 1;
         }
       };
       auto step = [&](int slots) {          // past the ring's current tile
@@ -424,7 +493,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         }
       };
       Unit U;
-      for (Walk walk(A); ok && walk.next(U);) {
+      for (Walk walk(B, A.err); ok && walk.next<false>(U);) {
         const int steps = max(U.tiles[0], U.tiles[1]);
         if (steps == 0) continue;
         if (!need(&B->full[entry], phase)) break;
@@ -448,10 +517,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           bool keys = false;
           for (int i = 0; i < 2; ++i) {
             if (j >= U.tiles[i]) continue;
-            if (!need(&B->p_full[i], p_phase[i])) break;
+            if (!need(&B->p_full[i][0], p_phase[i])) break;
+            tc::tc_fence_after();
+            product(i, v_slot, 0, j == 0);
+            if (!need(&B->p_full[i][1], p_phase[i])) break;
             p_phase[i] ^= 1u;
             tc::tc_fence_after();
-            product(i, v_slot, j == 0);
+            product(i, v_slot, 1, false);
             if (j + 1 == U.tiles[i]) {
               tc::umma_commit(&B->o_full[i]);
               continue;
@@ -506,7 +578,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         if (++entry == ENTRIES) entry = 0;
       };
       Unit U;
-      for (Walk walk(A); ok && walk.next(U);) {
+      for (Walk walk(B, A.err); ok && walk.next<false>(U);) {
         const int steps = max(U.tiles[0], U.tiles[1]);
         const int hk = U.head0 / A.g, span = TILE >> A.pack_shift;
         auto queries = [&](int i) {
@@ -517,12 +589,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)(S::KC * SLOT));
           for (int c = 0; c < S::KC; ++c)
             tma_load_4d(qs + (i * S::KC + c) * SLOT, &tq, c * 64, U.head0,
-                        (int)U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
+                        U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
         };
         for (int j = 0; j < steps && ok; ++j) {
           if (j == 0) queries(0);
           if (!ok || !begin(S::KC)) break;
-          const int key0 = (int)U.k0 + j * TILE;
+          const int key0 = U.k0 + j * TILE;
           for (int c = 0; c < S::KC; ++c)
             tma_load_4d(place(), &tk, c * 64, hk, key0, 0, &B->full[entry], keep);
           end();
@@ -549,7 +621,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         }
       }
     }
-    if (warp >= CLEAN_WARP) {
+    if (warp == CLEAN_WARP) {
       // ------------------------------------------------------------ odd elements
       int entry = 0, slot = 0;
       uint32_t phase = 0;
@@ -563,12 +635,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       };
       bool ok = true;
       Unit U;
-      for (Walk walk(A); ok && walk.next(U);) {
+      for (Walk walk(B, A.err); ok && walk.next<true>(U);) {
         const int steps = max(U.tiles[0], U.tiles[1]);
         for (int j = 0; j < steps; ++j) {
           step(S::KC);
-          // Every tile is waited for, so that these warps stay within one
-          // round of the ring of the others.
+          // Every tile is waited for, so that this warp stays within one round
+          // of the ring of the others.
           ok = wait_phase(&B->full[entry], phase, abort_f, A.err);
           if (!ok) break;
           if (j >= U.whole) {
@@ -576,20 +648,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             for (int c = 0; c < S::VC; ++c) {
               int sl = slot + c;
               if (sl >= S::SLOTS) sl -= S::SLOTS;
-              uint4* at = reinterpret_cast<uint4*>(ring + sl * SLOT) + (warp - CLEAN_WARP) * 32 +
-                          lane;
+              uint4* at = reinterpret_cast<uint4*>(ring + sl * SLOT) + lane;
 #pragma unroll 8
-              for (int i = 0; i < SLOT / 1024; ++i) {
-                uint4 x = at[i * 64];
+              for (int i = 0; i < SLOT / 512; ++i) {
+                uint4 x = at[i * 32];
                 if (has_odd<F16>(x)) {
                   clear_odd<F16>(x);
-                  at[i * 64] = x;
+                  at[i * 32] = x;
                   any = true;
                 }
               }
             }
             if (any) {
-              B->odd[walk.count & 15] = walk.count;
+              B->odd[U.count & 15] = U.count;
               fence_proxy_async();
             }
           }
@@ -598,6 +669,66 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           step(S::VC);
         }
       }
+    } else if (warp == LIST_WARP) {
+      // ------------------------------------------------------------ list of units
+      const int groups = A.Hq >> A.pack_shift, span = TILE >> A.pack_shift;
+      int slot = 0, round = 0, count = 0, held = -1;
+      uint32_t phase = 1;
+      int want = blockIdx.x, before = 0;     // this CTA's next unit on the list; units before here
+      int64_t first = 0, end = 0;
+      bool ok = true;
+      auto tell = [&](const Unit& U) {
+        ok = wait_phase(&B->unit_empty[slot], phase, abort_f, A.err);
+        if (!ok) return;
+        if (lane == 0) {
+          B->unit[slot] = U;
+          mbar_arrive(&B->unit_full[slot]);
+        }
+        if (++slot == UNITS) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      };
+      for (int block = A.blocks - 1; block >= 0 && ok; --block) {
+        const int t0 = (block * 2 * TILE) >> A.pack_shift;
+        for (int b0 = 0; b0 < A.B && ok; b0 += 32) {
+          if (held != b0) {
+            held = b0;
+            first = end = 0;
+            if (b0 + lane < A.B) request_rows(A.cu_q, b0 + lane, A.total_q, first, end);
+          }
+          const unsigned late = __ballot_sync(0xffffffffu, end - first > t0);
+          const int limit = before + __popc(late) * groups;
+          while (ok && want < limit) {
+            const int at = (want - before) / groups;
+            const int from = __fns(late, 0, at + 1);
+            Unit U;
+            U.q0 = __shfl_sync(0xffffffffu, (int)first, from);
+            U.n = __shfl_sync(0xffffffffu, (int)(end - first), from);
+            int64_t k0, k1;
+            request_rows(A.cu_k, b0 + from, A.total_k, k0, k1);
+            U.k0 = (int)k0;
+            U.m = (int)(k1 - k0);
+            U.head0 = (want - before - at * groups) << A.pack_shift;
+            U.t0 = t0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int top = t0 + i * span, last = min(U.n, top + span) - 1;
+              const int keys = top < U.n ? min(max(last + U.m - U.n + 1, 0), U.m) : 0;
+              U.tiles[i] = (keys + TILE - 1) / TILE;
+            }
+            U.whole = max(t0 + U.m - U.n + 1, 0) / TILE;
+            U.count = count++;
+            tell(U);
+            ++round;
+            want = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+          }
+          before = limit;
+        }
+      }
+      Unit last = {};
+      last.count = -1;
+      if (ok) tell(last);
     }
     __syncwarp();
   }
