@@ -44,6 +44,12 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
   }
 }
 
+// The same for a whole warp in step: all of its lanes go on or none.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_f,
+                                          uint32_t* err) {
+  return __all_sync(0xffffffffu, wait_phase(bar, parity, abort_f, err)) != 0;
+}
+
 // Wait on the error path for copies in flight: short limit, nothing recorded.
 __device__ __forceinline__ void drain_phase(uint64_t* bar, uint32_t parity) {
   const long long t0 = now_ns();

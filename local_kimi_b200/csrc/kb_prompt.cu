@@ -19,7 +19,7 @@
 //     rows x 64 elements a slot) and values (64 or 128 rows) in use order, by
 //     tensor copies in the 128-byte swizzle; a barrier pair per key or value
 //     tile, not per slot.
-//   warp 8: one thread issues the MMAs.  S = Q K^T (both from shared memory)
+//   warp 8: issues the MMAs.  S = Q K^T (both from shared memory)
 //     into tensor memory, O += P V with P from tensor memory (it replaces the
 //     S it came from) and V from shared memory, rows of V as they lie
 //     (MN-major).  Order A, B, A, B: while the softmax of one tile runs, the
@@ -125,7 +125,9 @@ struct Walk {
   // The next unit; false at the end or on abort.
   template <bool WARP>
   __device__ __forceinline__ bool next(Unit& U) {
-    if (!wait_phase(&B->unit_full[slot], phase, &B->abort_flag, err)) return false;
+    if (!(WARP ? warp_wait(&B->unit_full[slot], phase, &B->abort_flag, err)
+               : wait_phase(&B->unit_full[slot], phase, &B->abort_flag, err)))
+      return false;
     U = B->unit[slot];
     if (WARP) __syncwarp();
     if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&B->unit_empty[slot]);
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       float top = -INFINITY, sum = 0.f;                     // in log2 units
       bool ok = true;
       for (int j = 0; j < U.tiles[tile]; ++j) {
-        if (!wait_phase(&B->s_full[tile], s_phase, abort_f, A.err)) {
+        if (!warp_wait(&B->s_full[tile], s_phase, abort_f, A.err)) {
           ok = false;
           break;
         }
@@ -398,7 +400,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       }
       bool odd = false;
       if (U.tiles[tile] > 0) {
-        if (!wait_phase(&B->o_full[tile], o_phase, abort_f, A.err)) break;
+        if (!warp_wait(&B->o_full[tile], o_phase, abort_f, A.err)) break;
         o_phase ^= 1u;
         tc::tc_fence_after();
         odd = *const_cast<volatile int*>(&B->odd[U.count & 15]) == U.count;
@@ -441,18 +443,22 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == MMA_WARP && lane == 0) {
+    if (warp == MMA_WARP) {
       // --------------------------------------------------------------- MMA issue
       constexpr uint32_t TYPE = F16 ? 0u : 1u;
       constexpr uint32_t COMMON = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((TILE >> 4) << 24);
       constexpr uint32_t ID_S = COMMON | ((TILE >> 3) << 17);
       constexpr uint32_t ID_O = COMMON | (1u << 16) | ((DVP >> 3) << 17);    // V: MN-major
+      // The warp goes through this in step (what it reads from memory is made
+      // uniform for the compiler), one lane issues.
+      const uint32_t one = tc::elect_one();
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_at = smem_addr(qs), r_at = smem_addr(ring);
       int entry = 0, slot = 0;            // next tile of the ring and its first slot
       uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
       bool ok = true;
       auto need = [&](uint64_t* bar, uint32_t ph) {
-        ok = ok && wait_phase(bar, ph, abort_f, A.err);
+        ok = ok && warp_wait(bar, ph, abort_f, A.err);
         return ok;
       };
       auto score = [&](int i, int at) {
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           const uint64_t b = tc::sw128_desc(r_at + sl * SLOT);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            tc::umma(tmem + i * TILE, a + k * 2, b + k * 2, ID_S, acc);
+            tc::umma_one(one, tm + i * TILE, a + k * 2, b + k * 2, ID_S, acc);
             acc = 1;
           }
         }
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                            (S::VC == 2 ? 0 : half * 4 * (2048 >> 4));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          tc::umma_ts(tmem + 256 + i * TILE, tmem + i * TILE + (half * 4 + k) * 8,
+          tc::umma_ts_one(one, tm + 256 + i * TILE, tm + i * TILE + (half * 4 + k) * 8,
                       b + k * (2048 >> 4), ID_O, acc);
           acc = 1;
         }
@@ -493,21 +499,23 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         }
       };
       Unit U;
-      for (Walk walk(B, A.err); ok && walk.next<false>(U);) {
-        const int steps = max(U.tiles[0], U.tiles[1]);
+      for (Walk walk(B, A.err); ok && walk.next<true>(U);) {
+        const int tiles[2] = {__shfl_sync(0xffffffffu, U.tiles[0], 0),
+                              __shfl_sync(0xffffffffu, U.tiles[1], 0)};
+        const int steps = max(tiles[0], tiles[1]);
         if (steps == 0) continue;
         if (!need(&B->full[entry], phase)) break;
         for (int i = 0; i < 2; ++i) {
-          if (U.tiles[i] == 0) continue;
+          if (tiles[i] == 0) continue;
           if (!need(&B->q_full[i], q_phase[i])) break;
           q_phase[i] ^= 1u;
           tc::tc_fence_after();
           score(i, slot);
-          tc::umma_commit(&B->s_full[i]);
-          if (U.tiles[i] == 1) tc::umma_commit(&B->q_empty[i]);
+          tc::umma_commit_one(one, &B->s_full[i]);
+          if (tiles[i] == 1) tc::umma_commit_one(one, &B->q_empty[i]);
         }
         if (!ok) break;
-        tc::umma_commit(&B->empty[entry]);
+        tc::umma_commit_one(one, &B->empty[entry]);
         step(S::KC);
         for (int j = 0; j < steps; ++j) {
           // This step's values, and the next step's keys behind them.
@@ -516,7 +524,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           step(S::VC);
           bool keys = false;
           for (int i = 0; i < 2; ++i) {
-            if (j >= U.tiles[i]) continue;
+            if (j >= tiles[i]) continue;
             if (!need(&B->p_full[i][0], p_phase[i])) break;
             tc::tc_fence_after();
             product(i, v_slot, 0, j == 0);
@@ -524,26 +532,26 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             p_phase[i] ^= 1u;
             tc::tc_fence_after();
             product(i, v_slot, 1, false);
-            if (j + 1 == U.tiles[i]) {
-              tc::umma_commit(&B->o_full[i]);
+            if (j + 1 == tiles[i]) {
+              tc::umma_commit_one(one, &B->o_full[i]);
               continue;
             }
             if (!keys && !need(&B->full[entry], phase)) break;
             keys = true;
             score(i, slot);
-            tc::umma_commit(&B->s_full[i]);
-            if (j + 2 == U.tiles[i]) tc::umma_commit(&B->q_empty[i]);
+            tc::umma_commit_one(one, &B->s_full[i]);
+            if (j + 2 == tiles[i]) tc::umma_commit_one(one, &B->q_empty[i]);
           }
           if (!ok) break;
-          tc::umma_commit(&B->empty[v_entry]);
+          tc::umma_commit_one(one, &B->empty[v_entry]);
           if (j + 1 < steps) {
-            tc::umma_commit(&B->empty[entry]);
+            tc::umma_commit_one(one, &B->empty[entry]);
             step(S::KC);
           }
         }
       }
       // Every product issued is done before the tensor memory goes.
-      tc::umma_commit(&B->drain);
+      tc::umma_commit_one(one, &B->drain);
       drain_phase(&B->drain, 0);
     } else if (warp == COPY_WARP && lane == 0) {
       // ------------------------------------------------------------------ copies
@@ -641,7 +649,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           step(S::KC);
           // Every tile is waited for, so that this warp stays within one round
           // of the ring of the others.
-          ok = wait_phase(&B->full[entry], phase, abort_f, A.err);
+          ok = warp_wait(&B->full[entry], phase, abort_f, A.err);
           if (!ok) break;
           if (j >= U.whole) {
             bool any = false;
@@ -678,7 +686,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       int64_t first = 0, end = 0;
       bool ok = true;
       auto tell = [&](const Unit& U) {
-        ok = wait_phase(&B->unit_empty[slot], phase, abort_f, A.err);
+        ok = warp_wait(&B->unit_empty[slot], phase, abort_f, A.err);
         if (!ok) return;
         if (lane == 0) {
           B->unit[slot] = U;

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       pos = until;
       if (t1 <= t0) continue;                           // the run ends in the unit's start
       const int sb = seg & 1;
-      if (seg >= 2 && !wait_phase(&B->q_empty[sb], ((seg >> 1) - 1) & 1, abort_f, A.err)) break;
+      if (seg >= 2 && !warp_wait(&B->q_empty[sb], ((seg >> 1) - 1) & 1, abort_f, A.err)) break;
       const int row0 = rb * S::RB;
       const int rows = (int)min((int64_t)S::RB, (int64_t)R.n * A.g - row0);
       if (lane == 0) {
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       int64_t have = -1;         // first table entry held by lane 0
       int ids = -1;
       for (int64_t tile = t0; tile < t1; ++tile) {
-        if (again && !wait_phase(&B->empty[stage], phase ^ 1u, abort_f, A.err)) {
+        if (again && !warp_wait(&B->empty[stage], phase ^ 1u, abort_f, A.err)) {
           ok = false;
           break;
         }
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       }
       ++seg;
     }
-    if (seg < 2 || wait_phase(&B->q_empty[seg & 1], ((seg >> 1) - 1) & 1, abort_f, A.err)) {
+    if (seg < 2 || warp_wait(&B->q_empty[seg & 1], ((seg >> 1) - 1) & 1, abort_f, A.err)) {
       if (lane == 0) {
         B->seg[seg & 1].end = 1;
         mbar_arrive(&B->q_full[seg & 1]);
@@ -401,13 +401,13 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
   auto meet = [&](uint64_t* bar, uint32_t& ph) {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
-    const bool ok = wait_phase(bar, ph, abort_f, A.err);
+    const bool ok = warp_wait(bar, ph, abort_f, A.err);
     ph ^= 1u;
     return ok;
   };
   for (;; ++seg) {
     const int sb = seg & 1;
-    if (!wait_phase(&B->q_full[sb], (seg >> 1) & 1, abort_f, A.err)) return;
+    if (!warp_wait(&B->q_full[sb], (seg >> 1) & 1, abort_f, A.err)) return;
     const Segment& G = B->seg[sb];     // the producer waits for q_empty to reuse it
     if (G.end) return;
     const int64_t ctx = G.ctx;
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (bool last = false; !last;) {
-      if (!wait_phase(&B->full[stage], phase, abort_f, A.err)) return;
+      if (!warp_wait(&B->full[stage], phase, abort_f, A.err)) return;
       last = B->last[stage] != 0;
       const uint64_t valid = B->valid[stage];
       const int64_t key0 = B->key0[stage];
