@@ -6,43 +6,44 @@
 // visible: j <= i + (Lk - Lq).  A row that sees no key gives 0 and lse -infinity.
 //
 // One persistent CTA per SM.  A unit is 256 rows of one request, two tiles A
-// and B of 128, against all the keys they see, 128 at a time.  The heads of a
+// and B of 128, against all the keys they see, 64 a step.  The heads of a
 // group that share keys lie side by side in the rows (row = token * pack +
 // head, pack the largest power of two in the group), so short prompts fill
 // tiles and keys are read once for them.  Units go out heaviest (latest rows)
 // first, there and back over the CTAs.
 //
-//   warp 11: the list of units.  It counts, 32 requests at a time, which have
-//     rows that late, and tells the other warps this CTA's units through a
-//     ring of four.
-//   warp 9: copies.  Q tiles, and a ring of 16 KB slots with the keys (128
-//     rows x 64 elements a slot) and values (64 or 128 rows) in use order, by
-//     tensor copies in the 128-byte swizzle; a barrier pair per key or value
-//     tile, not per slot.
-//   warp 8: issues the MMAs.  S = Q K^T (both from shared memory)
-//     into tensor memory, O += P V with P from tensor memory (it replaces the
-//     S it came from) and V from shared memory, rows of V as they lie
-//     (MN-major).  Order A, B, A, B: while the softmax of one tile runs, the
-//     tensor core works for the other.  P V of a tile is issued before the
-//     next S of the same tile, so S never overwrites a P still being read.
+//   warp 10: the list of units, and copies.  It counts, 32 requests at a time,
+//     which have rows that late, tells the other warps this CTA's units through
+//     a ring of four, and brings in Q tiles and a ring of stages with a step's
+//     keys and values (8 KB blocks of 64 rows x 64 elements), by tensor copies
+//     in the 128-byte swizzle; keys and values have barriers of their own,
+//     since keys are used two steps before the values beside them.
+//   warps 8 and 9: issue the MMAs of tiles A and B (one warp for both spent as
+//     long in its waits and commits as the tensor core in the products).
+//     S = Q K^T (both from shared memory) into tensor memory, O += P V with P
+//     from tensor memory (it replaces the S it came from) and V from shared
+//     memory, rows of V as they lie (MN-major).  Each tile has two S buffers,
+//     so S of step h + 2 is issued behind P V of step h, and the softmax finds
+//     its next scores waiting.  P V of a step is issued before the S that
+//     overwrites its P, by the same thread, and MMAs run in order.
 //   warps 0-3 and 4-7: softmax of tiles A and B, a row per thread: maximum,
 //     exponentials in base 2, row sum in fp32, and P rounded once to the
-//     inputs' type, handed over in two halves of 64 keys.  The running maximum
-//     only moves, and O is only rescaled, when a row's maximum rose by more
-//     than 2^8: weights stay within fp32 and the 16-bit types, and the final
-//     division makes up for the rest.
+//     inputs' type.  The running maximum only moves, and O is only rescaled,
+//     when a row's maximum rose by more than 2^8: weights stay within fp32
+//     and the 16-bit types, and the final division makes up for the rest.
 //
-// 512 columns of tensor memory: S A, S B, O A, O B.  MMAs are 2 (Dk + Dv) flops
-// a pair, 1024 to 1280 clocks a tile of 128 x 128 at 128 to 192 + 128 wide
-// heads; the exponentials at 16 a clock and SM are 1024 clocks a tile.  With
-// two tiles in turn the period is one tile's softmax plus its MMAs, so every
-// clock of the softmax counts: measured on the way, maximum 500 -> 250 clocks
-// with three-input maxima, exponentials 1650 with the special function unit
-// alone.  One in POLY_EVERY pairs is computed on the FMA pipes instead.
+// 512 columns of tensor memory: two S of 64 for A and for B, O A, O B.  Bound:
+// MMAs, 51 clocks each for S (128 x 64 x 16, both operands from shared
+// memory: the copies of A set the rate; 64 clocks at 128 x 128 x 16) and 64
+// for P V, which is 2644 clocks for 128 keys of A and B at 128-wide heads,
+// 3452 at 192 + 128.  With steps of 128 keys and one S a tile the MMAs are 2048
+// and 2560 clocks, but each waits for the softmax of its own tile in turn:
+// 3600 and 4430 measured.  The exponentials (16 a clock and SM) would take
+// 2048; one pair in POLY_EVERY goes to the FMA pipes.
 //
 // In the last tiles of a unit some rows do not see some keys, or the tile
 // reaches past the request's end into its neighbour.  A value there that is
-// infinite or not a number must not meet a zero weight: warp 10 zeroes such
+// infinite or not a number must not meet a zero weight: warp 11 zeroes such
 // elements in those tiles before the MMA reads them, and at the end the rows
 // that do see them take them from memory.
 #include <algorithm>
@@ -54,13 +55,14 @@
 namespace kb {
 namespace attn {
 
-constexpr int TILE = 128;                  // rows of a tile, keys of a step
-constexpr int SLOT = 16384;                // bytes of a ring slot
+constexpr int TILE = 128;                  // rows of a tile
+constexpr int STEP = 64;                   // keys of a step
+constexpr int BLOCK = STEP * 128;          // bytes of 64 rows x 64 elements
 constexpr int PROMPT_THREADS = 384;
-constexpr int MMA_WARP = 8, COPY_WARP = 9, CLEAN_WARP = 10, LIST_WARP = 11;
+constexpr int MMA_WARP = 8, COPY_WARP = 10, CLEAN_WARP = 11;   // MMA: and 9
 constexpr int UNITS = 4;                   // units told ahead
+constexpr int MAX_STAGES = 8;
 constexpr int POLY_EVERY = 4;              // one in so many pairs of exponentials on the FMA pipes
-constexpr int ENTRIES = 8;                 // key and value tiles with a barrier pair
 constexpr float RESCALE = 8.0f;            // log2 of the growth that moves the maximum
 
 struct PromptArgs {
@@ -79,34 +81,36 @@ struct PromptArgs {
 
 template <int DKP, int DVP>
 struct PromptShape {
-  static constexpr int KC = DKP / 64;                    // slots of a key tile
-  static constexpr int VC = DVP / 64;                    // ... of a value tile
-  static constexpr int VKEYS = TILE / VC;                // keys of a value slot
-  static constexpr int Q_BYTES = 2 * KC * SLOT;
+  static constexpr int KC = DKP / 64;                    // blocks of a step's keys
+  static constexpr int VC = DVP / 64;                    // ... and values
+  static constexpr int Q_TILE = 2 * KC * BLOCK;          // bytes of a Q tile (128 rows)
+  static constexpr int STAGE = (KC + VC) * BLOCK;
   static constexpr int FIXED = 1024 + 1024;              // alignment, barriers
-  static constexpr int FIT = (227 * 1024 - FIXED - Q_BYTES) / SLOT;
-  static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
-  static constexpr int SMEM = FIXED + Q_BYTES + SLOTS * SLOT;
-  static_assert(SLOTS >= KC + 2 * VC, "a key tile beside the value tile in use, and one to come");
+  static constexpr int FIT = (227 * 1024 - FIXED - 2 * Q_TILE) / STAGE;
+  static constexpr int STAGES = FIT > MAX_STAGES ? MAX_STAGES : FIT;
+  static constexpr int SMEM = FIXED + 2 * Q_TILE + STAGES * STAGE;
+  static_assert(STAGES >= 3, "keys two steps ahead of the values");
 };
 
-// A unit as warp 11 tells it to the others.
+// A unit as warp 10 tells it to the others.
 struct Unit {
   int q0, k0;               // first query and key of the request
   int n, m;                 // its queries and keys
   int head0;                // first head
   int t0;                   // first token of tile A
-  int tiles[2];             // key tiles that tiles A and B see
-  int whole;                // of them, those that every row of A and B sees whole
+  int steps[2];             // steps of keys that tiles A and B see
+  int whole;                // of them, those that every row of A sees whole
   int count;                // number of the unit in this CTA, -1: the end
 };
 
 struct PromptBars {
-  uint64_t full[ENTRIES], empty[ENTRIES];
-  uint64_t clean[ENTRIES];  // a value tile is there, without odd elements
+  uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES], v_full[MAX_STAGES], v_empty[MAX_STAGES];
+  uint64_t clean[MAX_STAGES];   // a step's values are there, without odd elements
   uint64_t unit_full[UNITS], unit_empty[UNITS];
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2], p_full[2][2], o_full[2];
+  uint64_t s_full[2][2], p_full[2][2];   // of a tile's two buffers
+  uint64_t o_done[2];           // a step's P V is in O
+  uint64_t o_full[2];           // ... and it was the unit's last
   uint64_t drain;
   Unit unit[UNITS];
   int odd[16];              // units that had odd elements, by their number's last four bits
@@ -115,7 +119,7 @@ struct PromptBars {
 };
 static_assert(sizeof(PromptBars) <= 1024, "barrier block");
 
-// A warp's (or single thread's) way through the CTA's units.
+// A warp's way through the CTA's units.
 struct Walk {
   PromptBars* B;
   uint32_t* err;
@@ -123,14 +127,11 @@ struct Walk {
   uint32_t phase;
   __device__ __forceinline__ Walk(PromptBars* b, uint32_t* e) : B(b), err(e), slot(0), phase(0) {}
   // The next unit; false at the end or on abort.
-  template <bool WARP>
   __device__ __forceinline__ bool next(Unit& U) {
-    if (!(WARP ? warp_wait(&B->unit_full[slot], phase, &B->abort_flag, err)
-               : wait_phase(&B->unit_full[slot], phase, &B->abort_flag, err)))
-      return false;
+    if (!warp_wait(&B->unit_full[slot], phase, &B->abort_flag, err)) return false;
     U = B->unit[slot];
-    if (WARP) __syncwarp();
-    if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&B->unit_empty[slot]);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&B->unit_empty[slot]);
     if (++slot == UNITS) {
       slot = 0;
       phase ^= 1u;
@@ -138,7 +139,7 @@ struct Walk {
     return U.count >= 0;
   }
 };
-constexpr int WALKERS = 8 + 3;               // softmax warps, MMA, copies, cleaning
+constexpr int WALKERS = 8 + 3;               // softmax warps, two of MMAs, cleaning
 
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   uint64_t d;
@@ -218,32 +219,36 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   uint8_t* smem =
       smem_raw + ((1024u - (static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw)) & 1023u)) &
                   1023u);
-  uint8_t* qs = smem;                           // [2][KC] slots
-  uint8_t* ring = qs + S::Q_BYTES;              // [SLOTS]
-  PromptBars* B = reinterpret_cast<PromptBars*>(ring + S::SLOTS * SLOT);
+  uint8_t* qs = smem;                           // [2] tiles
+  uint8_t* ring = qs + 2 * S::Q_TILE;           // [STAGES] keys, values
+  PromptBars* B = reinterpret_cast<PromptBars*>(ring + S::STAGES * S::STAGE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_f = &B->abort_flag;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < ENTRIES; ++i) {
-      mbar_init(&B->full[i], 1);
-      mbar_init(&B->empty[i], 1);
+    for (int i = 0; i < S::STAGES; ++i) {
+      mbar_init(&B->k_full[i], 1);
+      mbar_init(&B->k_empty[i], 2);
+      mbar_init(&B->v_full[i], 1);
+      mbar_init(&B->v_empty[i], 2);
+      mbar_init(&B->clean[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B->q_full[i], 1);
       mbar_init(&B->q_empty[i], 1);
-      mbar_init(&B->s_full[i], 1);
-      mbar_init(&B->p_full[i][0], 4);
-      mbar_init(&B->p_full[i][1], 4);
+      mbar_init(&B->o_done[i], 1);
       mbar_init(&B->o_full[i], 1);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&B->s_full[i][j], 1);
+        mbar_init(&B->p_full[i][j], 4);
+      }
     }
-    for (int i = 0; i < ENTRIES; ++i) mbar_init(&B->clean[i], 1);
     for (int i = 0; i < UNITS; ++i) {
       mbar_init(&B->unit_full[i], 1);
       mbar_init(&B->unit_empty[i], WALKERS);
     }
     for (int i = 0; i < 16; ++i) B->odd[i] = -1;
-    mbar_init(&B->drain, 1);
+    mbar_init(&B->drain, 2);
     B->abort_flag = 0;
     mbar_fence_init();
     prefetch_map(&tq);
@@ -278,13 +283,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     const int tile = warp >> 2;
     const int row = threadIdx.x & (TILE - 1);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + tile * TILE;
+    const uint32_t s_at = tmem + lanes + tile * 2 * STEP;
     const uint32_t o_at = tmem + lanes + 256 + tile * TILE;
     const float scale2 = A.scale2;
     const int span = TILE >> A.pack_shift;
-    uint32_t s_phase = 0, o_phase = 0;
+    int buf = 0;                          // the next step's S buffer
+    uint32_t s_phase = 0, o_phase = 1;    // o_phase: of the last step handed over
+    uint32_t end_phase = 0;
     Unit U;
-    for (Walk walk(B, A.err); walk.next<true>(U);) {
+    for (Walk walk(B, A.err); walk.next(U);) {
       const int first = U.t0 + tile * span;
       if (first >= U.n) continue;
       const int tok = first + (row >> A.pack_shift);
@@ -294,45 +301,53 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       const int clear = first + U.m - U.n;                  // ... and the tile's first row
       float top = -INFINITY, sum = 0.f;                     // in log2 units
       bool ok = true;
-      for (int j = 0; j < U.tiles[tile]; ++j) {
-        if (!warp_wait(&B->s_full[tile], s_phase, abort_f, A.err)) {
+      const int steps = U.steps[tile];
+      for (int j = 0; j < steps; ++j) {
+        if (!warp_wait(&B->s_full[tile][buf], s_phase, abort_f, A.err)) {
           ok = false;
           break;
         }
-        s_phase ^= 1u;
         tc::tc_fence_after();
-        float s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_at + c * 32, s[c]);
+        const uint32_t here = s_at + buf * STEP;
+        float s[2][32];
+        tc::tmem_ld32(here, s[0]);
+        tc::tmem_ld32(here + 32, s[1]);
         tc::tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc::hold_regs(s[c]);
-        const bool edge = j * TILE + TILE - 1 > clear;     // keys that some rows do not see
+        tc::hold_regs(s[0]);
+        tc::hold_regs(s[1]);
+        const bool edge = j * STEP + STEP - 1 > clear;     // keys that some rows do not see
         if (edge) {
-          const int last = limit - j * TILE;
+          const int last = limit - j * STEP;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i > last) s[c][i] = -INFINITY;
         }
-        float mx[4] = {s[0][0], s[1][0], s[2][0], s[3][0]};
+        float mx[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
 #pragma unroll
-        for (int i = 1; i < 31; i += 2)
+        for (int i = 2; i < 30; i += 4)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], s[c][i], s[c][i + 1]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], s[c][31]);
-        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-        // S being there means that every MMA issued before it is done, the
-        // last P V of this tile among them: O may be touched.
-        const bool grow = mine > top + RESCALE || top == -INFINITY;
-        if (__any_sync(0xffffffffu, grow && j > 0)) {
-          const float now = grow ? fmaxf(mine, top) : top;
+          for (int c = 0; c < 4; ++c)
+            mx[c] = max3(mx[c], s[c >> 1][i + (c & 1) * 2], s[c >> 1][i + (c & 1) * 2 + 1]);
+        mx[0] = max3(mx[0], s[0][30], s[0][31]);
+        mx[2] = max3(mx[2], s[1][30], s[1][31]);
+        const float mine = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale2;
+        if (j == 0) {
+          top = mine;
+        } else if (__any_sync(0xffffffffu, mine > top + RESCALE)) {
+          // O may be touched once P V of the last step is done (that of the step
+          // before was issued ahead of this step's S, so it is).
+          if (!warp_wait(&B->o_done[tile], o_phase, abort_f, A.err)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const float now = mine > top + RESCALE ? mine : top;
           const float fix = now == top ? 1.f : exp2_fast(top - now);
           sum *= fix;
           top = now;
-          // 16 columns at a time: the 128 scores stay in registers beside them.
+          // 16 columns at a time: the scores stay in registers beside them.
 #pragma unroll 1
           for (int c = 0; c < DVP / 16; ++c) {
             uint32_t o[16];
@@ -344,8 +359,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             tc::tmem_st16(o_at + c * 16, o);
           }
           tc::tmem_st_wait();
-        } else if (j == 0) {
-          top = mine;
         }
         const float at = top == -INFINITY ? 0.f : top;
         const float2 mul = make_float2(scale2, scale2), off = make_float2(-at, -at);
@@ -353,37 +366,37 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         // A masked key's weight has to be zero, which the polynomial's is not.
         auto weights = [&](auto every) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t p[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float2 x = make_float2(s[h * 2 + c][2 * i], s[h * 2 + c][2 * i + 1]);
-                x = ffma2(x, mul, off);
-                if (i % decltype(every)::value + 1 == decltype(every)::value) {
-                  x = exp2_poly(x);
-                } else {
-                  x.x = exp2_fast(x.x);
-                  x.y = exp2_fast(x.y);
-                }
-                part[i & 3] = fadd2(part[i & 3], x);
-                p[i] = pack2<F16>(x.x, x.y);
+            for (int i = 0; i < 16; ++i) {
+              float2 x = make_float2(s[c][2 * i], s[c][2 * i + 1]);
+              x = ffma2(x, mul, off);
+              if (i % decltype(every)::value + 1 == decltype(every)::value) {
+                x = exp2_poly(x);
+              } else {
+                x.x = exp2_fast(x.x);
+                x.y = exp2_fast(x.y);
               }
-              tc::tmem_st16(s_at + h * 32 + c * 16, p);
+              part[i & 3] = fadd2(part[i & 3], x);
+              p[i] = pack2<F16>(x.x, x.y);
             }
-            tc::tmem_st_wait();
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B->p_full[tile][h]);
+            tc::tmem_st16(here + c * 16, p);
           }
         };
         if (edge)
           weights(std::integral_constant<int, 64>{});   // none
         else
           weights(std::integral_constant<int, POLY_EVERY>{});
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->p_full[tile][buf]);
         part[0] = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
         sum += part[0].x + part[0].y;
+        o_phase ^= 1u;
+        if (buf) s_phase ^= 1u;
+        buf ^= 1;
       }
       if (!ok) break;
       const int64_t at = (int64_t)(U.q0 + tok) * A.Hq + head;
@@ -399,9 +412,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                          : nullptr;
       }
       bool odd = false;
-      if (U.tiles[tile] > 0) {
-        if (!warp_wait(&B->o_full[tile], o_phase, abort_f, A.err)) break;
-        o_phase ^= 1u;
+      if (steps > 0) {
+        if (!warp_wait(&B->o_full[tile], end_phase, abort_f, A.err)) break;
+        end_phase ^= 1u;
         tc::tc_fence_after();
         odd = *const_cast<volatile int*>(&B->odd[U.count & 15]) == U.count;
       }
@@ -411,12 +424,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 #pragma unroll
       for (int c = 0; c < DVP / 32; ++c) {
         float o[32];
-        if (U.tiles[tile] > 0) {
+        if (steps > 0) {
           tc::tmem_ld32(o_at + c * 32, o);
           tc::tmem_ld_wait();
           tc::hold_regs(o);
           if (odd)
-            add_odd<F16>(A, A.v + U.k0 * A.v_tok + head / A.g * A.v_head, U.whole * TILE, limit,
+            add_odd<F16>(A, A.v + U.k0 * A.v_tok + head / A.g * A.v_head, U.whole * STEP, limit,
                          c * 32, o);
         }
         uint4 w[4];
@@ -443,258 +456,172 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == MMA_WARP) {
+    if (warp < COPY_WARP) {
       // --------------------------------------------------------------- MMA issue
       constexpr uint32_t TYPE = F16 ? 0u : 1u;
       constexpr uint32_t COMMON = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((TILE >> 4) << 24);
-      constexpr uint32_t ID_S = COMMON | ((TILE >> 3) << 17);
+      constexpr uint32_t ID_S = COMMON | ((STEP >> 3) << 17);
       constexpr uint32_t ID_O = COMMON | (1u << 16) | ((DVP >> 3) << 17);    // V: MN-major
       // The warp goes through this in step (what it reads from memory is made
       // uniform for the compiler), one lane issues.
       const uint32_t one = tc::elect_one();
+      const int tile = __shfl_sync(0xffffffffu, warp - MMA_WARP, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t q_at = smem_addr(qs), r_at = smem_addr(ring);
-      int entry = 0, slot = 0;            // next tile of the ring and its first slot
-      uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      const uint32_t q_at = smem_addr(qs) + tile * S::Q_TILE, r_at = smem_addr(ring);
+      const uint32_t s_to = tm + tile * 2 * STEP, o_to = tm + 256 + tile * TILE;
+      int k_st = 0, v_st = 0;             // stages of the next keys and values
+      uint32_t k_ph = 0, v_ph = 0, q_phase = 0, p_phase = 0;
+      int s_buf = 0, p_buf = 0;           // S buffers of the next scores and weights
       bool ok = true;
       auto need = [&](uint64_t* bar, uint32_t ph) {
-        ok = ok && warp_wait(bar, ph, abort_f, A.err);
+        ok = warp_wait(bar, ph, abort_f, A.err);
         return ok;
       };
-      auto score = [&](int i, int at) {
+      // S of the tile's next step, from the keys of stage k_st.
+      auto score = [&]() {
+        const uint32_t d = s_to + s_buf * STEP;
         uint32_t acc = 0;
 #pragma unroll
         for (int c = 0; c < S::KC; ++c) {
-          int sl = at + c;
-          if (sl >= S::SLOTS) sl -= S::SLOTS;
-          const uint64_t a = tc::sw128_desc(q_at + (i * S::KC + c) * SLOT);
-          const uint64_t b = tc::sw128_desc(r_at + sl * SLOT);
+          const uint64_t a = tc::sw128_desc(q_at + c * 2 * BLOCK);
+          const uint64_t b = tc::sw128_desc(r_at + k_st * S::STAGE + c * BLOCK);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            tc::umma_one(one, tm + i * TILE, a + k * 2, b + k * 2, ID_S, acc);
+            tc::umma_one(one, d, a + k * 2, b + k * 2, ID_S, acc);
             acc = 1;
           }
         }
+        tc::umma_commit_one(one, &B->s_full[tile][s_buf]);
+        s_buf ^= 1;
       };
-      // O += P V for one half of the tile's keys.
-      auto product = [&](int i, int at, int half, bool first) {
+      // O += P V of its next step, with the values of stage v_st.
+      auto product = [&](bool first) {
+        const uint32_t p = s_to + p_buf * STEP;
+        const uint64_t b = tc::sw128_desc_mn(r_at + v_st * S::STAGE + S::KC * BLOCK, BLOCK);
         uint32_t acc = first ? 0 : 1;
-        int sl = at + (S::VC == 2 ? half : 0);
-        if (sl >= S::SLOTS) sl -= S::SLOTS;
-        const uint64_t b = tc::sw128_desc_mn(r_at + sl * SLOT, S::VKEYS * 128) +
-                           (S::VC == 2 ? 0 : half * 4 * (2048 >> 4));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          tc::umma_ts_one(one, tm + 256 + i * TILE, tm + i * TILE + (half * 4 + k) * 8,
-                      b + k * (2048 >> 4), ID_O, acc);
+        for (int k = 0; k < STEP / 16; ++k) {
+          tc::umma_ts_one(one, o_to, p + k * 8, b + k * (2048 >> 4), ID_O, acc);
           acc = 1;
         }
+        tc::umma_commit_one(one, &B->o_done[tile]);
       };
-      auto step = [&](int slots) {          // past the ring's current tile
-        slot += slots;
-        if (slot >= S::SLOTS) slot -= S::SLOTS;
-        if (++entry == ENTRIES) {
-          entry = 0;
-          phase ^= 1u;
+      auto next = [&](int& st, uint32_t& ph) {
+        if (++st == S::STAGES) {
+          st = 0;
+          ph ^= 1u;
         }
       };
       Unit U;
-      for (Walk walk(B, A.err); ok && walk.next<true>(U);) {
-        const int tiles[2] = {__shfl_sync(0xffffffffu, U.tiles[0], 0),
-                              __shfl_sync(0xffffffffu, U.tiles[1], 0)};
-        const int steps = max(tiles[0], tiles[1]);
-        if (steps == 0) continue;
-        if (!need(&B->full[entry], phase)) break;
-        for (int i = 0; i < 2; ++i) {
-          if (tiles[i] == 0) continue;
-          if (!need(&B->q_full[i], q_phase[i])) break;
-          q_phase[i] ^= 1u;
-          tc::tc_fence_after();
-          score(i, slot);
-          tc::umma_commit_one(one, &B->s_full[i]);
-          if (tiles[i] == 1) tc::umma_commit_one(one, &B->q_empty[i]);
+      for (Walk walk(B, A.err); ok && walk.next(U);) {
+        const int mine = __shfl_sync(0xffffffffu, U.steps[tile], 0);
+        const int all = __shfl_sync(0xffffffffu, max(U.steps[0], U.steps[1]), 0);
+        if (mine > 0) {
+          if (!need(&B->q_full[tile], q_phase)) break;
+          q_phase ^= 1u;
         }
-        if (!ok) break;
-        tc::umma_commit_one(one, &B->empty[entry]);
-        step(S::KC);
-        for (int j = 0; j < steps; ++j) {
-          // This step's values, and the next step's keys behind them.
-          const int v_entry = entry, v_slot = slot;
-          if (!need(&B->clean[v_entry], phase)) break;
-          step(S::VC);
-          bool keys = false;
-          for (int i = 0; i < 2; ++i) {
-            if (j >= tiles[i]) continue;
-            if (!need(&B->p_full[i][0], p_phase[i])) break;
+        // Scores of step j, two steps ahead of the products.  A step that only the
+        // other tile has is waited for too and passed on: both warps stay within
+        // one round of the ring.
+        auto ahead = [&](int j) {
+          if (!need(&B->k_full[k_st], k_ph)) return;
+          if (j < mine) {
             tc::tc_fence_after();
-            product(i, v_slot, 0, j == 0);
-            if (!need(&B->p_full[i][1], p_phase[i])) break;
-            p_phase[i] ^= 1u;
+            score();
+            if (j + 1 == mine) tc::umma_commit_one(one, &B->q_empty[tile]);
+          }
+          tc::umma_commit_one(one, &B->k_empty[k_st]);
+          next(k_st, k_ph);
+        };
+        for (int j = 0; j < min(all, 2) && ok; ++j) ahead(j);
+        for (int j = 0; j < all && ok; ++j) {
+          if (!need(&B->clean[v_st], v_ph)) break;
+          if (j < mine) {
+            if (!need(&B->p_full[tile][p_buf], p_phase)) break;
             tc::tc_fence_after();
-            product(i, v_slot, 1, false);
-            if (j + 1 == tiles[i]) {
-              tc::umma_commit_one(one, &B->o_full[i]);
-              continue;
-            }
-            if (!keys && !need(&B->full[entry], phase)) break;
-            keys = true;
-            score(i, slot);
-            tc::umma_commit_one(one, &B->s_full[i]);
-            if (j + 2 == tiles[i]) tc::umma_commit_one(one, &B->q_empty[i]);
+            product(j == 0);
+            if (j + 1 == mine) tc::umma_commit_one(one, &B->o_full[tile]);
+            p_phase ^= (uint32_t)p_buf;
+            p_buf ^= 1;
           }
-          if (!ok) break;
-          tc::umma_commit_one(one, &B->empty[v_entry]);
-          if (j + 1 < steps) {
-            tc::umma_commit_one(one, &B->empty[entry]);
-            step(S::KC);
-          }
+          tc::umma_commit_one(one, &B->v_empty[v_st]);
+          next(v_st, v_ph);
+          if (j + 2 < all) ahead(j + 2);
         }
       }
       // Every product issued is done before the tensor memory goes.
       tc::umma_commit_one(one, &B->drain);
       drain_phase(&B->drain, 0);
-    } else if (warp == COPY_WARP && lane == 0) {
-      // ------------------------------------------------------------------ copies
+    } else if (warp == COPY_WARP) {
+      // -------------------------------------------------- list of units, and copies
       const uint64_t keep = l2_evict_last_policy(), once = l2_evict_first_policy();
-      int entry = 0, slot = 0;             // next tile of the ring and its first slot
-      int oldest = 0, held = 0, used = 0;  // oldest tile not known to be free; tiles, slots held
-      uint32_t old_phase = 0, q_phase[2] = {1, 1};
-      bool ok = true;
-      // Starts the next tile of the ring, once it has a barrier pair and slots.
-      auto begin = [&](int slots) {
-        while (held == ENTRIES || used + slots > S::SLOTS) {
-          ok = ok && wait_phase(&B->empty[oldest], old_phase, abort_f, A.err);
-          if (!ok) return false;
-          used -= (oldest & 1) ? S::VC : S::KC;      // keys and values alternate
-          --held;
-          if (++oldest == ENTRIES) {
-            oldest = 0;
-            old_phase ^= 1u;
-          }
-        }
-        used += slots;
-        ++held;
-        mbar_arrive_expect_tx(&B->full[entry], (uint32_t)(slots * SLOT));
-        return true;
-      };
-      auto place = [&]() {                 // the next slot
-        uint8_t* at = ring + slot * SLOT;
-        if (++slot == S::SLOTS) slot = 0;
-        return at;
-      };
-      auto end = [&]() {
-        if (++entry == ENTRIES) entry = 0;
-      };
-      Unit U;
-      for (Walk walk(B, A.err); ok && walk.next<false>(U);) {
-        const int steps = max(U.tiles[0], U.tiles[1]);
-        const int hk = U.head0 / A.g, span = TILE >> A.pack_shift;
-        auto queries = [&](int i) {
-          if (U.tiles[i] == 0) return;
-          ok = ok && wait_phase(&B->q_empty[i], q_phase[i], abort_f, A.err);
-          if (!ok) return;
-          q_phase[i] ^= 1u;
-          mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)(S::KC * SLOT));
-          for (int c = 0; c < S::KC; ++c)
-            tma_load_4d(qs + (i * S::KC + c) * SLOT, &tq, c * 64, U.head0,
-                        U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
-        };
-        for (int j = 0; j < steps && ok; ++j) {
-          if (j == 0) queries(0);
-          if (!ok || !begin(S::KC)) break;
-          const int key0 = U.k0 + j * TILE;
-          for (int c = 0; c < S::KC; ++c)
-            tma_load_4d(place(), &tk, c * 64, hk, key0, 0, &B->full[entry], keep);
-          end();
-          if (j == 0) queries(1);
-          if (!ok || !begin(S::VC)) break;
-          for (int c = 0; c < S::VC; ++c) {
-            uint8_t* at = place();
-            for (int d = 0; d < DVP / 64; ++d)
-              tma_load_4d(at + d * S::VKEYS * 128, &tv, d * 64, hk, key0 + c * S::VKEYS, 0,
-                          &B->full[entry], keep);
-          }
-          end();
-        }
-      }
-      // On the error path, copies in flight land before the CTA may exit.
-      if (*abort_f) {
-        for (int i = 0; i < ENTRIES; ++i) {
-          drain_phase(&B->full[i], 0);
-          drain_phase(&B->full[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-          drain_phase(&B->q_full[i], 0);
-          drain_phase(&B->q_full[i], 1);
-        }
-      }
-    }
-    if (warp == CLEAN_WARP) {
-      // ------------------------------------------------------------ odd elements
-      int entry = 0, slot = 0;
-      uint32_t phase = 0;
-      auto step = [&](int slots) {
-        slot += slots;
-        if (slot >= S::SLOTS) slot -= S::SLOTS;
-        if (++entry == ENTRIES) {
-          entry = 0;
-          phase ^= 1u;
-        }
-      };
-      bool ok = true;
-      Unit U;
-      for (Walk walk(B, A.err); ok && walk.next<true>(U);) {
-        const int steps = max(U.tiles[0], U.tiles[1]);
-        for (int j = 0; j < steps; ++j) {
-          step(S::KC);
-          // Every tile is waited for, so that this warp stays within one round
-          // of the ring of the others.
-          ok = warp_wait(&B->full[entry], phase, abort_f, A.err);
-          if (!ok) break;
-          if (j >= U.whole) {
-            bool any = false;
-            for (int c = 0; c < S::VC; ++c) {
-              int sl = slot + c;
-              if (sl >= S::SLOTS) sl -= S::SLOTS;
-              uint4* at = reinterpret_cast<uint4*>(ring + sl * SLOT) + lane;
-#pragma unroll 8
-              for (int i = 0; i < SLOT / 512; ++i) {
-                uint4 x = at[i * 32];
-                if (has_odd<F16>(x)) {
-                  clear_odd<F16>(x);
-                  at[i * 32] = x;
-                  any = true;
-                }
-              }
-            }
-            if (any) {
-              B->odd[U.count & 15] = U.count;
-              fence_proxy_async();
-            }
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B->clean[entry]);
-          step(S::VC);
-        }
-      }
-    } else if (warp == LIST_WARP) {
-      // ------------------------------------------------------------ list of units
       const int groups = A.Hq >> A.pack_shift, span = TILE >> A.pack_shift;
       int slot = 0, round = 0, count = 0, held = -1;
-      uint32_t phase = 1;
+      uint32_t told = 1;
       int want = blockIdx.x, before = 0;     // this CTA's next unit on the list; units before here
       int64_t first = 0, end = 0;
+      int st = 0;                            // stage of the next step
+      uint32_t ph = 1, q_phase[2] = {1, 1};
       bool ok = true;
+      auto need = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && warp_wait(bar, parity, abort_f, A.err);
+        return ok;
+      };
       auto tell = [&](const Unit& U) {
-        ok = warp_wait(&B->unit_empty[slot], phase, abort_f, A.err);
-        if (!ok) return;
+        if (!need(&B->unit_empty[slot], told)) return;
         if (lane == 0) {
           B->unit[slot] = U;
           mbar_arrive(&B->unit_full[slot]);
         }
         if (++slot == UNITS) {
           slot = 0;
-          phase ^= 1u;
+          told ^= 1u;
+        }
+      };
+      auto copy = [&](const Unit& U) {
+        const int steps = max(U.steps[0], U.steps[1]);
+        const int hk = U.head0 / A.g;
+        auto queries = [&](int i) {
+          if (U.steps[i] == 0 || !need(&B->q_empty[i], q_phase[i])) return;
+          q_phase[i] ^= 1u;
+          if (lane != 0) return;
+          mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)S::Q_TILE);
+          for (int c = 0; c < S::KC; ++c)
+            tma_load_4d(qs + i * S::Q_TILE + c * 2 * BLOCK, &tq, c * 64, U.head0,
+                        U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
+        };
+        // Keys go two steps ahead of the values, as they are used.
+        int v_st = st;
+        uint32_t v_ph = ph;
+        for (int j = 0; j < steps + 2 && ok; ++j) {
+          if (j < steps) {
+            if (j == 0) queries(0);
+            if (!need(&B->k_empty[st], ph)) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&B->k_full[st], (uint32_t)(S::KC * BLOCK));
+              for (int c = 0; c < S::KC; ++c)
+                tma_load_4d(ring + st * S::STAGE + c * BLOCK, &tk, c * 64, hk, U.k0 + j * STEP,
+                            0, &B->k_full[st], keep);
+            }
+            if (++st == S::STAGES) {
+              st = 0;
+              ph ^= 1u;
+            }
+            if (j == 0) queries(1);
+          }
+          if (j >= 2) {
+            if (!need(&B->v_empty[v_st], v_ph)) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&B->v_full[v_st], (uint32_t)(S::VC * BLOCK));
+              for (int d = 0; d < S::VC; ++d)
+                tma_load_4d(ring + v_st * S::STAGE + (S::KC + d) * BLOCK, &tv, d * 64, hk,
+                            U.k0 + (j - 2) * STEP, 0, &B->v_full[v_st], keep);
+            }
+            if (++v_st == S::STAGES) {
+              v_st = 0;
+              v_ph ^= 1u;
+            }
+          }
         }
       };
       for (int block = A.blocks - 1; block >= 0 && ok; --block) {
@@ -723,11 +650,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             for (int i = 0; i < 2; ++i) {
               const int top = t0 + i * span, last = min(U.n, top + span) - 1;
               const int keys = top < U.n ? min(max(last + U.m - U.n + 1, 0), U.m) : 0;
-              U.tiles[i] = (keys + TILE - 1) / TILE;
+              U.steps[i] = (keys + STEP - 1) / STEP;
             }
-            U.whole = max(t0 + U.m - U.n + 1, 0) / TILE;
+            U.whole = max(t0 + U.m - U.n + 1, 0) / STEP;
             U.count = count++;
             tell(U);
+            if (ok) copy(U);
             ++round;
             want = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
           }
@@ -737,6 +665,57 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       Unit last = {};
       last.count = -1;
       if (ok) tell(last);
+      // On the error path, copies in flight land before the CTA may exit.
+      if (*abort_f) {
+        for (int i = 0; i < S::STAGES; ++i)
+          for (uint32_t parity = 0; parity < 2; ++parity) {
+            drain_phase(&B->k_full[i], parity);
+            drain_phase(&B->v_full[i], parity);
+          }
+        for (int i = 0; i < 2; ++i) {
+          drain_phase(&B->q_full[i], 0);
+          drain_phase(&B->q_full[i], 1);
+        }
+      }
+    }
+    if (warp == CLEAN_WARP) {
+      // ------------------------------------------------------------ odd elements
+      int st = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      Unit U;
+      for (Walk walk(B, A.err); ok && walk.next(U);) {
+        const int steps = max(U.steps[0], U.steps[1]);
+        for (int j = 0; j < steps; ++j) {
+          // Every step is waited for, so that this warp stays within one round
+          // of the ring of the others.
+          ok = warp_wait(&B->v_full[st], ph, abort_f, A.err);
+          if (!ok) break;
+          if (j >= U.whole) {
+            bool any = false;
+            uint4* at = reinterpret_cast<uint4*>(ring + st * S::STAGE + S::KC * BLOCK) + lane;
+#pragma unroll 8
+            for (int i = 0; i < S::VC * BLOCK / 512; ++i) {
+              uint4 x = at[i * 32];
+              if (has_odd<F16>(x)) {
+                clear_odd<F16>(x);
+                at[i * 32] = x;
+                any = true;
+              }
+            }
+            if (any) {
+              B->odd[U.count & 15] = U.count;
+              fence_proxy_async();
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->clean[st]);
+          if (++st == S::STAGES) {
+            st = 0;
+            ph ^= 1u;
+          }
+        }
+      }
     }
     __syncwarp();
   }
@@ -763,9 +742,6 @@ static int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUt
   return launch(prompt_kernel<DKP, DVP, F16>, dim3(grid), dim3(PROMPT_THREADS), (size_t)S::SMEM,
                 stream, mq, mk, mv, A);
 }
-
-// Values up to 64 wide beside keys up to 64, else both padded to 128 (192).
-static int value_keys(int64_t Dk, int64_t Dv) { return Dk <= 64 && Dv <= 64 ? 128 : 64; }
 
 }  // namespace attn
 }  // namespace kb
@@ -838,10 +814,10 @@ extern "C" int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride,
   // Without keys no tile is ever copied: any valid map will do.
   const int64_t keys = std::max<int64_t>(total_k, 1);
   st = at::make_map_4d(&mk, total_k ? k : q, dtype, {Dk, Hkv, keys, 1},
-                       {k_head_stride, k_token_stride, 8}, 1, at::TILE);
+                       {k_head_stride, k_token_stride, 8}, 1, at::STEP);
   if (st != KB_OK) return st;
   st = at::make_map_4d(&mv, total_k ? v : q, dtype, {Dv, Hkv, keys, 1},
-                       {v_head_stride, v_token_stride, 8}, 1, at::value_keys(Dk, Dv));
+                       {v_head_stride, v_token_stride, 8}, 1, at::STEP);
   if (st != KB_OK) return st;
   const int grid = (int)std::min<int64_t>(kb::num_sms(dev), units);
   if (Dk <= 64 && Dv <= 64)
