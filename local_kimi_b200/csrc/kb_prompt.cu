@@ -14,10 +14,10 @@
 //
 //   warp 10: the list of units, and copies.  It counts, 32 requests at a time,
 //     which have rows that late, tells the other warps this CTA's units through
-//     a ring of four, and brings in Q tiles and a ring of stages with a step's
-//     keys and values (8 KB blocks of 64 rows x 64 elements), by tensor copies
-//     in the 128-byte swizzle; keys and values have barriers of their own,
-//     since keys are used two steps before the values beside them.
+//     a ring of four, and brings in Q tiles and a ring of stages (8 KB blocks
+//     of 64 rows x 64 elements), by tensor copies in the 128-byte swizzle.  A
+//     stage holds the keys of step h + 2 and the values of step h: what the
+//     MMAs read one after the other, under one barrier pair.
 //   warps 8 and 9: issue the MMAs of tiles A and B (one warp for both spent as
 //     long in its waits and commits as the tensor core in the products).
 //     S = Q K^T (both from shared memory) into tensor memory, O += P V with P
@@ -104,13 +104,12 @@ struct Unit {
 };
 
 struct PromptBars {
-  uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES], v_full[MAX_STAGES], v_empty[MAX_STAGES];
-  uint64_t clean[MAX_STAGES];   // a step's values are there, without odd elements
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+  uint64_t clean[MAX_STAGES];   // full, and the values without odd elements
   uint64_t unit_full[UNITS], unit_empty[UNITS];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2][2], p_full[2][2];   // of a tile's two buffers
-  uint64_t o_done[2];           // a step's P V is in O
-  uint64_t o_full[2];           // ... and it was the unit's last
+  uint64_t o_near[2], o_full[2];         // P V of the unit's last step but one, last step
   uint64_t drain;
   Unit unit[UNITS];
   int odd[16];              // units that had odd elements, by their number's last four bits
@@ -227,16 +226,14 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::STAGES; ++i) {
-      mbar_init(&B->k_full[i], 1);
-      mbar_init(&B->k_empty[i], 2);
-      mbar_init(&B->v_full[i], 1);
-      mbar_init(&B->v_empty[i], 2);
+      mbar_init(&B->full[i], 1);
+      mbar_init(&B->empty[i], 2);
       mbar_init(&B->clean[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B->q_full[i], 1);
       mbar_init(&B->q_empty[i], 1);
-      mbar_init(&B->o_done[i], 1);
+      mbar_init(&B->o_near[i], 1);
       mbar_init(&B->o_full[i], 1);
       for (int j = 0; j < 2; ++j) {
         mbar_init(&B->s_full[i][j], 1);
@@ -288,8 +285,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     const float scale2 = A.scale2;
     const int span = TILE >> A.pack_shift;
     int buf = 0;                          // the next step's S buffer
-    uint32_t s_phase = 0, o_phase = 1;    // o_phase: of the last step handed over
-    uint32_t end_phase = 0;
+    uint32_t s_phase = 0, near_phase = 0, end_phase = 0;
     Unit U;
     for (Walk walk(B, A.err); walk.next(U);) {
       const int first = U.t0 + tile * span;
@@ -336,9 +332,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         if (j == 0) {
           top = mine;
         } else if (__any_sync(0xffffffffu, mine > top + RESCALE)) {
-          // O may be touched once P V of the last step is done (that of the step
-          // before was issued ahead of this step's S, so it is).
-          if (!warp_wait(&B->o_done[tile], o_phase, abort_f, A.err)) {
+          // O may be touched once P V of the last step is done: the next step's
+          // S was issued behind it.
+          if (!(j + 1 < steps ? warp_wait(&B->s_full[tile][buf ^ 1], s_phase ^ (uint32_t)buf,
+                                          abort_f, A.err)
+                              : warp_wait(&B->o_near[tile], near_phase, abort_f, A.err))) {
             ok = false;
             break;
           }
@@ -394,7 +392,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         if (lane == 0) mbar_arrive(&B->p_full[tile][buf]);
         part[0] = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
         sum += part[0].x + part[0].y;
-        o_phase ^= 1u;
         if (buf) s_phase ^= 1u;
         buf ^= 1;
       }
@@ -411,6 +408,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         out[i] = t < U.n ? A.out + ((int64_t)(U.q0 + t) * A.Hq + h) * A.Dv + (lane & 3) * 8
                          : nullptr;
       }
+      if (steps > 1) near_phase ^= 1u;
       bool odd = false;
       if (steps > 0) {
         if (!warp_wait(&B->o_full[tile], end_phase, abort_f, A.err)) break;
@@ -469,22 +467,22 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_at = smem_addr(qs) + tile * S::Q_TILE, r_at = smem_addr(ring);
       const uint32_t s_to = tm + tile * 2 * STEP, o_to = tm + 256 + tile * TILE;
-      int k_st = 0, v_st = 0;             // stages of the next keys and values
-      uint32_t k_ph = 0, v_ph = 0, q_phase = 0, p_phase = 0;
+      int st = 0;                         // stage of the next keys and values
+      uint32_t ph = 0, q_phase = 0, p_phase = 0;
       int s_buf = 0, p_buf = 0;           // S buffers of the next scores and weights
       bool ok = true;
       auto need = [&](uint64_t* bar, uint32_t ph) {
         ok = warp_wait(bar, ph, abort_f, A.err);
         return ok;
       };
-      // S of the tile's next step, from the keys of stage k_st.
+      // S of the tile's next step, from the keys of the stage.
       auto score = [&]() {
         const uint32_t d = s_to + s_buf * STEP;
         uint32_t acc = 0;
 #pragma unroll
         for (int c = 0; c < S::KC; ++c) {
           const uint64_t a = tc::sw128_desc(q_at + c * 2 * BLOCK);
-          const uint64_t b = tc::sw128_desc(r_at + k_st * S::STAGE + c * BLOCK);
+          const uint64_t b = tc::sw128_desc(r_at + st * S::STAGE + c * BLOCK);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             tc::umma_one(one, d, a + k * 2, b + k * 2, ID_S, acc);
@@ -494,59 +492,49 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         tc::umma_commit_one(one, &B->s_full[tile][s_buf]);
         s_buf ^= 1;
       };
-      // O += P V of its next step, with the values of stage v_st.
+      // O += P V of its next step, with the values of the stage.
       auto product = [&](bool first) {
         const uint32_t p = s_to + p_buf * STEP;
-        const uint64_t b = tc::sw128_desc_mn(r_at + v_st * S::STAGE + S::KC * BLOCK, BLOCK);
+        const uint64_t b = tc::sw128_desc_mn(r_at + st * S::STAGE + S::KC * BLOCK, BLOCK);
         uint32_t acc = first ? 0 : 1;
 #pragma unroll
         for (int k = 0; k < STEP / 16; ++k) {
           tc::umma_ts_one(one, o_to, p + k * 8, b + k * (2048 >> 4), ID_O, acc);
           acc = 1;
         }
-        tc::umma_commit_one(one, &B->o_done[tile]);
-      };
-      auto next = [&](int& st, uint32_t& ph) {
-        if (++st == S::STAGES) {
-          st = 0;
-          ph ^= 1u;
-        }
       };
       Unit U;
       for (Walk walk(B, A.err); ok && walk.next(U);) {
         const int mine = __shfl_sync(0xffffffffu, U.steps[tile], 0);
         const int all = __shfl_sync(0xffffffffu, max(U.steps[0], U.steps[1]), 0);
-        if (mine > 0) {
-          if (!need(&B->q_full[tile], q_phase)) break;
-          q_phase ^= 1u;
-        }
-        // Scores of step j, two steps ahead of the products.  A step that only the
-        // other tile has is waited for too and passed on: both warps stay within
-        // one round of the ring.
-        auto ahead = [&](int j) {
-          if (!need(&B->k_full[k_st], k_ph)) return;
-          if (j < mine) {
-            tc::tc_fence_after();
-            score();
-            if (j + 1 == mine) tc::umma_commit_one(one, &B->q_empty[tile]);
-          }
-          tc::umma_commit_one(one, &B->k_empty[k_st]);
-          next(k_st, k_ph);
-        };
-        for (int j = 0; j < min(all, 2) && ok; ++j) ahead(j);
-        for (int j = 0; j < all && ok; ++j) {
-          if (!need(&B->clean[v_st], v_ph)) break;
-          if (j < mine) {
+        // Products of step j and scores of step j + 2.  A stage that only the other
+        // tile uses is waited for too and passed on: both warps stay within one round
+        // of the ring.
+        for (int j = -2; j < all && all > 0; ++j) {
+          if (!need(&B->clean[st], ph)) break;
+          if (j >= 0 && j < mine) {
             if (!need(&B->p_full[tile][p_buf], p_phase)) break;
             tc::tc_fence_after();
             product(j == 0);
-            if (j + 1 == mine) tc::umma_commit_one(one, &B->o_full[tile]);
             p_phase ^= (uint32_t)p_buf;
             p_buf ^= 1;
+            if (j + 2 == mine) tc::umma_commit_one(one, &B->o_near[tile]);
+            if (j + 1 == mine) tc::umma_commit_one(one, &B->o_full[tile]);
           }
-          tc::umma_commit_one(one, &B->v_empty[v_st]);
-          next(v_st, v_ph);
-          if (j + 2 < all) ahead(j + 2);
+          if (j + 2 < mine) {
+            if (j == -2) {
+              if (!need(&B->q_full[tile], q_phase)) break;
+              q_phase ^= 1u;
+            }
+            tc::tc_fence_after();
+            score();
+            if (j + 3 == mine) tc::umma_commit_one(one, &B->q_empty[tile]);
+          }
+          tc::umma_commit_one(one, &B->empty[st]);
+          if (++st == S::STAGES) {
+            st = 0;
+            ph ^= 1u;
+          }
         }
       }
       // Every product issued is done before the tensor memory goes.
@@ -590,38 +578,28 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             tma_load_4d(qs + i * S::Q_TILE + c * 2 * BLOCK, &tq, c * 64, U.head0,
                         U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
         };
-        // Keys go two steps ahead of the values, as they are used.
-        int v_st = st;
-        uint32_t v_ph = ph;
-        for (int j = 0; j < steps + 2 && ok; ++j) {
-          if (j < steps) {
-            if (j == 0) queries(0);
-            if (!need(&B->k_empty[st], ph)) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&B->k_full[st], (uint32_t)(S::KC * BLOCK));
+        for (int j = -2; j < steps && steps > 0; ++j) {
+          if (j == -2) queries(0);
+          if (!need(&B->empty[st], ph)) break;
+          const bool keys = j + 2 < steps, values = j >= 0;
+          if (lane == 0) {
+            uint8_t* at = ring + st * S::STAGE;
+            mbar_arrive_expect_tx(&B->full[st], (uint32_t)(((keys ? S::KC : 0) +
+                                                            (values ? S::VC : 0)) * BLOCK));
+            if (keys)
               for (int c = 0; c < S::KC; ++c)
-                tma_load_4d(ring + st * S::STAGE + c * BLOCK, &tk, c * 64, hk, U.k0 + j * STEP,
-                            0, &B->k_full[st], keep);
-            }
-            if (++st == S::STAGES) {
-              st = 0;
-              ph ^= 1u;
-            }
-            if (j == 0) queries(1);
-          }
-          if (j >= 2) {
-            if (!need(&B->v_empty[v_st], v_ph)) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&B->v_full[v_st], (uint32_t)(S::VC * BLOCK));
+                tma_load_4d(at + c * BLOCK, &tk, c * 64, hk, U.k0 + (j + 2) * STEP, 0,
+                            &B->full[st], keep);
+            if (values)
               for (int d = 0; d < S::VC; ++d)
-                tma_load_4d(ring + v_st * S::STAGE + (S::KC + d) * BLOCK, &tv, d * 64, hk,
-                            U.k0 + (j - 2) * STEP, 0, &B->v_full[v_st], keep);
-            }
-            if (++v_st == S::STAGES) {
-              v_st = 0;
-              v_ph ^= 1u;
-            }
+                tma_load_4d(at + (S::KC + d) * BLOCK, &tv, d * 64, hk, U.k0 + j * STEP, 0,
+                            &B->full[st], keep);
           }
+          if (++st == S::STAGES) {
+            st = 0;
+            ph ^= 1u;
+          }
+          if (j == -2) queries(1);
         }
       };
       for (int block = A.blocks - 1; block >= 0 && ok; --block) {
@@ -669,8 +647,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       if (*abort_f) {
         for (int i = 0; i < S::STAGES; ++i)
           for (uint32_t parity = 0; parity < 2; ++parity) {
-            drain_phase(&B->k_full[i], parity);
-            drain_phase(&B->v_full[i], parity);
+            drain_phase(&B->full[i], parity);
           }
         for (int i = 0; i < 2; ++i) {
           drain_phase(&B->q_full[i], 0);
@@ -686,12 +663,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       Unit U;
       for (Walk walk(B, A.err); ok && walk.next(U);) {
         const int steps = max(U.steps[0], U.steps[1]);
-        for (int j = 0; j < steps; ++j) {
-          // Every step is waited for, so that this warp stays within one round
+        for (int j = -2; j < steps && steps > 0; ++j) {
+          // Every stage is waited for, so that this warp stays within one round
           // of the ring of the others.
-          ok = warp_wait(&B->v_full[st], ph, abort_f, A.err);
+          ok = warp_wait(&B->full[st], ph, abort_f, A.err);
           if (!ok) break;
-          if (j >= U.whole) {
+          if (j >= 0 && j >= U.whole) {
             bool any = false;
             uint4* at = reinterpret_cast<uint4*>(ring + st * S::STAGE + S::KC * BLOCK) + lane;
 #pragma unroll 8
