@@ -20,7 +20,7 @@ namespace kb {
 namespace paged {
 
 constexpr int THREADS = 256;
-constexpr int MAX_REQUESTS = 12288;          // two int arrays of shared memory
+constexpr int MAX_REQUESTS = 12288;          // three int arrays of shared memory
 
 struct PlanArgs {
   const int* context;
@@ -40,7 +40,12 @@ struct PlanArgs {
   uint32_t* err;
 };
 
-__device__ __forceinline__ int pages_of(int64_t tokens, int ps) {
+// Lengths count up to 2^30 (32-bit sums and divisions; a page too).
+__device__ __forceinline__ uint32_t length_of(const int* lens, int b) {
+  return (uint32_t)min(max(__ldg(lens + b), 0), 1 << 30);
+}
+
+__device__ __forceinline__ int pages_of(uint32_t tokens, uint32_t ps) {
   return (int)((tokens + ps - 1) / ps);
 }
 
@@ -66,20 +71,24 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
   extern __shared__ int sums[];
   int* s_tok = sums;                 // [B + 1] first token of each request
   int* s_page = sums + A.B + 1;      // [B + 1] first fresh page of each request
+  int* s_ctx = s_page + A.B + 1;     // [B] cached tokens
   __shared__ int s_part[THREADS / 32][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t ps = (uint32_t)A.ps;
   pdl_wait();
   // Each thread takes a run of consecutive requests.
   const int per = (A.B + THREADS - 1) / THREADS;
   const int b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
   int tok = 0, page = 0, lost = 0;
+#pragma unroll 4
   for (int b = b0; b < b1; ++b) {
-    const int c = max(0, A.context[b]), n = max(0, A.fresh[b]);
-    const int have = pages_of(c, A.ps), want = pages_of((int64_t)c + n, A.ps);
+    const uint32_t c = length_of(A.context, b), n = length_of(A.fresh, b);
+    const int have = pages_of(c, ps), want = pages_of(c + n, ps);
     const int need = max(0, min(want, A.width) - have);
     s_tok[b] = tok;
     s_page[b] = page;
-    tok += n;
+    s_ctx[b] = (int)c;
+    tok += (int)n;
     page += need;
     lost += want - have - need;
   }
@@ -123,36 +132,46 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
   }
   for (int i = at; i < pages; i += step) {
     const int b = find(s_page, A.B, i);
-    const int col = pages_of(max(0, A.context[b]), A.ps) + i - s_page[b];
-    A.table[(int64_t)b * A.table_stride + col] = i < avail ? A.free_pages[head + i] : -1;
+    const int col = pages_of((uint32_t)s_ctx[b], ps) + i - s_page[b];
+    A.table[(int64_t)b * A.table_stride + col] = i < avail ? __ldg(A.free_pages + head + i) : -1;
   }
-  for (int i = at; i < A.N; i += step) {
-    int64_t slot = -1, word = 0;
-    int position = 0;
-    if (i < tokens) {
-      const int b = find(s_tok, A.B, i);
-      const int t = i - s_tok[b];
-      const int c = max(0, A.context[b]);
-      const int64_t place = (int64_t)c + t;
-      const int col = (int)(place / A.ps), have = pages_of(c, A.ps);
-      int id = -1;
-      if (col < A.width) {
-        if (col < have) {
-          id = A.table[(int64_t)b * A.table_stride + col];
-        } else {
-          const int f = s_page[b] + col - have;
-          id = f < avail ? A.free_pages[head + f] : -1;
-        }
-      }
-      if (id >= 0) slot = (int64_t)id * A.ps + place % A.ps;
-      position = (int)place;
-      if (A.parents != nullptr) {
+  // The page of a token: a fresh one, or an entry that no CTA writes.
+  auto place_of = [&](int i, uint32_t& place, int& b) {
+    b = find(s_tok, A.B, i);
+    const uint32_t c = (uint32_t)s_ctx[b];
+    place = c + (uint32_t)(i - s_tok[b]);
+    const int col = (int)(place / ps), have = pages_of(c, ps);
+    if (col >= A.width) return -1;
+    if (col < have) return __ldg(A.table + (int64_t)b * A.table_stride + col);
+    const int f = s_page[b] + col - have;
+    return f < avail ? __ldg(A.free_pages + head + f) : -1;
+  };
+  constexpr int BATCH = 4;
+  for (int i0 = at; i0 < A.N; i0 += BATCH * step) {
+    int id[BATCH], b[BATCH];
+    uint32_t place[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * step;
+      id[u] = -1;
+      place[u] = 0;
+      b[u] = 0;
+      if (i < min(tokens, A.N)) id[u] = place_of(i, place[u], b[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * step;
+      if (i >= A.N) break;
+      int64_t word = 0;
+      int position = (int)place[u];
+      if (A.parents != nullptr && i < tokens) {
         // Up the tree: parents come before their children, so this ends.
+        const int t = i - s_tok[b[u]];
         int node = t, depth = 0;
         if (t < 64) {
           word = (int64_t)1 << t;
           while (node > 0) {
-            const int up = A.parents[s_tok[b] + node];
+            const int up = __ldg(A.parents + s_tok[b[u]] + node);
             if (up < 0 || up >= node) {
               atomicOr(A.err, ERR_TREE);
               break;
@@ -164,12 +183,12 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
         } else {
           atomicOr(A.err, ERR_TREE);
         }
-        position = c + depth;
+        position = s_ctx[b[u]] + depth;
       }
+      A.slots[i] = id[u] >= 0 ? (int64_t)id[u] * A.ps + place[u] % ps : -1;
+      A.positions[i] = position;
+      if (A.mask != nullptr) A.mask[i] = word;
     }
-    A.slots[i] = slot;
-    A.positions[i] = position;
-    if (A.mask != nullptr) A.mask[i] = word;
   }
 }
 
@@ -188,37 +207,48 @@ struct AppendArgs {
   uint32_t* err;
 };
 
-// A thread per 16-byte piece; a token's pieces are its heads' key rows and
-// then its heads' value rows, so neighbouring threads read neighbouring bytes.
+// Four 16-byte pieces per thread, loaded before any is stored; a token's pieces
+// are its heads' key rows and then its heads' value rows, so neighbouring threads
+// move neighbouring bytes.  Bound by the bytes, once in and once out.
+constexpr int PIECES = 4;
+
 __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs A) {
   pdl_wait();
   pdl_launch_dependents();
-  const int pieces = A.H * (A.ck + A.cv);
-  const int64_t total = (int64_t)A.N * pieces;
-  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * THREADS) {
-    const int t = (int)(i / pieces);
-    int r = (int)(i - (int64_t)t * pieces);
-    const int64_t slot = A.slots[t];
+  const int keys = A.H * A.ck, pieces = keys + A.H * A.cv;      // of a token
+  const int64_t base = (int64_t)blockIdx.x * (THREADS * PIECES);
+  const int64_t t0 = base / pieces;
+  const int r0 = (int)(base - t0 * pieces) + threadIdx.x;
+  uint4 x[PIECES];
+  uint16_t* to[PIECES];
+#pragma unroll
+  for (int u = 0; u < PIECES; ++u) {
+    const int over = (r0 + u * THREADS) / pieces;
+    int r = r0 + u * THREADS - over * pieces;
+    const int64_t t = t0 + over;
+    to[u] = nullptr;
+    if (t >= A.N) continue;
+    const int64_t slot = __ldg(A.slots + t);
     if (slot < 0) continue;
     if (slot >= A.nslots) {
       atomicOr(A.err, ERR_PAGE);
       continue;
     }
     const int64_t page = slot / A.ps, row = slot - page * A.ps;
-    if (r < A.H * A.ck) {
+    if (r < keys) {
       const int h = r / A.ck, c = r - h * A.ck;
-      const uint4 x = *reinterpret_cast<const uint4*>(A.k + t * A.k_tok + h * A.k_head + c * 8);
-      *reinterpret_cast<uint4*>(A.kc + page * A.kc_page + row * A.kc_row + h * A.kc_head +
-                                c * 8) = x;
+      x[u] = ldg_stream_v4(A.k + t * A.k_tok + h * A.k_head + c * 8);
+      to[u] = A.kc + page * A.kc_page + row * A.kc_row + h * A.kc_head + c * 8;
     } else {
-      r -= A.H * A.ck;
+      r -= keys;
       const int h = r / A.cv, c = r - h * A.cv;
-      const uint4 x = *reinterpret_cast<const uint4*>(A.v + t * A.v_tok + h * A.v_head + c * 8);
-      *reinterpret_cast<uint4*>(A.vc + page * A.vc_page + row * A.vc_row + h * A.vc_head +
-                                c * 8) = x;
+      x[u] = ldg_stream_v4(A.v + t * A.v_tok + h * A.v_head + c * 8);
+      to[u] = A.vc + page * A.vc_page + row * A.vc_row + h * A.vc_head + c * 8;
     }
   }
+#pragma unroll
+  for (int u = 0; u < PIECES; ++u)
+    if (to[u] != nullptr) *reinterpret_cast<uint4*>(to[u]) = x[u];
 }
 
 }  // namespace paged
@@ -266,11 +296,11 @@ extern "C" int kb_paged_plan(const int32_t* context_lens, const int32_t* new_len
   A.missing = missing;
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  const size_t smem = (size_t)(2 * (B + 1)) * sizeof(int);
-  static_assert(2 * (kb::paged::MAX_REQUESTS + 1) * sizeof(int) <= 100 * 1024, "shared memory");
+  const size_t smem = (size_t)(3 * B + 2) * sizeof(int);
+  static_assert((3 * kb::paged::MAX_REQUESTS + 2) * sizeof(int) <= 160 * 1024, "shared memory");
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kb::paged::plan_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     KB_REQUIRE(e == cudaSuccess, KB_ERR_DEVICE, "paged plan: shared-memory limit: %s",
                cudaGetErrorString(e));
   }
@@ -328,10 +358,9 @@ extern "C" int kb_paged_append(const uint16_t* k, int64_t k_token_stride, int64_
   A.cv = (int)(Dv / 8);
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  const int64_t total = N * H * (A.ck + A.cv);
-  int64_t grid = (total + kb::paged::THREADS - 1) / kb::paged::THREADS;
-  const int64_t most = (int64_t)kb::num_sms(dev) * 8;
-  if (grid > most) grid = most;
+  constexpr int64_t kBlock = kb::paged::THREADS * kb::paged::PIECES;
+  const int64_t grid = (N * H * (A.ck + A.cv) + kBlock - 1) / kBlock;
+  KB_REQUIRE(grid < ((int64_t)1 << 31), KB_ERR_UNSUPPORTED, "paged append: too many tokens");
   return kb::launch(kb::paged::append_kernel, dim3((unsigned)grid), dim3(kb::paged::THREADS), 0,
                     stream, A);
 }

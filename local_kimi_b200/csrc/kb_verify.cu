@@ -14,12 +14,19 @@
 // is left of p by rounding, the row's own p is used.  Temperature 0 takes
 // the child that is the row's argmax (lowest index) and ends with the argmax.
 //
-// Two launches.  row_kernel reads every logit once: (max, sum of exp) or the
-// argmax of each row segment, fp32.  pick_kernel joins the segments, walks
-// the tree from shared memory, and scans the last node's row with the noise
-// (and q): its CTAs split the vocabulary, each joins its best (value, index)
-// key with a 64-bit atomicMax, and the request's last CTA writes the token.
-// Bound by the bytes of the logits.
+// Two launches.  row_kernel reads every logit once, 16 bytes a load, with a
+// running maximum and sum of exponentials per thread (or the argmax) of each
+// row segment, fp32.  pick_kernel joins the segments, walks the tree from
+// shared memory, and scans the last node's row with the noise (and q): its
+// CTAs split the vocabulary, each joins its best (value, index) key with a
+// 64-bit atomicMax, and the request's last CTA writes the token.  Bound by the
+// bytes: the logits once, and of one row a request logits, noise and q again.
+// The exponentials (16 a clock and SM) take three quarters of that time.
+//
+// Rows start anywhere (an odd vocabulary): the loads begin at the row's first
+// 16-byte boundary, what lies before and after goes one by one.  The fast
+// loops assume finite sums; a segment whose sum is not finite or zero is
+// read again with not-a-number as absent and infinity as the largest number.
 #include <cuda_fp16.h>
 
 #include <float.h>
@@ -51,6 +58,7 @@ struct Race {               // of a request's CTAs for its next token
 struct Args {
   const void* logits;
   int64_t row_stride;
+  int64_t skew;             // elements from `logits`, moved down to a 16-byte boundary, to row 0
   int64_t rows;
   int V;
   const int64_t* tokens;
@@ -97,10 +105,159 @@ __device__ __forceinline__ void request(const Args& A, int b, int64_t& first, in
   n = (int)min(e - s, (int64_t)A.most);
 }
 
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -1e30f;       // start of a running maximum
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Elements of a 16-byte load.
+template <int TYPE>
+constexpr int PIECE = TYPE == F32 ? 4 : 8;
+
+template <int TYPE>
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[PIECE<TYPE>]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (TYPE == F32) {
+      x[i] = __uint_as_float(w[i]);
+    } else if (TYPE == BF16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// The 16-byte pieces within elements [lo, hi) of a row that starts at element
+// `base` of a 16-byte aligned array: first element of the first whole piece
+// (relative to the row) and their number.
+template <int TYPE>
+__device__ __forceinline__ void whole_pieces(int64_t base, int lo, int hi, int& first,
+                                             int& count) {
+  constexpr int P = PIECE<TYPE>;
+  const int skew = (int)((base + lo) & (P - 1));
+  first = min(hi, skew ? lo + P - skew : lo);
+  count = (hi - first) / P;
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint4 piece(const void* p, int64_t element) {
+  return ldg_stream_v4(static_cast<const uint8_t*>(p) + element * (TYPE == F32 ? 4 : 2));
+}
+
+// Running (maximum, sum) of a thread over its share of [lo, hi).
+template <int TYPE>
+__device__ __forceinline__ void sum_segment(const Args& A, int64_t base, int lo, int hi, float c2,
+                                            float& top, float& sum) {
+  constexpr int P = PIECE<TYPE>, BATCH = 4;
+  int first, count;
+  whole_pieces<TYPE>(base, lo, hi, first, count);
+  const int tid = threadIdx.x;
+  top = LOWEST;
+  sum = 0.f;
+  auto take = [&](float x) {
+    if (x > top) {
+      sum *= exp2_fast((top - x) * c2);
+      top = x;
+    }
+    sum += exp2_fast((x - top) * c2);
+  };
+  for (int i = tid; i < count; i += THREADS * BATCH) {
+    float x[BATCH * P];
+    uint4 v[BATCH];
+    const bool all = i + (BATCH - 1) * THREADS < count;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+      v[u] = piece<TYPE>(A.logits, base + first + (int64_t)min(i + u * THREADS, count - 1) * P);
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      unpack<TYPE>(v[u], *reinterpret_cast<float(*)[P]>(&x[u * P]));
+      if (!all && i + u * THREADS >= count)
+#pragma unroll
+        for (int j = 0; j < P; ++j) x[u * P + j] = -INFINITY;
+    }
+    float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+    for (int j = 4; j < BATCH * P; ++j) m[j & 3] = fmaxf(m[j & 3], x[j]);
+    const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    if (most > top) {
+      sum *= exp2_fast((top - most) * c2);
+      top = most;
+    }
+    // (x - top) first: the difference is exact where it matters, x * c2 is not.
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < BATCH * P; ++j) part[j & 3] += exp2_fast((x[j] - top) * c2);
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  // Before the first whole piece and after the last.
+  for (int i = lo + tid; i < first; i += THREADS) take(logit<TYPE>(A.logits, base + i));
+  for (int i = first + count * P + tid; i < hi; i += THREADS)
+    take(logit<TYPE>(A.logits, base + i));
+}
+
+// Largest logit of a thread's share and its index (lowest among equals).
+template <int TYPE>
+__device__ __forceinline__ void best_segment(const Args& A, int64_t base, int lo, int hi,
+                                             float& top, int& arg) {
+  constexpr int P = PIECE<TYPE>;
+  int first, count;
+  whole_pieces<TYPE>(base, lo, hi, first, count);
+  const int tid = threadIdx.x;
+  top = -INFINITY;
+  arg = INT_MAX;
+  auto take = [&](float x, int i) {
+    if (x > top || arg == INT_MAX) {
+      top = fmaxf(x, -INFINITY);       // not-a-number: absent
+      arg = i;
+    }
+  };
+  for (int i = lo + tid; i < first; i += THREADS) take(logit<TYPE>(A.logits, base + i), i);
+#pragma unroll 4
+  for (int i = tid; i < count; i += THREADS) {
+    float x[P];
+    const int at = first + i * P;
+    unpack<TYPE>(piece<TYPE>(A.logits, base + at), x);
+#pragma unroll
+    for (int j = 0; j < P; ++j) take(x[j], at + j);
+  }
+  for (int i = first + count * P + tid; i < hi; i += THREADS)
+    take(logit<TYPE>(A.logits, base + i), i);
+}
+
+__device__ __forceinline__ float block_max(float v, float* red) {
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+  for (int w = 1; w < THREADS / 32; ++w) v = fmaxf(v, red[w]);
+  __syncthreads();
+  return v;
+}
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+  for (int w = 1; w < THREADS / 32; ++w) v += red[w];
+  __syncthreads();
+  return v;
+}
+
 template <int TYPE>
 __global__ void __launch_bounds__(THREADS) row_kernel(const Args A) {
-  __shared__ float s_a[THREADS / 32], s_b[THREADS / 32];
-  __shared__ int s_i[THREADS / 32];
+  __shared__ float red[THREADS / 32];
+  __shared__ float s_top[THREADS / 32];
+  __shared__ int s_arg[THREADS / 32];
   pdl_wait();
   pdl_launch_dependents();
   const int t = blockIdx.x / A.segments, seg = blockIdx.x - t * A.segments;
@@ -110,61 +267,57 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const Args A) {
   if (t >= n) return;
   const int64_t row = first + t;
   const float temp = A.temps[blockIdx.y];
-  const float inv_t = inverse(temp);
   const int lo = (int)((int64_t)A.V * seg / A.segments);
   const int hi = (int)((int64_t)A.V * (seg + 1) / A.segments);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t base = row * A.row_stride;
-  float top = -INFINITY;
-  int arg = INT_MAX;
-  for (int i = lo + tid; i < hi; i += THREADS) {
-    const float x = tidy(logit<TYPE>(A.logits, base + i));
-    if (x > top || arg == INT_MAX) {
-      top = x;
-      arg = i;
+  const int64_t base = row * A.row_stride + A.skew;
+  float top, sum = 0.f;
+  int arg = 0;
+  if (temp > 0.f) {
+    const float inv_t = inverse(temp), c2 = inv_t * LOG2E;
+    float mine, part;
+    sum_segment<TYPE>(A, base, lo, hi, c2, mine, part);
+    top = block_max(mine, red);
+    sum = block_sum(part * exp2_fast((mine - top) * c2), red);
+    if (!(sum > 0.f && sum < INFINITY)) {
+      // Something that is no number, or nothing above the start of the maximum.
+      float m = -INFINITY;
+      for (int i = lo + threadIdx.x; i < hi; i += THREADS)
+        m = fmaxf(m, tidy(logit<TYPE>(A.logits, base + i)));
+      top = block_max(m, red);
+      float p = 0.f;
+      for (int i = lo + threadIdx.x; i < hi; i += THREADS)
+        p += weight(tidy(logit<TYPE>(A.logits, base + i)), top, inv_t);
+      sum = block_sum(p, red);
     }
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    const float y = __shfl_xor_sync(0xffffffffu, top, o);
-    const int j = __shfl_xor_sync(0xffffffffu, arg, o);
-    if (y > top || (y == top && j < arg)) {
-      top = y;
-      arg = j;
+  } else {
+    best_segment<TYPE>(A, base, lo, hi, top, arg);
+    for (int o = 16; o > 0; o >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, top, o);
+      const int j = __shfl_xor_sync(0xffffffffu, arg, o);
+      if (y > top || (y == top && j < arg)) {
+        top = y;
+        arg = j;
+      }
     }
-  }
-  if (lane == 0) {
-    s_a[warp] = top;
-    s_i[warp] = arg;
-  }
-  __syncthreads();
-  top = s_a[0];
-  arg = s_i[0];
-  for (int w = 1; w < THREADS / 32; ++w)
-    if (s_a[w] > top || (s_a[w] == top && s_i[w] < arg)) {
-      top = s_a[w];
-      arg = s_i[w];
+    if ((threadIdx.x & 31) == 0) {
+      s_top[threadIdx.x >> 5] = top;
+      s_arg[threadIdx.x >> 5] = arg;
     }
-  float sum = 0.f;
-  if (temp > 0.f)
-    for (int i = lo + tid; i < hi; i += THREADS)
-      sum += weight(tidy(logit<TYPE>(A.logits, base + i)), top, inv_t);
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) s_b[warp] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    float s = 0.f;
-    for (int w = 0; w < THREADS / 32; ++w) s += s_b[w];
-    A.stats[row * A.segments + seg] = Stat{top, s, arg, 0};
+    __syncthreads();
+    top = s_top[0];
+    arg = s_arg[0];
+    for (int w = 1; w < THREADS / 32; ++w)
+      if (s_top[w] > top || (s_top[w] == top && s_arg[w] < arg)) {
+        top = s_top[w];
+        arg = s_arg[w];
+      }
   }
+  if (threadIdx.x == 0) A.stats[row * A.segments + seg] = Stat{top, sum, arg, 0};
 }
 
-// Joins two keys of the race: (class, value, lowest index).  Class 1: a
-// weight is left; class 0: nothing is left and the row's own p stands in.
-__device__ __forceinline__ unsigned long long race_key(float left, float p, float e, int i) {
-  const bool some = left > 0.f;
-  const float v = (some ? left : p) / e;
-  const uint32_t bits = __float_as_uint(fmaxf(v, 0.f));
-  return ((unsigned long long)some << 63) | ((unsigned long long)bits << 32) |
+// A key of the race: the value, then the lowest index.
+__device__ __forceinline__ unsigned long long race_key(float v, int i) {
+  return ((unsigned long long)__float_as_uint(v) << 32) |
          (unsigned long long)(0xffffffffu - (uint32_t)i);
 }
 
@@ -175,7 +328,8 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Args A) {
   __shared__ int s_arg[MAX_TOKENS], s_par[MAX_TOKENS], s_lost[MAX_TOKENS], s_path[MAX_TOKENS];
   __shared__ int64_t s_tok[MAX_TOKENS];
   __shared__ int s_cur, s_count, s_nlost, s_refused;
-  __shared__ unsigned long long s_best[THREADS / 32];
+  __shared__ unsigned long long s_best[THREADS / 32], s_won;
+  __shared__ bool s_last;
   const int b = blockIdx.y, part = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
@@ -198,20 +352,30 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Args A) {
   const float temp = A.temps[b];
   const float inv_t = inverse(temp);
   const bool greedy = !(temp > 0.f);
-  for (int t = tid; t < n; t += THREADS) {
-    const Stat* st = A.stats + (first + t) * A.segments;
-    float top = st[0].top;
-    int arg = st[0].arg;
-    for (int s = 1; s < A.segments; ++s)
-      if (st[s].top > top) {
-        top = st[s].top;
-        arg = st[s].arg;
+  // A warp joins the segments of a row, a lane each.
+  static_assert(MAX_SEGMENTS <= 32, "a lane for each segment");
+  for (int t = warp; t < n; t += THREADS / 32) {
+    Stat st = {-INFINITY, 0.f, INT_MAX, 0};
+    if (lane < A.segments) st = A.stats[(first + t) * A.segments + lane];
+    float top = st.top;
+    int arg = st.arg;
+    for (int o = 16; o > 0; o >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, top, o);
+      const int j = __shfl_xor_sync(0xffffffffu, arg, o);
+      if (y > top || (y == top && j < arg)) {
+        top = y;
+        arg = j;
       }
-    float sum = 0.f;
-    for (int s = 0; s < A.segments; ++s) sum += st[s].sum * weight(st[s].top, top, inv_t);
-    s_top[t] = top;
-    s_sum[t] = sum;
-    s_arg[t] = arg;
+    }
+    float sum = st.sum * weight(st.top, top, inv_t);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      s_top[t] = top;
+      s_sum[t] = sum;
+      s_arg[t] = arg;
+    }
+  }
+  for (int t = tid; t < n; t += THREADS) {
     int up = t == 0 ? -1 : (A.parents ? A.parents[first + t] : t - 1);
     const int64_t x = A.tokens[first + t];
     if (t > 0 && (up < 0 || up >= t || x < 0 || x >= A.V)) {
@@ -228,7 +392,8 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Args A) {
     const int up = s_par[t];
     float p = 0.f;
     if (up >= 0 && !greedy)
-      p = weight(tidy(logit<TYPE>(A.logits, (first + up) * A.row_stride + s_tok[t])), s_top[up],
+      p = weight(tidy(logit<TYPE>(A.logits, (first + up) * A.row_stride + A.skew +
+                                                    s_tok[t])), s_top[up],
                  inv_t) / s_sum[up];
     s_px[t] = p;
   }
@@ -266,58 +431,131 @@ __global__ void __launch_bounds__(THREADS) pick_kernel(const Args A) {
     s_refused = refused;
   }
   __syncthreads();
-  const int cur = s_cur, count = s_count, nlost = s_nlost;
+  const int cur = s_cur, taken = s_count, nlost = s_nlost;
   if (part == 0) {
     for (int i = tid; i < A.most; i += THREADS) {
-      path[i] = i <= count ? s_path[i] : -1;
-      if (i != count) out[i] = i < count ? s_tok[s_path[i + 1]] : -1;
+      path[i] = i <= taken ? s_path[i] : -1;
+      if (i != taken) out[i] = i < taken ? s_tok[s_path[i + 1]] : -1;
     }
     if (tid == 0) {
-      A.accepted[b] = count;
-      if (greedy) out[count] = s_arg[cur];
+      A.accepted[b] = taken;
+      if (greedy) out[taken] = s_arg[cur];
     }
   }
   if (greedy) return;
   const float* q = A.probs && s_refused >= 0 ? A.probs + (first + s_refused) * A.probs_stride
                                              : nullptr;
   const float* noise = A.noise + (int64_t)b * A.noise_stride;
-  const int64_t base = (first + cur) * A.row_stride;
-  const float top = s_top[cur], sum = s_sum[cur];
+  const int64_t base = (first + cur) * A.row_stride + A.skew;
+  const float top = s_top[cur], c2 = inv_t * LOG2E;
+  const float share = q ? 1.0f / s_sum[cur] : 1.0f;
   const int lo = (int)((int64_t)A.V * part / A.parts);
   const int hi = (int)((int64_t)A.V * (part + 1) / A.parts);
-  unsigned long long best = 0;
-  for (int i = lo + tid; i < hi; i += THREADS) {
-    const float p = weight(tidy(logit<TYPE>(A.logits, base + i)), top, inv_t) / sum;
-    float left = q ? fmaxf(p - q[i], 0.f) : p;
-    if (!A.probs)
-      for (int j = 0; j < nlost; ++j)
-        if (s_lost[j] == i) left = 0.f;
-    const unsigned long long key = race_key(left, p, noise[i], i);
-    if (key > best) best = key;
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-    if (other > best) best = other;
-  }
-  if (lane == 0) s_best[warp] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < THREADS / 32; ++w)
-      if (s_best[w] > best) best = s_best[w];
-    atomicMax(&A.race[b].best, best);
-    __threadfence();
-    if (atomicAdd(&A.race[b].arrived, 1) == A.parts - 1) {
-      const unsigned long long won = atomicExch(&A.race[b].best, 0ull);
-      A.race[b].arrived = 0;
-      out[count] = (int64_t)(0xffffffffu - (uint32_t)won);
+  float best = 0.f;
+  int arg = -1;
+  // Strictly larger wins, so equal values go to the lower index.  Without draft
+  // probabilities the sum of the weights does not matter; the refused tokens are
+  // looked up for a new best only.
+  auto take = [&](float x, float e, float qi, int i) {
+    // Not-a-number loses every comparison, as does a row of nothing but -infinity.
+    const float v = __fdividef(exp2_fast((x - top) * c2) * share - qi, e);
+    if (v > best) {
+      bool lost = false;
+      if (!A.probs)
+        for (int j = 0; j < nlost; ++j) lost = lost || s_lost[j] == i;
+      if (!lost) {
+        best = v;
+        arg = i;
+      }
+    }
+  };
+  constexpr int P = PIECE<TYPE>;
+  int start, count;
+  whole_pieces<TYPE>(base, lo, hi, start, count);
+  for (int i = lo + tid; i < start; i += THREADS)
+    take(logit<TYPE>(A.logits, base + i), noise[i], q ? q[i] : 0.f, i);
+  const bool wide = ((uintptr_t)(noise + start) & 15) == 0 && (!q || ((uintptr_t)(q + start) & 15) == 0);
+  constexpr int BATCH = 2;
+  for (int i0 = tid; i0 < count; i0 += THREADS * BATCH) {
+    uint4 v[BATCH];
+    float e[BATCH][P], qv[BATCH][P];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = min(i0 + u * THREADS, count - 1);
+      const int at = start + i * P;
+      v[u] = piece<TYPE>(A.logits, base + at);
+#pragma unroll
+      for (int j = 0; j < P; j += 4) {
+        if (wide) {
+          *reinterpret_cast<uint4*>(&e[u][j]) = ldg_stream_v4(noise + at + j);
+          if (q) *reinterpret_cast<uint4*>(&qv[u][j]) = ldg_stream_v4(q + at + j);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            e[u][j + k] = noise[at + j + k];
+            if (q) qv[u][j + k] = q[at + j + k];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * THREADS;
+      if (i >= count) break;
+      float x[P];
+      unpack<TYPE>(v[u], x);
+#pragma unroll
+      for (int j = 0; j < P; ++j) take(x[j], e[u][j], q ? qv[u][j] : 0.f, start + i * P + j);
     }
   }
+  for (int i = start + count * P + tid; i < hi; i += THREADS)
+    take(logit<TYPE>(A.logits, base + i), noise[i], q ? q[i] : 0.f, i);
+  unsigned long long key = arg < 0 ? 0 : race_key(best, arg);
+  auto join = [&]() {
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+      if (other > key) key = other;
+    }
+    if (lane == 0) s_best[warp] = key;
+    __syncthreads();
+    for (int w = 0; w < THREADS / 32; ++w)
+      if (s_best[w] > key) key = s_best[w];
+  };
+  join();
+  if (tid == 0) {
+    atomicMax(&A.race[b].best, key);
+    __threadfence();
+    s_last = atomicAdd(&A.race[b].arrived, 1) == A.parts - 1;
+    if (s_last) {
+      s_won = atomicExch(&A.race[b].best, 0ull);
+      A.race[b].arrived = 0;
+    }
+  }
+  __syncthreads();
+  if (!s_last) return;
+  key = s_won;
+  if (key == 0) {
+    // Nothing is left by rounding: the row's own p, from the first token on.
+    float v = -1.f;
+    int at = INT_MAX;
+    for (int i = tid; i < A.V; i += THREADS) {
+      const float w = weight(tidy(logit<TYPE>(A.logits, base + i)), top, inv_t) / noise[i];
+      if (w > v) {
+        v = w;
+        at = i;
+      }
+    }
+    key = at == INT_MAX ? 0 : race_key(v, at);
+    join();
+  }
+  if (tid == 0) out[taken] = (int64_t)(0xffffffffu - (uint32_t)key);
 }
 
-// Segments of a row and CTAs of a request: enough CTAs to fill the GPU.
+// Segments of a row and CTAs of a request: enough CTAs (16 an SM, of at least
+// 4096 elements) that the last ones to run do not leave most SMs idle.
 static void split(int64_t B, int64_t most, int64_t V, int sms, int* segments, int* parts) {
   auto pick = [&](int64_t units) {
-    int64_t s = (2 * (int64_t)sms + units - 1) / units;
+    int64_t s = (16 * (int64_t)sms + units - 1) / units;
     const int64_t by_size = (V + 4095) / 4096;
     if (s > by_size) s = by_size;
     if (s > MAX_SEGMENTS) s = MAX_SEGMENTS;
@@ -377,7 +615,11 @@ extern "C" int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t 
              need, workspace_bytes);
   const int dev = kb::bind_stream_device(stream);
   v::Args A = {};
-  A.logits = logits;
+  const int size = dtype == v::F32 ? 4 : 2;
+  KB_REQUIRE(rows == 0 || (uintptr_t)logits % size == 0, KB_ERR_ALIGNMENT,
+             "verify: logits must be aligned to their elements");
+  A.skew = (int64_t)((uintptr_t)logits & 15) / size;
+  A.logits = static_cast<const uint8_t*>(logits) - A.skew * size;
   A.row_stride = row_stride;
   A.rows = rows;
   A.V = (int)V;

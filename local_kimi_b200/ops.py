@@ -1019,12 +1019,12 @@ def paged_plan(
     par = mask = None
     if parents is not None:
         par = _vector(parents, torch.int32, "parents", device, num_tokens)
-        mask = torch.empty((num_tokens,), dtype=torch.long, device=device)
-    cu = torch.empty((requests + 1,), dtype=torch.int32, device=device)
-    slots = torch.empty((num_tokens,), dtype=torch.long, device=device)
-    positions = torch.empty((num_tokens,), dtype=torch.int32, device=device)
-    head_out = torch.empty((1,), dtype=torch.int32, device=device)
-    missing = torch.empty((1,), dtype=torch.int32, device=device)
+        mask = torch.empty(num_tokens, dtype=torch.long, device=device)
+    cu = torch.empty(requests + 1, dtype=torch.int32, device=device)
+    slots = torch.empty(num_tokens, dtype=torch.long, device=device)
+    positions = torch.empty(num_tokens, dtype=torch.int32, device=device)
+    head_out = torch.empty(1, dtype=torch.int32, device=device)
+    missing = torch.empty(1, dtype=torch.int32, device=device)
     _lib.call(
         "kb_paged_plan", ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
         max(block_table.stride(0), width), width, free.data_ptr(), free.shape[0],
@@ -1168,8 +1168,8 @@ def prompt_attention(
         ck = _vector(cu_seqlens_k, torch.int32, "cu_seqlens_k", device, requests + 1)
     if max_seqlen < 0 or (total and not max_seqlen):
         raise ValueError("max_seqlen must not be negative, nor 0 with tokens")
-    out = torch.empty((total, hq, dv), dtype=q.dtype, device=device)
-    lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
+    out = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
+    lse = torch.empty(total, hq, dtype=torch.float32, device=device) if return_lse else None
     _lib.call(
         "kb_prompt_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), kr.data_ptr(),
         kr.stride(0), kr.stride(1), vr.data_ptr(), vr.stride(0), vr.stride(1),
@@ -1237,8 +1237,8 @@ def tree_attention(
         if max_tokens > MAX_TREE_TOKENS:
             raise ValueError(f"a masked tree has at most {MAX_TREE_TOKENS} tokens")
         mask = _vector(tree_mask, torch.long, "tree_mask", device, total)
-    out = torch.empty((total, hq, dv), dtype=q.dtype, device=device)
-    lse = torch.empty((total, hq), dtype=torch.float32, device=device) if return_lse else None
+    out = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
+    lse = torch.empty(total, hq, dtype=torch.float32, device=device) if return_lse else None
     if total == 0 or requests == 0:
         return out if lse is None else (out, lse)
     stream = _raw_stream(device)
@@ -1308,9 +1308,9 @@ def verify_drafts(
         if draft_probs.shape != (rows, vocab) or draft_probs.device != device:
             raise ValueError("draft_probs must have the shape and device of the logits")
         probs = _unit_rows(draft_probs)
-    out = torch.empty((requests, max_tokens), dtype=torch.long, device=device)
-    path = torch.empty((requests, max_tokens), dtype=torch.int32, device=device)
-    accepted = torch.empty((requests,), dtype=torch.int32, device=device)
+    out = torch.empty(requests, max_tokens, dtype=torch.long, device=device)
+    path = torch.empty(requests, max_tokens, dtype=torch.int32, device=device)
+    accepted = torch.empty(requests, dtype=torch.int32, device=device)
     if requests == 0:
         return Verification(out, path, accepted)
     x, e = _unit_rows(logits), _unit_rows(noise)
