@@ -9,7 +9,7 @@
 
 #include <mutex>
 
-#include "kb_common.cuh"
+#include "kb_math.cuh"
 
 namespace kb {
 namespace attn {
@@ -18,7 +18,6 @@ constexpr uint32_t ERR_WAIT = 2u;               // bounded wait ran out (device 
 constexpr long long WAIT_NS = 2000000000LL;
 constexpr long long DRAIN_NS = 200000000LL;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ long long now_ns() {
   long long t;
@@ -55,12 +54,6 @@ __device__ __forceinline__ void drain_phase(uint64_t* bar, uint32_t parity) {
   const long long t0 = now_ns();
   while (!mbar_try_wait(bar, parity))
     if (now_ns() - t0 > DRAIN_NS) return;
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Two fp32 values rounded to a pair of 16-bit elements, `lo` in the low half.

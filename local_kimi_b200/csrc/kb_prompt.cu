@@ -140,29 +140,6 @@ struct Walk {
 };
 constexpr int WALKERS = 8 + 3;               // softmax warps, two of MMAs, cleaning
 
-__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
-        "l"(*reinterpret_cast<uint64_t*>(&c)));
-  return *reinterpret_cast<float2*>(&d);
-}
-
-__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // 2^x for a pair of x <= 64 on the FMA pipes: x = n + f with n the nearest
 // whole number (left in the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a
 // polynomial of degree 4 fitted here to least relative error (2.7e-6, and
@@ -775,7 +752,7 @@ extern "C" int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride,
   A.Dk = (int)Dk;
   A.Dv = (int)Dv;
   while (A.pack_shift < 7 && A.g % (2 << A.pack_shift) == 0) ++A.pack_shift;
-  A.scale2 = scale * at::LOG2E;
+  A.scale2 = scale * kb::LOG2E;
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
   const int pack = 1 << A.pack_shift;

@@ -879,7 +879,7 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   A.g = (int)(Hq / Hkv);
   A.Dk = (int)Dk;
   A.Dv = (int)Dv;
-  A.scale2 = scale * at::LOG2E;
+  A.scale2 = scale * kb::LOG2E;
   const int mt = at::row_tiles(max_tokens * A.g);
   A.counters = static_cast<int*>(workspace);
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at::COUNTER_BYTES);
