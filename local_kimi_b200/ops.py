@@ -924,6 +924,8 @@ def quantise(weight: torch.Tensor, group_size: int = 128) -> tuple[torch.Tensor,
 # ---------------------------------------------------------------------------
 
 _ELEMENT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_HALF = (torch.bfloat16, torch.float16)
+_STRIDES = c_int64 * 3
 MAX_TREE_TOKENS = 64
 
 
@@ -949,6 +951,9 @@ class Verification(NamedTuple):
 def _vector(t: torch.Tensor, dtype: torch.dtype, what: str, device: torch.device,
             length: int | None = None) -> torch.Tensor:
     """A 1-D contiguous tensor of a type, length and device."""
+    if (t.dtype == dtype and t.dim() == 1 and t.device == device and t.is_contiguous()
+            and (length is None or t.numel() == length)):
+        return t
     if t.dtype != dtype or t.dim() != 1:
         raise TypeError(f"{what} must be a one-dimensional {dtype} tensor")
     if length is not None and t.numel() != length:
@@ -1016,15 +1021,16 @@ def paged_plan(
         raise ValueError("block_table is updated in place and needs rows of unit stride")
     if page_size <= 0 or num_tokens < 0:
         raise ValueError("page_size must be positive and num_tokens not negative")
+    # The outputs are parts of two buffers: six allocations would take longer
+    # than the kernel.
+    ints = torch.empty(requests + num_tokens + 3, dtype=torch.int32, device=device)
+    head_out, missing, cu, positions = ints.split_with_sizes((1, 1, requests + 1, num_tokens))
     par = mask = None
-    if parents is not None:
+    if parents is None:
+        slots = torch.empty(num_tokens, dtype=torch.long, device=device)
+    else:
         par = _vector(parents, torch.int32, "parents", device, num_tokens)
-        mask = torch.empty(num_tokens, dtype=torch.long, device=device)
-    cu = torch.empty(requests + 1, dtype=torch.int32, device=device)
-    slots = torch.empty(num_tokens, dtype=torch.long, device=device)
-    positions = torch.empty(num_tokens, dtype=torch.int32, device=device)
-    head_out = torch.empty(1, dtype=torch.int32, device=device)
-    missing = torch.empty(1, dtype=torch.int32, device=device)
+        slots, mask = torch.empty(2, num_tokens, dtype=torch.long, device=device).unbind()
     _lib.call(
         "kb_paged_plan", ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
         max(block_table.stride(0), width), width, free.data_ptr(), free.shape[0],
@@ -1041,7 +1047,7 @@ def _rows_of_heads(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.ndim != 3:
         raise ValueError(f"{what} must have shape [tokens, heads, width]")
     s = t.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+    if s[2] != 1 or (s[0] | s[1]) & 7 or t.data_ptr() & 15:
         t = t.contiguous()
     return t
 
@@ -1051,10 +1057,10 @@ def _cache_strides(t: torch.Tensor, what: str) -> object:
     if t.ndim != 4:
         raise ValueError(f"{what} must have shape [pages, page_size, heads, width]")
     s = t.stride()
-    if t.numel() and (s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8 or t.data_ptr() % 16):
+    if (s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or t.data_ptr() & 15) and t.numel():
         raise ValueError(f"{what} needs unit stride along the width, other strides multiples "
                          "of 8 and a 16-byte aligned start")
-    return (c_int64 * 3)(s[0], s[1], s[2])
+    return _STRIDES(s[0], s[1], s[2])
 
 
 def _check_widths(dk: int, dv: int) -> None:
@@ -1076,9 +1082,10 @@ def paged_append(
     at page ``slot // page_size``, row ``slot % page_size``; a negative slot
     is skipped.  No two tokens may name one slot.
     """
-    if k.dtype not in (torch.bfloat16, torch.float16):
+    dtype = k.dtype
+    if dtype not in _HALF:
         raise TypeError("keys and values must be BF16 or FP16")
-    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+    if not (dtype == v.dtype == k_cache.dtype == v_cache.dtype):
         raise TypeError("keys, values and caches must share one type")
     _require_cuda(k, "paged append")
     device = k.device
