@@ -1,9 +1,11 @@
-// kb_prompt.cu - causal attention over packed prompts on the 5th-generation
-// tensor cores.
+// kb_prompt.cu - causal attention over packed prompts, and attention of many
+// rows (drafted trees, grouped heads) over the paged cache, on the
+// 5th-generation tensor cores.
 //
 //   o_i = sum_j exp(s_ij - m_i) v_j / l_i,  s_ij = scale * q_i . k_j over the visible j,
 //   m_i = max_j s_ij, l_i = sum_j exp(s_ij - m_i), lse_i = m_i + log(l_i)
-// visible: j <= i + (Lk - Lq).  A row that sees no key gives 0 and lse -infinity.
+// visible: j <= i + (Lk - Lq), or the token's tree word (kb_tree.cu).  A row that
+// sees no key gives 0 and lse -infinity.
 //
 // One persistent CTA per SM.  A unit is 256 rows of one request, two tiles A
 // and B of 128, against all the keys they see, 64 a step.  The heads of a
@@ -41,6 +43,14 @@
 // 3600 and 4430 measured.  The exponentials (16 a clock and SM) would take
 // 2048; one pair in POLY_EVERY goes to the FMA pipes.
 //
+// Paged cache (PAGED).  A unit is up to 256 rows (token * group + head) of one
+// request and key/value head, against the cache in 64-key steps; with few rows
+// tile B is idle and the bytes of the cache bound the work.  All units' steps
+// form one line cut into equal runs, one per CTA, as in kb_tree.cu; a unit that
+// falls to several CTAs is joined from fp32 partial sums by the CTA that finishes
+// last.  Keys and values come page by page, q by gathered 16-byte copies into the
+// same swizzled layout.
+//
 // In the last tiles of a unit some rows do not see some keys, or the tile
 // reaches past the request's end into its neighbour.  A value there that is
 // infinite or not a number must not meet a zero weight: warp 11 zeroes such
@@ -49,7 +59,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "kb_attn.cuh"
+#include "kb_runs.cuh"
 #include "kb_tcgen05.cuh"
 
 namespace kb {
@@ -77,6 +87,18 @@ struct PromptArgs {
   int blocks;               // 256-row units of the longest request
   float scale2;             // scale * log2(e)
   uint32_t* err;
+  // Paged: k and v are the caches, k_tok and v_tok the strides of a page's rows.
+  const int* table;
+  int64_t table_stride;
+  const int* context;
+  const int64_t* mask;      // NULL: causal
+  int64_t n_pages, v_page;
+  int width, ps, Hkv;
+  int most;                 // tokens of a request at most
+  int* counters;            // [2 * CTAs], zero between calls
+  int part_rows;            // rows of a unit: 128 or 256
+  float* part_ml;           // [2 * CTAs][part_rows][2]: m (log2), l
+  float* part_o;            // [2 * CTAs][part_rows][DVP]
 };
 
 template <int DKP, int DVP>
@@ -85,7 +107,7 @@ struct PromptShape {
   static constexpr int VC = DVP / 64;                    // ... and values
   static constexpr int Q_TILE = 2 * KC * BLOCK;          // bytes of a Q tile (128 rows)
   static constexpr int STAGE = (KC + VC) * BLOCK;
-  static constexpr int FIXED = 1024 + 1024;              // alignment, barriers
+  static constexpr int FIXED = 1024 + 1536;              // alignment, barriers
   static constexpr int FIT = (227 * 1024 - FIXED - 2 * Q_TILE) / STAGE;
   static constexpr int STAGES = FIT > MAX_STAGES ? MAX_STAGES : FIT;
   static constexpr int SMEM = FIXED + 2 * Q_TILE + STAGES * STAGE;
@@ -97,11 +119,15 @@ struct Unit {
   int q0, k0;               // first query and key of the request
   int n, m;                 // its queries and keys
   int head0;                // first head
-  int t0;                   // first token of tile A
+  int t0;                   // first token of tile A (paged: first row)
   int steps[2];             // steps of keys that tiles A and B see
   int whole;                // of them, those that every row of A sees whole
   int count;                // number of the unit in this CTA, -1: the end
+  // Paged: the request, the run's first step of the unit, the steps this CTA had
+  // before; whether the run has all steps, or the first; the CTAs that share it.
+  int b, j0, base, all, starts, c0, parts;
 };
+constexpr int SEEN = 16;                   // steps whose key words are kept
 
 struct PromptBars {
   uint64_t full[MAX_STAGES], empty[MAX_STAGES];
@@ -113,10 +139,14 @@ struct PromptBars {
   uint64_t drain;
   Unit unit[UNITS];
   int odd[16];              // units that had odd elements, by their number's last four bits
+  uint64_t valid[SEEN];     // paged: which keys of a step exist, by the CTA's count of steps
+  uint64_t meet[2];         // paged: a tile's softmax warps together
+  int joined[2];
+  RunStart start;
   uint32_t tmem;
   int abort_flag;
 };
-static_assert(sizeof(PromptBars) <= 1024, "barrier block");
+static_assert(sizeof(PromptBars) <= 1536, "barrier block");
 
 // A warp's way through the CTA's units.
 struct Walk {
@@ -165,15 +195,23 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // Adds to a row's outputs d0..d0+31 the values that are no numbers of the keys
 // [first, last]: they were kept out of the tile products.
 template <bool F16>
-__device__ __forceinline__ void add_odd(const PromptArgs& A, const uint16_t* v, int first,
-                                        int last, int d0, float (&o)[32]) {
-  for (int64_t j = first; j <= last; ++j) {
+__device__ __forceinline__ void add_odd(const PromptArgs& A, const uint16_t* v, int d0,
+                                        float (&o)[32]) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const uint16_t u = d0 + i < A.Dv ? v[j * A.v_tok + d0 + i] : 0;
-      if (odd_element<F16>(u)) o[i] += element<F16>(u);
-    }
+  for (int i = 0; i < 32; ++i) {
+    const uint16_t u = d0 + i < A.Dv ? v[d0 + i] : 0;
+    if (odd_element<F16>(u)) o[i] += element<F16>(u);
   }
+}
+
+// Which of 64 keys from `key` on a row sees: those up to `limit`, or (word) the
+// context and the tree's bits.
+__device__ __forceinline__ uint64_t low_bits(int n) {
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
+}
+__device__ __forceinline__ uint64_t tree_bits(uint64_t word, int ctx, int key) {
+  const int d = ctx - key;
+  return d >= 64 ? ~0ull : d >= 0 ? low_bits(d) | (word << d) : d > -64 ? word >> -d : 0ull;
 }
 
 // Half of a transposition: lanes `step` apart keep one piece and swap the other.
@@ -186,7 +224,65 @@ __device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int upper, int s
   if (upper) a = give; else b = give;
 }
 
-template <int DKP, int DVP, bool F16>
+// Sums of the rows of a tile whose keys several CTAs had: a thread takes 16
+// values of a row, four parts at a time.
+template <int DVP, bool F16>
+__device__ __forceinline__ void join_parts(const PromptArgs& A, const Unit& U, int tile,
+                                           int thread) {
+  const int rows = min(TILE, U.n * A.g - U.t0 - tile * TILE);
+  constexpr int GROUPS = DVP / 16, BATCH = 2;
+  for (int it = thread; it < rows * GROUPS; it += TILE) {
+    const int r = it / GROUPS, d = (it - r * GROUPS) * 16;
+    float top = -INFINITY, sum = 0.f, o[16] = {};
+    for (int c = 0; c < U.parts; c += BATCH) {
+      float2 ml[BATCH];
+      float4 v[BATCH][4];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int cc = min(c + u, U.parts - 1);
+        const int64_t at = ((int64_t)(U.c0 + cc) * 2 + (cc == 0)) * A.part_rows + tile * TILE + r;
+        ml[u] = __ldcg(reinterpret_cast<const float2*>(A.part_ml + at * 2));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[u][k] = __ldcg(reinterpret_cast<const float4*>(A.part_o + at * DVP + d + 4 * k));
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const float t = fmaxf(top, ml[u].x);
+        if (c + u >= U.parts || t == -INFINITY) continue;
+        const float f0 = exp2_fast(top - t), f1 = exp2_fast(ml[u].x - t);
+        top = t;
+        sum = sum * f0 + ml[u].y * f1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[4 * k] = o[4 * k] * f0 + v[u][k].x * f1;
+          o[4 * k + 1] = o[4 * k + 1] * f0 + v[u][k].y * f1;
+          o[4 * k + 2] = o[4 * k + 2] * f0 + v[u][k].z * f1;
+          o[4 * k + 3] = o[4 * k + 3] * f0 + v[u][k].w * f1;
+        }
+      }
+    }
+    const int at_row = U.t0 + tile * TILE + r, t = at_row / A.g;
+    const int64_t at = (int64_t)(U.q0 + t) * A.Hq + U.head0 + at_row - t * A.g;
+    const bool none = sum == 0.f;
+    const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 16; k += 8)
+      if (d + k < A.Dv) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (!none) {
+          w.x = pack2<F16>(o[k] * inv, o[k + 1] * inv);
+          w.y = pack2<F16>(o[k + 2] * inv, o[k + 3] * inv);
+          w.z = pack2<F16>(o[k + 4] * inv, o[k + 5] * inv);
+          w.w = pack2<F16>(o[k + 6] * inv, o[k + 7] * inv);
+        }
+        *reinterpret_cast<uint4*>(A.out + at * A.Dv + d + k) = w;
+      }
+    if (A.lse && d == 0) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
+  }
+}
+
+template <int DKP, int DVP, bool F16, bool PAGED>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                   const __grid_constant__ CUtensorMap tv, const PromptArgs A) {
@@ -208,7 +304,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       mbar_init(&B->clean[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&B->q_full[i], 1);
+      mbar_init(&B->q_full[i], PAGED ? 32 : 1);
+      mbar_init(&B->meet[i], 4);
       mbar_init(&B->q_empty[i], 1);
       mbar_init(&B->o_near[i], 1);
       mbar_init(&B->o_full[i], 1);
@@ -225,17 +322,27 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     mbar_init(&B->drain, 2);
     B->abort_flag = 0;
     mbar_fence_init();
-    prefetch_map(&tq);
+    if (!PAGED) prefetch_map(&tq);
     prefetch_map(&tk);
     prefetch_map(&tv);
   }
   if (warp == CLEAN_WARP) tc::tmem_alloc_all(&B->tmem);
+  // Columns of q past the head's width stay zero (the gather does not write them).
+  if (PAGED && A.Dk < DKP) {
+    for (int i = threadIdx.x; i < 2 * S::Q_TILE / 16; i += PROMPT_THREADS)
+      reinterpret_cast<uint4*>(qs)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+  }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = B->tmem;
   pdl_wait();
   pdl_launch_dependents();
+  Run run = {};
+  if (PAGED)
+    run = find_run<2 * TILE, PROMPT_THREADS>(A.cu_q, A.context, A.total_q, A.B, A.g, A.Hkv,
+                                             A.most, &B->start);
 
   // Rows outside every request: zero.
   {
@@ -262,16 +369,23 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     const float scale2 = A.scale2;
     const int span = TILE >> A.pack_shift;
     int buf = 0;                          // the next step's S buffer
-    uint32_t s_phase = 0, near_phase = 0, end_phase = 0;
+    uint32_t s_phase = 0, near_phase = 0, end_phase = 0, meet_phase = 0;
     Unit U;
     for (Walk walk(B, A.err); walk.next(U);) {
-      const int first = U.t0 + tile * span;
+      // The row's token and head; keys are limited by `limit`, or in a tree by `word`.
+      const int at_row = U.t0 + tile * TILE + row;          // paged
+      const int first = PAGED ? (U.t0 + tile * TILE) / A.g : U.t0 + tile * span;
       if (first >= U.n) continue;
-      const int tok = first + (row >> A.pack_shift);
-      const int head = U.head0 + (row & ((1 << A.pack_shift) - 1));
+      const int tok = PAGED ? at_row / A.g : first + (row >> A.pack_shift);
+      const int head = U.head0 + (PAGED ? at_row - tok * A.g
+                                        : (row & ((1 << A.pack_shift) - 1)));
       const bool real = tok < U.n;
       const int limit = min(tok, U.n - 1) + U.m - U.n;      // last key the row sees
-      const int clear = first + U.m - U.n;                  // ... and the tile's first row
+      const bool tree = PAGED && A.mask != nullptr;
+      const uint64_t word = tree ? (uint64_t)A.mask[U.q0 + min(tok, U.n - 1)] : 0;
+      // Steps up to this key are seen whole by every row of the tile.
+      const int clear = tree ? U.m - U.n - 1 : first + U.m - U.n;
+      const int j0 = PAGED ? U.j0 : 0;
       float top = -INFINITY, sum = 0.f;                     // in log2 units
       bool ok = true;
       const int steps = U.steps[tile];
@@ -288,14 +402,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         tc::tmem_ld_wait();
         tc::hold_regs(s[0]);
         tc::hold_regs(s[1]);
-        const bool edge = j * STEP + STEP - 1 > clear;     // keys that some rows do not see
+        const int key = (j0 + j) * STEP;
+        uint64_t there = ~0ull;                            // keys that exist
+        if (PAGED) there = *const_cast<volatile uint64_t*>(&B->valid[(U.base + j) & (SEEN - 1)]);
+        const bool edge = key + STEP - 1 > clear || there != ~0ull;   // not seen by all rows
         if (edge) {
-          const int last = limit - j * STEP;
+          const uint64_t seen =
+              there & (tree ? tree_bits(word, U.m - U.n, key) : low_bits(limit - key + 1));
+          const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c * 32 + i > last) s[c][i] = -INFINITY;
+              if (!((half[c] >> i) & 1)) s[c][i] = -INFINITY;
         }
         float mx[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
 #pragma unroll
@@ -377,14 +496,17 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       // The four rows whose pieces this lane stores: four lanes side by side
       // exchange 16-byte pieces, so a store covers 64 bytes of eight rows and not
       // 16 bytes of 32.
+      const bool whole = !PAGED || U.all;
       uint16_t* out[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = (row & ~3) + i, t = first + (r >> A.pack_shift);
-        const int h = U.head0 + (r & ((1 << A.pack_shift) - 1));
+        const int r = (row & ~3) + i, paged_row = U.t0 + tile * TILE + r;
+        const int t = PAGED ? paged_row / A.g : first + (r >> A.pack_shift);
+        const int h = U.head0 + (PAGED ? paged_row - t * A.g : (r & ((1 << A.pack_shift) - 1)));
         out[i] = t < U.n ? A.out + ((int64_t)(U.q0 + t) * A.Hq + h) * A.Dv + (lane & 3) * 8
                          : nullptr;
       }
+      const int64_t part_row = ((int64_t)blockIdx.x * 2 + U.starts) * A.part_rows + tile * TILE;
       if (steps > 1) near_phase ^= 1u;
       bool odd = false;
       if (steps > 0) {
@@ -394,8 +516,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         odd = *const_cast<volatile int*>(&B->odd[U.count & 15]) == U.count;
       }
       // A row that saw no key (or only keys of score -infinity) is zero.
-      const bool none = sum == 0.f || limit < 0;
-      const float inv = none ? 0.f : 1.f / sum;
+      const bool none = sum == 0.f || (!PAGED && limit < 0);
+      const float inv = !whole ? 1.f : none ? 0.f : 1.f / sum;
 #pragma unroll
       for (int c = 0; c < DVP / 32; ++c) {
         float o[32];
@@ -403,9 +525,43 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           tc::tmem_ld32(o_at + c * 32, o);
           tc::tmem_ld_wait();
           tc::hold_regs(o);
-          if (odd)
-            add_odd<F16>(A, A.v + U.k0 * A.v_tok + head / A.g * A.v_head, U.whole * STEP, limit,
-                         c * 32, o);
+          if (odd) {
+            if (PAGED) {
+              for (int key = j0 * STEP; key < min((j0 + steps) * STEP, U.m); ++key) {
+                const int e = key / A.ps;
+                const int id = e < A.width ? A.table[(int64_t)U.b * A.table_stride + e] : -1;
+                const bool sees = tree ? (tree_bits(word, U.m - U.n, key) & 1) != 0 : key <= limit;
+                if (id >= 0 && id < A.n_pages && sees)
+                  add_odd<F16>(A, A.v + id * A.v_page + (key - e * A.ps) * A.v_tok +
+                                      U.head0 / A.g * A.v_head, c * 32, o);
+              }
+            } else {
+              for (int key = U.whole * STEP; key <= limit; ++key)
+                add_odd<F16>(A, A.v + (U.k0 + (int64_t)key) * A.v_tok + head / A.g * A.v_head,
+                             c * 32, o);
+            }
+          }
+        }
+        if (!whole) {
+          // This CTA's share of the sums, 64 bytes of eight rows a store too.
+#pragma unroll
+          for (int i = 0; i < 32; i += 16) {
+            uint4 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = make_uint4(__float_as_uint(o[i + 4 * k]), __float_as_uint(o[i + 4 * k + 1]),
+                                __float_as_uint(o[i + 4 * k + 2]), __float_as_uint(o[i + 4 * k + 3]));
+            swap_pieces(w[0], w[1], lane & 1, 1);
+            swap_pieces(w[2], w[3], lane & 1, 1);
+            swap_pieces(w[0], w[2], lane & 2, 2);
+            swap_pieces(w[1], w[3], lane & 2, 2);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (out[k])
+                *reinterpret_cast<uint4*>(A.part_o + (part_row + (row & ~3) + k) * DVP + c * 32 + i +
+                                          (lane & 3) * 4) = w[k];
+          }
+          continue;
         }
         uint4 w[4];
 #pragma unroll
@@ -426,8 +582,35 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             *reinterpret_cast<uint4*>(out[i] + c * 32) = w[i];
       }
       tc::tc_fence_before();
-      if (real && A.lse) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
-      __syncwarp();
+      if (whole) {
+        if (real && A.lse) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
+        __syncwarp();
+        continue;
+      }
+      if (real)
+        *reinterpret_cast<float2*>(A.part_ml + (part_row + row) * 2) = make_float2(top, sum);
+      // The last of the unit's CTAs joins the tile's sums, in CTA order.
+      auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->meet[tile]);
+        ok = warp_wait(&B->meet[tile], meet_phase, abort_f, A.err);
+        meet_phase ^= 1u;
+        return ok;
+      };
+      __threadfence();
+      if (!meet()) break;
+      if (row == 0) {
+        int* counter = A.counters + U.c0 * 2 + tile;
+        const int old = atomicAdd(counter, 1);
+        B->joined[tile] = old == U.parts - 1;
+        if (old == U.parts - 1) *counter = 0;
+      }
+      if (!meet()) break;
+      if (*const_cast<volatile int*>(&B->joined[tile])) {
+        __threadfence();
+        join_parts<DVP, F16>(A, U, tile, row);
+      }
+      if (!meet()) break;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
@@ -502,6 +685,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             if (j == -2) {
               if (!need(&B->q_full[tile], q_phase)) break;
               q_phase ^= 1u;
+              if (PAGED) fence_proxy_async();      // q came by ordinary copies
             }
             tc::tc_fence_after();
             score();
@@ -543,12 +727,28 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           told ^= 1u;
         }
       };
+      const int box = min(A.ps, STEP), pages = STEP / max(box, 1);      // paged
+      int ids_k = -1, ids_v = -1, have_k = -1, have_v = -1;
       auto copy = [&](const Unit& U) {
         const int steps = max(U.steps[0], U.steps[1]);
         const int hk = U.head0 / A.g;
+        have_k = have_v = -1;
         auto queries = [&](int i) {
           if (U.steps[i] == 0 || !need(&B->q_empty[i], q_phase[i])) return;
           q_phase[i] ^= 1u;
+          if (PAGED) {
+            const int pieces = A.Dk / 8, rows = min(TILE, U.n * A.g - U.t0 - i * TILE);
+            for (int x = lane; x < rows * pieces; x += 32) {
+              const int r = x / pieces, c = x - r * pieces, at = U.t0 + i * TILE + r;
+              const int t = at / A.g;
+              cp_async16(qs + i * S::Q_TILE + (c >> 3) * 2 * BLOCK + r * 128 +
+                             (((c ^ r) & 7) << 4),
+                         A.q + (U.q0 + (int64_t)t) * A.q_tok +
+                             (U.head0 + (int64_t)(at - t * A.g)) * A.q_head + c * 8);
+            }
+            cp_async_arrive_noinc(&B->q_full[i]);
+            return;
+          }
           if (lane != 0) return;
           mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)S::Q_TILE);
           for (int c = 0; c < S::KC; ++c)
@@ -559,7 +759,50 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           if (j == -2) queries(0);
           if (!need(&B->empty[st], ph)) break;
           const bool keys = j + 2 < steps, values = j >= 0;
-          if (lane == 0) {
+          if (PAGED) {
+            unsigned live_k = 0, live_v = 0;
+            int id_k = -1, id_v = -1;
+            if (keys) {
+              id_k = page_ids(A, U.b, U.m, (U.j0 + j + 2) * STEP, ids_k, have_k);
+              live_k = __ballot_sync(0xffffffffu, lane < pages && id_k >= 0);
+              uint64_t there = low_bits(U.m - (U.j0 + j + 2) * STEP);
+              if (live_k != low_bits(pages)) {
+                uint64_t got = 0;
+                for (int i = 0; i < pages; ++i)
+                  if ((live_k >> i) & 1) got |= low_bits(box) << (i * box);
+                if (lane == 0 && (there & ~got)) atomicOr(A.err, ERR_PAGE);
+                there &= got;
+              }
+              if (lane == 0) B->valid[(U.base + j + 2) & (SEEN - 1)] = there;
+            }
+            if (values) {
+              id_v = page_ids(A, U.b, U.m, (U.j0 + j) * STEP, ids_v, have_v);
+              live_v = __ballot_sync(0xffffffffu, lane < pages && id_v >= 0);
+            }
+            uint8_t* at = ring + st * S::STAGE;
+            if (lane == 0)
+              mbar_arrive_expect_tx(&B->full[st], (uint32_t)((__popc(live_k) * S::KC +
+                                                              __popc(live_v) * S::VC) * box * 128));
+            __syncwarp();
+            for (int x0 = 0; x0 < pages * (S::KC + S::VC); x0 += 32) {
+              const int x = x0 + lane;
+              const int i = min(x / (S::KC + S::VC), pages - 1), c = x - i * (S::KC + S::VC);
+              const int k_page = __shfl_sync(0xffffffffu, id_k, i);
+              const int v_page = __shfl_sync(0xffffffffu, id_v, i);
+              if (x >= pages * (S::KC + S::VC)) continue;
+              if (c < S::KC) {
+                if ((live_k >> i) & 1)
+                  tma_load_4d(at + c * BLOCK + i * box * 128, &tk, c * 64,
+                              ((U.j0 + j + 2) * STEP + i * box) & (A.ps - 1), hk, k_page,
+                              &B->full[st], once);
+              } else if ((live_v >> i) & 1) {
+                tma_load_4d(at + c * BLOCK + i * box * 128, &tv, (c - S::KC) * 64,
+                            ((U.j0 + j) * STEP + i * box) & (A.ps - 1), hk, v_page, &B->full[st],
+                            once);
+              }
+            }
+            __syncwarp();
+          } else if (lane == 0) {
             uint8_t* at = ring + st * S::STAGE;
             mbar_arrive_expect_tx(&B->full[st], (uint32_t)(((keys ? S::KC : 0) +
                                                             (values ? S::VC : 0)) * BLOCK));
@@ -579,7 +822,46 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           if (j == -2) queries(1);
         }
       };
-      for (int block = A.blocks - 1; block >= 0 && ok; --block) {
+      if (PAGED && run.lo < run.hi) {
+        // This CTA's run of the line of steps.
+        int64_t pos = run.lo, line = B->start.base;
+        Request R = B->start.r;
+        int b = B->start.b, base = 0;
+        const Lengths L = {A.cu_q, A.context, A.total_q, A.g, A.Hkv, 2 * TILE, A.most};
+        while (pos < run.hi && ok) {
+          const int64_t w = L.length(R);
+          if (pos >= line + w) {
+            line += w;
+            R = L.look(++b);
+            continue;
+          }
+          const RunPart P = run_part(R, pos, line, run);
+          pos = P.until;
+          if (P.t1 <= P.t0) continue;          // the run ends in the unit's start
+          Unit U = {};
+          U.q0 = (int)R.first;
+          U.n = R.n;
+          U.m = (int)(R.ctx + R.n);
+          U.head0 = P.hk * A.g;
+          U.t0 = P.block * 2 * TILE;
+          const int rows = R.n * A.g - U.t0;
+          U.steps[0] = (int)(P.t1 - P.t0);
+          U.steps[1] = rows > TILE ? U.steps[0] : 0;
+          U.whole = max((int)(R.ctx / STEP - P.t0), 0);
+          U.count = count++;
+          U.b = b;
+          U.j0 = (int)P.t0;
+          U.base = base;
+          U.all = P.t0 == 0 && P.t1 == R.tiles;
+          U.starts = P.t0 == 0;
+          U.c0 = P.c0;
+          U.parts = P.parts;
+          base += U.steps[0];
+          tell(U);
+          if (ok) copy(U);
+        }
+      }
+      for (int block = A.blocks - 1; !PAGED && block >= 0 && ok; --block) {
         const int t0 = (block * 2 * TILE) >> A.pack_shift;
         for (int b0 = 0; b0 < A.B && ok; b0 += 32) {
           if (held != b0) {
@@ -645,7 +927,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           // of the ring of the others.
           ok = warp_wait(&B->full[st], ph, abort_f, A.err);
           if (!ok) break;
-          if (j >= 0 && j >= U.whole) {
+          // (Paged: a page outside the cache was not copied, the place holds anything.)
+          if (j >= 0 && (j >= U.whole || (PAGED && *const_cast<volatile uint64_t*>(
+                                              &B->valid[(U.base + j) & (SEEN - 1)]) != ~0ull))) {
             bool any = false;
             uint4* at = reinterpret_cast<uint4*>(ring + st * S::STAGE + S::KC * BLOCK) + lane;
 #pragma unroll 8
@@ -684,17 +968,79 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 // Host.
 // ---------------------------------------------------------------------------
 
-template <int DKP, int DVP, bool F16>
+template <int DKP, int DVP, bool F16, bool PAGED>
 static int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                          const PromptArgs& A, int grid, void* stream) {
   using S = PromptShape<DKP, DVP>;
   static std::mutex mu;
   static bool done[64] = {};
-  const void* fn = reinterpret_cast<const void*>(&prompt_kernel<DKP, DVP, F16>);
+  const void* fn = reinterpret_cast<const void*>(&prompt_kernel<DKP, DVP, F16, PAGED>);
   const int st = allow_smem(fn, S::SMEM, done, mu);
   if (st != KB_OK) return st;
-  return launch(prompt_kernel<DKP, DVP, F16>, dim3(grid), dim3(PROMPT_THREADS), (size_t)S::SMEM,
+  return launch(prompt_kernel<DKP, DVP, F16, PAGED>, dim3(grid), dim3(PROMPT_THREADS), (size_t)S::SMEM,
                 stream, mq, mk, mv, A);
+}
+
+template <bool PAGED>
+static int launch_widths(int64_t Dk, int64_t Dv, int f16, const CUtensorMap& mq,
+                         const CUtensorMap& mk, const CUtensorMap& mv, const PromptArgs& A,
+                         int grid, void* stream) {
+  if (Dk <= 64 && Dv <= 64)
+    return f16 ? launch_prompt<64, 64, true, PAGED>(mq, mk, mv, A, grid, stream)
+               : launch_prompt<64, 64, false, PAGED>(mq, mk, mv, A, grid, stream);
+  if (Dk <= 128)
+    return f16 ? launch_prompt<128, 128, true, PAGED>(mq, mk, mv, A, grid, stream)
+               : launch_prompt<128, 128, false, PAGED>(mq, mk, mv, A, grid, stream);
+  return f16 ? launch_prompt<192, 128, true, PAGED>(mq, mk, mv, A, grid, stream)
+             : launch_prompt<192, 128, false, PAGED>(mq, mk, mv, A, grid, stream);
+}
+
+constexpr int ROW_CTAS = 160;                // CTAs the workspace of the paged form is made for
+constexpr size_t ROW_COUNTERS = 2 * ROW_CTAS * sizeof(int);
+
+// Counters, then two partial sums a CTA: maximum and sum, 128 values, of the 128 or
+// 256 rows of a unit.
+static int part_rows(int64_t rows) { return rows > TILE ? 2 * TILE : TILE; }
+
+size_t rows_workspace(int64_t rows) {
+  return ROW_COUNTERS + (size_t)2 * ROW_CTAS * part_rows(rows) * (2 + 128) * sizeof(float);
+}
+
+int launch_rows(const TreeCall& T, int64_t rows, const CUtensorMap& mk, const CUtensorMap& mv,
+                int sms, void* workspace, void* stream) {
+  PromptArgs A = {};
+  A.q = T.q;
+  A.v = T.v;
+  A.q_tok = T.q_tok;
+  A.q_head = T.q_head;
+  A.v_page = T.v_page;
+  A.v_tok = T.v_row;
+  A.v_head = T.v_head;
+  A.out = T.out;
+  A.lse = T.lse;
+  A.cu_q = T.cu;
+  A.total_q = T.total;
+  A.B = T.B;
+  A.Hq = T.Hq;
+  A.Hkv = T.Hkv;
+  A.g = T.Hq / T.Hkv;
+  A.Dk = T.Dk;
+  A.Dv = T.Dv;
+  A.scale2 = T.scale2;
+  A.err = T.err;
+  A.table = T.table;
+  A.table_stride = T.table_stride;
+  A.context = T.context;
+  A.mask = T.mask;
+  A.n_pages = T.n_pages;
+  A.width = T.width;
+  A.ps = T.ps;
+  A.most = T.most;
+  A.counters = static_cast<int*>(workspace);
+  A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ROW_COUNTERS);
+  A.part_rows = part_rows(rows);
+  A.part_o = A.part_ml + (size_t)2 * ROW_CTAS * A.part_rows * 2;
+  return launch_widths<true>(T.Dk, T.Dv, T.f16, mk, mk, mv, A, std::min(sms, ROW_CTAS), stream);
 }
 
 }  // namespace attn
@@ -774,12 +1120,5 @@ extern "C" int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride,
                        {v_head_stride, v_token_stride, 8}, 1, at::STEP);
   if (st != KB_OK) return st;
   const int grid = (int)std::min<int64_t>(kb::num_sms(dev), units);
-  if (Dk <= 64 && Dv <= 64)
-    return dtype ? at::launch_prompt<64, 64, true>(mq, mk, mv, A, grid, stream)
-                 : at::launch_prompt<64, 64, false>(mq, mk, mv, A, grid, stream);
-  if (Dk <= 128)
-    return dtype ? at::launch_prompt<128, 128, true>(mq, mk, mv, A, grid, stream)
-                 : at::launch_prompt<128, 128, false>(mq, mk, mv, A, grid, stream);
-  return dtype ? at::launch_prompt<192, 128, true>(mq, mk, mv, A, grid, stream)
-               : at::launch_prompt<192, 128, false>(mq, mk, mv, A, grid, stream);
+  return at::launch_widths<false>(Dk, Dv, dtype, mq, mk, mv, A, grid, stream);
 }

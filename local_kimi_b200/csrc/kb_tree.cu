@@ -33,16 +33,13 @@
 // see them take them from the cache.
 #include <algorithm>
 
-#include "kb_attn.cuh"
+#include "kb_runs.cuh"
 
 namespace kb {
 namespace attn {
 
-constexpr int KT = 64;                     // keys of a tile
 constexpr int CHUNK = KT * 128;            // bytes of 64 keys x 64 elements
 constexpr int MAX_CTAS = 320;              // counters in the workspace
-constexpr int MIN_TILES = 2;               // tiles that make another CTA worth its partial sums
-constexpr int UNIT_COST = 1;               // a unit's start and end, in tiles
 
 struct TreeArgs {
   const uint16_t* q;
@@ -58,6 +55,7 @@ struct TreeArgs {
   const int64_t* mask;
   int64_t n_pages, total;
   int B, width, ps, Hq, Hkv, g, Dk, Dv;
+  int most;                 // tokens of a request at most
   float scale2;             // scale * log2(e)
   int* counters;            // [MAX_CTAS], zero between calls
   float* part_ml;           // [2 * CTAs][rows][2]: m (log2), l
@@ -99,19 +97,6 @@ struct TreeShape {
   static_assert(STAGES >= 2, "two tiles in flight at least");
 };
 
-// A request: its rows, context, tiles of KT keys and blocks of rows.
-struct Request {
-  int64_t first, ctx, tiles;
-  int n, blocks;
-};
-
-// The request a run starts in, and where its tiles start on the line.
-struct Start {
-  Request r;
-  int64_t base;
-  int b;
-};
-
 template <int STAGES>
 struct TreeBars {
   uint64_t full[STAGES], empty[STAGES];
@@ -121,25 +106,10 @@ struct TreeBars {
   int64_t key0[STAGES];       // first key of the tile
   int last[STAGES];           // last tile of its segment
   Segment seg[2];
-  int64_t scan[16];
   int odd[2];                 // a value of the segment's step is no number
-  Start start;
+  RunStart start;
   int abort_flag, joined;
 };
-
-// Quotient of non-negative numbers; the 64-bit division takes most of a
-// microsecond of the producer's start.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
-
-// Where run c of n starts on a line of tiles, and the run that holds place x.
-__device__ __forceinline__ int64_t run_start(int64_t tiles, int n, int c) {
-  return quotient(tiles * c, n);
-}
-__device__ __forceinline__ int run_of(int64_t tiles, int n, int64_t x) {
-  return (int)quotient((x + 1) * n - 1, tiles);
-}
 
 template <int DKP, int DVP, int MT, bool F16>
 __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
@@ -185,44 +155,8 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
   pdl_wait();
   pdl_launch_dependents();
 
-  // Tiles of each request and their running sum; the request this run starts in.
-  const int per = (A.B + S::THREADS - 1) / S::THREADS;
-  const int b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
-  // A request's rows, tiles and blocks; a unit counts one tile more than it
-  // has, for the cost of its start and its end.
-  auto look = [&](int b) {
-    Request R;
-    int64_t end;
-    const int ctx = A.context[b];
-    request_rows(A.cu, b, A.total, R.first, end);
-    R.n = (int)(end - R.first);
-    R.ctx = max(ctx, 0);
-    R.tiles = R.n ? (R.ctx + R.n + KT - 1) / KT : 0;
-    R.blocks = (int)(((int64_t)R.n * A.g + S::RB - 1) / S::RB);
-    return R;
-  };
-  auto length = [&](const Request& R) {
-    return R.n ? (R.tiles + UNIT_COST) * R.blocks * A.Hkv : (int64_t)0;
-  };
-  int64_t mine = 0;
-  Request R0 = {};
-  for (int b = b0; b < b1; ++b) {
-    const Request R = look(b);
-    if (b == b0) R0 = R;
-    mine += length(R);
-  }
-  int64_t incl = mine;
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
-  }
-  if (lane == 31) B->scan[warp] = incl;
-  __syncthreads();
-  int64_t excl = incl - mine, total = 0;
-  for (int w = 0; w < S::NW + 1; ++w) {
-    if (w < warp) excl += B->scan[w];
-    total += B->scan[w];
-  }
+  const Run run = find_run<S::RB, S::THREADS>(A.cu, A.context, A.total, A.B, A.g, A.Hkv,
+                                              A.most, &B->start);
   // Rows outside every request: zero.
   {
     const int64_t lead = min(max((int64_t)A.cu[0], (int64_t)0), A.total);
@@ -236,55 +170,34 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       if (A.lse) A.lse[r] = -INFINITY;
     }
   }
-  const int ctas = (int)min((int64_t)gridDim.x, max((total + MIN_TILES - 1) / MIN_TILES,
-                                                    (int64_t)1));
   const int cta = blockIdx.x;
-  if (cta >= ctas || total == 0) return;
-  const int64_t lo = run_start(total, ctas, cta), hi = run_start(total, ctas, cta + 1);
-  if (mine > 0 && excl <= lo && lo < excl + mine) {
-    int64_t at = excl;
-    for (int b = b0; b < b1; ++b) {
-      if (b > b0) R0 = look(b);
-      const int64_t w = length(R0);
-      if (lo < at + w) {
-        B->start.r = R0;
-        B->start.base = at;
-        B->start.b = b;
-        break;
-      }
-      at += w;
-    }
-  }
-  __syncthreads();
+  if (run.lo >= run.hi) return;
 
   if (warp == S::NW) {
     // ---------------------------------------------------------------- producer
     const uint64_t pol = l2_evict_first_policy();
-    const int ps = A.ps, shift = 31 - __clz(ps);
-    const int box = min(ps, KT), ppt = KT / box;
-    int64_t pos = lo, base = B->start.base;
+    const int ps = A.ps, box = min(ps, KT), ppt = KT / box;
+    const Lengths L = {A.cu, A.context, A.total, A.g, A.Hkv, S::RB, A.most};
+    int64_t pos = run.lo, base = B->start.base;
     Request R = B->start.r;
     int b = B->start.b, seg = 0, stage = 0;
     uint32_t phase = 0;
     bool ok = true, again = false;
-    while (pos < hi && ok) {
-      const int64_t w = length(R);
+    while (pos < run.hi && ok) {
+      const int64_t w = L.length(R);
       if (pos >= base + w) {
         base += w;
-        R = look(++b);
+        R = L.look(++b);
         continue;
       }
-      const int64_t len = R.tiles + UNIT_COST;
-      const int unit = (int)quotient(pos - base, len);       // of the request: head, row block
-      const int hk = unit / R.blocks, rb = unit - hk * R.blocks;
-      const int64_t u0 = base + unit * len + UNIT_COST;   // where the unit's first tile is
-      const int64_t until = min(hi, u0 + R.tiles);
-      const int64_t t0 = max(pos - u0, (int64_t)0), t1 = until - u0;
-      pos = until;
+      const RunPart P = run_part(R, pos, base, run);
+      const int64_t t0 = P.t0, t1 = P.t1;
+      const int hk = P.hk;
+      pos = P.until;
       if (t1 <= t0) continue;                           // the run ends in the unit's start
       const int sb = seg & 1;
       if (seg >= 2 && !warp_wait(&B->q_empty[sb], ((seg >> 1) - 1) & 1, abort_f, A.err)) break;
-      const int row0 = rb * S::RB;
+      const int row0 = P.block * S::RB;
       const int rows = (int)min((int64_t)S::RB, (int64_t)R.n * A.g - row0);
       if (lane == 0) {
         Segment& G = B->seg[sb];
@@ -299,8 +212,8 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
         G.rows = rows;
         G.whole = t0 == 0 && t1 == R.tiles;
         G.starts = t0 == 0;
-        G.c0 = run_of(total, ctas, u0);
-        G.parts = run_of(total, ctas, u0 + R.tiles - 1) - G.c0 + 1;
+        G.c0 = P.c0;
+        G.parts = P.parts;
         G.end = 0;
         mbar_arrive_expect_tx(&B->q_full[sb], (uint32_t)(rows * A.Dk * 2));
       }
@@ -312,23 +225,15 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
                  (uint32_t)(A.Dk * 2), &B->q_full[sb], pol);
       }
       const int64_t end = R.ctx + R.n;
-      int64_t have = -1;         // first table entry held by lane 0
-      int ids = -1;
+      int have = -1, ids = -1;   // table entries held by the lanes
       for (int64_t tile = t0; tile < t1; ++tile) {
         if (again && !warp_wait(&B->empty[stage], phase ^ 1u, abort_f, A.err)) {
           ok = false;
           break;
         }
-        const int64_t key0 = tile * KT, entry = key0 >> shift;
-        if (have < 0 || entry + ppt > have + 32) {
-          have = entry;
-          const int64_t e = have + lane;
-          ids = e < A.width && e * ps < end ? A.table[(int64_t)b * A.table_stride + e] : -1;
-        }
-        const int at = (int)(entry - have);
-        const int mine_id = __shfl_sync(0xffffffffu, ids, min(at + min(lane, ppt - 1), 31));
-        const bool there = mine_id >= 0 && mine_id < A.n_pages;
-        const unsigned live = __ballot_sync(0xffffffffu, lane < ppt && there);
+        const int64_t key0 = tile * KT;
+        const int mine_id = page_ids(A, b, end, key0, ids, have);
+        const unsigned live = __ballot_sync(0xffffffffu, lane < ppt && mine_id >= 0);
         const int64_t left = end - key0;
         uint64_t valid = left >= KT ? ~0ull : (1ull << left) - 1ull;
         if (live != (ppt == 32 ? 0xffffffffu : (1u << ppt) - 1u)) {
@@ -767,6 +672,10 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
 // CTAs of a launch at most: two an SM for 16-row blocks, else one.
 static int max_ctas(int mt) { return mt == 1 ? MAX_CTAS : MAX_CTAS / 2; }
 
+// Rows (tokens x heads of a group) up to which the warp-level matrix steps are
+// used; more rows go to the 5th-generation tensor cores (kb_prompt.cu).
+constexpr int64_t MMA_ROWS = 32;
+
 static int row_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 template <int DKP, int DVP, int MT, bool F16>
@@ -784,7 +693,7 @@ static int launch_tree(const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A
 }
 
 template <int DKP, int DVP>
-static int launch_rows(int mt, int f16, const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A,
+static int launch_mma(int mt, int f16, const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A,
                        int sms, void* stream) {
   if (f16) {
     if (mt == 1) return launch_tree<DKP, DVP, 1, true>(mk, mv, A, sms, stream);
@@ -800,7 +709,9 @@ constexpr size_t COUNTER_BYTES = MAX_CTAS * sizeof(int);
 
 // Counters, then two partial sums a CTA (the end of one unit and the start of
 // another): maximum and sum of a row, and up to 128 values of it.
-static size_t tree_workspace(int mt) {
+static size_t tree_workspace(int64_t rows) {
+  if (rows > MMA_ROWS) return rows_workspace(rows);
+  const int mt = row_tiles(rows);
   return COUNTER_BYTES + (size_t)2 * max_ctas(mt) * 16 * mt * (2 + 128) * sizeof(float);
 }
 
@@ -809,7 +720,7 @@ static size_t tree_workspace(int mt) {
 
 extern "C" size_t kb_tree_attention_workspace_size(int64_t group, int64_t max_tokens) {
   if (group <= 0 || max_tokens <= 0) return 0;
-  return kb::attn::tree_workspace(kb::attn::row_tiles(group * max_tokens));
+  return kb::attn::tree_workspace(group * max_tokens);
 }
 
 extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -840,7 +751,8 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   KB_REQUIRE(!tree_mask || max_tokens <= 64, KB_ERR_UNSUPPORTED,
              "tree attention: a masked tree has at most 64 tokens");
   constexpr int64_t kMax = (int64_t)1 << 30;
-  KB_REQUIRE(B <= kMax && total <= kMax && n_pages <= kMax && table_width <= kMax && Hq <= 65535,
+  KB_REQUIRE(B <= kMax && total <= kMax && n_pages <= kMax && table_width <= kMax &&
+                 max_tokens * (Hq / Hkv) <= kMax && Hq <= 65535,
              KB_ERR_UNSUPPORTED, "tree attention: more than 2^30 tokens, pages or requests");
   bool ok = (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) == 0 &&
             ((q_token_stride | q_head_stride) & 7) == 0;
@@ -854,6 +766,49 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
              "%zu given",
              need, workspace_bytes);
   const int dev = kb::bind_stream_device(stream);
+  uint32_t* err = kb::device_error_word(dev);
+  KB_REQUIRE(err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
+  const int rows = (int)std::min<int64_t>(page_size, at::KT);
+  CUtensorMap mk, mv;
+  st = at::make_map_4d(&mk, k_cache, dtype, {Dk, page_size, Hkv, n_pages},
+                       {k_strides[1], k_strides[2], k_strides[0]}, rows, 1);
+  if (st != KB_OK) return st;
+  st = at::make_map_4d(&mv, v_cache, dtype, {Dv, page_size, Hkv, n_pages},
+                       {v_strides[1], v_strides[2], v_strides[0]}, rows, 1);
+  if (st != KB_OK) return st;
+  const int sms = kb::num_sms(dev);
+  const int64_t block_rows = max_tokens * (Hq / Hkv);
+  if (block_rows > at::MMA_ROWS) {
+    at::TreeCall T = {};
+    T.q = q;
+    T.v = v_cache;
+    T.q_tok = q_token_stride;
+    T.q_head = q_head_stride;
+    T.v_page = v_strides[0];
+    T.v_row = v_strides[1];
+    T.v_head = v_strides[2];
+    T.out = out;
+    T.lse = lse;
+    T.cu = cu_tokens;
+    T.table = block_table;
+    T.context = context_lens;
+    T.mask = tree_mask;
+    T.table_stride = table_stride;
+    T.n_pages = n_pages;
+    T.total = total;
+    T.B = (int)B;
+    T.width = (int)table_width;
+    T.ps = (int)page_size;
+    T.Hq = (int)Hq;
+    T.Hkv = (int)Hkv;
+    T.Dk = (int)Dk;
+    T.Dv = (int)Dv;
+    T.f16 = dtype;
+    T.scale2 = scale * kb::LOG2E;
+    T.most = (int)max_tokens;
+    T.err = err;
+    return at::launch_rows(T, block_rows, mk, mv, sms, workspace, stream);
+  }
   at::TreeArgs A = {};
   A.q = q;
   A.q_tok = q_token_stride;
@@ -880,22 +835,13 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   A.Dk = (int)Dk;
   A.Dv = (int)Dv;
   A.scale2 = scale * kb::LOG2E;
-  const int mt = at::row_tiles(max_tokens * A.g);
+  const int mt = at::row_tiles(block_rows);
   A.counters = static_cast<int*>(workspace);
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at::COUNTER_BYTES);
   A.part_o = A.part_ml + (size_t)2 * at::max_ctas(mt) * 16 * mt * 2;
-  A.err = kb::device_error_word(dev);
-  KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  const int rows = (int)std::min<int64_t>(page_size, at::KT);
-  CUtensorMap mk, mv;
-  st = at::make_map_4d(&mk, k_cache, dtype, {Dk, page_size, Hkv, n_pages},
-                       {k_strides[1], k_strides[2], k_strides[0]}, rows, 1);
-  if (st != KB_OK) return st;
-  st = at::make_map_4d(&mv, v_cache, dtype, {Dv, page_size, Hkv, n_pages},
-                       {v_strides[1], v_strides[2], v_strides[0]}, rows, 1);
-  if (st != KB_OK) return st;
-  const int sms = kb::num_sms(dev);
-  if (Dk <= 64 && Dv <= 64) return at::launch_rows<64, 64>(mt, dtype, mk, mv, A, sms, stream);
-  if (Dk <= 128) return at::launch_rows<128, 128>(mt, dtype, mk, mv, A, sms, stream);
-  return at::launch_rows<192, 128>(mt, dtype, mk, mv, A, sms, stream);
+  A.most = (int)max_tokens;
+  A.err = err;
+  if (Dk <= 64 && Dv <= 64) return at::launch_mma<64, 64>(mt, dtype, mk, mv, A, sms, stream);
+  if (Dk <= 128) return at::launch_mma<128, 128>(mt, dtype, mk, mv, A, sms, stream);
+  return at::launch_mma<192, 128>(mt, dtype, mk, mv, A, sms, stream);
 }
