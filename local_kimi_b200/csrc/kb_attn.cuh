@@ -138,6 +138,28 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// A value that all lanes have, or lane `from`'s, as one the compiler knows to be the
+// same for the warp.
+__device__ __forceinline__ int uniform(int x) { return __reduce_min_sync(0xffffffffu, x); }
+__device__ __forceinline__ int uniform_of(int x, int from) {
+  return __reduce_max_sync(0xffffffffu, (int)(threadIdx.x & 31) == from ? x : (int)0x80000000);
+}
+
+// The same for a whole warp in step, of which one lane (`one`) issues it: with no
+// branch around it, and the operands made uniform for the compiler, they stay in
+// the uniform registers that the instruction reads.
+__device__ __forceinline__ void tma_load_4d_one(uint32_t one, void* dst, const CUtensorMap* map,
+                                                int x, int y, int z, int w, uint64_t* bar,
+                                                uint64_t policy) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %8, 0;\n"
+      " @q cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;\n}"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z),
+        "r"(w), "r"(smem_addr(bar)), "l"(policy), "r"(one)
+      : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }

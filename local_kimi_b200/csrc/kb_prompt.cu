@@ -92,7 +92,7 @@ struct PromptArgs {
   int64_t table_stride;
   const int* context;
   const int64_t* mask;      // NULL: causal
-  int64_t n_pages, v_page;
+  int64_t n_pages, k_page, v_page;
   int width, ps, Hkv;
   int most;                 // tokens of a request at most
   int* counters;            // [2 * CTAs], zero between calls
@@ -282,6 +282,74 @@ __device__ __forceinline__ void join_parts(const PromptArgs& A, const Unit& U, i
   }
 }
 
+// 16 rows of a step of the paged cache, CHUNKS x 64 elements each, into the 128-byte
+// swizzle by 16-byte copies: eight lanes to a row, four rows at a time.  Lane i
+// (< 16) has row i's page in `id` (-1: none).
+template <int CHUNKS>
+__device__ __forceinline__ void gather_rows(uint8_t* to, const uint16_t* cache,
+                                            int64_t page_stride, int64_t row_stride, int width,
+                                            int ps, int id, int key) {
+  const int lane = threadIdx.x & 31, piece = lane & 7, sub = lane >> 3;
+#pragma unroll
+  for (int r = sub; r < 16; r += 4) {
+    const int page = __shfl_sync(0xffffffffu, id, r);
+    const uint16_t* from =
+        cache + page * page_stride + (int64_t)((key + r) & (ps - 1)) * row_stride + piece * 8;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+      if (page >= 0 && c * 64 + piece * 8 < width)
+        cp_async16(to + c * BLOCK + r * 128 + ((piece ^ (r & 7)) << 4), from + c * 64);
+  }
+}
+
+// The copies of a CTA whose tile B is idle: four of its warps take 16 rows of every
+// step each.  (One warp issuing tensor copies, page by page and 64 elements at a
+// time, needs 100 to 190 clocks each: 2100 a step at 64 rows a page, 2800 at 16,
+// where the softmax takes 1500.)
+template <int KC, int VC, int STAGES>
+__device__ __forceinline__ void gather_steps(const PromptArgs& A, PromptBars* B, uint8_t* ring,
+                                             int quarter) {
+  constexpr int STAGE = (KC + VC) * BLOCK;
+  const int lane = threadIdx.x & 31, r0 = quarter * 16, shift = 31 - __clz(A.ps);
+  int st = 0;
+  uint32_t ph = 1;
+  bool ok = true;
+  Unit U;
+  for (Walk walk(B, A.err); ok && walk.next(U);) {
+    const int steps = U.steps[0], hk = U.head0 / A.g;
+    const uint16_t* k = A.k + hk * A.k_head;
+    const uint16_t* v = A.v + hk * A.v_head;
+    auto page_of = [&](int step) {
+      const int key = (U.j0 + step) * STEP + r0 + (lane & 15), e = key >> shift;
+      if (step >= steps || key >= U.m || e >= A.width) return -1;
+      const int id = __ldg(A.table + (int64_t)U.b * A.table_stride + e);
+      return id < A.n_pages ? id : -1;
+    };
+    int ids[4] = {-1, -1, page_of(0), -1};     // steps j, j + 1, j + 2, j + 3
+    for (int j = -2; j < steps; ++j) {
+      ids[3] = page_of(j + 3);                 // in time for the next round
+      ok = warp_wait(&B->empty[st], ph, &B->abort_flag, A.err);
+      if (!ok) break;
+      uint8_t* at = ring + st * STAGE + r0 * 128;
+      if (j + 2 < steps)
+        gather_rows<KC>(at, k, A.k_page, A.k_tok, A.Dk, A.ps, ids[2],
+                        (U.j0 + j + 2) * STEP + r0);
+      if (j >= 0)
+        gather_rows<VC>(at + KC * BLOCK, v, A.v_page, A.v_tok, A.Dv, A.ps, ids[0],
+                        (U.j0 + j) * STEP + r0);
+      cp_async_arrive_noinc(&B->full[st]);
+      ids[0] = ids[1];
+      ids[1] = ids[2];
+      ids[2] = ids[3];
+      if (++st == STAGES) {
+        st = 0;
+        ph ^= 1u;
+      }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 template <int DKP, int DVP, bool F16, bool PAGED>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -296,10 +364,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   PromptBars* B = reinterpret_cast<PromptBars*>(ring + S::STAGES * S::STAGE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_f = &B->abort_flag;
+  // No request has rows for tile B: its warps bring in keys and values.
+  const bool solo = PAGED && A.part_rows == TILE;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::STAGES; ++i) {
-      mbar_init(&B->full[i], 1);
+      mbar_init(&B->full[i], solo ? 4 * 32 + 1 : 1);
       mbar_init(&B->empty[i], 2);
       mbar_init(&B->clean[i], 1);
     }
@@ -327,9 +397,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     prefetch_map(&tv);
   }
   if (warp == CLEAN_WARP) tc::tmem_alloc_all(&B->tmem);
-  // Columns of q past the head's width stay zero (the gather does not write them).
-  if (PAGED && A.Dk < DKP) {
-    for (int i = threadIdx.x; i < 2 * S::Q_TILE / 16; i += PROMPT_THREADS)
+  // Columns past the heads' widths stay zero (gathered rows do not write them).
+  if (PAGED && (A.Dk < DKP || A.Dv < DVP)) {
+    for (int i = threadIdx.x; i < (2 * S::Q_TILE + S::STAGES * S::STAGE) / 16;
+         i += PROMPT_THREADS)
       reinterpret_cast<uint4*>(qs)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
   }
@@ -371,7 +442,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     int buf = 0;                          // the next step's S buffer
     uint32_t s_phase = 0, near_phase = 0, end_phase = 0, meet_phase = 0;
     Unit U;
-    for (Walk walk(B, A.err); walk.next(U);) {
+    const bool copies = solo && tile == 1;
+    if (copies) gather_steps<S::KC, S::VC, S::STAGES>(A, B, ring, warp & 3);
+    for (Walk walk(B, A.err); !copies && walk.next(U);) {
       // The row's token and head; keys are limited by `limit`, or in a tree by `word`.
       const int at_row = U.t0 + tile * TILE + row;          // paged
       const int first = PAGED ? (U.t0 + tile * TILE) / A.g : U.t0 + tile * span;
@@ -672,6 +745,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         // of the ring.
         for (int j = -2; j < all && all > 0; ++j) {
           if (!need(&B->clean[st], ph)) break;
+          if (solo) fence_proxy_async();       // keys and values came by ordinary copies
           if (j >= 0 && j < mine) {
             if (!need(&B->p_full[tile][p_buf], p_phase)) break;
             tc::tc_fence_after();
@@ -727,12 +801,14 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           told ^= 1u;
         }
       };
+      // Copies are issued by the warp in step, one lane doing it.
+      const uint32_t one = tc::elect_one();
       const int box = min(A.ps, STEP), pages = STEP / max(box, 1);      // paged
-      int ids_k = -1, ids_v = -1, have_k = -1, have_v = -1;
+      int ids = -1, have = -1, id_k = -1, id_w = -1, id_v = -1;
       auto copy = [&](const Unit& U) {
-        const int steps = max(U.steps[0], U.steps[1]);
-        const int hk = U.head0 / A.g;
-        have_k = have_v = -1;
+        const int steps = uniform(max(U.steps[0], U.steps[1]));
+        const int hk = uniform(U.head0 / A.g), key0 = uniform(U.k0), j0 = uniform(U.j0);
+        have = -1;
         auto queries = [&](int i) {
           if (U.steps[i] == 0 || !need(&B->q_empty[i], q_phase[i])) return;
           q_phase[i] ^= 1u;
@@ -759,61 +835,70 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           if (j == -2) queries(0);
           if (!need(&B->empty[st], ph)) break;
           const bool keys = j + 2 < steps, values = j >= 0;
+          uint8_t* at = ring + st * S::STAGE;
           if (PAGED) {
-            unsigned live_k = 0, live_v = 0;
-            int id_k = -1, id_v = -1;
+            // Pages of the keys; those of the values are the keys' of two steps ago.
+            id_v = id_w;
+            id_w = id_k;
+            id_k = -1;
+            const int k_row = (j0 + j + 2) * STEP, v_row = (j0 + j) * STEP;
             if (keys) {
-              id_k = page_ids(A, U.b, U.m, (U.j0 + j + 2) * STEP, ids_k, have_k);
-              live_k = __ballot_sync(0xffffffffu, lane < pages && id_k >= 0);
-              uint64_t there = low_bits(U.m - (U.j0 + j + 2) * STEP);
-              if (live_k != low_bits(pages)) {
+              id_k = page_ids(A, U.b, U.m, k_row, ids, have);
+              uint64_t there = low_bits(U.m - k_row);
+              const unsigned live = __ballot_sync(0xffffffffu, lane < pages && id_k >= 0);
+              if (live != (1u << pages) - 1u) {
                 uint64_t got = 0;
                 for (int i = 0; i < pages; ++i)
-                  if ((live_k >> i) & 1) got |= low_bits(box) << (i * box);
+                  if ((live >> i) & 1) got |= low_bits(box) << (i * box);
                 if (lane == 0 && (there & ~got)) atomicOr(A.err, ERR_PAGE);
                 there &= got;
               }
               if (lane == 0) B->valid[(U.base + j + 2) & (SEEN - 1)] = there;
             }
-            if (values) {
-              id_v = page_ids(A, U.b, U.m, (U.j0 + j) * STEP, ids_v, have_v);
-              live_v = __ballot_sync(0xffffffffu, lane < pages && id_v >= 0);
-            }
-            uint8_t* at = ring + st * S::STAGE;
-            if (lane == 0)
-              mbar_arrive_expect_tx(&B->full[st], (uint32_t)((__popc(live_k) * S::KC +
-                                                              __popc(live_v) * S::VC) * box * 128));
-            __syncwarp();
-            for (int x0 = 0; x0 < pages * (S::KC + S::VC); x0 += 32) {
-              const int x = x0 + lane;
-              const int i = min(x / (S::KC + S::VC), pages - 1), c = x - i * (S::KC + S::VC);
-              const int k_page = __shfl_sync(0xffffffffu, id_k, i);
-              const int v_page = __shfl_sync(0xffffffffu, id_v, i);
-              if (x >= pages * (S::KC + S::VC)) continue;
-              if (c < S::KC) {
-                if ((live_k >> i) & 1)
-                  tma_load_4d(at + c * BLOCK + i * box * 128, &tk, c * 64,
-                              ((U.j0 + j + 2) * STEP + i * box) & (A.ps - 1), hk, k_page,
-                              &B->full[st], once);
-              } else if ((live_v >> i) & 1) {
-                tma_load_4d(at + c * BLOCK + i * box * 128, &tv, (c - S::KC) * 64,
-                            ((U.j0 + j) * STEP + i * box) & (A.ps - 1), hk, v_page, &B->full[st],
-                            once);
+            if (solo) {
+              // Warps 4-7 bring the rows in; this adds the word.
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&B->full[st]);
+            } else {
+              const unsigned in = __ballot_sync(0xffffffffu, lane < pages && id_k >= 0);
+              const unsigned out = __ballot_sync(0xffffffffu, values && lane < pages && id_v >= 0);
+              if (lane == 0)
+                mbar_arrive_expect_tx(&B->full[st], (uint32_t)((__popc(in) * S::KC +
+                                                                __popc(out) * S::VC) * box * 128));
+              __syncwarp();
+              // A copy per page and 64-element column block, a lane each.
+              for (int x0 = 0; x0 < pages * (S::KC + S::VC); x0 += 32) {
+                const int x = x0 + lane;
+                const int i = min(x / (S::KC + S::VC), pages - 1), c = x - i * (S::KC + S::VC);
+                const int k_page = __shfl_sync(0xffffffffu, id_k, i);
+                const int v_page = __shfl_sync(0xffffffffu, id_v, i);
+                if (x >= pages * (S::KC + S::VC)) continue;
+                const int row = i * box;
+                if (c < S::KC) {
+                  if ((in >> i) & 1)
+                    tma_load_4d(at + c * BLOCK + row * 128, &tk, c * 64,
+                                (k_row + row) & (A.ps - 1), hk, k_page, &B->full[st], once);
+                } else if ((out >> i) & 1) {
+                  tma_load_4d(at + c * BLOCK + row * 128, &tv, (c - S::KC) * 64,
+                              (v_row + row) & (A.ps - 1), hk, v_page, &B->full[st], once);
+                }
               }
+              __syncwarp();
             }
+          } else {
+            if (lane == 0)
+              mbar_arrive_expect_tx(&B->full[st], (uint32_t)(((keys ? S::KC : 0) +
+                                                              (values ? S::VC : 0)) * BLOCK));
             __syncwarp();
-          } else if (lane == 0) {
-            uint8_t* at = ring + st * S::STAGE;
-            mbar_arrive_expect_tx(&B->full[st], (uint32_t)(((keys ? S::KC : 0) +
-                                                            (values ? S::VC : 0)) * BLOCK));
-            if (keys)
-              for (int c = 0; c < S::KC; ++c)
-                tma_load_4d(at + c * BLOCK, &tk, c * 64, hk, U.k0 + (j + 2) * STEP, 0,
-                            &B->full[st], keep);
-            if (values)
-              for (int d = 0; d < S::VC; ++d)
-                tma_load_4d(at + (S::KC + d) * BLOCK, &tv, d * 64, hk, U.k0 + j * STEP, 0,
-                            &B->full[st], keep);
+            const uint32_t k_one = keys ? one : 0, v_one = values ? one : 0;
+#pragma unroll
+            for (int c = 0; c < S::KC; ++c)
+              tma_load_4d_one(k_one, at + c * BLOCK, &tk, c * 64, hk, key0 + (j + 2) * STEP, 0,
+                              &B->full[st], keep);
+#pragma unroll
+            for (int d = 0; d < S::VC; ++d)
+              tma_load_4d_one(v_one, at + (S::KC + d) * BLOCK, &tv, d * 64, hk, key0 + j * STEP, 0,
+                              &B->full[st], keep);
           }
           if (++st == S::STAGES) {
             st = 0;
@@ -1010,9 +1095,13 @@ int launch_rows(const TreeCall& T, int64_t rows, const CUtensorMap& mk, const CU
                 int sms, void* workspace, void* stream) {
   PromptArgs A = {};
   A.q = T.q;
+  A.k = T.k;
   A.v = T.v;
   A.q_tok = T.q_tok;
   A.q_head = T.q_head;
+  A.k_page = T.k_page;
+  A.k_tok = T.k_row;
+  A.k_head = T.k_head;
   A.v_page = T.v_page;
   A.v_tok = T.v_row;
   A.v_head = T.v_head;

@@ -161,8 +161,8 @@ __device__ __forceinline__ int page_ids(const Args& A, int b, int64_t end, int64
 
 // What the tensor-core form for many rows needs of a tree attention call.
 struct TreeCall {
-  const uint16_t *q, *v;
-  int64_t q_tok, q_head, v_page, v_row, v_head;
+  const uint16_t *q, *k, *v;
+  int64_t q_tok, q_head, k_page, k_row, k_head, v_page, v_row, v_head;
   uint16_t* out;
   float* lse;
   const int *cu, *table, *context;

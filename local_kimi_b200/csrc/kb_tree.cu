@@ -781,7 +781,11 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   if (block_rows > at::MMA_ROWS) {
     at::TreeCall T = {};
     T.q = q;
+    T.k = k_cache;
     T.v = v_cache;
+    T.k_page = k_strides[0];
+    T.k_row = k_strides[1];
+    T.k_head = k_strides[2];
     T.q_tok = q_token_stride;
     T.q_head = q_head_stride;
     T.v_page = v_strides[0];
