@@ -48,8 +48,8 @@
 // tile B is idle and the bytes of the cache bound the work.  All units' steps
 // form one line cut into equal runs, one per CTA, as in kb_tree.cu; a unit that
 // falls to several CTAs is joined from fp32 partial sums by the CTA that finishes
-// last.  Keys and values come page by page, q by gathered 16-byte copies into the
-// same swizzled layout.
+// last.  Keys and values come page by page; q too by tensor copies where one tile
+// holds a request's rows, else by gathered 16-byte copies into the same layout.
 //
 // In the last tiles of a unit some rows do not see some keys, or the tile
 // reaches past the request's end into its neighbour.  A value there that is
@@ -92,13 +92,13 @@ struct PromptArgs {
   int64_t table_stride;
   const int* context;
   const int64_t* mask;      // NULL: causal
-  int64_t n_pages, k_page, v_page;
+  int64_t n_pages, v_page;
   int width, ps, Hkv;
   int most;                 // tokens of a request at most
   int* counters;            // [2 * CTAs], zero between calls
   int part_rows;            // rows of a unit: 128 or 256
   float* part_ml;           // [2 * CTAs][part_rows][2]: m (log2), l
-  float* part_o;            // [2 * CTAs][part_rows][DVP]
+  float* part_o;            // [2 * CTAs][DVP / 4][part_rows][4]
 };
 
 template <int DKP, int DVP>
@@ -224,103 +224,81 @@ __device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int upper, int s
   if (upper) a = give; else b = give;
 }
 
-// Sums of the rows of a tile whose keys several CTAs had: a thread takes 16
-// values of a row, four parts at a time.
+// A row whose keys several CTAs had: their sums joined, 64 columns at a time.
 template <int DVP, bool F16>
-__device__ __forceinline__ void join_parts(const PromptArgs& A, const Unit& U, int tile,
-                                           int thread) {
-  const int rows = min(TILE, U.n * A.g - U.t0 - tile * TILE);
-  constexpr int GROUPS = DVP / 16, BATCH = 2;
-  for (int it = thread; it < rows * GROUPS; it += TILE) {
-    const int r = it / GROUPS, d = (it - r * GROUPS) * 16;
-    float top = -INFINITY, sum = 0.f, o[16] = {};
-    for (int c = 0; c < U.parts; c += BATCH) {
-      float2 ml[BATCH];
-      float4 v[BATCH][4];
+__device__ __forceinline__ void join_parts(const PromptArgs& A, const Unit& U, int row,
+                                           int64_t at) {
+  auto slot = [&](int c) { return (int64_t)(U.c0 + c) * 2 + (c == 0); };
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < U.parts; ++c) {
+    const float2 ml =
+        __ldcg(reinterpret_cast<const float2*>(A.part_ml + (slot(c) * A.part_rows + row) * 2));
+    const float t = fmaxf(top, ml.x);
+    if (t == -INFINITY) continue;
+    sum = sum * exp2_fast(top - t) + ml.y * exp2_fast(ml.x - t);
+    top = t;
+  }
+  const bool none = sum == 0.f;
+  const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const int cc = min(c + u, U.parts - 1);
-        const int64_t at = ((int64_t)(U.c0 + cc) * 2 + (cc == 0)) * A.part_rows + tile * TILE + r;
-        ml[u] = __ldcg(reinterpret_cast<const float2*>(A.part_ml + at * 2));
+  for (int d = 0; d < DVP; d += 64) {
+    float o[64] = {};
+    for (int c = 0; c < U.parts && !none; ++c) {
+      const float m = __ldcg(A.part_ml + (slot(c) * A.part_rows + row) * 2);
+      float4 v[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          v[u][k] = __ldcg(reinterpret_cast<const float4*>(A.part_o + at * DVP + d + 4 * k));
-      }
+      for (int k = 0; k < 16; ++k)
+        v[k] = __ldcg(reinterpret_cast<const float4*>(
+            A.part_o + ((slot(c) * (DVP / 4) + d / 4 + k) * A.part_rows + row) * 4));
+      const float f = m == -INFINITY ? 0.f : exp2_fast(m - top) * inv;
+      if (f == 0.f) continue;
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const float t = fmaxf(top, ml[u].x);
-        if (c + u >= U.parts || t == -INFINITY) continue;
-        const float f0 = exp2_fast(top - t), f1 = exp2_fast(ml[u].x - t);
-        top = t;
-        sum = sum * f0 + ml[u].y * f1;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          o[4 * k] = o[4 * k] * f0 + v[u][k].x * f1;
-          o[4 * k + 1] = o[4 * k + 1] * f0 + v[u][k].y * f1;
-          o[4 * k + 2] = o[4 * k + 2] * f0 + v[u][k].z * f1;
-          o[4 * k + 3] = o[4 * k + 3] * f0 + v[u][k].w * f1;
-        }
+      for (int k = 0; k < 16; ++k) {
+        o[4 * k] += v[k].x * f;
+        o[4 * k + 1] += v[k].y * f;
+        o[4 * k + 2] += v[k].z * f;
+        o[4 * k + 3] += v[k].w * f;
       }
     }
-    const int at_row = U.t0 + tile * TILE + r, t = at_row / A.g;
-    const int64_t at = (int64_t)(U.q0 + t) * A.Hq + U.head0 + at_row - t * A.g;
-    const bool none = sum == 0.f;
-    const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int k = 0; k < 16; k += 8)
+    for (int k = 0; k < 64; k += 8)
       if (d + k < A.Dv) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (!none) {
-          w.x = pack2<F16>(o[k] * inv, o[k + 1] * inv);
-          w.y = pack2<F16>(o[k + 2] * inv, o[k + 3] * inv);
-          w.z = pack2<F16>(o[k + 4] * inv, o[k + 5] * inv);
-          w.w = pack2<F16>(o[k + 6] * inv, o[k + 7] * inv);
-        }
+        uint4 w;
+        w.x = pack2<F16>(o[k], o[k + 1]);
+        w.y = pack2<F16>(o[k + 2], o[k + 3]);
+        w.z = pack2<F16>(o[k + 4], o[k + 5]);
+        w.w = pack2<F16>(o[k + 6], o[k + 7]);
         *reinterpret_cast<uint4*>(A.out + at * A.Dv + d + k) = w;
       }
-    if (A.lse && d == 0) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
   }
+  if (A.lse) A.lse[at] = none ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// 16 rows of a step of the paged cache, CHUNKS x 64 elements each, into the 128-byte
-// swizzle by 16-byte copies: eight lanes to a row, four rows at a time.  Lane i
-// (< 16) has row i's page in `id` (-1: none).
-template <int CHUNKS>
-__device__ __forceinline__ void gather_rows(uint8_t* to, const uint16_t* cache,
-                                            int64_t page_stride, int64_t row_stride, int width,
-                                            int ps, int id, int key) {
-  const int lane = threadIdx.x & 31, piece = lane & 7, sub = lane >> 3;
-#pragma unroll
-  for (int r = sub; r < 16; r += 4) {
-    const int page = __shfl_sync(0xffffffffu, id, r);
-    const uint16_t* from =
-        cache + page * page_stride + (int64_t)((key + r) & (ps - 1)) * row_stride + piece * 8;
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-      if (page >= 0 && c * 64 + piece * 8 < width)
-        cp_async16(to + c * BLOCK + r * 128 + ((piece ^ (r & 7)) << 4), from + c * 64);
-  }
-}
-
-// The copies of a CTA whose tile B is idle: four of its warps take 16 rows of every
-// step each.  (One warp issuing tensor copies, page by page and 64 elements at a
-// time, needs 100 to 190 clocks each: 2100 a step at 64 rows a page, 2800 at 16,
-// where the softmax takes 1500.)
+// The copies of a CTA whose tile B is idle: four of its warps bring in 16 rows of every
+// step each, in boxes of 16 rows (8 in pages of 8) x 64 elements.  A copy takes the
+// warp that issues it 100 to 190 clocks whatever its size, so one warp needs 1600
+// to 3150 a step where the softmax takes 1500; 16-byte copies by these four warps
+// get in the way of the softmax (2300 a step).
 template <int KC, int VC, int STAGES>
-__device__ __forceinline__ void gather_steps(const PromptArgs& A, PromptBars* B, uint8_t* ring,
+__device__ __forceinline__ void copy_quarter(const CUtensorMap& tk, const CUtensorMap& tv,
+                                             const PromptArgs& A, PromptBars* B, uint8_t* ring,
                                              int quarter) {
   constexpr int STAGE = (KC + VC) * BLOCK;
-  const int lane = threadIdx.x & 31, r0 = quarter * 16, shift = 31 - __clz(A.ps);
+  const uint64_t once = l2_evict_first_policy();
+  const uint32_t one = tc::elect_one();
+  const int lane = threadIdx.x & 31, shift = 31 - __clz(A.ps);
+  const int box = min(A.ps, 16), boxes = 16 / box;
+  const int r0 = uniform(quarter) * 16;
   int st = 0;
   uint32_t ph = 1;
   bool ok = true;
   Unit U;
   for (Walk walk(B, A.err); ok && walk.next(U);) {
-    const int steps = U.steps[0], hk = U.head0 / A.g;
-    const uint16_t* k = A.k + hk * A.k_head;
-    const uint16_t* v = A.v + hk * A.v_head;
+    const int steps = uniform(U.steps[0]), hk = uniform(U.head0 / A.g), j0 = uniform(U.j0);
+    // Page of the step's rows r0 (lane 0) and r0 + 8 (lane 1); -1: none.
     auto page_of = [&](int step) {
-      const int key = (U.j0 + step) * STEP + r0 + (lane & 15), e = key >> shift;
+      const int key = (j0 + step) * STEP + r0 + (lane & 1) * 8, e = key >> shift;
       if (step >= steps || key >= U.m || e >= A.width) return -1;
       const int id = __ldg(A.table + (int64_t)U.b * A.table_stride + e);
       return id < A.n_pages ? id : -1;
@@ -331,13 +309,30 @@ __device__ __forceinline__ void gather_steps(const PromptArgs& A, PromptBars* B,
       ok = warp_wait(&B->empty[st], ph, &B->abort_flag, A.err);
       if (!ok) break;
       uint8_t* at = ring + st * STAGE + r0 * 128;
-      if (j + 2 < steps)
-        gather_rows<KC>(at, k, A.k_page, A.k_tok, A.Dk, A.ps, ids[2],
-                        (U.j0 + j + 2) * STEP + r0);
-      if (j >= 0)
-        gather_rows<VC>(at + KC * BLOCK, v, A.v_page, A.v_tok, A.Dv, A.ps, ids[0],
-                        (U.j0 + j) * STEP + r0);
-      cp_async_arrive_noinc(&B->full[st]);
+      const int k_row = (j0 + j + 2) * STEP + r0, v_row = (j0 + j) * STEP + r0;
+      int k_page[2], v_page[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        k_page[i] = i < boxes ? uniform_of(ids[2], i) : -1;
+        v_page[i] = i < boxes ? uniform_of(ids[0], i) : -1;
+      }
+      const int copies = KC * ((k_page[0] >= 0) + (k_page[1] >= 0)) +
+                         VC * ((v_page[0] >= 0) + (v_page[1] >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(&B->full[st], (uint32_t)(copies * box * 128));
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= boxes) break;
+        const uint32_t k_one = k_page[i] >= 0 ? one : 0, v_one = v_page[i] >= 0 ? one : 0;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+          tma_load_4d_one(k_one, at + c * BLOCK + i * 1024, &tk, c * 64,
+                          (k_row + i * 8) & (A.ps - 1), hk, k_page[i], &B->full[st], once);
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+          tma_load_4d_one(v_one, at + (KC + c) * BLOCK + i * 1024, &tv, c * 64,
+                          (v_row + i * 8) & (A.ps - 1), hk, v_page[i], &B->full[st], once);
+      }
       ids[0] = ids[1];
       ids[1] = ids[2];
       ids[2] = ids[3];
@@ -347,7 +342,6 @@ __device__ __forceinline__ void gather_steps(const PromptArgs& A, PromptBars* B,
       }
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <int DKP, int DVP, bool F16, bool PAGED>
@@ -369,12 +363,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::STAGES; ++i) {
-      mbar_init(&B->full[i], solo ? 4 * 32 + 1 : 1);
+      mbar_init(&B->full[i], solo ? 5 : 1);
       mbar_init(&B->empty[i], 2);
       mbar_init(&B->clean[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&B->q_full[i], PAGED ? 32 : 1);
+      mbar_init(&B->q_full[i], PAGED && !solo ? 32 : 1);
       mbar_init(&B->meet[i], 4);
       mbar_init(&B->q_empty[i], 1);
       mbar_init(&B->o_near[i], 1);
@@ -392,15 +386,14 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     mbar_init(&B->drain, 2);
     B->abort_flag = 0;
     mbar_fence_init();
-    if (!PAGED) prefetch_map(&tq);
+    if (!PAGED || solo) prefetch_map(&tq);
     prefetch_map(&tk);
     prefetch_map(&tv);
   }
   if (warp == CLEAN_WARP) tc::tmem_alloc_all(&B->tmem);
-  // Columns past the heads' widths stay zero (gathered rows do not write them).
-  if (PAGED && (A.Dk < DKP || A.Dv < DVP)) {
-    for (int i = threadIdx.x; i < (2 * S::Q_TILE + S::STAGES * S::STAGE) / 16;
-         i += PROMPT_THREADS)
+  // Columns of q past the head's width stay zero (gathered rows do not write them).
+  if (PAGED && !solo && A.Dk < DKP) {
+    for (int i = threadIdx.x; i < 2 * S::Q_TILE / 16; i += PROMPT_THREADS)
       reinterpret_cast<uint4*>(qs)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async();
   }
@@ -443,7 +436,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     uint32_t s_phase = 0, near_phase = 0, end_phase = 0, meet_phase = 0;
     Unit U;
     const bool copies = solo && tile == 1;
-    if (copies) gather_steps<S::KC, S::VC, S::STAGES>(A, B, ring, warp & 3);
+    if (copies) copy_quarter<S::KC, S::VC, S::STAGES>(tk, tv, A, B, ring, warp & 3);
     for (Walk walk(B, A.err); !copies && walk.next(U);) {
       // The row's token and head; keys are limited by `limit`, or in a tree by `word`.
       const int at_row = U.t0 + tile * TILE + row;          // paged
@@ -579,7 +572,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         out[i] = t < U.n ? A.out + ((int64_t)(U.q0 + t) * A.Hq + h) * A.Dv + (lane & 3) * 8
                          : nullptr;
       }
-      const int64_t part_row = ((int64_t)blockIdx.x * 2 + U.starts) * A.part_rows + tile * TILE;
+      const int64_t part_slot = (int64_t)blockIdx.x * 2 + U.starts;
       if (steps > 1) near_phase ^= 1u;
       bool odd = false;
       if (steps > 0) {
@@ -616,24 +609,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           }
         }
         if (!whole) {
-          // This CTA's share of the sums, 64 bytes of eight rows a store too.
+          // This CTA's share of the sums, columns by fours: a warp stores 512 bytes.
 #pragma unroll
-          for (int i = 0; i < 32; i += 16) {
-            uint4 w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = make_uint4(__float_as_uint(o[i + 4 * k]), __float_as_uint(o[i + 4 * k + 1]),
-                                __float_as_uint(o[i + 4 * k + 2]), __float_as_uint(o[i + 4 * k + 3]));
-            swap_pieces(w[0], w[1], lane & 1, 1);
-            swap_pieces(w[2], w[3], lane & 1, 1);
-            swap_pieces(w[0], w[2], lane & 2, 2);
-            swap_pieces(w[1], w[3], lane & 2, 2);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (out[k])
-                *reinterpret_cast<uint4*>(A.part_o + (part_row + (row & ~3) + k) * DVP + c * 32 + i +
-                                          (lane & 3) * 4) = w[k];
-          }
+          for (int i = 0; i < 32; i += 4)
+            if (real)
+              *reinterpret_cast<float4*>(A.part_o + ((part_slot * (DVP / 4) + c * 8 + i / 4) *
+                                                     A.part_rows + tile * TILE + row) * 4) =
+                  make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           continue;
         }
         uint4 w[4];
@@ -661,7 +643,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         continue;
       }
       if (real)
-        *reinterpret_cast<float2*>(A.part_ml + (part_row + row) * 2) = make_float2(top, sum);
+        *reinterpret_cast<float2*>(A.part_ml + (part_slot * A.part_rows + tile * TILE + row) * 2) =
+            make_float2(top, sum);
       // The last of the unit's CTAs joins the tile's sums, in CTA order.
       auto meet = [&]() {
         __syncwarp();
@@ -681,7 +664,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       if (!meet()) break;
       if (*const_cast<volatile int*>(&B->joined[tile])) {
         __threadfence();
-        join_parts<DVP, F16>(A, U, tile, row);
+        if (real) join_parts<DVP, F16>(A, U, tile * TILE + row, at);
       }
       if (!meet()) break;
     }
@@ -745,7 +728,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         // of the ring.
         for (int j = -2; j < all && all > 0; ++j) {
           if (!need(&B->clean[st], ph)) break;
-          if (solo) fence_proxy_async();       // keys and values came by ordinary copies
           if (j >= 0 && j < mine) {
             if (!need(&B->p_full[tile][p_buf], p_phase)) break;
             tc::tc_fence_after();
@@ -759,7 +741,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             if (j == -2) {
               if (!need(&B->q_full[tile], q_phase)) break;
               q_phase ^= 1u;
-              if (PAGED) fence_proxy_async();      // q came by ordinary copies
+              if (PAGED && !solo) fence_proxy_async();      // q came by ordinary copies
             }
             tc::tc_fence_after();
             score();
@@ -812,7 +794,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         auto queries = [&](int i) {
           if (U.steps[i] == 0 || !need(&B->q_empty[i], q_phase[i])) return;
           q_phase[i] ^= 1u;
-          if (PAGED) {
+          if (PAGED && !solo) {
             const int pieces = A.Dk / 8, rows = min(TILE, U.n * A.g - U.t0 - i * TILE);
             for (int x = lane; x < rows * pieces; x += 32) {
               const int r = x / pieces, c = x - r * pieces, at = U.t0 + i * TILE + r;
@@ -826,10 +808,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             return;
           }
           if (lane != 0) return;
-          mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)S::Q_TILE);
+          // Paged: the group's heads of as many tokens as a tile has room for.
+          const int rows = PAGED ? TILE / A.g * A.g : TILE;
+          mbar_arrive_expect_tx(&B->q_full[i], (uint32_t)(S::KC * 128 * rows));
           for (int c = 0; c < S::KC; ++c)
             tma_load_4d(qs + i * S::Q_TILE + c * 2 * BLOCK, &tq, c * 64, U.head0,
-                        U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
+                        PAGED ? U.q0 : U.q0 + U.t0 + i * span, 0, &B->q_full[i], once);
         };
         for (int j = -2; j < steps && steps > 0; ++j) {
           if (j == -2) queries(0);
@@ -1091,17 +1075,12 @@ size_t rows_workspace(int64_t rows) {
   return ROW_COUNTERS + (size_t)2 * ROW_CTAS * part_rows(rows) * (2 + 128) * sizeof(float);
 }
 
-int launch_rows(const TreeCall& T, int64_t rows, const CUtensorMap& mk, const CUtensorMap& mv,
-                int sms, void* workspace, void* stream) {
+int launch_rows(const TreeCall& T, int64_t rows, int sms, void* workspace, void* stream) {
   PromptArgs A = {};
   A.q = T.q;
-  A.k = T.k;
   A.v = T.v;
   A.q_tok = T.q_tok;
   A.q_head = T.q_head;
-  A.k_page = T.k_page;
-  A.k_tok = T.k_row;
-  A.k_head = T.k_head;
   A.v_page = T.v_page;
   A.v_tok = T.v_row;
   A.v_head = T.v_head;
@@ -1129,7 +1108,19 @@ int launch_rows(const TreeCall& T, int64_t rows, const CUtensorMap& mk, const CU
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ROW_COUNTERS);
   A.part_rows = part_rows(rows);
   A.part_o = A.part_ml + (size_t)2 * ROW_CTAS * A.part_rows * 2;
-  return launch_widths<true>(T.Dk, T.Dv, T.f16, mk, mk, mv, A, std::min(sms, ROW_CTAS), stream);
+  // One tile of rows: q by tensor copies, keys and values in boxes of 16 rows.
+  const bool solo = A.part_rows == TILE;
+  const int box = std::min(T.ps, solo ? 16 : STEP);
+  CUtensorMap mq = {}, mk, mv;
+  int st = KB_OK;
+  if (solo) st = make_map_4d(&mq, T.q, T.f16, {T.Dk, T.Hq, T.total, 1}, {T.q_head, T.q_tok, 8},
+                             A.g, TILE / A.g);
+  if (st == KB_OK) st = make_map_4d(&mk, T.k, T.f16, {T.Dk, T.ps, T.Hkv, T.n_pages},
+                                    {T.k_row, T.k_head, T.k_page}, box, 1);
+  if (st == KB_OK) st = make_map_4d(&mv, T.v, T.f16, {T.Dv, T.ps, T.Hkv, T.n_pages},
+                                    {T.v_row, T.v_head, T.v_page}, box, 1);
+  if (st != KB_OK) return st;
+  return launch_widths<true>(T.Dk, T.Dv, T.f16, mq, mk, mv, A, std::min(sms, ROW_CTAS), stream);
 }
 
 }  // namespace attn

@@ -174,8 +174,7 @@ struct TreeCall {
 };
 // `rows`: tokens x heads of a group, of the request with most.
 size_t rows_workspace(int64_t rows);
-int launch_rows(const TreeCall& T, int64_t rows, const CUtensorMap& mk, const CUtensorMap& mv,
-                int sms, void* workspace, void* stream);
+int launch_rows(const TreeCall& T, int64_t rows, int sms, void* workspace, void* stream);
 
 }  // namespace attn
 }  // namespace kb

@@ -768,14 +768,6 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   const int dev = kb::bind_stream_device(stream);
   uint32_t* err = kb::device_error_word(dev);
   KB_REQUIRE(err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  const int rows = (int)std::min<int64_t>(page_size, at::KT);
-  CUtensorMap mk, mv;
-  st = at::make_map_4d(&mk, k_cache, dtype, {Dk, page_size, Hkv, n_pages},
-                       {k_strides[1], k_strides[2], k_strides[0]}, rows, 1);
-  if (st != KB_OK) return st;
-  st = at::make_map_4d(&mv, v_cache, dtype, {Dv, page_size, Hkv, n_pages},
-                       {v_strides[1], v_strides[2], v_strides[0]}, rows, 1);
-  if (st != KB_OK) return st;
   const int sms = kb::num_sms(dev);
   const int64_t block_rows = max_tokens * (Hq / Hkv);
   if (block_rows > at::MMA_ROWS) {
@@ -811,8 +803,16 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
     T.scale2 = scale * kb::LOG2E;
     T.most = (int)max_tokens;
     T.err = err;
-    return at::launch_rows(T, block_rows, mk, mv, sms, workspace, stream);
+    return at::launch_rows(T, block_rows, sms, workspace, stream);
   }
+  const int rows = (int)std::min<int64_t>(page_size, at::KT);
+  CUtensorMap mk, mv;
+  st = at::make_map_4d(&mk, k_cache, dtype, {Dk, page_size, Hkv, n_pages},
+                       {k_strides[1], k_strides[2], k_strides[0]}, rows, 1);
+  if (st != KB_OK) return st;
+  st = at::make_map_4d(&mv, v_cache, dtype, {Dv, page_size, Hkv, n_pages},
+                       {v_strides[1], v_strides[2], v_strides[0]}, rows, 1);
+  if (st != KB_OK) return st;
   at::TreeArgs A = {};
   A.q = q;
   A.q_tok = q_token_stride;
