@@ -25,15 +25,29 @@ __device__ __forceinline__ long long now_ns() {
   return t;
 }
 
+// A try that lets the hardware put the thread to sleep for up to `ns`.
+__device__ __forceinline__ bool mbar_try_wait_for(uint64_t* bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(ns)
+      : "memory");
+  return ok != 0;
+}
+
 // Bounded wait on a barrier phase; false on abort or after 2 s (recorded, and
 // the CTA's other roles are told through the abort flag).
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_f,
                                            uint32_t* err) {
-  if (mbar_try_wait(bar, parity)) return true;
+  // A few plain tries (waking up takes longer), then asleep: many polling warps
+  // would take issue slots from the working ones.
+  for (int i = 0; i < 2; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = now_ns();
   while (true) {
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_for(bar, parity, 200000u)) return true;
     if (*abort_f) return false;
     if (now_ns() - t0 > WAIT_NS) {
       *abort_f = 1;

@@ -72,6 +72,7 @@ constexpr int PROMPT_THREADS = 384;
 constexpr int MMA_WARP = 8, COPY_WARP = 10, CLEAN_WARP = 11;   // MMA: and 9
 constexpr int UNITS = 4;                   // units told ahead
 constexpr int MAX_STAGES = 8;
+constexpr int ROWS_COST = 4;               // paged: a unit's start and end, in steps
 constexpr int POLY_EVERY = 4;              // one in so many pairs of exponentials on the FMA pipes
 constexpr float RESCALE = 8.0f;            // log2 of the growth that moves the maximum
 
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   pdl_launch_dependents();
   Run run = {};
   if (PAGED)
-    run = find_run<2 * TILE, PROMPT_THREADS>(A.cu_q, A.context, A.total_q, A.B, A.g, A.Hkv,
+    run = find_run<2 * TILE, ROWS_COST, PROMPT_THREADS>(A.cu_q, A.context, A.total_q, A.B, A.g, A.Hkv,
                                              A.most, &B->start);
 
   // Rows outside every request: zero.
@@ -896,7 +897,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         int64_t pos = run.lo, line = B->start.base;
         Request R = B->start.r;
         int b = B->start.b, base = 0;
-        const Lengths L = {A.cu_q, A.context, A.total_q, A.g, A.Hkv, 2 * TILE, A.most};
+        const Lengths L = {A.cu_q, A.context, A.total_q, A.g, A.Hkv, 2 * TILE, A.most, ROWS_COST};
         while (pos < run.hi && ok) {
           const int64_t w = L.length(R);
           if (pos >= line + w) {
@@ -904,7 +905,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             R = L.look(++b);
             continue;
           }
-          const RunPart P = run_part(R, pos, line, run);
+          const RunPart P = run_part(R, pos, line, run, ROWS_COST);
           pos = P.until;
           if (P.t1 <= P.t0) continue;          // the run ends in the unit's start
           Unit U = {};

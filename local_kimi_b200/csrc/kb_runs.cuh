@@ -10,7 +10,6 @@ namespace attn {
 
 constexpr int KT = 64;                     // keys of a tile
 constexpr int MIN_TILES = 2;               // tiles that make another CTA worth its partial sums
-constexpr int UNIT_COST = 1;               // a unit's start and end, in tiles
 
 // A request: its rows, context, tiles of KT keys and blocks of rows.
 struct Request {
@@ -26,12 +25,13 @@ struct RunStart {
   int64_t scan[16];         // of find_run
 };
 
-// Lengths on the line.  A unit counts a tile more than it has, for the cost of its
-// start and its end.
+// Lengths on the line.  A unit counts `cost` tiles more than it has, for its start
+// and its end.
 struct Lengths {
   const int *cu, *context;
   int64_t total;
   int g, heads, rows, most; // query heads of a key/value head; rows of a block; tokens at most
+  int cost;
   __device__ __forceinline__ Request look(int b) const {
     Request R;
     int64_t end;
@@ -44,7 +44,7 @@ struct Lengths {
     return R;
   }
   __device__ __forceinline__ int64_t length(const Request& R) const {
-    return R.n ? (R.tiles + UNIT_COST) * R.blocks * heads : (int64_t)0;
+    return R.n ? (R.tiles + cost) * R.blocks * heads : (int64_t)0;
   }
 };
 
@@ -71,13 +71,13 @@ struct RunPart {
 };
 
 __device__ __forceinline__ RunPart run_part(const Request& R, int64_t pos, int64_t base,
-                                            const Run& run) {
+                                            const Run& run, int cost) {
   RunPart P;
-  const int64_t len = R.tiles + UNIT_COST;
+  const int64_t len = R.tiles + cost;
   const int unit = (int)quotient(pos - base, len);
   P.hk = unit / R.blocks;
   P.block = unit - P.hk * R.blocks;
-  const int64_t u0 = base + unit * len + UNIT_COST;     // where the unit's first tile is
+  const int64_t u0 = base + unit * len + cost;     // where the unit's first tile is
   P.until = min(run.hi, u0 + R.tiles);
   P.t0 = max(pos - u0, (int64_t)0);
   P.t1 = P.until - u0;
@@ -88,10 +88,10 @@ __device__ __forceinline__ RunPart run_part(const Request& R, int64_t pos, int64
 
 // All threads of the CTA: the line's length, this CTA's run, and in `start` (shared
 // memory, valid on return) the request it starts in.
-template <int ROWS, int THREADS>
+template <int ROWS, int COST, int THREADS>
 __device__ __forceinline__ Run find_run(const int* cu, const int* context, int64_t total_rows,
                                         int B, int g, int heads, int most, RunStart* start) {
-  const Lengths L = {cu, context, total_rows, g, heads, ROWS, most};
+  const Lengths L = {cu, context, total_rows, g, heads, ROWS, most, COST};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int WARPS = THREADS / 32;
   static_assert(WARPS <= 16, "a sum for each warp");

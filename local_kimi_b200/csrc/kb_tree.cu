@@ -8,10 +8,9 @@
 //
 // Every cached key and value is read once and meets few rows (tokens x heads
 // of a group), so the bytes of the cache bound the work.  The rows of one
-// (request, key/value head) are one A operand of 16, 32 or 64 rows for the
-// warp-level matrix instruction (more rows: several blocks, which find the
-// cache in L2); at 16 rows the 5th-generation tensor core would spend 7/8 of
-// its 128-row tile on padding and need its results moved back for the softmax.
+// (request, key/value head), at most 16 here, are one A operand of the warp-level
+// matrix instruction, whose results the softmax has in registers; the 5th-generation
+// tensor core would spend 7/8 of its 128-row tile on padding.
 //
 // Work split.  All (request, head, row block, 64-key tile) units form one line
 // of tiles, cut into equal runs, one per CTA: any mix of lengths keeps every SM
@@ -22,9 +21,9 @@
 // A CTA: one producer warp walks the run, looks pages up (32 table entries at a
 // time) and brings each tile in by tensor copies in the 128-byte swizzle (box:
 // one page's rows, 64 elements), several tiles ahead; the rows of q come the
-// same way, one row a copy.  4 or 8 consumer warps: each takes 16 rows and a
-// share of the tile's keys with its own running maximum and sum in registers,
-// so no barrier among them is needed until the run's or the unit's end.
+// same way, one row a copy.  Four consumer warps: each takes 16 of the tile's keys
+// with its own running maximum and sum in registers, so no barrier among them is
+// needed until the unit's or the run's end.
 //
 // Rows of a page past the request's end were never written and may hold
 // anything: they are masked as keys and zeroed as values.  A value that is
@@ -39,6 +38,7 @@ namespace kb {
 namespace attn {
 
 constexpr int CHUNK = KT * 128;            // bytes of 64 keys x 64 elements
+constexpr int UNIT_COST = 2;               // a unit's start and end, in tiles
 constexpr int MAX_CTAS = 320;              // counters in the workspace
 
 struct TreeArgs {
@@ -76,20 +76,19 @@ struct Segment {
   int c0, parts;            // the CTAs that share the unit: first, number
 };
 
-template <int DKP, int DVP, int MT>
+template <int DKP, int DVP>
 struct TreeShape {
-  static constexpr int RB = 16 * MT;                       // rows of a block
-  static constexpr int WK = MT == 4 ? 2 : 4;               // warps sharing a tile's keys
-  static constexpr int NW = MT * WK;                       // consumer warps
-  static constexpr int KPW = KT / WK;                      // keys of a warp
+  static constexpr int RB = 16;                            // rows of a unit
+  static constexpr int NW = 4;                             // consumer warps, sharing a tile's keys
+  static constexpr int KPW = KT / NW;                      // keys of a warp
   static constexpr int THREADS = (NW + 1) * 32;
   static constexpr int KC = DKP / 64, VC = DVP / 64;
   static constexpr int STAGE = (KC + VC) * CHUNK;
   static constexpr int QP = DKP * 2 + 16;                  // row pitch of q: no bank conflicts
   static constexpr int Q_BYTES = RB * QP;
-  static constexpr int X_BYTES = MT * (WK / 2) * 32 * (DVP / 2 + 4) * 4;
-  static constexpr int CTAS_PER_SM = MT == 1 ? 2 : 1;
-  static constexpr int BUDGET = MT == 1 ? 113 * 1024 : 224 * 1024;
+  static constexpr int X_BYTES = NW / 2 * 32 * (DVP / 2 + 4) * 4;
+  static constexpr int CTAS_PER_SM = 2;
+  static constexpr int BUDGET = 113 * 1024;
   static constexpr int FIXED = 2 * Q_BYTES + X_BYTES + 1024 + 2048;   // alignment, barriers
   static constexpr int FIT = (BUDGET - FIXED) / STAGE;
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
@@ -111,12 +110,12 @@ struct TreeBars {
   int abort_flag, joined;
 };
 
-template <int DKP, int DVP, int MT, bool F16>
-__global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
-                                  TreeShape<DKP, DVP, MT>::CTAS_PER_SM)
+template <int DKP, int DVP, bool F16>
+__global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
+                                  TreeShape<DKP, DVP>::CTAS_PER_SM)
     tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                 const TreeArgs A) {
-  using S = TreeShape<DKP, DVP, MT>;
+  using S = TreeShape<DKP, DVP>;
   using Bars = TreeBars<S::STAGES>;
   static_assert(sizeof(Bars) <= 2048, "barrier block");
   extern __shared__ uint8_t smem_raw[];
@@ -155,7 +154,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
   pdl_wait();
   pdl_launch_dependents();
 
-  const Run run = find_run<S::RB, S::THREADS>(A.cu, A.context, A.total, A.B, A.g, A.Hkv,
+  const Run run = find_run<S::RB, UNIT_COST, S::THREADS>(A.cu, A.context, A.total, A.B, A.g, A.Hkv,
                                               A.most, &B->start);
   // Rows outside every request: zero.
   {
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
     // ---------------------------------------------------------------- producer
     const uint64_t pol = l2_evict_first_policy();
     const int ps = A.ps, box = min(ps, KT), ppt = KT / box;
-    const Lengths L = {A.cu, A.context, A.total, A.g, A.Hkv, S::RB, A.most};
+    const Lengths L = {A.cu, A.context, A.total, A.g, A.Hkv, S::RB, A.most, UNIT_COST};
     int64_t pos = run.lo, base = B->start.base;
     Request R = B->start.r;
     int b = B->start.b, seg = 0, stage = 0;
@@ -190,7 +189,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
         R = L.look(++b);
         continue;
       }
-      const RunPart P = run_part(R, pos, base, run);
+      const RunPart P = run_part(R, pos, base, run, UNIT_COST);
       const int64_t t0 = P.t0, t1 = P.t1;
       const int hk = P.hk;
       pos = P.until;
@@ -297,7 +296,6 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
   }
 
   // ------------------------------------------------------------------ consumers
-  const int wm = warp / S::WK, wk = warp - wm * S::WK;
   int stage = 0, seg = 0;
   uint32_t phase = 0;
   const int frow = lane >> 2, fcol = (lane & 3) * 2;     // accumulator row and column
@@ -319,7 +317,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
     uint32_t qf[DKP / 16][4];
     {
       const uint32_t base = smem_addr(qbuf + sb * S::Q_BYTES) +
-                            (uint32_t)((wm * 16 + (lane & 15)) * S::QP + (lane >> 4) * 16);
+                            (uint32_t)(((lane & 15)) * S::QP + (lane >> 4) * 16);
 #pragma unroll
       for (int k = 0; k < DKP / 16; ++k) ldmatrix_x4(qf[k], base + k * 32);
     }
@@ -328,7 +326,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
     uint64_t word[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = wm * 16 + frow + i * 8;
+      const int r = frow + i * 8;
       tok[i] = (G.row0 + min(r, G.rows - 1)) / A.g;
       word[i] = A.mask ? (uint64_t)A.mask[G.first + tok[i]] : 0;
     }
@@ -361,7 +359,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       for (int k = 0; k < DKP / 16; ++k) {
 #pragma unroll
         for (int n = 0; n < S::KPW / 16; ++n) {
-          const int row = wk * S::KPW + n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+          const int row = warp * S::KPW + n * 16 + (lane & 7) + ((lane >> 4) & 1) * 8;
           const int piece = (k & 3) * 2 + ((lane >> 3) & 1);
           uint32_t b[4];
           ldmatrix_x4(b, smem_addr(kt) + (uint32_t)((k >> 2) * CHUNK + row * 128 +
@@ -379,19 +377,19 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
         for (int i = 0; i < S::KPW / 8; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int c = wk * S::KPW + i * 8 + fcol + (j & 1);
+            const int c = warp * S::KPW + i * 8 + fcol + (j & 1);
             if (!((valid >> c) & 1) || !sees(j >> 1, key0 + c)) s[i][j] = -INFINITY;
           }
         // Values of keys that do not exist become zero, and so do elements of
         // this step's values that are no numbers (noted for the end).  Warps
         // with the same keys may do so at the same time: they write the same.
         const bool scan = step_keys && (G.n > 1 || A.mask);
-        const uint32_t there = (uint32_t)(valid >> (wk * S::KPW));
+        const uint32_t there = (uint32_t)(valid >> (warp * S::KPW));
         bool wrote = false;
         if (scan || valid != ~0ull)
 #pragma unroll 4
           for (int x = lane; x < S::KPW * (DVP / 8); x += 32) {
-            const int r = x / (DVP / 8), c = wk * S::KPW + r, piece = x - r * (DVP / 8);
+            const int r = x / (DVP / 8), c = warp * S::KPW + r, piece = x - r * (DVP / 8);
             uint4* at = reinterpret_cast<uint4*>(vt + (piece >> 3) * CHUNK + c * 128 +
                                                  (((piece & 7) ^ (c & 7)) << 4));
             if (!((there >> r) & 1)) {
@@ -451,7 +449,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       }
 #pragma unroll
       for (int n = 0; n < S::KPW / 16; ++n) {
-        const int row = wk * S::KPW + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+        const int row = warp * S::KPW + n * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
         for (int i = 0; i < DVP / 16; ++i) {
           const int piece = (i & 3) * 2 + (lane >> 4);
@@ -478,11 +476,11 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
     constexpr int XF = DVP / 2 + 4;
-    const bool upper = G.rows > wm * 16 + 8;      // rows in the second half of the 16
+    const bool upper = G.rows > 8;      // rows in the second half of the 16
 #pragma unroll
-    for (int half = S::WK / 2; half >= 1; half >>= 1) {
-      float* x = xbuf + (size_t)(wm * (S::WK / 2) + (wk & (half - 1))) * 32 * XF + lane;
-      if (wk >= half && wk < 2 * half) {
+    for (int half = S::NW / 2; half >= 1; half >>= 1) {
+      float* x = xbuf + (size_t)(warp & (half - 1)) * 32 * XF + lane;
+      if (warp >= half && warp < 2 * half) {
 #pragma unroll
         for (int i = 0; i < DVP / 8; ++i) {
           x[(i * 4) * 32] = o[i][0];
@@ -500,7 +498,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
         x[(XF - 1) * 32] = l[1];
       }
       if (!meet(&B->all, all_phase)) return;
-      if (wk < half) {
+      if (warp < half) {
         float f0[2], f1[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -526,7 +524,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       if (!meet(&B->all, all_phase)) return;
     }
 
-    if (wk == 0) {
+    if (warp == 0) {
       if (B->odd[sb]) {
         // Values that are no numbers, from the cache, to the rows that see them.
         for (int64_t key = max(ctx, G.t0 * KT); key < min(ctx + G.n, G.t1 * KT); ++key) {
@@ -547,7 +545,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = wm * 16 + frow + h * 8;
+        const int r = frow + h * 8;
         if (r >= G.rows) continue;
         if (G.whole) {
           const int t = (G.row0 + r) / A.g;
@@ -669,40 +667,31 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP, MT>::THREADS,
 // Host.
 // ---------------------------------------------------------------------------
 
-// CTAs of a launch at most: two an SM for 16-row blocks, else one.
-static int max_ctas(int mt) { return mt == 1 ? MAX_CTAS : MAX_CTAS / 2; }
-
 // Rows (tokens x heads of a group) up to which the warp-level matrix steps are
-// used; more rows go to the 5th-generation tensor cores (kb_prompt.cu).
-constexpr int64_t MMA_ROWS = 32;
+// used; more rows go to the 5th-generation tensor cores (kb_prompt.cu), which pad
+// to 128.  Measured, 16 requests of up to 4095 tokens, 128 wide, 4 heads a group:
+// 16 rows 33 us here and 41 there, 32 rows 50 and 41.
+constexpr int64_t MMA_ROWS = 16;
 
-static int row_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-
-template <int DKP, int DVP, int MT, bool F16>
+template <int DKP, int DVP, bool F16>
 static int launch_tree(const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A, int sms,
                        void* stream) {
-  using S = TreeShape<DKP, DVP, MT>;
+  using S = TreeShape<DKP, DVP>;
   static std::mutex mu;
   static bool done[64] = {};
-  const void* fn = reinterpret_cast<const void*>(&tree_kernel<DKP, DVP, MT, F16>);
+  const void* fn = reinterpret_cast<const void*>(&tree_kernel<DKP, DVP, F16>);
   const int st = allow_smem(fn, S::SMEM, done, mu);
   if (st != KB_OK) return st;
-  const int grid = std::min(sms * S::CTAS_PER_SM, max_ctas(MT));
-  return launch(tree_kernel<DKP, DVP, MT, F16>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM,
+  const int grid = std::min(sms * S::CTAS_PER_SM, MAX_CTAS);
+  return launch(tree_kernel<DKP, DVP, F16>, dim3(grid), dim3(S::THREADS), (size_t)S::SMEM,
                 stream, mk, mv, A);
 }
 
 template <int DKP, int DVP>
-static int launch_mma(int mt, int f16, const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A,
-                       int sms, void* stream) {
-  if (f16) {
-    if (mt == 1) return launch_tree<DKP, DVP, 1, true>(mk, mv, A, sms, stream);
-    if (mt == 2) return launch_tree<DKP, DVP, 2, true>(mk, mv, A, sms, stream);
-    return launch_tree<DKP, DVP, 4, true>(mk, mv, A, sms, stream);
-  }
-  if (mt == 1) return launch_tree<DKP, DVP, 1, false>(mk, mv, A, sms, stream);
-  if (mt == 2) return launch_tree<DKP, DVP, 2, false>(mk, mv, A, sms, stream);
-  return launch_tree<DKP, DVP, 4, false>(mk, mv, A, sms, stream);
+static int launch_mma(int f16, const CUtensorMap& mk, const CUtensorMap& mv, TreeArgs& A, int sms,
+                      void* stream) {
+  return f16 ? launch_tree<DKP, DVP, true>(mk, mv, A, sms, stream)
+             : launch_tree<DKP, DVP, false>(mk, mv, A, sms, stream);
 }
 
 constexpr size_t COUNTER_BYTES = MAX_CTAS * sizeof(int);
@@ -711,8 +700,7 @@ constexpr size_t COUNTER_BYTES = MAX_CTAS * sizeof(int);
 // another): maximum and sum of a row, and up to 128 values of it.
 static size_t tree_workspace(int64_t rows) {
   if (rows > MMA_ROWS) return rows_workspace(rows);
-  const int mt = row_tiles(rows);
-  return COUNTER_BYTES + (size_t)2 * max_ctas(mt) * 16 * mt * (2 + 128) * sizeof(float);
+  return COUNTER_BYTES + (size_t)2 * MAX_CTAS * MMA_ROWS * (2 + 128) * sizeof(float);
 }
 
 }  // namespace attn
@@ -839,13 +827,12 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   A.Dk = (int)Dk;
   A.Dv = (int)Dv;
   A.scale2 = scale * kb::LOG2E;
-  const int mt = at::row_tiles(block_rows);
   A.counters = static_cast<int*>(workspace);
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at::COUNTER_BYTES);
-  A.part_o = A.part_ml + (size_t)2 * at::max_ctas(mt) * 16 * mt * 2;
+  A.part_o = A.part_ml + (size_t)2 * at::MAX_CTAS * at::MMA_ROWS * 2;
   A.most = (int)max_tokens;
   A.err = err;
-  if (Dk <= 64 && Dv <= 64) return at::launch_mma<64, 64>(mt, dtype, mk, mv, A, sms, stream);
-  if (Dk <= 128) return at::launch_mma<128, 128>(mt, dtype, mk, mv, A, sms, stream);
-  return at::launch_mma<192, 128>(mt, dtype, mk, mv, A, sms, stream);
+  if (Dk <= 64 && Dv <= 64) return at::launch_mma<64, 64>(dtype, mk, mv, A, sms, stream);
+  if (Dk <= 128) return at::launch_mma<128, 128>(dtype, mk, mv, A, sms, stream);
+  return at::launch_mma<192, 128>(dtype, mk, mv, A, sms, stream);
 }
