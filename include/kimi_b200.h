@@ -423,9 +423,11 @@ KB_API int64_t kb_step_trace_entries(const kb_step* step);
 /* 1 f16, 2 f32.                                                               */
 /* ------------------------------------------------------------------------- */
 
-/* Pages and slots for the new tokens.  Request b takes the pages it lacks for
- * context_lens[b] + new_lens[b] tokens from free_pages, from *free_head on, in
- * request order, and their ids are written to its row of block_table.
+/* Pages and slots for the new tokens.  Request b, whose pages reach
+ * reserved_lens[b] tokens (NULL, or less than the context: context_lens[b]),
+ * takes the pages it lacks for context_lens[b] + new_lens[b] tokens from
+ * free_pages, from *free_head on, in request order, and their ids are written
+ * to its row of block_table.  Lengths count up to 2^30.
  * cu_tokens [B+1]: running sums of new_lens; slots [n_tokens]: page * page_size
  * + row of each new token, -1 past the last token or without a page; positions
  * [n_tokens]: context + index, or context + depth with parents [n_tokens];
@@ -433,7 +435,8 @@ KB_API int64_t kb_step_trace_entries(const kb_step* step);
  * the token itself or an ancestor (at most 64 tokens a request).
  * *free_head_out: the next free_head; *missing: pages that were needed and not
  * given (the pool is empty, or the table too narrow).  B <= 12288. */
-KB_API int kb_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+KB_API int kb_paged_plan(const int32_t* context_lens, const int32_t* reserved_lens,
+                   const int32_t* new_lens, int64_t B,
                    int32_t* block_table, int64_t table_stride, int64_t table_width,
                    const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
                    int64_t page_size, int64_t n_tokens, const int32_t* parents,

@@ -174,7 +174,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kb_step_trace_entries": (c_int64, [c_void_p]),
     "kb_paged_plan": (
         c_int,
-        [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
          c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p],
     ),

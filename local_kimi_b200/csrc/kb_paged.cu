@@ -1,10 +1,12 @@
 // kb_paged.cu - block tables, slot maps and tree masks from request lengths,
 // and storing new keys and values by slot.
 //
-// Request b has c_b cached tokens and n_b new ones; a page holds ps token rows.
-//   need_b  = ceil((c_b + n_b) / ps) - ceil(c_b / ps)          pages to take
+// Request b has c_b cached tokens and n_b new ones; a page holds ps token rows, and
+// the request's pages reach r_b >= c_b tokens (drafted tokens that were refused leave
+// their pages to it).
+//   need_b  = max(0, ceil((c_b + n_b) / ps) - ceil(r_b / ps))  pages to take
 //   first_b = head + sum_{a < b} need_a                        in the free list
-//   table[b, ceil(c_b / ps) + i] = free[first_b + i]
+//   table[b, ceil(r_b / ps) + i] = free[first_b + i]
 //   token t of b: place p = c_b + t, slot = table[b, p / ps] * ps + p % ps
 //   with a tree: mask_t = bit t | mask_parent(t), position = c_b + depth(t)
 //
@@ -20,10 +22,11 @@ namespace kb {
 namespace paged {
 
 constexpr int THREADS = 256;
-constexpr int MAX_REQUESTS = 12288;          // three int arrays of shared memory
+constexpr int MAX_REQUESTS = 12288;          // four int arrays of shared memory
 
 struct PlanArgs {
   const int* context;
+  const int* reserved;     // NULL: context
   const int* fresh;        // new tokens of each request
   int* table;
   int64_t table_stride;
@@ -72,6 +75,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
   int* s_tok = sums;                 // [B + 1] first token of each request
   int* s_page = sums + A.B + 1;      // [B + 1] first fresh page of each request
   int* s_ctx = s_page + A.B + 1;     // [B] cached tokens
+  int* s_have = s_ctx + A.B;         // [B] pages
   __shared__ int s_part[THREADS / 32][3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t ps = (uint32_t)A.ps;
@@ -83,14 +87,15 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
 #pragma unroll 4
   for (int b = b0; b < b1; ++b) {
     const uint32_t c = length_of(A.context, b), n = length_of(A.fresh, b);
-    const int have = pages_of(c, ps), want = pages_of(c + n, ps);
-    const int need = max(0, min(want, A.width) - have);
+    const int have = pages_of(A.reserved ? max(c, length_of(A.reserved, b)) : c, ps);
+    const int want = pages_of(c + n, ps), need = max(0, min(want, A.width) - have);
     s_tok[b] = tok;
     s_page[b] = page;
     s_ctx[b] = (int)c;
+    s_have[b] = have;
     tok += (int)n;
     page += need;
-    lost += want - have - need;
+    lost += max(0, want - have) - need;
   }
   const int tok_in = warp_scan(tok, lane), page_in = warp_scan(page, lane);
   const int lost_in = warp_scan(lost, lane);
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
   }
   for (int i = at; i < pages; i += step) {
     const int b = find(s_page, A.B, i);
-    const int col = pages_of((uint32_t)s_ctx[b], ps) + i - s_page[b];
+    const int col = s_have[b] + i - s_page[b];
     A.table[(int64_t)b * A.table_stride + col] = i < avail ? __ldg(A.free_pages + head + i) : -1;
   }
   // The page of a token: a fresh one, or an entry that no CTA writes.
@@ -140,7 +145,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
     b = find(s_tok, A.B, i);
     const uint32_t c = (uint32_t)s_ctx[b];
     place = c + (uint32_t)(i - s_tok[b]);
-    const int col = (int)(place / ps), have = pages_of(c, ps);
+    const int col = (int)(place / ps), have = s_have[b];
     if (col >= A.width) return -1;
     if (col < have) return __ldg(A.table + (int64_t)b * A.table_stride + col);
     const int f = s_page[b] + col - have;
@@ -254,7 +259,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs A) {
 }  // namespace paged
 }  // namespace kb
 
-extern "C" int kb_paged_plan(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+extern "C" int kb_paged_plan(const int32_t* context_lens, const int32_t* reserved_lens,
+                             const int32_t* new_lens, int64_t B,
                              int32_t* block_table, int64_t table_stride, int64_t table_width,
                              const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
                              int64_t page_size, int64_t n_tokens, const int32_t* parents,
@@ -277,6 +283,7 @@ extern "C" int kb_paged_plan(const int32_t* context_lens, const int32_t* new_len
   const int dev = kb::bind_stream_device(stream);
   kb::paged::PlanArgs A = {};
   A.context = context_lens;
+  A.reserved = reserved_lens;
   A.fresh = new_lens;
   A.table = block_table;
   A.table_stride = table_stride;
@@ -296,11 +303,11 @@ extern "C" int kb_paged_plan(const int32_t* context_lens, const int32_t* new_len
   A.missing = missing;
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  const size_t smem = (size_t)(3 * B + 2) * sizeof(int);
-  static_assert((3 * kb::paged::MAX_REQUESTS + 2) * sizeof(int) <= 160 * 1024, "shared memory");
+  const size_t smem = (size_t)(4 * B + 2) * sizeof(int);
+  static_assert((4 * kb::paged::MAX_REQUESTS + 2) * sizeof(int) <= 200 * 1024, "shared memory");
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kb::paged::plan_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     KB_REQUIRE(e == cudaSuccess, KB_ERR_DEVICE, "paged plan: shared-memory limit: %s",
                cudaGetErrorString(e));
   }

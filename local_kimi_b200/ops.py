@@ -992,6 +992,7 @@ def paged_plan(
     num_tokens: int,
     *,
     parents: torch.Tensor | None = None,
+    reserved_lens: torch.Tensor | None = None,
 ) -> PagedPlan:
     """Pages, slots and positions for every request's new tokens.
 
@@ -1002,7 +1003,9 @@ def paged_plan(
     outputs: the sum of ``new_lens``, or more (the rest gets slot -1).  With
     ``parents`` (int32 [num_tokens], the tree parent's index in the request,
     -1 for the root) positions count the depth and ``tree_mask`` holds each
-    token's ancestors for ``tree_attention``.
+    token's ancestors for ``tree_attention``.  ``reserved_lens`` (int32, at
+    least the context) says how many tokens a request's pages already reach,
+    where refused drafted tokens left it pages beyond its context.
     """
     device = context_lens.device
     if block_table.dtype != torch.int32 or block_table.ndim != 2:
@@ -1013,6 +1016,9 @@ def paged_plan(
     new = _vector(new_lens, torch.int32, "new_lens", device, requests)
     free = _vector(free_pages, torch.int32, "free_pages", device)
     head = _vector(free_head, torch.int32, "free_head", device, 1)
+    held = None
+    if reserved_lens is not None:
+        held = _vector(reserved_lens, torch.int32, "reserved_lens", device, requests)
     if block_table.device != device:
         raise ValueError("block_table must be on the device of the other tensors")
     if requests == 0 or width == 0:
@@ -1032,7 +1038,8 @@ def paged_plan(
         par = _vector(parents, torch.int32, "parents", device, num_tokens)
         slots, mask = torch.empty(2, num_tokens, dtype=torch.long, device=device).unbind()
     _lib.call(
-        "kb_paged_plan", ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
+        "kb_paged_plan", ctx.data_ptr(), None if held is None else held.data_ptr(),
+        new.data_ptr(), requests, block_table.data_ptr(),
         max(block_table.stride(0), width), width, free.data_ptr(), free.shape[0],
         head.data_ptr(), page_size, num_tokens, None if par is None else par.data_ptr(),
         cu.data_ptr(), slots.data_ptr(), positions.data_ptr(),

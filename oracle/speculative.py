@@ -23,14 +23,15 @@ def tree_words(parents: list[int]) -> list[int]:
     return [w - (1 << 64) if w >> 63 else w for w in words]
 
 
-def plan(context, new, table, free, head, page_size, num_tokens, parents=None):
+def plan(context, new, table, free, head, page_size, num_tokens, parents=None, reserved=None):
     """(cu, slots, positions, masks, table, head, missing) as Python lists."""
     table = [list(row) for row in table]
     width, pool = len(table[0]), list(free[head:])
     cu, slots, positions, masks = [0], [], [], []
     given = missing = 0
     for b, (c, n) in enumerate(zip(context, new)):
-        have, want = -(-c // page_size), -(-(c + n) // page_size)
+        reach = c if reserved is None else max(c, reserved[b])
+        have, want = -(-reach // page_size), -(-(c + n) // page_size)
         for col in range(have, want):
             if col >= width:
                 missing += 1

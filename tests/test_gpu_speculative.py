@@ -354,6 +354,27 @@ def test_paged_plan(cuda, requests, ps, longest, most, tree, pool, narrow):
         assert got.tree_mask is None
 
 
+def test_paged_plan_with_reserved_pages(cuda):
+    # Pages that refused drafts left behind are used before new ones.
+    r = random.Random(4)
+    ps, requests = 8, 50
+    ctx = [r.randint(0, 60) for _ in range(requests)]
+    reserved = [c + r.choice([0, 0, 3, 9, 40]) for c in ctx]
+    reserved[7] = 0                          # below the context: the context counts
+    new = [r.randint(0, 30) for _ in range(requests)]
+    table = [[r.randint(0, 999) if i < -(-max(c, h) // ps) else -1 for i in range(20)]
+             for c, h in zip(ctx, reserved)]
+    free = [r.randint(0, 999) for _ in range(300)]
+    dev_table = ints(table, cuda)
+    got = ops.paged_plan(ints(ctx, cuda), ints(new, cuda), dev_table, ints(free, cuda),
+                         ints([0], cuda), ps, sum(new), reserved_lens=ints(reserved, cuda))
+    cu, slots, positions, _, want_table, head, missing = ref.plan(
+        ctx, new, table, free, 0, ps, sum(new), reserved=reserved)
+    assert got.slots.tolist() == slots and got.positions.tolist() == positions
+    assert dev_table.tolist() == want_table and got.cu_tokens.tolist() == cu
+    assert got.free_head.tolist() == [head] and got.missing.tolist() == [missing]
+
+
 def test_paged_plan_flags_bad_trees_and_short_outputs(cuda):
     _lib_errors()
     table = torch.full((1, 4), -1, dtype=torch.int32, device=cuda)

@@ -180,7 +180,7 @@ def test_c_abi_checks_arguments_before_any_launch(library):
                                      None) == 1
     assert library.kb_paged_append(16, 64, 64, 16, 64, 64, 1, 1, 64, 64, 24, s3, 16, s3, 1, 8,
                                    16, None) == 4
-    assert library.kb_paged_plan(None, None, 20000, None, 1, 1, None, 0, None, 8, 1, None, None,
+    assert library.kb_paged_plan(None, None, None, 20000, None, 1, 1, None, 0, None, 8, 1, None, None,
                                  None, None, None, None, None, None) == 6
     assert library.kb_verify_drafts(None, 10, 1, 10, 0, None, None, None, 1, 65, None, None, 10,
                                     None, None, 10, None, None, None, None, 0, None) == 6
