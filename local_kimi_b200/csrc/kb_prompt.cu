@@ -345,6 +345,18 @@ __device__ __forceinline__ void copy_quarter(const CUtensorMap& tk, const CUtens
   }
 }
 
+__device__ __forceinline__ float row_max(const float (&s)[2][32]) {
+  float m[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
+#pragma unroll
+  for (int i = 2; i < 30; i += 4)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      m[c] = max3(m[c], s[c >> 1][i + (c & 1) * 2], s[c >> 1][i + (c & 1) * 2 + 1]);
+  m[0] = max3(m[0], s[0][30], s[0][31]);
+  m[2] = max3(m[2], s[1][30], s[1][31]);
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+
 template <int DKP, int DVP, bool F16, bool PAGED>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -483,15 +495,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             for (int i = 0; i < 32; ++i)
               if (!((half[c] >> i) & 1)) s[c][i] = -INFINITY;
         }
-        float mx[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
-#pragma unroll
-        for (int i = 2; i < 30; i += 4)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            mx[c] = max3(mx[c], s[c >> 1][i + (c & 1) * 2], s[c >> 1][i + (c & 1) * 2 + 1]);
-        mx[0] = max3(mx[0], s[0][30], s[0][31]);
-        mx[2] = max3(mx[2], s[1][30], s[1][31]);
-        const float mine = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale2;
+        const float mine = row_max(s) * scale2;
         if (j == 0) {
           top = mine;
         } else if (__any_sync(0xffffffffu, mine > top + RESCALE)) {
@@ -1000,18 +1004,26 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           // (Paged: a page outside the cache was not copied, the place holds anything.)
           if (j >= 0 && (j >= U.whole || (PAGED && *const_cast<volatile uint64_t*>(
                                               &B->valid[(U.base + j) & (SEEN - 1)]) != ~0ull))) {
-            bool any = false;
+            // A quick look first: the largest magnitude of each half, as bits.
             uint4* at = reinterpret_cast<uint4*>(ring + st * S::STAGE + S::KC * BLOCK) + lane;
-#pragma unroll 8
+            uint32_t most[4] = {0, 0, 0, 0};
+#pragma unroll
             for (int i = 0; i < S::VC * BLOCK / 512; ++i) {
-              uint4 x = at[i * 32];
-              if (has_odd<F16>(x)) {
+              const uint4 x = at[i * 32];
+              most[0] = __vmaxu2(most[0], x.x & 0x7fff7fffu);
+              most[1] = __vmaxu2(most[1], x.y & 0x7fff7fffu);
+              most[2] = __vmaxu2(most[2], x.z & 0x7fff7fffu);
+              most[3] = __vmaxu2(most[3], x.w & 0x7fff7fffu);
+            }
+            const uint32_t top = __vmaxu2(__vmaxu2(most[0], most[1]), __vmaxu2(most[2], most[3]));
+            const bool odd = odd_element<F16>((uint16_t)top) || odd_element<F16>((uint16_t)(top >> 16));
+            if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+              for (int i = 0; i < S::VC * BLOCK / 512; ++i) {
+                uint4 x = at[i * 32];
                 clear_odd<F16>(x);
                 at[i * 32] = x;
-                any = true;
               }
-            }
-            if (any) {
               B->odd[U.count & 15] = U.count;
               fence_proxy_async();
             }
