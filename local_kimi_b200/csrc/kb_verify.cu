@@ -21,7 +21,9 @@
 // CTAs split the vocabulary, each joins its best (value, index) key with a
 // 64-bit atomicMax, and the request's last CTA writes the token.  Bound by the
 // bytes: the logits once, and of one row a request logits, noise and q again.
-// The exponentials (16 a clock and SM) take three quarters of that time.
+// Measured: 256 requests of up to 5 tokens, 163840 wide, with q: 121 us, 54 for the
+// rows (4.7 TB/s; special function unit 62 % busy) and 70 for the picks (6 TB/s of
+// logits, noise and q); one request of 9 tokens: 12 us, two launches and the walk.
 //
 // Rows start anywhere (an odd vocabulary): the loads begin at the row's first
 // 16-byte boundary, what lies before and after goes one by one.  The fast
