@@ -22,8 +22,8 @@
 // 64-bit atomicMax, and the request's last CTA writes the token.  Bound by the
 // bytes: the logits once, and of one row a request logits, noise and q again.
 // Measured: 256 requests of up to 5 tokens, 163840 wide, with q: 121 us, 54 for the
-// rows (4.7 TB/s; special function unit 62 % busy) and 70 for the picks (6 TB/s of
-// logits, noise and q); one request of 9 tokens: 12 us, two launches and the walk.
+// rows (4.7 TB/s; special function unit 62 % busy) and 70 for the picks (4.3
+// TB/s); one request of 9 tokens: 18.4 us with a cold cache, 14.4 replayed at once.
 //
 // Rows start anywhere (an odd vocabulary): the loads begin at the row's first
 // 16-byte boundary, what lies before and after goes one by one.  The fast
@@ -559,17 +559,20 @@ __global__ void __launch_bounds__(THREADS, 4) pick_kernel(const Args A) {
 // Segments of a row: enough CTAs (48 an SM, of at least 4096 elements) that the
 // last ones to run do not leave most SMs idle.  CTAs of a request in the second
 // kernel: about the four an SM that run at once, since each walks the tree first
-// (ten a request instead of two: 126 instead of 70 us for 256 requests).
+// (ten a request instead of two: 126 instead of 70 us for 256 requests), of at
+// least 2048 elements: for one request 163840 wide, 80 CTAs take both kernels to
+// 18.4 us, 32 CTAs 24.6, 40 CTAs 20.5, 160 CTAs 18.7 to 20.4; 16 requests and more
+// are the same with each.
 static void split(int64_t B, int64_t most, int64_t V, int sms, int* segments, int* parts) {
-  auto pick = [&](int64_t units, int64_t per_sm) {
+  auto pick = [&](int64_t units, int64_t per_sm, int64_t least, int64_t limit) {
     int64_t s = per_sm * sms / units;
-    const int64_t by_size = (V + 4095) / 4096;
+    const int64_t by_size = (V + least - 1) / least;
     if (s > by_size) s = by_size;
-    if (s > MAX_SEGMENTS) s = MAX_SEGMENTS;
+    if (s > limit) s = limit;
     return (int)(s < 1 ? 1 : s);
   };
-  *segments = pick(B * most, 48);
-  *parts = pick(B, 4);
+  *segments = pick(B * most, 48, 4096, MAX_SEGMENTS);
+  *parts = pick(B, 4, 2048, 65535);
 }
 
 static size_t power_of_two(int64_t n) {
