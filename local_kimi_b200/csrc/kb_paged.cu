@@ -15,8 +15,8 @@
 // memory and then takes its share of the fresh pages and of the new tokens,
 // each found by a binary search in the sums.  A token in a fresh page reads
 // the free list, not the table entry another CTA may be writing.  A few
-// kilobytes of traffic: the time is launch and dependent-load latency (4 us for 32
-// requests, 12 for 2048 with 200 thousand tokens).
+// kilobytes of traffic: the time is launch and dependent-load latency (32 requests:
+// 6 us; 2048: 13 us).
 #include "kb_common.cuh"
 
 namespace kb {

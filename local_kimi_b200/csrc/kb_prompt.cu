@@ -36,21 +36,21 @@
 //
 // 512 columns of tensor memory: two S of 64 for A and for B, O A, O B.  The
 // registers of the softmax are full (200 of them): holding all of O at the end
-// spills and costs a fifth of the time.
+// spills and costs a quarter more time (8192 tokens: 545 -> 696 us).
 //
 // Bound.  MMAs: 51 clocks each for S (128 x 64 x 16, both operands from shared
 // memory: reading A sets the rate; 64 clocks at 128 x 128 x 16) and 64 for P V,
 // which is 1322 clocks for a step of A and B at 128-wide heads, 1726 at 192 + 128.
-// The softmax of both tiles takes 1690 a step whatever the width: its exponentials
-// (16 a clock and SM) are half of that, the rest are the latencies of its chain
-// (wait, load, maximum, vote).  One pair of exponentials in POLY_EVERY is computed on
-// the FMA pipes (2 to 4 % at 192 + 128; every second pair loses that again).  Taking
+// The softmax of both tiles takes 1630 to 1700 a step whatever the width: its exponentials
+// (16 a clock and SM) are 768 of that by count, three in four of 16384; the rest is
+// its chain of wait, load, maximum and vote.  One pair of exponentials in POLY_EVERY is computed on
+// the FMA pipes (2 to 4 % at 192 + 128; every second or third pair is no better).  Taking
 // the weights relative to the last step's maximum, beside the new one, is slower
-// (1850).  With steps of 128 keys and one S a tile, each tile's MMAs waited for its
+// (1830).  With steps of 128 keys and one S a tile, each tile's MMAs waited for its
 // softmax in turn: 3600 clocks for 128 keys at 128 wide, 4430 at 192 + 128.
 // Measured: 8192 tokens x 32 heads, 192 + 128: 545 us alone (1260 TFLOP/s), 656 back
 // to back under the power cap (1047; cuBLAS 1403); 24 prompts of 1 to 2047 tokens,
-// 32/8 heads of 128: 139 us (736 TFLOP/s; units of few steps, 5600 clocks of start and
+// 32/8 heads of 128: 139 us (736 TFLOP/s; units of few steps, 5500 clocks of start and
 // end each).
 //
 // Paged cache (PAGED).  A unit is up to 256 rows (token * group + head) of one
@@ -59,8 +59,9 @@
 // form one line cut into equal runs, one per CTA, as in kb_tree.cu; a unit that
 // falls to several CTAs is joined from fp32 partial sums by the CTA that finishes
 // last.  16 trees of up to 24 tokens, 4 heads a group, up to 4095 cached: 44 us; the
-// softmax of one tile takes 1600 clocks a step (its 32 KB would take 1380 from
-// memory), a CTA's start 6 us, partial sums and joining 5 to 8 us.  Keys and values come page by page; q too by tensor copies where one tile
+// a step of one tile
+// takes 1.1 us, a CTA's first scores are there after 6, and partial sums take 3 us,
+// counting them 1, joining them 5.  Keys and values come page by page; q too by tensor copies where one tile
 // holds a request's rows, else by gathered 16-byte copies into the same layout.
 //
 // In the last tiles of a unit some rows do not see some keys, or the tile

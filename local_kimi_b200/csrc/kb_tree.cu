@@ -19,8 +19,8 @@
 // (in CTA order, so results do not change from run to run).
 //
 // Measured: 32 requests of 512 to 8192 tokens, 32 heads of 192 + 128: 315 us, 6.56
-// TB/s (the measured copy bandwidth); one request of 4096: 23 us of 12.8, its start
-// (lengths, table, first page: 4 us) and the joining of its 9 parts (3 us) on top.
+// TB/s (the measured copy bandwidth); one request of 4096: 23 us, of which its bytes
+// are 12.8; the rest is a start of dependent loads and the joining of 9 parts a head.
 //
 // A CTA: one producer warp walks the run, looks pages up (32 table entries at a
 // time) and brings each tile in by tensor copies in the 128-byte swizzle (box:
