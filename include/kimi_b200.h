@@ -457,6 +457,7 @@ KB_API int kb_paged_append(const uint16_t* k, int64_t k_token_stride, int64_t k_
  * fp32 or NULL (natural logarithm).  A query without keys gives 0 and
  * -infinity.  Hq a multiple of Hkv; Dk <= 192, Dv <= 128, multiples of 8.
  * max_q: no request has more queries (rows past it are not written).  scale > 0.
+ * Without requests (B 0) nothing is written, here and in kb_tree_attention.
  * dtype 0 or 1, the outputs' type too; products and sums in fp32. */
 KB_API int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                    const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,

@@ -1136,6 +1136,15 @@ def _scale_of(scale: float | None, dk: int) -> float:
     return float(scale)
 
 
+def _no_requests(q: torch.Tensor, dv: int, return_lse: bool):
+    """What rows outside every request get, where there is no request."""
+    total, hq, _ = q.shape
+    out = q.new_zeros(total, hq, dv)
+    if not return_lse:
+        return out
+    return out, torch.full((total, hq), float("-inf"), device=q.device)
+
+
 def prompt_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -1182,13 +1191,16 @@ def prompt_attention(
         ck = _vector(cu_seqlens_k, torch.int32, "cu_seqlens_k", device, requests + 1)
     if max_seqlen < 0 or (total and not max_seqlen):
         raise ValueError("max_seqlen must not be negative, nor 0 with tokens")
+    scale = _scale_of(scale, dk)
+    if requests == 0:
+        return _no_requests(q, dv, return_lse)
     out = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
     lse = torch.empty(total, hq, dtype=torch.float32, device=device) if return_lse else None
     _lib.call(
         "kb_prompt_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), kr.data_ptr(),
         kr.stride(0), kr.stride(1), vr.data_ptr(), vr.stride(0), vr.stride(1),
         _ELEMENT[q.dtype], cq.data_ptr(), ck.data_ptr(), requests, total, keys, max_seqlen, hq,
-        hkv, dk, dv, _scale_of(scale, dk), out.data_ptr(),
+        hkv, dk, dv, scale, out.data_ptr(),
         None if lse is None else lse.data_ptr(), _raw_stream(device),
     )
     return out if lse is None else (out, lse)
@@ -1251,9 +1263,12 @@ def tree_attention(
         if max_tokens > MAX_TREE_TOKENS:
             raise ValueError(f"a masked tree has at most {MAX_TREE_TOKENS} tokens")
         mask = _vector(tree_mask, torch.long, "tree_mask", device, total)
+    scale = _scale_of(scale, dk)
+    if requests == 0:
+        return _no_requests(q, dv, return_lse)
     out = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
     lse = torch.empty(total, hq, dtype=torch.float32, device=device) if return_lse else None
-    if total == 0 or requests == 0:
+    if total == 0:
         return out if lse is None else (out, lse)
     stream = _raw_stream(device)
     ws = _zeroed("tree_attention", device, stream,
@@ -1263,7 +1278,7 @@ def tree_attention(
         v_cache.data_ptr(), vs, _ELEMENT[q.dtype], pages, page_size, table.data_ptr(),
         max(table.stride(0), width), width, ctx.data_ptr(), cu.data_ptr(),
         None if mask is None else mask.data_ptr(), requests, total, max_tokens, hq, hkv, dk, dv,
-        _scale_of(scale, dk), out.data_ptr(),
+        scale, out.data_ptr(),
         None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream,
     )
     return out if lse is None else (out, lse)

@@ -220,3 +220,30 @@ def test_oracle_verification_known_answers():
     got = ref.verify(logits, torch.tensor([0, 0, 1]), [-1, 0, 0], [0, 3], 3,
                      torch.tensor([0.0, 0.9, 0.99]), torch.ones(1, 2), torch.ones(1))
     assert got == ([[1, 0, -1]], [[0, 2, -1]], [1])
+
+
+def test_scales_must_be_positive(any_device):
+    x, cache = heads(), torch.zeros((2, 8, 2, 64), dtype=torch.bfloat16)
+    for scale in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="scale must be positive"):
+            ops.prompt_attention(x, x, x, i32(0, 4), 4, scale=scale)
+        with pytest.raises(ValueError, match="scale must be positive"):
+            ops.tree_attention(x, cache, cache, i32(0, 1)[None], i32(3), i32(0, 4), 4,
+                               scale=scale)
+
+
+def test_prompts_with_tokens_need_a_longest_length(any_device):
+    x = heads()
+    with pytest.raises(ValueError, match="max_seqlen"):
+        ops.prompt_attention(x, x, x, i32(0, 4), 0)
+
+
+def test_rows_without_a_request_are_zero(any_device):
+    x, cache = heads(), torch.zeros((2, 8, 2, 64), dtype=torch.bfloat16)
+    none = torch.zeros(0, dtype=torch.int32)
+    for out, lse in (
+            ops.prompt_attention(x, x, x, i32(0), 4, return_lse=True),
+            ops.tree_attention(x, cache, cache, torch.zeros((0, 2), dtype=torch.int32), none,
+                               i32(0), 4, return_lse=True)):
+        assert out.shape == (4, 2, 64) and not out.any()
+        assert lse.shape == (4, 2) and (lse == -float("inf")).all()
