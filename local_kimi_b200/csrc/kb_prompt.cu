@@ -249,8 +249,7 @@ __device__ __forceinline__ void join_parts(const PromptArgs& A, const Unit& U, i
     const float2 ml =
         __ldcg(reinterpret_cast<const float2*>(A.part_ml + (slot(c) * A.part_rows + row) * 2));
     const float t = fmaxf(top, ml.x);
-    if (t == -INFINITY) continue;
-    sum = sum * exp2_fast(top - t) + ml.y * exp2_fast(ml.x - t);
+    sum = sum * part_factor(top, t) + ml.y * part_factor(ml.x, t);
     top = t;
   }
   const bool none = sum == 0.f;
@@ -265,8 +264,9 @@ __device__ __forceinline__ void join_parts(const PromptArgs& A, const Unit& U, i
       for (int k = 0; k < 16; ++k)
         v[k] = __ldcg(reinterpret_cast<const float4*>(
             A.part_o + ((slot(c) * (DVP / 4) + d / 4 + k) * A.part_rows + row) * 4));
-      const float f = m == -INFINITY ? 0.f : exp2_fast(m - top) * inv;
-      if (f == 0.f) continue;
+      // A part that counts nothing still hands on values that are no numbers, as a
+      // weight of zero does in a tile.
+      const float f = part_factor(m, top) * inv;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         o[4 * k] += v[k].x * f;

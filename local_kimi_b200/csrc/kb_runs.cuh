@@ -159,6 +159,13 @@ __device__ __forceinline__ int page_ids(const Args& A, int b, int64_t end, int64
   return __shfl_sync(0xffffffffu, ids, entry - have + min(lane, pages - 1));
 }
 
+// What the sums of a part with the maximum m (log2) count in sums relative to t, at least
+// m.  Where neither saw a score above -infinity both count as they are: their sums are
+// zero, or not a number where their scores were, and that has to stay.
+__device__ __forceinline__ float part_factor(float m, float t) {
+  return t == -INFINITY ? 1.f : exp2_fast(m - t);
+}
+
 // What the tensor-core form for many rows needs of a tree attention call.
 struct TreeCall {
   const uint16_t *q, *k, *v;

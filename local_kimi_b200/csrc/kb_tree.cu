@@ -508,8 +508,8 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
         for (int i = 0; i < 2; ++i) {
           const float om = x[(XF - 4 + i) * 32], ol = x[(XF - 2 + i) * 32];
           const float t = fmaxf(m[i], om);
-          f0[i] = t == -INFINITY ? 1.f : exp2_fast(m[i] - t);
-          f1[i] = t == -INFINITY ? 1.f : exp2_fast(om - t);
+          f0[i] = part_factor(m[i], t);
+          f1[i] = part_factor(om, t);
           m[i] = t;
           l[i] = l[i] * f0[i] + ol * f1[i];
         }
@@ -613,8 +613,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
               const float t = fmaxf(tm, ml[u].x);
-              if (t == -INFINITY) continue;
-              const float f0 = exp2_fast(tm - t), f1 = exp2_fast(ml[u].x - t);
+              const float f0 = part_factor(tm, t), f1 = part_factor(ml[u].x, t);
               tm = t;
               tl = tl * f0 + ml[u].y * f1;
               acc[0] = acc[0] * f0 + v[u].x * f1;
@@ -635,8 +634,7 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
               for (int u = 1; u < share; ++u) {
                 const float* y = xbuf + (tid + u * (T / share)) * 6;
                 const float t = fmaxf(tm, y[0]);
-                if (t == -INFINITY) continue;
-                const float f0 = exp2_fast(tm - t), f1 = exp2_fast(y[0] - t);
+                const float f0 = part_factor(tm, t), f1 = part_factor(y[0], t);
                 tm = t;
                 tl = tl * f0 + y[1] * f1;
 #pragma unroll

@@ -557,3 +557,42 @@ def test_operators_in_a_cuda_graph(cuda):
     assert torch.equal(held[1].tokens, eager[1].tokens)
     check_attention(held[0], None, want[0], None, want[2], torch.bfloat16)
     assert math.isfinite(float(held[0].float().sum()))
+
+
+# ---------------------------------------------------------------------------
+# what is visible and no finite number
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("new,heads,kv", [([1, 1], 4, 2), ([5, 2], 6, 2), ([24, 5], 8, 2),
+                                          ([60, 3], 8, 2)])
+def test_tree_attention_a_query_that_is_no_number_is_seen(cuda, new, heads, kv):
+    # Over a context that several CTAs share, as over one that a single CTA has.
+    dev, _ = paged_case(cuda, torch.bfloat16, [6000, 20], new, heads, kv, 128, 128, 16, 41)
+    base, base_lse = ops.tree_attention(**dev, return_lse=True)
+    last = sum(new) - 1
+    for value in (float("nan"), float("inf")):
+        q = dev["q"].clone()
+        q[0, 1] = value
+        q[last, 0] = value
+        out, lse = ops.tree_attention(**{**dev, "q": q}, return_lse=True)
+        for t, h in ((0, 1), (last, 0)):
+            assert torch.isnan(out[t, h]).all() and torch.isnan(lse[t, h])
+            out[t, h], lse[t, h] = base[t, h], base_lse[t, h]
+        assert torch.equal(out, base) and torch.equal(lse, base_lse)
+
+
+@pytest.mark.parametrize("ctx", [40, 6000])
+@pytest.mark.parametrize("new", [1, 24])
+def test_tree_attention_infinite_values_meet_weights_of_zero(cuda, ctx, new):
+    # The last cached key takes all the weight; the first one's value is infinite, and
+    # zero times infinity is no number, whichever CTA had the key.
+    dev, _ = paged_case(cuda, torch.bfloat16, [ctx], [new], 4, 2, 128, 128, 16, 42)
+    table, kc, vc = dev["block_table"][0], dev["k_cache"], dev["v_cache"]
+    dev["q"].copy_(torch.ones_like(dev["q"]))
+    page, row = divmod(ctx - 1, 16)
+    kc[int(table[page]), row] = 64.0          # score 724, the others' are of order ten
+    vc[int(table[0]), 0, :, :8] = float("inf")
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    assert torch.isfinite(lse).all() and torch.isfinite(out[..., 8:]).all()
+    assert not torch.isfinite(out[..., :8]).any()
