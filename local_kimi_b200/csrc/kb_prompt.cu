@@ -188,7 +188,7 @@ constexpr int WALKERS = 8 + 3;               // softmax warps, two of MMAs, clea
 // whole number (left in the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a
 // polynomial of degree 4 fitted here to least relative error (2.7e-6, and
 // 4e-8 on average, far below the rounding of the weights), n added to the exponent.  Below
-// 2^-126 the result stays there.
+// 2^-126, at -infinity and for what is no number the result is 2^-126.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
   const float2 big = make_float2(12582912.f, 12582912.f);
   const float2 nbig = make_float2(-12582912.f, -12582912.f);
@@ -358,16 +358,17 @@ __device__ __forceinline__ void copy_quarter(const CUtensorMap& tk, const CUtens
   }
 }
 
+// Largest score of a row's step; not a number where a score is none.
 __device__ __forceinline__ float row_max(const float (&s)[2][32]) {
   float m[4] = {s[0][0], s[0][1], s[1][0], s[1][1]};
 #pragma unroll
   for (int i = 2; i < 30; i += 4)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      m[c] = max3(m[c], s[c >> 1][i + (c & 1) * 2], s[c >> 1][i + (c & 1) * 2 + 1]);
-  m[0] = max3(m[0], s[0][30], s[0][31]);
-  m[2] = max3(m[2], s[1][30], s[1][31]);
-  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+      m[c] = max3_nan(m[c], s[c >> 1][i + (c & 1) * 2], s[c >> 1][i + (c & 1) * 2 + 1]);
+  m[0] = max3_nan(m[0], s[0][30], s[0][31]);
+  m[2] = max3_nan(m[2], s[1][30], s[1][31]);
+  return max_nan(max3_nan(m[0], m[1], m[2]), m[3]);
 }
 
 template <int DKP, int DVP, bool F16, bool PAGED>
@@ -509,6 +510,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
               if (!((half[c] >> i) & 1)) s[c][i] = -INFINITY;
         }
         const float mine = row_max(s) * scale2;
+        // A score that is no number or infinite (also only once scaled) makes the row no
+        // number, whatever the polynomial makes of its weight.
+        if (!(mine < INFINITY)) sum = NAN;
         if (j == 0) {
           top = mine;
         } else if (__any_sync(0xffffffffu, mine > top + RESCALE)) {
@@ -599,7 +603,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         tc::tc_fence_after();
         odd = *const_cast<volatile int*>(&B->odd[U.count & 15]) == U.count;
       }
-      // A row that saw no key (or only keys of score -infinity) is zero.
+      // A row that saw no key (or only keys of score -infinity, to which the polynomial
+      // gives its least weight) is zero.
+      if (top == -INFINITY && sum == sum) sum = 0.f;
       const bool none = sum == 0.f || (!PAGED && limit < 0);
       const float inv = !whole ? 1.f : none ? 0.f : 1.f / sum;
 #pragma unroll

@@ -596,3 +596,69 @@ def test_tree_attention_infinite_values_meet_weights_of_zero(cuda, ctx, new):
     out, lse = ops.tree_attention(**dev, return_lse=True)
     assert torch.isfinite(lse).all() and torch.isfinite(out[..., 8:]).all()
     assert not torch.isfinite(out[..., :8]).any()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("key", list(range(64, 80)) + [127])
+def test_prompt_attention_a_visible_key_that_is_no_number_is_seen(cuda, value, key):
+    # At any place of a step that all rows of a tile see whole.
+    gen = torch.Generator().manual_seed(11)
+    q = torch.rand(400, 4, 64, generator=gen).add_(0.1).bfloat16().to(cuda)
+    k, v = (torch.randn(400, 2, 64, generator=gen).bfloat16().to(cuda) for _ in range(2))
+    cu = ints([0, 400], cuda)
+    base, base_lse = ops.prompt_attention(q, k, v, cu, 400, return_lse=True)
+    k[key, 1] = value                        # its score is infinite or not a number
+    out, lse = ops.prompt_attention(q, k, v, cu, 400, return_lse=True)
+    assert torch.equal(out[:, :2], base[:, :2]) and torch.equal(lse[:, :2], base_lse[:, :2])
+    assert torch.equal(out[:key], base[:key]) and torch.equal(lse[:key], base_lse[:key])
+    assert torch.isnan(out[key:, 2:]).all() and not torch.isfinite(lse[key:, 2:]).any()
+
+
+@pytest.mark.parametrize("new", [1, 24, 60])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_tree_attention_a_visible_key_that_is_no_number_is_seen(cuda, new, value):
+    dev, _ = paged_case(cuda, torch.float16, [3000], [new], 8, 2, 64, 64, 16, 43)
+    dev["q"].abs_().add_(0.1)
+    base, base_lse = ops.tree_attention(**dev, return_lse=True)
+    for key in (0, 6, 15, 70, 1031, 2990):
+        page, row = int(dev["block_table"][0, key // 16]), key % 16
+        held = dev["k_cache"][page, row, 1].clone()
+        dev["k_cache"][page, row, 1] = value
+        out, lse = ops.tree_attention(**dev, return_lse=True)
+        assert torch.equal(out[:, :4], base[:, :4]) and torch.equal(lse[:, :4], base_lse[:, :4])
+        assert torch.isnan(out[:, 4:]).all() and not torch.isfinite(lse[:, 4:]).any()
+        dev["k_cache"][page, row, 1] = held
+
+
+def test_attention_scores_of_minus_infinity_count_nothing(cuda):
+    # Rows with no other score are zero; the others see the finite keys alone.
+    gen = torch.Generator().manual_seed(12)
+    q = torch.rand(100, 2, 64, generator=gen).add_(0.1).bfloat16().to(cuda)
+    k, v = (torch.randn(400, 2, 64, generator=gen).bfloat16().to(cuda) for _ in range(2))
+    k[:350] = float("-inf")
+    out, lse = ops.prompt_attention(q, k, v, ints([0, 100], cuda), 100,
+                                    cu_seqlens_k=ints([0, 400], cuda), return_lse=True)
+    assert not out[:50].any() and (lse[:50] == float("-inf")).all()
+    # Queries 50 to 99 see the finite keys 350 to 350 + t - 50.
+    want = ref.prompt_attention(q[50:].cpu(), k[350:].cpu(), v[350:].cpu(), [0, 50], [0, 50],
+                                0.125)
+    check_attention(out[50:], lse[50:], *want, torch.bfloat16)
+    # The same over pages: one token a request, and more than 16 rows.
+    for n in (1, 40):
+        cache = [t[:384].view(24, 16, 2, 64) for t in (k, v)]
+        table = torch.arange(24, dtype=torch.int32, device=cuda)[None]
+        out, lse = ops.tree_attention(q[:n], *cache, table, ints([340 - n], cuda), ints([0, n], cuda),
+                                      n, return_lse=True)
+        assert not out.any() and (lse == float("-inf")).all()
+
+
+def test_attention_scores_that_leave_fp32_are_no_numbers(cuda):
+    # Finite products of 1.6e38 times a scale of 4.
+    for n in (1, 300):
+        q = torch.zeros(n, 1, 64, dtype=torch.bfloat16, device=cuda)
+        k, v = q.clone(), torch.ones_like(q)
+        q[:, :, 0] = 1.25e19
+        k[:, :, 0] = 1.25e19
+        out, lse = ops.prompt_attention(q, k, v, ints([0, n], cuda), n, scale=4.0,
+                                        return_lse=True)
+        assert torch.isnan(out).all() and not torch.isfinite(lse).any()
