@@ -19,7 +19,9 @@
 // row segment, fp32.  pick_kernel joins the segments, walks the tree from
 // shared memory, and scans the last node's row with the noise (and q): its
 // CTAs split the vocabulary, each joins its best (value, index) key with a
-// 64-bit atomicMax, and the request's last CTA writes the token.  Bound by the
+// 64-bit atomicMax, and the request's last CTA writes the token.  What the second launch
+// takes from the first is in the call's own workspace, so calls from several threads
+// may meet on a stream in any order.  Bound by the
 // bytes: the logits once, and of one row a request logits, noise and q again.
 // Measured: 256 requests of up to 5 tokens, 163840 wide, with q: 121 us, 54 for the
 // rows (4.7 TB/s; special function unit 62 % busy) and 70 for the picks (4.3
@@ -77,7 +79,7 @@ struct Args {
   int* path;                // [B, most]
   int* accepted;            // [B]
   Stat* stats;              // [rows][segments]
-  Race* race;               // [B], zero between calls
+  Race* race;               // [B], zeroed by row_kernel
   int segments;             // of a row in row_kernel
   int parts;                // CTAs of a request in pick_kernel
   uint32_t* err;
@@ -266,6 +268,7 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const Args A) {
   pdl_wait();
   pdl_launch_dependents();
   const int t = blockIdx.x / A.segments, seg = blockIdx.x - t * A.segments;
+  if (blockIdx.x == 0 && threadIdx.x == 0) A.race[blockIdx.y] = Race{0, 0, 0};
   int64_t first;
   int n;
   request(A, blockIdx.y, first, n);
@@ -531,10 +534,7 @@ __global__ void __launch_bounds__(THREADS, 4) pick_kernel(const Args A) {
     atomicMax(&A.race[b].best, key);
     __threadfence();
     s_last = atomicAdd(&A.race[b].arrived, 1) == A.parts - 1;
-    if (s_last) {
-      s_won = atomicExch(&A.race[b].best, 0ull);
-      A.race[b].arrived = 0;
-    }
+    if (s_last) s_won = atomicMax(&A.race[b].best, 0ull);
   }
   __syncthreads();
   if (!s_last) return;
@@ -581,17 +581,14 @@ static size_t power_of_two(int64_t n) {
   return p;
 }
 
-// The counters of up to MAX_REQUESTS requests come first, at the same place
-// for every call, so that whatever call used the buffer before left them zero.
-constexpr int MAX_REQUESTS = 65536;
-constexpr size_t COUNTER_BYTES = MAX_REQUESTS * sizeof(Race);
+static size_t race_bytes(int64_t B) { return power_of_two(B) * sizeof(Race); }
 
 }  // namespace verify
 }  // namespace kb
 
 extern "C" size_t kb_verify_drafts_workspace_size(int64_t B, int64_t rows) {
   if (B <= 0 || rows < 0) return 0;
-  return kb::verify::COUNTER_BYTES +
+  return kb::verify::race_bytes(B) +
          kb::verify::power_of_two(rows) * kb::verify::MAX_SEGMENTS * sizeof(kb::verify::Stat);
 }
 
@@ -621,7 +618,7 @@ extern "C" int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t 
              KB_ERR_NULL_POINTER, "verify: NULL pointer");
   const size_t need = kb_verify_drafts_workspace_size(B, rows);
   KB_REQUIRE(workspace_bytes >= need && ((uintptr_t)workspace & 255) == 0, KB_ERR_WORKSPACE,
-             "verify: workspace of %zu bytes (256-byte aligned, zeroed once) required, %zu given",
+             "verify: workspace of %zu bytes (256-byte aligned) required, %zu given",
              need, workspace_bytes);
   const int dev = kb::bind_stream_device(stream);
   v::Args A = {};
@@ -648,7 +645,7 @@ extern "C" int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t 
   A.path = path;
   A.accepted = accepted;
   A.race = static_cast<v::Race*>(workspace);
-  A.stats = reinterpret_cast<v::Stat*>(static_cast<uint8_t*>(workspace) + v::COUNTER_BYTES);
+  A.stats = reinterpret_cast<v::Stat*>(static_cast<uint8_t*>(workspace) + v::race_bytes(B));
   v::split(B, max_tokens, V, kb::num_sms(dev), &A.segments, &A.parts);
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");

@@ -28,6 +28,7 @@ prompt_attention, tree_attention, verify_drafts.
 
 from __future__ import annotations
 
+import threading
 from ctypes import c_float, c_int64, c_size_t, c_void_p
 from typing import NamedTuple
 
@@ -969,6 +970,11 @@ def _raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _capturing() -> bool:
+    """Whether the current stream records a CUDA graph."""
+    return torch._C._cuda_isCurrentStreamCapturing()
+
+
 def _zeroed(kind: str, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of the operators below, kept per (kind, device, stream, size).
 
@@ -979,6 +985,33 @@ def _zeroed(kind: str, device: torch.device, stream: int, nbytes: int) -> torch.
     ws = _WORKSPACES.get(key)
     if ws is None:
         ws = _WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return ws
+
+
+class _ThreadScratch(threading.local):
+    def __init__(self) -> None:
+        self.held: dict[tuple, torch.Tensor] = {}
+
+
+_THREAD_SCRATCH = _ThreadScratch()
+
+
+def _verify_scratch(device: torch.device, stream: int, requests: int, rows: int) -> torch.Tensor:
+    """Scratch of verify_drafts, with anything in it.
+
+    Its calls are two launches, and another thread's may come between them on the
+    stream, so each thread keeps its own, for sizes up to the next power of two; calls
+    of one thread follow each other on a stream.  A call in a graph gets its own from
+    the graph's memory, since graphs may be replayed on other streams.
+    """
+    most = (requests - 1).bit_length(), max(rows - 1, 0).bit_length()
+    key = (device.index, stream, *most)
+    ws = None if _capturing() else _THREAD_SCRATCH.held.get(key)
+    if ws is None:
+        nbytes = _lib.lib().kb_verify_drafts_workspace_size(1 << most[0], 1 << most[1])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        if not _capturing():
+            _THREAD_SCRATCH.held[key] = ws
     return ws
 
 
@@ -1344,8 +1377,7 @@ def verify_drafts(
         return Verification(out, path, accepted)
     x, e = _unit_rows(logits), _unit_rows(noise)
     stream = _raw_stream(device)
-    ws = _zeroed("verify_drafts", device, stream,
-                 _lib.lib().kb_verify_drafts_workspace_size(requests, rows))
+    ws = _verify_scratch(device, stream, requests, rows)
     _lib.call(
         "kb_verify_drafts", x.data_ptr(), max(x.stride(0), vocab), rows, vocab,
         _ELEMENT[x.dtype], tok.data_ptr(), None if par is None else par.data_ptr(),

@@ -662,3 +662,20 @@ def test_attention_scores_that_leave_fp32_are_no_numbers(cuda):
         out, lse = ops.prompt_attention(q, k, v, ints([0, n], cuda), n, scale=4.0,
                                         return_lse=True)
         assert torch.isnan(out).all() and not torch.isfinite(lse).any()
+
+
+@pytest.mark.parametrize("greedy", [0, 9])
+def test_verify_drafts_scratch_may_hold_anything(cuda, greedy, monkeypatch):
+    c = verify_case(9, 5000, 5, True, False, greedy, torch.bfloat16, 44)
+    want = ref.verify(c["logits"], c["tokens"], c["parents"], c["cu"], 5, c["coin"], c["noise"],
+                      c["temps"])
+    real, kept = _lib.call, []
+
+    def call(name, *args):
+        for fill in (255, 1):
+            kept.append(torch.full((args[-2],), fill, dtype=torch.uint8, device=cuda))
+            real(name, *args[:-3], kept[-1].data_ptr(), *args[-2:])
+
+    monkeypatch.setattr(_lib, "call", call)
+    got = run_verify(c, cuda, True)
+    assert got.accepted.tolist() == want[2] and got.tokens.tolist() == want[0]

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -247,3 +248,29 @@ def test_rows_without_a_request_are_zero(any_device):
                                i32(0), 4, return_lse=True)):
         assert out.shape == (4, 2, 64) and not out.any()
         assert lse.shape == (4, 2) and (lse == -float("inf")).all()
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+def test_verification_calls_in_flight_share_no_scratch(library, any_device, monkeypatch, capturing):
+    # Another thread's call on the same stream may come before the first one is done, and
+    # a graph may be replayed while another runs.
+    seen = []
+
+    def call(name, *args):
+        seen.append((args[-3], args[-2]))
+        if len(seen) == 1:
+            other = threading.Thread(target=again)
+            other.start()
+            other.join()
+
+    def again():
+        return ops.verify_drafts(torch.zeros(3, 10), torch.zeros(3, dtype=torch.long), i32(0, 3),
+                                 3, torch.zeros(3), torch.ones(1, 10), torch.ones(1))
+
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(ops, "_capturing", lambda: capturing, raising=False)
+    monkeypatch.setattr(_lib, "call", call)
+    again()
+    (a, n), (b, m) = seen
+    assert min(n, m) >= library.kb_verify_drafts_workspace_size(1, 3) > 0
+    assert a + n <= b or b + m <= a
