@@ -75,6 +75,11 @@ KB_API int kb_get_pdl(void);
  * outside the vocabulary (the token is never taken). */
 KB_API int kb_device_errors(void* stream, uint32_t* out_bits);
 
+/* *out_id: a number of the graph capture that the stream is in, another one for
+ * each capture, or 0 outside of one.  For callers that keep workspaces: scratch
+ * with counters belongs to one graph, which zeroes it. */
+KB_API int kb_stream_capture_id(void* stream, uint64_t* out_id);
+
 /* ------------------------------------------------------------------------- */
 /* Codec (engine/quant/w4a16.py:68-105 quantise).                              */
 /* ------------------------------------------------------------------------- */
@@ -471,9 +476,9 @@ KB_API int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_
  * context and, of its step, the tokens whose bit is set in its tree_mask word
  * (NULL: itself and those before it).  max_tokens: no request has more tokens
  * (at most 64 with tree_mask).  page_size: a power of two from 8 to 4096.
- * Other arguments as kb_prompt_attention; the workspace of
- * kb_tree_attention_workspace_size bytes is zeroed once and left zeroed where
- * a call needs it so. */
+ * Other arguments as kb_prompt_attention; the first 4096 bytes of the workspace of
+ * kb_tree_attention_workspace_size bytes are zeroed once and left zero by each call.
+ * Calls that share a workspace follow each other on a stream, or in a graph. */
 KB_API size_t kb_tree_attention_workspace_size(int64_t group, int64_t max_tokens);
 KB_API int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                    const uint16_t* k_cache, const int64_t* k_strides, const uint16_t* v_cache,

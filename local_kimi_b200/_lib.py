@@ -9,7 +9,7 @@ implementation: a missing library raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libkimi_b200.so")
@@ -54,6 +54,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kb_set_pdl": (None, [c_int]),
     "kb_get_pdl": (c_int, []),
     "kb_device_errors": (c_int, [c_void_p, ctypes.POINTER(c_uint32)]),
+    "kb_stream_capture_id": (c_int, [c_void_p, ctypes.POINTER(c_uint64)]),
     "kb_w4a16_quantise": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],

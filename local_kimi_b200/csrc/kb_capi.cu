@@ -95,4 +95,17 @@ int kb_device_errors(void* stream, uint32_t* out_bits) {
   return KB_OK;
 }
 
+int kb_stream_capture_id(void* stream, uint64_t* out_id) {
+  kb::clear_error();
+  KB_REQUIRE(out_id != nullptr, KB_ERR_NULL_POINTER, "out_id is NULL");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e =
+      cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id);
+  KB_REQUIRE(e == cudaSuccess, KB_ERR_LAUNCH, "reading the stream's capture failed: %s",
+             cudaGetErrorString(e));
+  *out_id = status == cudaStreamCaptureStatusNone ? 0 : id;
+  return KB_OK;
+}
+
 }  // extern "C"

@@ -1098,6 +1098,7 @@ static int launch_widths(int64_t Dk, int64_t Dv, int f16, const CUtensorMap& mq,
 
 constexpr int ROW_CTAS = 160;                // CTAs the workspace of the paged form is made for
 constexpr size_t ROW_COUNTERS = 2 * ROW_CTAS * sizeof(int);
+static_assert(ROW_COUNTERS <= ZEROED, "counters where callers zero");
 
 // Counters, then two partial sums a CTA: maximum and sum, 128 values, of the 128 or
 // 256 rows of a unit.

@@ -9,6 +9,7 @@ namespace kb {
 namespace attn {
 
 constexpr int KT = 64;                     // keys of a tile
+constexpr size_t ZEROED = 4096;            // bytes at a workspace's start that callers zero
 constexpr int MIN_TILES = 2;               // tiles that make another CTA worth its partial sums
 
 // A request: its rows, context, tiles of KT keys and blocks of rows.

@@ -697,6 +697,7 @@ static int launch_mma(int f16, const CUtensorMap& mk, const CUtensorMap& mv, Tre
 }
 
 constexpr size_t COUNTER_BYTES = MAX_CTAS * sizeof(int);
+static_assert(COUNTER_BYTES <= ZEROED, "counters where callers zero");
 
 // Counters, then two partial sums a CTA (the end of one unit and the start of
 // another): maximum and sum of a row, and up to 128 values of it.

@@ -6,9 +6,8 @@ its outputs through the torch caching allocator, and launches the CUDA kernels
 of ``libkimi_b200.so`` on ``torch.cuda.current_stream()``.  There is no CPU or
 library fallback: CPU tensors raise ``ValueError`` and a missing library
 raises ``RuntimeError``.  No call synchronizes the host, so the operators can
-be captured in a CUDA graph after one warm-up call per shape (the warm-up
-allocates the scratch buffers that the router and the down+combine kernels
-keep between calls).
+be captured in a CUDA graph after one warm-up call per shape (which loads the
+kernels).  Scratch with counters is kept between calls; a graph has its own.
 
 Reference entry points mirrored here:
   w4a16_dense       engine/kernels/w4a16_dense_gemv.py:312-336 (validation :171-197)
@@ -29,7 +28,7 @@ prompt_attention, tree_attention, verify_drafts.
 from __future__ import annotations
 
 import threading
-from ctypes import c_float, c_int64, c_size_t, c_void_p
+from ctypes import byref, c_float, c_int64, c_size_t, c_uint64, c_void_p
 from typing import NamedTuple
 
 import torch
@@ -86,6 +85,42 @@ def _dense_contig(t: torch.Tensor) -> torch.Tensor:
 
 
 _WORKSPACES: dict[tuple, torch.Tensor] = {}
+_CAPTURED: dict[tuple, tuple[int, torch.Tensor]] = {}
+
+
+def _capturing() -> bool:
+    """Whether the current stream records a CUDA graph."""
+    return torch._C._cuda_isCurrentStreamCapturing()
+
+
+def _capture_id(stream: int) -> int:
+    """Which capture the stream is in (another one for each)."""
+    out = c_uint64(0)
+    _lib.call("kb_stream_capture_id", stream, byref(out))
+    return out.value
+
+
+def _kept_scratch(key: tuple, device: torch.device, stream: int, nbytes: int,
+                  counters: int) -> torch.Tensor:
+    """Scratch whose first ``counters`` bytes are zero, and are left zero by each call.
+
+    Kept per key (which names the stream) for calls that follow each other there.  A
+    graph has scratch of its own, made and zeroed by its first call in the graph's
+    memory: graphs are replayed in any order and on any stream, beside each other and
+    beside calls outside of them.
+    """
+    if not _capturing():
+        ws = _WORKSPACES.get(key)
+        if ws is None:
+            ws = _WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        return ws
+    capture = _capture_id(stream)
+    held = _CAPTURED.get(key)
+    if held is None or held[0] != capture:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:counters].zero_()
+        held = _CAPTURED[key] = (capture, ws)
+    return held[1]
 
 
 def _workspace(kind: str, device: torch.device, nbytes: int, shape: tuple) -> torch.Tensor:
@@ -99,12 +134,8 @@ def _workspace(kind: str, device: torch.device, nbytes: int, shape: tuple) -> to
     """
     stream = torch.cuda.current_stream(device).cuda_stream
     index = device.index if device.index is not None else torch.cuda.current_device()
-    key = (kind, index, stream, shape)
-    ws = _WORKSPACES.get(key)
-    if ws is None:
-        ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=device)
-        _WORKSPACES[key] = ws
-    return ws
+    nbytes = max(int(nbytes), 256)
+    return _kept_scratch((kind, index, stream, shape), device, stream, nbytes, nbytes)
 
 
 # ---------------------------------------------------------------------------
@@ -970,22 +1001,8 @@ def _raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _capturing() -> bool:
-    """Whether the current stream records a CUDA graph."""
-    return torch._C._cuda_isCurrentStreamCapturing()
-
-
-def _zeroed(kind: str, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Scratch of the operators below, kept per (kind, device, stream, size).
-
-    Calls of one kind and size share one layout and leave the counters in it
-    at zero (see _workspace).
-    """
-    key = (kind, device.index, stream, nbytes)
-    ws = _WORKSPACES.get(key)
-    if ws is None:
-        ws = _WORKSPACES[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return ws
+# Bytes at the start of tree_attention's workspace that have to be zero (kimi_b200.h).
+_TREE_COUNTERS = 4096
 
 
 class _ThreadScratch(threading.local):
@@ -1304,8 +1321,10 @@ def tree_attention(
     if total == 0:
         return out if lse is None else (out, lse)
     stream = _raw_stream(device)
-    ws = _zeroed("tree_attention", device, stream,
-                 _lib.lib().kb_tree_attention_workspace_size(hq // hkv, max_tokens))
+    # Calls of one size share one layout.
+    nbytes = _lib.lib().kb_tree_attention_workspace_size(hq // hkv, max_tokens)
+    ws = _kept_scratch(("tree_attention", device.index, stream, nbytes), device, stream, nbytes,
+                       _TREE_COUNTERS)
     _lib.call(
         "kb_tree_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), k_cache.data_ptr(), ks,
         v_cache.data_ptr(), vs, _ELEMENT[q.dtype], pages, page_size, table.data_ptr(),

@@ -679,3 +679,43 @@ def test_verify_drafts_scratch_may_hold_anything(cuda, greedy, monkeypatch):
     monkeypatch.setattr(_lib, "call", call)
     got = run_verify(c, cuda, True)
     assert got.accepted.tolist() == want[2] and got.tokens.tolist() == want[0]
+
+
+def test_graphs_of_one_capture_stream_replay_in_any_order(cuda):
+    # Captured one after the other without a stream, so that both record on torch's own;
+    # the second one is replayed first, then both beside each other.
+    trees = [paged_case(cuda, torch.bfloat16, [2000, 90], [n, 2], 4, 2, 64, 64, 16, 45 + n)[0]
+             for n in (1, 24)]
+    c = verify_case(6, 3000, 4, False, True, 1, torch.bfloat16, 46)
+    gen = torch.Generator().manual_seed(47)
+    hidden = torch.randn(24, 512, generator=gen).bfloat16().to(cuda)
+    weight = torch.randn(64, 512, generator=gen).bfloat16().to(cuda)
+    cd = {n: (t.to(cuda) if torch.is_tensor(t) else t) for n, t in c.items()}
+    cu = ints(c["cu"], cuda)
+
+    def step():
+        got = ops.verify_drafts(cd["logits"], cd["tokens"], cu, 4, cd["coin"], cd["noise"],
+                                cd["temps"], draft_probs=cd["probs"])
+        return [ops.tree_attention(**dev) for dev in trees] + [
+            got.tokens, got.path, *ops.moe_router(hidden, weight, None, 4)]
+
+    want = step()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step())
+    sides = [torch.cuda.Stream() for _ in graphs]
+    for order in ([1], [0], [1, 0, 1, 0, 0, 1]):
+        for held in outs:
+            for t in held:
+                t.zero_()
+        torch.cuda.synchronize()
+        for i in order:
+            with torch.cuda.stream(sides[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in order:
+            for got, expected in zip(outs[i], want):
+                assert torch.equal(got, expected)
+    for got, expected in zip(step(), want):
+        assert torch.equal(got, expected)

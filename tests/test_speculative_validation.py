@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+import types
 
 import pytest
 import torch
@@ -274,3 +275,25 @@ def test_verification_calls_in_flight_share_no_scratch(library, any_device, monk
     (a, n), (b, m) = seen
     assert min(n, m) >= library.kb_verify_drafts_workspace_size(1, 3) > 0
     assert a + n <= b or b + m <= a
+
+
+def test_graphs_have_scratch_of_their_own(monkeypatch):
+    # Scratch made while a graph is captured is zeroed by that graph alone: no other graph
+    # and no call outside may find it, nor a graph the scratch of calls outside.
+    state = {"capture": 0}
+    monkeypatch.setattr(ops, "_capturing", lambda: state["capture"] > 0, raising=False)
+    monkeypatch.setattr(ops, "_capture_id", lambda stream: state["capture"], raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capture"] > 0)
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda device: types.SimpleNamespace(cuda_stream=7))
+    cpu = torch.device("cpu", 0)
+    for scratch in (lambda: ops._kept_scratch(("tree", 0, 7, 512), cpu, 7, 512, 64),
+                    lambda: ops._workspace("router", cpu, 512, (3, 4))):
+        found = {}
+        for capture in (0, 1, 2, 0, 3):
+            state["capture"] = capture
+            ws = scratch()
+            assert ws.numel() == 512 and not ws[:64].any()
+            assert scratch() is ws                    # calls of one capture share it
+            assert found.setdefault(capture, ws) is ws
+            assert all(ws is not other for c, other in found.items() if c != capture)
