@@ -448,6 +448,13 @@ KB_API int kb_paged_plan(const int32_t* context_lens, const int32_t* reserved_le
                    int32_t* cu_tokens, int64_t* slots, int32_t* positions, int64_t* tree_mask,
                    int32_t* free_head_out, int32_t* missing, void* stream);
 
+/* After kb_paged_plan of the same arguments: reserved_lens[b], updated in place,
+ * becomes the tokens that request b's pages reach, at least what it was and the
+ * context, and up to context + new_lens as far as the plan gave pages. */
+KB_API int kb_paged_reserve(const int32_t* context_lens, const int32_t* new_lens, int64_t B,
+                   const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                   int64_t page_size, int32_t* reserved_lens, void* stream);
+
 /* k_cache[slot] = k[t], v_cache[slot] = v[t] for every token t with slots[t] >=
  * 0.  16-bit elements; Dk and Dv multiples of 8; pointers 16-byte aligned and
  * strides multiples of 8.  Two tokens must not name one slot. */

@@ -1099,6 +1099,42 @@ def paged_plan(
     return PagedPlan(cu, slots, positions, mask, head_out, missing)
 
 
+def paged_reserve(
+    context_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    reserved_lens: torch.Tensor,
+    page_size: int,
+) -> None:
+    """What each request's pages reach after a ``paged_plan`` of the same arguments.
+
+    ``reserved_lens`` (int32 [requests], the plan's) is updated in place: at least
+    what it was and the context, and ``context_lens + new_lens`` as far as the plan
+    gave pages, so that the next plan asks again for those that were missing.
+    """
+    device = context_lens.device
+    if block_table.dtype != torch.int32 or block_table.ndim != 2:
+        raise TypeError("block_table must be an int32 [requests, pages] matrix")
+    _require_cuda(context_lens, "paged reserve")
+    requests, width = block_table.shape
+    ctx = _vector(context_lens, torch.int32, "context_lens", device, requests)
+    new = _vector(new_lens, torch.int32, "new_lens", device, requests)
+    held = _vector(reserved_lens, torch.int32, "reserved_lens", device, requests)
+    if block_table.device != device:
+        raise ValueError("block_table must be on the device of the other tensors")
+    if requests == 0 or width == 0 or page_size <= 0:
+        raise ValueError("paged reserve requires a request, a table column and a page size")
+    if held is not reserved_lens:
+        raise ValueError("reserved_lens is updated in place and needs unit stride")
+    if block_table.stride(1) != 1 or (requests > 1 and block_table.stride(0) < width):
+        raise ValueError("block_table needs rows of unit stride")
+    _lib.call(
+        "kb_paged_reserve", ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
+        max(block_table.stride(0), width), width, page_size, held.data_ptr(),
+        _raw_stream(device),
+    )
+
+
 def _rows_of_heads(t: torch.Tensor, what: str) -> torch.Tensor:
     """[tokens, heads, width] with unit inner stride and 16-byte aligned rows."""
     if t.ndim != 3:

@@ -53,12 +53,17 @@ class PagedCache:
 
     def plan(self, new_lens: torch.Tensor, num_tokens: int,
              parents: torch.Tensor | None = None) -> ops.PagedPlan:
-        """Pages and slots for ``new_lens`` more tokens of each request."""
+        """Pages and slots for ``new_lens`` more tokens of each request.
+
+        Where the pool or the table runs out, ``plan.missing`` counts the pages and the
+        tokens without one have slot -1: they are not stored and do not become context.
+        A later plan asks for the pages again (more may be put at the end of ``free``).
+        """
         plan = ops.paged_plan(self.context, new_lens, self.table, self.free, self.head,
                               self.page_size, num_tokens, parents=parents,
                               reserved_lens=self.reserved)
         self.head = plan.free_head
-        self.reserved = torch.maximum(self.reserved, self.context + new_lens)
+        ops.paged_reserve(self.context, new_lens, self.table, self.reserved, self.page_size)
         return plan
 
     def append(self, k: torch.Tensor, v: torch.Tensor, plan: ops.PagedPlan) -> None:
@@ -71,16 +76,23 @@ class PagedCache:
                                   max_tokens, tree_mask=plan.tree_mask, scale=scale)
 
     def advance(self, lens: torch.Tensor) -> None:
-        """The last ``lens`` appended tokens of each request become context."""
-        self.context = self.context + lens
+        """The last ``lens`` appended tokens of each request become context.
+
+        Tokens that the plan found no page for do not.
+        """
+        self.context = torch.minimum(self.context + lens, self.reserved)
 
     def keep(self, plan: ops.PagedPlan, got: ops.Verification) -> None:
-        """The root and the accepted tokens become context, in a row behind it."""
+        """The root and the accepted tokens become context, in a row behind it.
+
+        From the first of them on that the plan found no page for, they do not.
+        """
         first = plan.cu_tokens[:-1, None].long()
         places = torch.arange(got.path.shape[1], device=self.k.device)[None, :]
-        kept = got.path >= 0
         last = plan.slots.shape[0] - 1
         source = plan.slots[(first + got.path.clamp_min(0)).clamp_max(last)]
+        # Paths ascend and the tokens with slots come first.
+        kept = torch.minimum(got.path, source) >= 0
         target = plan.slots[(first + places).clamp_max(last)].masked_fill(~kept, -1)
         # The rows are read before any is written: targets of one token are
         # sources of another.

@@ -719,3 +719,27 @@ def test_graphs_of_one_capture_stream_replay_in_any_order(cuda):
                 assert torch.equal(got, expected)
     for got, expected in zip(step(), want):
         assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize("requests,ps,longest,most,pool,narrow", [
+    (1, 8, 30, 40, 3, 0), (60, 16, 500, 900, 700, 0), (300, 64, 4000, 5, 40, 0),
+    (40, 8, 100, 60, 10 ** 4, 3),
+])
+def test_paged_reserve(cuda, requests, ps, longest, most, pool, narrow):
+    # What is reached after a plan: the places up to the last one with a page.
+    r = random.Random(requests + most)
+    ctx = [r.randint(0, longest) for _ in range(requests)]
+    reserved = [c + r.choice([0, 0, 3, most]) for c in ctx]
+    new = [r.choice([0, 1, most, r.randint(0, most)]) for _ in range(requests)]
+    width = -(-max(longest + 2 * most, 1) // ps) - narrow
+    table = [[r.randint(0, 999) if i < -(-max(c, h) // ps) else -1 for i in range(width)]
+             for c, h in zip(ctx, reserved)]
+    dev_table, held = ints(table, cuda), ints(reserved, cuda)
+    got = ops.paged_plan(ints(ctx, cuda), ints(new, cuda), dev_table,
+                         ints([r.randint(0, 999) for _ in range(pool)], cuda), ints([0], cuda), ps,
+                         sum(new), reserved_lens=held)
+    ops.paged_reserve(ints(ctx, cuda), ints(new, cuda), dev_table, held, ps)
+    cu, slots = got.cu_tokens.tolist(), got.slots.tolist()
+    want = [max(c, h, *[c + t + 1 for t in range(n) if slots[cu[b] + t] >= 0], 0)
+            for b, (c, h, n) in enumerate(zip(ctx, reserved, new))]
+    assert held.tolist() == want

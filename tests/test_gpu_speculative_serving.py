@@ -83,3 +83,76 @@ def test_cache_keeps_the_accepted_rows_in_a_row(cuda):
         assert got == want
     # Pages left by refused tokens were used again: 14 and 11 places were reached.
     assert int(cache.head) == 2 + 2
+
+
+def fill(cache, plan, base):
+    """Appends rows that hold base, base + 1, ... and returns how many there are."""
+    n = plan.slots.shape[0]
+    value = torch.arange(n, device=cache.k.device, dtype=torch.half) + base
+    x = value[:, None, None].expand(n, 1, 64).contiguous()
+    cache.append(x, x, plan)
+
+
+def held(cache, b):
+    return [float(cache.v[int(cache.table[b, p // 8]), p % 8, 0, 0])
+            for p in range(int(cache.context[b]))]
+
+
+def test_cache_that_runs_out_of_pages_recovers(cuda):
+    # Three pages for two requests that ask for four, then more pages.
+    cache = PagedCache(2, 3, 8, 1, 64, 64, dtype=torch.half, max_pages=6)
+    lens = torch.tensor([10, 12], dtype=torch.int32, device=cuda)
+    plan = cache.plan(lens, 22)
+    assert plan.missing.tolist() == [1]
+    fill(cache, plan, 0)
+    cache.advance(lens)
+    # What has no page is not in the context.
+    assert cache.context.tolist() == [10, 8]
+    assert held(cache, 0) == list(range(10)) and held(cache, 1) == list(range(10, 18))
+    # Another plan still misses the page, and the tree's tokens have no slots.
+    counts = torch.tensor([5, 5], dtype=torch.int32, device=cuda)
+    parents = children_first_tree(2, 2)
+    tree = torch.tensor(parents * 2, dtype=torch.int32, device=cuda)
+    plan = cache.plan(counts, 10, tree)
+    assert plan.missing.tolist() == [1]
+    assert plan.slots[5:].tolist() == [-1] * 5 and min(plan.slots[:5].tolist()) >= 0
+    fill(cache, plan, 100)
+    path = torch.tensor([[0, 3, 4, -1, -1], [0, 1, -1, -1, -1]], dtype=torch.int32, device=cuda)
+    got = ops.Verification(path.long(), path, torch.tensor([2, 1], device=cuda))
+    cache.keep(plan, got)
+    assert cache.context.tolist() == [13, 8]
+    assert held(cache, 0) == [*range(10), 100, 103, 104]
+    assert held(cache, 1) == list(range(10, 18))
+    # With pages in the pool again, the same tokens find their places.
+    k, v = cache.k, cache.v
+    more = PagedCache(2, 6, 8, 1, 64, 64, dtype=torch.half, max_pages=6)
+    more.k[:3], more.v[:3] = k, v
+    cache.k, cache.v = more.k, more.v
+    cache.free = torch.arange(6, dtype=torch.int32, device=cuda)
+    plan = cache.plan(counts, 10, tree)
+    assert plan.missing.tolist() == [0] and min(plan.slots.tolist()) >= 0
+    fill(cache, plan, 200)
+    cache.keep(plan, got)
+    assert cache.context.tolist() == [16, 10]
+    assert held(cache, 0) == [*range(10), 100, 103, 104, 200, 203, 204]
+    assert held(cache, 1) == [*range(10, 18), 205, 206]
+    pages = [p for row in cache.table.tolist() for p in row if p >= 0]
+    assert len(pages) == len(set(pages)) == int(cache.head)
+
+
+def test_cache_keeps_drafts_up_to_the_last_slot(cuda):
+    # A pool that ends inside a tree: an accepted token without a slot stays out, and
+    # nothing is copied from another request's rows in its place.
+    cache = PagedCache(2, 2, 8, 1, 64, 64, dtype=torch.half, max_pages=3)
+    lens = torch.tensor([1, 6], dtype=torch.int32, device=cuda)
+    fill(cache, cache.plan(lens, 7), 0)
+    cache.advance(lens)
+    counts = torch.tensor([5, 5], dtype=torch.int32, device=cuda)
+    tree = torch.tensor(children_first_tree(2, 2) * 2, dtype=torch.int32, device=cuda)
+    plan = cache.plan(counts, 10, tree)
+    assert plan.missing.tolist() == [1] and plan.slots[5:].tolist()[2:] == [-1] * 3
+    fill(cache, plan, 50)
+    path = torch.tensor([[0, 1, 2, -1, -1], [0, 3, 4, -1, -1]], dtype=torch.int32, device=cuda)
+    cache.keep(plan, ops.Verification(path.long(), path, torch.tensor([2, 2], device=cuda)))
+    assert cache.context.tolist() == [4, 7]
+    assert held(cache, 0) == [0, 50, 51, 52] and held(cache, 1) == [*range(1, 7), 55]

@@ -297,3 +297,24 @@ def test_graphs_have_scratch_of_their_own(monkeypatch):
             assert scratch() is ws                    # calls of one capture share it
             assert found.setdefault(capture, ws) is ws
             assert all(ws is not other for c, other in found.items() if c != capture)
+
+
+def test_paged_reserve_refusals(any_device, library):
+    args = dict(context_lens=i32(1), new_lens=i32(1), block_table=i32(0, 1)[None],
+                reserved_lens=i32(1), page_size=8)
+    call = lambda **kw: ops.paged_reserve(**{**args, **kw})  # noqa: E731
+    with pytest.raises(TypeError, match="reserved_lens"):
+        call(reserved_lens=torch.tensor([1]))
+    with pytest.raises(ValueError, match="1 entries"):
+        call(reserved_lens=i32(1, 2))
+    with pytest.raises(ValueError, match="in place"):
+        call(context_lens=i32(1, 2), new_lens=i32(1, 2), block_table=i32(0, 1, 2, 3).view(2, 2),
+             reserved_lens=i32(1, 2, 3, 4)[::2])
+    with pytest.raises(ValueError, match="page size"):
+        call(page_size=0)
+    assert library.kb_paged_reserve(None, None, 1, None, 1, 1, 8, None, None) == 1
+    assert library.kb_paged_reserve(16, 16, 1, 16, 1, 2, 8, 16, None) == 2
+    assert library.kb_paged_reserve(16, 16, 20000, 16, 1, 1, 8, 16, None) == 6
+    # A call that succeeds clears the message.
+    assert library.kb_paged_append(None, 0, 0, None, 0, 0, 0, 1, 64, 64, None, None, None, None,
+                                   0, 8, None, None) == 0
