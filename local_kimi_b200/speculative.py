@@ -19,7 +19,8 @@ the cache, and keeps what the target model accepts.
   cache.keep(plan, got)
 
 Nothing here synchronizes the host; lengths, tables and the free list stay on
-the device.
+the device and are updated in place, so a step captured in a CUDA graph moves on
+with every replay.
 """
 
 from __future__ import annotations
@@ -62,7 +63,7 @@ class PagedCache:
         plan = ops.paged_plan(self.context, new_lens, self.table, self.free, self.head,
                               self.page_size, num_tokens, parents=parents,
                               reserved_lens=self.reserved)
-        self.head = plan.free_head
+        self.head.copy_(plan.free_head)
         ops.paged_reserve(self.context, new_lens, self.table, self.reserved, self.page_size)
         return plan
 
@@ -80,7 +81,7 @@ class PagedCache:
 
         Tokens that the plan found no page for do not.
         """
-        self.context = torch.minimum(self.context + lens, self.reserved)
+        torch.minimum(self.context + lens, self.reserved, out=self.context)
 
     def keep(self, plan: ops.PagedPlan, got: ops.Verification) -> None:
         """The root and the accepted tokens become context, in a row behind it.
@@ -99,7 +100,7 @@ class PagedCache:
         source = source.clamp_min(0).flatten()
         page, row = source // self.page_size, source % self.page_size
         ops.paged_append(self.k[page, row], self.v[page, row], self.k, self.v, target.flatten())
-        self.context = self.context + kept.sum(dim=1, dtype=torch.int32)
+        self.context += kept.sum(dim=1, dtype=torch.int32)
 
 
 def children_first_tree(width: int, depth: int) -> list[int]:

@@ -156,3 +156,37 @@ def test_cache_keeps_drafts_up_to_the_last_slot(cuda):
     cache.keep(plan, ops.Verification(path.long(), path, torch.tensor([2, 2], device=cuda)))
     assert cache.context.tolist() == [4, 7]
     assert held(cache, 0) == [0, 50, 51, 52] and held(cache, 1) == [*range(1, 7), 55]
+
+
+def test_cache_steps_replay_from_a_graph(cuda):
+    # Lengths, the free list's head and the reserved pages move on with every replay.
+    parents = children_first_tree(2, 2)
+    counts = torch.tensor([5, 5], dtype=torch.int32, device=cuda)
+    tree = torch.tensor(parents * 2, dtype=torch.int32, device=cuda)
+    path = torch.tensor([[0, 3, 4, -1, -1], [0, 1, -1, -1, -1]], dtype=torch.int32, device=cuda)
+    got = ops.Verification(path.long(), path, torch.tensor([2, 1], device=cuda))
+    gen = torch.Generator().manual_seed(16)
+    rows = torch.randn(10, 1, 64, generator=gen).half().to(cuda)
+
+    def step(cache):
+        plan = cache.plan(counts, 10, tree)
+        cache.append(rows, rows, plan)
+        out = cache.attend(rows, plan, 5)
+        cache.keep(plan, got)
+        return out
+
+    eager, captured = (PagedCache(2, 12, 8, 1, 64, 64, dtype=torch.half) for _ in range(2))
+    for cache in (eager, captured):
+        cache.k.zero_()
+        cache.v.zero_()
+        step(cache)                           # the warm-up
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(captured)
+    for _ in range(3):
+        want = step(eager)
+        graph.replay()
+        assert torch.equal(out, want)
+    for name in ("context", "reserved", "head", "table", "k", "v"):
+        assert torch.equal(getattr(captured, name), getattr(eager, name)), name
+    assert captured.context.tolist() == [12, 8]
