@@ -398,6 +398,10 @@ extern "C" int kb_paged_append(const uint16_t* k, int64_t k_token_stride, int64_
   for (int i = 0; i < 3; ++i) ok = ok && ((k_strides[i] | v_strides[i]) & 7) == 0;
   KB_REQUIRE(ok, KB_ERR_ALIGNMENT,
              "paged append: pointers must be 16-byte aligned and strides multiples of 8");
+  const int64_t extents[3] = {n_pages, page_size, H};
+  for (int i = 0; i < 3; ++i)
+    KB_REQUIRE(extents[i] <= 1 || (k_strides[i] > 0 && v_strides[i] > 0), KB_ERR_BAD_SHAPE,
+               "paged append: strides of the caches must be positive");
   const int dev = kb::bind_stream_device(stream);
   kb::paged::AppendArgs A = {};
   A.k = k;

@@ -1135,12 +1135,14 @@ def paged_reserve(
     )
 
 
-def _rows_of_heads(t: torch.Tensor, what: str) -> torch.Tensor:
-    """[tokens, heads, width] with unit inner stride and 16-byte aligned rows."""
+def _rows_of_heads(t: torch.Tensor, what: str, expanded: bool = False) -> torch.Tensor:
+    """[tokens, heads, width] with unit inner stride, 16-byte aligned rows and, unless
+    ``expanded`` ones will do, positive strides (tensor copies take no other)."""
     if t.ndim != 3:
         raise ValueError(f"{what} must have shape [tokens, heads, width]")
     s = t.stride()
-    if s[2] != 1 or (s[0] | s[1]) & 7 or t.data_ptr() & 15:
+    if (s[2] != 1 or (s[0] | s[1]) & 7 or not (s[0] and s[1] or expanded)
+            or t.data_ptr() & 15):
         t = t.contiguous()
     return t
 
@@ -1153,6 +1155,9 @@ def _cache_strides(t: torch.Tensor, what: str) -> object:
     if (s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or t.data_ptr() & 15) and t.numel():
         raise ValueError(f"{what} needs unit stride along the width, other strides multiples "
                          "of 8 and a 16-byte aligned start")
+    if not (s[0] and s[1] and s[2]) and any(n > 1 and not x for n, x in zip(t.shape, s)):
+        raise ValueError(f"{what} needs positive strides: rows of its own for every page, "
+                         "place and head")
     return _STRIDES(s[0], s[1], s[2])
 
 
@@ -1185,7 +1190,7 @@ def paged_append(
     if not (v.device == k_cache.device == v_cache.device == device):
         raise ValueError("paged append inputs must share one device")
     ks, vs = _cache_strides(k_cache, "k_cache"), _cache_strides(v_cache, "v_cache")
-    kr, vr = _rows_of_heads(k, "k"), _rows_of_heads(v, "v")
+    kr, vr = _rows_of_heads(k, "k", expanded=True), _rows_of_heads(v, "v", expanded=True)
     n, heads, dk = k.shape
     dv = v.shape[2]
     if v.shape[:2] != (n, heads):

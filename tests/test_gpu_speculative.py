@@ -743,3 +743,26 @@ def test_paged_reserve(cuda, requests, ps, longest, most, pool, narrow):
     want = [max(c, h, *[c + t + 1 for t in range(n) if slots[cu[b] + t] >= 0], 0)
             for b, (c, h, n) in enumerate(zip(ctx, reserved, new))]
     assert held.tolist() == want
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_attention_takes_expanded_heads_and_tokens(cuda, tokens):
+    # One key/value head, or one query, expanded to all of them (strides of zero).
+    gen = torch.Generator().manual_seed(15)
+    one = torch.randn(tokens, 1, 64, generator=gen).bfloat16().to(cuda)
+    q = torch.randn(tokens, 4, 64, generator=gen).bfloat16().to(cuda)
+    cu, k = ints([0, tokens], cuda), one.expand(tokens, 4, 64)
+    want = ops.prompt_attention(q, k.contiguous(), k.contiguous(), cu, tokens)
+    assert torch.equal(ops.prompt_attention(q, k, k, cu, tokens), want)
+    same = q[:1].expand(tokens, 4, 64)
+    want = ops.prompt_attention(same.contiguous(), k.contiguous(), k.contiguous(), cu, tokens)
+    assert torch.equal(ops.prompt_attention(same, k, k, cu, tokens), want)
+    pages = -(-tokens // 16)
+    kc, vc = (torch.zeros(pages, 16, 4, 64, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    ops.paged_append(k, k, kc, vc, torch.arange(tokens, device=cuda))
+    assert torch.equal(kc.flatten(0, 1)[:tokens], k) and torch.equal(vc, kc)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+    for wide in (q, same):
+        got, want = (ops.tree_attention(x, kc, vc, table, ints([0], cuda), cu, tokens)
+                     for x in (wide, wide.contiguous()))
+        assert torch.equal(got, want)

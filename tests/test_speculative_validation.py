@@ -318,3 +318,33 @@ def test_paged_reserve_refusals(any_device, library):
     # A call that succeeds clears the message.
     assert library.kb_paged_append(None, 0, 0, None, 0, 0, 0, 1, 64, 64, None, None, None, None,
                                    0, 8, None, None) == 0
+
+
+def test_expanded_caches_are_refused(any_device, library):
+    # Heads, places or pages that share memory: a token would write over another's rows.
+    x, cache = heads(), torch.zeros((2, 8, 2, 64), dtype=torch.bfloat16)
+    for wide in (cache[:, :, :1].expand(2, 8, 2, 64), cache[:, :1].expand(2, 8, 2, 64),
+                 cache[:1].expand(2, 8, 2, 64)):
+        for caches in ((wide, cache), (cache, wide)):
+            with pytest.raises(ValueError, match="positive strides"):
+                ops.paged_append(x, x, *caches, torch.arange(4))
+            with pytest.raises(ValueError, match="positive strides"):
+                ops.tree_attention(x, *caches, i32(0, 1)[None], i32(3), i32(0, 4), 4)
+    # An extent of one has no use for its stride.
+    one = torch.zeros((1, 8, 1, 64), dtype=torch.bfloat16).as_strided((1, 8, 1, 64), (0, 64, 0, 1))
+    ops.paged_append(heads(0, 1), heads(0, 1), one, one, torch.arange(0))
+    s3, bad = (ctypes.c_int64 * 3)(1024, 128, 64), (ctypes.c_int64 * 3)(1024, 64, 0)
+    assert library.kb_paged_append(16, 128, 64, 16, 128, 64, 4, 2, 64, 64, 16, bad, 16, s3, 2, 8,
+                                   16, None) == 2
+    assert library.kb_paged_append(None, 0, 0, None, 0, 0, 0, 1, 64, 64, None, None, None, None,
+                                   0, 8, None, None) == 0
+
+
+def test_expanded_rows_are_copied():
+    x = heads(4, 1).expand(4, 2, 64)
+    assert ops._rows_of_heads(x, "k").stride() == (128, 64, 1)
+    x = heads(1, 2).expand(4, 2, 64)
+    assert ops._rows_of_heads(x, "q").stride() == (128, 64, 1)
+    assert ops._rows_of_heads(x, "k", expanded=True) is x
+    x = heads(4, 2)
+    assert ops._rows_of_heads(x, "v") is x
