@@ -260,7 +260,9 @@ def check(function: str, status: int) -> None:
 
 
 def call(function: str, *args: object) -> None:
-    check(function, getattr(lib(), function)(*args))
+    status = getattr(_LIB or lib(), function)(*args)
+    if status != KB_OK:
+        check(function, status)
 
 
 def set_pdl(enabled: bool) -> None:

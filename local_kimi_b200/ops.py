@@ -29,7 +29,8 @@ from __future__ import annotations
 
 import threading
 from ctypes import byref, c_float, c_int64, c_size_t, c_uint64, c_void_p
-from typing import NamedTuple
+from functools import partial
+from typing import Callable, NamedTuple
 
 import torch
 
@@ -45,6 +46,21 @@ REFERENCE_GROUP_SIZE = 32
 
 def _stream(device: torch.device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on(device: torch.device) -> Callable[..., None]:
+    """The C call for tensors of a device, which need not be the current one (kernels are
+    launched on the current one)."""
+    index = device.index
+    return _lib.call if index is None or index == _current_device() else partial(_call_on, device)
+
+
+def _call_on(device: torch.device, function: str, *args: object) -> None:
+    with torch.cuda.device(device):
+        _lib.call(function, *args)
+
+
+_current_device = torch._C._cuda_getDevice
 
 
 def _p(tensor: torch.Tensor | None) -> c_void_p:
@@ -220,7 +236,7 @@ def w4a16_dense_engine(
     x = _rows_16b(activations)
     packed = _dense_contig(packed_weights)
     sc = _dense_contig(scales)
-    _lib.call(
+    _on(x.device)(
         "kb_w4a16_dense",
         _p(x), c_int64(x.stride(0)), c_int64(m), c_int64(k), _p(packed), _p(sc), c_int64(n),
         c_int64(group), _p(out), c_int64(out.stride(0)), _stream(x.device),
@@ -269,7 +285,7 @@ def w4a16_dense_multi(
         arr[i].y = out.data_ptr()
         arr[i].y_stride = out.stride(0)
     if device is not None:
-        _lib.call("kb_w4a16_dense_multi", arr, len(problems), _stream(device))
+        _on(device)("kb_w4a16_dense_multi", arr, len(problems), _stream(device))
     return outs
 
 
@@ -305,7 +321,7 @@ def w4a16_dense_tc(
     sc = _dense_contig(scales)
     need = int(_lib.lib().kb_w4a16_dense_tc_workspace_size(m, k, n))
     ws = _workspace("dense_tc", x.device, need, (m, k, n)) if need else None
-    _lib.call(
+    _on(x.device)(
         "kb_w4a16_dense_tc",
         _p(x), c_int64(x.stride(0)), c_int64(m), c_int64(k), _p(packed), _p(sc), c_int64(n),
         c_int64(group), _p(out), c_int64(out.stride(0)), _p(ws),
@@ -376,7 +392,7 @@ def w4a16_grouped(
     idx = _dense_contig(expert_indices)
     packed = _dense_contig(packed_weights)
     sc = _dense_contig(scales)
-    _lib.call(
+    _on(x.device)(
         "kb_w4a16_grouped",
         _p(x), c_int64(x.stride(0)), c_int64(t), c_int64(k), _p(idx), c_int64(r), _p(packed),
         _p(sc), c_int64(e), c_int64(n), c_int64(group), _p(out), _stream(x.device),
@@ -399,7 +415,7 @@ def w4a16_grouped_tc(
     idx = _dense_contig(expert_indices)
     packed = _dense_contig(packed_weights)
     sc = _dense_contig(scales)
-    _lib.call(
+    _on(x.device)(
         "kb_w4a16_grouped_tc",
         _p(x), c_int64(x.stride(0)), c_int64(t), c_int64(k), _p(idx), c_int64(r), _p(packed),
         _p(sc), c_int64(e), c_int64(n), c_int64(group), _p(out), _stream(x.device),
@@ -429,7 +445,7 @@ def w4a16_swiglu_tc(
     idx = _dense_contig(expert_indices)
     p1, s1 = _dense_contig(w1_packed), _dense_contig(w1_scales)
     p3, s3 = _dense_contig(w3_packed), _dense_contig(w3_scales)
-    _lib.call(
+    _on(x.device)(
         "kb_w4a16_swiglu_tc",
         _p(x), c_int64(x.stride(0)), c_int64(t), c_int64(k), _p(idx), c_int64(r), _p(p1),
         _p(s1), _p(p3), _p(s3), c_int64(e), c_int64(n), c_int64(group), _p(out),
@@ -463,7 +479,7 @@ def w4a16_swiglu(
     idx = _dense_contig(expert_indices)
     p1, s1 = _dense_contig(w1_packed), _dense_contig(w1_scales)
     p3, s3 = _dense_contig(w3_packed), _dense_contig(w3_scales)
-    _lib.call(
+    _on(x.device)(
         "kb_w4a16_swiglu",
         _p(x), c_int64(x.stride(0)), c_int64(t), c_int64(k), _p(idx), c_int64(r), _p(p1),
         _p(s1), _p(p3), _p(s3), c_int64(e), c_int64(n), c_int64(group), _p(out),
@@ -543,7 +559,7 @@ def _down_combine(
     lib = _lib.lib()
     need = int(lib.kb_w4a16_w2_combine_workspace_size(t, r, n))
     ws = _workspace("w2_combine", act.device, need, (t, r, n))
-    _lib.call(
+    _on(act.device)(
         "kb_w4a16_w2_combine",
         _p(act), c_int64(t), c_int64(r), c_int64(k), _p(idx), _p(cw), c_int64(cw.stride(0)),
         _p(p2), _p(s2), c_int64(e), c_int64(n), c_int64(group), _p(out), _p(ws),
@@ -612,7 +628,7 @@ def moe_combine_routes(routes: torch.Tensor, weights: torch.Tensor) -> torch.Ten
         return out
     y = routes.contiguous()
     w = weights if weights.stride(1) == 1 else weights.contiguous()
-    _lib.call("kb_moe_combine_routes", _p(y), c_int64(t), c_int64(r), c_int64(n), _p(w),
+    _on(y.device)("kb_moe_combine_routes", _p(y), c_int64(t), c_int64(r), c_int64(n), _p(w),
               c_int64(w.stride(0)), _p(out), _stream(y.device))
     return out
 
@@ -654,7 +670,7 @@ def ep_dispatch(hidden: torch.Tensor, routed: torch.Tensor, per_rank: int, world
         return payload, slots
     x = _rows_16b(hidden)
     r = routed if routed.stride(1) == 1 else routed.contiguous()
-    _lib.call("kb_ep_dispatch", _p(x), c_int64(x.stride(0)), c_int64(t), c_int64(h), _p(r),
+    _on(x.device)("kb_ep_dispatch", _p(x), c_int64(x.stride(0)), c_int64(t), c_int64(h), _p(r),
               c_int64(r.stride(0)), c_int64(k), c_int64(per_rank), c_int64(world),
               c_int64(capacity), c_int64(shared_id), _p(payload), _p(slots), _stream(x.device))
     return payload, slots
@@ -687,7 +703,7 @@ def ep_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor,
     sc = slots.contiguous()
     s = _rows_16b(shared)
     w = weights if weights.stride(1) == 1 else weights.contiguous()
-    _lib.call("kb_ep_combine", _p(yc), _p(sc), c_int64(t), c_int64(k), c_int64(h), _p(w),
+    _on(yc.device)("kb_ep_combine", _p(yc), _p(sc), c_int64(t), c_int64(k), c_int64(h), _p(w),
               c_int64(w.stride(0)), _p(s), c_int64(s.stride(0)), _p(out), c_int64(out.stride(0)),
               _stream(yc.device))
     return out
@@ -742,7 +758,7 @@ def moe_router(
     lib = _lib.lib()
     need = int(lib.kb_router_workspace_size(tokens, experts))
     ws = _workspace("router", flat.device, need, (tokens, experts))
-    _lib.call(
+    _on(flat.device)(
         "kb_router_topk",
         _p(x), c_int64(x.stride(0)), c_int64(tokens), c_int64(hidden), _p(w), _p(b),
         c_int64(experts), c_int64(top_k), 1 if renormalize else 0,
@@ -802,7 +818,7 @@ def kda_decode_step(
         work = state.contiguous()
     qc, kc, vc = q.contiguous(), k.contiguous(), v.contiguous()
     dc, bc = decay.contiguous(), beta.contiguous()
-    _lib.call(
+    _on(state.device)(
         "kb_kda_decode_step",
         _p(work), c_int64(work.stride(0)), c_int64(work.stride(1)), c_int64(work.stride(2)),
         _p(qc), _p(kc), _p(vc), _p(dc), _p(bc), c_int64(batch), c_int64(heads), c_int64(d_k),
@@ -837,7 +853,7 @@ def kda_prepare(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor,
     beta = torch.empty((batch, num_heads), dtype=torch.float32, device=q_in.device)
     if batch == 0:
         return (*outs, beta)
-    _lib.call("kb_kda_prepare", _p(x[0]), _p(x[1]), _p(x[2]), c_int64(x[0].stride(0)),
+    _on(q_in.device)("kb_kda_prepare", _p(x[0]), _p(x[1]), _p(x[2]), c_int64(x[0].stride(0)),
               _p(q_state), _p(k_state), _p(v_state), _p(weights[0]), _p(weights[1]),
               _p(weights[2]), _p(rd), c_int64(rd.stride(0)), _p(dt), _p(a), _p(rb),
               c_int64(rb.stride(0)), c_int64(batch), c_int64(num_heads), c_int64(head_dim),
@@ -912,7 +928,8 @@ def kda_prepare_step(state: torch.Tensor, q_in: torch.Tensor, k_in: torch.Tensor
         raise ValueError("out_bf16 must be a contiguous BF16 tensor with B*H*D elements")
     if batch == 0:
         return out
-    _lib.call("kb_kda_prepare_step", _p(x[0]), _p(x[1]), _p(x[2]), c_int64(x[0].stride(0)),
+    _on(q_in.device)("kb_kda_prepare_step", _p(x[0]), _p(x[1]), _p(x[2]),
+            c_int64(x[0].stride(0)),
               _p(q_state), _p(k_state), _p(v_state), _p(weights[0]), _p(weights[1]),
               _p(weights[2]), _p(rd), c_int64(rd.stride(0)), _p(dt), _p(a), _p(rb),
               c_int64(rb.stride(0)), c_float(eps), _p(state), c_int64(state.stride(0)),
@@ -941,7 +958,7 @@ def quantise(weight: torch.Tensor, group_size: int = 128) -> tuple[torch.Tensor,
     packed = torch.empty((n, k // 2), dtype=torch.uint8, device=weight.device)
     scales = torch.empty((n, k // group_size), dtype=torch.bfloat16, device=weight.device)
     flag = torch.zeros((1,), dtype=torch.int32, device=weight.device)
-    _lib.call(
+    _on(weight.device)(
         "kb_w4a16_quantise",
         _p(w), c_int64(w.stride(0)), c_int64(n), c_int64(k), c_int64(group_size), _p(packed),
         _p(scales), _p(flag), _stream(weight.device),
@@ -1087,8 +1104,9 @@ def paged_plan(
     else:
         par = _vector(parents, torch.int32, "parents", device, num_tokens)
         slots, mask = torch.empty(2, num_tokens, dtype=torch.long, device=device).unbind()
-    _lib.call(
-        "kb_paged_plan", ctx.data_ptr(), None if held is None else held.data_ptr(),
+    _on(device)(
+        "kb_paged_plan",
+        ctx.data_ptr(), None if held is None else held.data_ptr(),
         new.data_ptr(), requests, block_table.data_ptr(),
         max(block_table.stride(0), width), width, free.data_ptr(), free.shape[0],
         head.data_ptr(), page_size, num_tokens, None if par is None else par.data_ptr(),
@@ -1128,8 +1146,9 @@ def paged_reserve(
         raise ValueError("reserved_lens is updated in place and needs unit stride")
     if block_table.stride(1) != 1 or (requests > 1 and block_table.stride(0) < width):
         raise ValueError("block_table needs rows of unit stride")
-    _lib.call(
-        "kb_paged_reserve", ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
+    _on(device)(
+        "kb_paged_reserve",
+        ctx.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
         max(block_table.stride(0), width), width, page_size, held.data_ptr(),
         _raw_stream(device),
     )
@@ -1192,21 +1211,25 @@ def paged_append(
     ks, vs = _cache_strides(k_cache, "k_cache"), _cache_strides(v_cache, "v_cache")
     kr, vr = _rows_of_heads(k, "k", expanded=True), _rows_of_heads(v, "v", expanded=True)
     n, heads, dk = k.shape
-    dv = v.shape[2]
-    if v.shape[:2] != (n, heads):
+    v_tokens, v_heads, dv = v.shape
+    if v_tokens != n or v_heads != heads:
         raise ValueError("k and v must have the same tokens and heads")
-    if k_cache.shape[2:] != (heads, dk) or v_cache.shape[2:] != (heads, dv):
+    pages, page_size, k_cache_heads, k_cache_width = k_cache.shape
+    v_pages, v_page_size, v_cache_heads, v_cache_width = v_cache.shape
+    if not (k_cache_heads == v_cache_heads == heads
+            and k_cache_width == dk and v_cache_width == dv):
         raise ValueError("the caches' heads and widths must match k and v")
-    if k_cache.shape[:2] != v_cache.shape[:2]:
+    if pages != v_pages or page_size != v_page_size:
         raise ValueError("the caches must have the same pages")
     _check_widths(dk, dv)
     sl = _vector(slots, torch.long, "slots", device, n)
     if n == 0 or heads == 0:
         return
-    _lib.call(
-        "kb_paged_append", kr.data_ptr(), kr.stride(0), kr.stride(1), vr.data_ptr(),
+    _on(device)(
+        "kb_paged_append",
+        kr.data_ptr(), kr.stride(0), kr.stride(1), vr.data_ptr(),
         vr.stride(0), vr.stride(1), n, heads, dk, dv, k_cache.data_ptr(), ks,
-        v_cache.data_ptr(), vs, k_cache.shape[0], k_cache.shape[1], sl.data_ptr(),
+        v_cache.data_ptr(), vs, pages, page_size, sl.data_ptr(),
         _raw_stream(device),
     )
 
@@ -1287,8 +1310,9 @@ def prompt_attention(
         return _no_requests(q, dv, return_lse)
     out = torch.empty(total, hq, dv, dtype=q.dtype, device=device)
     lse = torch.empty(total, hq, dtype=torch.float32, device=device) if return_lse else None
-    _lib.call(
-        "kb_prompt_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), kr.data_ptr(),
+    _on(device)(
+        "kb_prompt_attention",
+        qr.data_ptr(), qr.stride(0), qr.stride(1), kr.data_ptr(),
         kr.stride(0), kr.stride(1), vr.data_ptr(), vr.stride(0), vr.stride(1),
         _ELEMENT[q.dtype], cq.data_ptr(), ck.data_ptr(), requests, total, keys, max_seqlen, hq,
         hkv, dk, dv, scale, out.data_ptr(),
@@ -1366,8 +1390,9 @@ def tree_attention(
     nbytes = _lib.lib().kb_tree_attention_workspace_size(hq // hkv, max_tokens)
     ws = _kept_scratch(("tree_attention", device.index, stream, nbytes), device, stream, nbytes,
                        _TREE_COUNTERS)
-    _lib.call(
-        "kb_tree_attention", qr.data_ptr(), qr.stride(0), qr.stride(1), k_cache.data_ptr(), ks,
+    _on(device)(
+        "kb_tree_attention",
+        qr.data_ptr(), qr.stride(0), qr.stride(1), k_cache.data_ptr(), ks,
         v_cache.data_ptr(), vs, _ELEMENT[q.dtype], pages, page_size, table.data_ptr(),
         max(table.stride(0), width), width, ctx.data_ptr(), cu.data_ptr(),
         None if mask is None else mask.data_ptr(), requests, total, max_tokens, hq, hkv, dk, dv,
@@ -1419,7 +1444,7 @@ def verify_drafts(
         raise TypeError("noise must be an FP32 [requests, vocabulary] matrix")
     if noise.shape != (requests, vocab) or noise.device != device:
         raise ValueError("noise must have a row for each request, on the logits' device")
-    par = probs = None
+    par, probs, probs_stride = None, None, vocab
     if parents is not None:
         par = _vector(parents, torch.int32, "parents", device, rows)
     if draft_probs is not None:
@@ -1429,28 +1454,30 @@ def verify_drafts(
             raise TypeError("draft_probs must be an FP32 [rows, vocabulary] matrix")
         if draft_probs.shape != (rows, vocab) or draft_probs.device != device:
             raise ValueError("draft_probs must have the shape and device of the logits")
-        probs = _unit_rows(draft_probs)
+        probs, probs_stride = _unit_rows(draft_probs, vocab)
     out = torch.empty(requests, max_tokens, dtype=torch.long, device=device)
     path = torch.empty(requests, max_tokens, dtype=torch.int32, device=device)
     accepted = torch.empty(requests, dtype=torch.int32, device=device)
     if requests == 0:
         return Verification(out, path, accepted)
-    x, e = _unit_rows(logits), _unit_rows(noise)
+    (x, x_stride), (e, e_stride) = _unit_rows(logits, vocab), _unit_rows(noise, vocab)
     stream = _raw_stream(device)
     ws = _verify_scratch(device, stream, requests, rows)
-    _lib.call(
-        "kb_verify_drafts", x.data_ptr(), max(x.stride(0), vocab), rows, vocab,
+    _on(device)(
+        "kb_verify_drafts",
+        x.data_ptr(), x_stride, rows, vocab,
         _ELEMENT[x.dtype], tok.data_ptr(), None if par is None else par.data_ptr(),
         cu.data_ptr(), requests, max_tokens, coin.data_ptr(), e.data_ptr(),
-        max(e.stride(0), vocab), temps.data_ptr(), None if probs is None else probs.data_ptr(),
-        vocab if probs is None else max(probs.stride(0), vocab), out.data_ptr(),
+        e_stride, temps.data_ptr(), None if probs is None else probs.data_ptr(),
+        probs_stride, out.data_ptr(),
         path.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), stream,
     )
     return Verification(out, path, accepted)
 
 
-def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    """A matrix whose rows have unit stride and do not overlap."""
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
+def _unit_rows(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
+    """A matrix whose rows have unit stride and do not overlap, and their stride."""
+    row, column = t.stride()
+    if column != 1 or (row < width and t.shape[0] > 1):
+        t, row = t.contiguous(), width
+    return t, max(row, width)

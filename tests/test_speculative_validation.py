@@ -348,3 +348,44 @@ def test_expanded_rows_are_copied():
     assert ops._rows_of_heads(x, "k", expanded=True) is x
     x = heads(4, 2)
     assert ops._rows_of_heads(x, "v") is x
+
+
+def test_calls_go_to_the_tensors_device(library, any_device, monkeypatch):
+    # A kernel is launched on the current device, so the call makes the tensors' current.
+    state, seen = {"device": 0}, []
+
+    class device:
+        def __init__(self, to):
+            self.to = to
+
+        def __enter__(self):
+            self.back, state["device"] = state["device"], self.to.index
+
+        def __exit__(self, *_):
+            state["device"] = self.back
+
+    monkeypatch.setattr(ops, "_current_device", lambda: state["device"], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append((name, state["device"])))
+    ops._on(torch.device("cuda", 1))("kb_x", 1, 2)
+    ops._on(torch.device("cuda", 0))("kb_y")
+    assert seen == [("kb_x", 1), ("kb_y", 0)] and state["device"] == 0
+
+    # Every operator says which device its tensors are on.
+    monkeypatch.setattr(ops, "_on",
+                        lambda device: lambda name, *args: seen.append((name, device)))
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(ops, "_capturing", lambda: False)
+    seen.clear()
+    x, cache = heads(), torch.zeros((2, 8, 2, 64), dtype=torch.bfloat16)
+    table = i32(0, 1)[None]
+    ops.paged_plan(i32(1), i32(1), table, i32(0), i32(0), 8, 1)
+    ops.paged_reserve(i32(1), i32(1), table, i32(1), 8)
+    ops.paged_append(x, x, cache, cache, torch.arange(4))
+    ops.prompt_attention(x, x, x, i32(0, 4), 4)
+    ops.tree_attention(x, cache, cache, table, i32(3), i32(0, 4), 4)
+    ops.verify_drafts(torch.zeros(3, 10), torch.zeros(3, dtype=torch.long), i32(0, 3), 3,
+                      torch.zeros(3), torch.ones(1, 10), torch.ones(1))
+    assert seen == [(f"kb_{name}", torch.device("cpu")) for name in (
+        "paged_plan", "paged_reserve", "paged_append", "prompt_attention", "tree_attention",
+        "verify_drafts")]
