@@ -508,7 +508,8 @@ KB_API int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int64_t 
  * is accepted and emitted.  out_tokens [B, max_tokens]: the accepted tokens and
  * the last one, then -1; path [B, max_tokens]: 0 and the accepted tokens' tree
  * indices, then -1; accepted [B].  parents NULL: chains.  max_tokens <= 64; a
- * not-a-number logit counts as -infinity.  Two launches: the workspace may hold
+ * not-a-number logit counts as -infinity, +infinity as the largest number.  Two
+ * launches: the workspace may hold
  * anything, but is this call's alone until it is done on the stream. */
 KB_API size_t kb_verify_drafts_workspace_size(int64_t B, int64_t rows);
 KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows, int64_t V,

@@ -480,8 +480,13 @@ __global__ void __launch_bounds__(THREADS, 4) pick_kernel(const Args A) {
   constexpr int P = PIECE<TYPE>;
   int start, count;
   whole_pieces<TYPE>(base, lo, hi, start, count);
+  // A row with an infinite logit goes one by one, with infinity as the largest number.
+  if (top == FLT_MAX) {
+    start = hi;
+    count = 0;
+  }
   for (int i = lo + tid; i < start; i += THREADS)
-    take(logit<TYPE>(A.logits, base + i), noise[i], q ? q[i] : 0.f, i);
+    take(tidy(logit<TYPE>(A.logits, base + i)), noise[i], q ? q[i] : 0.f, i);
   const bool wide = ((uintptr_t)(noise + start) & 15) == 0 && (!q || ((uintptr_t)(q + start) & 15) == 0);
   constexpr int BATCH = 2;
   for (int i0 = tid; i0 < count; i0 += THREADS * BATCH) {

@@ -766,3 +766,18 @@ def test_attention_takes_expanded_heads_and_tokens(cuda, tokens):
         got, want = (ops.tree_attention(x, kc, vc, table, ints([0], cuda), cu, tokens)
                      for x in (wide, wide.contiguous()))
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_drafts_infinite_logits_share_the_draw(cuda, probs):
+    # Several infinite logits count as equally likely, in the acceptance and in the draw.
+    c = verify_case(60, 700, 3, False, probs, 0, torch.float32, 13)
+    c["logits"][:, [5, 17, 300, 698]] = float("inf")
+    x = c["logits"].clone()
+    x[torch.isinf(x)] = 1e30               # what is largest by far, for the oracle
+    want = ref.verify(x, c["tokens"], c["parents"], c["cu"], 3, c["coin"], c["noise"],
+                      c["temps"], c["probs"])
+    got = run_verify(c, cuda, False)
+    assert got.tokens.tolist() == want[0] and got.path.tolist() == want[1]
+    last = got.tokens.gather(1, got.accepted.long()[:, None])
+    assert len(set(last.flatten().tolist())) > 1
