@@ -99,7 +99,11 @@ __device__ __forceinline__ float weight(float x, float top, float inv_t) {
   return top == -INFINITY ? 0.f : expf((x - top) * inv_t);
 }
 
-__device__ __forceinline__ float inverse(float t) { return t > 0.f ? 1.0f / t : 1.0f; }
+// 1 / T, kept where its products stay numbers: a T next to zero leaves the largest logits
+// alone, one without bound gives every finite logit the same weight.
+__device__ __forceinline__ float inverse(float t) {
+  return t > 0.f ? fminf(fmaxf(1.0f / t, FLT_MIN), FLT_MAX / 2) : 1.0f;
+}
 
 // Tokens [first, first + n) of request b, cut to the rows there are.
 __device__ __forceinline__ void request(const Args& A, int b, int64_t& first, int& n) {
@@ -557,6 +561,7 @@ __global__ void __launch_bounds__(THREADS, 4) pick_kernel(const Args A) {
     }
     key = at == INT_MAX ? 0 : race_key(v, at);
     join();
+    if (key == 0) key = race_key(0.f, 0);      // noise that compares with nothing: token 0
   }
   if (tid == 0) out[taken] = (int64_t)(0xffffffffu - (uint32_t)key);
 }

@@ -781,3 +781,22 @@ def test_verify_drafts_infinite_logits_share_the_draw(cuda, probs):
     assert got.tokens.tolist() == want[0] and got.path.tolist() == want[1]
     last = got.tokens.gather(1, got.accepted.long()[:, None])
     assert len(set(last.flatten().tolist())) > 1
+
+
+def test_verify_drafts_emits_tokens_of_the_vocabulary_whatever_the_inputs(cuda):
+    # Temperatures without a usable inverse, and noise that compares with nothing.
+    c = verify_case(6, 300, 3, False, False, 0, torch.float32, 14)
+    c["logits"][:, 40:60] = float("-inf")
+    c["temps"] = torch.tensor([1e-40, 1e-44, float("inf"), 3e38, 0.8, 0.8])
+    c["noise"][4:] = float("nan")
+    got = run_verify(c, cuda, False)
+    last = got.tokens.gather(1, got.accepted.long()[:, None])[:, 0]
+    assert bool(((last >= 0) & (last < 300)).all())
+    # Next to temperature 0 the draw is the argmax, and so is what is accepted.
+    cold = run_verify({**c, "temps": torch.zeros(6)}, cuda, False)
+    assert torch.equal(got.tokens[:2], cold.tokens[:2])
+    # Without bound the finite logits are all as likely.
+    x = torch.where(torch.isinf(c["logits"]), c["logits"], torch.zeros(()))
+    want = ref.verify(x, c["tokens"], c["parents"], c["cu"], 3, c["coin"], c["noise"],
+                      torch.ones(6))
+    assert got.tokens[2].tolist() == want[0][2]
