@@ -483,6 +483,8 @@ KB_API int kb_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_
  * context and, of its step, the tokens whose bit is set in its tree_mask word
  * (NULL: itself and those before it).  max_tokens: no request has more tokens
  * (at most 64 with tree_mask).  page_size: a power of two from 8 to 4096.
+ * Contexts count up to 2^30 - 128; places past the table have no keys and set
+ * device error bit 2.
  * Other arguments as kb_prompt_attention; the first 4096 bytes of the workspace of
  * kb_tree_attention_workspace_size bytes are zeroed once and left zero by each call.
  * Calls that share a workspace follow each other on a stream, or in a graph. */

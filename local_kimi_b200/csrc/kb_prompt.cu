@@ -108,6 +108,7 @@ struct PromptArgs {
   const int64_t* mask;      // NULL: causal
   int64_t n_pages, v_page;
   int width, ps, Hkv;
+  int places;               // of a table's row
   int most;                 // tokens of a request at most
   int* counters;            // [2 * CTAs], zero between calls
   int part_rows;            // rows of a unit: 128 or 256
@@ -430,10 +431,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   const uint32_t tmem = B->tmem;
   pdl_wait();
   pdl_launch_dependents();
+  const Lengths L = {A.cu_q, A.context, A.total_q, A.places, A.g,
+                     A.Hkv, 2 * TILE, A.most, ROWS_COST};
   Run run = {};
-  if (PAGED)
-    run = find_run<2 * TILE, ROWS_COST, PROMPT_THREADS>(A.cu_q, A.context, A.total_q, A.B, A.g, A.Hkv,
-                                             A.most, &B->start);
+  if (PAGED) run = find_run<PROMPT_THREADS>(L, A.B, &B->start, A.err);
 
   // Rows outside every request: zero.
   {
@@ -920,7 +921,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         int64_t pos = run.lo, line = B->start.base;
         Request R = B->start.r;
         int b = B->start.b, base = 0;
-        const Lengths L = {A.cu_q, A.context, A.total_q, A.g, A.Hkv, 2 * TILE, A.most, ROWS_COST};
         while (pos < run.hi && ok) {
           const int64_t w = L.length(R);
           if (pos >= line + w) {
@@ -1136,6 +1136,7 @@ int launch_rows(const TreeCall& T, int64_t rows, int sms, void* workspace, void*
   A.n_pages = T.n_pages;
   A.width = T.width;
   A.ps = T.ps;
+  A.places = T.places;
   A.most = T.most;
   A.counters = static_cast<int*>(workspace);
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ROW_COUNTERS);

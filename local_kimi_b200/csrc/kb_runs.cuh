@@ -27,20 +27,24 @@ struct RunStart {
 };
 
 // Lengths on the line.  A unit counts `cost` tiles more than it has, for its start
-// and its end.
+// and its end.  Places past the table have no keys and no tiles, so a length that is
+// wrong costs no more than the table's; contexts count up to MAX_CONTEXT (places and
+// their tiles stay within 32 bits).
+constexpr int MAX_CONTEXT = (1 << 30) - 2 * KT, MAX_PLACES = 0x7fffffff - KT;
 struct Lengths {
   const int *cu, *context;
   int64_t total;
+  int places;               // of a table's row
   int g, heads, rows, most; // query heads of a key/value head; rows of a block; tokens at most
   int cost;
   __device__ __forceinline__ Request look(int b) const {
     Request R;
     int64_t end;
-    const int ctx = context[b];
+    const int ctx = min(max(context[b], 0), MAX_CONTEXT);
     request_rows(cu, b, total, R.first, end);
     R.n = (int)min(end - R.first, (int64_t)most);
-    R.ctx = max(ctx, 0);
-    R.tiles = R.n ? (R.ctx + R.n + KT - 1) / KT : 0;
+    R.ctx = ctx;
+    R.tiles = R.n ? max((min(ctx + R.n, places) + KT - 1) / KT, 1) : 0;
     R.blocks = (int)(((int64_t)R.n * g + rows - 1) / rows);
     return R;
   }
@@ -88,11 +92,9 @@ __device__ __forceinline__ RunPart run_part(const Request& R, int64_t pos, int64
 }
 
 // All threads of the CTA: the line's length, this CTA's run, and in `start` (shared
-// memory, valid on return) the request it starts in.
-template <int ROWS, int COST, int THREADS>
-__device__ __forceinline__ Run find_run(const int* cu, const int* context, int64_t total_rows,
-                                        int B, int g, int heads, int most, RunStart* start) {
-  const Lengths L = {cu, context, total_rows, g, heads, ROWS, most, COST};
+// memory, valid on return) the request it starts in.  Tokens past the table are recorded.
+template <int THREADS>
+__device__ __forceinline__ Run find_run(const Lengths& L, int B, RunStart* start, uint32_t* err) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int WARPS = THREADS / 32;
   static_assert(WARPS <= 16, "a sum for each warp");
@@ -104,6 +106,7 @@ __device__ __forceinline__ Run find_run(const int* cu, const int* context, int64
     const Request R = L.look(b);
     if (b == b0) R0 = R;
     mine += L.length(R);
+    if (blockIdx.x == 0 && R.n && (int)R.ctx + R.n > L.places) atomicOr(err, ERR_PAGE);
   }
   int64_t incl = mine;
   for (int o = 1; o < 32; o <<= 1) {
@@ -176,7 +179,7 @@ struct TreeCall {
   const int *cu, *table, *context;
   const int64_t* mask;
   int64_t table_stride, n_pages, total;
-  int B, width, ps, Hq, Hkv, Dk, Dv, f16, most;
+  int B, width, ps, places, Hq, Hkv, Dk, Dv, f16, most;
   float scale2;
   uint32_t* err;
 };

@@ -59,6 +59,7 @@ struct TreeArgs {
   const int64_t* mask;
   int64_t n_pages, total;
   int B, width, ps, Hq, Hkv, g, Dk, Dv;
+  int places;               // of a table's row, up to MAX_PLACES
   int most;                 // tokens of a request at most
   float scale2;             // scale * log2(e)
   int* counters;            // [MAX_CTAS], zero between calls
@@ -158,8 +159,9 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
   pdl_wait();
   pdl_launch_dependents();
 
-  const Run run = find_run<S::RB, UNIT_COST, S::THREADS>(A.cu, A.context, A.total, A.B, A.g, A.Hkv,
-                                              A.most, &B->start);
+  const Lengths L = {A.cu, A.context, A.total, A.places, A.g,
+                     A.Hkv, S::RB, A.most, UNIT_COST};
+  const Run run = find_run<S::THREADS>(L, A.B, &B->start, A.err);
   // Rows outside every request: zero.
   {
     const int64_t lead = min(max((int64_t)A.cu[0], (int64_t)0), A.total);
@@ -180,7 +182,6 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
     // ---------------------------------------------------------------- producer
     const uint64_t pol = l2_evict_first_policy();
     const int ps = A.ps, box = min(ps, KT), ppt = KT / box;
-    const Lengths L = {A.cu, A.context, A.total, A.g, A.Hkv, S::RB, A.most, UNIT_COST};
     int64_t pos = run.lo, base = B->start.base;
     Request R = B->start.r;
     int b = B->start.b, seg = 0, stage = 0;
@@ -786,6 +787,7 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
     T.B = (int)B;
     T.width = (int)table_width;
     T.ps = (int)page_size;
+    T.places = (int)std::min<int64_t>(table_width * page_size, at::MAX_PLACES);
     T.Hq = (int)Hq;
     T.Hkv = (int)Hkv;
     T.Dk = (int)Dk;
@@ -824,6 +826,7 @@ extern "C" int kb_tree_attention(const uint16_t* q, int64_t q_token_stride, int6
   A.B = (int)B;
   A.width = (int)table_width;
   A.ps = (int)page_size;
+  A.places = (int)std::min<int64_t>(table_width * page_size, at::MAX_PLACES);
   A.Hq = (int)Hq;
   A.Hkv = (int)Hkv;
   A.g = (int)(Hq / Hkv);

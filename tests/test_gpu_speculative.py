@@ -800,3 +800,24 @@ def test_verify_drafts_emits_tokens_of_the_vocabulary_whatever_the_inputs(cuda):
     want = ref.verify(x, c["tokens"], c["parents"], c["cu"], 3, c["coin"], c["noise"],
                       torch.ones(6))
     assert got.tokens[2].tolist() == want[0][2]
+
+
+@pytest.mark.parametrize("new,heads", [([3, 2], 4), ([9, 30], 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tree_attention_contexts_past_the_table(cuda, dtype, new, heads):
+    # Lengths that nobody meant: what the table has is seen, the rest is absent, and the
+    # call takes no longer than for a full table.
+    dev, _ = paged_case(cuda, dtype, [58, 20], new, heads, 2, 64, 64, 16, 17, tree=False)
+    dev["block_table"] = dev["block_table"][:, :3].contiguous()
+    q, kc, vc = (dev[n].cpu() for n in ("q", "k_cache", "v_cache"))
+    want = ref.tree_attention(q, kc, vc, dev["block_table"].tolist(), [10 ** 4, 20], sums(new),
+                              None, 0.125)
+    for length in (10 ** 4, 2 ** 30, 2 ** 31 - 1):
+        dev["context_lens"] = ints([length, 20], cuda)
+        _lib_errors()
+        out, lse = ops.tree_attention(**dev, return_lse=True)
+        assert _lib_errors() == 4
+        check_attention(out, lse, *want, dtype)
+    dev["block_table"] = dev["block_table"][:, :0]
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    assert _lib_errors() == 4 and not out.any() and torch.isinf(lse).all()
