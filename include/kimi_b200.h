@@ -432,7 +432,7 @@ KB_API int64_t kb_step_trace_entries(const kb_step* step);
  * reserved_lens[b] tokens (NULL, or less than the context: context_lens[b]),
  * takes the pages it lacks for context_lens[b] + new_lens[b] tokens from
  * free_pages, from *free_head on, in request order, and their ids are written
- * to its row of block_table.  Lengths count up to 2^30.
+ * to its row of block_table.  Lengths count up to 2^30 - 1.
  * cu_tokens [B+1]: running sums of new_lens; slots [n_tokens]: page * page_size
  * + row of each new token, -1 past the last token or without a page; positions
  * [n_tokens]: context + index, or context + depth with parents [n_tokens];

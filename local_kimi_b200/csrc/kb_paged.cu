@@ -44,9 +44,11 @@ struct PlanArgs {
   uint32_t* err;
 };
 
-// Lengths count up to 2^30 (32-bit sums and divisions; a page too).
+// Lengths count up to 2^30 - 1, so that two and their pages stay within 31 bits (a page's
+// rows up to 2^30).
+constexpr int LONGEST = (1 << 30) - 1;
 __device__ __forceinline__ uint32_t length_of(const int* lens, int b) {
-  return (uint32_t)min(max(__ldg(lens + b), 0), 1 << 30);
+  return (uint32_t)min(max(__ldg(lens + b), 0), LONGEST);
 }
 
 __device__ __forceinline__ int pages_of(uint32_t tokens, uint32_t ps) {
@@ -63,11 +65,20 @@ __device__ __forceinline__ int find(const int* sums, int n, int v) {
   return lo;
 }
 
-__device__ __forceinline__ int warp_scan(int v, int lane) {
+// Sums stop above the 2^30 that any output holds: lengths that nobody meant must not
+// wrap around to places before it.
+__device__ __forceinline__ int add(int a, int b) {
+  return (int)min((uint32_t)a + (uint32_t)b, (1u << 30) + 1u);
+}
+
+// Running sums over a warp, and those of the lanes before.
+__device__ __forceinline__ int warp_scan(int v, int lane, int& before) {
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    if (lane >= o) v = add(v, u);
   }
+  before = __shfl_up_sync(0xffffffffu, v, 1);
+  if (lane == 0) before = 0;
   return v;
 }
 
@@ -94,31 +105,32 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
     s_page[b] = page;
     s_ctx[b] = (int)c;
     s_have[b] = have;
-    tok += (int)n;
-    page += need;
-    lost += max(0, want - have) - need;
+    tok = add(tok, (int)n);
+    page = add(page, need);
+    lost = add(lost, max(0, want - have) - need);
   }
-  const int tok_in = warp_scan(tok, lane), page_in = warp_scan(page, lane);
-  const int lost_in = warp_scan(lost, lane);
+  int tok0, page0, lost0;
+  const int tok_in = warp_scan(tok, lane, tok0), page_in = warp_scan(page, lane, page0);
+  const int lost_in = warp_scan(lost, lane, lost0);
   if (lane == 31) {
     s_part[warp][0] = tok_in;
     s_part[warp][1] = page_in;
     s_part[warp][2] = lost_in;
   }
   __syncthreads();
-  int tok0 = tok_in - tok, page0 = page_in - page, tokens = 0, pages = 0, beyond = 0;
+  int tokens = 0, pages = 0, beyond = 0;
   for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) {
-      tok0 += s_part[w][0];
-      page0 += s_part[w][1];
+      tok0 = add(tok0, s_part[w][0]);
+      page0 = add(page0, s_part[w][1]);
     }
-    tokens += s_part[w][0];
-    pages += s_part[w][1];
-    beyond += s_part[w][2];
+    tokens = add(tokens, s_part[w][0]);
+    pages = add(pages, s_part[w][1]);
+    beyond = add(beyond, s_part[w][2]);
   }
   for (int b = b0; b < b1; ++b) {
-    s_tok[b] += tok0;
-    s_page[b] += page0;
+    s_tok[b] = add(s_tok[b], tok0);
+    s_page[b] = add(s_page[b], page0);
   }
   if (tid == 0) {
     s_tok[A.B] = tokens;
@@ -133,7 +145,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanArgs A) {
   for (int b = at; b <= A.B; b += step) A.cu[b] = min(s_tok[b], A.N);
   if (at == 0) {
     *A.head_out = head + min(pages, avail);
-    *A.missing = beyond + max(0, pages - avail);
+    *A.missing = add(beyond, max(0, pages - avail));
     if (tokens > A.N) atomicOr(A.err, ERR_PAGE);
   }
   for (int i = at; i < pages; i += step) {
@@ -217,14 +229,14 @@ __global__ void __launch_bounds__(THREADS) reserve_kernel(const ReserveArgs A) {
   const int b = blockIdx.x * THREADS + threadIdx.x;
   if (b >= A.B) return;
   const uint32_t ps = (uint32_t)A.ps, c = length_of(A.context, b), n = length_of(A.fresh, b);
-  const uint32_t before = max(c, (uint32_t)min(max(A.reserved[b], 0), 1 << 30));
+  const uint32_t before = max(c, (uint32_t)min(max(A.reserved[b], 0), LONGEST));
   int pages = pages_of(before, ps), end = max(pages, min(pages_of(c + n, ps), A.width));
   while (pages < end) {
     const int mid = pages + ((end - pages) >> 1);
     if (A.table[(int64_t)b * A.table_stride + mid] >= 0) pages = mid + 1; else end = mid;
   }
   const uint32_t reach = max(before, min(c + n, (uint32_t)pages * ps));
-  A.reserved[b] = (int)min(reach, 1u << 30);
+  A.reserved[b] = (int)min(reach, (uint32_t)LONGEST);
 }
 
 // ---------------------------------------------------------------------------

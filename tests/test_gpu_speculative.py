@@ -821,3 +821,30 @@ def test_tree_attention_contexts_past_the_table(cuda, dtype, new, heads):
     dev["block_table"] = dev["block_table"][:, :0]
     out, lse = ops.tree_attention(**dev, return_lse=True)
     assert _lib_errors() == 4 and not out.any() and torch.isinf(lse).all()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("ps,rows,slots,missing", [
+    (1, [[9, 8], [-1, -1], [-1, -1], [7, 6], [-1, -1]], [9, 8, *[-1] * 62], 2 ** 30 + 1),
+    (8, [[9, -1], [-1, 8], [-1, -1], [7, 6], [-1, -1]],
+     [72, 73, 74, *[-1] * 4, *range(64, 72), *[-1] * 49], 3 * 2 ** 27 - 2),
+])
+def test_paged_plan_of_lengths_that_nobody_meant(cuda, ps, rows, slots, missing, tree):
+    # Lengths and sums past 2^30: what comes before is planned, the rest has no place.
+    _lib_errors()
+    table = torch.full((5, 2), -1, dtype=torch.int32, device=cuda)
+    parents = ints([-1, 0, 1, -1, *range(60)], cuda) if tree else None
+    ctx = ints([0, 4, 2 ** 31 - 1, 0, -7], cuda)
+    new = ints([3, 2 ** 30, 2 ** 31 - 1, 2 ** 30, 5], cuda)
+    got = ops.paged_plan(ctx, new, table, ints([9, 8, 7, 6], cuda), ints([0], cuda), ps, 64,
+                         parents=parents)
+    assert _lib_errors() == 4
+    assert got.cu_tokens.tolist() == [0, 3, 64, 64, 64, 64]
+    assert table.tolist() == rows and got.slots.tolist() == slots
+    assert got.missing.tolist() == [missing] and got.free_head.tolist() == [4]
+    if tree:
+        assert got.positions.tolist() == [0, 1, 2, *range(4, 65)]
+        assert got.tree_mask[:4].tolist() == [1, 3, 7, 1]
+    held = ints([0, 0, 0, 0, 0], cuda)
+    ops.paged_reserve(ctx, new, table, held, ps)
+    assert held.tolist() == ([2, 4, 2 ** 30 - 1, 2, 0] if ps == 1 else [3, 16, 2 ** 30 - 1, 16, 0])
