@@ -848,3 +848,91 @@ def test_paged_plan_of_lengths_that_nobody_meant(cuda, ps, rows, slots, missing,
     held = ints([0, 0, 0, 0, 0], cuda)
     ops.paged_reserve(ctx, new, table, held, ps)
     assert held.tolist() == ([2, 4, 2 ** 30 - 1, 2, 0] if ps == 1 else [3, 16, 2 ** 30 - 1, 16, 0])
+
+
+@pytest.mark.parametrize("requests,longest,heads,kv,dk,dv", [
+    (33, 90, 4, 2, 64, 64), (100, 150, 6, 2, 128, 128), (257, 40, 8, 8, 192, 128),
+])
+def test_prompt_attention_many_requests(cuda, requests, longest, heads, kv, dk, dv):
+    # More requests than a warp counts at once, empty and long ones among them.
+    r, gen = random.Random(requests), torch.Generator(device=cuda).manual_seed(requests)
+    lens = [r.choice([0, 1, r.randint(0, longest)]) for _ in range(requests)]
+    lens[requests // 2] = 700
+    keys = [n + r.choice([0, 0, 65]) if n else r.choice([0, 3]) for n in lens]
+    q = torch.randn(sum(lens), heads, dk, generator=gen, device=cuda).bfloat16()
+    k = torch.randn(sum(keys), kv, dk, generator=gen, device=cuda).bfloat16()
+    v = torch.randn(sum(keys), kv, dv, generator=gen, device=cuda).bfloat16()
+    cq, ck = sums(lens), sums(keys)
+    out, lse = ops.prompt_attention(q, k, v, ints(cq, cuda), 700, cu_seqlens_k=ints(ck, cuda),
+                                    return_lse=True)
+    for b in range(requests):
+        n, m = lens[b], keys[b]
+        if n == 0:
+            continue
+        x = q[cq[b]:cq[b + 1]].double().view(n, kv, heads // kv, dk)
+        s = torch.einsum("tkgd,skd->kgts", x, k[ck[b]:ck[b + 1]].double()) * dk ** -0.5
+        s.masked_fill_(torch.ones(n, m, dtype=torch.bool, device=cuda).triu(1 + m - n),
+                       float("-inf"))
+        w, p, vb = s.logsumexp(-1), s.softmax(-1), v[ck[b]:ck[b + 1]].double()
+        want, size = (torch.einsum("kgts,skd->tkgd", p, y).reshape(n, heads, dv).cpu()
+                      for y in (vb, vb.abs()))
+        check_attention(out[cq[b]:cq[b + 1]], lse[cq[b]:cq[b + 1]], want,
+                        w.permute(2, 0, 1).reshape(n, heads).cpu(), size, torch.bfloat16)
+
+
+@pytest.mark.parametrize("most", [17, 64, 5000])
+def test_tree_attention_longest_length_far_above_the_lengths(cuda, most):
+    # The kernel is chosen by max_tokens; what it computes is not.
+    dev, want = paged_case(cuda, torch.bfloat16, [300, 0, 70, 1000], [1, 2, 0, 5], 8, 2, 128, 128,
+                           16, 48, tree=False)
+    dev["max_tokens"] = most
+    out, lse = ops.tree_attention(**dev, return_lse=True)
+    check_attention(out, lse, *want, torch.bfloat16)
+    assert torch.equal(out, ops.tree_attention(**dev))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [5, 3], [30, 64]])
+def test_caches_past_32_bit_offsets(cuda, new):
+    # The same pages at the end of a cache of over 2^32 bytes (and 2^31 elements), written
+    # by paged_append; an infinite value of the step is taken from the cache itself.
+    dev, _ = paged_case(cuda, torch.bfloat16, [70, 500], new, 8, 4, 128, 128, 16, 49)
+    pages = dev["k_cache"].shape[0]
+    most = (2 ** 31 + 2 ** 25) // (4 * 16 * 128)
+    table = dev["block_table"].clone()
+    slots = torch.tensor([int(table[b, p // 16]) * 16 + p % 16 for b, n in enumerate(new)
+                          for p in range([70, 500][b] + n)], device=cuda)
+    last = int(table[1, (500 + new[1] - 1) // 16])
+    dev["v_cache"][last, (500 + new[1] - 1) % 16, 0, 3] = float("inf")
+    want, want_lse = ops.tree_attention(**dev, return_lse=True)
+    big = [torch.empty(most, 4, 16, 128, dtype=torch.bfloat16, device=cuda).transpose(1, 2)
+           for _ in range(2)]
+    k, v = (dev[n].flatten(0, 1)[slots] for n in ("k_cache", "v_cache"))
+    ops.paged_append(k, v, *big, slots + (most - pages) * 16)
+    out, lse = ops.tree_attention(**{**dev, "k_cache": big[0], "v_cache": big[1],
+                                     "block_table": table + (most - pages)}, return_lse=True)
+    assert torch.equal(lse, want_lse)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[~out.isnan()], want[~want.isnan()])
+    assert not torch.isfinite(out[-1, 0, 3]) and torch.isfinite(out[..., 4:]).all()
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_drafts_past_32_bit_offsets(cuda, probs):
+    # The last rows of over 2^31 logits, as a batch of their own and as they lie.
+    c = verify_case(3, 163840, 4, False, probs, 0, torch.bfloat16, 50)
+    want = run_verify(c, cuda, False)
+    n, rows = c["cu"][-1], 2 ** 31 // 163840 + 20
+    logits = torch.empty(rows, 163840, dtype=torch.bfloat16, device=cuda)
+    logits[-n:] = c["logits"].to(cuda)
+    tokens = torch.zeros(rows, dtype=torch.long, device=cuda)
+    tokens[-n:] = c["tokens"].to(cuda)
+    coin = torch.zeros(rows, device=cuda)
+    coin[-n:] = c["coin"].to(cuda)
+    q = None
+    if probs:
+        q = torch.empty(rows, 163840, device=cuda)
+        q[-n:] = c["probs"].to(cuda)
+    got = ops.verify_drafts(logits, tokens, ints([rows - n + x for x in c["cu"]], cuda), 4, coin,
+                            c["noise"].to(cuda), c["temps"].to(cuda), draft_probs=q)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
