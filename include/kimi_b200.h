@@ -69,7 +69,8 @@ KB_API int kb_get_pdl(void);
  * and set a bit here.
  * kb_device_errors() copies the word to the host (synchronizes the stream)
  * and clears it.  Bit 0: expert index out of range.  Bit 1: a bounded wait
- * ran out.  Bit 2: a page, slot or token outside its table, cache or buffer
+ * ran out (the call ended early: its outputs are not valid, and workspaces with counters
+ * have to be zeroed again).  Bit 2: a page, slot or token outside its table, cache or buffer
  * (skipped; attention treats its keys as absent).  Bit 3: a tree parent that
  * is not before its child, a tree of over 64 tokens, or a drafted token id
  * outside the vocabulary (the token is never taken). */

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 from ctypes import c_float, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
+from typing import Callable
 
 LIB_PATH = Path(__file__).resolve().with_name("libkimi_b200.so")
 
@@ -273,8 +274,22 @@ def pdl_enabled() -> bool:
     return bool(lib().kb_get_pdl())
 
 
+ERR_WAIT = 2    # device error bit 1: a bounded wait ran out
+
+# Called when a wait ran out: the call ended early, and counters in kept scratch, that
+# every call leaves at zero, may not be.
+on_wait_error: list[Callable[[], None]] = []
+
+
 def device_errors(stream: int | None = None) -> int:
-    """Read and clear the device error word (synchronizes ``stream``)."""
+    """Read and clear the device error word (synchronizes ``stream``).
+
+    After bit 1 (a bounded wait ran out) the kept scratch is given up: the next
+    calls make their own.
+    """
     out = c_uint32(0)
     check("kb_device_errors", lib().kb_device_errors(c_void_p(stream or 0), ctypes.byref(out)))
+    if out.value & ERR_WAIT:
+        for forget in on_wait_error:
+            forget()
     return int(out.value)

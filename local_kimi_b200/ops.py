@@ -101,6 +101,7 @@ def _dense_contig(t: torch.Tensor) -> torch.Tensor:
 
 
 _WORKSPACES: dict[tuple, torch.Tensor] = {}
+_lib.on_wait_error.append(_WORKSPACES.clear)
 _CAPTURED: dict[tuple, tuple[int, torch.Tensor]] = {}
 
 

@@ -389,3 +389,26 @@ def test_calls_go_to_the_tensors_device(library, any_device, monkeypatch):
     assert seen == [(f"kb_{name}", torch.device("cpu")) for name in (
         "paged_plan", "paged_reserve", "paged_append", "prompt_attention", "tree_attention",
         "verify_drafts")]
+
+
+def test_scratch_is_given_up_after_a_wait_ran_out(monkeypatch):
+    # A call that ended early may leave counters that the next call would go on from.
+    bits = {"now": 0}
+
+    class fake:
+        @staticmethod
+        def kb_device_errors(stream, out):
+            out._obj.value = bits["now"]
+            return 0
+
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    monkeypatch.setattr(ops, "_capturing", lambda: False)
+    cpu = torch.device("cpu", 0)
+    held = lambda: ops._kept_scratch(("wait", 0, 7, 256), cpu, 7, 256, 64)  # noqa: E731
+    first = held()
+    first.fill_(1)
+    for word, kept in ((0, True), (4, True), (2, False)):
+        bits["now"] = word
+        assert _lib.device_errors() == word
+        assert (held() is first) == kept
+    assert not held().any()
