@@ -15,8 +15,9 @@
 // memory and then takes its share of the fresh pages and of the new tokens,
 // each found by a binary search in the sums.  A token in a fresh page reads
 // the free list, not the table entry another CTA may be writing.  A few
-// kilobytes of traffic: the time is launch and dependent-load latency (32 requests:
-// 6 us; 2048: 13 us).
+// kilobytes of traffic.  A few requests cost launch and dependent-load latency, many the
+// sums that every CTA makes, whatever the tokens (replayed: 32 requests 3.2 us, 256 3.6,
+// 1024 4.5, 2048 6.5, with masks 10.9; 8192 46).
 #include "kb_common.cuh"
 
 namespace kb {
@@ -256,8 +257,10 @@ struct AppendArgs {
 
 // Four 16-byte pieces per thread, loaded before any is stored; a token's pieces
 // are its heads' key rows and then its heads' value rows, so neighbouring threads
-// move neighbouring bytes.  Bound by the bytes, once in and once out (8192 tokens of 8
-// heads of 128 + 128 to random slots of 256 bytes: 16 us, 4 TB/s).
+// move neighbouring bytes.  8192 tokens of 8 heads of 128 + 128: 15.3 us replayed (4.4
+// TB/s), bound by instructions: 85 a piece, most of them the divisions that find its
+// head, page and row, at 66 % of the issue slots.  The order of the slots is of no
+// account (in order 15.2 us, single rows at random 15.3).
 constexpr int PIECES = 4;
 
 __global__ void __launch_bounds__(THREADS) append_kernel(const AppendArgs A) {

@@ -51,18 +51,19 @@
 // Measured: 8192 tokens x 32 heads, 192 + 128: 545 us alone (1260 TFLOP/s), 656 back
 // to back under the power cap (1047; cuBLAS 1403); 24 prompts of 1 to 2047 tokens,
 // 32/8 heads of 128: 139 us (736 TFLOP/s; units of few steps, 5500 clocks of start and
-// end each).
+// end each); 5 prompts of 37 tokens over up to 2048 keys, 8/2 heads of 64: 5.9 us and
+// 0.83 a step (replayed).
 //
 // Paged cache (PAGED).  A unit is up to 256 rows (token * group + head) of one
 // request and key/value head, against the cache in 64-key steps; with few rows
 // tile B is idle and the bytes of the cache bound the work.  All units' steps
 // form one line cut into equal runs, one per CTA, as in kb_tree.cu; a unit that
 // falls to several CTAs is joined from fp32 partial sums by the CTA that finishes
-// last.  16 trees of up to 24 tokens, 4 heads a group, up to 4095 cached: 44 us; the
-// a step of one tile
-// takes 1.1 us, a CTA's first scores are there after 6, and partial sums take 3 us,
-// counting them 1, joining them 5.  Keys and values come page by page; q too by tensor copies where one tile
-// holds a request's rows, else by gathered 16-byte copies into the same layout.
+// last.  16 trees of up to 24 tokens, 4 heads a group, up to 4095 cached: 43 us; a step
+// of one tile takes 1.1 us, a CTA's first scores are there after 6, and partial sums
+// take 3 us, counting them 1, joining them 5.  Keys and values come page by page; q too
+// by tensor copies where one tile holds a request's rows, else by gathered 16-byte copies
+// into the same layout.
 //
 // In the last tiles of a unit some rows do not see some keys, or the tile
 // reaches past the request's end into its neighbour.  A value there that is
@@ -1035,7 +1036,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
               most[3] = __vmaxu2(most[3], x.w & 0x7fff7fffu);
             }
             const uint32_t top = __vmaxu2(__vmaxu2(most[0], most[1]), __vmaxu2(most[2], most[3]));
-            const bool odd = odd_element<F16>((uint16_t)top) || odd_element<F16>((uint16_t)(top >> 16));
+            const bool odd =
+                odd_element<F16>((uint16_t)top) || odd_element<F16>((uint16_t)(top >> 16));
             if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll 1
               for (int i = 0; i < S::VC * BLOCK / 512; ++i) {
@@ -1078,8 +1080,8 @@ static int launch_prompt(const CUtensorMap& mq, const CUtensorMap& mk, const CUt
   const void* fn = reinterpret_cast<const void*>(&prompt_kernel<DKP, DVP, F16, PAGED>);
   const int st = allow_smem(fn, S::SMEM, done, mu);
   if (st != KB_OK) return st;
-  return launch(prompt_kernel<DKP, DVP, F16, PAGED>, dim3(grid), dim3(PROMPT_THREADS), (size_t)S::SMEM,
-                stream, mq, mk, mv, A);
+  return launch(prompt_kernel<DKP, DVP, F16, PAGED>, dim3(grid), dim3(PROMPT_THREADS),
+                (size_t)S::SMEM, stream, mq, mk, mv, A);
 }
 
 template <bool PAGED>

@@ -386,8 +386,8 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
             if (!((valid >> c) & 1) || !sees(j >> 1, key0 + c)) s[i][j] = -INFINITY;
           }
         // Values of keys that do not exist become zero, and so do elements of
-        // this step's values that are no numbers (noted for the end).  Warps
-        // with the same keys may do so at the same time: they write the same.
+        // this step's values that are no numbers (noted for the end).  Each warp
+        // does so for its own 16 keys, which no other reads.
         const bool scan = step_keys && (G.n > 1 || A.mask);
         const uint32_t there = (uint32_t)(valid >> (warp * S::KPW));
         bool wrote = false;
@@ -672,8 +672,12 @@ __global__ void __launch_bounds__(TreeShape<DKP, DVP>::THREADS,
 
 // Rows (tokens x heads of a group) up to which the warp-level matrix steps are
 // used; more rows go to the 5th-generation tensor cores (kb_prompt.cu), which pad
-// to 128.  Measured, 16 requests of up to 4095 tokens, 128 wide, 4 heads a group:
-// 16 rows 33 us here and 41 there, 32 rows 50 and 41.
+// to 128.  Measured (replayed, us, here / there):
+//   16 rows: 16 requests of 2048, 8 key/value heads of 128: 35 / 47, of 64: 23 / 44;
+//     64 requests of 1024: 57 / 98; 16 of 2048, 32 heads of 192 + 128: 112 / 141;
+//     4 of 16000, 2 heads of 128: 49 / 53;
+//   32 rows (two blocks here, which read the keys twice): 53 / 48, 34 / 44, 99 / 98,
+//     213 / 161, 45 / 48.
 constexpr int64_t MMA_ROWS = 16;
 
 template <int DKP, int DVP, bool F16>

@@ -23,9 +23,10 @@
 // takes from the first is in the call's own workspace, so calls from several threads
 // may meet on a stream in any order.  Bound by the
 // bytes: the logits once, and of one row a request logits, noise and q again.
-// Measured: 256 requests of up to 5 tokens, 163840 wide, with q: 121 us, 54 for the
-// rows (4.7 TB/s; special function unit 62 % busy) and 70 for the picks (4.3
-// TB/s); one request of 9 tokens: 18.4 us with a cold cache, 14.4 replayed at once.
+// Measured: 256 requests of up to 5 tokens, 163840 wide, with q: 122 us, 54 for the
+// rows (4.7 TB/s; special function unit 63 % busy) and 70 for the picks (4.3
+// TB/s; 41 % of the warps there, which wait for loads: 8.5 of them stalled for each
+// that issues); one request of 9 tokens: 18.4 us with a cold cache, 12.5 replayed at once.
 //
 // Rows start anywhere (an odd vocabulary): the loads begin at the row's first
 // 16-byte boundary, what lies before and after goes one by one.  The fast
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 4) pick_kernel(const Args A) {
     }
     s_par[t] = up;
     s_tok[t] = x;
-    s_coin[t] = A.coin ? A.coin[first + t] : 0.f;
+    s_coin[t] = A.coin[first + t];
     s_qx[t] = A.probs && up >= 0 ? A.probs[(first + t) * A.probs_stride + x] : 1.f;
   }
   __syncthreads();
@@ -491,7 +492,8 @@ __global__ void __launch_bounds__(THREADS, 4) pick_kernel(const Args A) {
   }
   for (int i = lo + tid; i < start; i += THREADS)
     take(tidy(logit<TYPE>(A.logits, base + i)), noise[i], q ? q[i] : 0.f, i);
-  const bool wide = ((uintptr_t)(noise + start) & 15) == 0 && (!q || ((uintptr_t)(q + start) & 15) == 0);
+  const bool wide =
+      ((uintptr_t)(noise + start) & 15) == 0 && (!q || ((uintptr_t)(q + start) & 15) == 0);
   constexpr int BATCH = 2;
   for (int i0 = tid; i0 < count; i0 += THREADS * BATCH) {
     uint4 v[BATCH];
