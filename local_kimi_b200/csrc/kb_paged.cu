@@ -16,8 +16,8 @@
 // each found by a binary search in the sums.  A token in a fresh page reads
 // the free list, not the table entry another CTA may be writing.  A few
 // kilobytes of traffic.  A few requests cost launch and dependent-load latency, many the
-// sums that every CTA makes, whatever the tokens (replayed: 32 requests 3.2 us, 256 3.6,
-// 1024 4.5, 2048 6.5, with masks 10.9; 8192 46).
+// sums that every CTA makes (replayed, with few tokens: 32 requests 3.2 us, 256 3.6,
+// 1024 4.5, 2048 6.5, 8192 46; 2048 with 200 thousand tokens 10.9).
 #include "kb_common.cuh"
 
 namespace kb {
@@ -258,7 +258,7 @@ struct AppendArgs {
 // Four 16-byte pieces per thread, loaded before any is stored; a token's pieces
 // are its heads' key rows and then its heads' value rows, so neighbouring threads
 // move neighbouring bytes.  8192 tokens of 8 heads of 128 + 128: 15.3 us replayed (4.4
-// TB/s), bound by instructions: 85 a piece, most of them the divisions that find its
+// TB/s), bound by instructions: 168 a piece, most of them the divisions that find its
 // head, page and row, at 66 % of the issue slots.  The order of the slots is of no
 // account (in order 15.2 us, single rows at random 15.3).
 constexpr int PIECES = 4;
