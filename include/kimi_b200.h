@@ -523,6 +523,113 @@ KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows
                    int64_t* out_tokens, int32_t* path, int32_t* accepted, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Requests that share a prompt (no counterpart in the reference).             */
+/* ------------------------------------------------------------------------- */
+
+/* Linear attention with a decay for each head.  With S [Dk, Dv] of each request
+ * and head in fp32: S_t = exp(g_t) S_{t-1} + k_t v_t^T, o_t = scale * q_t S_t.
+ * q [tokens, Hq, Dk], k [tokens, Hk, Dk], v [tokens, H, Dv] with token and head
+ * strides; H a multiple of Hq and of Hk (head h takes q head h / (H / Hq));
+ * dtype 0 bf16, 1 f16, 2 f32.  Widths multiples of 8 up to 128; pointers and rows
+ * 16-byte aligned.  log_decay fp32 [tokens, H], or [H] with per_token 0; values
+ * above 0 count as 0.  state fp32 [slots][H][Dk][Dv] with slot and head strides
+ * (blocks dense), NULL: from zero and not kept; request b's slot is
+ * state_index[b], or b; negative: from zero and not kept.  S is read before the
+ * first token and written after the last; no two requests name one slot.  out
+ * [tokens, H, Dv] contiguous; rows outside every request are zero, rows of a
+ * request past max_tokens are not written.  A value that is no number reaches the
+ * outputs of its own and later tokens only, there as not-a-number.
+ * The workspace of kb_linear_attention_workspace_size bytes (often 0) may hold
+ * anything, but is this call's alone until it is done on the stream.
+ * The step takes one token of each of B requests. */
+KB_API size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64_t Dk, int64_t Dv,
+                   int dtype, int64_t total, int64_t max_tokens);
+KB_API int kb_linear_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                   int64_t Hq, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                   int64_t Hk, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                   int64_t H, int64_t Dk, int64_t Dv, int dtype, const float* log_decay,
+                   int per_token, float* state, int64_t state_slot_stride,
+                   int64_t state_head_stride, int64_t slots, const int32_t* state_index,
+                   const int32_t* cu_tokens, int64_t B, int64_t total, int64_t max_tokens,
+                   float scale, void* out, void* workspace, size_t workspace_bytes,
+                   void* stream);
+KB_API int kb_linear_attention_step(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                   int64_t Hq, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                   int64_t Hk, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                   int64_t H, int64_t Dk, int64_t Dv, int dtype, const float* log_decay,
+                   int per_token, float* state, int64_t state_slot_stride,
+                   int64_t state_head_stride, int64_t slots, const int32_t* state_index,
+                   int64_t B, float scale, void* out, void* stream);
+
+/* Row targets[i] of the block table goes on from the context of row sources[i]:
+ * it gets that row's full pages (shared from then on) and, where the context ends
+ * inside a page, the next page of free_pages from *free_head on, in the order of
+ * the pairs.  block_table, context_lens and reserved_lens (may be NULL) are
+ * written at the targets.  The fresh page is to be filled by kb_paged_copy:
+ * copy_from, copy_to [n] (-1: nothing to copy) and copy_rows [n].  A pair without
+ * a page leaves its target empty; *missing counts those.  Pairs with a negative
+ * row are skipped, those whose target is a source, named before or past the table
+ * too (device error bit 2).  B, n <= 12288. */
+KB_API int kb_paged_fork(int32_t* context_lens, int32_t* reserved_lens, int64_t B,
+                   int32_t* block_table, int64_t table_stride, int64_t table_width,
+                   const int32_t* sources, const int32_t* targets, int64_t n,
+                   const int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                   int64_t page_size, int32_t* copy_from, int32_t* copy_to, int32_t* copy_rows,
+                   int32_t* free_head_out, int32_t* missing, void* stream);
+
+/* Row b's pages reach reserved_lens[b] tokens, of which it keeps the first
+ * keep_lens[b].  Pages that a row gives up and no row keeps are written in
+ * ascending order to free_pages in front of *free_head; *free_head_out is the
+ * first.  Where more pages come back than the list has places there, the highest
+ * are kept (device error bit 2).  n_pages <= 524288, B <= 12288. */
+KB_API int kb_paged_free(const int32_t* reserved_lens, const int32_t* keep_lens, int64_t B,
+                   const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                   int32_t* free_pages, int64_t n_free, const int32_t* free_head,
+                   int64_t page_size, int64_t n_pages, int32_t* free_head_out, void* stream);
+
+/* The used pages (of the table, within reserved_lens) take the lowest ids of those
+ * that are used or free (free_pages from *free_head on): the i-th used page above
+ * them moves to the i-th free one among them.  table_out [B, table_width]: the new
+ * places, -1 past a row's pages; free_out [n_free]: the old list, its free pages in
+ * ascending order; copy_from, copy_to [n_pages / 2]: the moves in ascending order,
+ * then -1; scratch [n_pages], with anything in it.  Limits as kb_paged_free. */
+KB_API int kb_paged_compact(const int32_t* reserved_lens, int64_t B, const int32_t* block_table,
+                   int64_t table_stride, int64_t table_width, const int32_t* free_pages,
+                   int64_t n_free, const int32_t* free_head, int64_t page_size, int64_t n_pages,
+                   int32_t* table_out, int32_t* free_out, int32_t* copy_from, int32_t* copy_to,
+                   int32_t* free_head_out, int32_t* scratch, void* stream);
+
+/* The first copy_rows[i] rows (NULL: all) of page copy_from[i] to page copy_to[i]
+ * of both caches; pairs with a negative page are skipped, those with one past the
+ * caches too (device error bit 2).  No page is a target twice, or source and
+ * target.  16-bit elements; pointers 16-byte aligned, strides multiples of 8. */
+KB_API int kb_paged_copy(uint16_t* k_cache, const int64_t* k_strides, uint16_t* v_cache,
+                   const int64_t* v_strides, int64_t n_pages, int64_t page_size, int64_t H,
+                   int64_t Dk, int64_t Dv, const int32_t* copy_from, const int32_t* copy_to,
+                   const int32_t* copy_rows, int64_t n, void* stream);
+
+/* out = logits [rows, V] (dtype as above) with each request's penalties, biases and
+ * mask, in fp32 and in this order: a token in the request's history is divided by
+ * repetition[b] where positive, else multiplied; its count in the answer (history
+ * from prompt_lens[b] on, and the drafted tokens above the row) times frequency[b]
+ * is subtracted, and presence[b] where it counts; biases are added; tokens whose
+ * bit is not set in the row's words of allowed are -infinity.  Row b belongs to
+ * request b, or rows [cu_tokens[b], cu_tokens[b+1]) do.  history [B, longest]
+ * int64, of which history_lens[b] count; tokens [rows] (with cu_tokens): drafted
+ * tokens, of which row r has those whose bits tree_mask[r] has, or without masks
+ * its own and those before it; bias_ids [B, n_biases] (at most 4096), negative ids
+ * unused.  Every pointer but logits and out may be NULL.  out may be logits, with
+ * the same stride.  Token ids past V are skipped (device error bit 3). */
+KB_API int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t rows, int64_t V,
+                   int dtype, void* out, int64_t out_stride, int64_t B, const int64_t* history,
+                   int64_t history_stride, int64_t longest, const int32_t* history_lens,
+                   const int32_t* prompt_lens, const float* repetition, const float* presence,
+                   const float* frequency, const int64_t* bias_ids, int64_t ids_stride,
+                   const float* bias_values, int64_t values_stride, int64_t n_biases,
+                   const int32_t* allowed, int64_t allowed_stride, const int32_t* cu_tokens,
+                   const int64_t* tokens, const int64_t* tree_mask, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

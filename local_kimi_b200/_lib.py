@@ -216,6 +216,49 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
          c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p],
     ),
+    "kb_linear_attention_workspace_size": (
+        c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int, c_int64, c_int64],
+    ),
+    "kb_linear_attention": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+         c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64,
+         c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p,
+         c_void_p, c_size_t, c_void_p],
+    ),
+    "kb_linear_attention_step": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+         c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_int64,
+         c_int64, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p],
+    ),
+    "kb_paged_fork": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+         c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p],
+    ),
+    "kb_paged_free": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+         c_int64, c_int64, c_void_p, c_void_p],
+    ),
+    "kb_paged_compact": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+         c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "kb_paged_copy": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "kb_adjust_logits": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
+         c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
 }
 
 _LIB: ctypes.CDLL | None = None

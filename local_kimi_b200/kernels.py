@@ -44,6 +44,13 @@ PAGED_APPEND = "paged_append"
 PROMPT_ATTENTION = "prompt_attention"
 TREE_ATTENTION = "tree_attention"
 VERIFY_DRAFTS = "verify_drafts"
+LINEAR_ATTENTION = "linear_attention"
+LINEAR_STEP = "linear_attention_step"
+PAGED_FORK = "paged_fork"
+PAGED_FREE = "paged_free"
+PAGED_COMPACT = "paged_compact"
+PAGED_COPY = "paged_copy"
+ADJUST_LOGITS = "adjust_logits"
 
 _DESCRIPTIONS = {
     W4A16_DENSE: "sm_100a W4A16 projection: HBM-streamed INT4 codes, bf16x2 decode in "
@@ -64,6 +71,13 @@ _DESCRIPTIONS = {
     TREE_ATTENTION: "sm_100a attention of drafted trees (or single tokens) over the paged cache.",
     VERIFY_DRAFTS: "sm_100a acceptance of drafted tokens against the target's logits, and the "
     "token after them.",
+    LINEAR_ATTENTION: "sm_100a linear attention with a decay a head over packed prompts.",
+    LINEAR_STEP: "sm_100a linear attention of one token a request, states in place.",
+    PAGED_FORK: "sm_100a block table rows that share another row's full pages.",
+    PAGED_FREE: "sm_100a pages that no request holds any more, back to the free list.",
+    PAGED_COMPACT: "sm_100a used pages to the lowest places of the pool.",
+    PAGED_COPY: "sm_100a copies of cache pages by lists.",
+    ADJUST_LOGITS: "sm_100a penalties, biases and grammar masks on logits, drafted trees included.",
 }
 
 _OPS = {
@@ -79,6 +93,13 @@ _OPS = {
     PROMPT_ATTENTION: ops.prompt_attention,
     TREE_ATTENTION: ops.tree_attention,
     VERIFY_DRAFTS: ops.verify_drafts,
+    LINEAR_ATTENTION: ops.linear_attention,
+    LINEAR_STEP: ops.linear_attention_step,
+    PAGED_FORK: ops.paged_fork,
+    PAGED_FREE: ops.paged_free,
+    PAGED_COMPACT: ops.paged_compact,
+    PAGED_COPY: ops.paged_copy,
+    ADJUST_LOGITS: ops.adjust_logits,
 }
 
 

@@ -23,6 +23,11 @@ Operators of a speculative serving step that the reference has no kernel for
 (its MLA attention is torch einsum and softmax over projected keys and values,
 engine/klinear/attention.py:586-598): paged_plan, paged_append,
 prompt_attention, tree_attention, verify_drafts.
+
+Operators of requests that share a prompt, without a counterpart there either:
+linear_attention, linear_attention_step (one decay a head; the reference's KDA
+has one a channel), paged_fork, paged_free, paged_compact, paged_copy,
+adjust_logits.
 """
 
 from __future__ import annotations
@@ -1482,3 +1487,520 @@ def _unit_rows(t: torch.Tensor, width: int) -> tuple[torch.Tensor, int]:
     if column != 1 or (row < width and t.shape[0] > 1):
         t, row = t.contiguous(), width
     return t, max(row, width)
+
+
+# ---------------------------------------------------------------------------
+# linear attention
+# ---------------------------------------------------------------------------
+
+MAX_LINEAR_WIDTH = 128
+
+
+def _linear_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                 state: torch.Tensor | None, state_index: torch.Tensor | None, requests: int,
+                 expanded: bool):
+    """Checked inputs of linear attention: (q, k, v, decay, per_token, state strides, index)."""
+    if q.dtype not in _ELEMENT:
+        raise TypeError("queries, keys and values must be BF16, FP16 or FP32")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("queries, keys and values must share one type")
+    if log_decay.dtype != torch.float32 or log_decay.ndim not in (1, 2):
+        raise TypeError("log_decay must be an FP32 [tokens, heads] matrix or [heads] vector")
+    _require_cuda(q, "linear attention")
+    device = q.device
+    if not (k.device == v.device == log_decay.device == device):
+        raise ValueError("linear attention inputs must share one device")
+    qr, kr, vr = (_rows_of_heads(x, what, expanded) for x, what in ((q, "q"), (k, "k"), (v, "v")))
+    total, heads, dv = v.shape
+    dk = q.shape[2]
+    if q.shape[0] != total or k.shape[0] != total or k.shape[2] != dk:
+        raise ValueError("q, k and v must have the same tokens, and q and k one width")
+    if not heads or any(not x.shape[1] or heads % x.shape[1] for x in (q, k)):
+        raise ValueError("value heads must be a multiple of the query heads and of the key heads")
+    if not (0 < dk <= MAX_LINEAR_WIDTH and dk % 8 == 0 and 0 < dv <= MAX_LINEAR_WIDTH
+            and dv % 8 == 0):
+        raise ValueError(f"head widths must be multiples of 8 up to {MAX_LINEAR_WIDTH}")
+    if log_decay.shape not in ((total, heads), (heads,)):
+        raise ValueError("log_decay must have a row for each token, or one for all, of all heads")
+    index, strides = None, (0, 0)
+    if state is not None:
+        if state.dtype != torch.float32 or state.ndim != 4:
+            raise TypeError("state must be an FP32 [slots, heads, Dk, Dv] tensor")
+        if state.device != device:
+            raise ValueError("state must be on the device of the other tensors")
+        if state.shape[1:] != (heads, dk, dv):
+            raise ValueError("state must have the heads and widths of the values and keys")
+        s = state.stride()
+        if (s[3] != 1 or s[2] != dv or (s[0] | s[1]) & 3 or state.data_ptr() & 15
+                or (heads > 1 and s[1] < dk * dv)
+                or (state.shape[0] > 1 and s[0] < dk * dv)) and state.numel():
+            raise ValueError("state is updated in place and needs dense, 16-byte aligned [Dk, Dv] "
+                             "blocks of its own for every slot and head")
+        strides = s[:2]
+    if state_index is not None:
+        if state is None:
+            raise ValueError("state_index goes with state")
+        index = _vector(state_index, torch.int32, "state_index", device, requests)
+    elif state is not None and state.shape[0] < requests:
+        raise ValueError("state needs a slot for every request")
+    decay = log_decay if log_decay.is_contiguous() else log_decay.contiguous()
+    return qr, kr, vr, decay, int(log_decay.ndim == 2), strides, index
+
+
+def linear_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    log_decay: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    max_seqlen: int,
+    *,
+    state: torch.Tensor | None = None,
+    state_index: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Linear attention with a decay for each head, over packed prompts.
+
+    For each head, ``S_t = exp(log_decay_t) * S_{t-1} + k_t v_t^T`` and
+    ``o_t = scale * q_t S_t``.  ``q`` [tokens, Hq, Dk], ``k`` [tokens, Hk, Dk],
+    ``v`` [tokens, H, Dv] (bf16, f16 or f32; H a multiple of Hq and of Hk: head h
+    takes query head ``h // (H / Hq)``), ``log_decay`` fp32 [tokens, H] or, for a
+    fixed decay a head, [H]; values above 0 count as 0.  Request b has the tokens
+    ``cu_seqlens[b]:cu_seqlens[b+1]`` (int32), at most ``max_seqlen``.  ``state``
+    fp32 [slots, H, Dk, Dv] holds each request's S in its slot, ``state_index[b]``
+    (default: b): read as S before the first token, and updated in place.  A
+    negative slot, or no ``state``: S starts from zero and is not kept.  No two
+    requests may name one slot.  Returns [tokens, H, Dv] of the inputs' type; rows
+    outside every request are zero.
+    """
+    if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must have one entry more than there are requests")
+    requests = cu_seqlens.shape[0] - 1
+    qr, kr, vr, decay, per_token, strides, index = _linear_args(
+        q, k, v, log_decay, state, state_index, requests, expanded=False)
+    device = q.device
+    cu = _vector(cu_seqlens, torch.int32, "cu_seqlens", device)
+    total, heads, dv = v.shape
+    dk = q.shape[2]
+    if max_seqlen < 0 or (total and not max_seqlen):
+        raise ValueError("max_seqlen must not be negative, nor 0 with tokens")
+    scale = _scale_of(scale, dk)
+    if requests == 0:
+        return v.new_zeros(total, heads, dv)
+    out = torch.empty(total, heads, dv, dtype=v.dtype, device=device)
+    if total == 0:
+        return out
+    nbytes = _lib.lib().kb_linear_attention_workspace_size(requests, heads, dk, dv,
+                                                           _ELEMENT[q.dtype], total, max_seqlen)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _on(device)(
+        "kb_linear_attention",
+        qr.data_ptr(), qr.stride(0), qr.stride(1), q.shape[1], kr.data_ptr(), kr.stride(0),
+        kr.stride(1), k.shape[1], vr.data_ptr(), vr.stride(0), vr.stride(1), heads, dk, dv,
+        _ELEMENT[q.dtype], decay.data_ptr(), per_token,
+        None if state is None else state.data_ptr(), strides[0], strides[1],
+        0 if state is None else state.shape[0], None if index is None else index.data_ptr(),
+        cu.data_ptr(), requests, total, max_seqlen, scale, out.data_ptr(),
+        None if ws is None else ws.data_ptr(), nbytes, _raw_stream(device),
+    )
+    return out
+
+
+def linear_attention_step(
+    state: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    log_decay: torch.Tensor,
+    *,
+    state_index: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """``linear_attention`` of one token for every request (decoding): ``q`` [B, Hq, Dk],
+    ``k`` [B, Hk, Dk], ``v`` [B, H, Dv], ``log_decay`` fp32 [B, H] or [H].
+
+    ``state`` fp32 [slots, H, Dk, Dv] is updated in place.  Returns [B, H, Dv].
+    """
+    requests = q.shape[0]
+    qr, kr, vr, decay, per_token, strides, index = _linear_args(
+        q, k, v, log_decay, state, state_index, requests, expanded=True)
+    device = q.device
+    _, heads, dv = v.shape
+    dk = q.shape[2]
+    scale = _scale_of(scale, dk)
+    out = torch.empty(requests, heads, dv, dtype=v.dtype, device=device)
+    if requests == 0:
+        return out
+    _on(device)(
+        "kb_linear_attention_step",
+        qr.data_ptr(), qr.stride(0), qr.stride(1), q.shape[1], kr.data_ptr(), kr.stride(0),
+        kr.stride(1), k.shape[1], vr.data_ptr(), vr.stride(0), vr.stride(1), heads, dk, dv,
+        _ELEMENT[q.dtype], decay.data_ptr(), per_token, state.data_ptr(), strides[0], strides[1],
+        state.shape[0], None if index is None else index.data_ptr(), requests, scale,
+        out.data_ptr(), _raw_stream(device),
+    )
+    return out
+
+
+# ---------------------------------------------------------------------------
+# pages that come and go
+# ---------------------------------------------------------------------------
+
+
+class Fork(NamedTuple):
+    """What ``paged_fork`` returns (all on the device)."""
+
+    copy_from: torch.Tensor  # int32 [pairs]: the page to copy from, -1: none
+    copy_to: torch.Tensor    # int32 [pairs]: the fresh page
+    copy_rows: torch.Tensor  # int32 [pairs]: rows to copy
+    free_head: torch.Tensor  # int32 [1], the next call's free_head
+    missing: torch.Tensor    # int32 [1], pairs that were not made for want of a page
+
+
+class Compaction(NamedTuple):
+    """What ``paged_compact`` returns (all on the device)."""
+
+    block_table: torch.Tensor  # int32 [B, width]: the pages' new places, -1 past them
+    free_pages: torch.Tensor   # the free list, in ascending order from free_head on
+    free_head: torch.Tensor    # int32 [1]
+    copy_from: torch.Tensor    # int32 [num_pages // 2]: pages to copy, then -1
+    copy_to: torch.Tensor      # int32 [num_pages // 2]
+
+
+def _table_args(table: torch.Tensor, what: str, page_size: int) -> tuple[int, int, int]:
+    """Requests, width and row stride of a block table used in place."""
+    if table.dtype != torch.int32 or table.ndim != 2:
+        raise TypeError("block_table must be an int32 [requests, pages] matrix")
+    _require_cuda(table, what)
+    requests, width = table.shape
+    if requests == 0 or width == 0 or page_size <= 0:
+        raise ValueError(f"{what} requires a request, a table column and a page size")
+    if table.stride(1) != 1 or (requests > 1 and table.stride(0) < width):
+        raise ValueError("block_table needs rows of unit stride")
+    return requests, width, max(table.stride(0), width)
+
+
+def _in_place(t: torch.Tensor, what: str, device: torch.device, length: int | None = None):
+    """An int32 vector that is updated in place."""
+    if _vector(t, torch.int32, what, device, length) is not t:
+        raise ValueError(f"{what} is updated in place and needs unit stride")
+    return t
+
+
+def paged_fork(
+    context_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    sources: torch.Tensor,
+    targets: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_head: torch.Tensor,
+    page_size: int,
+    *,
+    reserved_lens: torch.Tensor | None = None,
+) -> Fork:
+    """Requests ``targets`` go on from the contexts of ``sources``, sharing their full pages.
+
+    For each pair (int32 [pairs]), ``block_table[target]`` gets the source's full pages and,
+    where the context ends inside a page, the next page of ``free_pages`` (from ``free_head``
+    on, in the order of the pairs); ``context_lens[target]`` (and ``reserved_lens[target]``)
+    become the source's context.  The fresh page is to be filled by ``paged_copy`` with the
+    lists returned, for every layer whose cache the table describes.  A pair that gets no page
+    leaves its target empty and counts in ``missing``.  A negative number skips the pair.  A
+    target holds no pages before (``paged_free``), is in one pair only and no source.
+    """
+    requests, width, stride = _table_args(block_table, "paged fork", page_size)
+    device = block_table.device
+    ctx = _in_place(context_lens, "context_lens", device, requests)
+    held = None
+    if reserved_lens is not None:
+        held = _in_place(reserved_lens, "reserved_lens", device, requests)
+    src = _vector(sources, torch.int32, "sources", device)
+    n = src.shape[0]
+    dst = _vector(targets, torch.int32, "targets", device, n)
+    free = _vector(free_pages, torch.int32, "free_pages", device)
+    head = _vector(free_head, torch.int32, "free_head", device, 1)
+    ints = torch.empty(3 * n + 2, dtype=torch.int32, device=device)
+    head_out, missing, copy_from, copy_to, rows = ints.split_with_sizes((1, 1, n, n, n))
+    if n == 0:
+        head_out.copy_(head)
+        missing.zero_()
+        return Fork(copy_from, copy_to, rows, head_out, missing)
+    _on(device)(
+        "kb_paged_fork",
+        ctx.data_ptr(), None if held is None else held.data_ptr(), requests,
+        block_table.data_ptr(), stride, width, src.data_ptr(), dst.data_ptr(), n,
+        free.data_ptr(), free.shape[0], head.data_ptr(), page_size, copy_from.data_ptr(),
+        copy_to.data_ptr(), rows.data_ptr(), head_out.data_ptr(), missing.data_ptr(),
+        _raw_stream(device),
+    )
+    return Fork(copy_from, copy_to, rows, head_out, missing)
+
+
+def paged_free(
+    block_table: torch.Tensor,
+    reserved_lens: torch.Tensor,
+    keep_lens: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_head: torch.Tensor,
+    page_size: int,
+    num_pages: int,
+) -> torch.Tensor:
+    """Gives pages back that no request holds any more; returns the next ``free_head``.
+
+    Request b's pages reach ``reserved_lens[b]`` tokens (int32 [requests], of every row of the
+    table), of which it keeps the first ``keep_lens[b]`` (0: it is done).  A page that a row
+    gives up and no row keeps goes to the free list: in ascending order, in front of
+    ``free_head``, where pages that were handed out once stood (a list without that room keeps
+    the highest, and device error bit 2 is set).  The table is not changed; the caller's
+    ``reserved_lens`` become ``min(reserved_lens, keep_lens)``.  Pages have ids below
+    ``num_pages``.
+    """
+    requests, width, stride = _table_args(block_table, "paged free", page_size)
+    device = block_table.device
+    held = _vector(reserved_lens, torch.int32, "reserved_lens", device, requests)
+    keep = _vector(keep_lens, torch.int32, "keep_lens", device, requests)
+    free = _in_place(free_pages, "free_pages", device)
+    head = _vector(free_head, torch.int32, "free_head", device, 1)
+    if num_pages <= 0:
+        raise ValueError("num_pages must be positive")
+    out = torch.empty(1, dtype=torch.int32, device=device)
+    _on(device)(
+        "kb_paged_free",
+        held.data_ptr(), keep.data_ptr(), requests, block_table.data_ptr(), stride, width,
+        free.data_ptr(), free.shape[0], head.data_ptr(), page_size, num_pages, out.data_ptr(),
+        _raw_stream(device),
+    )
+    return out
+
+
+def paged_compact(
+    block_table: torch.Tensor,
+    reserved_lens: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_head: torch.Tensor,
+    page_size: int,
+    num_pages: int,
+) -> Compaction:
+    """Moves the pages in use to the lowest ids of the pool (those in use or free).
+
+    Used are the pages of the table within ``reserved_lens`` (int32 [requests], every row's),
+    free those of the list from ``free_head`` on.  The k-th used page above the lowest ids
+    moves to the k-th free one among them: ``paged_copy`` with the lists returned moves the
+    data, for every layer whose cache the table describes.  Nothing is changed in place.
+    """
+    requests, width, stride = _table_args(block_table, "paged compact", page_size)
+    device = block_table.device
+    held = _vector(reserved_lens, torch.int32, "reserved_lens", device, requests)
+    free = _vector(free_pages, torch.int32, "free_pages", device)
+    head = _vector(free_head, torch.int32, "free_head", device, 1)
+    if num_pages <= 0:
+        raise ValueError("num_pages must be positive")
+    half, places = num_pages // 2, free.shape[0]
+    table, listed, head_out, copy_from, copy_to, scratch = torch.empty(
+        requests * width + places + 1 + 2 * half + num_pages, dtype=torch.int32,
+        device=device).split_with_sizes((requests * width, places, 1, half, half, num_pages))
+    _on(device)(
+        "kb_paged_compact",
+        held.data_ptr(), requests, block_table.data_ptr(), stride, width, free.data_ptr(), places,
+        head.data_ptr(), page_size, num_pages, table.data_ptr(), listed.data_ptr(),
+        copy_from.data_ptr(), copy_to.data_ptr(), head_out.data_ptr(), scratch.data_ptr(),
+        _raw_stream(device),
+    )
+    return Compaction(table.view(requests, width), listed, head_out, copy_from, copy_to)
+
+
+def paged_copy(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    copy_from: torch.Tensor,
+    copy_to: torch.Tensor,
+    copy_rows: torch.Tensor | None = None,
+) -> None:
+    """Copies pages of the caches [pages, page_size, heads, width]: the first ``copy_rows[i]``
+    rows (default: all) of page ``copy_from[i]`` to page ``copy_to[i]`` (int32 [n]).
+
+    Pairs with a negative page are skipped.  No page may be copied to twice, or be copied from
+    and to.
+    """
+    dtype = k_cache.dtype
+    if dtype not in _HALF or v_cache.dtype != dtype:
+        raise TypeError("caches must both be BF16 or FP16")
+    _require_cuda(k_cache, "paged copy")
+    device = k_cache.device
+    if v_cache.device != device:
+        raise ValueError("paged copy inputs must share one device")
+    ks, vs = _cache_strides(k_cache, "k_cache"), _cache_strides(v_cache, "v_cache")
+    if k_cache.shape[:3] != v_cache.shape[:3]:
+        raise ValueError("the caches must have the same pages and heads")
+    pages, page_size, heads, dk = k_cache.shape
+    dv = v_cache.shape[3]
+    _check_widths(dk, dv)
+    src = _vector(copy_from, torch.int32, "copy_from", device)
+    n = src.shape[0]
+    dst = _vector(copy_to, torch.int32, "copy_to", device, n)
+    rows = None if copy_rows is None else _vector(copy_rows, torch.int32, "copy_rows", device, n)
+    if n == 0 or not pages or not page_size or not heads:
+        return
+    _on(device)(
+        "kb_paged_copy",
+        k_cache.data_ptr(), ks, v_cache.data_ptr(), vs, pages, page_size, heads, dk, dv,
+        src.data_ptr(), dst.data_ptr(), None if rows is None else rows.data_ptr(), n,
+        _raw_stream(device),
+    )
+
+
+# ---------------------------------------------------------------------------
+# penalties, biases and grammar masks
+# ---------------------------------------------------------------------------
+
+MAX_BIASES = 4096
+
+
+def _request_rows(t: torch.Tensor, dtype: torch.dtype, what: str, device: torch.device,
+                  requests: int) -> torch.Tensor:
+    """A matrix with a row for each request (or logits row) and unit stride along it."""
+    if t.dtype != dtype or t.ndim != 2:
+        raise TypeError(f"{what} must be a two-dimensional {dtype} tensor")
+    if t.shape[0] != requests:
+        raise ValueError(f"{what} must have {requests} rows")
+    if t.device != device:
+        raise ValueError(f"{what} must be on the device of the other tensors")
+    return t if t.stride(1) == 1 else t.contiguous()
+
+
+def adjust_logits(
+    logits: torch.Tensor,
+    *,
+    history: torch.Tensor | None = None,
+    history_lens: torch.Tensor | None = None,
+    prompt_lens: torch.Tensor | None = None,
+    repetition: torch.Tensor | None = None,
+    presence: torch.Tensor | None = None,
+    frequency: torch.Tensor | None = None,
+    bias_ids: torch.Tensor | None = None,
+    bias_values: torch.Tensor | None = None,
+    allowed: torch.Tensor | None = None,
+    cu_tokens: torch.Tensor | None = None,
+    tokens: torch.Tensor | None = None,
+    tree_mask: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Logits with each request's penalties, biases and grammar mask, for ``verify_drafts`` or a
+    sampler.
+
+    ``logits`` [rows, V] (bf16, f16 or f32).  Row b belongs to request b, or, with
+    ``cu_tokens`` (int32 [B + 1]), rows ``cu_tokens[b]:cu_tokens[b+1]`` do.  Request b's
+    tokens so far are the first ``history_lens[b]`` (int32) of ``history[b]`` (int64), the
+    first ``prompt_lens[b]`` of them (default: none) its prompt, the others its answer.  With
+    ``tokens`` (int64 [rows], the drafted tokens of ``verify_drafts``) a row's answer goes on
+    with the tokens whose bits its ``tree_mask`` word has (int64, as ``paged_plan`` gives
+    them), without masks with itself and those before it.  For each token, in this order and
+    in fp32:
+
+      in the prompt or the answer: divided by ``repetition[b]`` where positive, else multiplied
+      in the answer: minus ``frequency[b]`` times its count, and minus ``presence[b]``
+      plus the request's ``bias_values[b, i]`` wherever ``bias_ids[b, i]`` (int64) names it
+      -infinity where its bit (``t % 32`` of word ``t // 32``) is not set in the row of
+      ``allowed`` (int32 [rows, (V + 31) // 32])
+
+    Parameters are fp32 [B].  Negative tokens and ids are skipped.  A row whose mask allows
+    nothing is -infinity throughout; rows outside every request are passed on as they are.
+    ``out`` may be ``logits`` itself; then what does not change is neither read nor written.
+    """
+    if logits.ndim != 2 or logits.dtype not in _ELEMENT:
+        raise TypeError("logits must be a BF16, FP16 or FP32 [rows, vocabulary] matrix")
+    _require_cuda(logits, "logit adjustment")
+    device = logits.device
+    rows, vocab = logits.shape
+    if vocab == 0:
+        raise ValueError("logit adjustment requires a vocabulary")
+    cu = mask = tok = None
+    if cu_tokens is None:
+        if tokens is not None or tree_mask is not None:
+            raise ValueError("tokens and tree_mask go with cu_tokens")
+        requests = rows
+    else:
+        cu = _vector(cu_tokens, torch.int32, "cu_tokens", device)
+        requests = cu.shape[0] - 1
+        if requests < 0:
+            raise ValueError("cu_tokens must have one entry more than there are requests")
+        if tokens is not None:
+            tok = _vector(tokens, torch.long, "tokens", device, rows)
+        if tree_mask is not None:
+            if tokens is None:
+                raise ValueError("tree_mask goes with tokens")
+            mask = _vector(tree_mask, torch.long, "tree_mask", device, rows)
+    if history is None:
+        if history_lens is not None or prompt_lens is not None:
+            raise ValueError("history_lens and prompt_lens go with history")
+        hist, lens, longest, hist_stride = None, None, 0, 0
+    else:
+        if history_lens is None:
+            raise ValueError("history needs history_lens")
+        hist = _request_rows(history, torch.long, "history", device, requests)
+        lens = _vector(history_lens, torch.int32, "history_lens", device, requests)
+        longest, hist_stride = hist.shape[1], hist.stride(0)
+    prompts = None
+    if prompt_lens is not None:
+        prompts = _vector(prompt_lens, torch.int32, "prompt_lens", device, requests)
+    rep, pres, freq = (
+        None if p is None else _vector(p, torch.float32, what, device, requests)
+        for p, what in ((repetition, "repetition"), (presence, "presence"),
+                        (frequency, "frequency")))
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    ids, values, biases = None, None, 0
+    if bias_ids is not None:
+        ids = _request_rows(bias_ids, torch.long, "bias_ids", device, requests)
+        values = _request_rows(bias_values, torch.float32, "bias_values", device, requests)
+        biases = ids.shape[1]
+        if values.shape != ids.shape:
+            raise ValueError("bias_values must have the shape of bias_ids")
+        if biases > MAX_BIASES:
+            raise ValueError(f"a request has at most {MAX_BIASES} biases")
+    words = None
+    if allowed is not None:
+        words = _request_rows(allowed, torch.int32, "allowed", device, rows)
+        if words.shape[1] != (vocab + 31) // 32:
+            raise ValueError("allowed must have a bit for every token: (V + 31) // 32 words a row")
+    if out is None:
+        x, x_stride = _unit_rows(logits, vocab)
+        y = torch.empty(rows, vocab, dtype=logits.dtype, device=device)
+    else:
+        if out.dtype != logits.dtype or out.shape != logits.shape or out.device != device:
+            raise ValueError("out must have the type, shape and device of the logits")
+        if rows and (out.stride(1) != 1 or (rows > 1 and out.stride(0) < vocab)):
+            raise ValueError("out needs rows of unit stride that do not overlap")
+        y = out
+        x, x_stride = ((logits, max(logits.stride(0), vocab)) if out is logits
+                       else _unit_rows(logits, vocab))
+        if out is not logits and _overlap(x, y):
+            if x.data_ptr() != y.data_ptr() or x.stride() != y.stride():
+                raise ValueError("out must be the logits themselves or lie apart from them")
+    if rows == 0:
+        return y
+    _on(device)(
+        "kb_adjust_logits",
+        x.data_ptr(), x_stride, rows, vocab, _ELEMENT[x.dtype], y.data_ptr(),
+        max(y.stride(0), vocab), requests, None if hist is None else hist.data_ptr(), hist_stride,
+        longest, None if lens is None else lens.data_ptr(),
+        None if prompts is None else prompts.data_ptr(), None if rep is None else rep.data_ptr(),
+        None if pres is None else pres.data_ptr(), None if freq is None else freq.data_ptr(),
+        None if ids is None else ids.data_ptr(), 0 if ids is None else ids.stride(0),
+        None if values is None else values.data_ptr(), 0 if values is None else values.stride(0),
+        biases, None if words is None else words.data_ptr(),
+        0 if words is None else max(words.stride(0), words.shape[1]),
+        None if cu is None else cu.data_ptr(), None if tok is None else tok.data_ptr(),
+        None if mask is None else mask.data_ptr(), _raw_stream(device),
+    )
+    return y
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices of unit inner stride share memory (their spans meet)."""
+    def span(t: torch.Tensor) -> tuple[int, int]:
+        size = ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+        return t.data_ptr(), t.data_ptr() + size
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return bool(a.numel()) and a0 < b1 and b0 < a1

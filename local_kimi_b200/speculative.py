@@ -18,6 +18,10 @@ the cache, and keeps what the target model accepts.
   got = ops.verify_drafts(logits, tokens, plan.cu_tokens, most, u, noise, temps, parents=parents)
   cache.keep(plan, got)
 
+Requests may share a prompt: ``cache.fork(sources, targets)`` lets requests go on from
+another's context with its full pages, ``cache.release(keep_lens)`` gives pages back that no
+request holds any more, and ``cache.compact()`` moves those in use to the lowest places.
+
 Nothing here synchronizes the host; lengths, tables and the free list stay on
 the device and are updated in place, so a step captured in a CUDA graph moves on
 with every replay.
@@ -101,6 +105,40 @@ class PagedCache:
         page, row = source // self.page_size, source % self.page_size
         ops.paged_append(self.k[page, row], self.v[page, row], self.k, self.v, target.flatten())
         self.context += kept.sum(dim=1, dtype=torch.int32)
+
+    def fork(self, sources: torch.Tensor, targets: torch.Tensor) -> ops.Fork:
+        """Requests ``targets`` go on from the contexts of ``sources`` (int32 [pairs]).
+
+        They share the full pages; a page that the context ends inside is copied.  Targets hold
+        no pages (``release`` them first); a target for which the pool has no page stays empty
+        (``missing``).  A request that shares pages is not to be cut back into them.
+        """
+        got = ops.paged_fork(self.context, self.table, sources, targets, self.free, self.head,
+                             self.page_size, reserved_lens=self.reserved)
+        self.head.copy_(got.free_head)
+        ops.paged_copy(self.k, self.v, got.copy_from, got.copy_to, got.copy_rows)
+        return got
+
+    def release(self, keep_lens: torch.Tensor) -> None:
+        """Each request keeps its first ``keep_lens`` tokens (int32 [requests]; 0: it is done,
+        its context: pages that refused drafts left it go back).  Pages that no request holds
+        any more are free again."""
+        head = ops.paged_free(self.table, self.reserved, keep_lens, self.free, self.head,
+                              self.page_size, self.k.shape[0])
+        self.head.copy_(head)
+        keep = keep_lens.clamp_min(0)
+        torch.minimum(self.reserved, keep, out=self.reserved)
+        torch.minimum(self.context, keep, out=self.context)
+
+    def compact(self) -> ops.Compaction:
+        """Moves the pages in use to the lowest places of the pool."""
+        got = ops.paged_compact(self.table, self.reserved, self.free, self.head, self.page_size,
+                                self.k.shape[0])
+        ops.paged_copy(self.k, self.v, got.copy_from, got.copy_to)
+        self.table.copy_(got.block_table)
+        self.free.copy_(got.free_pages)
+        self.head.copy_(got.free_head)
+        return got
 
 
 def children_first_tree(width: int, depth: int) -> list[int]:
