@@ -29,7 +29,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 int make_map_4d(CUtensorMap* map, const void* base, int f16, const int64_t (&dims)[4],
-                const int64_t (&strides)[3], int rows, int box2) {
+                const int64_t (&strides)[3], int rows, int box2, int width) {
   auto enc = encode_fn();
   KB_REQUIRE(enc != nullptr, KB_ERR_DEVICE, "cuTensorMapEncodeTiled is unavailable");
   cuuint64_t d[4], s[3];
@@ -40,12 +40,12 @@ int make_map_4d(CUtensorMap* map, const void* base, int f16, const int64_t (&dim
                "attention: strides must be positive");
     s[i] = (cuuint64_t)(dims[i + 1] == 1 ? 16 : strides[i] * 2);
   }
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, (cuuint32_t)box2, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)width, (cuuint32_t)rows, (cuuint32_t)box2, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = enc(
       map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
       const_cast<void*>(base), d, s, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+      width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   KB_REQUIRE(r == CUDA_SUCCESS, KB_ERR_DEVICE, "attention: tensor map encoding failed (%d)",
              (int)r);

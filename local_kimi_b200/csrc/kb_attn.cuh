@@ -206,10 +206,10 @@ __device__ __forceinline__ void request_rows(const int* cu, int b, int64_t total
 int check_heads(int64_t Hq, int64_t Hkv, int64_t Dk, int64_t Dv, int dtype);
 
 // Tensor map over 16-bit elements [dims[3]][dims[2]][dims[1]][dims[0]], element
-// strides of the outer three, boxes of 64 x rows x box2 x 1 elements written in
-// the 128-byte swizzle; what lies outside the tensor reads as zero.
+// strides of the outer three, boxes of width x rows x box2 x 1 elements in the swizzle
+// of that width (64: 128 bytes, 32: 64 bytes); what lies outside the tensor reads as zero.
 int make_map_4d(CUtensorMap* map, const void* base, int f16, const int64_t (&dims)[4],
-                const int64_t (&strides)[3], int rows, int box2);
+                const int64_t (&strides)[3], int rows, int box2, int width = 64);
 
 // Dynamic shared-memory limit of a kernel, set once per device.
 int allow_smem(const void* kernel, int bytes, bool (&done)[64], std::mutex& mu);

@@ -5,27 +5,31 @@
 //   P_ij = (q_i . k_j) exp(b_i - b_j)
 //   o_i  = scale * (exp(b_i) q_i S + sum_j P_ij v_j)
 //   S'   = exp(b_C) S + sum_j k_j (exp(b_C - b_j) v_j)^T
-// Every exponent is at most 0.  The sums of logarithms are made in 64 bits; a decay that is 0
-// in fp32 (below e^-104, -infinity too) is a reset: what lies before it does not count.
+// Every exponent is at most 0.  Rows and keys in groups of 32: within one, exp(b_i - b_j) is
+// computed; across groups it is exp(b_e - b_j) exp(b_i - b_e), e the last row of j's group, so
+// that a row needs one exponential a group.  A decay that is 0 in fp32 (below e^-104, -infinity
+// too) is a reset: what lies before it does not count.
 //
 // One persistent CTA per SM; a unit is one head of one request (or of a segment of it), its
 // chunks one after the other.  Q, K and V tiles (128 rows, 64-element blocks in the 128-byte
 // swizzle) arrive by tensor copies in two stages.
 //
-//   warp 18: the units, the copies and the decays of each chunk.
-//   warp 16: issues S = Q K^T, O = Q S (the state), O += P V.
-//   warp 17: issues S^T += V'^T K, V' = the values with their decay to the chunk's end.
+//   warp 26: the copies, warp 27: the decays of each chunk (each walks the units).
+//   warp 24: issues S = Q K^T, O = Q S (the state), O += P V.
+//   warp 25: issues S^T += V'^T K, V' = the values with their decay to the chunk's end.
+//   warps 0-7: the state, in their registers in fp32 (a value column a thread, half of the key
+//     rows each); its bf16 copy is what Q S reads.
 //   warps 8-15: P from the scores, a row per thread and half the columns each; the part of the
-//     state scaled by exp(b_i) in tensor memory before P V is added to it; the outputs.
-//   warps 0-7: V' and the state.  The state lives in these warps' registers in fp32 (a value
-//     column a thread, half of the key rows each); its bf16 copy is what Q S reads.
+//     state scaled by exp(b_i) in tensor memory before P V is added to it; the outputs, which
+//     leave by tensor copies from the place of the chunk's values.
+//   warps 16-23: V', 32 rows at a time in two buffers, transposed on the way from shared to
+//     tensor memory (eight by eight pieces, ldmatrix and 16-lane stores).
 //
 // Roundings.  P and the copy of the state are rounded once to bf16 before they meet the values
 // and the queries: the outputs have 8 bits themselves.  The state must not lose bits: V' (fp32
 // products) enters the tensor cores as the sum of three bf16 values, 24 bits in all.
 //
-// 512 columns of tensor memory: scores and P 128, O 128, the state's gain 128, and two of the
-// three parts of V' (the third replaces the first once that is used).
+// 512 columns of tensor memory: scores and P 128, O 128, the state's gain 128, V' 2 x 48.
 //
 // A row past the request's end belongs to a neighbour: its keys and values are zeroed in shared
 // memory.  A value that is no number is zeroed too, since it would meet zero weights; the rows
@@ -38,22 +42,22 @@
 namespace kb {
 namespace linear {
 
-using attn::wait_phase;
-using attn::warp_wait;
 
 constexpr int CHUNK = 128;
 constexpr int BLOCK = CHUNK * 128;           // bytes of 128 rows x 64 elements
-constexpr int THREADS = 640;
-constexpr int STAGES = 2;
-constexpr int PREPARE_WARPS = 8;             // and as many of outputs
-constexpr int MMA_WARP = 16, GAIN_WARP = 17, COPY_WARP = 18;
+constexpr int THREADS = 896;
+constexpr int MOST_STAGES = 3;
+constexpr int STATE_WARPS = 8, OUT_WARPS = 8, VALUE_WARPS = 8;
+constexpr int VALUE_FIRST = STATE_WARPS + OUT_WARPS;
+constexpr int MMA_WARP = 24, GAIN_WARP = 25, COPY_WARP = 26, DECAY_WARP = 27;
 constexpr float RESET = -104.f;
-constexpr uint32_t S_AT = 0, O_AT = 128, GAIN_AT = 256, V1_AT = 384, V2_AT = 448;
+constexpr int GROUP = 32;                    // rows of V' that are made at a time
+constexpr uint32_t S_AT = 0, O_AT = 128, GAIN_AT = 256, PARTS_AT = 384, PARTS_STEP = 64;
 
 struct ChunkArgs {
   Args a;
   int segments, segment;                     // of a request at most; tokens of one
-  float* sums;                               // [B][segments][H][Dk][Dv]: a segment's gain
+  float* sums;                               // [B][segments][H][DKP][DVP]: a segment's gain
   float* keeps;                              // [B][segments][H]: its decay
 };
 
@@ -63,53 +67,83 @@ struct Item {
   int b, h, seg;
   int starts, ends;                          // the unit's first, last chunk; 2: the request's
   int odd;                                   // values that are no numbers
-  int resets;
   float keep;                                // exp(b_C)
 };
 
-template <int DKP, int DVP>
+template <int DKP, int DVP, bool STATES>
 struct ChunkShape {
   static constexpr int KC = DKP / 64, VC = DVP / 64;
-  static constexpr int STAGE = (2 * KC + VC) * BLOCK;
-  static constexpr int STATE = KC * DVP * 128;           // bytes of the bf16 copy
-  static constexpr int FIXED = 3072;
+  static constexpr int K_AT = STATES ? 0 : KC * BLOCK;   // of a stage: Q, K, V
+  static constexpr int V_AT = K_AT + KC * BLOCK;
+  static constexpr int STAGE = V_AT + VC * BLOCK;
+  static constexpr int STATE = STATES ? 0 : KC * DVP * 128;   // bytes of the bf16 copy
+  static constexpr int FIT = (227 * 1024 - 3072 - STATE) / STAGE;
+  static_assert(FIT >= 2, "stages");
+  static constexpr int STAGES = FIT < MOST_STAGES ? FIT : MOST_STAGES;
+  // (Three stages leave room for their arrays.)
+  static constexpr int FIXED = STAGES > 2 ? 4608 : 3072;
   static constexpr int SMEM = STAGES * STAGE + STATE + FIXED;
 };
 
+template <int N>                             // stages
 struct ChunkShared {
-  float at[STAGES][CHUNK];                   // b_i, base 2
-  float left[STAGES][CHUNK];                 // exp(b_C - b_j)
-  uint8_t since[STAGES][CHUNK];              // the last reset up to the row, plus 1; 0: none
-  uint8_t odd_from[2][CHUNK];                // of each value column, of a chunk's halves
-  Item item[STAGES];
-  uint64_t full[STAGES], info[STAGES], empty[STAGES];
-  uint64_t s_full, q_done, p_full, o_full, o_free, state_ready, clean, v_two, v_half, v_three,
-      gain_done, drain;
+  float at[N][CHUNK];                   // b_i, base 2
+  float left[N][CHUNK];                 // exp(b_e - b_j), e the last row of j's group
+  uint8_t since[N][CHUNK];              // the last reset up to the row, plus 1; 0: none
+  uint8_t odd_from[2][CHUNK];                // of each value column, of every other group
+  alignas(16) float on[N][CHUNK / GROUP];           // exp(b_C - b_e) of each group
+  Item item[N];
+  uint64_t full[N], info[N], empty[N], staged[N];
+  uint64_t v_full[2], v_free[2];             // of the groups of V'
+  uint64_t s_full, q_done, p_full, o_full, o_free, state_ready, clean, gain_done, gain_free, drain;
   uint32_t tmem;
   int abort_flag;
 };
-static_assert(sizeof(ChunkShared) <= 3072, "fixed shared memory");
+static_assert(sizeof(ChunkShared<2>) <= 3072 && sizeof(ChunkShared<3>) <= 4608, "shared memory");
 
-// Half of a transposition: lanes `step` apart keep one piece and swap the other.
-__device__ __forceinline__ void swap_pieces(uint4& a, uint4& b, int upper, int step) {
-  uint4 give = upper ? a : b;
-  give.x = __shfl_xor_sync(0xffffffffu, give.x, step);
-  give.y = __shfl_xor_sync(0xffffffffu, give.y, step);
-  give.z = __shfl_xor_sync(0xffffffffu, give.z, step);
-  give.w = __shfl_xor_sync(0xffffffffu, give.w, step);
-  if (upper) a = give; else b = give;
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, const void* from, int x, int y,
+                                           int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];"
+      ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(0),
+        "r"(smem_addr(from))
+      : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-                 "r"(v[6]), "r"(v[7])
+__device__ __forceinline__ void stored_from_shared() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+// 16 lanes of tensor memory x 8 columns from 8 x 8 pieces as ldmatrix transposes them: thread t
+// has row t / 4 (v[0], v[2]) and 8 + t / 4 (v[1], v[3]), column t % 4 of four and of the next.
+__device__ __forceinline__ void tmem_st_pieces(uint32_t taddr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
 }
 
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) {
   return __uint_as_float(w & 0xffff0000u);
+}
+
+// A bounded wait of a warp in step (kb_attn.cuh's in fewer instructions: two dozen places wait,
+// and all roles' code has to fit the instruction cache).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_f,
+                                          uint32_t* err) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const long long t0 = attn::now_ns();
+    do {
+      ok = attn::mbar_try_wait_for(bar, parity, 200000u);
+    } while (!ok && !*abort_f && attn::now_ns() - t0 <= attn::WAIT_NS);
+    if (!ok && !*abort_f) {
+      *abort_f = 1;
+      atomicOr(err, attn::ERR_WAIT);
+    }
+  }
+  return __all_sync(0xffffffffu, ok) != 0;
 }
 
 // The units of this CTA and their chunks, in order.
@@ -156,14 +190,15 @@ struct Items {
 template <int DKP, int DVP, bool STATES>
 __global__ void __launch_bounds__(THREADS, 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                 const __grid_constant__ CUtensorMap tv, const ChunkArgs C) {
-  using Sh = ChunkShape<DKP, DVP>;
-  constexpr int KC = Sh::KC, VC = Sh::VC;
+                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
+                 const ChunkArgs C) {
+  using Sh = ChunkShape<DKP, DVP, STATES>;
+  constexpr int KC = Sh::KC, VC = Sh::VC, STAGES = Sh::STAGES;
   constexpr int HALF = DKP / 2;              // key rows of a thread's part of the state
   const Args& A = C.a;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* copy_of_state = smem + STAGES * Sh::STAGE;
-  ChunkShared* B = reinterpret_cast<ChunkShared*>(copy_of_state + Sh::STATE);
+  auto* B = reinterpret_cast<ChunkShared<STAGES>*>(copy_of_state + Sh::STATE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_f = &B->abort_flag;
 
@@ -171,25 +206,30 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&B->full[i], 1);
       mbar_init(&B->info[i], 1);
-      mbar_init(&B->empty[i], STATES ? 1 + PREPARE_WARPS : 2 + 2 * PREPARE_WARPS);
+      mbar_init(&B->empty[i], STATES ? 1 + VALUE_WARPS + STATE_WARPS
+                                     : 3 + VALUE_WARPS + STATE_WARPS);
+      mbar_init(&B->staged[i], OUT_WARPS);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->v_full[i], VALUE_WARPS / 2);
+      mbar_init(&B->v_free[i], 1);
     }
     mbar_init(&B->s_full, 1);
     mbar_init(&B->q_done, 1);
-    mbar_init(&B->p_full, PREPARE_WARPS);
+    mbar_init(&B->p_full, OUT_WARPS);
     mbar_init(&B->o_full, 1);
-    mbar_init(&B->o_free, PREPARE_WARPS);
-    mbar_init(&B->state_ready, PREPARE_WARPS);
-    mbar_init(&B->clean, PREPARE_WARPS);
-    mbar_init(&B->v_two, PREPARE_WARPS);
-    mbar_init(&B->v_half, 1);
-    mbar_init(&B->v_three, PREPARE_WARPS);
+    mbar_init(&B->o_free, OUT_WARPS);
+    mbar_init(&B->state_ready, STATE_WARPS);
+    mbar_init(&B->clean, VALUE_WARPS);
     mbar_init(&B->gain_done, 1);
+    mbar_init(&B->gain_free, STATE_WARPS);
     mbar_init(&B->drain, STATES ? 1 : 2);
     B->abort_flag = 0;
     mbar_fence_init();
     if (!STATES) attn::prefetch_map(&tq);
     attn::prefetch_map(&tk);
     attn::prefetch_map(&tv);
+    if (!STATES) attn::prefetch_map(&to);
   }
   if (warp == COPY_WARP) tc::tmem_alloc_all(&B->tmem);
   tc::tc_fence_before();
@@ -210,26 +250,38 @@ __global__ void __launch_bounds__(THREADS, 1)
           make_uint4(0, 0, 0, 0);
   }
 
-  if (warp < PREPARE_WARPS) {
+  // Bounded waits of a warp in step; one arrival a warp.
+  bool ok = true;
+  auto need = [&](uint64_t* bar, uint32_t parity) {
+    ok = warp_wait(bar, parity, abort_f, A.err);
+    return ok;
+  };
+  auto arrive = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  int st = 0;
+  uint32_t ph = 0, one_phase = 0;            // of the stages; of the barriers met once a chunk
+  auto turn = [&]() {
+    one_phase ^= 1u;
+    if (++st == STAGES) {
+      st = 0;
+      ph ^= 1u;
+    }
+  };
+
+  if (warp < STATE_WARPS) {
     // ------------------------------------------------------------------ the state
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-    const int part = warp >> 2;              // key rows part * HALF .., chunk rows part * 64 ..
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int part = warp >> 2;              // key rows part * HALF ..
     const int dv = (warp & 3) * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t gain_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + GAIN_AT + part * HALF;
     const bool active = (warp & 3) * 32 < DVP;
+    const int rows = dv < A.Dv ? min(max(A.Dk - part * HALF, 0), HALF) : 0;   // that there are
     float s[HALF];
     float all = 1.f;                         // the unit's decay so far
-    int st = 0;
-    uint32_t ph = 0, one_phase = 0;          // of the stages; of the barriers met once a chunk
-    bool ok = true;
-    auto need = [&](uint64_t* bar, uint32_t parity) {
-      ok = warp_wait(bar, parity, abort_f, A.err);
-      return ok;
-    };
-    auto arrive = [&](uint64_t* bar) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
+    // Segments' gains lie [DKP][DVP], zero where the head is narrower.
+    const int64_t gain_mine = part * HALF * DVP + dv;
     // The bf16 copy, a value column's key rows side by side: what Q S reads.
     auto copy_state = [&]() {
       if (active) {
@@ -251,172 +303,94 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     while (true) {
       if (!need(&B->info[st], ph)) break;
-      const Item I = B->item[st];
-      if (I.n < 0) break;
-      if (I.starts) {
+      const int n = B->item[st].n, b = B->item[st].b, h = B->item[st].h, seg = B->item[st].seg;
+      const int starts = B->item[st].starts, ends = B->item[st].ends;
+      const float keep = B->item[st].keep;
+      if (n < 0) break;
+      arrive(&B->empty[st]);
+      if (starts) {
         // What the unit starts from: the request's state, and the gains of the segments before.
-        const float* from = STATES ? nullptr : request_state(A, I.b, I.h);
-        const bool mine = active && dv < A.Dv;
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) {
-          const int dk = part * HALF + i;
-          s[i] = from != nullptr && mine && dk < A.Dk ? __ldcg(from + (int64_t)dk * A.Dv + dv) : 0.f;
-        }
+        for (int i = 0; i < HALF; ++i) s[i] = 0.f;
         if (!STATES) {
-          for (int g = 0; g < I.seg; ++g) {
-            const int64_t u = ((int64_t)I.b * C.segments + g) * A.H + I.h;
-            const float keep = __ldcg(C.keeps + u);
-            const float* gain = C.sums + u * A.Dk * A.Dv;
+          const float* from = request_state(A, b, h);
+          if (from != nullptr && rows > 0) {
+            from += (int64_t)part * HALF * A.Dv + dv;
 #pragma unroll
-            for (int i = 0; i < HALF; ++i) {
-              const int dk = part * HALF + i;
-              const float x = mine && dk < A.Dk ? __ldcg(gain + (int64_t)dk * A.Dv + dv) : 0.f;
-              s[i] = fmaf(s[i], keep, x);
+            for (int c = 0; c < HALF; c += 8, from += 8 * A.Dv) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c < rows) s[c + i] = __ldcg(from + i * A.Dv);      // (rows: eights)
+              asm volatile("" : "+l"(from));
             }
+          }
+          for (int g = 0; g < seg; ++g) {
+            const int64_t u = ((int64_t)b * C.segments + g) * A.H + h;
+            const float all_of_it = __ldcg(C.keeps + u);
+            const float* gain = C.sums + u * (DKP * DVP) + gain_mine;
+            if (active)
+#pragma unroll
+              for (int c = 0; c < HALF; c += 16) {
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = __ldcg(gain + (c + i) * DVP);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[c + i] = fmaf(s[c + i], all_of_it, x[i]);
+              }
           }
           copy_state();
         }
-      }
-      if (!need(&B->full[st], ph)) break;
-      uint8_t* k_tile = smem + st * Sh::STAGE + KC * BLOCK;
-      uint8_t* v_tile = k_tile + KC * BLOCK;
-      if (I.n < CHUNK) {
-        // Rows of a neighbour: zero.  (Of the values, those that this warp reads.)
-        for (int x = threadIdx.x; x < (CHUNK - I.n) * 8 * KC; x += PREPARE_WARPS * 32) {
-          const int r = x >> 3, c = r / (CHUNK - I.n);
-          *reinterpret_cast<uint4*>(k_tile + c * BLOCK + (I.n + r - c * (CHUNK - I.n)) * 128 +
-                                    (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        if (active)
-          for (int j = max(I.n, part * 64) + (lane >> 2); j < part * 64 + 64; j += 8) {
-            const int piece = (((warp & 1) * 4 + (lane & 3)) ^ (j & 7)) << 4;
-            *reinterpret_cast<uint4*>(v_tile + ((warp & 3) >> 1) * BLOCK + j * 128 + piece) =
-                make_uint4(0, 0, 0, 0);
-          }
-        __syncwarp();
-      }
-      uint32_t last[32];                     // the third part of V', pairs of chunk rows
-      if (active) {
-        const uint8_t* column = v_tile + (dv >> 6) * BLOCK + (dv & 7) * 2;
-        const int piece = (dv & 63) >> 3;
-        const float* left = &B->left[st][part * 64];
-        float odd = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {        // 16 rows a round
-          uint32_t lo[8], mid[8];
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float4 d = *reinterpret_cast<const float4*>(left + c * 16 + i * 2);
-            float x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int j = part * 64 + c * 16 + i * 2 + u;
-              x[u] = bf16_bits_to_float(*reinterpret_cast<const uint16_t*>(
-                  column + j * 128 + ((piece ^ (j & 7)) << 4)));
-              odd = fmaf(x[u], 0.f, odd);
-            }
-            x[0] *= d.x;
-            x[1] *= d.y;
-            x[2] *= d.z;
-            x[3] *= d.w;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint32_t h = attn::pack2<false>(x[2 * u], x[2 * u + 1]);
-              const float r0 = x[2 * u] - low_half(h), r1 = x[2 * u + 1] - high_half(h);
-              const uint32_t m = attn::pack2<false>(r0, r1);
-              lo[i + u] = attn::pack2<false>(r0 - low_half(m), r1 - high_half(m));
-              mid[i + u] = m;
-              last[c * 8 + i + u] = h;
-            }
-          }
-          tmem_st8(lanes + V1_AT + part * 32 + c * 8, lo);
-          tmem_st8(lanes + V2_AT + part * 32 + c * 8, mid);
-        }
-        if (__any_sync(0xffffffffu, odd != 0.f)) {     // true of not-a-number
-          int from = 255;
-          for (int j = part * 64; j < part * 64 + 64; ++j) {
-            uint16_t* e = reinterpret_cast<uint16_t*>(v_tile + (dv >> 6) * BLOCK + (dv & 7) * 2 +
-                                                      j * 128 + ((piece ^ (j & 7)) << 4));
-            if (attn::odd_element<false>(*e)) {
-              from = min(from, j);
-              *e = 0;
-            }
-          }
-          B->odd_from[part][dv] = (uint8_t)from;
-          __syncwarp();
-          if (lane == 0) atomicOr(&B->item[st].odd, 1 << warp);
-        }
-        tc::tmem_st_wait();
-      }
-      attn::fence_proxy_async();
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (!STATES) mbar_arrive(&B->clean);
-        mbar_arrive(&B->v_two);
-      }
-      if (!need(&B->v_half, one_phase)) break;
-      tc::tc_fence_after();
-      if (active) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_st8(lanes + V1_AT + part * 32 + c * 8, last + c * 8);
-        tc::tmem_st_wait();
-      }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&B->v_three);
-        mbar_arrive(&B->empty[st]);
       }
       if (!need(&B->gain_done, one_phase)) break;
       tc::tc_fence_after();
       if (active)
 #pragma unroll
-        for (int c = 0; c < HALF / 32; ++c) {
-          float gain[32];
-          tc::tmem_ld32(lanes + GAIN_AT + part * HALF + c * 32, gain);
+        for (int c = 0; c < HALF; c += 16) {
+          uint32_t gain[16];
+          tc::tmem_ld16(gain_at + c, gain);
           tc::tmem_ld_wait();
           tc::hold_regs(gain);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[c * 32 + i] = fmaf(s[c * 32 + i], I.keep, gain[i]);
+          for (int i = 0; i < 16; ++i)
+            s[c + i] = fmaf(s[c + i], keep, __uint_as_float(gain[i]));
         }
       tc::tc_fence_before();
+      arrive(&B->gain_free);
       if (!STATES && !need(&B->q_done, one_phase)) break;
-      if (I.ends) {
-        const int64_t u = ((int64_t)I.b * C.segments + I.seg) * A.H + I.h;
-        float* to = STATES ? C.sums + u * A.Dk * A.Dv
-                           : I.ends == 2 ? request_state(A, I.b, I.h) : nullptr;
-        if (STATES && threadIdx.x == 0) C.keeps[u] = all * I.keep;
-        if (to != nullptr && active && dv < A.Dv)
+      if (ends) {
+        const int64_t u = ((int64_t)b * C.segments + seg) * A.H + h;
+        if (STATES) {
+          if (threadIdx.x == 0) C.keeps[u] = all * keep;
+          float* to = C.sums + u * (DKP * DVP) + gain_mine;
+          if (active)
 #pragma unroll
-          for (int i = 0; i < HALF; ++i) {
-            const int dk = part * HALF + i;
-            if (dk < A.Dk) to[(int64_t)dk * A.Dv + dv] = s[i];
+            for (int i = 0; i < HALF; ++i) to[i * DVP] = s[i];
+        } else if (ends == 2) {
+          float* to = request_state(A, b, h);
+          if (to != nullptr && rows > 0) {
+            to += (int64_t)part * HALF * A.Dv + dv;
+#pragma unroll
+            for (int c = 0; c < HALF; c += 8, to += 8 * A.Dv) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c < rows) to[i * A.Dv] = s[c + i];
+              asm volatile("" : "+l"(to));
+            }
           }
+        }
       } else if (!STATES) {
         copy_state();
       }
-      all = I.ends ? 1.f : all * I.keep;
-      one_phase ^= 1u;
-      if (++st == STAGES) {
-        st = 0;
-        ph ^= 1u;
-      }
+      all = ends ? 1.f : all * keep;
+      turn();
     }
-  } else if (warp < 2 * PREPARE_WARPS) {
+  } else if (warp < VALUE_FIRST) {
     // ---------------------------------------------------------------- the outputs
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int part = (warp >> 2) & 1;        // columns part * 64 .. of the scores
     const int q0 = (warp & 3) * 32, row = q0 + lane;
     const uint32_t lanes = tmem + ((uint32_t)q0 << 16);
     constexpr int COLS = DVP / 2;            // of the outputs a thread has
-    int st = 0;
-    uint32_t ph = 0, one_phase = 0;
-    bool ok = true;
-    auto need = [&](uint64_t* bar, uint32_t parity) {
-      ok = warp_wait(bar, parity, abort_f, A.err);
-      return ok;
-    };
     while (!STATES) {
       if (!need(&B->info[st], ph)) break;
       const Item I = B->item[st];
@@ -425,7 +399,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int since = B->since[st][row];
       if (!need(&B->s_full, one_phase)) break;
       tc::tc_fence_after();
-#pragma unroll
+      // (Loops that stay loops: all roles' code has to fit the instruction cache.)
+#pragma unroll 1
       for (int c = 0; c < 2; ++c) {
         const int j0 = part * 64 + c * 32;
         uint32_t p[16];
@@ -437,30 +412,33 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc::tmem_ld32(lanes + S_AT + j0, x);
           tc::tmem_ld_wait();
           tc::hold_regs(x);
-          const float* at = &B->at[st][j0];
-          const float2 here = make_float2(mine, mine), minus = make_float2(-1.f, -1.f);
+          if (j0 < q0) {
+            // All before the rows: the decay to the group's end, and on to the row.
+            const float on = since > j0 + GROUP ? 0.f : exp2_fast(mine - B->at[st][j0 + GROUP - 1]);
+            const float2 on2 = make_float2(on, on);
+            const float* left = &B->left[st][j0];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(at + i);
-            float2 e = ffma2(make_float2(b.x, b.y), minus, here);
-            float2 f = ffma2(make_float2(b.z, b.w), minus, here);
-            e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-            f = make_float2(exp2_fast(f.x), exp2_fast(f.y));
-            e = fmul2(make_float2(x[i], x[i + 1]), e);
-            f = fmul2(make_float2(x[i + 2], x[i + 3]), f);
-            x[i] = e.x;
-            x[i + 1] = e.y;
-            x[i + 2] = f.x;
-            x[i + 3] = f.y;
+            for (int i = 0; i < 32; i += 4) {
+              const float4 d = *reinterpret_cast<const float4*>(left + i);
+              const float2 a = fmul2(fmul2(make_float2(x[i], x[i + 1]), make_float2(d.x, d.y)), on2);
+              const float2 b =
+                  fmul2(fmul2(make_float2(x[i + 2], x[i + 3]), make_float2(d.z, d.w)), on2);
+              p[i / 2] = attn::pack2<false>(a.x, a.y);
+              p[i / 2 + 1] = attn::pack2<false>(b.x, b.y);
+            }
+          } else {
+            const float* at = &B->at[st][j0];
+            const float2 here = make_float2(mine, mine), minus = make_float2(-1.f, -1.f);
+            const int lo = since - 1 - j0;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float2 e = ffma2(*reinterpret_cast<const float2*>(at + i), minus, here);
+              e = fmul2(make_float2(x[i], x[i + 1]), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+              if (i > lane || i < lo) e.x = 0.f;
+              if (i + 1 > lane || i + 1 < lo) e.y = 0.f;
+              p[i / 2] = attn::pack2<false>(e.x, e.y);
+            }
           }
-          if (j0 == q0 || I.resets) {
-            const int lo = since - 1 - j0, hi = row - j0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i > hi || i < lo) x[i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = attn::pack2<false>(x[2 * i], x[2 * i + 1]);
         }
         // (In place of scores that this thread has read.)
         tc::tmem_st16(lanes + S_AT + part * 64 + c * 16, p);
@@ -468,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!need(&B->q_done, one_phase)) break;
       tc::tc_fence_after();
       const float gain = since ? 0.f : exp2_fast(mine);
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < COLS / 16; ++c) {
         uint32_t o[16];
         tc::tmem_ld16(lanes + O_AT + part * COLS + c * 16, o);
@@ -485,74 +463,155 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!need(&B->o_full, one_phase)) break;
       tc::tc_fence_after();
       const int odd = *const_cast<volatile int*>(&B->item[st].odd);
-      // Four lanes side by side exchange 16-byte pieces, so that a store covers 64 bytes of
-      // eight rows and not 16 of 32.
-      uint16_t* out[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = (row & ~3) + i;
-        out[i] = r < I.n ? static_cast<uint16_t*>(A.out) + ((I.first + r) * A.H + I.h) * A.Dv +
-                               part * COLS + (lane & 3) * 8
-                         : nullptr;
-      }
-#pragma unroll
+      // The warp's 32 rows and COLS columns go through the place of the values, which nobody
+      // reads any more; the rows at a request's end go out by themselves.
+      uint16_t* out = static_cast<uint16_t*>(A.out) +
+                      ((I.first + row) * A.H + I.h) * A.Dv + part * COLS;
+      uint8_t* tile = smem + st * Sh::STAGE + Sh::V_AT + (part * CHUNK + q0) * COLS * 2;
+      const bool whole = q0 + 32 <= I.n && odd == 0;
+#pragma unroll 1
       for (int c = 0; c < COLS / 32; ++c) {
-        const int d0 = part * COLS + c * 32;
         float o[32];
-        tc::tmem_ld32(lanes + O_AT + d0, o);
+        tc::tmem_ld32(lanes + O_AT + part * COLS + c * 32, o);
         tc::tmem_ld_wait();
         tc::hold_regs(o);
-        if (odd)
-          for (int half = 0; half < 2; ++half)
-            if ((odd >> (half * 4 + (d0 >> 5))) & 1)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (row >= B->odd_from[half][d0 + i]) o[i] = NAN;
-        uint4 w[4];
+        const float2 scale2 = make_float2(A.scale, A.scale);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          w[i].x = attn::pack2<false>(o[8 * i] * A.scale, o[8 * i + 1] * A.scale);
-          w[i].y = attn::pack2<false>(o[8 * i + 2] * A.scale, o[8 * i + 3] * A.scale);
-          w[i].z = attn::pack2<false>(o[8 * i + 4] * A.scale, o[8 * i + 5] * A.scale);
-          w[i].w = attn::pack2<false>(o[8 * i + 6] * A.scale, o[8 * i + 7] * A.scale);
-        }
-        swap_pieces(w[0], w[1], lane & 1, 1);
-        swap_pieces(w[2], w[3], lane & 1, 1);
-        swap_pieces(w[0], w[2], lane & 2, 2);
-        swap_pieces(w[1], w[3], lane & 2, 2);
+          uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (out[i] && d0 + (lane & 3) * 8 < A.Dv)
-            *reinterpret_cast<uint4*>(out[i] + c * 32) = w[i];
+          for (int k = 0; k < 4; ++k) {
+            const float2 x = fmul2(make_float2(o[8 * i + 2 * k], o[8 * i + 2 * k + 1]), scale2);
+            w[k] = attn::pack2<false>(x.x, x.y);
+          }
+          const uint4 piece = make_uint4(w[0], w[1], w[2], w[3]);
+          const int at = COLS == 64 ? (c * 4 + i) ^ (lane & 7) : i ^ ((lane >> 1) & 3);
+          if (whole)
+            *reinterpret_cast<uint4*>(tile + lane * COLS * 2 + at * 16) = piece;
+          else if (row < I.n && part * COLS + c * 32 + i * 8 < A.Dv)
+            *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = piece;
+        }
       }
+      if (odd && row < I.n)
+        for (int d = part * COLS; d < min(A.Dv, (part + 1) * COLS); ++d)
+          for (int buffer = 0; buffer < 2; ++buffer)
+            if (((odd >> (buffer * 4 + (d >> 5))) & 1) && row >= B->odd_from[buffer][d])
+              out[d - part * COLS] = 0x7fff;
       tc::tc_fence_before();
+      if (whole) attn::fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&B->o_free);
+        mbar_arrive(&B->staged[st]);
+      }
+      turn();
+    }
+  } else if (warp < MMA_WARP) {
+    // ------------------------------------------- the values with their decay, V'
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // A strip of 32 columns; the groups of rows of one of the two buffers.
+    const int strip = warp & 3, buffer = (warp >> 2) & 1;
+    const uint32_t to = tmem + ((uint32_t)(strip * 32) << 16) + PARTS_AT + buffer * PARTS_STEP;
+    const bool active = strip * 32 < DVP;
+    uint32_t free_phase = 1;
+    while (ok) {
+      if (!need(&B->info[st], ph)) break;
+      const int n = B->item[st].n;
+      if (n < 0) break;
+      if (!need(&B->full[st], ph)) break;
+      uint8_t* k_tile = smem + st * Sh::STAGE + Sh::K_AT;
+      uint8_t* v_tile = smem + st * Sh::STAGE + Sh::V_AT + (active ? (strip >> 1) * BLOCK : 0);
+      if (n < CHUNK) {
+        // Rows of a neighbour: zero.  (Of the values, those that this warp reads.)
+        for (int x = threadIdx.x - VALUE_FIRST * 32; x < (CHUNK - n) * 8 * KC;
+             x += VALUE_WARPS * 32) {
+          const int r = x >> 3, c = r / (CHUNK - n);
+          *reinterpret_cast<uint4*>(k_tile + c * BLOCK + (n + r - c * (CHUNK - n)) * 128 +
+                                    (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        if (active)
+          for (int j = n + (lane >> 2); j < CHUNK; j += 8)
+            if (((j / GROUP) & 1) == buffer)
+              *reinterpret_cast<uint4*>(v_tile + j * 128 +
+                                        ((((strip & 1) * 4 + (lane & 3)) ^ (j & 7)) << 4)) =
+                  make_uint4(0, 0, 0, 0);
+        __syncwarp();
+      }
+      float2 odd = make_float2(0.f, 0.f);
+#pragma unroll 1
+      for (int g = buffer; g < CHUNK / GROUP; g += 2) {
+        const float on = B->on[st][g];
+        const float2 on2 = make_float2(on, on);
+        if (!need(&B->v_free[buffer], free_phase)) break;
+        free_phase ^= 1u;
+        tc::tc_fence_after();
+        // Eight rows a piece: pairs of rows of column 8 c + lane / 4, rows 2 (lane % 4) and on.
+        const uint32_t from = smem_addr(v_tile) + (g * GROUP + (lane & 7)) * 128 +
+                              ((((strip & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
+        const float* left = &B->left[st][g * GROUP + (lane & 3) * 2];
+#pragma unroll 1
+        for (int r = 0; r < 4; r += 2) {
+          uint32_t part[3][2][4];            // low, middle, high; upper and lower 16 columns
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t w[4];
+            attn::ldmatrix_x4_trans(w, from + (r + u) * 8 * 128);
+            const float2 d =
+                fmul2(*reinterpret_cast<const float2*>(left + (r + u) * 8), on2);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float2 x = make_float2(low_half(w[c]), high_half(w[c]));
+              odd = ffma2(x, make_float2(0.f, 0.f), odd);
+              x = fmul2(x, d);
+              const float2 minus = make_float2(-1.f, -1.f);
+              const uint32_t hi = attn::pack2<false>(x.x, x.y);
+              x = ffma2(make_float2(low_half(hi), high_half(hi)), minus, x);
+              const uint32_t mid = attn::pack2<false>(x.x, x.y);
+              x = ffma2(make_float2(low_half(mid), high_half(mid)), minus, x);
+              part[0][c >> 1][u * 2 + (c & 1)] = attn::pack2<false>(x.x, x.y);
+              part[1][c >> 1][u * 2 + (c & 1)] = mid;
+              part[2][c >> 1][u * 2 + (c & 1)] = hi;
+            }
+          }
+          if (active)
+#pragma unroll
+            for (int t = 0; t < 3; ++t)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                tmem_st_pieces(to + ((uint32_t)(h * 16) << 16) + t * 16 + r * 4, part[t][h]);
+        }
+        tc::tmem_st_wait();
+        attn::fence_proxy_async();           // the zeroed keys
+        tc::tc_fence_before();
+        arrive(&B->v_full[buffer]);
+      }
+      if (!ok) break;
+      if (active && __any_sync(0xffffffffu, odd.x + odd.y != 0.f)) {   // true of not-a-number
+        const int dv = strip * 32 + lane, piece = (dv & 63) >> 3;
+        int first = 255;
+        for (int j = 0; j < n; ++j) {
+          if (((j / GROUP) & 1) != buffer) continue;
+          uint16_t* e = reinterpret_cast<uint16_t*>(v_tile + j * 128 + (dv & 7) * 2 +
+                                                    ((piece ^ (j & 7)) << 4));
+          if (attn::odd_element<false>(*e)) {
+            first = min(first, j);
+            *e = 0;
+          }
+        }
+        B->odd_from[buffer][dv] = (uint8_t)first;
+        __syncwarp();
+        if (lane == 0) atomicOr(&B->item[st].odd, 1 << (buffer * 4 + strip));
+        attn::fence_proxy_async();
+      }
+      __syncwarp();
+      if (lane == 0) {
+        if (!STATES) mbar_arrive(&B->clean);
         mbar_arrive(&B->empty[st]);
       }
-      one_phase ^= 1u;
-      if (++st == STAGES) {
-        st = 0;
-        ph ^= 1u;
-      }
+      turn();
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    int st = 0;
-    uint32_t ph = 0, one_phase = 0;
-    bool ok = true;
-    auto need = [&](uint64_t* bar, uint32_t parity) {
-      ok = warp_wait(bar, parity, abort_f, A.err);
-      return ok;
-    };
-    auto turn = [&]() {
-      one_phase ^= 1u;
-      if (++st == STAGES) {
-        st = 0;
-        ph ^= 1u;
-      }
-    };
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // A and B bf16, sums fp32, 128 rows.
     constexpr uint32_t COMMON = (1u << 4) | (1u << 7) | (1u << 10) | ((CHUNK >> 4) << 24);
     constexpr uint32_t MN = 1u << 16;        // B as it lies: rows along the products' axis
@@ -570,8 +629,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (B->item[st].n < 0) break;
         if (!need(&B->full[st], ph)) break;
         tc::tc_fence_after();
-        const uint32_t q_at = base + st * Sh::STAGE, k_at = q_at + KC * BLOCK;
-        const uint32_t v_at = k_at + KC * BLOCK;
+        const uint32_t q_at = base + st * Sh::STAGE, k_at = q_at + Sh::K_AT;
+        const uint32_t v_at = q_at + Sh::V_AT;
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
           const uint64_t a = tc::sw128_desc(q_at + c * BLOCK);
@@ -608,24 +667,28 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else if (warp == GAIN_WARP) {
       // --------------------------------------------------------- the state's gain
       constexpr uint32_t ID_V = COMMON | MN | ((DKP >> 3) << 17);
-      while (true) {
+      uint32_t full_phase = 0;
+      while (ok) {
         if (!need(&B->info[st], ph)) break;
         if (B->item[st].n < 0) break;
-        if (!need(&B->full[st], ph) || !need(&B->v_two, one_phase)) break;
-        tc::tc_fence_after();
-        const uint64_t b = tc::sw128_desc_mn(base + st * Sh::STAGE + KC * BLOCK, BLOCK);
-        auto product = [&](uint32_t from, uint32_t more) {
+        if (!need(&B->full[st], ph) || !need(&B->gain_free, one_phase ^ 1u)) break;
+        const uint64_t b = tc::sw128_desc_mn(base + st * Sh::STAGE + Sh::K_AT, BLOCK);
+#pragma unroll 1
+        for (int g = 0; g < CHUNK / GROUP; ++g) {
+          if (!need(&B->v_full[g & 1], full_phase)) break;
+          tc::tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < CHUNK / 16; ++k)
-            tc::umma_ts_one(one, tm + GAIN_AT, tm + from + k * 8, b + k * (2048 >> 4), ID_V,
-                            more | (uint32_t)(k > 0));
-        };
-        product(V1_AT, 0);
-        tc::umma_commit_one(one, &B->v_half);
-        product(V2_AT, 1);
-        if (!need(&B->v_three, one_phase)) break;
-        tc::tc_fence_after();
-        product(V1_AT, 1);
+          for (int t = 0; t < 3; ++t)
+#pragma unroll
+            for (int k = 0; k < GROUP / 16; ++k)
+              tc::umma_ts_one(one, tm + GAIN_AT,
+                              tm + PARTS_AT + (g & 1) * PARTS_STEP + t * 16 + k * 8,
+                              b + (g * (GROUP / 16) + k) * (2048 >> 4), ID_V,
+                              (uint32_t)(g + t + k > 0));
+          tc::umma_commit_one(one, &B->v_free[g & 1]);
+          full_phase ^= (uint32_t)(g & 1);
+        }
+        if (!ok) break;
         tc::umma_commit_one(one, &B->gain_done);
         tc::umma_commit_one(one, &B->empty[st]);
         turn();
@@ -633,106 +696,135 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc::umma_commit_one(one, &B->drain);
       attn::drain_phase(&B->drain, 0);
     } else if (warp == COPY_WARP) {
-      // --------------------------------------------------------- units and copies
+      // -------------------------------------------------------------------- copies
       const uint64_t keep_in_l2 = l2_evict_last_policy(), once = l2_evict_first_policy();
       const uint64_t k_policy = STATES || A.k_group > 1 ? keep_in_l2 : once;
       const uint64_t q_policy = A.q_group > 1 ? keep_in_l2 : once;
       const uint64_t v_policy = STATES ? keep_in_l2 : once;
-      Items items(C, STATES);
-      float g[4], ahead[4];
-      auto fetch = [&](float (&x)[4]) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = lane * 4 + u;
-          x[u] = j < items.next.n ? __ldg(A.decay + (items.next.first + j) * A.decay_tok +
-                                          items.next.h)
-                                  : 0.f;
+      // The outputs of a stage leave before its next loads.  Lanes 0 to 7: 32 rows and COLS
+      // columns each.
+      auto send = [&](int st, uint32_t parity) {
+        if (!need(&B->staged[st], parity)) return;
+        const Item I = B->item[st];
+        const int part = lane >> 2, q0 = (lane & 3) * 32;
+        if (lane < 8 && q0 + 32 <= I.n && I.odd == 0 && part * (DVP / 2) < A.Dv) {
+          store_tile(&to, smem + st * Sh::STAGE + Sh::V_AT + (part * CHUNK + q0) * DVP,
+                     part * (DVP / 2), I.h, (int)I.first + q0);
+          stored_from_shared();
         }
+        arrive(&B->empty[st]);
       };
-      fetch(ahead);
+      Items items(C, STATES);
       int sent = 0;
-      while (true) {
-        Item I = items.next;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) g[u] = ahead[u];
-        if (!need(&B->empty[st], ph ^ 1u)) break;
-        if (I.n < 0) {
-          if (lane == 0) {
-            B->item[st].n = -1;
-            mbar_arrive(&B->info[st]);
-          }
-          break;
-        }
+      for (; items.next.n >= 0; ++sent) {
+        const int token = (int)items.next.first, h = items.next.h;
+        if (!STATES && sent >= STAGES) send(st, ph ^ 1u);
+        if (!ok || !need(&B->empty[st], ph ^ 1u)) break;
         if (lane == 0) {
           uint8_t* to = smem + st * Sh::STAGE;
-          const int token = (int)I.first;
           mbar_arrive_expect_tx(&B->full[st],
                                 (uint32_t)((STATES ? KC + VC : 2 * KC + VC) * BLOCK));
           for (int c = 0; c < KC; ++c) {
-            if (!STATES)
-              attn::tma_load_4d(to + c * BLOCK, &tq, c * 64, I.h / A.q_group, token, 0,
-                                &B->full[st], q_policy);
-            attn::tma_load_4d(to + (KC + c) * BLOCK, &tk, c * 64, I.h / A.k_group, token, 0,
+            attn::tma_load_4d(to + Sh::K_AT + c * BLOCK, &tk, c * 64, h / A.k_group, token, 0,
                               &B->full[st], k_policy);
+            if (!STATES)
+              attn::tma_load_4d(to + c * BLOCK, &tq, c * 64, h / A.q_group, token, 0,
+                                &B->full[st], q_policy);
           }
           for (int c = 0; c < VC; ++c)
-            attn::tma_load_4d(to + (2 * KC + c) * BLOCK, &tv, c * 64, I.h, token, 0,
+            attn::tma_load_4d(to + Sh::V_AT + c * BLOCK, &tv, c * 64, h, token, 0,
                               &B->full[st], v_policy);
         }
         __syncwarp();
-        ++sent;
         items.advance();
-        fetch(ahead);
-        // The chunk's decays: sums in 64 bits, and the last reset up to each row.
-        double sum[4];
-        int since[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float x = decay_of(g[u]);
-          const bool reset = x <= RESET;
-          sum[u] = (u ? sum[u - 1] : 0.0) + (reset ? 0.0 : (double)x);
-          since[u] = reset ? lane * 4 + u + 1 : u ? since[u - 1] : 0;
-        }
-        double run = sum[3];
-        int last = since[3];
-        for (int o = 1; o < 32; o <<= 1) {
-          const double r = __shfl_up_sync(0xffffffffu, run, o);
-          const int l = __shfl_up_sync(0xffffffffu, last, o);
-          if (lane >= o) {
-            run += r;
-            last = max(last, l);
-          }
-        }
-        const double all = __shfl_sync(0xffffffffu, run, 31);
-        const int resets = __shfl_sync(0xffffffffu, last, 31);
-        double before = __shfl_up_sync(0xffffffffu, run, 1);
-        int earlier = __shfl_up_sync(0xffffffffu, last, 1);
-        if (lane == 0) {
-          before = 0.0;
-          earlier = 0;
-        }
-        constexpr double TO_2 = 1.4426950408889634;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = lane * 4 + u;
-          const double b = before + sum[u];
-          B->at[st][j] = (float)(b * TO_2);
-          B->left[st][j] =
-              j < I.n && j + 1 >= resets ? exp2f((float)((all - b) * TO_2)) : 0.f;
-          B->since[st][j] = (uint8_t)max(since[u], earlier);
-        }
-        I.odd = 0;
-        I.resets = resets;
-        I.keep = resets ? 0.f : exp2f((float)(all * TO_2));
-        if (lane == 0) B->item[st] = I;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->info[st]);
         turn();
       }
+      // (`st` is the oldest stage, if all are in use.)
+      if (!STATES && ok)
+        for (int i = max(0, STAGES - sent); i < STAGES && ok; ++i) {
+          const int at = (st + i) % STAGES;
+          send(at, (uint32_t)((sent - STAGES + i) / STAGES) & 1u);
+        }
       // On the error path, copies in flight land before the CTA may exit.
       if (*abort_f)
         for (int i = 0; i < STAGES; ++i)
           for (uint32_t parity = 0; parity < 2; ++parity) attn::drain_phase(&B->full[i], parity);
+    } else if (warp == DECAY_WARP) {
+      // ------------------------------------------------------- the decays of a chunk
+      // A row a lane, four groups side by side.  The sums behind a row (to its group's end, then
+      // group by group) are those that V' and the state need: where they matter they are small,
+      // and exact to 2^-24 of themselves.  The sums up to a row, for P, whose weights have 8
+      // bits, are the group's less those behind.
+      constexpr int GROUPS = CHUNK / GROUP;
+      Items items(C, STATES);
+      float ahead[GROUPS];
+      auto fetch = [&]() {
+        const float* from = A.decay + items.next.first * A.decay_tok + items.next.h;
+#pragma unroll
+        for (int p = 0; p < GROUPS; ++p)     // (always a row of the chunk: nothing waits here)
+          ahead[p] = __ldg(from + min(p * GROUP + lane, items.next.n - 1) * A.decay_tok);
+      };
+      if (items.next.n > 0) fetch();
+      while (true) {
+        Item I = items.next;
+        float up[GROUPS], behind[GROUPS];
+        unsigned marks[GROUPS];
+#pragma unroll
+        for (int p = 0; p < GROUPS; ++p) {
+          const float x = p * GROUP + lane < I.n ? decay_of(ahead[p]) : 0.f;
+          marks[p] = __ballot_sync(0xffffffffu, x <= RESET);
+          up[p] = x <= RESET ? 0.f : x * LOG2E;
+          behind[p] = __shfl_down_sync(0xffffffffu, up[p], 1);
+          if (lane == 31) behind[p] = 0.f;
+        }
+        if (I.n >= 0) {
+          items.advance();
+          if (items.next.n > 0) fetch();
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+          for (int p = 0; p < GROUPS; ++p) {
+            const float z = __shfl_down_sync(0xffffffffu, behind[p], o);
+            if (lane + o < 32) behind[p] += z;
+          }
+        float whole[GROUPS], on[GROUPS], before = 0.f, after = 0.f;
+        int since[GROUPS], last = 0, later = 0;
+#pragma unroll
+        for (int p = 0; p < GROUPS; ++p) {
+          whole[p] = __shfl_sync(0xffffffffu, up[p] + behind[p], 0);
+          before += whole[p];
+          up[p] = before - behind[p];
+          const unsigned seen = marks[p] & (0xffffffffu >> (31 - lane));
+          since[p] = seen ? p * GROUP + 32 - __clz(seen) : last;
+          if (marks[p]) last = p * GROUP + 32 - __clz(marks[p]);
+        }
+#pragma unroll
+        for (int p = GROUPS - 1; p >= 0; --p) {
+          on[p] = later ? 0.f : exp2_fast(after);
+          after += whole[p];
+          later |= marks[p] != 0;
+          // A reset behind the row, in its group.
+          const unsigned rest = lane < 31 ? marks[p] >> (lane + 1) : 0u;
+          behind[p] = p * GROUP + lane >= I.n || rest ? 0.f : exp2_fast(behind[p]);
+        }
+        I.odd = 0;
+        I.keep = later ? 0.f : exp2_fast(after);
+        if (!need(&B->empty[st], ph ^ 1u)) break;
+#pragma unroll
+        for (int p = 0; p < GROUPS; ++p) {
+          B->at[st][p * GROUP + lane] = up[p];
+          B->left[st][p * GROUP + lane] = behind[p];
+          B->since[st][p * GROUP + lane] = (uint8_t)since[p];
+        }
+        if (lane == 0)
+          *reinterpret_cast<float4*>(B->on[st]) = make_float4(on[0], on[1], on[2], on[3]);
+        if (lane == 0) B->item[st] = I;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->info[st]);
+        if (I.n < 0) break;
+        turn();
+      }
     }
     __syncwarp();
   }
@@ -749,31 +841,46 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 template <int DKP, int DVP, bool STATES>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                        const ChunkArgs& C, int grid, void* stream) {
-  using Sh = ChunkShape<DKP, DVP>;
+                        const CUtensorMap& mo, const ChunkArgs& C, int grid, void* stream) {
+  using Sh = ChunkShape<DKP, DVP, STATES>;
+  static_assert(Sh::SMEM <= 227 * 1024, "shared memory");
   static std::mutex mu;
   static bool done[64] = {};
   const void* fn = reinterpret_cast<const void*>(&chunk_kernel<DKP, DVP, STATES>);
   const int st = attn::allow_smem(fn, Sh::SMEM, done, mu);
   if (st != KB_OK) return st;
   return launch(chunk_kernel<DKP, DVP, STATES>, dim3((unsigned)grid), dim3(THREADS),
-                (size_t)Sh::SMEM, stream, mq, mk, mv, C);
+                (size_t)Sh::SMEM, stream, mq, mk, mv, mo, C);
 }
 
-// Segments of a request: where there are fewer heads of requests than SMs, about two units an
-// SM, of 4 chunks at least (a segment but the last is read twice, for its gain and its outputs).
+static int64_t padded(int64_t width) { return width <= 64 ? 64 : 128; }
+
+// Segments of a request: as many as make the longest way of a CTA shortest, in chunks.  A unit
+// costs START beside its chunks, each segment's gain that it starts from GAIN; a segment but
+// the last is read twice, for its gain (half a chunk's cost) and its outputs.
 static void segments_of(int64_t heads, int64_t longest, int sms, int& segments, int& segment) {
-  const int64_t want = heads < sms ? (2 * sms + heads - 1) / heads : 1;
-  int64_t each = ((longest + want - 1) / want + CHUNK - 1) / CHUNK * CHUNK;
-  if (each < 4 * CHUNK) each = 4 * CHUNK;
-  segments = (int)((longest + each - 1) / each);
-  segment = (int)each;
+  constexpr double START = 2.0, GAIN = 0.4;
+  const int64_t chunks = (longest + CHUNK - 1) / CHUNK;
+  double best = 0.0;
+  segments = 1;
+  segment = (int)(chunks * CHUNK);
+  for (int64_t n = 1; n <= chunks && n <= 64 && (n == 1 || heads * n <= 2 * sms); ++n) {
+    const int64_t each = (chunks + n - 1) / n, parts = (chunks + each - 1) / each;
+    const int64_t turns = (heads * parts + sms - 1) / sms;
+    double cost = turns * (each + START) + GAIN * (parts - 1);
+    if (parts > 1) cost += ((heads * (parts - 1) + sms - 1) / sms) * (0.5 * each + START);
+    if (n > 1 && cost >= best) continue;
+    best = cost;
+    segments = (int)parts;
+    segment = (int)(each * CHUNK);
+  }
 }
 
 size_t chunk_workspace(int64_t B, int64_t H, int64_t Dk, int64_t Dv, int64_t longest, int sms) {
   int segments, segment;
   segments_of(B * H, longest, sms, segments, segment);
-  return segments > 1 ? (size_t)(B * segments * H) * (Dk * Dv + 1) * sizeof(float) : 0;
+  return segments > 1 ? (size_t)(B * segments * H) * (padded(Dk) * padded(Dv) + 1) * sizeof(float)
+                      : 0;
 }
 
 int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspace,
@@ -785,8 +892,8 @@ int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspac
   KB_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), KB_ERR_WORKSPACE,
              "linear attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   C.sums = static_cast<float*>(workspace);
-  C.keeps = C.sums + (size_t)A.B * C.segments * A.H * A.Dk * A.Dv;
-  CUtensorMap mq, mk, mv;
+  C.keeps = C.sums + (size_t)A.B * C.segments * A.H * padded(A.Dk) * padded(A.Dv);
+  CUtensorMap mq, mk, mv, mo;
   int st = attn::make_map_4d(&mq, A.q, 0, {A.Dk, Hq, A.total, 1}, {A.q_head, A.q_tok, 8}, 1,
                              CHUNK);
   if (st == KB_OK)
@@ -794,22 +901,26 @@ int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspac
   if (st == KB_OK)
     st = attn::make_map_4d(&mv, A.v, 0, {A.Dv, A.H, A.total, 1}, {A.v_head, A.v_tok, 8}, 1,
                            CHUNK);
+  // The outputs in boxes of 32 rows and the columns of a warp.
+  if (st == KB_OK)
+    st = attn::make_map_4d(&mo, A.out, 0, {A.Dv, A.H, A.total, 1},
+                           {A.Dv, (int64_t)A.H * A.Dv, 8}, 1, 32, A.Dv <= 64 ? 32 : 64);
   if (st != KB_OK) return st;
   const int grid = (int)std::min<int64_t>((int64_t)A.B * C.segments * A.H, sms);
   for (int pass = C.segments > 1 ? 0 : 1; pass < 2 && st == KB_OK; ++pass) {
     const bool states = pass == 0;
     if (A.Dk <= 64 && A.Dv <= 64)
-      st = states ? launch_chunk<64, 64, true>(mq, mk, mv, C, grid, stream)
-                  : launch_chunk<64, 64, false>(mq, mk, mv, C, grid, stream);
+      st = states ? launch_chunk<64, 64, true>(mq, mk, mv, mo, C, grid, stream)
+                  : launch_chunk<64, 64, false>(mq, mk, mv, mo, C, grid, stream);
     else if (A.Dk <= 64)
-      st = states ? launch_chunk<64, 128, true>(mq, mk, mv, C, grid, stream)
-                  : launch_chunk<64, 128, false>(mq, mk, mv, C, grid, stream);
+      st = states ? launch_chunk<64, 128, true>(mq, mk, mv, mo, C, grid, stream)
+                  : launch_chunk<64, 128, false>(mq, mk, mv, mo, C, grid, stream);
     else if (A.Dv <= 64)
-      st = states ? launch_chunk<128, 64, true>(mq, mk, mv, C, grid, stream)
-                  : launch_chunk<128, 64, false>(mq, mk, mv, C, grid, stream);
+      st = states ? launch_chunk<128, 64, true>(mq, mk, mv, mo, C, grid, stream)
+                  : launch_chunk<128, 64, false>(mq, mk, mv, mo, C, grid, stream);
     else
-      st = states ? launch_chunk<128, 128, true>(mq, mk, mv, C, grid, stream)
-                  : launch_chunk<128, 128, false>(mq, mk, mv, C, grid, stream);
+      st = states ? launch_chunk<128, 128, true>(mq, mk, mv, mo, C, grid, stream)
+                  : launch_chunk<128, 128, false>(mq, mk, mv, mo, C, grid, stream);
   }
   return st;
 }
