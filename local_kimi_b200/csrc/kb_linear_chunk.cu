@@ -52,7 +52,7 @@ constexpr int VALUE_FIRST = STATE_WARPS + OUT_WARPS;
 constexpr int MMA_WARP = 24, GAIN_WARP = 25, COPY_WARP = 26, DECAY_WARP = 27;
 constexpr float RESET = -104.f;
 constexpr int GROUP = 32;                    // rows of V' that are made at a time
-constexpr uint32_t S_AT = 0, O_AT = 128, GAIN_AT = 256, PARTS_AT = 384, PARTS_STEP = 64;
+constexpr uint32_t S_AT = 0, O_AT = 128, GAIN_AT = 256, PARTS_STEP = 64;
 
 struct ChunkArgs {
   Args a;
@@ -77,6 +77,9 @@ struct ChunkShape {
   static constexpr int V_AT = K_AT + KC * BLOCK;
   static constexpr int STAGE = V_AT + VC * BLOCK;
   static constexpr int STATE = STATES ? 0 : KC * DVP * 128;   // bytes of the bf16 copy
+  // Groups of V' at a time: without scores and outputs their warps and columns serve it too.
+  static constexpr int BUFFERS = STATES ? 4 : 2;
+  static constexpr uint32_t PARTS_AT = STATES ? 0 : 384;
   static constexpr int FIT = (227 * 1024 - 3072 - STATE) / STAGE;
   static_assert(FIT >= 2, "stages");
   static constexpr int STAGES = FIT < MOST_STAGES ? FIT : MOST_STAGES;
@@ -94,7 +97,7 @@ struct ChunkShared {
   alignas(16) float on[N][CHUNK / GROUP];           // exp(b_C - b_e) of each group
   Item item[N];
   uint64_t full[N], info[N], empty[N], staged[N];
-  uint64_t v_full[2], v_free[2];             // of the groups of V'
+  uint64_t v_full[4], v_free[4];             // of the groups of V'
   uint64_t s_full, q_done, p_full, o_full, o_free, state_ready, clean, gain_done, gain_free, drain;
   uint32_t tmem;
   int abort_flag;
@@ -115,11 +118,25 @@ __device__ __forceinline__ void stored_from_shared() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
-// 16 lanes of tensor memory x 8 columns from 8 x 8 pieces as ldmatrix transposes them: thread t
-// has row t / 4 (v[0], v[2]) and 8 + t / 4 (v[1], v[3]), column t % 4 of four and of the next.
-__device__ __forceinline__ void tmem_st_pieces(uint32_t taddr, const uint32_t (&v)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};"
-               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 16 lanes of tensor memory x 4 columns from 8 x 8 pieces as ldmatrix transposes them: thread t
+// has column t % 4 of row t / 4 (v0) and of row 8 + t / 4 (v1).
+__device__ __forceinline__ void tmem_st_pieces(uint32_t taddr, uint32_t v0, uint32_t v1) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x1.b32 [%0], {%1,%2};"
+               ::"r"(taddr), "r"(v0), "r"(v1)
+               : "memory");
+}
+
+// (Beside a store to global memory, plain code makes one store of both whose space is unknown.)
+__device__ __forceinline__ void store_shared(uint32_t to, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
+               ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
 
@@ -206,12 +223,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&B->full[i], 1);
       mbar_init(&B->info[i], 1);
-      mbar_init(&B->empty[i], STATES ? 1 + VALUE_WARPS + STATE_WARPS
+      mbar_init(&B->empty[i], STATES ? 1 + 4 * Sh::BUFFERS + STATE_WARPS
                                      : 3 + VALUE_WARPS + STATE_WARPS);
       mbar_init(&B->staged[i], OUT_WARPS);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&B->v_full[i], VALUE_WARPS / 2);
+    for (int i = 0; i < Sh::BUFFERS; ++i) {
+      mbar_init(&B->v_full[i], 4);
       mbar_init(&B->v_free[i], 1);
     }
     mbar_init(&B->s_full, 1);
@@ -338,9 +355,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int i = 0; i < 16; ++i) s[c + i] = fmaf(s[c + i], all_of_it, x[i]);
               }
           }
-          copy_state();
         }
       }
+      if (!STATES) copy_state();
       if (!need(&B->gain_done, one_phase)) break;
       tc::tc_fence_after();
       if (active)
@@ -378,20 +395,18 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
         }
-      } else if (!STATES) {
-        copy_state();
       }
       all = ends ? 1.f : all * keep;
       turn();
     }
-  } else if (warp < VALUE_FIRST) {
+  } else if (!STATES && warp < VALUE_FIRST) {
     // ---------------------------------------------------------------- the outputs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int part = (warp >> 2) & 1;        // columns part * 64 .. of the scores
     const int q0 = (warp & 3) * 32, row = q0 + lane;
     const uint32_t lanes = tmem + ((uint32_t)q0 << 16);
     constexpr int COLS = DVP / 2;            // of the outputs a thread has
-    while (!STATES) {
+    while (true) {
       if (!need(&B->info[st], ph)) break;
       const Item I = B->item[st];
       if (I.n < 0) break;
@@ -399,49 +414,62 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int since = B->since[st][row];
       if (!need(&B->s_full, one_phase)) break;
       tc::tc_fence_after();
-      // (Loops that stay loops: all roles' code has to fit the instruction cache.)
+      // (Loops that stay loops, here and below: each scheduler runs warps of every role, whose
+      // code does not fit its instruction cache together.)
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        const int j0 = part * 64 + c * 32;
-        uint32_t p[16];
-        if (j0 > q0) {                       // all behind the rows
+      for (int c = 0; c < 4; ++c) {
+        const int j0 = part * 64 + c * 16;   // columns of the scores
+        uint32_t p[8];
+        if (j0 >= q0 + GROUP) {              // all behind the rows
 #pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = 0;
+          for (int i = 0; i < 8; ++i) p[i] = 0;
         } else {
-          float x[32];
-          tc::tmem_ld32(lanes + S_AT + j0, x);
+          uint32_t x[16];
+          tc::tmem_ld16(lanes + S_AT + j0, x);
           tc::tmem_ld_wait();
           tc::hold_regs(x);
+          auto scores = [&](int i) {
+            return make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          };
           if (j0 < q0) {
             // All before the rows: the decay to the group's end, and on to the row.
-            const float on = since > j0 + GROUP ? 0.f : exp2_fast(mine - B->at[st][j0 + GROUP - 1]);
+            const int last = j0 | (GROUP - 1);
+            const float on = since > last + 1 ? 0.f : exp2_fast(mine - B->at[st][last]);
             const float2 on2 = make_float2(on, on);
             const float* left = &B->left[st][j0];
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
+            for (int i = 0; i < 16; i += 4) {
               const float4 d = *reinterpret_cast<const float4*>(left + i);
-              const float2 a = fmul2(fmul2(make_float2(x[i], x[i + 1]), make_float2(d.x, d.y)), on2);
-              const float2 b =
-                  fmul2(fmul2(make_float2(x[i + 2], x[i + 3]), make_float2(d.z, d.w)), on2);
+              const float2 a = fmul2(fmul2(scores(i), make_float2(d.x, d.y)), on2);
+              const float2 b = fmul2(fmul2(scores(i + 2), make_float2(d.z, d.w)), on2);
               p[i / 2] = attn::pack2<false>(a.x, a.y);
               p[i / 2 + 1] = attn::pack2<false>(b.x, b.y);
             }
           } else {
-            const float* at = &B->at[st][j0];
             const float2 here = make_float2(mine, mine), minus = make_float2(-1.f, -1.f);
-            const int lo = since - 1 - j0;
+            const float* at = &B->at[st][j0];
+            // Columns up to the row, and from its last reset on.
+            uint32_t seen = 0xffffffffu >> (31 - lane);
+            if (since > q0 + 1) seen &= 0xffffffffu << (since - 1 - q0);
+            seen >>= j0 - q0;
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 e = ffma2(*reinterpret_cast<const float2*>(at + i), minus, here);
-              e = fmul2(make_float2(x[i], x[i + 1]), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
-              if (i > lane || i < lo) e.x = 0.f;
-              if (i + 1 > lane || i + 1 < lo) e.y = 0.f;
+            for (int i = 0; i < 16; i += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(at + i);
+              float2 e = ffma2(make_float2(b.x, b.y), minus, here);
+              float2 f = ffma2(make_float2(b.z, b.w), minus, here);
+              e = fmul2(scores(i), make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+              f = fmul2(scores(i + 2), make_float2(exp2_fast(f.x), exp2_fast(f.y)));
+              if (!((seen >> i) & 1)) e.x = 0.f;
+              if (!((seen >> (i + 1)) & 1)) e.y = 0.f;
+              if (!((seen >> (i + 2)) & 1)) f.x = 0.f;
+              if (!((seen >> (i + 3)) & 1)) f.y = 0.f;
               p[i / 2] = attn::pack2<false>(e.x, e.y);
+              p[i / 2 + 1] = attn::pack2<false>(f.x, f.y);
             }
           }
         }
         // (In place of scores that this thread has read.)
-        tc::tmem_st16(lanes + S_AT + part * 64 + c * 16, p);
+        tmem_st8(lanes + S_AT + part * 64 + c * 8, p);
       }
       if (!need(&B->q_done, one_phase)) break;
       tc::tc_fence_after();
@@ -469,27 +497,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                       ((I.first + row) * A.H + I.h) * A.Dv + part * COLS;
       uint8_t* tile = smem + st * Sh::STAGE + Sh::V_AT + (part * CHUNK + q0) * COLS * 2;
       const bool whole = q0 + 32 <= I.n && odd == 0;
+      const float2 scale2 = make_float2(A.scale, A.scale);
 #pragma unroll 1
-      for (int c = 0; c < COLS / 32; ++c) {
-        float o[32];
-        tc::tmem_ld32(lanes + O_AT + part * COLS + c * 32, o);
+      for (int c = 0; c < COLS / 16; ++c) {
+        uint32_t o[16];
+        tc::tmem_ld16(lanes + O_AT + part * COLS + c * 16, o);
         tc::tmem_ld_wait();
         tc::hold_regs(o);
-        const float2 scale2 = make_float2(A.scale, A.scale);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float2 x = fmul2(make_float2(o[8 * i + 2 * k], o[8 * i + 2 * k + 1]), scale2);
+            const float2 x = fmul2(make_float2(__uint_as_float(o[8 * i + 2 * k]),
+                                               __uint_as_float(o[8 * i + 2 * k + 1])), scale2);
             w[k] = attn::pack2<false>(x.x, x.y);
           }
           const uint4 piece = make_uint4(w[0], w[1], w[2], w[3]);
-          const int at = COLS == 64 ? (c * 4 + i) ^ (lane & 7) : i ^ ((lane >> 1) & 3);
+          const int at = (c * 2 + i) ^ (COLS == 64 ? lane & 7 : (lane >> 1) & 3);
           if (whole)
-            *reinterpret_cast<uint4*>(tile + lane * COLS * 2 + at * 16) = piece;
-          else if (row < I.n && part * COLS + c * 32 + i * 8 < A.Dv)
-            *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = piece;
+            store_shared(smem_addr(tile) + lane * COLS * 2 + at * 16, piece);
+          else if (row < I.n && part * COLS + c * 16 + i * 8 < A.Dv)
+            *reinterpret_cast<uint4*>(out + c * 16 + i * 8) = piece;
         }
       }
       if (odd && row < I.n)
@@ -509,9 +538,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp < MMA_WARP) {
     // ------------------------------------------- the values with their decay, V'
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    // A strip of 32 columns; the groups of rows of one of the two buffers.
-    const int strip = warp & 3, buffer = (warp >> 2) & 1;
-    const uint32_t to = tmem + ((uint32_t)(strip * 32) << 16) + PARTS_AT + buffer * PARTS_STEP;
+    // A strip of 32 columns; the groups of rows of one of the buffers.
+    constexpr int FIRST = STATES ? STATE_WARPS : VALUE_FIRST, WARPS = 4 * Sh::BUFFERS;
+    const int strip = warp & 3, buffer = (warp - FIRST) >> 2;
+    const uint32_t to =
+        tmem + ((uint32_t)(strip * 32) << 16) + Sh::PARTS_AT + buffer * PARTS_STEP;
     const bool active = strip * 32 < DVP;
     uint32_t free_phase = 1;
     while (ok) {
@@ -523,15 +554,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint8_t* v_tile = smem + st * Sh::STAGE + Sh::V_AT + (active ? (strip >> 1) * BLOCK : 0);
       if (n < CHUNK) {
         // Rows of a neighbour: zero.  (Of the values, those that this warp reads.)
-        for (int x = threadIdx.x - VALUE_FIRST * 32; x < (CHUNK - n) * 8 * KC;
-             x += VALUE_WARPS * 32) {
+        for (int x = threadIdx.x - FIRST * 32; x < (CHUNK - n) * 8 * KC; x += WARPS * 32) {
           const int r = x >> 3, c = r / (CHUNK - n);
           *reinterpret_cast<uint4*>(k_tile + c * BLOCK + (n + r - c * (CHUNK - n)) * 128 +
                                     (x & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         if (active)
           for (int j = n + (lane >> 2); j < CHUNK; j += 8)
-            if (((j / GROUP) & 1) == buffer)
+            if ((j / GROUP) % Sh::BUFFERS == buffer)
               *reinterpret_cast<uint4*>(v_tile + j * 128 +
                                         ((((strip & 1) * 4 + (lane & 3)) ^ (j & 7)) << 4)) =
                   make_uint4(0, 0, 0, 0);
@@ -539,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       float2 odd = make_float2(0.f, 0.f);
 #pragma unroll 1
-      for (int g = buffer; g < CHUNK / GROUP; g += 2) {
+      for (int g = buffer; g < CHUNK / GROUP; g += Sh::BUFFERS) {
         const float on = B->on[st][g];
         const float2 on2 = make_float2(on, on);
         if (!need(&B->v_free[buffer], free_phase)) break;
@@ -550,35 +580,30 @@ __global__ void __launch_bounds__(THREADS, 1)
                               ((((strip & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
         const float* left = &B->left[st][g * GROUP + (lane & 3) * 2];
 #pragma unroll 1
-        for (int r = 0; r < 4; r += 2) {
-          uint32_t part[3][2][4];            // low, middle, high; upper and lower 16 columns
+        for (int r = 0; r < 4; ++r) {
+          uint32_t w[4], part[3][4];         // low, middle, high
+          attn::ldmatrix_x4_trans(w, from + r * 8 * 128);
+          const float2 d = fmul2(*reinterpret_cast<const float2*>(left + r * 8), on2);
+          const float2 minus = make_float2(-1.f, -1.f);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t w[4];
-            attn::ldmatrix_x4_trans(w, from + (r + u) * 8 * 128);
-            const float2 d =
-                fmul2(*reinterpret_cast<const float2*>(left + (r + u) * 8), on2);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float2 x = make_float2(low_half(w[c]), high_half(w[c]));
-              odd = ffma2(x, make_float2(0.f, 0.f), odd);
-              x = fmul2(x, d);
-              const float2 minus = make_float2(-1.f, -1.f);
-              const uint32_t hi = attn::pack2<false>(x.x, x.y);
-              x = ffma2(make_float2(low_half(hi), high_half(hi)), minus, x);
-              const uint32_t mid = attn::pack2<false>(x.x, x.y);
-              x = ffma2(make_float2(low_half(mid), high_half(mid)), minus, x);
-              part[0][c >> 1][u * 2 + (c & 1)] = attn::pack2<false>(x.x, x.y);
-              part[1][c >> 1][u * 2 + (c & 1)] = mid;
-              part[2][c >> 1][u * 2 + (c & 1)] = hi;
-            }
+          for (int c = 0; c < 4; ++c) {
+            float2 x = make_float2(low_half(w[c]), high_half(w[c]));
+            odd = ffma2(x, make_float2(0.f, 0.f), odd);
+            x = fmul2(x, d);
+            const uint32_t hi = attn::pack2<false>(x.x, x.y);
+            x = ffma2(make_float2(low_half(hi), high_half(hi)), minus, x);
+            const uint32_t mid = attn::pack2<false>(x.x, x.y);
+            x = ffma2(make_float2(low_half(mid), high_half(mid)), minus, x);
+            part[0][c] = attn::pack2<false>(x.x, x.y);
+            part[1][c] = mid;
+            part[2][c] = hi;
           }
           if (active)
 #pragma unroll
-            for (int t = 0; t < 3; ++t)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                tmem_st_pieces(to + ((uint32_t)(h * 16) << 16) + t * 16 + r * 4, part[t][h]);
+            for (int t = 0; t < 3; ++t) {
+              tmem_st_pieces(to + t * 16 + r * 4, part[t][0], part[t][1]);
+              tmem_st_pieces(to + (16u << 16) + t * 16 + r * 4, part[t][2], part[t][3]);
+            }
         }
         tc::tmem_st_wait();
         attn::fence_proxy_async();           // the zeroed keys
@@ -586,11 +611,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         arrive(&B->v_full[buffer]);
       }
       if (!ok) break;
-      if (active && __any_sync(0xffffffffu, odd.x + odd.y != 0.f)) {   // true of not-a-number
+      // (The test is true of not-a-number.)
+      if (!STATES && active && __any_sync(0xffffffffu, odd.x + odd.y != 0.f)) {
         const int dv = strip * 32 + lane, piece = (dv & 63) >> 3;
         int first = 255;
         for (int j = 0; j < n; ++j) {
-          if (((j / GROUP) & 1) != buffer) continue;
+          if ((j / GROUP) % Sh::BUFFERS != buffer) continue;
           uint16_t* e = reinterpret_cast<uint16_t*>(v_tile + j * 128 + (dv & 7) * 2 +
                                                     ((piece ^ (j & 7)) << 4));
           if (attn::odd_element<false>(*e)) {
@@ -631,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc::tc_fence_after();
         const uint32_t q_at = base + st * Sh::STAGE, k_at = q_at + Sh::K_AT;
         const uint32_t v_at = q_at + Sh::V_AT;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < KC; ++c) {
           const uint64_t a = tc::sw128_desc(q_at + c * BLOCK);
           const uint64_t b = tc::sw128_desc(k_at + c * BLOCK);
@@ -642,7 +668,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc::umma_commit_one(one, &B->s_full);
         if (!need(&B->state_ready, one_phase) || !need(&B->o_free, one_phase ^ 1u)) break;
         tc::tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < KC; ++c) {
           const uint64_t a = tc::sw128_desc(q_at + c * BLOCK);
           const uint64_t b = tc::sw128_desc(state_at + c * DVP * 128);
@@ -654,7 +680,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!need(&B->clean, one_phase) || !need(&B->p_full, one_phase)) break;
         tc::tc_fence_after();
         const uint64_t b = tc::sw128_desc_mn(v_at, BLOCK);
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < CHUNK / 16; ++k)
           tc::umma_ts_one(one, tm + O_AT, tm + S_AT + (k >> 2) * 64 + (k & 3) * 8,
                           b + k * (2048 >> 4), ID_P, 1);
@@ -675,18 +701,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint64_t b = tc::sw128_desc_mn(base + st * Sh::STAGE + Sh::K_AT, BLOCK);
 #pragma unroll 1
         for (int g = 0; g < CHUNK / GROUP; ++g) {
-          if (!need(&B->v_full[g & 1], full_phase)) break;
+          const int buffer = g % Sh::BUFFERS;
+          if (!need(&B->v_full[buffer], full_phase)) break;
           tc::tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int t = 0; t < 3; ++t)
 #pragma unroll
             for (int k = 0; k < GROUP / 16; ++k)
               tc::umma_ts_one(one, tm + GAIN_AT,
-                              tm + PARTS_AT + (g & 1) * PARTS_STEP + t * 16 + k * 8,
+                              tm + Sh::PARTS_AT + buffer * PARTS_STEP + t * 16 + k * 8,
                               b + (g * (GROUP / 16) + k) * (2048 >> 4), ID_V,
                               (uint32_t)(g + t + k > 0));
-          tc::umma_commit_one(one, &B->v_free[g & 1]);
-          full_phase ^= (uint32_t)(g & 1);
+          tc::umma_commit_one(one, &B->v_free[buffer]);
+          full_phase ^= (uint32_t)(buffer == Sh::BUFFERS - 1);
         }
         if (!ok) break;
         tc::umma_commit_one(one, &B->gain_done);
