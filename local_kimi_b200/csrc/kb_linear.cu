@@ -291,5 +291,6 @@ extern "C" size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64
   namespace ln = kb::linear;
   const int64_t longest = max_tokens < total ? max_tokens : total;
   if (B <= 0 || H <= 0 || Dk <= 0 || Dv <= 0 || !ln::in_chunks(dtype, longest)) return 0;
-  return ln::chunk_workspace(B, H, Dk, Dv, longest, kb::num_sms(kb::bind_stream_device(nullptr)));
+  return ln::chunk_workspace(B, H, Dk, Dv, total, longest,
+                             kb::num_sms(kb::bind_stream_device(nullptr)));
 }

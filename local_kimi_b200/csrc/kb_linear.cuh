@@ -51,7 +51,8 @@ __device__ __forceinline__ float* request_state(const Args& A, int b, int h) {
 __device__ __forceinline__ float decay_of(float g) { return g > 0.f ? 0.f : g; }
 
 // Prompts in chunks on the tensor cores (kb_linear_chunk.cu), bf16.
-size_t chunk_workspace(int64_t B, int64_t H, int64_t Dk, int64_t Dv, int64_t longest, int sms);
+size_t chunk_workspace(int64_t B, int64_t H, int64_t Dk, int64_t Dv, int64_t total,
+                       int64_t longest, int sms);
 int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspace,
                   size_t workspace_bytes, void* stream);
 

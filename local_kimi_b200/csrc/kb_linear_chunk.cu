@@ -14,7 +14,7 @@
 // chunks one after the other.  Q, K and V tiles (128 rows, 64-element blocks in the 128-byte
 // swizzle) arrive by tensor copies in two stages.
 //
-//   warp 26: the copies, warp 27: the decays of each chunk (each walks the units).
+//   warp 26: the units and the copies.
 //   warp 24: issues S = Q K^T, O = Q S (the state), O += P V.
 //   warp 25: issues S^T += V'^T K, V' = the values with their decay to the chunk's end.
 //   warps 0-7: the state, in their registers in fp32 (a value column a thread, half of the key
@@ -49,13 +49,27 @@ constexpr int THREADS = 896;
 constexpr int MOST_STAGES = 3;
 constexpr int STATE_WARPS = 8, OUT_WARPS = 8, VALUE_WARPS = 8;
 constexpr int VALUE_FIRST = STATE_WARPS + OUT_WARPS;
-constexpr int MMA_WARP = 24, GAIN_WARP = 25, COPY_WARP = 26, DECAY_WARP = 27;
+constexpr int MMA_WARP = 24, GAIN_WARP = 25, COPY_WARP = 26;
 constexpr float RESET = -104.f;
 constexpr int GROUP = 32;                    // rows of V' that are made at a time
 constexpr uint32_t S_AT = 0, O_AT = 128, GAIN_AT = 256, PARTS_STEP = 64;
 
+// The decays of a chunk and head.
+struct Decays {
+  float at[CHUNK];                           // b_i, base 2
+  float left[CHUNK];                         // exp(b_e - b_j), e the last row of j's group
+  float on[CHUNK / GROUP];                   // exp(b_C - b_e) of each group
+  float keep;                                // exp(b_C)
+  float unused[3];
+  uint8_t since[CHUNK];                      // the last reset up to the row, plus 1; 0: none
+};
+static_assert(sizeof(Decays) % 16 == 0, "bulk copies");
+
 struct ChunkArgs {
   Args a;
+  Decays* decays;                            // [chunks][H], place_of() chunks
+  const int* order;                          // requests, longest first; NULL: units by number
+  int* taken;                                // with it: units taken beyond each CTA's first
   int segments, segment;                     // of a request at most; tokens of one
   float* sums;                               // [B][segments][H][DKP][DVP]: a segment's gain
   float* keeps;                              // [B][segments][H]: its decay
@@ -64,10 +78,10 @@ struct ChunkArgs {
 struct Item {
   int64_t first;                             // the chunk's first token
   int n;                                     // its tokens, -1: the end
+  int64_t place;                             // of its decays
   int b, h, seg;
   int starts, ends;                          // the unit's first, last chunk; 2: the request's
   int odd;                                   // values that are no numbers
-  float keep;                                // exp(b_C)
 };
 
 template <int DKP, int DVP, bool STATES>
@@ -90,11 +104,8 @@ struct ChunkShape {
 
 template <int N>                             // stages
 struct ChunkShared {
-  float at[N][CHUNK];                   // b_i, base 2
-  float left[N][CHUNK];                 // exp(b_e - b_j), e the last row of j's group
-  uint8_t since[N][CHUNK];              // the last reset up to the row, plus 1; 0: none
+  alignas(16) Decays decays[N];
   uint8_t odd_from[2][CHUNK];                // of each value column, of every other group
-  alignas(16) float on[N][CHUNK / GROUP];           // exp(b_C - b_e) of each group
   Item item[N];
   uint64_t full[N], info[N], empty[N], staged[N];
   uint64_t v_full[4], v_free[4];             // of the groups of V'
@@ -163,14 +174,22 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
+// Where a request's chunks' decays start: places enough for all before, without a sum over them.
+__device__ __forceinline__ int64_t place_of(int64_t first, int b) { return first / CHUNK + b; }
+
 // The units of this CTA and their chunks, in order.
+//
+// With more units than CTAs a CTA takes its next from a counter, one ahead, requests longest
+// first.
 struct Items {
   const ChunkArgs& C;
   int64_t unit, units;
-  int64_t at, end, last;                     // tokens of the unit left; the request's end
+  int64_t at, first, end, last;              // tokens: the unit's left; the request's
   Item next;
   bool states;
-  __device__ __forceinline__ Items(const ChunkArgs& c, bool s) : C(c), at(0), end(0), last(0), states(s) {
+  int ahead;
+  __device__ __forceinline__ Items(const ChunkArgs& c, bool s)
+      : C(c), at(0), first(0), end(0), last(0), states(s), ahead(blockIdx.x) {
     unit = (int64_t)blockIdx.x - gridDim.x;
     units = (int64_t)C.a.B * C.segments * C.a.H;
     advance();
@@ -179,7 +198,13 @@ struct Items {
     const Args& A = C.a;
     next.starts = 0;
     while (at >= end) {
-      unit += gridDim.x;
+      if (C.order == nullptr) {
+        unit += gridDim.x;
+      } else {
+        unit = __shfl_sync(0xffffffffu, ahead, 0);
+        if ((threadIdx.x & 31) == 0 && unit < units)
+          ahead = (int)gridDim.x + atomicAdd(C.taken, 1);
+      }
       if (unit >= units) {
         next.n = -1;
         return;
@@ -188,7 +213,7 @@ struct Items {
       next.h = (int)(unit - bs * A.H);
       next.b = (int)(bs / C.segments);
       next.seg = (int)(bs - (int64_t)next.b * C.segments);
-      int64_t first;
+      if (C.order != nullptr) next.b = __ldg(C.order + next.b);
       const int n = request_tokens(A, next.b, first);
       at = first + (int64_t)next.seg * C.segment;
       last = first + n;
@@ -199,10 +224,156 @@ struct Items {
     }
     next.first = at;
     next.n = (int)min(end - at, (int64_t)CHUNK);
+    next.place = (place_of(first, next.b) + (at - first) / CHUNK) * A.H + next.h;
     at += CHUNK;
     next.ends = at < end ? 0 : end < last ? 1 : 2;
   }
 };
+
+// ---------------------------------------------------------------------------
+// The decays of every chunk, a warp a chunk and head; the last CTA orders the requests.
+// (A warp of the chunks' kernel that made them beside its other work took 5000 to 8000 clocks a
+// chunk, more than the chunk: 8192 tokens x 32 heads 122 us.)
+// ---------------------------------------------------------------------------
+
+constexpr int PREPARE_THREADS = 256;
+
+// A row a lane, four groups side by side.  The sums behind a row (to its group's end, then group
+// by group) are those that V' and the state need: where they matter they are small, and exact to
+// 2^-24 of themselves.  The sums up to a row, for P, whose weights have 8 bits, are the group's
+// less those behind.
+__device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n, int h,
+                                             Decays* D) {
+  constexpr int GROUPS = CHUNK / GROUP;
+  const int lane = threadIdx.x & 31;
+  float up[GROUPS], behind[GROUPS];
+  unsigned marks[GROUPS];
+  int none = CHUNK;                          // the first logarithm that is no number
+#pragma unroll
+  for (int p = 0; p < GROUPS; ++p) {
+    const int j = p * GROUP + lane;
+    up[p] = j < n ? __ldg(A.decay + (first + j) * A.decay_tok + h) : 0.f;
+  }
+#pragma unroll
+  for (int p = 0; p < GROUPS; ++p) {
+    const float x = decay_of(up[p]);
+    marks[p] = __ballot_sync(0xffffffffu, x <= RESET);
+    const unsigned odd = __ballot_sync(0xffffffffu, x != x);
+    if (odd) none = min(none, p * GROUP + __ffs(odd) - 1);
+    up[p] = x > RESET ? x * LOG2E : 0.f;
+    behind[p] = __shfl_down_sync(0xffffffffu, up[p], 1);
+    if (lane == 31) behind[p] = 0.f;
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int p = 0; p < GROUPS; ++p) {
+      const float z = __shfl_down_sync(0xffffffffu, behind[p], o);
+      if (lane + o < 32) behind[p] += z;
+    }
+  float whole[GROUPS], on[GROUPS], before = 0.f, after = 0.f;
+  int since[GROUPS], last = 0, later = 0;
+#pragma unroll
+  for (int p = 0; p < GROUPS; ++p) {
+    whole[p] = __shfl_sync(0xffffffffu, up[p] + behind[p], 0);
+    before += whole[p];
+    up[p] = before - behind[p];
+    const unsigned seen = marks[p] & (0xffffffffu >> (31 - lane));
+    since[p] = seen ? p * GROUP + 32 - __clz(seen) : last;
+    if (marks[p]) last = p * GROUP + 32 - __clz(marks[p]);
+  }
+#pragma unroll
+  for (int p = GROUPS - 1; p >= 0; --p) {
+    on[p] = later ? 0.f : exp2f(after);
+    after += whole[p];
+    later |= marks[p] != 0;
+    // A reset behind the row, in its group.
+    const unsigned rest = lane < 31 ? marks[p] >> (lane + 1) : 0u;
+    behind[p] = p * GROUP + lane >= n || rest ? 0.f : exp2f(behind[p]);
+  }
+  float keep = later ? 0.f : exp2f(after);
+  if (none < CHUNK) {                        // all sums over it are none either
+    keep = NAN;
+#pragma unroll
+    for (int p = 0; p < GROUPS; ++p) {
+      if (p * GROUP + lane >= none) up[p] = NAN;
+      if (p == none / GROUP && p * GROUP + lane < none) behind[p] = NAN;
+      on[p] = NAN;
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < GROUPS; ++p) {
+    const int j = p * GROUP + lane;
+    D->at[j] = up[p];
+    D->left[j] = behind[p];
+    D->since[j] = (uint8_t)since[p];
+  }
+  if (lane == 0) {
+    *reinterpret_cast<float4*>(D->on) = make_float4(on[0], on[1], on[2], on[3]);
+    D->keep = keep;
+  }
+}
+
+__global__ void __launch_bounds__(PREPARE_THREADS)
+    prepare_kernel(const Args A, Decays* decays, int64_t places, int* order, int* taken) {
+  constexpr int BUCKETS = 4 * PREPARE_THREADS;
+  __shared__ int starts[BUCKETS];
+  __shared__ int sums[PREPARE_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (order == nullptr || blockIdx.x + 1 < gridDim.x) {
+    const int64_t at = (int64_t)blockIdx.x * (PREPARE_THREADS / 32) + warp;
+    if (at >= places * A.H) return;
+    const int64_t place = at / A.H;
+    const int h = (int)(at - place * A.H);
+    // The request: the last whose chunks start at or before the place.
+    int lo = 0, hi = A.B - 1;
+    auto start = [&](int b) {
+      return place_of(min(max((int64_t)__ldg(A.cu + b), (int64_t)0), A.total), b);
+    };
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (start(mid) <= place) lo = mid; else hi = mid - 1;
+    }
+    int64_t first;
+    const int n = request_tokens(A, lo, first);
+    const int64_t skip = (place - place_of(first, lo)) * CHUNK;
+    if (skip < 0 || skip >= n) return;
+    chunk_decays(A, first + skip, (int)min(n - skip, (int64_t)CHUNK), h, decays + at);
+    return;
+  }
+  // Requests by number of chunks, most first; the longest ones together.
+  auto bucket = [&](int b) {
+    int64_t first;
+    const int n = request_tokens(A, b, first);
+    return BUCKETS - 1 - min((n + CHUNK - 1) / CHUNK, BUCKETS - 1);
+  };
+  if (tid == 0) *taken = 0;
+  for (int i = tid; i < BUCKETS; i += PREPARE_THREADS) starts[i] = 0;
+  __syncthreads();
+  for (int b = tid; b < A.B; b += PREPARE_THREADS) atomicAdd(&starts[bucket(b)], 1);
+  __syncthreads();
+  int mine[4], in = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) in += mine[i] = starts[tid * 4 + i];
+  const int own = in;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) in += u;
+  }
+  if (lane == 31) sums[warp] = in;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) in += sums[w];
+  in -= own;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    starts[tid * 4 + i] = in;
+    in += mine[i];
+  }
+  __syncthreads();
+  for (int b = tid; b < A.B; b += PREPARE_THREADS) order[atomicAdd(&starts[bucket(b)], 1)] = b;
+}
 
 template <int DKP, int DVP, bool STATES>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -322,9 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!need(&B->info[st], ph)) break;
       const int n = B->item[st].n, b = B->item[st].b, h = B->item[st].h, seg = B->item[st].seg;
       const int starts = B->item[st].starts, ends = B->item[st].ends;
-      const float keep = B->item[st].keep;
       if (n < 0) break;
-      arrive(&B->empty[st]);
       if (starts) {
         // What the unit starts from: the request's state, and the gains of the segments before.
 #pragma unroll
@@ -358,6 +527,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       if (!STATES) copy_state();
+      if (!need(&B->full[st], ph)) break;
+      const float keep = B->decays[st].keep;
+      arrive(&B->empty[st]);
       if (!need(&B->gain_done, one_phase)) break;
       tc::tc_fence_after();
       if (active)
@@ -410,8 +582,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!need(&B->info[st], ph)) break;
       const Item I = B->item[st];
       if (I.n < 0) break;
-      const float mine = B->at[st][row];
-      const int since = B->since[st][row];
+      if (!need(&B->full[st], ph)) break;
+      const Decays& D = B->decays[st];
+      const float mine = D.at[row];
+      const int since = D.since[row];
       if (!need(&B->s_full, one_phase)) break;
       tc::tc_fence_after();
       // (Loops that stay loops, here and below: each scheduler runs warps of every role, whose
@@ -434,9 +608,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (j0 < q0) {
             // All before the rows: the decay to the group's end, and on to the row.
             const int last = j0 | (GROUP - 1);
-            const float on = since > last + 1 ? 0.f : exp2_fast(mine - B->at[st][last]);
+            const float on = since > last + 1 ? 0.f : exp2_fast(mine - D.at[last]);
             const float2 on2 = make_float2(on, on);
-            const float* left = &B->left[st][j0];
+            const float* left = &D.left[j0];
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
               const float4 d = *reinterpret_cast<const float4*>(left + i);
@@ -447,7 +621,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           } else {
             const float2 here = make_float2(mine, mine), minus = make_float2(-1.f, -1.f);
-            const float* at = &B->at[st][j0];
+            const float* at = &D.at[j0];
             // Columns up to the row, and from its last reset on.
             uint32_t seen = 0xffffffffu >> (31 - lane);
             if (since > q0 + 1) seen &= 0xffffffffu << (since - 1 - q0);
@@ -570,7 +744,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       float2 odd = make_float2(0.f, 0.f);
 #pragma unroll 1
       for (int g = buffer; g < CHUNK / GROUP; g += Sh::BUFFERS) {
-        const float on = B->on[st][g];
+        const float on = B->decays[st].on[g];
         const float2 on2 = make_float2(on, on);
         if (!need(&B->v_free[buffer], free_phase)) break;
         free_phase ^= 1u;
@@ -578,7 +752,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // Eight rows a piece: pairs of rows of column 8 c + lane / 4, rows 2 (lane % 4) and on.
         const uint32_t from = smem_addr(v_tile) + (g * GROUP + (lane & 7)) * 128 +
                               ((((strip & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4);
-        const float* left = &B->left[st][g * GROUP + (lane & 3) * 2];
+        const float* left = &B->decays[st].left[g * GROUP + (lane & 3) * 2];
 #pragma unroll 1
         for (int r = 0; r < 4; ++r) {
           uint32_t w[4], part[3][4];         // low, middle, high
@@ -743,14 +917,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       Items items(C, STATES);
       int sent = 0;
-      for (; items.next.n >= 0; ++sent) {
-        const int token = (int)items.next.first, h = items.next.h;
+      while (true) {
         if (!STATES && sent >= STAGES) send(st, ph ^ 1u);
         if (!ok || !need(&B->empty[st], ph ^ 1u)) break;
         if (lane == 0) {
+          Item I = items.next;
+          I.odd = 0;
+          B->item[st] = I;
+          mbar_arrive(&B->info[st]);
+        }
+        if (items.next.n < 0) break;
+        if (lane == 0) {
+          const int token = (int)items.next.first, h = items.next.h;
           uint8_t* to = smem + st * Sh::STAGE;
-          mbar_arrive_expect_tx(&B->full[st],
-                                (uint32_t)((STATES ? KC + VC : 2 * KC + VC) * BLOCK));
+          mbar_arrive_expect_tx(&B->full[st], (uint32_t)(Sh::STAGE + sizeof(Decays)));
+          bulk_g2s(&B->decays[st], C.decays + items.next.place, sizeof(Decays), &B->full[st],
+                   once);
           for (int c = 0; c < KC; ++c) {
             attn::tma_load_4d(to + Sh::K_AT + c * BLOCK, &tk, c * 64, h / A.k_group, token, 0,
                               &B->full[st], k_policy);
@@ -763,6 +945,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                               &B->full[st], v_policy);
         }
         __syncwarp();
+        ++sent;
         items.advance();
         turn();
       }
@@ -776,82 +959,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (*abort_f)
         for (int i = 0; i < STAGES; ++i)
           for (uint32_t parity = 0; parity < 2; ++parity) attn::drain_phase(&B->full[i], parity);
-    } else if (warp == DECAY_WARP) {
-      // ------------------------------------------------------- the decays of a chunk
-      // A row a lane, four groups side by side.  The sums behind a row (to its group's end, then
-      // group by group) are those that V' and the state need: where they matter they are small,
-      // and exact to 2^-24 of themselves.  The sums up to a row, for P, whose weights have 8
-      // bits, are the group's less those behind.
-      constexpr int GROUPS = CHUNK / GROUP;
-      Items items(C, STATES);
-      float ahead[GROUPS];
-      auto fetch = [&]() {
-        const float* from = A.decay + items.next.first * A.decay_tok + items.next.h;
-#pragma unroll
-        for (int p = 0; p < GROUPS; ++p)     // (always a row of the chunk: nothing waits here)
-          ahead[p] = __ldg(from + min(p * GROUP + lane, items.next.n - 1) * A.decay_tok);
-      };
-      if (items.next.n > 0) fetch();
-      while (true) {
-        Item I = items.next;
-        float up[GROUPS], behind[GROUPS];
-        unsigned marks[GROUPS];
-#pragma unroll
-        for (int p = 0; p < GROUPS; ++p) {
-          const float x = p * GROUP + lane < I.n ? decay_of(ahead[p]) : 0.f;
-          marks[p] = __ballot_sync(0xffffffffu, x <= RESET);
-          up[p] = x <= RESET ? 0.f : x * LOG2E;
-          behind[p] = __shfl_down_sync(0xffffffffu, up[p], 1);
-          if (lane == 31) behind[p] = 0.f;
-        }
-        if (I.n >= 0) {
-          items.advance();
-          if (items.next.n > 0) fetch();
-        }
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-          for (int p = 0; p < GROUPS; ++p) {
-            const float z = __shfl_down_sync(0xffffffffu, behind[p], o);
-            if (lane + o < 32) behind[p] += z;
-          }
-        float whole[GROUPS], on[GROUPS], before = 0.f, after = 0.f;
-        int since[GROUPS], last = 0, later = 0;
-#pragma unroll
-        for (int p = 0; p < GROUPS; ++p) {
-          whole[p] = __shfl_sync(0xffffffffu, up[p] + behind[p], 0);
-          before += whole[p];
-          up[p] = before - behind[p];
-          const unsigned seen = marks[p] & (0xffffffffu >> (31 - lane));
-          since[p] = seen ? p * GROUP + 32 - __clz(seen) : last;
-          if (marks[p]) last = p * GROUP + 32 - __clz(marks[p]);
-        }
-#pragma unroll
-        for (int p = GROUPS - 1; p >= 0; --p) {
-          on[p] = later ? 0.f : exp2_fast(after);
-          after += whole[p];
-          later |= marks[p] != 0;
-          // A reset behind the row, in its group.
-          const unsigned rest = lane < 31 ? marks[p] >> (lane + 1) : 0u;
-          behind[p] = p * GROUP + lane >= I.n || rest ? 0.f : exp2_fast(behind[p]);
-        }
-        I.odd = 0;
-        I.keep = later ? 0.f : exp2_fast(after);
-        if (!need(&B->empty[st], ph ^ 1u)) break;
-#pragma unroll
-        for (int p = 0; p < GROUPS; ++p) {
-          B->at[st][p * GROUP + lane] = up[p];
-          B->left[st][p * GROUP + lane] = behind[p];
-          B->since[st][p * GROUP + lane] = (uint8_t)since[p];
-        }
-        if (lane == 0)
-          *reinterpret_cast<float4*>(B->on[st]) = make_float4(on[0], on[1], on[2], on[3]);
-        if (lane == 0) B->item[st] = I;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->info[st]);
-        if (I.n < 0) break;
-        turn();
-      }
     }
     __syncwarp();
   }
@@ -903,23 +1010,57 @@ static void segments_of(int64_t heads, int64_t longest, int sms, int& segments, 
   }
 }
 
-size_t chunk_workspace(int64_t B, int64_t H, int64_t Dk, int64_t Dv, int64_t longest, int sms) {
+// Requests of several lengths on fewer CTAs than units.  (24 prompts of 1 to 2047 tokens, 24
+// heads: 80 us with the units dealt out by number, 66 from a counter in this order.)
+static bool by_order(int64_t B, int64_t H, int segments, int sms) {
+  return segments == 1 && B > 1 && B * H > sms && B * H < ((int64_t)1 << 30);
+}
+
+// The workspace: decays, then segments' gains and decays, or the order and its counter.
+struct Layout {
   int segments, segment;
-  segments_of(B * H, longest, sms, segments, segment);
-  return segments > 1 ? (size_t)(B * segments * H) * (padded(Dk) * padded(Dv) + 1) * sizeof(float)
-                      : 0;
+  bool order;
+  int64_t places;
+  size_t sums, keeps, taken, bytes;
+  Layout(int64_t B, int64_t H, int64_t Dk, int64_t Dv, int64_t total, int64_t longest, int sms) {
+    segments_of(B * H, longest, sms, segments, segment);
+    order = by_order(B, H, segments, sms);
+    places = total / CHUNK + B + 1;
+    sums = (size_t)(places * H) * sizeof(Decays);
+    const size_t units = segments > 1 ? (size_t)(B * segments * H) : 0;
+    keeps = sums + units * padded(Dk) * padded(Dv) * sizeof(float);
+    taken = keeps + units * sizeof(float);
+    bytes = taken + (order ? (size_t)(B + 1) * sizeof(int) : 0);
+  }
+};
+
+size_t chunk_workspace(int64_t B, int64_t H, int64_t Dk, int64_t Dv, int64_t total,
+                       int64_t longest, int sms) {
+  return Layout(B, H, Dk, Dv, total, longest, sms).bytes;
 }
 
 int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspace,
                   size_t workspace_bytes, void* stream) {
+  const Layout L(A.B, A.H, A.Dk, A.Dv, A.total, A.longest, sms);
+  KB_REQUIRE(workspace_bytes >= L.bytes && workspace, KB_ERR_WORKSPACE,
+             "linear attention: workspace of %zu bytes, %zu needed", workspace_bytes, L.bytes);
+  KB_REQUIRE(((uintptr_t)workspace & 15) == 0, KB_ERR_ALIGNMENT,
+             "linear attention: the workspace must be 16-byte aligned");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
   ChunkArgs C = {};
   C.a = A;
-  segments_of((int64_t)A.B * A.H, A.longest, sms, C.segments, C.segment);
-  const size_t need = chunk_workspace(A.B, A.H, A.Dk, A.Dv, A.longest, sms);
-  KB_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), KB_ERR_WORKSPACE,
-             "linear attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  C.sums = static_cast<float*>(workspace);
-  C.keeps = C.sums + (size_t)A.B * C.segments * A.H * padded(A.Dk) * padded(A.Dv);
+  C.segments = L.segments;
+  C.segment = L.segment;
+  C.decays = reinterpret_cast<Decays*>(ws);
+  C.sums = reinterpret_cast<float*>(ws + L.sums);
+  C.keeps = reinterpret_cast<float*>(ws + L.keeps);
+  if (L.order) {
+    C.taken = reinterpret_cast<int*>(ws + L.taken);
+    C.order = C.taken + 1;
+  }
+  const int64_t warps = PREPARE_THREADS / 32, ctas = (L.places * A.H + warps - 1) / warps;
+  KB_REQUIRE(ctas < ((int64_t)1 << 31) - 1, KB_ERR_UNSUPPORTED,
+             "linear attention: too many tokens and heads");
   CUtensorMap mq, mk, mv, mo;
   int st = attn::make_map_4d(&mq, A.q, 0, {A.Dk, Hq, A.total, 1}, {A.q_head, A.q_tok, 8}, 1,
                              CHUNK);
@@ -933,6 +1074,8 @@ int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspac
     st = attn::make_map_4d(&mo, A.out, 0, {A.Dv, A.H, A.total, 1},
                            {A.Dv, (int64_t)A.H * A.Dv, 8}, 1, 32, A.Dv <= 64 ? 32 : 64);
   if (st != KB_OK) return st;
+  st = launch(prepare_kernel, dim3((unsigned)(ctas + (L.order ? 1 : 0))), dim3(PREPARE_THREADS), 0,
+              stream, A, C.decays, L.places, L.order ? C.taken + 1 : nullptr, C.taken);
   const int grid = (int)std::min<int64_t>((int64_t)A.B * C.segments * A.H, sms);
   for (int pass = C.segments > 1 ? 0 : 1; pass < 2 && st == KB_OK; ++pass) {
     const bool states = pass == 0;

@@ -9,13 +9,17 @@
 //   x = x + the request's biases of t, summed in their order
 //   x = -infinity                                        if the row's mask does not have t
 //
-// Bound: HBM, the logits read and written once.  A CTA takes a slice of the vocabulary and a
-// request, counts the history's tokens of its slice in shared memory (a 32-bit word a token:
-// bit 0 the prompt, from bit 1 up the count; integers, so the order of the atomics does not
-// show) and then streams its part of each of the request's rows, eight tokens a thread and
-// step.  A bit a token says whether there is anything to do: eight bits, read beside eight
-// bits of the mask, let most pieces pass with a copy, and pieces that the mask empties are
-// written without being read.  The history is read again by every slice, from L2.
+// Bound: HBM, the logits read and written once.  A CTA has a slice of the vocabulary and a few
+// rows.  It asks for its part of a row (eight tokens a thread and piece, all of them under way),
+// counts the request's history in shared memory while they arrive, and writes the part once.
+// Counts: a word a token, bit 0 the prompt, from bit 1 up how often (integers, so the order of
+// the atomics does not show); 16 bits where no history can have 2^15 tokens, else 32.  A bit a
+// token says whether there is anything to do: eight bits, beside eight bits of the mask, let
+// most pieces pass with a copy, and pieces that the mask empties are written without being
+// read.  Every slice reads the history again, from L2: slices are as wide as leaves several
+// CTAs an SM.
+#include <algorithm>
+
 #include "kb_common.cuh"
 
 #include <cuda_fp16.h>
@@ -31,7 +35,7 @@ struct Args {
   uint8_t* y;
   int64_t x_row, y_row;                      // elements
   int64_t rows;
-  int V, slice;
+  int V, rows_each;
   const int64_t* history;                    // [B, ...]
   int64_t history_row;
   const int *lens, *prompts;                 // prompts may be NULL: all of it is answer
@@ -83,213 +87,243 @@ __device__ __forceinline__ uint32_t eight(const uint32_t* row, int t, int words)
   return __funnelshift_r(lo, hi, s) & 0xffu;
 }
 
-struct Slice {
-  const uint32_t* count;                     // words of the slice's tokens
-  const uint32_t* flag;                      // bits: something to do
-  const int* bias_at;                        // biases of the slice in their order
-  const float* bias;
-  int biases;
-  float repetition, presence, frequency;
+// Words of counts: bit 0: in the prompt, from bit 1 up: how often in the answer.
+template <bool WIDE>
+struct Counts {
+  uint32_t* words;
+  static constexpr int BYTES = WIDE ? 4 : 2;
+  __device__ __forceinline__ uint32_t get(int at) const {
+    return WIDE ? words[at] : reinterpret_cast<const uint16_t*>(words)[at];
+  }
+  __device__ __forceinline__ void add(int at, uint32_t v) const {
+    if (WIDE)
+      atomicAdd(words + at, v);
+    else
+      atomicAdd(words + (at >> 1), v << (16 * (at & 1)));
+  }
+  __device__ __forceinline__ void sub(int at, uint32_t v) const {
+    if (WIDE)
+      atomicSub(words + at, v);
+    else
+      atomicSub(words + (at >> 1), v << (16 * (at & 1)));
+  }
+  __device__ __forceinline__ void prompt(int at) const {
+    if (WIDE)
+      atomicOr(words + at, 1u);
+    else
+      atomicOr(words + (at >> 1), 1u << (16 * (at & 1)));
+  }
 };
-constexpr uint32_t BIASED = 0x80000000u;
 
-__device__ __forceinline__ float adjust(float x, uint32_t word, int t, const Slice& S) {
-  const uint32_t c = (word & ~BIASED) >> 1;
-  if (word & ~BIASED) x = x > 0.f ? x / S.repetition : x * S.repetition;
-  if (c) {
-    x = __fsub_rn(x, __fmul_rn(S.frequency, (float)c));
-    x = __fsub_rn(x, S.presence);
-  }
-  if (word & BIASED) {
-    float sum = 0.f;
-    for (int i = 0; i < S.biases; ++i)
-      if (S.bias_at[i] == t) sum += S.bias[i];
-    x += sum;
-  }
-  return x;
-}
+struct Request {
+  float repetition, presence, frequency;
+  int biases;                                // of the slice
+};
 
-template <int TYPE>
+template <int TYPE, bool WIDE, int PIECES>   // pieces of eight tokens a thread
 __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
   using E = Element<TYPE>;
   using T = typename E::T;
-  constexpr int VECS = sizeof(T) / 2;        // 16-byte pieces of eight tokens
-  extern __shared__ uint32_t smem[];
-  uint32_t* count = smem;                                 // [slice]
-  uint32_t* flag = count + A.slice;                       // [slice / 32]
-  int* bias_at = reinterpret_cast<int*>(flag + A.slice / 32);   // [biases]
+  constexpr int VECS = sizeof(T) / 2;        // 16-byte loads of a piece
+  constexpr int SLICE = THREADS * 8 * PIECES;
+  extern __shared__ __align__(16) uint32_t smem[];
+  uint32_t* flag = smem;                                  // [SLICE / 32] something to do
+  uint32_t* biased = flag + SLICE / 32;                   // [SLICE / 32]
+  const Counts<WIDE> count = {biased + SLICE / 32};       // [SLICE]
+  int* bias_at = reinterpret_cast<int*>(smem + SLICE / 16 + SLICE * Counts<WIDE>::BYTES / 4);
   float* bias = reinterpret_cast<float*>(bias_at + A.biases);
   __shared__ int s_biases, s_warp[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.y, v0 = blockIdx.x * A.slice, v1 = min(A.V, v0 + A.slice);
-  for (int i = tid; i < A.slice + A.slice / 32; i += THREADS) smem[i] = 0;
-  if (tid == 0) s_biases = 0;
-  __syncthreads();
+  const int v0 = blockIdx.x * SLICE, v1 = min(A.V, v0 + SLICE);
+  const int words = (A.V + 31) / 32;
+  const bool same = A.x == A.y;              // in place: what does not change stays
   pdl_wait();
   pdl_launch_dependents();
 
-  // The request's rows; the last block of rows takes those outside every request.
-  int64_t r0 = b, r1 = b + 1, skip0 = 0, skip1 = 0;
-  const bool spare = b == A.B;
-  if (A.cu != nullptr) {
-    const int64_t lo = min(max((int64_t)A.cu[spare ? 0 : b], (int64_t)0), A.rows);
-    const int64_t hi = min(max((int64_t)A.cu[spare ? A.B : b + 1], lo), A.rows);
-    r0 = spare ? 0 : lo;
-    r1 = spare ? A.rows : hi;
-    if (spare) {
-      skip0 = lo;
-      skip1 = hi;
+  int current = -1;                          // the request whose counts these are
+  Request R = {1.f, 0.f, 0.f, 0};
+  bool counts = false;
+  const int64_t last = min(A.rows, ((int64_t)blockIdx.y + 1) * A.rows_each);
+  for (int64_t r = (int64_t)blockIdx.y * A.rows_each; r < last; ++r) {
+    // The row's request: the last that starts at or before it.  -1: outside all.
+    int b = (int)min(r, (int64_t)A.B);
+    int64_t first = r;
+    if (A.cu != nullptr) {
+      b = -1;
+      for (int i0 = 0; i0 <= A.B; i0 += THREADS)
+        b += __syncthreads_count(i0 + tid <= A.B && (int64_t)__ldg(A.cu + i0 + tid) <= r);
+      if (b >= 0) first = max((int64_t)A.cu[b], (int64_t)0);
     }
-  } else if (spare) {
-    r0 = A.B;
-    r1 = A.rows;
-  }
-  if (r0 >= r1) return;
-  Slice S = {count, flag, bias_at, bias, 0, 1.f, 0.f, 0.f};
-  if (!spare) {
-    if (A.repetition) S.repetition = A.repetition[b];
-    if (A.presence) S.presence = A.presence[b];
-    if (A.frequency) S.frequency = A.frequency[b];
-  }
-  const bool counts = S.repetition != 1.f || S.presence != 0.f || S.frequency != 0.f;
-  if (counts && A.history != nullptr) {
-    const int64_t* h = A.history + (int64_t)b * A.history_row;
-    const int n = min(max(A.lens[b], 0), A.longest);
-    const int p = A.prompts ? min(max(A.prompts[b], 0), n) : 0;
-#pragma unroll 4
-    for (int i = tid; i < n; i += THREADS) {
-      const int64_t t = __ldg(h + i);
-      if (t >= A.V) atomicOr(A.err, ERR_TREE);
-      if (t < v0 || t >= v1) continue;
-      const int at = (int)(t - v0);
-      if (i < p)
-        atomicOr(&count[at], 1u);
-      else
-        atomicAdd(&count[at], 2u);
-      atomicOr(&flag[at >> 5], 1u << (at & 31));
-    }
-  }
-  if (A.bias_ids != nullptr && !spare) {
-    // The slice's biases, kept in their order.
-    for (int i0 = 0; i0 < A.biases; i0 += THREADS) {
-      const int i = i0 + tid;
-      const int64_t t = i < A.biases ? __ldg(A.bias_ids + (int64_t)b * A.ids_row + i) : -1;
-      if (t >= A.V) atomicOr(A.err, ERR_TREE);
-      const bool here = t >= v0 && t < v1;
-      const unsigned votes = __ballot_sync(0xffffffffu, here);
-      if (lane == 0) s_warp[warp] = __popc(votes);
-      __syncthreads();
-      int at = s_biases + __popc(votes & ((1u << lane) - 1u)), all = 0;
-      for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) at += s_warp[w];
-        all += s_warp[w];
-      }
-      if (here) {
-        bias_at[at] = (int)t;
-        bias[at] = __ldg(A.bias_values + (int64_t)b * A.values_row + i);
-        atomicOr(&count[t - v0], BIASED);
-        atomicOr(&flag[(t - v0) >> 5], 1u << ((t - v0) & 31));
-      }
-      __syncthreads();
-      if (tid == 0) s_biases += all;
-      __syncthreads();
-    }
-    S.biases = s_biases;
-  }
-  __syncthreads();
+    if (b >= A.B) b = -1;
 
-  const bool same = A.x == A.y;              // in place: what does not change stays
-  for (int64_t r = r0; r < r1; ++r) {
-    if (r >= skip0 && r < skip1) continue;
-    // The drafted tokens above the row's prediction.
-    auto drafted = [&](bool on) {
-      const int64_t j = r - r0;
-      const uint64_t word = A.mask ? (uint64_t)A.mask[r] : 0;
-      for (int64_t i = tid; i <= (A.mask ? (int64_t)63 : j); i += THREADS) {
-        if (r0 + i >= r1 || (A.mask && !((word >> i) & 1))) continue;
-        const int64_t t = A.tokens[r0 + i];
-        if (t >= A.V) atomicOr(A.err, ERR_TREE);
-        if (t < v0 || t >= v1) continue;
-        const int at = (int)(t - v0);
-        if (on) {
-          atomicAdd(&count[at], 2u);
-          atomicOr(&flag[at >> 5], 1u << (at & 31));
-        } else {
-          atomicSub(&count[at], 2u);         // (its flag may stay: it only means looking)
-        }
-      }
-    };
-    const bool draft = counts && A.tokens != nullptr && !spare;
-    if (draft) {
-      drafted(true);
-      __syncthreads();
-    }
+    // The row's part: 16-byte pieces where input and output lie alike, single tokens at the ends.
     const T* x = reinterpret_cast<const T*>(A.x) + r * A.x_row;
     T* y = reinterpret_cast<T*>(A.y) + r * A.y_row;
-    const uint32_t* allowed = A.allowed && !spare ? A.allowed + r * A.allowed_row : nullptr;
-    const int words = (A.V + 31) / 32;
-    // 16-byte pieces where input and output lie alike, single tokens at the ends.
+    const uint32_t* allowed = A.allowed && b >= 0 ? A.allowed + r * A.allowed_row : nullptr;
     const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x + v0) & 15);
     const bool alike = lead == (uint32_t)(reinterpret_cast<uintptr_t>(y + v0) & 15);
     int a = min(v1, v0 + (int)(((16u - lead) & 15u) / sizeof(T)));
     int z = a + (v1 - a) / 8 * 8;
     if (!alike) a = z = v1;
+    uint32_t in[PIECES];
+    uint4 v[PIECES][VECS];
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
+      const int t = a + (tid + u * THREADS) * 8;
+      in[u] = t < z ? allowed ? eight(allowed, t, words) : 0xffu : 0u;
+    }
+    // (In place a part that nothing changes is not read; that is not known yet.)
+    if (!same)
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u)
+        if (in[u])
+#pragma unroll
+          for (int k = 0; k < VECS; ++k)
+            v[u][k] = ldg_stream_v4(reinterpret_cast<const uint4*>(
+                                        x + a + (tid + u * THREADS) * 8) + k);
+
+    if (b != current) {
+      // The request's parameters, and the counts of its history.
+      __syncthreads();
+      current = b;
+      R = {1.f, 0.f, 0.f, 0};
+      if (b >= 0) {
+        if (A.repetition) R.repetition = A.repetition[b];
+        if (A.presence) R.presence = A.presence[b];
+        if (A.frequency) R.frequency = A.frequency[b];
+      }
+      counts = R.repetition != 1.f || R.presence != 0.f || R.frequency != 0.f;
+      constexpr int ZEROS = (SLICE / 16 + SLICE * Counts<WIDE>::BYTES / 4) / 4;
+      // (Without penalties only the flags are looked at, and the biases' counts are 0.)
+      for (int i = tid; i < (counts || A.biases ? ZEROS : SLICE / 64); i += THREADS)
+        reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+      if (tid == 0) s_biases = 0;
+      __syncthreads();
+      if (counts && A.history != nullptr) {
+        const int64_t* h = A.history + (int64_t)b * A.history_row;
+        const int n = min(max(A.lens[b], 0), A.longest);
+        const int p = A.prompts ? min(max(A.prompts[b], 0), n) : 0;
+#pragma unroll 8
+        for (int i = tid; i < n; i += THREADS) {
+          const int64_t t = __ldg(h + i);
+          if (t < v0 || t >= v1) {
+            if (t >= A.V) atomicOr(A.err, ERR_TREE);
+            continue;
+          }
+          const int at = (int)(t - v0);
+          if (i < p)
+            count.prompt(at);
+          else
+            count.add(at, 2u);
+          atomicOr(&flag[at >> 5], 1u << (at & 31));
+        }
+      }
+      if (A.biases && b >= 0) {
+        // The slice's biases, kept in their order.
+        for (int i0 = 0; i0 < A.biases; i0 += THREADS) {
+          const int i = i0 + tid;
+          const int64_t t = i < A.biases ? __ldg(A.bias_ids + (int64_t)b * A.ids_row + i) : -1;
+          if (t >= A.V) atomicOr(A.err, ERR_TREE);
+          const bool here = t >= v0 && t < v1;
+          const unsigned votes = __ballot_sync(0xffffffffu, here);
+          if (lane == 0) s_warp[warp] = __popc(votes);
+          __syncthreads();
+          int at = s_biases + __popc(votes & ((1u << lane) - 1u)), all = 0;
+          for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) at += s_warp[w];
+            all += s_warp[w];
+          }
+          if (here) {
+            bias_at[at] = (int)t;
+            bias[at] = __ldg(A.bias_values + (int64_t)b * A.values_row + i);
+            atomicOr(&biased[(t - v0) >> 5], 1u << ((t - v0) & 31));
+            atomicOr(&flag[(t - v0) >> 5], 1u << ((t - v0) & 31));
+          }
+          __syncthreads();
+          if (tid == 0) s_biases += all;
+          __syncthreads();
+        }
+        R.biases = s_biases;
+      }
+      __syncthreads();
+    }
+    // The drafted tokens above the row's prediction.
+    const bool draft = counts && A.tokens != nullptr && b >= 0;
+    auto drafted = [&](bool on) {
+      const uint64_t word = A.mask ? (uint64_t)A.mask[r] : 0;
+      const int64_t end = min(A.rows, (int64_t)A.cu[b + 1]);
+      for (int64_t i = tid; i <= (A.mask ? (int64_t)63 : r - first); i += THREADS) {
+        if (first + i >= end || (A.mask && !((word >> i) & 1))) continue;
+        const int64_t t = A.tokens[first + i];
+        if (t >= A.V) atomicOr(A.err, ERR_TREE);
+        if (t < v0 || t >= v1) continue;
+        const int at = (int)(t - v0);
+        if (on) {
+          count.add(at, 2u);
+          atomicOr(&flag[at >> 5], 1u << (at & 31));
+        } else {
+          count.sub(at, 2u);                 // (its flag may stay: it only means looking)
+        }
+      }
+    };
+    if (draft) {
+      drafted(true);
+      __syncthreads();
+    }
+    auto adjust = [&](float f, int t) {
+      const int at = t - v0;
+      const uint32_t word = count.get(at), c = word >> 1;
+      if (word) f = f > 0.f ? f / R.repetition : f * R.repetition;
+      if (c) {
+        f = __fsub_rn(f, __fmul_rn(R.frequency, (float)c));
+        f = __fsub_rn(f, R.presence);
+      }
+      if ((biased[at >> 5] >> (at & 31)) & 1) {
+        float sum = 0.f;
+        for (int i = 0; i < R.biases; ++i)
+          if (bias_at[i] == t) sum += bias[i];
+        f += sum;
+      }
+      return f;
+    };
     for (int k = tid; k < (a - v0) + (v1 - z); k += THREADS) {
       const int t = k < a - v0 ? v0 + k : z + k - (a - v0);
-      const bool out = allowed && !((__ldg(allowed + (t >> 5)) >> (t & 31)) & 1);
-      const uint32_t word = count[t - v0];
-      if (out)
+      if (allowed && !((__ldg(allowed + (t >> 5)) >> (t & 31)) & 1))
         y[t] = E::NONE;
-      else if (word)
-        y[t] = E::store(adjust(E::load(x[t]), word, t, S));
+      else if ((flag[(t - v0) >> 5] >> ((t - v0) & 31)) & 1)
+        y[t] = E::store(adjust(E::load(x[t]), t));
       else if (!same)
         y[t] = x[t];
     }
-    constexpr int UNDERWAY = 4 / VECS;
-    for (int t0 = a + tid * 8; t0 < z; t0 += THREADS * 8 * UNDERWAY) {
-      uint32_t todo[UNDERWAY], in[UNDERWAY];
-      uint4 v[UNDERWAY][VECS];
 #pragma unroll
-      for (int u = 0; u < UNDERWAY; ++u) {
-        const int t = t0 + u * THREADS * 8;
-        in[u] = 0xffu;
-        if (allowed && t < z) in[u] = eight(allowed, t, words);
+    for (int u = 0; u < PIECES; ++u) {
+      const int t = a + (tid + u * THREADS) * 8;
+      if (t >= z) break;
+      const uint32_t todo = eight(flag, t - v0, SLICE / 32) & in[u];
+      if (same) {
+        if (todo == 0 && in[u] == 0xffu) continue;
+        if (in[u])
+#pragma unroll
+          for (int k = 0; k < VECS; ++k) v[u][k] = *(reinterpret_cast<const uint4*>(x + t) + k);
       }
+      union {
+        uint4 q[VECS];
+        T e[8];
+      } w;
 #pragma unroll
-      for (int u = 0; u < UNDERWAY; ++u) {
-        const int t = t0 + u * THREADS * 8;
-        todo[u] = t < z ? eight(flag, t - v0, A.slice / 32) & in[u] : 0;
-        if (t < z && in[u] != 0 && !(same && todo[u] == 0 && in[u] == 0xffu))
+      for (int k = 0; k < VECS; ++k) w.q[k] = in[u] ? v[u][k] : make_uint4(0, 0, 0, 0);
+      if (in[u] != 0xffu)
 #pragma unroll
-          for (int k = 0; k < VECS; ++k)
-            v[u][k] = *(reinterpret_cast<const uint4*>(x + t) + k);
-      }
+        for (int i = 0; i < 8; ++i)
+          if (!((in[u] >> i) & 1)) w.e[i] = E::NONE;
+      if (todo)
 #pragma unroll
-      for (int u = 0; u < UNDERWAY; ++u) {
-        const int t = t0 + u * THREADS * 8;
-        if (t >= z || (same && todo[u] == 0 && in[u] == 0xffu)) continue;
-        union {
-          uint4 q[VECS];
-          T e[8];
-        } w;
+        for (int i = 0; i < 8; ++i)
+          if ((todo >> i) & 1) w.e[i] = E::store(adjust(E::load(w.e[i]), t + i));
 #pragma unroll
-        for (int k = 0; k < VECS; ++k) w.q[k] = in[u] ? v[u][k] : make_uint4(0, 0, 0, 0);
-        if (in[u] != 0xffu)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (!((in[u] >> i) & 1)) w.e[i] = E::NONE;
-        if (todo[u])
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if ((todo[u] >> i) & 1) {
-              const uint32_t word = count[t + i - v0];
-              if (word) w.e[i] = E::store(adjust(E::load(w.e[i]), word, t + i, S));
-            }
-#pragma unroll
-        for (int k = 0; k < VECS; ++k) *(reinterpret_cast<uint4*>(y + t) + k) = w.q[k];
-      }
+      for (int k = 0; k < VECS; ++k) *(reinterpret_cast<uint4*>(y + t) + k) = w.q[k];
     }
-    if (draft) {
+    if (draft && r + 1 < last) {
       __syncthreads();
       drafted(false);
       __syncthreads();
@@ -297,15 +331,43 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
   }
 }
 
-template <int TYPE>
-static int launch_adjust(const Args& A, dim3 grid, size_t smem, void* stream) {
+template <int TYPE, bool WIDE, int PIECES>
+static int launch_slices(Args A, int sms, void* stream) {
+  constexpr int SLICE = THREADS * 8 * PIECES;
+  constexpr size_t FIXED = (size_t)SLICE / 4 + (size_t)SLICE * Counts<WIDE>::BYTES;
+  const size_t smem = FIXED + (size_t)A.biases * 8;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        adjust_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(adjust_kernel<TYPE, WIDE, PIECES>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(FIXED + MOST_BIASES * 8));
     KB_REQUIRE(e == cudaSuccess, KB_ERR_DEVICE, "adjust logits: shared-memory limit: %s",
                cudaGetErrorString(e));
   }
-  return launch(adjust_kernel<TYPE>, grid, dim3(THREADS), smem, stream, A);
+  const int64_t slices = (A.V + SLICE - 1) / SLICE;
+  // Several rows of drafts a CTA, whose requests' histories are counted once, where that
+  // leaves eight CTAs an SM.
+  A.rows_each = 1;
+  if (A.cu != nullptr)
+    A.rows_each = (int)std::min<int64_t>(64, std::max<int64_t>(1, slices * A.rows / (8 * sms)));
+  const int64_t y = (A.rows + A.rows_each - 1) / A.rows_each;
+  KB_REQUIRE(y <= 65535, KB_ERR_UNSUPPORTED, "adjust logits: more than 65535 rows");
+  return launch(adjust_kernel<TYPE, WIDE, PIECES>, dim3((unsigned)slices, (unsigned)y),
+                dim3(THREADS), smem, stream, A);
+}
+
+template <int TYPE, bool WIDE>
+static int launch_wide(const Args& A, int sms, void* stream) {
+  // Slices of 8192 tokens, or, where those are fewer than the SMs, of 2048.
+  if ((A.V + 8191) / 8192 * A.rows >= sms) return launch_slices<TYPE, WIDE, 4>(A, sms, stream);
+  return launch_slices<TYPE, WIDE, 1>(A, sms, stream);
+}
+
+template <int TYPE>
+static int launch_adjust(const Args& A, int sms, void* stream) {
+  // 15 bits count a history of fewer tokens, drafted ones included.
+  const int64_t most = (A.history ? A.longest : 0) + (A.mask ? 64 : A.tokens ? A.rows : 0);
+  return most < 32768 ? launch_wide<TYPE, false>(A, sms, stream)
+                      : launch_wide<TYPE, true>(A, sms, stream);
 }
 
 }  // namespace logits
@@ -327,7 +389,8 @@ extern "C" int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t 
                  out_stride >= V && (!allowed || allowed_stride >= (V + 31) / 32),
              KB_ERR_BAD_SHAPE, "adjust logits: bad shape");
   KB_REQUIRE(dtype >= 0 && dtype <= 2, KB_ERR_UNSUPPORTED, "adjust logits: unknown element type");
-  KB_REQUIRE(V < ((int64_t)1 << 30) && B < 65535 && longest < ((int64_t)1 << 30),
+  KB_REQUIRE(V < ((int64_t)1 << 30) && B < 65535 && longest < ((int64_t)1 << 30) &&
+                 rows < ((int64_t)1 << 30),
              KB_ERR_UNSUPPORTED, "adjust logits: more than 65534 requests or 2^30 tokens");
   KB_REQUIRE(n_biases <= lg::MOST_BIASES, KB_ERR_UNSUPPORTED,
              "adjust logits: more than %d biases a request", lg::MOST_BIASES);
@@ -368,14 +431,8 @@ extern "C" int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t 
   A.B = (int)B;
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  // Slices as wide as leaves four CTAs an SM: each reads the whole history.
-  const int64_t want = (int64_t)kb::num_sms(dev) * 4;
-  int slice = 1024;
-  while (slice < 16384 && (V + slice - 1) / slice * (B > 0 ? B : 1) > want) slice *= 2;
-  A.slice = slice;
-  const size_t smem = (size_t)slice * 4 + slice / 8 + (size_t)A.biases * 8;
-  const dim3 grid((unsigned)((V + slice - 1) / slice), (unsigned)(B + 1));
-  if (dtype == 0) return lg::launch_adjust<0>(A, grid, smem, stream);
-  if (dtype == 1) return lg::launch_adjust<1>(A, grid, smem, stream);
-  return lg::launch_adjust<2>(A, grid, smem, stream);
+  const int sms = kb::num_sms(dev);
+  if (dtype == 0) return lg::launch_adjust<0>(A, sms, stream);
+  if (dtype == 1) return lg::launch_adjust<1>(A, sms, stream);
+  return lg::launch_adjust<2>(A, sms, stream);
 }

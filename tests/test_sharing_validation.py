@@ -248,7 +248,7 @@ def test_c_checks(library):
         None, cu, 1, total, longest, 1.0, some, None, ws, None)
     assert lin(total=0) == 0 and lin(cu=None) == 1 and lin(longest=0) == 2
     assert library.kb_linear_attention_workspace_size(1, 2, 64, 64, 0, 5000, 5000) > 0
-    assert library.kb_linear_attention_workspace_size(400, 2, 64, 64, 0, 5000, 5000) == 0
+    assert library.kb_linear_attention_workspace_size(1, 400, 64, 64, 0, 5, 5) == 0
     assert library.kb_linear_attention_workspace_size(1, 2, 64, 64, 2, 5000, 5000) == 0
     assert library.kb_linear_attention_workspace_size(0, 2, 64, 64, 0, 0, 0) == 0
     fork = lambda b=2, n=1, free=some, w=4: library.kb_paged_fork(  # noqa: E731
