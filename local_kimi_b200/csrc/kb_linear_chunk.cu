@@ -92,6 +92,8 @@ struct ChunkShape {
   static constexpr int STAGE = V_AT + VC * BLOCK;
   static constexpr int STATE = STATES ? 0 : KC * DVP * 128;   // bytes of the bf16 copy
   // Groups of V' at a time: without scores and outputs their warps and columns serve it too.
+  // Outputs leave through the place of Q where that is as wide.
+  static constexpr bool STAGED = DKP >= DVP;
   static constexpr int BUFFERS = STATES ? 4 : 2;
   static constexpr uint32_t PARTS_AT = STATES ? 0 : 384;
   static constexpr int FIT = (227 * 1024 - 3072 - STATE) / STAGE;
@@ -106,10 +108,11 @@ template <int N>                             // stages
 struct ChunkShared {
   alignas(16) Decays decays[N];
   uint8_t odd_from[2][CHUNK];                // of each value column, of every other group
-  Item item[N];
-  uint64_t full[N], info[N], empty[N], staged[N];
+  Item item[N], out[N];                      // out: whose outputs are to be sent
+  uint64_t full[N], q_full[N], info[N], empty[N], staged[N];
+  uint64_t clean[N];                         // (the values may run ahead of the outputs)
   uint64_t v_full[4], v_free[4];             // of the groups of V'
-  uint64_t s_full, q_done, p_full, o_full, o_free, state_ready, clean, gain_done, gain_free, drain;
+  uint64_t s_full, q_done, p_full, o_full, o_free, state_ready, gain_done, gain_free, drain;
   uint32_t tmem;
   int abort_flag;
 };
@@ -393,9 +396,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&B->full[i], 1);
+      mbar_init(&B->q_full[i], 1);
+      mbar_init(&B->clean[i], VALUE_WARPS);
       mbar_init(&B->info[i], 1);
       mbar_init(&B->empty[i], STATES ? 1 + 4 * Sh::BUFFERS + STATE_WARPS
-                                     : 3 + VALUE_WARPS + STATE_WARPS);
+                                     : 2 + VALUE_WARPS + STATE_WARPS + OUT_WARPS);
       mbar_init(&B->staged[i], OUT_WARPS);
     }
     for (int i = 0; i < Sh::BUFFERS; ++i) {
@@ -408,7 +413,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(&B->o_full, 1);
     mbar_init(&B->o_free, OUT_WARPS);
     mbar_init(&B->state_ready, STATE_WARPS);
-    mbar_init(&B->clean, VALUE_WARPS);
     mbar_init(&B->gain_done, 1);
     mbar_init(&B->gain_free, STATE_WARPS);
     mbar_init(&B->drain, STATES ? 1 : 2);
@@ -516,12 +520,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float* gain = C.sums + u * (DKP * DVP) + gain_mine;
             if (active)
 #pragma unroll
-              for (int c = 0; c < HALF; c += 16) {
-                float x[16];
+              for (int c = 0; c < HALF; c += 32) {
+                float x[32];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = __ldcg(gain + (c + i) * DVP);
+                for (int i = 0; i < 32; ++i) x[i] = __ldcg(gain + (c + i) * DVP);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[c + i] = fmaf(s[c + i], all_of_it, x[i]);
+                for (int i = 0; i < 32; ++i) s[c + i] = fmaf(s[c + i], all_of_it, x[i]);
               }
           }
         }
@@ -665,12 +669,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!need(&B->o_full, one_phase)) break;
       tc::tc_fence_after();
       const int odd = *const_cast<volatile int*>(&B->item[st].odd);
-      // The warp's 32 rows and COLS columns go through the place of the values, which nobody
+      // The warp's 32 rows and COLS columns go through the place of the queries, which nobody
       // reads any more; the rows at a request's end go out by themselves.
       uint16_t* out = static_cast<uint16_t*>(A.out) +
                       ((I.first + row) * A.H + I.h) * A.Dv + part * COLS;
-      uint8_t* tile = smem + st * Sh::STAGE + Sh::V_AT + (part * CHUNK + q0) * COLS * 2;
-      const bool whole = q0 + 32 <= I.n && odd == 0;
+      uint8_t* tile = smem + st * Sh::STAGE + (part * CHUNK + q0) * COLS * 2;
+      const bool whole = Sh::STAGED && q0 + 32 <= I.n && odd == 0;
+      if (odd == 0) arrive(&B->empty[st]);
       const float2 scale2 = make_float2(A.scale, A.scale);
 #pragma unroll 1
       for (int c = 0; c < COLS / 16; ++c) {
@@ -706,6 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) {
         mbar_arrive(&B->o_free);
         mbar_arrive(&B->staged[st]);
+        if (odd) mbar_arrive(&B->empty[st]);
       }
       turn();
     }
@@ -805,7 +811,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) {
-        if (!STATES) mbar_arrive(&B->clean);
+        if (!STATES) mbar_arrive(&B->clean[st]);
         mbar_arrive(&B->empty[st]);
       }
       turn();
@@ -827,7 +833,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       while (true) {
         if (!need(&B->info[st], ph)) break;
         if (B->item[st].n < 0) break;
-        if (!need(&B->full[st], ph)) break;
+        if (!need(&B->full[st], ph) || !need(&B->q_full[st], ph)) break;
         tc::tc_fence_after();
         const uint32_t q_at = base + st * Sh::STAGE, k_at = q_at + Sh::K_AT;
         const uint32_t v_at = q_at + Sh::V_AT;
@@ -851,7 +857,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc::umma_one(one, tm + O_AT, a + k * 2, b + k * 2, ID_Q, c + k > 0);
         }
         tc::umma_commit_one(one, &B->q_done);
-        if (!need(&B->clean, one_phase) || !need(&B->p_full, one_phase)) break;
+        if (!need(&B->clean[st], ph) || !need(&B->p_full, one_phase)) break;
         tc::tc_fence_after();
         const uint64_t b = tc::sw128_desc_mn(v_at, BLOCK);
 #pragma unroll 2
@@ -902,63 +908,81 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t k_policy = STATES || A.k_group > 1 ? keep_in_l2 : once;
       const uint64_t q_policy = A.q_group > 1 ? keep_in_l2 : once;
       const uint64_t v_policy = STATES ? keep_in_l2 : once;
-      // The outputs of a stage leave before its next loads.  Lanes 0 to 7: 32 rows and COLS
-      // columns each.
+      // A stage's outputs leave before its next queries.  Lanes 0 to 7: 32 rows and COLS columns
+      // each.
       auto send = [&](int st, uint32_t parity) {
         if (!need(&B->staged[st], parity)) return;
-        const Item I = B->item[st];
+        const Item& I = B->out[st];
         const int part = lane >> 2, q0 = (lane & 3) * 32;
-        if (lane < 8 && q0 + 32 <= I.n && I.odd == 0 && part * (DVP / 2) < A.Dv) {
-          store_tile(&to, smem + st * Sh::STAGE + Sh::V_AT + (part * CHUNK + q0) * DVP,
-                     part * (DVP / 2), I.h, (int)I.first + q0);
+        if (Sh::STAGED && lane < 8 && q0 + 32 <= I.n && I.odd == 0 && part * (DVP / 2) < A.Dv) {
+          store_tile(&to, smem + st * Sh::STAGE + (part * CHUNK + q0) * DVP, part * (DVP / 2), I.h,
+                     (int)I.first + q0);
           stored_from_shared();
         }
-        arrive(&B->empty[st]);
+        __syncwarp();
       };
       Items items(C, STATES);
       int sent = 0;
       while (true) {
-        if (!STATES && sent >= STAGES) send(st, ph ^ 1u);
-        if (!ok || !need(&B->empty[st], ph ^ 1u)) break;
+        if (!need(&B->empty[st], ph ^ 1u)) break;
+        const bool more = items.next.n >= 0;
+        const int token = (int)items.next.first, h = items.next.h;
+        uint8_t* to_stage = smem + st * Sh::STAGE;
         if (lane == 0) {
+          if (!STATES && sent >= STAGES) B->out[st] = B->item[st];
           Item I = items.next;
           I.odd = 0;
           B->item[st] = I;
           mbar_arrive(&B->info[st]);
-        }
-        if (items.next.n < 0) break;
-        if (lane == 0) {
-          const int token = (int)items.next.first, h = items.next.h;
-          uint8_t* to = smem + st * Sh::STAGE;
-          mbar_arrive_expect_tx(&B->full[st], (uint32_t)(Sh::STAGE + sizeof(Decays)));
-          bulk_g2s(&B->decays[st], C.decays + items.next.place, sizeof(Decays), &B->full[st],
-                   once);
-          for (int c = 0; c < KC; ++c) {
-            attn::tma_load_4d(to + Sh::K_AT + c * BLOCK, &tk, c * 64, h / A.k_group, token, 0,
-                              &B->full[st], k_policy);
-            if (!STATES)
-              attn::tma_load_4d(to + c * BLOCK, &tq, c * 64, h / A.q_group, token, 0,
-                                &B->full[st], q_policy);
+          if (more) {
+            mbar_arrive_expect_tx(&B->full[st],
+                                  (uint32_t)((KC + VC) * BLOCK + sizeof(Decays)));
+            bulk_g2s(&B->decays[st], C.decays + items.next.place, sizeof(Decays), &B->full[st],
+                     once);
+            for (int c = 0; c < KC; ++c)
+              attn::tma_load_4d(to_stage + Sh::K_AT + c * BLOCK, &tk, c * 64, h / A.k_group, token,
+                                0, &B->full[st], k_policy);
+            for (int c = 0; c < VC; ++c)
+              attn::tma_load_4d(to_stage + Sh::V_AT + c * BLOCK, &tv, c * 64, h, token, 0,
+                                &B->full[st], v_policy);
           }
-          for (int c = 0; c < VC; ++c)
-            attn::tma_load_4d(to + Sh::V_AT + c * BLOCK, &tv, c * 64, h, token, 0,
-                              &B->full[st], v_policy);
         }
         __syncwarp();
+        if (!more) break;
+        if (!STATES) {
+          if (sent >= STAGES) send(st, ph ^ 1u);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&B->q_full[st], (uint32_t)(KC * BLOCK));
+            for (int c = 0; c < KC; ++c)
+              attn::tma_load_4d(to_stage + c * BLOCK, &tq, c * 64, h / A.q_group, token, 0,
+                                &B->q_full[st], q_policy);
+          }
+          __syncwarp();
+        }
         ++sent;
         items.advance();
         turn();
       }
-      // (`st` is the oldest stage, if all are in use.)
+      // The last outputs: `st` is the oldest stage, if all are in use, its item set aside.
       if (!STATES && ok)
         for (int i = max(0, STAGES - sent); i < STAGES && ok; ++i) {
           const int at = (st + i) % STAGES;
-          send(at, (uint32_t)((sent - STAGES + i) / STAGES) & 1u);
+          const uint32_t parity = (uint32_t)((sent - STAGES + i) / STAGES) & 1u;
+          if (i > 0) {
+            if (!need(&B->staged[at], parity)) break;
+            if (lane == 0) B->out[at] = B->item[at];
+            __syncwarp();
+          }
+          send(at, parity);
         }
       // On the error path, copies in flight land before the CTA may exit.
       if (*abort_f)
         for (int i = 0; i < STAGES; ++i)
-          for (uint32_t parity = 0; parity < 2; ++parity) attn::drain_phase(&B->full[i], parity);
+          for (uint32_t parity = 0; parity < 2; ++parity) {
+            attn::drain_phase(&B->full[i], parity);
+            if (!STATES) attn::drain_phase(&B->q_full[i], parity);
+          }
     }
     __syncwarp();
   }
