@@ -725,6 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem + ((uint32_t)(strip * 32) << 16) + Sh::PARTS_AT + buffer * PARTS_STEP;
     const bool active = strip * 32 < DVP;
     uint32_t free_phase = 1;
+    bool any = false;                        // a chunk before this one
     while (ok) {
       if (!need(&B->info[st], ph)) break;
       const int n = B->item[st].n;
@@ -792,6 +793,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok) break;
       // (The test is true of not-a-number.)
+      const bool first_one = !any;
+      any = true;
       if (!STATES && active && __any_sync(0xffffffffu, odd.x + odd.y != 0.f)) {
         const int dv = strip * 32 + lane, piece = (dv & 63) >> 3;
         int first = 255;
@@ -804,6 +807,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             *e = 0;
           }
         }
+        // (The outputs of the chunk before may still be reading theirs.)
+        if (!first_one && !need(&B->staged[st == 0 ? STAGES - 1 : st - 1],
+                                st == 0 ? ph ^ 1u : ph))
+          break;
         B->odd_from[buffer][dv] = (uint8_t)first;
         __syncwarp();
         if (lane == 0) atomicOr(&B->item[st].odd, 1 << (buffer * 4 + strip));
