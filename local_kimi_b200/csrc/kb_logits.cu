@@ -54,6 +54,15 @@ struct Args {
   uint32_t* err;
 };
 
+__device__ __forceinline__ void mask_pairs(uint4& q, uint32_t bits, uint32_t none) {
+  // Bytes of w, or of `none` where the bit is not set.
+  auto pair = [&](uint32_t w, int at) {
+    const uint32_t off = ~bits >> at;
+    return prmt(w, none, 0x3210u + (off & 1) * 0x44u + (off & 2) * 0x2200u);
+  };
+  q = make_uint4(pair(q.x, 0), pair(q.y, 2), pair(q.z, 4), pair(q.w, 6));
+}
+
 template <int TYPE>                          // 0 bf16, 1 f16, 2 f32
 struct Element;
 template <>
@@ -62,6 +71,10 @@ struct Element<0> {
   static __device__ __forceinline__ float load(T v) { return bf16_bits_to_float(v); }
   static __device__ __forceinline__ T store(float v) { return float_to_bf16_bits(v); }
   static constexpr T NONE = 0xff80u;         // -infinity
+  // Elements of a 16-byte piece whose bit is not set: -infinity.
+  static __device__ __forceinline__ void mask(uint4& q, uint32_t bits) {
+    mask_pairs(q, bits, 0xff80ff80u);
+  }
 };
 template <>
 struct Element<1> {
@@ -71,6 +84,9 @@ struct Element<1> {
     return __half_as_ushort(__float2half_rn(v));
   }
   static constexpr T NONE = 0xfc00u;
+  static __device__ __forceinline__ void mask(uint4& q, uint32_t bits) {
+    mask_pairs(q, bits, 0xfc00fc00u);
+  }
 };
 template <>
 struct Element<2> {
@@ -78,10 +94,17 @@ struct Element<2> {
   static __device__ __forceinline__ float load(T v) { return __uint_as_float(v); }
   static __device__ __forceinline__ T store(float v) { return __float_as_uint(v); }
   static constexpr T NONE = 0xff800000u;
+  static __device__ __forceinline__ void mask(uint4& q, uint32_t bits) {
+    if (!(bits & 1)) q.x = NONE;
+    if (!(bits & 2)) q.y = NONE;
+    if (!(bits & 4)) q.z = NONE;
+    if (!(bits & 8)) q.w = NONE;
+  }
 };
 
-// Eight bits from bit t on of a row of `words` words.
-__device__ __forceinline__ uint32_t eight(const uint32_t* row, int t, int words) {
+// Eight bits from bit t on of a row of `words` words; a byte where rows start at one.
+__device__ __forceinline__ uint32_t eight(const uint32_t* row, int t, int words, bool bytes) {
+  if (bytes) return reinterpret_cast<const uint8_t*>(row)[t >> 3];
   const int w = t >> 5, s = t & 31;
   const uint32_t lo = row[w], hi = s > 24 && w + 1 < words ? row[w + 1] : 0u;
   return __funnelshift_r(lo, hi, s) & 0xffu;
@@ -121,7 +144,7 @@ struct Request {
 };
 
 template <int TYPE, bool WIDE, int PIECES>   // pieces of eight tokens a thread
-__global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
+__global__ void __launch_bounds__(THREADS, TYPE == 2 ? 3 : 4) adjust_kernel(const Args A) {
   using E = Element<TYPE>;
   using T = typename E::T;
   constexpr int VECS = sizeof(T) / 2;        // 16-byte loads of a piece
@@ -130,7 +153,9 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
   uint32_t* flag = smem;                                  // [SLICE / 32] something to do
   uint32_t* biased = flag + SLICE / 32;                   // [SLICE / 32]
   const Counts<WIDE> count = {biased + SLICE / 32};       // [SLICE]
-  int* bias_at = reinterpret_cast<int*>(smem + SLICE / 16 + SLICE * Counts<WIDE>::BYTES / 4);
+  uint16_t* list = reinterpret_cast<uint16_t*>(smem + SLICE / 16 +
+                                               SLICE * Counts<WIDE>::BYTES / 4);   // [SLICE]
+  int* bias_at = reinterpret_cast<int*>(list + SLICE);
   float* bias = reinterpret_cast<float*>(bias_at + A.biases);
   __shared__ int s_biases, s_warp[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -165,12 +190,42 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
     int a = min(v1, v0 + (int)(((16u - lead) & 15u) / sizeof(T)));
     int z = a + (v1 - a) / 8 * 8;
     if (!alike) a = z = v1;
+    const bool bytes = (a & 7) == 0;
+    // What a new request needs, the start of its history before its length is known, and the
+    // row's mask: one wait for all of them.
+    const bool fresh = b != current;
+    const bool told = fresh && b >= 0 && A.history != nullptr;
+    constexpr int EARLY = 4;
+    int64_t h[EARLY];
+    int n = 0, p = 0;
+    const int64_t* history = A.history + (int64_t)max(b, 0) * A.history_row;
+    if (fresh) {
+      R = {1.f, 0.f, 0.f, 0};
+      if (b >= 0) {
+        if (A.repetition) R.repetition = A.repetition[b];
+        if (A.presence) R.presence = A.presence[b];
+        if (A.frequency) R.frequency = A.frequency[b];
+      }
+      if (told) {
+        n = A.lens[b];
+        p = A.prompts ? A.prompts[b] : 0;
+#pragma unroll
+        for (int u = 0; u < EARLY; ++u)
+          h[u] = tid + u * THREADS < A.longest ? __ldg(history + tid + u * THREADS) : -1;
+      }
+    }
     uint32_t in[PIECES];
     uint4 v[PIECES][VECS];
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
       const int t = a + (tid + u * THREADS) * 8;
-      in[u] = t < z ? allowed ? eight(allowed, t, words) : 0xffu : 0u;
+      in[u] = t < z ? allowed ? eight(allowed, t, words, bytes) : 0xffu : 0u;
+    }
+    if (fresh) {
+      __syncthreads();
+      for (int i = tid; i < (SLICE / 16 + SLICE * Counts<WIDE>::BYTES / 4) / 4; i += THREADS)
+        reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+      if (tid == 0) s_biases = 0;
     }
     // (In place a part that nothing changes is not read; that is not known yet.)
     if (!same)
@@ -182,33 +237,18 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
             v[u][k] = ldg_stream_v4(reinterpret_cast<const uint4*>(
                                         x + a + (tid + u * THREADS) * 8) + k);
 
-    if (b != current) {
-      // The request's parameters, and the counts of its history.
-      __syncthreads();
+    if (fresh) {
+      // The counts of the request's history.
       current = b;
-      R = {1.f, 0.f, 0.f, 0};
-      if (b >= 0) {
-        if (A.repetition) R.repetition = A.repetition[b];
-        if (A.presence) R.presence = A.presence[b];
-        if (A.frequency) R.frequency = A.frequency[b];
-      }
       counts = R.repetition != 1.f || R.presence != 0.f || R.frequency != 0.f;
-      constexpr int ZEROS = (SLICE / 16 + SLICE * Counts<WIDE>::BYTES / 4) / 4;
-      // (Without penalties only the flags are looked at, and the biases' counts are 0.)
-      for (int i = tid; i < (counts || A.biases ? ZEROS : SLICE / 64); i += THREADS)
-        reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-      if (tid == 0) s_biases = 0;
       __syncthreads();
-      if (counts && A.history != nullptr) {
-        const int64_t* h = A.history + (int64_t)b * A.history_row;
-        const int n = min(max(A.lens[b], 0), A.longest);
-        const int p = A.prompts ? min(max(A.prompts[b], 0), n) : 0;
-#pragma unroll 8
-        for (int i = tid; i < n; i += THREADS) {
-          const int64_t t = __ldg(h + i);
+      if (counts && told) {
+        n = min(max(n, 0), A.longest);
+        p = min(max(p, 0), n);
+        auto seen = [&](int64_t t, int i) {
           if (t < v0 || t >= v1) {
             if (t >= A.V) atomicOr(A.err, ERR_TREE);
-            continue;
+            return;
           }
           const int at = (int)(t - v0);
           if (i < p)
@@ -216,6 +256,18 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
           else
             count.add(at, 2u);
           atomicOr(&flag[at >> 5], 1u << (at & 31));
+        };
+#pragma unroll
+        for (int u = 0; u < EARLY; ++u)
+          if (tid + u * THREADS < n) seen(h[u], tid + u * THREADS);
+#pragma unroll 1
+        for (int i0 = EARLY * THREADS + tid; i0 < n; i0 += EARLY * THREADS) {
+#pragma unroll
+          for (int u = 0; u < EARLY; ++u)
+            h[u] = i0 + u * THREADS < n ? __ldg(history + i0 + u * THREADS) : -1;
+#pragma unroll
+          for (int u = 0; u < EARLY; ++u)
+            if (i0 + u * THREADS < n) seen(h[u], i0 + u * THREADS);
         }
       }
       if (A.biases && b >= 0) {
@@ -286,42 +338,51 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
       }
       return f;
     };
+#pragma unroll 1
     for (int k = tid; k < (a - v0) + (v1 - z); k += THREADS) {
       const int t = k < a - v0 ? v0 + k : z + k - (a - v0);
       if (allowed && !((__ldg(allowed + (t >> 5)) >> (t & 31)) & 1))
         y[t] = E::NONE;
-      else if ((flag[(t - v0) >> 5] >> ((t - v0) & 31)) & 1)
-        y[t] = E::store(adjust(E::load(x[t]), t));
       else if (!same)
         y[t] = x[t];
     }
+    // The pieces: copied, or masked.
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
       const int t = a + (tid + u * THREADS) * 8;
-      if (t >= z) break;
-      const uint32_t todo = eight(flag, t - v0, SLICE / 32) & in[u];
-      if (same) {
-        if (todo == 0 && in[u] == 0xffu) continue;
-        if (in[u])
+      if (t >= z || (same && in[u] == 0xffu)) continue;
 #pragma unroll
-          for (int k = 0; k < VECS; ++k) v[u][k] = *(reinterpret_cast<const uint4*>(x + t) + k);
+      for (int k = 0; k < VECS; ++k) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (in[u]) q = same ? *(reinterpret_cast<const uint4*>(x + t) + k) : v[u][k];
+        if (in[u] != 0xffu) E::mask(q, in[u] >> (8 / VECS * k));
+        *(reinterpret_cast<uint4*>(y + t) + k) = q;
       }
-      union {
-        uint4 q[VECS];
-        T e[8];
-      } w;
-#pragma unroll
-      for (int k = 0; k < VECS; ++k) w.q[k] = in[u] ? v[u][k] : make_uint4(0, 0, 0, 0);
-      if (in[u] != 0xffu)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (!((in[u] >> i) & 1)) w.e[i] = E::NONE;
-      if (todo)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if ((todo >> i) & 1) w.e[i] = E::store(adjust(E::load(w.e[i]), t + i));
-#pragma unroll
-      for (int k = 0; k < VECS; ++k) *(reinterpret_cast<uint4*>(y + t) + k) = w.q[k];
+    }
+    if (!counts && !R.biases) continue;
+    // The tokens that change, listed by each warp for its words of flags and dealt out to its
+    // lanes, over what has just been written.
+    __syncthreads();
+    constexpr int WORDS = SLICE / 32 / (THREADS / 32);     // of a warp, at most one a lane
+    static_assert(WORDS <= 32, "flags of a warp");
+    uint16_t* mine = list + warp * WORDS * 32;
+    uint32_t bits = lane < WORDS ? flag[warp * WORDS + lane] : 0u;
+    int found = __popc(bits);
+    int at = -found;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, found, o);
+      if (lane >= o) found += before;
+    }
+    at += found;
+    for (; bits != 0; bits &= bits - 1)
+      mine[at++] = (uint16_t)((warp * WORDS + lane) * 32 + __ffs(bits) - 1);
+    found = __shfl_sync(0xffffffffu, found, 31);
+    __syncwarp();
+#pragma unroll 1
+    for (int i = lane; i < found; i += 32) {
+      const int t = v0 + mine[i];
+      if (t < v1 && (!allowed || ((__ldg(allowed + (t >> 5)) >> (t & 31)) & 1)))
+        y[t] = E::store(adjust(E::load(x[t]), t));
     }
     if (draft && r + 1 < last) {
       __syncthreads();
@@ -334,7 +395,7 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const Args A) {
 template <int TYPE, bool WIDE, int PIECES>
 static int launch_slices(Args A, int sms, void* stream) {
   constexpr int SLICE = THREADS * 8 * PIECES;
-  constexpr size_t FIXED = (size_t)SLICE / 4 + (size_t)SLICE * Counts<WIDE>::BYTES;
+  constexpr size_t FIXED = (size_t)SLICE / 4 + (size_t)SLICE * (Counts<WIDE>::BYTES + 2);
   const size_t smem = FIXED + (size_t)A.biases * 8;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(adjust_kernel<TYPE, WIDE, PIECES>,
