@@ -147,8 +147,10 @@ __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
 template <int TYPE>
 static int launch_tokens(const Args& A, int sms, void* stream) {
   const int64_t heads = (int64_t)A.B * A.H;
-  // Few heads: their columns on several CTAs each.
-  if (heads < 2 * sms && A.Dv > 32)
+  // Few heads: their columns on several CTAs each.  (32 heads of 128 x 128, one token: 1 request
+  // 3.3 us split and 5.0 whole, 2 requests 3.2 and 4.5, 4 requests 5.5 and 5.1, 9 requests 8.1
+  // and 7.2; eight tokens: 8.7 and 10.4 for 1 request, 15.5 and 10.7 for 4.)
+  if (heads * 2 < sms && A.Dv > 32)
     return launch(token_kernel<TYPE, 32>, dim3((unsigned)(heads * ((A.Dv + 31) / 32))),
                   dim3(THREADS), 0, stream, A);
   return launch(token_kernel<TYPE, 128>, dim3((unsigned)heads), dim3(THREADS), 0, stream, A);
@@ -213,8 +215,12 @@ static Args arguments(const void* q, int64_t q_tok, int64_t q_head, int64_t Hq, 
 }
 
 // Token by token for a few tokens, and for types that the tensor cores' form does not take.
-constexpr int64_t FEW = 8;
-static bool in_chunks(int dtype, int64_t longest) { return dtype == 0 && longest > FEW; }
+// (32 heads, token by token and in chunks: 1 request of 8 tokens 8.5 and 11.2 us, of 16 14.5 and
+// 11.2; 16 requests of 8 tokens 25 and 32, of 16 42 and 32; 256 requests of 4 tokens 308 and 376,
+// of 8 463 and 381.)
+static bool in_chunks(int dtype, int64_t heads, int64_t longest, int sms) {
+  return dtype == 0 && longest > (heads > 16 * sms ? 5 : 8);
+}
 
 static int run_tokens(const Args& A, int dtype, int sms, void* stream) {
   if (dtype == 0) return launch_tokens<0>(A, sms, stream);
@@ -280,9 +286,10 @@ extern "C" int kb_linear_attention(const void* q, int64_t q_token_stride, int64_
   const int dev = kb::bind_stream_device(stream);
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  if (ln::in_chunks(dtype, A.longest))
-    return ln::launch_chunks(A, Hq, Hk, kb::num_sms(dev), workspace, workspace_bytes, stream);
-  return ln::run_tokens(A, dtype, kb::num_sms(dev), stream);
+  const int sms = kb::num_sms(dev);
+  if (ln::in_chunks(dtype, B * H, A.longest, sms))
+    return ln::launch_chunks(A, Hq, Hk, sms, workspace, workspace_bytes, stream);
+  return ln::run_tokens(A, dtype, sms, stream);
 }
 
 extern "C" size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64_t Dk, int64_t Dv,
@@ -290,7 +297,8 @@ extern "C" size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64
                                                      int64_t max_tokens) {
   namespace ln = kb::linear;
   const int64_t longest = max_tokens < total ? max_tokens : total;
-  if (B <= 0 || H <= 0 || Dk <= 0 || Dv <= 0 || !ln::in_chunks(dtype, longest)) return 0;
-  return ln::chunk_workspace(B, H, Dk, Dv, total, longest,
-                             kb::num_sms(kb::bind_stream_device(nullptr)));
+  if (B <= 0 || H <= 0 || Dk <= 0 || Dv <= 0) return 0;
+  const int sms = kb::num_sms(kb::bind_stream_device(nullptr));
+  if (!ln::in_chunks(dtype, B * H, longest, sms)) return 0;
+  return ln::chunk_workspace(B, H, Dk, Dv, total, longest, sms);
 }

@@ -22,8 +22,8 @@
 // copies to places that the copying thread alone reads: 2048 tokens on their way.
 //
 // Measured, 163840 tokens in bf16, replayed: 256 rows 60.5 us (84 MB each way less what masks
-// leave out, 2.4 TB/s), with histories of 10 tokens 39, without any 31 (5.4 TB/s); one request of nine drafted
-// rows 10.6.  Slices of 16384 tokens and 512 threads: 61.0 (histories of 8000 tokens 78 instead
+// leave out, 2.4 TB/s), with histories of 10 tokens 39, without any 31 (5.4 TB/s); one request
+// of nine drafted rows 10.6.  Slices of 16384 tokens and 512 threads: 61.0 (histories of 8000 tokens 78 instead
 // of 92, none 35 instead of 31).
 #include <algorithm>
 
@@ -448,7 +448,8 @@ static int launch_slices(Args A, int sms, void* stream) {
   }
   const int64_t slices = (A.V + SLICE - 1) / SLICE;
   // Several rows of drafts a CTA, whose requests' histories are counted once, where that
-  // leaves eight CTAs an SM.
+  // leaves eight CTAs an SM.  (128 requests of nine rows: 297 us, 343 with a row a CTA; 32
+  // requests: 82 and 92.)
   A.rows_each = 1;
   if (A.cu != nullptr)
     A.rows_each = (int)std::min<int64_t>(64, std::max<int64_t>(1, slices * A.rows / (8 * sms)));

@@ -29,9 +29,12 @@ constexpr int THREADS = 256;                 // fork, copy
 constexpr int WIDE = 1024;                   // free, compact
 constexpr int CLUSTER = 8;
 constexpr int MAX_REQUESTS = 12288;
-constexpr int MAX_PAGES = 1 << 19;           // two bitmaps and a share: 192 KB at most
+constexpr int MAX_PAGES = 1 << 19;           // two bitmaps and a share: 144 KB at most
 constexpr int LONGEST = (1 << 30) - 1;
-// One CTA marks as many table entries in the time that a cluster takes to meet.
+// One CTA marks as many table entries in the time that a cluster takes to meet.  (Pages given
+// back, entries and pages together 4096: 6.3 us alone, 7.3 by eight CTAs; 8192: 7.7 and 7.3;
+// 16384: 10.9 and 7.3; 65536: 31 and 9.  Compaction: 8.4 and 11.6, 10 and 11.8, 13.4 and 12, 28
+// and 13.4.)
 constexpr int64_t ALONE = 8192;
 
 __device__ __forceinline__ int length_of(const int* lens, int b) {
