@@ -1499,52 +1499,59 @@ MAX_LINEAR_WIDTH = 128
 def _linear_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
                  state: torch.Tensor | None, state_index: torch.Tensor | None, requests: int,
                  expanded: bool):
-    """Checked inputs of linear attention: (q, k, v, decay, per_token, state strides, index)."""
-    if q.dtype not in _ELEMENT:
+    """Checked inputs of linear attention: the sizes (tokens, H, Dk, Dv), the C call's arguments
+    from q to the state's slots and its index, and what they point to."""
+    dtype, device = q.dtype, q.device
+    if dtype not in _ELEMENT:
         raise TypeError("queries, keys and values must be BF16, FP16 or FP32")
-    if not (q.dtype == k.dtype == v.dtype):
+    if k.dtype != dtype or v.dtype != dtype:
         raise TypeError("queries, keys and values must share one type")
-    if log_decay.dtype != torch.float32 or log_decay.ndim not in (1, 2):
+    per_token = log_decay.ndim == 2
+    if log_decay.dtype != torch.float32 or not (per_token or log_decay.ndim == 1):
         raise TypeError("log_decay must be an FP32 [tokens, heads] matrix or [heads] vector")
     _require_cuda(q, "linear attention")
-    device = q.device
-    if not (k.device == v.device == log_decay.device == device):
+    if k.device != device or v.device != device or log_decay.device != device:
         raise ValueError("linear attention inputs must share one device")
-    qr, kr, vr = (_rows_of_heads(x, what, expanded) for x, what in ((q, "q"), (k, "k"), (v, "v")))
-    total, heads, dv = v.shape
-    dk = q.shape[2]
-    if q.shape[0] != total or k.shape[0] != total or k.shape[2] != dk:
+    qr, kr, vr = (_rows_of_heads(q, "q", expanded), _rows_of_heads(k, "k", expanded),
+                  _rows_of_heads(v, "v", expanded))
+    (tq, hq, dk), (tk, hk, wk), (total, heads, dv) = q.shape, k.shape, v.shape
+    if tq != total or tk != total or wk != dk:
         raise ValueError("q, k and v must have the same tokens, and q and k one width")
-    if not heads or any(not x.shape[1] or heads % x.shape[1] for x in (q, k)):
+    if not (heads and hq and hk) or heads % hq or heads % hk:
         raise ValueError("value heads must be a multiple of the query heads and of the key heads")
     if not (0 < dk <= MAX_LINEAR_WIDTH and dk % 8 == 0 and 0 < dv <= MAX_LINEAR_WIDTH
             and dv % 8 == 0):
         raise ValueError(f"head widths must be multiples of 8 up to {MAX_LINEAR_WIDTH}")
-    if log_decay.shape not in ((total, heads), (heads,)):
+    if log_decay.shape != ((total, heads) if per_token else (heads,)):
         raise ValueError("log_decay must have a row for each token, or one for all, of all heads")
-    index, strides = None, (0, 0)
+    index, place, slots, slot_stride, head_stride = None, None, 0, 0, 0
     if state is not None:
         if state.dtype != torch.float32 or state.ndim != 4:
             raise TypeError("state must be an FP32 [slots, heads, Dk, Dv] tensor")
         if state.device != device:
             raise ValueError("state must be on the device of the other tensors")
-        if state.shape[1:] != (heads, dk, dv):
+        slots, *block = state.shape
+        if block != [heads, dk, dv]:
             raise ValueError("state must have the heads and widths of the values and keys")
-        s = state.stride()
-        if (s[3] != 1 or s[2] != dv or (s[0] | s[1]) & 3 or state.data_ptr() & 15
-                or (heads > 1 and s[1] < dk * dv)
-                or (state.shape[0] > 1 and s[0] < dk * dv)) and state.numel():
+        place = state.data_ptr()
+        slot_stride, head_stride, row, one = state.stride()
+        if (one != 1 or row != dv or (slot_stride | head_stride) & 3 or place & 15
+                or (heads > 1 and head_stride < dk * dv)
+                or (slots > 1 and slot_stride < dk * dv)) and slots:
             raise ValueError("state is updated in place and needs dense, 16-byte aligned [Dk, Dv] "
                              "blocks of its own for every slot and head")
-        strides = s[:2]
     if state_index is not None:
         if state is None:
             raise ValueError("state_index goes with state")
         index = _vector(state_index, torch.int32, "state_index", device, requests)
-    elif state is not None and state.shape[0] < requests:
+    elif state is not None and slots < requests:
         raise ValueError("state needs a slot for every request")
     decay = log_decay if log_decay.is_contiguous() else log_decay.contiguous()
-    return qr, kr, vr, decay, int(log_decay.ndim == 2), strides, index
+    (qt, qh, _), (kt, kh, _), (vt, vh, _) = qr.stride(), kr.stride(), vr.stride()
+    return (total, heads, dk, dv), (
+        qr.data_ptr(), qt, qh, hq, kr.data_ptr(), kt, kh, hk, vr.data_ptr(), vt, vh, heads, dk, dv,
+        _ELEMENT[dtype], decay.data_ptr(), per_token, place, slot_stride, head_stride, slots,
+        None if index is None else index.data_ptr()), (qr, kr, vr, decay, index)
 
 
 def linear_attention(
@@ -1576,12 +1583,10 @@ def linear_attention(
     if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must have one entry more than there are requests")
     requests = cu_seqlens.shape[0] - 1
-    qr, kr, vr, decay, per_token, strides, index = _linear_args(
+    (total, heads, dk, dv), args, held = _linear_args(
         q, k, v, log_decay, state, state_index, requests, expanded=False)
     device = q.device
     cu = _vector(cu_seqlens, torch.int32, "cu_seqlens", device)
-    total, heads, dv = v.shape
-    dk = q.shape[2]
     if max_seqlen < 0 or (total and not max_seqlen):
         raise ValueError("max_seqlen must not be negative, nor 0 with tokens")
     scale = _scale_of(scale, dk)
@@ -1595,12 +1600,7 @@ def linear_attention(
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _on(device)(
         "kb_linear_attention",
-        qr.data_ptr(), qr.stride(0), qr.stride(1), q.shape[1], kr.data_ptr(), kr.stride(0),
-        kr.stride(1), k.shape[1], vr.data_ptr(), vr.stride(0), vr.stride(1), heads, dk, dv,
-        _ELEMENT[q.dtype], decay.data_ptr(), per_token,
-        None if state is None else state.data_ptr(), strides[0], strides[1],
-        0 if state is None else state.shape[0], None if index is None else index.data_ptr(),
-        cu.data_ptr(), requests, total, max_seqlen, scale, out.data_ptr(),
+        *args, cu.data_ptr(), requests, total, max_seqlen, scale, out.data_ptr(),
         None if ws is None else ws.data_ptr(), nbytes, _raw_stream(device),
     )
     return out
@@ -1622,22 +1622,16 @@ def linear_attention_step(
     ``state`` fp32 [slots, H, Dk, Dv] is updated in place.  Returns [B, H, Dv].
     """
     requests = q.shape[0]
-    qr, kr, vr, decay, per_token, strides, index = _linear_args(
+    (_, heads, dk, dv), args, held = _linear_args(
         q, k, v, log_decay, state, state_index, requests, expanded=True)
     device = q.device
-    _, heads, dv = v.shape
-    dk = q.shape[2]
     scale = _scale_of(scale, dk)
     out = torch.empty(requests, heads, dv, dtype=v.dtype, device=device)
     if requests == 0:
         return out
     _on(device)(
         "kb_linear_attention_step",
-        qr.data_ptr(), qr.stride(0), qr.stride(1), q.shape[1], kr.data_ptr(), kr.stride(0),
-        kr.stride(1), k.shape[1], vr.data_ptr(), vr.stride(0), vr.stride(1), heads, dk, dv,
-        _ELEMENT[q.dtype], decay.data_ptr(), per_token, state.data_ptr(), strides[0], strides[1],
-        state.shape[0], None if index is None else index.data_ptr(), requests, scale,
-        out.data_ptr(), _raw_stream(device),
+        *args, requests, scale, out.data_ptr(), _raw_stream(device),
     )
     return out
 
