@@ -73,7 +73,7 @@ def _p(tensor: torch.Tensor | None) -> c_void_p:
 
 
 def _require_cuda(tensor: torch.Tensor, what: str) -> None:
-    if tensor.device.type != "cuda":
+    if not tensor.is_cuda:
         raise ValueError(f"{what} requires CUDA")
 
 
