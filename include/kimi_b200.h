@@ -540,8 +540,10 @@ KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows
  * [tokens, H, Dv] contiguous; rows outside every request are zero, rows of a
  * request past max_tokens are not written.  A value that is no number reaches the
  * outputs of its own and later tokens only, there as not-a-number.
- * The workspace of kb_linear_attention_workspace_size bytes (often 0) may hold
- * anything, but is this call's alone until it is done on the stream.
+ * The workspace of kb_linear_attention_workspace_size bytes (0 but for bf16 and
+ * more than a few tokens), 16-byte aligned, may hold anything, but is this call's
+ * alone until it is done on the stream.  bf16 prompts run in chunks of 128 tokens
+ * on the tensor cores, other types token by token.
  * The step takes one token of each of B requests. */
 KB_API size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64_t Dk, int64_t Dv,
                    int dtype, int64_t total, int64_t max_tokens);
@@ -620,7 +622,8 @@ KB_API int kb_paged_copy(uint16_t* k_cache, const int64_t* k_strides, uint16_t* 
  * tokens, of which row r has those whose bits tree_mask[r] has, or without masks
  * its own and those before it; bias_ids [B, n_biases] (at most 4096), negative ids
  * unused.  Every pointer but logits and out may be NULL.  out may be logits, with
- * the same stride.  Token ids past V are skipped (device error bit 3). */
+ * the same stride.  Token ids past V are skipped (device error bit 3).  At most
+ * 65535 rows, or with cu_tokens, where a CTA takes several, 64 times as many. */
 KB_API int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t rows, int64_t V,
                    int dtype, void* out, int64_t out_stride, int64_t B, const int64_t* history,
                    int64_t history_stride, int64_t longest, const int32_t* history_lens,

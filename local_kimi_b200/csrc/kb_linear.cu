@@ -5,7 +5,12 @@
 // One token a request (decoding), or a few: the state is read once, updated in registers
 // and written once.  A CTA has a head's state, or, where there are few heads, 32 of its
 // columns (they are independent): 256 threads, four columns and Dk / 8 (Dk / 32) rows each.
-// The sums over the rows meet in shared memory, one barrier a token.
+// The sums over the rows meet in shared memory, one barrier a token.  Longer bf16 prompts go in
+// chunks (kb_linear_chunk.cu).
+//
+// Bound: HBM, the states read and written: 256 requests of 32 heads of 128 x 128 move 1.08 GB in
+// 177 us, 6.07 TB/s.  One request, 2.8 us (4 MB): a launch and one trip to memory.
+// The state, the sums and the products are fp32; an output is rounded once, when it is stored.
 #include "kb_linear.cuh"
 
 namespace kb {

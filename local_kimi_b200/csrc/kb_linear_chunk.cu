@@ -12,7 +12,8 @@
 //
 // One persistent CTA per SM; a unit is one head of one request (or of a segment of it), its
 // chunks one after the other.  Q, K and V tiles (128 rows, 64-element blocks in the 128-byte
-// swizzle) arrive by tensor copies in two stages.
+// swizzle) arrive by tensor copies in two or three stages.  A kernel before makes the decays of all
+// chunks and orders the requests.
 //
 //   warp 26: the units and the copies.
 //   warp 24: issues S = Q K^T, O = Q S (the state), O += P V.
@@ -21,15 +22,33 @@
 //     rows each); its bf16 copy is what Q S reads.
 //   warps 8-15: P from the scores, a row per thread and half the columns each; the part of the
 //     state scaled by exp(b_i) in tensor memory before P V is added to it; the outputs, which
-//     leave by tensor copies from the place of the chunk's values.
+//     leave by tensor copies from the place of the chunk's queries.
 //   warps 16-23: V', 32 rows at a time in two buffers, transposed on the way from shared to
 //     tensor memory (eight by eight pieces, ldmatrix and 16-lane stores).
+//
+// Few heads: a request is cut into segments, and a first pass over all but the last makes each
+// one's gain and decay alone (warps 0-7 hold it, 8-23 make V' in four buffers, nothing else
+// runs); the second starts each segment from the gains before it.
+//
+// Bound: not the memory (8192 tokens of 32 heads of 128 x 128 move 269 MB, 41 us) nor the tensor
+// cores (51 GFLOP a pass, three of six products the parts of V'; active 31 % of the second pass),
+// but a chunk's way from the scores over P and P V to the outputs: 6000 clocks of latencies in
+// one CTA an SM, since the state and two stages take the shared memory.  Roles on warps of their
+// own let the state, V' and the copies of other chunks run beside it.  The first pass takes 2200
+// clocks a chunk.  Measured, replayed: 106 us; 24 prompts of 1 to 2047 tokens with 24 heads
+// 128 x 64 on 4 of queries and keys 68 us (108 MB at least: 16.4).  Token by token: 10700 and
+// 2630.
+//
+// The code is in short loops, not unrolled: all roles together have to fit the instruction cache
+// (126 -> 111 us).  Slower: outputs by warps apart from the weights' (114 to 135 us, one barrier
+// and one exchange more in the chunk's way), prefetching stages into L2 (111).
 //
 // Roundings.  P and the copy of the state are rounded once to bf16 before they meet the values
 // and the queries: the outputs have 8 bits themselves.  The state must not lose bits: V' (fp32
 // products) enters the tensor cores as the sum of three bf16 values, 24 bits in all.
 //
-// 512 columns of tensor memory: scores and P 128, O 128, the state's gain 128, V' 2 x 48.
+// 512 columns of tensor memory: scores and P 128, O 128, the state's gain 128, V' 2 x 48, 64
+// apart (in the first pass 4 x 48 in the place of scores and O).
 //
 // A row past the request's end belongs to a neighbour: its keys and values are zeroed in shared
 // memory.  A value that is no number is zeroed too, since it would meet zero weights; the rows
@@ -96,11 +115,11 @@ struct ChunkShape {
   static constexpr bool STAGED = DKP >= DVP;
   static constexpr int BUFFERS = STATES ? 4 : 2;
   static constexpr uint32_t PARTS_AT = STATES ? 0 : 384;
-  static constexpr int FIT = (227 * 1024 - 3072 - STATE) / STAGE;
+  static constexpr int FIT = (224 * 1024 - STATE) / STAGE;
   static_assert(FIT >= 2, "stages");
   static constexpr int STAGES = FIT < MOST_STAGES ? FIT : MOST_STAGES;
   // (Three stages leave room for their arrays.)
-  static constexpr int FIXED = STAGES > 2 ? 4608 : 3072;
+  static constexpr int FIXED = STAGES > 2 ? 4608 : 3 * 1024;
   static constexpr int SMEM = STAGES * STAGE + STATE + FIXED;
 };
 
@@ -116,7 +135,7 @@ struct ChunkShared {
   uint32_t tmem;
   int abort_flag;
 };
-static_assert(sizeof(ChunkShared<2>) <= 3072 && sizeof(ChunkShared<3>) <= 4608, "shared memory");
+static_assert(sizeof(ChunkShared<2>) <= 3 * 1024 && sizeof(ChunkShared<3>) <= 4608, "shared memory");
 
 __device__ __forceinline__ void store_tile(const CUtensorMap* map, const void* from, int x, int y,
                                            int z) {

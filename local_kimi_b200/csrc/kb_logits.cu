@@ -21,10 +21,10 @@
 // 2^15 tokens, else 32.  Every slice reads the whole history again, from L2, by asynchronous
 // copies to places that the copying thread alone reads: 2048 tokens on their way.
 //
-// Measured, 163840 tokens in bf16, replayed: 256 rows 60.5 us (84 MB each way less what masks
-// leave out, 2.4 TB/s), with histories of 10 tokens 39, without any 31 (5.4 TB/s); one request
-// of nine drafted rows 10.6.  Slices of 16384 tokens and 512 threads: 61.0 (histories of 8000 tokens 78 instead
-// of 92, none 35 instead of 31).
+// Measured, 163840 tokens in bf16, replayed: 256 rows 60.5 us (176 MB less what masks leave out,
+// 2.9 TB/s), with histories of 10 tokens 39, without any 31 (5.4 TB/s); one request of nine
+// drafted rows 10.6.  Slices of 16384 tokens and 512 threads: 61.0 (histories of 8000 tokens 78
+// instead of 92, none 35 instead of 31).
 #include <algorithm>
 
 #include "kb_common.cuh"

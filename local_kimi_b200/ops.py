@@ -1579,6 +1579,10 @@ def linear_attention(
     negative slot, or no ``state``: S starts from zero and is not kept.  No two
     requests may name one slot.  Returns [tokens, H, Dv] of the inputs' type; rows
     outside every request are zero.
+
+    BF16 prompts of more than a few tokens run in chunks on the tensor cores (the weights
+    between tokens rounded to BF16, the state kept to FP32); FP16 and FP32 ones token by
+    token in FP32, which for long prompts takes a hundred times as long.
     """
     if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must have one entry more than there are requests")

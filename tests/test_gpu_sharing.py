@@ -226,6 +226,45 @@ def test_linear_attention_values_that_are_no_numbers(cuda, lens, which):
             assert torch.equal(state[~keep], clean_state[~keep])
 
 
+def test_linear_attention_no_numbers_in_every_chunk(cuda):
+    # Chunk after chunk with values that are no numbers, in one piece and in segments.
+    lens = [700]
+    for h in (2, 160):
+        q, k, v, g, s = linear_inputs(lens, h, 1, 1, 64, 128, torch.bfloat16, 14)
+        args = [x.to(cuda) for x in (q, k, v, g)]
+        state, bad_state = s.to(cuda), s.to(cuda)
+        clean = ops.linear_attention(*args, ints([0, 700], cuda), 700, state=state)
+        odd = {(3, 0, 5): NAN, (3, 1, 90): INF, (130, 0, 6): -INF, (131, 0, 6): NAN,
+               (140, 1, 5): NAN, (255, 0, 127): INF, (256, 1, 0): INF, (390, 0, 64): NAN,
+               (511, 0, 65): NAN, (512, 0, 66): NAN, (699, 1, 67): -INF}
+        hit = torch.zeros(700, h, 128, dtype=torch.bool, device=cuda)
+        for (t, head, col), value in odd.items():
+            args[2][t, head, col] = value
+            hit[t:, head, col] = True
+        out = ops.linear_attention(*args, ints([0, 700], cuda), 700, state=bad_state)
+        assert torch.equal(~torch.isfinite(out), hit)
+        assert torch.equal(out[~hit], clean[~hit])
+        gone = hit[-1][None, :, None, :].expand_as(state)
+        assert torch.equal(~torch.isfinite(bad_state), gone)
+        assert torch.equal(bad_state[~gone], state[~gone])
+
+
+@pytest.mark.parametrize("b,h,longest", [
+    (1, 4, 8), (1, 4, 9), (592, 4, 5), (592, 4, 6), (593, 4, 5), (593, 4, 6), (593, 4, 8),
+    (36, 2, 3), (37, 2, 3), (75, 1, 3),
+])
+def test_linear_attention_around_its_forms(cuda, b, h, longest):
+    # Lengths and heads where another kernel takes over: outputs within the wider tolerance.
+    lens = [longest - i % 3 if longest > 2 else longest for i in range(b)]
+    q, k, v, g, s = linear_inputs(lens, h, h, 1, 64, 64, torch.bfloat16, b + longest)
+    want, size, end, weight = ref.linear_attention(q, k, v, g, sums(lens), 0.125, s)
+    state = s.to(cuda)
+    out = ops.linear_attention(q.to(cuda), k.to(cuda), v.to(cuda), g.to(cuda),
+                               ints(sums(lens), cuda), longest, state=state)
+    assert_within(out, want, room_of(torch.bfloat16, want, size, longest, 64, True), "outputs")
+    assert_within(state, end, 6e-5 * weight, "state")
+
+
 def test_linear_attention_views(cuda):
     # Slices of one projection, a transposed batch, decays of another order, expanded tokens.
     gen = torch.Generator(device=cuda).manual_seed(8)
@@ -670,6 +709,41 @@ def test_adjust_logits_long_histories(cuda):
     many = torch.full((2, 4096), 7, dtype=torch.long, device=cuda)
     got = ops.adjust_logits(x, bias_ids=many, bias_values=torch.ones(2, 4096, device=cuda))
     assert got[:, 7].tolist() == [4096.0] * 2 and float(got.abs().sum()) == 2 * 4096
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_adjust_logits_of_many_rows(cuda, dtype):
+    # More wide parts of rows than SMs.
+    check_logits(cuda, 21, dtype, 80, 8_211, [1] * 80, longest=90)
+    check_logits(cuda, 22, dtype, 80, 8_211, [1] * 80, in_place=True, odd=True, offset=3)
+    check_logits(cuda, 23, dtype, 40, 8_211, [4] * 40, tree=True, in_place=True)
+
+
+@pytest.mark.parametrize("rows", [1, 160])
+def test_adjust_logits_history_lengths(cuda, rows):
+    # Every token named once or more, by histories that end around the parts they are read in.
+    v = 9_001
+    gen = torch.Generator(device=cuda).manual_seed(24)
+    x = torch.randn(rows, v, generator=gen, device=cuda).bfloat16()
+    order = torch.stack([torch.randperm(v, generator=gen, device=cuda) for _ in range(rows)])
+    rep = torch.full((rows,), 2.0, device=cuda)
+    for n in (1, 255, 256, 1023, 1024, 1025, 2047, 2048, 2049, 3073, 4097, 9_001):
+        got = ops.adjust_logits(x, history=order, history_lens=ints([n] * rows, cuda),
+                                repetition=rep)
+        named = torch.zeros_like(x, dtype=torch.bool).scatter_(1, order[:, :n], True)
+        assert torch.equal(got, torch.where(named, torch.where(x > 0, x / 2, x * 2), x)), n
+
+
+def test_adjust_logits_wide_counts_of_many_rows(cuda):
+    rows, v, n = 160, 8_200, 40_000
+    history = (torch.arange(n, device=cuda) % 8_193).expand(rows, n).contiguous()
+    lens = [n - 7 * r for r in range(rows)]
+    got = ops.adjust_logits(torch.zeros(rows, v, device=cuda), history=history,
+                            history_lens=ints(lens, cuda), prompt_lens=ints([5] * rows, cuda),
+                            frequency=torch.ones(rows, device=cuda))
+    for r in (0, 1, 77, 159):
+        want = torch.bincount(history[r, 5:lens[r]], minlength=v)
+        assert torch.equal(got[r], -want.float())
 
 
 def test_adjust_logits_far_offsets(cuda):
