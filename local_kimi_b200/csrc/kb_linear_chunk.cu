@@ -31,7 +31,7 @@
 // runs); the second starts each segment from the gains before it.
 //
 // Bound: not the memory (8192 tokens of 32 heads of 128 x 128 move 269 MB, 41 us) nor the tensor
-// cores (51 GFLOP a pass, three of six products the parts of V'; active 31 % of the second pass),
+// cores (51 GFLOP a pass, three of six products the parts of V'; active 39 % of the second pass),
 // but a chunk's way from the scores over P and P V to the outputs: 6000 clocks of latencies in
 // one CTA an SM, since the state and two stages take the shared memory.  Roles on warps of their
 // own let the state, V' and the copies of other chunks run beside it.  The first pass takes 2200
