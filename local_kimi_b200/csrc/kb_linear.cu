@@ -1,12 +1,13 @@
-// kb_linear.cu - linear attention with a decay for each head, token by token.
+// kb_linear.cu - linear attention with a decay for each head in fp32: token by token, and in
+// blocks of 32 tokens.
 //
 // For head h of a request, with the state S [Dk, Dv] in fp32:
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t
 // One token a request (decoding), or a few: the state is read once, updated in registers
 // and written once.  A CTA has a head's state, or, where there are few heads, 32 of its
 // columns (they are independent): 256 threads, four columns and Dk / 8 (Dk / 32) rows each.
-// The sums over the rows meet in shared memory, one barrier a token.  Longer bf16 prompts go in
-// chunks (kb_linear_chunk.cu).
+// The sums over the rows meet in shared memory, one barrier a token.  Longer prompts go in
+// blocks (below), bf16 ones in chunks on the tensor cores (kb_linear_chunk.cu).
 //
 // Bound: HBM, the states read and written: 256 requests of 32 heads of 128 x 128 move 1.08 GB in
 // 177 us, 6.07 TB/s.  One request, 2.8 us (4 MB): a launch and one trip to memory.
@@ -42,6 +43,17 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
     static_cast<uint16_t*>(p)[i] = (uint16_t)attn::pack2<TYPE == 1>(v, 0.f);
 }
 
+// Rows outside every request: zero.
+template <int TYPE>
+__device__ __forceinline__ void clear_outside(const Args& A) {
+  const int64_t lead = min(max((int64_t)A.cu[0], (int64_t)0), A.total);
+  const int64_t tail = min(max((int64_t)A.cu[A.B], lead), A.total);
+  const int64_t width = (int64_t)A.H * A.Dv, spare = (lead + A.total - tail) * width;
+  for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < spare;
+       i += (int64_t)gridDim.x * THREADS)
+    store1<TYPE>(A.out, i < lead * width ? i : i - lead * width + tail * width, 0.f);
+}
+
 // COLS: columns of a CTA, 128 or 32.
 template <int TYPE, int COLS>
 __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
@@ -58,15 +70,7 @@ __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
   pdl_wait();
   pdl_launch_dependents();
 
-  // Rows outside every request: zero.
-  if (A.cu != nullptr) {
-    const int64_t lead = min(max((int64_t)A.cu[0], (int64_t)0), A.total);
-    const int64_t tail = min(max((int64_t)A.cu[A.B], lead), A.total);
-    const int64_t width = (int64_t)A.H * A.Dv, spare = (lead + A.total - tail) * width;
-    for (int64_t i = (int64_t)blockIdx.x * THREADS + tid; i < spare;
-         i += (int64_t)gridDim.x * THREADS)
-      store1<TYPE>(A.out, i < lead * width ? i : i - lead * width + tail * width, 0.f);
-  }
+  if (A.cu != nullptr) clear_outside<TYPE>(A);
   int64_t first;
   const int n = request_tokens(A, b, first);
   if (n <= 0) return;
@@ -149,6 +153,199 @@ __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// f16 and f32 prompts, 32 tokens at a time in fp32.
+//
+// With b_i the running sum of the decays' logarithms in a block, for its rows i and j <= i:
+//   P_ij = (q_i . k_j) exp(b_i - b_j),  o_i = exp(b_i) q_i S + sum_j P_ij v_j
+//   S'   = exp(b_31) S + sum_j k_j exp(b_31 - b_j) v_j
+// The sums are in 64 bits: their differences decide small exponents next to large ones.  A CTA
+// has 32 columns of a head's state, in registers (16 rows of a column a thread) and, for q S, in
+// shared memory.  Bound: shared-memory loads, 12 for 32 products a warp while scores and q S are
+// made (the scores again for each 32 columns), and with one CTA an SM their latencies.  Measured,
+// 32 heads of 128 x 128: one f16 prompt of 8192 tokens 1.72 ms, 6.4 us a block (token by token
+// 10.7), f32 1.64 (6.1); 16 prompts of 512 tokens 1.1 ms, 5 us a block and SM.
+// ---------------------------------------------------------------------------
+
+constexpr int BLOCK = 32;
+constexpr int K_ROW = WIDEST + 4;            // (k by rows: 16-byte loads without conflicts)
+
+struct BlockShared {
+  float q[BLOCK][WIDEST], k[BLOCK][K_ROW], s[WIDEST][BLOCK], v[BLOCK][BLOCK], p[BLOCK][BLOCK];
+  double b[BLOCK];                           // the running sums
+  float start[BLOCK], rest[BLOCK];           // exp(b_i); exp(b_31 - b_j)
+  int since[BLOCK];                          // the last reset up to the row, plus 1; 0: none
+  int none;                                  // the first logarithm that is no number
+};
+
+// exp of a difference in 64 bits, to expf's accuracy.
+__device__ __forceinline__ float exp_of(double d) {
+  const float high = (float)d, e = expf(high);
+  return high > -104.f ? fmaf(e, (float)(d - (double)high), e) : e;
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(THREADS, 2) block_kernel(const Args A) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  BlockShared& B = *reinterpret_cast<BlockShared*>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int parts = (A.Dv + BLOCK - 1) / BLOCK;
+  const int part = blockIdx.x % parts, bh = blockIdx.x / parts;
+  const int b = bh / A.H, h = bh - b * A.H;
+  const int col = part * BLOCK + lane;       // of the state and of the outputs
+  const bool live = col < A.Dv;
+  constexpr int ROWS = WIDEST / (THREADS / 32);          // of the state, a warp
+  pdl_wait();
+  pdl_launch_dependents();
+  clear_outside<TYPE>(A);
+  int64_t first;
+  const int n = request_tokens(A, b, first);
+  if (n <= 0) return;
+  float* state = request_state(A, b, h);
+  float s[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int d = warp * ROWS + r;
+    s[r] = state != nullptr && live && d < A.Dk ? state[(int64_t)d * A.Dv + col] : 0.f;
+    B.s[d][lane] = s[r];
+  }
+  const int64_t kh = (int64_t)(h / A.k_group) * A.k_head, qh = (int64_t)(h / A.q_group) * A.q_head;
+  // The next block's rows, four of q and of k a warp; a piece of v a thread.
+  float4 q[4], k[4], v;
+  float g = 0.f;
+  const int v_row = tid / (BLOCK / 4), v_col = tid % (BLOCK / 4) * 4;
+  auto fetch = [&](int t0) {
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t t = first + t0 + warp + 8 * u;
+      const bool real = t0 + warp + 8 * u < n && lane * 4 < A.Dk;
+      q[u] = real ? load4<TYPE>(A.q, t * A.q_tok + qh + lane * 4) : zero;
+      k[u] = real ? load4<TYPE>(A.k, t * A.k_tok + kh + lane * 4) : zero;
+    }
+    v = t0 + v_row < n && part * BLOCK + v_col < A.Dv
+            ? load4<TYPE>(A.v, (first + t0 + v_row) * A.v_tok + (int64_t)h * A.v_head +
+                                   part * BLOCK + v_col)
+            : zero;
+    if (warp == 0)
+      g = t0 + lane < n ? __ldg(A.decay + (first + t0 + lane) * A.decay_tok + h) : 0.f;
+  };
+  fetch(0);
+#pragma unroll 1
+  for (int t0 = 0; t0 < n; t0 += BLOCK) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float4 x = make_float4(q[u].x * A.scale, q[u].y * A.scale, q[u].z * A.scale,
+                                   q[u].w * A.scale);
+      *reinterpret_cast<float4*>(&B.q[warp + 8 * u][lane * 4]) = x;
+      *reinterpret_cast<float4*>(&B.k[warp + 8 * u][lane * 4]) = k[u];
+    }
+    *reinterpret_cast<float4*>(&B.v[v_row][v_col]) = v;
+    if (warp == 0) {
+      // A decay that is 0 in fp32 is a reset; it counts as such, not in the sums.
+      const float x = decay_of(g);
+      const unsigned resets = __ballot_sync(0xffffffffu, x <= -104.f);
+      const unsigned odd = __ballot_sync(0xffffffffu, x != x);
+      double sum = x <= -104.f ? 0.0 : (double)x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double before = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += before;
+      }
+      const unsigned up = resets & (0xffffffffu >> (31 - lane));
+      const int since = up ? 32 - __clz(up) : 0, last = resets ? 32 - __clz(resets) : 0;
+      const double all = __shfl_sync(0xffffffffu, sum, 31);
+      const int none = odd ? __ffs(odd) - 1 : BLOCK;
+      B.b[lane] = sum;
+      B.since[lane] = since;
+      B.start[lane] = lane >= none ? NAN : since ? 0.f : exp_of(sum);
+      B.rest[lane] = none < BLOCK ? NAN : lane + 1 < last ? 0.f : exp_of(all - sum);
+      if (lane == 0) B.none = none;
+    }
+    __syncthreads();
+    if (t0 + BLOCK < n) fetch(t0 + BLOCK);
+    // A warp's four rows: scores with key `lane`, and q S in column `lane`.
+    const int i0 = warp * 4;
+    float score[4] = {}, o[4] = {};
+#pragma unroll 4
+    for (int d = 0; d < A.Dk; d += 4) {
+      const float4 kk = *reinterpret_cast<const float4*>(&B.k[lane][d]);
+      const float s0 = B.s[d][lane], s1 = B.s[d + 1][lane], s2 = B.s[d + 2][lane],
+                  s3 = B.s[d + 3][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float4 qq = *reinterpret_cast<const float4*>(&B.q[i0 + r][d]);
+        score[r] = fmaf(qq.w, kk.w, fmaf(qq.z, kk.z, fmaf(qq.y, kk.y, fmaf(qq.x, kk.x, score[r]))));
+        o[r] = fmaf(qq.w, s3, fmaf(qq.z, s2, fmaf(qq.y, s1, fmaf(qq.x, s0, o[r]))));
+      }
+    }
+    const int none = B.none;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = i0 + r;
+      float w = 0.f;
+      if (lane <= i) w = i >= none ? NAN : lane + 1 < B.since[i] ? 0.f : exp_of(B.b[i] - B.b[lane]);
+      B.p[i][lane] = lane <= i ? score[r] * w : 0.f;
+      o[r] *= B.start[i];
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int j = 0; j < i0; ++j) {
+      const float x = B.v[j][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = fmaf(B.p[i0 + r][j], x, o[r]);
+    }
+    // (Values behind a row do not meet its zero weights: they may be no numbers.)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = B.v[i0 + j][lane];
+#pragma unroll
+      for (int r = j; r < 4; ++r) o[r] = fmaf(B.p[i0 + r][i0 + j], x, o[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (live && t0 + i0 + r < n)
+        store1<TYPE>(A.out, ((first + t0 + i0 + r) * A.H + h) * A.Dv + col, o[r]);
+    const float keep = B.start[BLOCK - 1];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) s[r] *= keep;
+    const int real = min(n - t0, BLOCK);
+#pragma unroll 2
+    for (int j = 0; j < real; ++j) {
+      const float x = B.v[j][lane] * B.rest[j];
+#pragma unroll
+      for (int r = 0; r < ROWS; r += 4) {
+        const float4 kk = *reinterpret_cast<const float4*>(&B.k[j][warp * ROWS + r]);
+        s[r] = fmaf(kk.x, x, s[r]);
+        s[r + 1] = fmaf(kk.y, x, s[r + 1]);
+        s[r + 2] = fmaf(kk.z, x, s[r + 2]);
+        s[r + 3] = fmaf(kk.w, x, s[r + 3]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) B.s[warp * ROWS + r][lane] = s[r];
+  }
+  if (state != nullptr && live)
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int d = warp * ROWS + r;
+      if (d < A.Dk) state[(int64_t)d * A.Dv + col] = s[r];
+    }
+}
+
+template <int TYPE>
+static int launch_blocks(const Args& A, void* stream) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(block_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)sizeof(BlockShared));
+  KB_REQUIRE(e == cudaSuccess, KB_ERR_DEVICE, "linear attention: shared-memory limit: %s",
+             cudaGetErrorString(e));
+  const int64_t ctas = (int64_t)A.B * A.H * ((A.Dv + BLOCK - 1) / BLOCK);
+  return launch(block_kernel<TYPE>, dim3((unsigned)ctas), dim3(THREADS), sizeof(BlockShared),
+                stream, A);
+}
+
 template <int TYPE>
 static int launch_tokens(const Args& A, int sms, void* stream) {
   const int64_t heads = (int64_t)A.B * A.H;
@@ -219,7 +416,7 @@ static Args arguments(const void* q, int64_t q_tok, int64_t q_head, int64_t Hq, 
   return A;
 }
 
-// Token by token for a few tokens, and for types that the tensor cores' form does not take.
+// On the tensor cores: bf16 prompts of more than a few tokens.
 // (32 heads, token by token and in chunks: 1 request of 8 tokens 8.5 and 11.2 us, of 16 14.5 and
 // 11.2; 16 requests of 8 tokens 25 and 32, of 16 42 and 32; 256 requests of 4 tokens 308 and 376,
 // of 8 463 and 381.)
@@ -228,6 +425,15 @@ static bool in_chunks(int dtype, int64_t heads, int64_t longest, int sms) {
 }
 
 static int run_tokens(const Args& A, int dtype, int sms, void* stream) {
+  // Blocks of 32 tokens: from 13 on where each SM has a CTA at most, else from 41.  (32 heads of
+  // 128 x 128, token by token and in blocks: 1 request of 12 tokens f16 11.5 and 8.1 us, f32 8.4
+  // and 8.1; of 32 26 and 9, 17 and 9; 16 requests of 32 tokens f16 74 and 81, f32 69 and 82; 256
+  // requests of 32 f16 1396 and 1260, f32 1082 and 1300.)
+  const bool few = (int64_t)A.B * A.H * ((A.Dv + BLOCK - 1) / BLOCK) <= sms;
+  if (A.cu != nullptr && A.longest > (few ? 12 : 40)) {
+    if (dtype == 1) return launch_blocks<1>(A, stream);
+    if (dtype == 2) return launch_blocks<2>(A, stream);
+  }
   if (dtype == 0) return launch_tokens<0>(A, sms, stream);
   if (dtype == 1) return launch_tokens<1>(A, sms, stream);
   return launch_tokens<2>(A, sms, stream);

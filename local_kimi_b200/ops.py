@@ -1581,8 +1581,8 @@ def linear_attention(
     outside every request are zero.
 
     BF16 prompts of more than a few tokens run in chunks on the tensor cores (the weights
-    between tokens rounded to BF16, the state kept to FP32); FP16 and FP32 ones token by
-    token in FP32, which for long prompts takes a hundred times as long.
+    between tokens rounded to BF16, the state kept to FP32); FP16 and FP32 ones in FP32, which
+    for long prompts takes ten to twenty times as long.
     """
     if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must have one entry more than there are requests")

@@ -226,6 +226,59 @@ def test_linear_attention_values_that_are_no_numbers(cuda, lens, which):
             assert torch.equal(state[~keep], clean_state[~keep])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_linear_attention_in_blocks(cuda, dtype):
+    # Resets, decays above 1 and far apart, in and across blocks of 32 tokens.
+    for lens, h, dk, dv in (([9, 100, 0, 31, 33], 3, 64, 40), ([200], 1, 128, 128)):
+        q, k, v, g, s = linear_inputs(lens, h, h, 1, dk, dv, dtype, 17)
+        check_linear(cuda, q, k, v, g, s, lens)
+        g[::5] = 2.0
+        g[7::31, 0] = -INF
+        g[33::40] = -150.0
+        g[34::9] = -80.0
+        g[64] = -INF
+        check_linear(cuda, q, k, v, g, s, lens)
+    check_linear(cuda, q, k, v, torch.full((200, 1), -103.9), s, lens)
+    check_linear(cuda, q, k, v, torch.full((200, 1), -104.1), s, lens)
+    check_linear(cuda, q, k, v, torch.zeros(200, 1), s, lens)
+
+
+@pytest.mark.parametrize("which", ["v", "k", "q", "g"])
+def test_linear_attention_no_numbers_in_blocks(cuda, which):
+    lens = [70, 50]
+    q, k, v, g, s = linear_inputs(lens, 2, 2, 2, 64, 64, torch.float32, 18)
+    clean, clean_state = check_linear(cuda, q, k, v, g, s, lens)
+    for at in (0, 30, 31, 32, 45, 69):
+        for bad in (NAN, INF):
+            args = dict(q=q.clone(), k=k.clone(), v=v.clone(), g=g.clone())
+            args[which][(at, 0, 5) if which != "g" else (at, 0)] = NAN if which == "g" else bad
+            state = s.to(cuda)
+            out = ops.linear_attention(*(args[x].to(cuda) for x in "qkvg"),
+                                       ints(sums(lens), cuda), max(lens), state=state)
+            hit = torch.zeros(120, 2, 64, dtype=torch.bool, device=cuda)
+            cols = slice(5, 6) if which == "v" else slice(None)
+            hit[at:(at + 1 if which == "q" else 70), 0, cols] = True
+            assert torch.equal(~torch.isfinite(out), hit)
+            assert torch.equal(out[~hit], clean[~hit])
+            keep = torch.zeros_like(state, dtype=torch.bool)
+            if which == "v":
+                keep[0, 0, :, 5] = True
+            elif which == "k":
+                keep[0, 0, 5] = True
+            elif which == "g":
+                keep[0, 0] = True
+            assert torch.equal(~torch.isfinite(state), keep)
+            assert torch.equal(state[~keep], clean_state[~keep])
+
+
+def test_linear_attention_blocks_of_many_heads(cuda):
+    # Around the lengths from which blocks are used, with more CTAs than SMs and fewer.
+    for dtype in (torch.float16, torch.float32):
+        for lens, h in (([12, 5], 9), ([13, 5], 9), ([40, 7] * 3, 32), ([41, 7] * 3, 32)):
+            q, k, v, g, s = linear_inputs(lens, h, h, h, 16, 64, dtype, 19)
+            check_linear(cuda, q, k, v, g, s, lens)
+
+
 def test_linear_attention_no_numbers_in_every_chunk(cuda):
     # Chunk after chunk with values that are no numbers, in one piece and in segments.
     lens = [700]
