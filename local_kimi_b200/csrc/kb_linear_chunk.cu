@@ -35,7 +35,7 @@
 // but a chunk's way from the scores over P and P V to the outputs: 6000 clocks of latencies in
 // one CTA an SM, since the state and two stages take the shared memory.  Roles on warps of their
 // own let the state, V' and the copies of other chunks run beside it.  The first pass takes 2200
-// clocks a chunk.  Measured, replayed: 106 us; 24 prompts of 1 to 2047 tokens with 24 heads
+// clocks a chunk.  Measured, replayed: 102 us; 24 prompts of 1 to 2047 tokens with 24 heads
 // 128 x 64 on 4 of queries and keys 68 us (108 MB at least: 16.4).  Token by token: 10700 and
 // 2630.
 //
@@ -87,11 +87,17 @@ static_assert(sizeof(Decays) % 16 == 0, "bulk copies");
 struct ChunkArgs {
   Args a;
   Decays* decays;                            // [chunks][H], place_of() chunks
-  const int* order;                          // requests, longest first; NULL: units by number
+  int* order;                                // requests, longest first; NULL: units by number
   int* taken;                                // with it: units taken beyond each CTA's first
   int segments, segment;                     // of a request at most; tokens of one
   float* sums;                               // [B][segments][H][DKP][DVP]: a segment's gain
   float* keeps;                              // [B][segments][H]: its decay
+  // In the place of a request's last segment's gain, which nobody starts from: the state that a
+  // request of several segments starts from.  (Its last segment may be done, and its state
+  // written, before another one begins.)
+  __device__ __forceinline__ float* kept(int b, int h, int unit) const {
+    return sums + (((int64_t)b * segments + segments - 1) * a.H + h) * unit;
+  }
 };
 
 struct Item {
@@ -99,7 +105,8 @@ struct Item {
   int n;                                     // its tokens, -1: the end
   int64_t place;                             // of its decays
   int b, h, seg;
-  int starts, ends;                          // the unit's first, last chunk; 2: the request's
+  int starts;                                // the unit's first chunk; 2: of several segments
+  int ends;                                  // the unit's last chunk; 2: the request's
   int odd;                                   // values that are no numbers
 };
 
@@ -242,7 +249,7 @@ struct Items {
       end = min(last, at + C.segment);
       // The last segment's gain is nobody's start.
       if (states && end >= last) end = at;
-      next.starts = 1;
+      next.starts = n > C.segment ? 2 : 1;
     }
     next.first = at;
     next.n = (int)min(end - at, (int64_t)CHUNK);
@@ -253,7 +260,8 @@ struct Items {
 };
 
 // ---------------------------------------------------------------------------
-// The decays of every chunk, a warp a chunk and head; the last CTA orders the requests.
+// The decays of every chunk, a warp a chunk and head; the last CTA orders the requests, or the
+// last ones copy states.
 // (A warp of the chunks' kernel that made them beside its other work took 5000 to 8000 clocks a
 // chunk, more than the chunk: 8192 tokens x 32 heads 122 us.)
 // ---------------------------------------------------------------------------
@@ -336,15 +344,41 @@ __device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n
   }
 }
 
+template <bool SEGMENTS>                     // (their copies' registers cost the others 2 us)
 __global__ void __launch_bounds__(PREPARE_THREADS)
-    prepare_kernel(const Args A, Decays* decays, int64_t places, int* order, int* taken) {
+    prepare_kernel(const ChunkArgs C, int64_t places, int unit) {
+  const Args& A = C.a;
   constexpr int BUCKETS = 4 * PREPARE_THREADS;
   __shared__ int starts[BUCKETS];
   __shared__ int sums[PREPARE_THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_launch_dependents();
-  if (order == nullptr || blockIdx.x + 1 < gridDim.x) {
+  const int64_t rest = (int64_t)blockIdx.x - (places * A.H + PREPARE_THREADS / 32 - 1) /
+                                                 (PREPARE_THREADS / 32);
+  if (SEGMENTS && rest >= 0) {
+    // A CTA a head: the states that segments start from.
+    const int b = (int)(rest / A.H), h = (int)(rest - (int64_t)b * A.H);
+    int64_t first;
+    const float* from = request_state(A, b, h);
+    if (from == nullptr || request_tokens(A, b, first) <= C.segment) return;
+    float* to = C.kept(b, h, unit);
+    constexpr int AT_ONCE = 16;
+    static_assert(AT_ONCE * PREPARE_THREADS * 4 >= 128 * 128, "a state");
+    float4 x[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = (tid + u * PREPARE_THREADS) * 4;
+      if (i < A.Dk * A.Dv) x[u] = __ldcg(reinterpret_cast<const float4*>(from + i));
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = (tid + u * PREPARE_THREADS) * 4;
+      if (i < A.Dk * A.Dv) *reinterpret_cast<float4*>(to + i) = x[u];
+    }
+    return;
+  }
+  if (rest < 0) {
     const int64_t at = (int64_t)blockIdx.x * (PREPARE_THREADS / 32) + warp;
     if (at >= places * A.H) return;
     const int64_t place = at / A.H;
@@ -362,7 +396,7 @@ __global__ void __launch_bounds__(PREPARE_THREADS)
     const int n = request_tokens(A, lo, first);
     const int64_t skip = (place - place_of(first, lo)) * CHUNK;
     if (skip < 0 || skip >= n) return;
-    chunk_decays(A, first + skip, (int)min(n - skip, (int64_t)CHUNK), h, decays + at);
+    chunk_decays(A, first + skip, (int)min(n - skip, (int64_t)CHUNK), h, C.decays + at);
     return;
   }
   // Requests by number of chunks, most first; the longest ones together.
@@ -371,7 +405,7 @@ __global__ void __launch_bounds__(PREPARE_THREADS)
     const int n = request_tokens(A, b, first);
     return BUCKETS - 1 - min((n + CHUNK - 1) / CHUNK, BUCKETS - 1);
   };
-  if (tid == 0) *taken = 0;
+  if (tid == 0) *C.taken = 0;
   for (int i = tid; i < BUCKETS; i += PREPARE_THREADS) starts[i] = 0;
   __syncthreads();
   for (int b = tid; b < A.B; b += PREPARE_THREADS) atomicAdd(&starts[bucket(b)], 1);
@@ -394,7 +428,7 @@ __global__ void __launch_bounds__(PREPARE_THREADS)
     in += mine[i];
   }
   __syncthreads();
-  for (int b = tid; b < A.B; b += PREPARE_THREADS) order[atomicAdd(&starts[bucket(b)], 1)] = b;
+  for (int b = tid; b < A.B; b += PREPARE_THREADS) C.order[atomicAdd(&starts[bucket(b)], 1)] = b;
 }
 
 template <int DKP, int DVP, bool STATES>
@@ -524,6 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!STATES) {
           const float* from = request_state(A, b, h);
           if (from != nullptr && rows > 0) {
+            if (starts == 2) from = C.kept(b, h, DKP * DVP);
             from += (int64_t)part * HALF * A.Dv + dv;
 #pragma unroll
             for (int c = 0; c < HALF; c += 8, from += 8 * A.Dv) {
@@ -1043,7 +1078,7 @@ static int64_t padded(int64_t width) { return width <= 64 ? 64 : 128; }
 // costs START beside its chunks, each segment's gain that it starts from GAIN; a segment but
 // the last is read twice, for its gain (half a chunk's cost) and its outputs.  (One request of 32
 // heads, in the segments chosen and whole: 512 tokens 20 us both, 1024 27 and 31, 2048 39 and 53,
-// 8192 106 and 190; 8 heads, 8192 tokens: 48 and 184.)
+// 8192 102 and 190; 8 heads, 8192 tokens: 48 and 184.)
 static void segments_of(int64_t heads, int64_t longest, int sms, int& segments, int& segment) {
   constexpr double START = 2.0, GAIN = 0.4;
   const int64_t chunks = (longest + CHUNK - 1) / CHUNK;
@@ -1126,8 +1161,11 @@ int launch_chunks(const Args& A, int64_t Hq, int64_t Hk, int sms, void* workspac
     st = attn::make_map_4d(&mo, A.out, 0, {A.Dv, A.H, A.total, 1},
                            {A.Dv, (int64_t)A.H * A.Dv, 8}, 1, 32, A.Dv <= 64 ? 32 : 64);
   if (st != KB_OK) return st;
-  st = launch(prepare_kernel, dim3((unsigned)(ctas + (L.order ? 1 : 0))), dim3(PREPARE_THREADS), 0,
-              stream, A, C.decays, L.places, L.order ? C.taken + 1 : nullptr, C.taken);
+  // Beside the decays: the order, or the states that segments start from.
+  const int64_t more = L.order ? 1 : L.segments > 1 && A.state ? (int64_t)A.B * A.H : 0;
+  st = launch(L.segments > 1 ? prepare_kernel<true> : prepare_kernel<false>,
+              dim3((unsigned)(ctas + more)), dim3(PREPARE_THREADS), 0, stream, C, L.places,
+              (int)(padded(A.Dk) * padded(A.Dv)));
   const int grid = (int)std::min<int64_t>((int64_t)A.B * C.segments * A.H, sms);
   for (int pass = C.segments > 1 ? 0 : 1; pass < 2 && st == KB_OK; ++pass) {
     const bool states = pass == 0;

@@ -111,6 +111,14 @@ def test_linear_attention_in_segments(cuda):
         check_linear(cuda, q, k, v, g * 0.05, s, lens)
 
 
+def test_linear_attention_segments_in_turns(cuda):
+    # More segments than SMs, of requests so uneven that a request's last one is done before its
+    # first has begun: that one still starts from the state as it was.
+    lens = [6144] + [100] * 7 + [5130] * 3 + [10] * 3
+    q, k, v, g, s = linear_inputs(lens, 4, 1, 4, 64, 64, torch.bfloat16, 6)
+    check_linear(cuda, q, k, v, g * 0.002, s, lens)
+
+
 def test_linear_attention_many_units(cuda):
     # More units than SMs: a CTA goes through several.
     lens = [3, 140, 0, 260, 1] * 5
