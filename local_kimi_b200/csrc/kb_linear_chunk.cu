@@ -1077,8 +1077,8 @@ static int64_t padded(int64_t width) { return width <= 64 ? 64 : 128; }
 // Segments of a request: as many as make the longest way of a CTA shortest, in chunks.  A unit
 // costs START beside its chunks, each segment's gain that it starts from GAIN; a segment but
 // the last is read twice, for its gain (half a chunk's cost) and its outputs.  (One request of 32
-// heads, in the segments chosen and whole: 512 tokens 20 us both, 1024 27 and 31, 2048 39 and 53,
-// 8192 102 and 190; 8 heads, 8192 tokens: 48 and 184.)
+// heads, in the segments chosen and whole: 512 tokens 20 us both, 1024 29 and 31, 2048 40 and 53,
+// 8192 102 and 190; 8 heads, 8192 tokens: 49 and 184.)
 static void segments_of(int64_t heads, int64_t longest, int sms, int& segments, int& segment) {
   constexpr double START = 2.0, GAIN = 0.4;
   const int64_t chunks = (longest + CHUNK - 1) / CHUNK;
