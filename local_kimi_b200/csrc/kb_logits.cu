@@ -506,8 +506,13 @@ extern "C" int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t 
                  (cu_tokens || B <= rows),
              KB_ERR_NULL_POINTER, "adjust logits: NULL pointer");
   const size_t size = dtype == 2 ? 4 : 2;
-  KB_REQUIRE((((uintptr_t)logits | (uintptr_t)out) & (size - 1)) == 0, KB_ERR_ALIGNMENT,
-             "adjust logits: unaligned pointer");
+  KB_REQUIRE((((uintptr_t)logits | (uintptr_t)out) & (size - 1)) == 0 &&
+                 (((uintptr_t)history | (uintptr_t)bias_ids | (uintptr_t)tokens |
+                   (uintptr_t)tree_mask) & 7) == 0 &&
+                 (((uintptr_t)history_lens | (uintptr_t)prompt_lens | (uintptr_t)repetition |
+                   (uintptr_t)presence | (uintptr_t)frequency | (uintptr_t)bias_values |
+                   (uintptr_t)allowed | (uintptr_t)cu_tokens) & 3) == 0,
+             KB_ERR_ALIGNMENT, "adjust logits: unaligned pointer");
   const int dev = kb::bind_stream_device(stream);
   lg::Args A = {};
   A.x = static_cast<const uint8_t*>(logits);

@@ -648,7 +648,6 @@ extern "C" int kb_paged_compact(const int32_t* reserved_lens, int64_t B,
   A.map = scratch;
   A.err = kb::device_error_word(dev);
   KB_REQUIRE(A.err != nullptr, KB_ERR_LAUNCH, "device error word unavailable");
-  // A list of fewer free pages than it has places: the pool is small against the bitmaps.
   const int ctas = pg::pool_ctas(B, table_width, n_pages);
   const size_t W = (size_t)(n_pages + 31) / 32, per = (W + ctas - 1) / ctas;
   return pg::launch_cluster(pg::compact_kernel, (2 * W + 2 * per) * 4, ctas, stream, A);

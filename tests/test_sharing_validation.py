@@ -278,6 +278,16 @@ def test_c_checks(library):
     assert adjust(x=ctypes.c_void_p((1 << 20) + 2)) == 4
 
 
+def test_c_checks_of_alignment(library):
+    at = lambda n: ctypes.c_void_p((1 << 20) + n)  # noqa: E731
+    adjust = lambda history=at(0), lens=at(0), ids=at(0), allowed=at(0): (  # noqa: E731
+        library.kb_adjust_logits(at(0), 40, 2, 40, 2, at(0), 40, 3, history, 9, 9, lens, None, None,
+                                 None, None, ids, 4, at(0), 4, 4, allowed, 2, at(0), None, None,
+                                 None))
+    assert adjust(history=at(4)) == 4 and adjust(ids=at(4)) == 4
+    assert adjust(lens=at(2)) == 4 and adjust(allowed=at(1)) == 4
+
+
 def test_the_definitions_themselves():
     # The oracle against closed forms.
     q = torch.ones(3, 1, 8)
