@@ -572,7 +572,8 @@ KB_API int kb_linear_attention_step(const void* q, int64_t q_token_stride, int64
  * copy_from, copy_to [n] (-1: nothing to copy) and copy_rows [n].  A pair without
  * a page leaves its target empty; *missing counts those.  Pairs with a negative
  * row are skipped, those whose target is a source, named before or past the table
- * too (device error bit 2).  B, n <= 12288. */
+ * too (device error bit 2).  Here and below free_head_out is another place than
+ * free_head, and lists written are others than those read.  B, n <= 12288. */
 KB_API int kb_paged_fork(int32_t* context_lens, int32_t* reserved_lens, int64_t B,
                    int32_t* block_table, int64_t table_stride, int64_t table_width,
                    const int32_t* sources, const int32_t* targets, int64_t n,
