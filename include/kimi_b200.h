@@ -622,9 +622,10 @@ KB_API int kb_paged_copy(uint16_t* k_cache, const int64_t* k_strides, uint16_t* 
  * int64, of which history_lens[b] count; tokens [rows] (with cu_tokens): drafted
  * tokens, of which row r has those whose bits tree_mask[r] has, or without masks
  * its own and those before it; bias_ids [B, n_biases] (at most 4096), negative ids
- * unused.  Every pointer but logits and out may be NULL.  out may be logits, with
- * the same stride.  Token ids past V are skipped (device error bit 3).  At most
- * 65535 rows, or with cu_tokens, where a CTA takes several, 64 times as many. */
+ * unused; allowed [rows, (V + 31) / 32].  Rows of history, biases and allowed may share
+ * memory (stride 0: one row for all).  Every pointer but logits and out may be NULL.  out
+ * may be logits, with the same stride.  Token ids past V are skipped (device error bit 3).
+ * At most 65535 rows, or with cu_tokens, where a CTA takes several, 64 times as many. */
 KB_API int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t rows, int64_t V,
                    int dtype, void* out, int64_t out_stride, int64_t B, const int64_t* history,
                    int64_t history_stride, int64_t longest, const int32_t* history_lens,

@@ -53,7 +53,7 @@ struct Args {
   const float* bias_values;
   int64_t ids_row, values_row;
   int biases;
-  const uint32_t* allowed;                   // [rows, words]
+  const uint32_t* allowed;                   // [rows, words], of any stride: rows may share them
   int64_t allowed_row;
   const int* cu;                             // NULL: row b is request b's
   const int64_t* tokens;                     // drafted tokens, with cu
@@ -492,7 +492,7 @@ extern "C" int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t 
   namespace lg = kb::logits;
   kb::clear_error();
   KB_REQUIRE(rows >= 0 && V > 0 && B >= 0 && longest >= 0 && n_biases >= 0 && row_stride >= V &&
-                 out_stride >= V && (!allowed || allowed_stride >= (V + 31) / 32),
+                 out_stride >= V && (!allowed || allowed_stride >= 0),
              KB_ERR_BAD_SHAPE, "adjust logits: bad shape");
   KB_REQUIRE(dtype >= 0 && dtype <= 2, KB_ERR_UNSUPPORTED, "adjust logits: unknown element type");
   KB_REQUIRE(V < ((int64_t)1 << 30) && B < 65535 && longest < ((int64_t)1 << 30) &&

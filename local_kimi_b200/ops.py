@@ -1901,7 +1901,8 @@ def adjust_logits(
       -infinity where its bit (``t % 32`` of word ``t // 32``) is not set in the row of
       ``allowed`` (int32 [rows, (V + 31) // 32])
 
-    Parameters are fp32 [B].  Negative tokens and ids are skipped.  A row whose mask allows
+    Parameters are fp32 [B].  Histories, biases and masks may be expanded (one row for all).
+    Negative tokens and ids are skipped.  A row whose mask allows
     nothing is -infinity throughout; rows outside every request are passed on as they are.
     ``out`` may be ``logits`` itself; then what does not change is neither read nor written.
     """
@@ -1987,7 +1988,7 @@ def adjust_logits(
         None if ids is None else ids.data_ptr(), 0 if ids is None else ids.stride(0),
         None if values is None else values.data_ptr(), 0 if values is None else values.stride(0),
         biases, None if words is None else words.data_ptr(),
-        0 if words is None else max(words.stride(0), words.shape[1]),
+        0 if words is None else words.stride(0),
         None if cu is None else cu.data_ptr(), None if tok is None else tok.data_ptr(),
         None if mask is None else mask.data_ptr(), _raw_stream(device),
     )

@@ -751,6 +751,30 @@ def test_adjust_logits_of_unaligned_rows(cuda):
     assert not target[:, :500].any() and not target[:, 2500:].any()
 
 
+def test_adjust_logits_of_expanded_rows(cuda):
+    # One grammar, one history and one list of biases for all rows.
+    gen = torch.Generator(device=cuda).manual_seed(30)
+    for rows, v in ((8, 100), (160, 8_201)):
+        x = torch.randn(rows, v, generator=gen, device=cuda).bfloat16()
+        words = torch.randint(-2 ** 31, 2 ** 31, (1, (v + 31) // 32), generator=gen,
+                              device=cuda).int()
+        history = torch.randint(0, v, (1, 50), generator=gen, device=cuda)
+        ids = torch.randint(0, v, (1, 6), generator=gen, device=cuda)
+        values = torch.randn(1, 6, generator=gen, device=cuda)
+        other = dict(history_lens=ints([50 - r % 7 for r in range(rows)], cuda),
+                     frequency=torch.full((rows,), 0.5, device=cuda))
+        one = dict(history=history, bias_ids=ids, bias_values=values, allowed=words)
+        spread = {k: t.expand(rows, -1) for k, t in one.items()}
+        copies = {k: t.contiguous() for k, t in spread.items()}
+        want = ops.adjust_logits(x, **copies, **other)
+        assert torch.equal(ops.adjust_logits(x, **spread, **other), want)
+        y = x.clone()
+        assert torch.equal(ops.adjust_logits(y, **spread, **other, out=y), want)
+        open_ = (words[0, torch.arange(v, device=cuda) // 32]
+                 >> (torch.arange(v, device=cuda) % 32)) & 1
+        assert torch.equal(torch.isinf(want), (open_ == 0).expand(rows, v))
+
+
 def test_adjust_logits_long_histories(cuda):
     # Counts far above 16 bits, histories longer than the columns say, ids past the vocabulary.
     _lib.device_errors()

@@ -234,6 +234,38 @@ def test_adjust_logits_refusals(any_device):
         run(both[:80].view(2, 40), out=both[10:90].view(2, 40))
 
 
+@pytest.fixture()
+def c_calls(monkeypatch, any_device):
+    # The arguments that reach the C entries, of CPU tensors.
+    calls: list = []
+    monkeypatch.setattr(ops, "_on", lambda device: lambda *args: calls.append(args))
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    return calls
+
+
+def test_rows_that_share_memory_keep_their_stride(c_calls):
+    # One grammar, one history, one list of biases for all rows: their rows stay where they are.
+    x, lens = torch.zeros(8, 100), i32(*[3] * 8)
+    one = lambda width, dtype: torch.zeros(1, width, dtype=dtype)  # noqa: E731
+    history, ids, values = one(5, torch.long), one(7, torch.long), one(7, torch.float32)
+    words = one(4, torch.int32)
+    spread = lambda t: t.expand(8, t.shape[1])  # noqa: E731
+    ops.adjust_logits(x, history=spread(history), history_lens=lens, bias_ids=spread(ids),
+                      bias_values=spread(values), allowed=spread(words))
+    # Rows that overlap (one word further each), and rows of a wider matrix.
+    sliding = torch.zeros(11, dtype=torch.int32).as_strided((8, 4), (1, 1))
+    ops.adjust_logits(x, allowed=sliding)
+    wide = torch.zeros(8, 9, dtype=torch.int32)[:, 2:6]
+    ops.adjust_logits(x, allowed=wide)
+    for args, held, stride in ((c_calls[0], words, 0), (c_calls[1], sliding, 1),
+                               (c_calls[2], wide, 9)):
+        assert args[0] == "kb_adjust_logits"
+        at = args.index(held.data_ptr())
+        assert args[at + 1] == stride
+    for t, stride_at in ((history, 1), (ids, 1), (values, 1)):
+        assert c_calls[0][c_calls[0].index(t.data_ptr()) + stride_at] == 0
+
+
 def test_c_checks(library):
     some = ctypes.c_void_p(1 << 20)       # never read: the checks come first
     step = lambda **kw: library.kb_linear_attention_step(  # noqa: E731
