@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ------------------------------------------- the values with their decay, V'
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // A strip of 32 columns; the groups of rows of one of the buffers.
-    constexpr int FIRST = STATES ? STATE_WARPS : VALUE_FIRST, WARPS = 4 * Sh::BUFFERS;
+    constexpr int FIRST = STATES ? STATE_WARPS : VALUE_FIRST;
     const int strip = warp & 3, buffer = (warp - FIRST) >> 2;
     const uint32_t to =
         tmem + ((uint32_t)(strip * 32) << 16) + Sh::PARTS_AT + buffer * PARTS_STEP;
@@ -788,12 +788,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint8_t* k_tile = smem + st * Sh::STAGE + Sh::K_AT;
       uint8_t* v_tile = smem + st * Sh::STAGE + Sh::V_AT + (active ? (strip >> 1) * BLOCK : 0);
       if (n < CHUNK) {
-        // Rows of a neighbour: zero.  (Of the values, those that this warp reads.)
-        for (int x = threadIdx.x - FIRST * 32; x < (CHUNK - n) * 8 * KC; x += WARPS * 32) {
-          const int r = x >> 3, c = r / (CHUNK - n);
-          *reinterpret_cast<uint4*>(k_tile + c * BLOCK + (n + r - c * (CHUNK - n)) * 128 +
-                                    (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
+        // Rows of a neighbour: zero.  (Of this buffer's groups, since a group's product waits for
+        // its buffer's warps alone; of the values, those that this warp reads.)
+        for (int j = n + strip * 4 + (lane >> 3); j < CHUNK; j += 16)
+          if ((j / GROUP) % Sh::BUFFERS == buffer)
+            for (int c = 0; c < KC; ++c)
+              *reinterpret_cast<uint4*>(k_tile + c * BLOCK + j * 128 + (lane & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
         if (active)
           for (int j = n + (lane >> 2); j < CHUNK; j += 8)
             if ((j / GROUP) % Sh::BUFFERS == buffer)

@@ -287,6 +287,40 @@ def test_linear_attention_blocks_of_many_heads(cuda):
             check_linear(cuda, q, k, v, g, s, lens)
 
 
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 64), (128, 128), (40, 72)])
+@pytest.mark.parametrize("end", [1, 5, 13, 20, 31, 33, 64, 100, 127, 128])
+@pytest.mark.parametrize("whole", [0, 2])
+def test_linear_attention_beside_values_that_are_no_numbers(cuda, dk, dv, end, whole):
+    # What lies behind a request's end, of the next request or of none, does not reach it, where
+    # its last chunk has `end` tokens: with `whole` chunks before, of values that are no numbers in
+    # their second and fourth 32 rows, which keep half of the warps that prepare a chunk busy.
+    n = 128 * whole + end
+    lens = [n, 40, 9]
+    q, k, v, g, s = linear_inputs(lens + [150], 3, 3, 3, dk, dv, torch.bfloat16, n, slots=3)
+    g *= 0.05
+    for c in range(whole):
+        v[128 * c + 32:128 * c + 64, 0, 3] = NAN
+        v[128 * c + 100:128 * c + 128, 1, 9] = INF
+    cu = ints(sums(lens), cuda)
+    run = lambda s: (ops.linear_attention(  # noqa: E731
+        q.to(cuda), k.to(cuda), v.to(cuda), g.to(cuda), cu, n + 40, state=s), s)
+    out, state = run(s.to(cuda))
+    for bad in (NAN, INF, -INF):
+        for x in (q, k, v):
+            x[n:n + 40] = bad
+            x[n + 49:] = bad
+        g[n:n + 40] = NAN
+        g[n + 49:] = NAN
+        got, end_state = run(s.to(cuda))
+        for a, z in ((got[:n], out[:n]), (got[n + 40:], out[n + 40:]),
+                     (end_state[::2], state[::2])):
+            assert torch.equal(torch.isfinite(a), torch.isfinite(z))
+            assert torch.equal(a[torch.isfinite(a)], z[torch.isfinite(z)])
+        assert bool(torch.isnan(got[n:n + 40]).all()) and bool(torch.isnan(end_state[1]).all())
+    if not whole:
+        assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(state).all())
+
+
 def test_linear_attention_no_numbers_in_every_chunk(cuda):
     # Chunk after chunk with values that are no numbers, in one piece and in segments.
     lens = [700]
