@@ -534,8 +534,9 @@ KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows
  * dtype 0 bf16, 1 f16, 2 f32.  Widths multiples of 8 up to 128; pointers and rows
  * 16-byte aligned.  log_decay fp32 [tokens, H], or [H] with per_token 0; values
  * above 0 count as 0.  state fp32 [slots][H][Dk][Dv] with slot and head strides
- * (blocks dense), NULL: from zero and not kept; request b's slot is
- * state_index[b], or b; negative: from zero and not kept.  S is read before the
+ * (blocks dense and apart: the slots' from all heads of one, or the heads' from all
+ * slots), NULL: from zero and not kept; request b's slot is state_index[b], or b;
+ * negative: from zero and not kept.  S is read before the
  * first token and written after the last; no two requests name one slot.  out
  * [tokens, H, Dv] contiguous; rows outside every request are zero, rows of a
  * request past max_tokens are not written.  A value that is no number reaches the

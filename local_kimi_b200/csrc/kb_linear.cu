@@ -372,6 +372,16 @@ static int check(const Args& A, int dtype, int64_t B, int64_t H, int64_t Hq, int
                  total <= ((int64_t)1 << 30),
              KB_ERR_UNSUPPORTED, "linear attention: more than 2^30 tokens or 2^28 heads");
   KB_REQUIRE(A.scale > 0.f, KB_ERR_BAD_SHAPE, "linear attention: the scale must be positive");
+  if (A.state != nullptr) {
+    // A block of its own for every slot and head: the slots' apart from all heads of one, or the
+    // heads' from all slots.
+    const int64_t block = Dk * Dv, heads = H - 1, slots = A.slots - 1;
+    const bool apart = (heads == 0 || A.state_head >= block) &&
+                       (slots == 0 || A.state_slot >= block) &&
+                       (heads == 0 || slots == 0 || (A.state_slot - block) / heads >= A.state_head ||
+                        (A.state_head - block) / slots >= A.state_slot);
+    KB_REQUIRE(apart, KB_ERR_BAD_SHAPE, "linear attention: the states overlap");
+  }
   if (B == 0 || total == 0) return KB_OK;
   KB_REQUIRE(A.q && A.k && A.v && A.decay && A.out, KB_ERR_NULL_POINTER,
              "linear attention: NULL pointer");

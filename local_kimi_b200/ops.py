@@ -1535,9 +1535,11 @@ def _linear_args(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: t
             raise ValueError("state must have the heads and widths of the values and keys")
         place = state.data_ptr()
         slot_stride, head_stride, row, one = state.stride()
+        size = dk * dv
         if (one != 1 or row != dv or (slot_stride | head_stride) & 3 or place & 15
-                or (heads > 1 and head_stride < dk * dv)
-                or (slots > 1 and slot_stride < dk * dv)) and slots:
+                or (heads > 1 and head_stride < size) or (slots > 1 and slot_stride < size)
+                or (heads > 1 and slots > 1 and slot_stride < (heads - 1) * head_stride + size
+                    and head_stride < (slots - 1) * slot_stride + size)) and slots:
             raise ValueError("state is updated in place and needs dense, 16-byte aligned [Dk, Dv] "
                              "blocks of its own for every slot and head")
     if state_index is not None:

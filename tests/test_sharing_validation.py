@@ -124,6 +124,29 @@ def test_linear_attention_refusals(any_device):
         ops.linear_attention_step(torch.zeros(4, 2, 64, 64), x, x, x, g, scale=-1.0)
 
 
+def test_states_that_overlap_are_refused(c_calls, library):
+    x, g, size = heads(), torch.zeros(2), 64 * 64
+    memory = torch.zeros(16 * size)
+    step = lambda slot, head: ops.linear_attention_step(  # noqa: E731
+        memory.as_strided((4, 2, 64, 64), (slot, head, 64, 1)), x, x, x, g)
+    for slot, head in ((size, size), (2 * size, 2 * size), (size, 3 * size), (size + 4, size),
+                       (2 * size, size + 4), (size, 4 * size - 4)):
+        with pytest.raises(ValueError, match="of its own"):
+            step(slot, head)
+    # Slots outside, heads outside, slots apart.
+    for slot, head in ((2 * size, size), (size, 4 * size), (4 * size, size), (2 * size + 4, size + 4)):
+        step(slot, head)
+    assert len(c_calls) == 4
+    some = ctypes.c_void_p(1 << 20)       # never read: without tokens a call only checks
+    call = lambda slot, head, slots=4, h=2: library.kb_linear_attention_step(  # noqa: E731
+        some, 128, 64, 2, some, 128, 64, 2, some, 128, 64, h, 64, 64, 0, some, 1, some, slot, head,
+        slots, None, 0, 1.0, some, None)
+    assert call(size, size) == call(size - 4, 4 * size) == call(2 * size, size - 4) == 2
+    assert call(size, 3 * size) == call(1 << 61, 1 << 61, slots=1 << 29) == 2
+    assert call(2 * size, size) == call(size, 4 * size) == call(1 << 61, size, slots=1 << 62) == 0
+    assert call(0, size, slots=1) == call(0, 0, slots=0) == 0
+
+
 def test_page_refusals(any_device):
     table, one = i32(0, 1, 2, 3).view(2, 2), i32(1, 1)
     fork = lambda c=one, t=table, s=i32(0), d=i32(1), f=i32(4), h=i32(0), n=8, **kw: (  # noqa: E731
