@@ -541,9 +541,9 @@ KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows
  * [tokens, H, Dv] contiguous; rows outside every request are zero, rows of a
  * request past max_tokens are not written.  A value that is no number reaches the
  * outputs of its own and later tokens only, there as not-a-number.
- * The workspace of kb_linear_attention_workspace_size bytes (0 but for bf16 and
- * more than a few tokens), 16-byte aligned, may hold anything, but is this call's
- * alone until it is done on the stream.  bf16 prompts run in chunks of 128 tokens
+ * The workspace of kb_linear_attention_workspace_size bytes (asked for with the
+ * call's device current; 0 but for bf16 and more than a few tokens), 16-byte aligned,
+ * may hold anything, but is this call's alone until it is done on the stream.  bf16 prompts run in chunks of 128 tokens
  * on the tensor cores, other types in blocks of 32 in fp32.
  * The step takes one token of each of B requests. */
 KB_API size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64_t Dk, int64_t Dv,

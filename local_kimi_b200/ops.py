@@ -65,6 +65,14 @@ def _call_on(device: torch.device, function: str, *args: object) -> None:
         _lib.call(function, *args)
 
 
+def _size_on(device: torch.device, function: str, *args: object) -> int:
+    """A workspace size that depends on the device: that of the tensors, whichever is current."""
+    if device.index is None or device.index == _current_device():
+        return getattr(_lib.lib(), function)(*args)
+    with torch.cuda.device(device):
+        return getattr(_lib.lib(), function)(*args)
+
+
 _current_device = torch._C._cuda_getDevice
 
 
@@ -1601,8 +1609,8 @@ def linear_attention(
     out = torch.empty(total, heads, dv, dtype=v.dtype, device=device)
     if total == 0:
         return out
-    nbytes = _lib.lib().kb_linear_attention_workspace_size(requests, heads, dk, dv,
-                                                           _ELEMENT[q.dtype], total, max_seqlen)
+    nbytes = _size_on(device, "kb_linear_attention_workspace_size", requests, heads, dk, dv,
+                      _ELEMENT[q.dtype], total, max_seqlen)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _on(device)(
         "kb_linear_attention",

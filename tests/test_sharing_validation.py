@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import pytest
@@ -145,6 +146,36 @@ def test_states_that_overlap_are_refused(c_calls, library):
     assert call(size, 3 * size) == call(1 << 61, 1 << 61, slots=1 << 29) == 2
     assert call(2 * size, size) == call(size, 4 * size) == call(1 << 61, size, slots=1 << 62) == 0
     assert call(0, size, slots=1) == call(0, 0, slots=0) == 0
+
+
+def test_workspace_size_is_asked_for_on_the_tensors_device(monkeypatch, c_calls):
+    # It depends on the SMs of the device that the call runs on, which need not be current.
+    current, asked = [0], []
+
+    class Library:
+        @staticmethod
+        def kb_linear_attention_workspace_size(*args):
+            asked.append((current[0], args))
+            return 640 + current[0]
+
+    @contextlib.contextmanager
+    def on(device):
+        before, current[0] = current[0], device.index
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(ops, "_current_device", lambda: current[0])
+    monkeypatch.setattr(ops._lib, "lib", lambda: Library)
+    monkeypatch.setattr(torch.cuda, "device", on)
+    size = "kb_linear_attention_workspace_size"
+    assert ops._size_on(torch.device("cuda", 1), size, 1, 2) == 641 and current == [0]
+    assert ops._size_on(torch.device("cuda", 0), size, 3) == 640
+    assert asked == [(1, (1, 2)), (0, (3,))]
+    ask = lambda device, *args: (asked.append(device), 4096)[1]  # noqa: E731
+    monkeypatch.setattr(ops, "_size_on", ask)
+    x = heads()
+    ops.linear_attention(x, x, x, torch.zeros(2), i32(0, 4), 4)
+    assert asked[-1] == x.device and c_calls[0][-2] == 4096
 
 
 def test_page_refusals(any_device):
