@@ -536,10 +536,10 @@ KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows
  * above 0 count as 0.  state fp32 [slots][H][Dk][Dv] with slot and head strides
  * (blocks dense and apart: the slots' from all heads of one, or the heads' from all
  * slots), NULL: from zero and not kept; request b's slot is state_index[b], or b;
- * negative: from zero and not kept.  S is read before the
- * first token and written after the last; no two requests name one slot.  out
- * [tokens, H, Dv] contiguous; rows outside every request are zero, rows of a
- * request past max_tokens are not written.  A value that is no number reaches the
+ * negative: from zero and not kept.  S is read before the first token and written
+ * after the last; no two requests name one slot.  out [tokens, H, Dv] contiguous;
+ * rows outside every request are zero, and a request's past its first max_tokens,
+ * which are all that counts of it.  A value that is no number reaches the
  * outputs of its own and later tokens only, there as not-a-number.
  * The workspace of kb_linear_attention_workspace_size bytes (asked for with the
  * call's device current; 0 but for bf16 and more than a few tokens), 16-byte aligned,

@@ -54,6 +54,15 @@ __device__ __forceinline__ void clear_outside(const Args& A) {
     store1<TYPE>(A.out, i < lead * width ? i : i - lead * width + tail * width, 0.f);
 }
 
+// Rows [row, end) of a request past its longest: zero in a CTA's columns [col, col + width).
+template <int TYPE>
+__device__ __forceinline__ void clear_past(const Args& A, int h, int64_t row, int64_t end, int col,
+                                           int width) {
+  width = min(width, A.Dv - col);
+  for (int64_t i = threadIdx.x; i < (end - row) * width; i += THREADS)
+    store1<TYPE>(A.out, ((row + i / width) * A.H + h) * A.Dv + col + i % width, 0.f);
+}
+
 // COLS: columns of a CTA, 128 or 32.
 template <int TYPE, int COLS>
 __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
@@ -71,9 +80,10 @@ __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
   pdl_launch_dependents();
 
   if (A.cu != nullptr) clear_outside<TYPE>(A);
-  int64_t first;
-  const int n = request_tokens(A, b, first);
+  int64_t first, end;
+  const int n = request_tokens(A, b, first, end);
   if (n <= 0) return;
+  clear_past<TYPE>(A, h, first + n, end, part * COLS, COLS);
   float* state = request_state(A, b, h);
   float4 s[ROWS];
 #pragma unroll
@@ -198,9 +208,10 @@ __global__ void __launch_bounds__(THREADS, 2) block_kernel(const Args A) {
   pdl_wait();
   pdl_launch_dependents();
   clear_outside<TYPE>(A);
-  int64_t first;
-  const int n = request_tokens(A, b, first);
+  int64_t first, end;
+  const int n = request_tokens(A, b, first, end);
   if (n <= 0) return;
+  clear_past<TYPE>(A, h, first + n, end, part * BLOCK, BLOCK);
   float* state = request_state(A, b, h);
   float s[ROWS];
 #pragma unroll

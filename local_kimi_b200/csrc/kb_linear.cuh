@@ -24,15 +24,21 @@ struct Args {
   uint32_t* err;
 };
 
-// A request's tokens [first, first + n).
-__device__ __forceinline__ int request_tokens(const Args& A, int b, int64_t& first) {
+// A request's tokens [first, first + n), and where its rows end: past first + n where it has more
+// tokens than it may.
+__device__ __forceinline__ int request_tokens(const Args& A, int b, int64_t& first, int64_t& end) {
   if (A.cu == nullptr) {
     first = b;
+    end = b + 1;
     return 1;
   }
-  int64_t end;
   attn::request_rows(A.cu, b, A.total, first, end);
   return (int)min(end - first, (int64_t)A.longest);
+}
+
+__device__ __forceinline__ int request_tokens(const Args& A, int b, int64_t& first) {
+  int64_t end;
+  return request_tokens(A, b, first, end);
 }
 
 // Where a request's state lies; NULL: it starts from zero and is not kept.

@@ -260,8 +260,8 @@ struct Items {
 };
 
 // ---------------------------------------------------------------------------
-// The decays of every chunk, a warp a chunk and head; the last CTA orders the requests, or the
-// last ones copy states.
+// The decays of every chunk, a warp a chunk and head (which clears rows past a request's longest
+// too); the last CTA orders the requests, or the last ones copy states.
 // (A warp of the chunks' kernel that made them beside its other work took 5000 to 8000 clocks a
 // chunk, more than the chunk: 8192 tokens x 32 heads 122 us.)
 // ---------------------------------------------------------------------------
@@ -392,10 +392,17 @@ __global__ void __launch_bounds__(PREPARE_THREADS)
       const int mid = (lo + hi + 1) >> 1;
       if (start(mid) <= place) lo = mid; else hi = mid - 1;
     }
-    int64_t first;
-    const int n = request_tokens(A, lo, first);
+    int64_t first, end;
+    const int n = request_tokens(A, lo, first, end);
     const int64_t skip = (place - place_of(first, lo)) * CHUNK;
-    if (skip < 0 || skip >= n) return;
+    if (skip < 0 || first + skip >= end) return;
+    // Rows of a request past its longest: zero.
+    const int64_t after = min(end, first + skip + CHUNK);
+    for (int64_t row = first + max(skip, (int64_t)n); row < after; ++row)
+      if (lane * 8 < A.Dv)
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(A.out) + (row * A.H + h) * A.Dv)[lane] =
+            make_uint4(0, 0, 0, 0);
+    if (skip >= n) return;
     chunk_decays(A, first + skip, (int)min(n - skip, (int64_t)CHUNK), h, C.decays + at);
     return;
   }

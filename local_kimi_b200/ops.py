@@ -1588,7 +1588,7 @@ def linear_attention(
     (default: b): read as S before the first token, and updated in place.  A
     negative slot, or no ``state``: S starts from zero and is not kept.  No two
     requests may name one slot.  Returns [tokens, H, Dv] of the inputs' type; rows
-    outside every request are zero.
+    outside every request, and a request's past its first ``max_seqlen``, are zero.
 
     BF16 prompts of more than a few tokens run in chunks on the tensor cores (the weights
     between tokens rounded to BF16, the state kept to FP32); FP16 and FP32 ones in FP32, which

@@ -321,6 +321,29 @@ def test_linear_attention_beside_values_that_are_no_numbers(cuda, dk, dv, end, w
         assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(state).all())
 
 
+@pytest.mark.parametrize("dtype,h,dv,longest", [
+    (torch.bfloat16, 2, 64, 5), (torch.bfloat16, 160, 80, 8), (torch.bfloat16, 3, 72, 100),
+    (torch.bfloat16, 1, 128, 1000), (torch.bfloat16, 80, 64, 129), (torch.float16, 2, 40, 13),
+    (torch.float32, 40, 128, 41), (torch.float32, 1, 8, 3),
+])
+def test_linear_attention_of_longer_requests_than_said(cuda, dtype, h, dv, longest):
+    # A request's first max_seqlen tokens count; its other rows are zero.
+    lens = [longest, 3 * longest + 70, 0, longest + 1, 2, longest + 300]
+    kept = [min(n, longest) for n in lens]
+    q, k, v, g, s = (x.to(cuda) for x in linear_inputs(lens, h, h, 1, 64, dv, dtype, longest))
+    at = torch.cat([torch.arange(a, a + n) for a, n in zip(sums(lens), kept)]).to(cuda)
+    want_state = s.clone()
+    want = ops.linear_attention(q[at], k[at], v[at], g[at], ints(sums(kept), cuda), longest,
+                                state=want_state)
+    junk = [torch.full_like(v, NAN) for _ in range(3)]      # what new memory may hold
+    del junk
+    out = ops.linear_attention(q, k, v, g, ints(sums(lens), cuda), longest, state=s)
+    assert torch.equal(out[at], want) and torch.equal(s, want_state)
+    rest = torch.ones(out.shape[0], dtype=torch.bool, device=cuda)
+    rest[at] = False
+    assert not out[rest].any()
+
+
 def test_linear_attention_no_numbers_in_every_chunk(cuda):
     # Chunk after chunk with values that are no numbers, in one piece and in segments.
     lens = [700]
