@@ -75,11 +75,11 @@ constexpr uint32_t S_AT = 0, O_AT = 128, GAIN_AT = 256, PARTS_STEP = 64;
 
 // The decays of a chunk and head.
 struct Decays {
-  float at[CHUNK];                           // b_i, base 2
+  float at[CHUNK];                           // b_i from the row's group's start on, base 2
   float left[CHUNK];                         // exp(b_e - b_j), e the last row of j's group
   float on[CHUNK / GROUP];                   // exp(b_C - b_e) of each group
   float keep;                                // exp(b_C)
-  float unused[3];
+  float whole[CHUNK / GROUP - 1];            // the sums of whole groups, base 2
   uint8_t since[CHUNK];                      // the last reset up to the row, plus 1; 0: none
 };
 static_assert(sizeof(Decays) % 16 == 0, "bulk copies");
@@ -268,79 +268,81 @@ struct Items {
 
 constexpr int PREPARE_THREADS = 256;
 
-// A row a lane, four groups side by side.  The sums behind a row (to its group's end, then group
-// by group) are those that V' and the state need: where they matter they are small, and exact to
-// 2^-24 of themselves.  The sums up to a row, for P, whose weights have 8 bits, are the group's
-// less those behind.
+// A row a lane, four groups side by side.  All sums are in 64 bits and rounded once, when they are
+// stored.  Nothing is summed across groups but what a weight needs: a sum over the chunk may reach
+// 19000 (base 2) beside differences next to nothing, where fp32's step is half of a bf16 weight's.
+// In a group it stays below 4800, and a difference within 2^-11.
 __device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n, int h,
                                              Decays* D) {
   constexpr int GROUPS = CHUNK / GROUP;
   const int lane = threadIdx.x & 31;
-  float up[GROUPS], behind[GROUPS];
+  float log[GROUPS];
+  double up[GROUPS], behind[GROUPS];
   unsigned marks[GROUPS];
   int none = CHUNK;                          // the first logarithm that is no number
 #pragma unroll
   for (int p = 0; p < GROUPS; ++p) {
     const int j = p * GROUP + lane;
-    up[p] = j < n ? __ldg(A.decay + (first + j) * A.decay_tok + h) : 0.f;
+    log[p] = j < n ? __ldg(A.decay + (first + j) * A.decay_tok + h) : 0.f;
   }
 #pragma unroll
   for (int p = 0; p < GROUPS; ++p) {
-    const float x = decay_of(up[p]);
+    const float x = decay_of(log[p]);
     marks[p] = __ballot_sync(0xffffffffu, x <= RESET);
     const unsigned odd = __ballot_sync(0xffffffffu, x != x);
     if (odd) none = min(none, p * GROUP + __ffs(odd) - 1);
-    up[p] = x > RESET ? x * LOG2E : 0.f;
+    up[p] = x > RESET ? x * 1.4426950408889634 : 0.0;
     behind[p] = __shfl_down_sync(0xffffffffu, up[p], 1);
-    if (lane == 31) behind[p] = 0.f;
+    if (lane == 31) behind[p] = 0.0;
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
     for (int p = 0; p < GROUPS; ++p) {
-      const float z = __shfl_down_sync(0xffffffffu, behind[p], o);
+      const double z = __shfl_down_sync(0xffffffffu, behind[p], o);
       if (lane + o < 32) behind[p] += z;
     }
-  float whole[GROUPS], on[GROUPS], before = 0.f, after = 0.f;
+  double whole[GROUPS], after = 0.0;
+  float at[GROUPS], left[GROUPS], on[GROUPS];
   int since[GROUPS], last = 0, later = 0;
 #pragma unroll
   for (int p = 0; p < GROUPS; ++p) {
     whole[p] = __shfl_sync(0xffffffffu, up[p] + behind[p], 0);
-    before += whole[p];
-    up[p] = before - behind[p];
+    at[p] = (float)(whole[p] - behind[p]);
     const unsigned seen = marks[p] & (0xffffffffu >> (31 - lane));
     since[p] = seen ? p * GROUP + 32 - __clz(seen) : last;
     if (marks[p]) last = p * GROUP + 32 - __clz(marks[p]);
   }
 #pragma unroll
   for (int p = GROUPS - 1; p >= 0; --p) {
-    on[p] = later ? 0.f : exp2f(after);
+    on[p] = later ? 0.f : exp2f((float)after);
     after += whole[p];
     later |= marks[p] != 0;
     // A reset behind the row, in its group.
     const unsigned rest = lane < 31 ? marks[p] >> (lane + 1) : 0u;
-    behind[p] = p * GROUP + lane >= n || rest ? 0.f : exp2f(behind[p]);
+    left[p] = p * GROUP + lane >= n || rest ? 0.f : exp2f((float)behind[p]);
   }
-  float keep = later ? 0.f : exp2f(after);
+  float keep = later ? 0.f : exp2f((float)after);
   if (none < CHUNK) {                        // all sums over it are none either
     keep = NAN;
 #pragma unroll
     for (int p = 0; p < GROUPS; ++p) {
-      if (p * GROUP + lane >= none) up[p] = NAN;
-      if (p == none / GROUP && p * GROUP + lane < none) behind[p] = NAN;
+      if (p * GROUP + lane >= none) at[p] = NAN;
+      if (p == none / GROUP && p * GROUP + lane < none) left[p] = NAN;
       on[p] = NAN;
     }
   }
 #pragma unroll
   for (int p = 0; p < GROUPS; ++p) {
     const int j = p * GROUP + lane;
-    D->at[j] = up[p];
-    D->left[j] = behind[p];
+    D->at[j] = at[p];
+    D->left[j] = left[p];
     D->since[j] = (uint8_t)since[p];
   }
   if (lane == 0) {
     *reinterpret_cast<float4*>(D->on) = make_float4(on[0], on[1], on[2], on[3]);
-    D->keep = keep;
+    *reinterpret_cast<float4*>(&D->keep) =
+        make_float4(keep, (float)whole[0], (float)whole[1], (float)whole[2]);
   }
 }
 
@@ -640,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---------------------------------------------------------------- the outputs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int part = (warp >> 2) & 1;        // columns part * 64 .. of the scores
-    const int q0 = (warp & 3) * 32, row = q0 + lane;
+    const int warp_group = warp & 3, q0 = warp_group * GROUP, row = q0 + lane;
     const uint32_t lanes = tmem + ((uint32_t)q0 << 16);
     constexpr int COLS = DVP / 2;            // of the outputs a thread has
     while (true) {
@@ -672,8 +674,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           };
           if (j0 < q0) {
             // All before the rows: the decay to the group's end, and on to the row.
-            const int last = j0 | (GROUP - 1);
-            const float on = since > last + 1 ? 0.f : exp2_fast(mine - D.at[last]);
+            const int last = j0 | (GROUP - 1), group = j0 / GROUP;
+            float b = mine;
+            if (warp_group - group > 1) b += D.whole[group + 1];
+            if (warp_group - group > 2) b += D.whole[2];
+            const float on = since > last + 1 ? 0.f : exp2_fast(b);
             const float2 on2 = make_float2(on, on);
             const float* left = &D.left[j0];
 #pragma unroll
@@ -712,7 +717,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!need(&B->q_done, one_phase)) break;
       tc::tc_fence_after();
-      const float gain = since ? 0.f : exp2_fast(mine);
+      float b = mine;
+      for (int g = 0; g < warp_group; ++g) b += D.whole[g];
+      const float gain = since ? 0.f : exp2_fast(b);
 #pragma unroll 1
       for (int c = 0; c < COLS / 16; ++c) {
         uint32_t o[16];

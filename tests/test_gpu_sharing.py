@@ -344,6 +344,34 @@ def test_linear_attention_of_longer_requests_than_said(cuda, dtype, h, dv, longe
     assert not out[rest].any()
 
 
+@pytest.mark.parametrize("first", [116, 84, 20])
+def test_linear_attention_weights_behind_strong_decays(cuda, first):
+    # Each query meets one key, a few tokens before it, and decays that leave next to nothing of
+    # what lies before `first`.  Queries, keys and values are powers of two, so a weight's rounding
+    # to bf16 (u) is the output's whole error but for the weight's exponent: sums of up to 20
+    # logarithms of 150 (base 2) lie below 4096 and are rounded to fp32 by up to 2^-13 each, two
+    # of them 2^-12 ln 2 = 0.044 u; the exponential adds 2^-22.
+    n, h, b, dk = 128, 32, 12, 128
+    gen = torch.Generator().manual_seed(first)
+    g = torch.full((b, n, h), -103.9)
+    g[:, first:] = -torch.rand(b, n - first, h, generator=gen) * 0.2
+    q = torch.zeros(b, n, h, dk)
+    k = torch.zeros(b, n, 1, dk)
+    k[:, torch.arange(n), 0, torch.arange(n)] = 1.0
+    to = [first + (i * 7) % (i - first) if i > first else i for i in range(n)]
+    to = [max(j, i - 40) for i, j in enumerate(to)]
+    q[:, torch.arange(n), :, torch.tensor(to)] = 1.0
+    v = torch.exp2(torch.randint(-2, 3, (b, n, h, 8), generator=gen).float())
+    q, k, v = (x.view(b * n, -1, x.shape[-1]).bfloat16() for x in (q, k, v))
+    run = g.double().cumsum(1)
+    want = torch.exp(run - run[:, to])[..., None] * v.view(b, n, h, 8).double()[:, to]
+    out = ops.linear_attention(q.to(cuda), k.to(cuda), v.to(cuda), g.view(b * n, h).to(cuda),
+                               ints([n * i for i in range(b + 1)], cuda), n, scale=1.0)
+    got, late = out.view(b, n, h, 8).double().cpu(), slice(first, None)
+    worst = float(((got - want) / want)[:, late].abs().max())
+    assert worst <= 1.05 * 2.0 ** -8, worst * 2.0 ** 8
+
+
 def test_linear_attention_no_numbers_in_every_chunk(cuda):
     # Chunk after chunk with values that are no numbers, in one piece and in segments.
     lens = [700]
