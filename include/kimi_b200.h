@@ -539,12 +539,14 @@ KB_API int kb_verify_drafts(const void* logits, int64_t row_stride, int64_t rows
  * negative: from zero and not kept.  S is read before the first token and written
  * after the last; no two requests name one slot.  out [tokens, H, Dv] contiguous;
  * rows outside every request are zero, and a request's past its first max_tokens,
- * which are all that counts of it.  A value that is no number reaches the
- * outputs of its own and later tokens only, there as not-a-number.
+ * which are all that counts of it.  A value that is no number (an infinity too)
+ * reaches the outputs of its own and later tokens only, past decays of 0 too, there
+ * as an infinity or not-a-number.
  * The workspace of kb_linear_attention_workspace_size bytes (asked for with the
  * call's device current; 0 but for bf16 and more than a few tokens), 16-byte aligned,
- * may hold anything, but is this call's alone until it is done on the stream.  bf16 prompts run in chunks of 128 tokens
- * on the tensor cores, other types in blocks of 32 in fp32.
+ * may hold anything, but is this call's alone until it is done on the stream.
+ * bf16 prompts run in chunks of 128 tokens on the tensor cores, other types in blocks
+ * of 32 in fp32.
  * The step takes one token of each of B requests. */
 KB_API size_t kb_linear_attention_workspace_size(int64_t B, int64_t H, int64_t Dk, int64_t Dv,
                    int dtype, int64_t total, int64_t max_tokens);

@@ -8,7 +8,7 @@
 // Every exponent is at most 0.  Rows and keys in groups of 32: within one, exp(b_i - b_j) is
 // computed; across groups it is exp(b_e - b_j) exp(b_i - b_e), e the last row of j's group, so
 // that a row needs one exponential a group.  A decay that is 0 in fp32 (below e^-104, -infinity
-// too) is a reset: what lies before it does not count.
+// too) counts as e^-104 in the sums, whose exponentials then are 0.
 //
 // One persistent CTA per SM; a unit is one head of one request (or of a segment of it), its
 // chunks one after the other.  Q, K and V tiles (128 rows, 64-element blocks in the 128-byte
@@ -80,7 +80,6 @@ struct Decays {
   float on[CHUNK / GROUP];                   // exp(b_C - b_e) of each group
   float keep;                                // exp(b_C)
   float whole[CHUNK / GROUP - 1];            // the sums of whole groups, base 2
-  uint8_t since[CHUNK];                      // the last reset up to the row, plus 1; 0: none
 };
 static_assert(sizeof(Decays) % 16 == 0, "bulk copies");
 
@@ -271,7 +270,7 @@ constexpr int PREPARE_THREADS = 256;
 // A row a lane, four groups side by side.  All sums are in 64 bits and rounded once, when they are
 // stored.  Nothing is summed across groups but what a weight needs: a sum over the chunk may reach
 // 19000 (base 2) beside differences next to nothing, where fp32's step is half of a bf16 weight's.
-// In a group it stays below 4800, and a difference within 2^-11.
+// In a group it stays below 4802, and a difference within 2^-11.
 __device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n, int h,
                                              Decays* D) {
   constexpr int GROUPS = CHUNK / GROUP;
@@ -291,7 +290,7 @@ __device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n
     marks[p] = __ballot_sync(0xffffffffu, x <= RESET);
     const unsigned odd = __ballot_sync(0xffffffffu, x != x);
     if (odd) none = min(none, p * GROUP + __ffs(odd) - 1);
-    up[p] = x > RESET ? x * 1.4426950408889634 : 0.0;
+    up[p] = x != x ? 0.0 : fmaxf(x, RESET) * 1.4426950408889634;
     behind[p] = __shfl_down_sync(0xffffffffu, up[p], 1);
     if (lane == 31) behind[p] = 0.0;
   }
@@ -304,14 +303,11 @@ __device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n
     }
   double whole[GROUPS], after = 0.0;
   float at[GROUPS], left[GROUPS], on[GROUPS];
-  int since[GROUPS], last = 0, later = 0;
+  int later = 0;
 #pragma unroll
   for (int p = 0; p < GROUPS; ++p) {
     whole[p] = __shfl_sync(0xffffffffu, up[p] + behind[p], 0);
     at[p] = (float)(whole[p] - behind[p]);
-    const unsigned seen = marks[p] & (0xffffffffu >> (31 - lane));
-    since[p] = seen ? p * GROUP + 32 - __clz(seen) : last;
-    if (marks[p]) last = p * GROUP + 32 - __clz(marks[p]);
   }
 #pragma unroll
   for (int p = GROUPS - 1; p >= 0; --p) {
@@ -337,7 +333,6 @@ __device__ __forceinline__ void chunk_decays(const Args& A, int64_t first, int n
     const int j = p * GROUP + lane;
     D->at[j] = at[p];
     D->left[j] = left[p];
-    D->since[j] = (uint8_t)since[p];
   }
   if (lane == 0) {
     *reinterpret_cast<float4*>(D->on) = make_float4(on[0], on[1], on[2], on[3]);
@@ -652,7 +647,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!need(&B->full[st], ph)) break;
       const Decays& D = B->decays[st];
       const float mine = D.at[row];
-      const int since = D.since[row];
       if (!need(&B->s_full, one_phase)) break;
       tc::tc_fence_after();
       // (Loops that stay loops, here and below: each scheduler runs warps of every role, whose
@@ -674,11 +668,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           };
           if (j0 < q0) {
             // All before the rows: the decay to the group's end, and on to the row.
-            const int last = j0 | (GROUP - 1), group = j0 / GROUP;
+            const int group = j0 / GROUP;
             float b = mine;
             if (warp_group - group > 1) b += D.whole[group + 1];
             if (warp_group - group > 2) b += D.whole[2];
-            const float on = since > last + 1 ? 0.f : exp2_fast(b);
+            const float on = exp2_fast(b);
             const float2 on2 = make_float2(on, on);
             const float* left = &D.left[j0];
 #pragma unroll
@@ -692,10 +686,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           } else {
             const float2 here = make_float2(mine, mine), minus = make_float2(-1.f, -1.f);
             const float* at = &D.at[j0];
-            // Columns up to the row, and from its last reset on.
-            uint32_t seen = 0xffffffffu >> (31 - lane);
-            if (since > q0 + 1) seen &= 0xffffffffu << (since - 1 - q0);
-            seen >>= j0 - q0;
+            // Columns up to the row.
+            const uint32_t seen = (0xffffffffu >> (31 - lane)) >> (j0 - q0);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
               const float4 b = *reinterpret_cast<const float4*>(at + i);
@@ -719,7 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc::tc_fence_after();
       float b = mine;
       for (int g = 0; g < warp_group; ++g) b += D.whole[g];
-      const float gain = since ? 0.f : exp2_fast(b);
+      const float gain = exp2_fast(b);
 #pragma unroll 1
       for (int c = 0; c < COLS / 16; ++c) {
         uint32_t o[16];

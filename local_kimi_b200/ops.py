@@ -1593,6 +1593,10 @@ def linear_attention(
     BF16 prompts of more than a few tokens run in chunks on the tensor cores (the weights
     between tokens rounded to BF16, the state kept to FP32); FP16 and FP32 ones in FP32, which
     for long prompts takes ten to twenty times as long.
+
+    A value that is no number, or an infinity, reaches its own and later tokens of its request
+    (where it is one of ``v``, in its column), past decays of 0 too: as an infinity or
+    not-a-number, which of them depends on how the prompt is run.
     """
     if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must have one entry more than there are requests")

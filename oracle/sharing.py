@@ -28,9 +28,8 @@ def linear_attention(q, k, v, log_decay, cu, scale, state=None):
         s, a = ends[b], weights[b]
         for t in range(cu[b], cu[b + 1]):
             keep = g[t].exp()[:, None, None]
-            # A decay of 0 ends what lies before, whatever it is.
-            s = torch.where(keep == 0, 0.0, s * keep) + k[t][:, :, None] * v[t][:, None, :]
-            a = torch.where(keep == 0, 0.0, a * keep) + (k[t][:, :, None] * v[t][:, None, :]).abs()
+            s = s * keep + k[t][:, :, None] * v[t][:, None, :]
+            a = a * keep + (k[t][:, :, None] * v[t][:, None, :]).abs()
             out[t] = torch.einsum("hk,hkv->hv", q[t], s)
             size[t] = torch.einsum("hk,hkv->hv", q[t].abs(), a)
         ends[b], weights[b] = s, a

@@ -372,6 +372,33 @@ def test_linear_attention_weights_behind_strong_decays(cuda, first):
     assert worst <= 1.05 * 2.0 ** -8, worst * 2.0 ** 8
 
 
+@pytest.mark.parametrize("dtype,n", [
+    (torch.bfloat16, 7), (torch.bfloat16, 300), (torch.bfloat16, 1500), (torch.float16, 100),
+    (torch.float32, 100), (torch.float32, 12)])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+def test_linear_attention_no_numbers_before_decays_of_zero(cuda, dtype, n, which, bad):
+    # 0 times what is no number is none: the same however a prompt is run, wherever in its 32 rows,
+    # its chunk or its segment the decay of 0 lies.
+    for h, (dk, dv) in ((2, (64, 64)), (160, (128, 40))):
+        q, k, v, g, s = linear_inputs([n], h, h, h, dk, dv, dtype, n)
+        at = min(n // 3, 70)
+        (k if which == "k" else v)[at, 1, 5] = bad
+        for reset in (1, 2, 20, 40, 130):
+            if at + reset < n:
+                g[at + reset] = -INF if reset % 40 else -300.0
+        state = s.to(cuda)
+        out = ops.linear_attention(q.to(cuda), k.to(cuda), v.to(cuda), g.to(cuda),
+                                   ints([0, n], cuda), n, state=state)
+        hit, gone = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(state, dtype=torch.bool)
+        if which == "k":
+            hit[at:, 1], gone[0, 1, 5] = True, True
+        else:
+            hit[at:, 1, 5], gone[0, 1, :, 5] = True, True
+        assert torch.equal(~torch.isfinite(out), hit)
+        assert torch.equal(~torch.isfinite(state), gone)
+
+
 def test_linear_attention_no_numbers_in_every_chunk(cuda):
     # Chunk after chunk with values that are no numbers, in one piece and in segments.
     lens = [700]
