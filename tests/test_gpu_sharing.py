@@ -372,6 +372,41 @@ def test_linear_attention_weights_behind_strong_decays(cuda, first):
     assert worst <= 1.05 * 2.0 ** -8, worst * 2.0 ** 8
 
 
+@pytest.mark.parametrize("n,h,dv", [(128, 2, 64), (2048, 1, 128), (4096, 3, 72), (1024, 160, 64)])
+def test_linear_attention_state_to_fp32(cuda, n, h, dv):
+    # The state of chunks keeps 24 bits (two bf16 parts of its values would keep 16), in segments
+    # and whole.  Each chunk names each key row once, so that few roundings meet in an element; in
+    # units of 2^-24 of the magnitudes: an exponential is off by 2 ulp (4), its argument, below 2,
+    # by 2^-24 ln 2 (0.7), and a term is a product of two of them (9.4) and its value (2 products,
+    # 2), split in three parts (the last is off by 2^-24: 1), summed in fp32 by the tensor cores,
+    # which may cut off (3 x 2): 18.4.  What lies before a chunk is multiplied by its decay (4.7,
+    # and 1 where segments multiply theirs) and added (1, and 1 more between segments).
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    c, dk = n // 128, 128
+    q = torch.zeros(n, 1, dk, device=cuda).bfloat16()
+    k = torch.eye(dk, device=cuda).repeat(c, 1)[:, None].bfloat16()
+    v = torch.randn(n, h, dv, generator=gen, device=cuda).bfloat16()
+    g = -(0.3 + torch.rand(n, h, generator=gen, device=cuda)) / 160
+    state = torch.zeros(1, h, dk, dv, device=cuda)
+    ops.linear_attention(q, k, v, g, ints([0, n], cuda), n, state=state)
+    run = g.double().view(c, 128, h).cumsum(1)
+    terms = (run[:, -1:] - run).exp()[..., None] * v.double().view(c, 128, h, dv)
+    high = terms.float().bfloat16().double()
+    parts = high + (terms - high).float().bfloat16().double()
+    want = torch.zeros(dk, h, dv, dtype=torch.float64, device=cuda)
+    size, units, two = want.clone(), want.clone(), want.clone()
+    for i in range(c):
+        keep = run[i, -1].exp()[:, None]
+        units = keep * (units + 5.7 * size)
+        two = keep * two + parts[i]
+        want, size = keep * want + terms[i], keep * size + terms[i].abs()
+        units += 18.4 * terms[i].abs() + 2 * size
+    off = (state[0].transpose(0, 1).double() - want).abs()
+    assert bool((off <= units * 2.0 ** -24).all()), float((off / size).max())
+    # (Two parts alone would not do.)
+    assert bool(((two - want).abs() > units * 2.0 ** -24).any())
+
+
 @pytest.mark.parametrize("dtype,n", [
     (torch.bfloat16, 7), (torch.bfloat16, 300), (torch.bfloat16, 1500), (torch.float16, 100),
     (torch.float32, 100), (torch.float32, 12)])
