@@ -61,7 +61,6 @@
 namespace kb {
 namespace linear {
 
-
 constexpr int CHUNK = 128;
 constexpr int BLOCK = CHUNK * 128;           // bytes of 128 rows x 64 elements
 constexpr int THREADS = 896;
@@ -182,24 +181,6 @@ __device__ __forceinline__ void store_shared(uint32_t to, const uint4& v) {
 __device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_half(uint32_t w) {
   return __uint_as_float(w & 0xffff0000u);
-}
-
-// A bounded wait of a warp in step (kb_attn.cuh's in fewer instructions: two dozen places wait,
-// and all roles' code has to fit the instruction cache).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_f,
-                                          uint32_t* err) {
-  bool ok = mbar_try_wait(bar, parity);
-  if (!ok) {
-    const long long t0 = attn::now_ns();
-    do {
-      ok = attn::mbar_try_wait_for(bar, parity, 200000u);
-    } while (!ok && !*abort_f && attn::now_ns() - t0 <= attn::WAIT_NS);
-    if (!ok && !*abort_f) {
-      *abort_f = 1;
-      atomicOr(err, attn::ERR_WAIT);
-    }
-  }
-  return __all_sync(0xffffffffu, ok) != 0;
 }
 
 // Where a request's chunks' decays start: places enough for all before, without a sum over them.
@@ -502,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   // Bounded waits of a warp in step; one arrival a warp.
   bool ok = true;
   auto need = [&](uint64_t* bar, uint32_t parity) {
-    ok = warp_wait(bar, parity, abort_f, A.err);
+    ok = attn::warp_wait(bar, parity, abort_f, A.err);
     return ok;
   };
   auto arrive = [&](uint64_t* bar) {
