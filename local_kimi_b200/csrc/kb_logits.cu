@@ -505,6 +505,8 @@ extern "C" int kb_adjust_logits(const void* logits, int64_t row_stride, int64_t 
                  (!bias_ids || bias_values) && (!tokens || cu_tokens) && (!tree_mask || tokens) &&
                  (cu_tokens || B <= rows),
              KB_ERR_NULL_POINTER, "adjust logits: NULL pointer");
+  KB_REQUIRE(logits != out || rows == 1 || row_stride == out_stride, KB_ERR_BAD_SHAPE,
+             "adjust logits: in place, the rows have one stride");
   const size_t size = dtype == 2 ? 4 : 2;
   KB_REQUIRE((((uintptr_t)logits | (uintptr_t)out) & (size - 1)) == 0 &&
                  (((uintptr_t)history | (uintptr_t)bias_ids | (uintptr_t)tokens |

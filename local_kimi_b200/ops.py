@@ -1988,7 +1988,7 @@ def adjust_logits(
         x, x_stride = ((logits, max(logits.stride(0), vocab)) if out is logits
                        else _unit_rows(logits, vocab))
         if out is not logits and _overlap(x, y):
-            if x.data_ptr() != y.data_ptr() or x.stride() != y.stride():
+            if x.data_ptr() != y.data_ptr() or (rows > 1 and x.stride(0) != y.stride(0)):
                 raise ValueError("out must be the logits themselves or lie apart from them")
     if rows == 0:
         return y

@@ -320,6 +320,22 @@ def test_rows_that_share_memory_keep_their_stride(c_calls):
         assert c_calls[0][c_calls[0].index(t.data_ptr()) + stride_at] == 0
 
 
+def test_adjust_logits_in_place_by_any_view(c_calls, library):
+    # The logits themselves are one row of a wider matrix here, of other strides there.
+    wide = torch.zeros(3, 100)
+    row, same = wide[:1, :40], wide[0, :40].view(1, 40)
+    assert row.stride() != same.stride()
+    assert ops.adjust_logits(row, out=same) is same
+    assert c_calls[0][1] == c_calls[0][6] == wide.data_ptr()
+    with pytest.raises(ValueError, match="lie apart"):
+        ops.adjust_logits(wide[:2, :40], out=wide.view(-1)[:80].view(2, 40))
+    some = ctypes.c_void_p(1 << 20)       # never read
+    call = lambda stride, n=2: library.kb_adjust_logits(  # noqa: E731
+        some, 50, n, 40, 2, some, stride, 0, None, 0, 0, *[None] * 6, 0, None, 0, 0, None, 0, some,
+        None, None, None)
+    assert call(60) == 2
+
+
 def test_c_checks(library):
     some = ctypes.c_void_p(1 << 20)       # never read: the checks come first
     step = lambda **kw: library.kb_linear_attention_step(  # noqa: E731
