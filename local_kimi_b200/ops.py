@@ -1639,7 +1639,7 @@ def linear_attention_step(
 
     ``state`` fp32 [slots, H, Dk, Dv] is updated in place.  Returns [B, H, Dv].
     """
-    requests = q.shape[0]
+    requests = q.shape[0] if q.ndim else 0
     (_, heads, dk, dv), args, held = _linear_args(
         q, k, v, log_decay, state, state_index, requests, expanded=True)
     device = q.device

@@ -125,6 +125,13 @@ def test_linear_attention_refusals(any_device):
         ops.linear_attention_step(torch.zeros(4, 2, 64, 64), x, x, x, g, scale=-1.0)
 
 
+def test_ranks_of_a_step(any_device):
+    x, g, s = heads(), torch.zeros(2), torch.zeros(4, 2, 64, 64)
+    for q in (x[0, 0, 0], x[0, 0], x[0], x[None]):
+        with pytest.raises(ValueError, match="q must have shape"):
+            ops.linear_attention_step(s, q, x, x, g)
+
+
 def test_states_that_overlap_are_refused(c_calls, library):
     x, g, size = heads(), torch.zeros(2), 64 * 64
     memory = torch.zeros(16 * size)
