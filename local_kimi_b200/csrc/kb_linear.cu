@@ -10,7 +10,9 @@
 // blocks (below), bf16 ones in chunks on the tensor cores (kb_linear_chunk.cu).
 //
 // Bound: HBM, the states read and written: 256 requests of 32 heads of 128 x 128 move 1.08 GB in
-// 177 us, 6.07 TB/s.  One request, 2.8 us (4 MB): a launch and one trip to memory.
+// 175 us, 6.2 TB/s.  One request, 2.8 us (4 MB): a launch and one trip to memory.  Each further
+// token of 256 requests takes about 44 us more, its barrier and its sums across threads one after
+// the other beside the states in registers (4 tokens 306 us, 170 at the copy's rate).
 // The state, the sums and the products are fp32; an output is rounded once, when it is stored.
 #include "kb_linear.cuh"
 
@@ -172,9 +174,10 @@ __global__ void __launch_bounds__(THREADS) token_kernel(const Args A) {
 // The sums are in 64 bits: their differences decide small exponents next to large ones.  A CTA
 // has 32 columns of a head's state, in registers (16 rows of a column a thread) and, for q S, in
 // shared memory.  Bound: shared-memory loads, 12 for 32 products a warp while scores and q S are
-// made (the scores again for each 32 columns), and with one CTA an SM their latencies.  Measured,
-// 32 heads of 128 x 128: one f16 prompt of 8192 tokens 1.72 ms, 6.4 us a block (token by token
-// 10.7), f32 1.64 (6.1); 16 prompts of 512 tokens 1.1 ms, 5 us a block and SM.
+// made (the scores again for each 32 columns), and with one CTA an SM their latencies; no tensor
+// cores, whose products would need these types in bf16 parts.  Measured, 32 heads of 128 x 128:
+// one f16 prompt of 8192 tokens 1.77 ms, 6.9 us a block (token by token 10.7), f32 1.61 (6.1); 16
+// prompts of 512 tokens 1.12 ms, 5 us a block and SM.
 // ---------------------------------------------------------------------------
 
 constexpr int BLOCK = 32;
@@ -362,7 +365,10 @@ static int launch_tokens(const Args& A, int sms, void* stream) {
   const int64_t heads = (int64_t)A.B * A.H;
   // Few heads: their columns on several CTAs each.  (32 heads of 128 x 128, one token: 1 request
   // 3.3 us split and 5.0 whole, 2 requests 3.2 and 4.5, 4 requests 5.5 and 5.1, 9 requests 8.1
-  // and 7.2; eight tokens: 8.7 and 10.4 for 1 request, 15.5 and 10.7 for 4.)
+  // and 7.2; eight tokens: 8.7 and 10.4 for 1 request, 15.5 and 10.7 for 4.  The rule is the
+  // widest heads'.  Narrower ones leave threads of a whole CTA idle and would gain from more
+  // splitting: 256 requests, one token, 128 x 64 114 split and 126 whole, 64 x 64 79 and 103,
+  // 16 x 16 77 both.)
   if (heads * 2 < sms && A.Dv > 32)
     return launch(token_kernel<TYPE, 32>, dim3((unsigned)(heads * ((A.Dv + 31) / 32))),
                   dim3(THREADS), 0, stream, A);
@@ -438,9 +444,12 @@ static Args arguments(const void* q, int64_t q_tok, int64_t q_head, int64_t Hq, 
 }
 
 // On the tensor cores: bf16 prompts of more than a few tokens.
-// (32 heads, token by token and in chunks: 1 request of 8 tokens 8.5 and 11.2 us, of 16 14.5 and
-// 11.2; 16 requests of 8 tokens 25 and 32, of 16 42 and 32; 256 requests of 4 tokens 308 and 376,
-// of 8 463 and 381.)
+// (32 heads of 128 x 128, token by token and in chunks: 1 request of 8 tokens 8.6 and 11.4 us, of
+// 16 14.5 and 11.4; 16 requests of 8 tokens 25 and 30, of 9 27 and 30, of 16 42 and 31; 256
+// requests of 4 tokens 306 and 373, of 8 463 and 373.  Other widths cross where these do: 16
+// requests of 8 and of 12 tokens, 128 x 64 24 and 28, 32 and 29; 64 x 64 22 and 25, 31 and 25;
+// 16 x 16 22 and 24, 30 and 24; 256 requests of 8 heads, of 8 tokens 128 x 64 88 and 75, 16 x 16
+// 74 and 62.)
 static bool in_chunks(int dtype, int64_t heads, int64_t longest, int sms) {
   return dtype == 0 && longest > (heads > 16 * sms ? 5 : 8);
 }
@@ -449,7 +458,10 @@ static int run_tokens(const Args& A, int dtype, int sms, void* stream) {
   // Blocks of 32 tokens: from 13 on where each SM has a CTA at most, else from 41.  (32 heads of
   // 128 x 128, token by token and in blocks: 1 request of 12 tokens f16 11.5 and 8.1 us, f32 8.4
   // and 8.1; of 32 26 and 9, 17 and 9; 16 requests of 32 tokens f16 74 and 81, f32 69 and 82; 256
-  // requests of 32 f16 1396 and 1260, f32 1082 and 1300.)
+  // requests of 32 f16 1396 and 1260, f32 1082 and 1300.  The rule is the widest heads': with
+  // fewer value columns to make the scores again for, blocks win sooner.  16 requests of 32 heads,
+  // f16, of 12 and of 40 tokens: 128 x 64 32 and 37, 90 and 71; 64 x 64 31 and 28, 88 and 54;
+  // 16 x 16 31 and 13, 88 and 24.)
   const bool few = (int64_t)A.B * A.H * ((A.Dv + BLOCK - 1) / BLOCK) <= sms;
   if (A.cu != nullptr && A.longest > (few ? 12 : 40)) {
     if (dtype == 1) return launch_blocks<1>(A, stream);

@@ -7,7 +7,8 @@
 //   S'   = exp(b_C) S + sum_j k_j (exp(b_C - b_j) v_j)^T
 // Every exponent is at most 0.  Rows and keys in groups of 32: within one, exp(b_i - b_j) is
 // computed; across groups it is exp(b_e - b_j) exp(b_i - b_e), e the last row of j's group, so
-// that a row needs one exponential a group.  A decay that is 0 in fp32 (below e^-104, -infinity
+// that a row needs one exponential a group.  The sums are made in 64 bits and kept for each group
+// from its start on, b_i - b_e from there and the sums of the groups between.  A decay that is 0 in fp32 (below e^-104, -infinity
 // too) counts as e^-104 in the sums, whose exponentials then are 0.
 //
 // One persistent CTA per SM; a unit is one head of one request (or of a segment of it), its
@@ -31,24 +32,31 @@
 // runs); the second starts each segment from the gains before it.
 //
 // Bound: not the memory (8192 tokens of 32 heads of 128 x 128 move 269 MB, 41 us) nor the tensor
-// cores (51 GFLOP a pass, three of six products the parts of V'; active 39 % of the second pass),
+// cores (51 GFLOP a pass, three of six products the parts of V'; active 38 % of the second pass),
 // but a chunk's way from the scores over P and P V to the outputs: 6000 clocks of latencies in
 // one CTA an SM, since the state and two stages take the shared memory.  Roles on warps of their
 // own let the state, V' and the copies of other chunks run beside it.  The first pass takes 2200
-// clocks a chunk.  Measured, replayed: 102 us; 24 prompts of 1 to 2047 tokens with 24 heads
-// 128 x 64 on 4 of queries and keys 68 us (108 MB at least: 16.4).  Token by token: 10700 and
-// 2630.
+// clocks a chunk.  Measured, replayed: 104 us; 24 prompts of 1 to 2047 tokens with 24 heads
+// 128 x 64 on 4 of queries and keys 67 us (108 MB at least: 16.4).  Token by token: 10700 and
+// 2630.  What does not fill the chain either: with values up to 64 wide half of the gain's 128
+// rows are empty, and each value head walks its chunks alone, also where it shares q and k with
+// others (their copies and Q K^T again for each).
 //
 // The code is in short loops, not unrolled: all roles together have to fit the instruction cache
 // (126 -> 111 us).  Slower: outputs by warps apart from the weights' (114 to 135 us, one barrier
 // and one exchange more in the chunk's way), prefetching stages into L2 (111).
 //
 // Roundings.  P and the copy of the state are rounded once to bf16 before they meet the values
-// and the queries: the outputs have 8 bits themselves.  The state must not lose bits: V' (fp32
-// products) enters the tensor cores as the sum of three bf16 values, 24 bits in all.
+// and the queries: the outputs have 8 bits themselves, and end 1.4 times as far from the exact
+// ones as fp32 products rounded once (0.0023 of their norm, 0.0017).  P's exponents are off by
+// at most 2^-11 (two fp32 values below 4802 of a group), their exponentials, the approximate
+// instruction's, by 2^-22 of themselves: together a tenth of P's rounding.  The state must not
+// lose bits: V' (fp32 products) enters the tensor cores as the sum of three bf16 values, 24 bits
+// in all.
 //
-// 512 columns of tensor memory: scores and P 128, O 128, the state's gain 128, V' 2 x 48, 64
-// apart (in the first pass 4 x 48 in the place of scores and O).
+// 512 columns of tensor memory, allocated in full: scores and P 128 (P takes 64 of them), O 128,
+// the state's gain 128, V' 2 x 48, 64 apart (in the first pass 4 x 48 in the place of scores and
+// O).
 //
 // A row past the request's end belongs to a neighbour: its keys and values are zeroed in shared
 // memory.  A value that is no number is zeroed too, since it would meet zero weights; the rows
@@ -1065,8 +1073,10 @@ static int64_t padded(int64_t width) { return width <= 64 ? 64 : 128; }
 // Segments of a request: as many as make the longest way of a CTA shortest, in chunks.  A unit
 // costs START beside its chunks, each segment's gain that it starts from GAIN; a segment but
 // the last is read twice, for its gain (half a chunk's cost) and its outputs.  (One request of 32
-// heads, in the segments chosen and whole: 512 tokens 20 us both, 1024 29 and 31, 2048 40 and 53,
-// 8192 102 and 190; 8 heads, 8192 tokens: 49 and 184.)
+// heads, in the segments chosen and whole: 512 tokens 21 us both, 1024 30 and 33, 2048 41 and 56,
+// 8192 104 and 198; 8 heads, 8192 tokens: 50 and 195.)  One length for all requests, as if
+// each were as long as the longest: a long request beside short ones is cut less or not at all (32 heads, 8192 tokens beside 300 175 us, beside four requests of
+// 100 to 500 208).
 static void segments_of(int64_t heads, int64_t longest, int sms, int& segments, int& segment) {
   constexpr double START = 2.0, GAIN = 0.4;
   const int64_t chunks = (longest + CHUNK - 1) / CHUNK;
